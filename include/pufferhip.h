@@ -377,6 +377,79 @@ int ph_mingru_step(const ph_mingru_dims* d, const ph_ppo_coefs* c, const ph_muon
                    const float* oldval, const float* rew, const float* done, const float* logrho,
                    const float* boot, float* G, double* losses, void* stream);
 
+/* ---------------------------------------------------------------------------------------------- */
+/* Operators of a state-space policy layer (no counterpart in the reference): layer normalisation, the selective
+ * state-space scan with its short causal convolution, the gated feed-forward block. dtype is PH_F32 or PH_BF16 and
+ * holds for the activations and their gradients; sums, statistics and states are fp32. Rows are [M][C] with the
+ * given row stride in elements. */
+
+/* y = (x - mean) rstd w + b per row of C columns, rstd = 1 / sqrt(var + eps). w, b: fp32 [C], each may be NULL (1 and
+ * 0); mean, rstd: fp32 [M] out for the gradient, each may be NULL. y may be x. */
+int ph_layer_norm(int dtype, const void* x, size_t ldx, size_t M, size_t C, const float* w, const float* b, float eps,
+                  void* y, size_t ldy, float* mean, float* rstd, void* stream);
+/* dx, and dw = sum_rows dy n, db = sum_rows dy (fp32 [C], overwritten, each may be NULL; zero for M = 0), with n =
+ * (x - mean) rstd from the forward's statistics. dx may be dy or x. The sums' order is fixed by the shape. */
+int ph_layer_norm_grad(int dtype, const void* x, size_t ldx, const void* dy, size_t lddy, size_t M, size_t C,
+                       const float* w, const float* mean, const float* rstd, void* dx, size_t lddx, float* dw,
+                       float* db, void* stream);
+
+/* Selective state-space scan of B sequences of T steps, C channels of N states (N <= 64), per channel c and step t:
+ *   u_t = silu(conv_b + sum_k conv_w[c][k] x_{t-K+1+k})   (K <= 4 taps; K = 0: u_t = x_t)
+ *   d_t = softplus(delta_t + dt_bias)
+ *   h_t = exp(d_t A) h_{t-1} + d_t u_t B_t
+ *   y_t = (<h_t, C_t> + D u_t) z_t sigma(z_t)              (z NULL: no gate)
+ * G groups of C / G channels share the rows of B and C. Element (t, b, i) of an array is at t * <name>_t + b * <name>_b
+ * + i, so time-major and batch-major arrays and column slices of a wider one are all taken in place. A, D, dt_bias,
+ * conv_w, conv_b are fp32 ([C][N], [C], [C], [C][K], [C]); D, dt_bias and conv_b may be NULL (0). done (fp32 [T][B], may
+ * be NULL): where nonzero, step t ends an episode, and step t + 1 starts from a cleared state and an empty window; first
+ * (fp32 [B], may be NULL): the same for the step before the call. h0 [B][C][N] and win0 [B][K-1][C] (fp32, each may
+ * be NULL: zero) are the state and the last K - 1 inputs carried in. */
+typedef struct {
+  int dtype;
+  size_t T, B, C, N, G, K;
+  const void *x, *z, *delta, *Bm, *Cm;
+  long x_t, x_b, z_t, z_b, delta_t, delta_b, Bm_t, Bm_b, Cm_t, Cm_b;
+  const float *A, *D, *dt_bias, *conv_w, *conv_b;
+  const float *done, *first, *h0, *win0;
+} ph_ssm_args;
+/* y; h_out and win_out (each may be NULL) receive the state and window after the last step, before done[T-1] clears
+ * them (the next call's `first` does); they may be h0 and win0. keep (may be NULL): fp32, ph_ssm_keep_floats values,
+ * the states that the gradient restarts from. Few long sequences run as chunks of time joined in order. */
+int ph_ssm_scan(const ph_ssm_args* a, void* y, long y_t, long y_b, float* h_out, float* win_out, float* keep,
+                void* stream);
+size_t ph_ssm_keep_floats(const ph_ssm_args* a);
+/* Gradients, each written where its pointer is not NULL: of the activations in their dtype and strides, of the parameters
+ * in fp32 (summed over T and B, overwritten). h0 and win0 are constants. */
+typedef struct {
+  void *dx, *dz, *ddelta, *dBm, *dCm;
+  long dx_t, dx_b, dz_t, dz_b, ddelta_t, ddelta_b, dBm_t, dBm_b, dCm_t, dCm_b;
+  float *dA, *dD, *ddt_bias, *dconv_w, *dconv_b;
+} ph_ssm_grads;
+/* The scan's gradient from the forward's arguments (h0 is not read: the kept states hold it) and its kept states. Sums are
+ * taken in an order fixed by the shape. */
+int ph_ssm_scan_grad(const ph_ssm_args* a, const float* keep, const void* dy, long dy_t, long dy_b,
+                     const ph_ssm_grads* g, void* stream);
+/* One step of B sequences (a->T = 1; its step strides, done, h0 and win0 are not read), the state h [B][C][N] and window
+ * win [B][K-1][C] (fp32) updated in place; first[b] nonzero clears both before the step. */
+int ph_ssm_step(const ph_ssm_args* a, void* y, long y_b, float* h, float* win, void* stream);
+
+/* Gated feed-forward block y = (act(x Wg^T) * (x Wv^T)) Wo^T on MFMA. w_in [2F][D] holds row 2j = gate and row 2j + 1 =
+ * value of unit j, so the two projections of a unit leave the matrix cores side by side and the activation and product
+ * are part of that product's epilogue; w_out [D][F]. Both in dtype; PH_BF16 runs bf16 MFMA with fp32 accumulation,
+ * PH_F32 fp32 MFMA. */
+typedef enum { PH_ACT_SILU = 0, PH_ACT_GELU = 1 } ph_act;
+/* ab [M][ph_ffn_pitch(2F)] and h [M][ph_ffn_pitch(F)] (dtype): the projections and the units for the gradient; both
+ * NULL where no gradient follows. */
+int ph_ffn(int dtype, int act, size_t M, size_t D, size_t F, const void* x, size_t ldx, const void* w_in,
+           const void* w_out, void* ab, void* h, void* y, size_t ldy, void* stream);
+/* Row pitch of ab and h: their columns rounded up to whole 16-byte accesses. */
+size_t ph_ffn_pitch(size_t columns);
+/* dx [M][D], dw_in [2F][D] and dw_out [D][F], each written where not NULL; the weights' gradients in dw_dtype (dtype or
+ * PH_F32), overwritten. */
+int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, const void* x, size_t ldx, const void* w_in,
+                const void* w_out, const void* ab, const void* h, const void* dy, size_t lddy, void* dx, size_t lddx,
+                int dw_dtype, void* dw_in, void* dw_out, void* stream);
+
 /* ============================================================================================== */
 /* Host-buffer entry points (layer 2). Each replaces the reference GPU symbol named beside it, with
  * the same argument order and meaning; FloatArray inputs become host `const double*`, the returned

@@ -14,6 +14,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libpufferhip.so"
 PH_OK, PH_ERR_ARG, PH_ERR_HIP, PH_ERR_NOMEM, PH_ERR_UNSUPPORTED = 0, -1, -2, -3, -4
 PH_F32, PH_F64, PH_BF16, PH_I32 = 0, 1, 2, 3
 PH_MATH_BF16, PH_MATH_F32, PH_MATH_BF16X3 = 0, 1, 2
+PH_ACT_SILU, PH_ACT_GELU = 0, 1
 PH_EPI_NONE, PH_EPI_BIAS, PH_EPI_BIAS_RELU, PH_EPI_RELU_MASK, PH_EPI_AXPBY = 0, 1, 2, 3, 4
 
 vp, sz, dbl, flt, i32, i64, u8, u64 = (C.c_void_p, C.c_size_t, C.c_double, C.c_float, C.c_int,
@@ -47,6 +48,20 @@ class ReplayCols(C.Structure):
     _fields_ = [("dtype", C.c_int), ("time_major", C.c_int), ("N", C.c_size_t), ("T", C.c_size_t),
                 ("K", C.c_size_t), ("adv", C.c_void_p), ("value", C.c_void_p), ("ratio", C.c_void_p),
                 ("act", C.c_void_p), ("logp", C.c_void_p), ("term", C.c_void_p)]
+
+
+
+class SsmArgs(C.Structure):
+    _fields_ = ([("dtype", C.c_int)] + [(n, C.c_size_t) for n in ("T", "B", "C", "N", "G", "K")]
+                + [(n, C.c_void_p) for n in ("x", "z", "delta", "Bm", "Cm")]
+                + [(n + s, C.c_long) for n in ("x", "z", "delta", "Bm", "Cm") for s in ("_t", "_b")]
+                + [(n, C.c_void_p) for n in ("A", "D", "dt_bias", "conv_w", "conv_b", "done", "first", "h0", "win0")])
+
+
+class SsmGrads(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("dx", "dz", "ddelta", "dBm", "dCm")]
+                + [(n + s, C.c_long) for n in ("dx", "dz", "ddelta", "dBm", "dCm") for s in ("_t", "_b")]
+                + [(n, C.c_void_p) for n in ("dA", "dD", "ddt_bias", "dconv_w", "dconv_b")])
 
 
 # name -> argtypes (all return int status unless listed in _RESTYPES)
@@ -95,6 +110,15 @@ SIGNATURES: dict[str, list] = {
     "ph_sample_actions_md": [i32, vp, sz, sz, vp, sz, u64, vp, vp],
     "ph_sample_actions_cont": [i32, vp, sz, sz, sz, u64, dbl, dbl, vp, vp],
     "ph_mingru_rollout_step": [vp, vp, vp, vp, vp, vp],
+    "ph_layer_norm": [i32, vp, sz, sz, sz, vp, vp, flt, vp, sz, vp, vp, vp],
+    "ph_layer_norm_grad": [i32, vp, sz, vp, sz, sz, sz, vp, vp, vp, vp, sz, vp, vp, vp],
+    "ph_ssm_scan": [vp, vp, i64, i64, vp, vp, vp, vp],
+    "ph_ssm_keep_floats": [vp],
+    "ph_ssm_scan_grad": [vp, vp, vp, i64, i64, vp, vp],
+    "ph_ssm_step": [vp, vp, i64, vp, vp, vp],
+    "ph_ffn": [i32, i32, sz, sz, sz, vp, sz, vp, vp, vp, vp, vp, sz, vp],
+    "ph_ffn_pitch": [sz],
+    "ph_ffn_grad": [i32, i32, sz, sz, sz, vp, sz, vp, vp, vp, vp, vp, sz, vp, sz, i32, vp, vp, vp],
     # host-buffer layer (reference Lean @[extern] GPU symbols)
     "ph_cuda_vtrace": [dptr, dptr, dptr, dptr, sz, sz, dbl, dbl, dbl, dbl, dptr],
     "ph_cuda_vtrace_mingru": [dptr, dptr, dptr, dptr, dptr, sz, sz, dbl, dbl, dbl, dbl, dptr],
@@ -153,7 +177,8 @@ SIGNATURES: dict[str, list] = {
     "ph_ffi_gather_seq_minibatch": [dptr, dptr, dptr, dptr, dptr, dptr, dptr, dptr, sz, sz, sz, sz, dptr],
     "ph_cuda_mingru_muon_resident": [sz, dptr, sz, sz, sz, sz, sz, dbl, dbl, dbl, dbl, dbl, dbl, dptr, szptr],
 }
-_RESTYPES = {"ph_last_error": C.c_char_p, "ph_mingru_param_count": C.c_long, "ph_mlp_param_count": C.c_long, "ph_ckpt_bytes": C.c_size_t,
+_RESTYPES = {"ph_last_error": C.c_char_p, "ph_mingru_param_count": C.c_long, "ph_mlp_param_count": C.c_long, "ph_ckpt_bytes": C.c_size_t, "ph_ssm_keep_floats": C.c_size_t,
+             "ph_ffn_pitch": C.c_size_t,
              "ph_ffi_bench_bf16_resident": C.c_double, "ph_ffi_bench_mlp2_bf16_resident": C.c_double,
              "ph_ffi_bench_mlp2_bf16_wres": C.c_double, "ph_ffi_mlp_policy_outputs": C.c_size_t, "ph_ffi_cuda_available": C.c_uint8}
 

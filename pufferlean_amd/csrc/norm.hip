@@ -1,0 +1,462 @@
+// Layer normalisation of rows, y = (x - mean) rstd w + b with rstd = 1/sqrt(var + eps), and its gradient.
+//
+// With n = (x - mean) rstd and dn = dy w, the row's gradient is dx = rstd (dn - avg(dn) - n avg(dn n)); the columns'
+// gradients are dw = sum_rows dy n and db = sum_rows dy. All sums are fp32 over values held in registers: the
+// variance is the mean of the squared deviations from the row's mean, so a large offset costs no digits.
+//
+// Both directions are bound by memory: the forward reads x and writes y, the backward reads x and dy and
+// writes dx. A row lives in the registers of LPR = 8..64 lanes (64 / LPR rows to a wavefront), so each value
+// is read once; the backward's wavefronts walk over many rows and keep their columns' dw and db in registers,
+// which leaves one partial row per block for a second, small launch to add in a fixed order.
+#include "common.hpp"
+#include "kernels.hpp"
+
+namespace ph {
+namespace {
+
+constexpr int kWaves = 4;        // wavefronts per block
+constexpr int kNormRegs = 32;    // values of a row that a lane holds at most: rows up to 2048 columns
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+// V consecutive elements at p as fp32: one 16-byte access for V = 8 (bf16) and V = 4 (fp32), else one element.
+template <int V> __device__ __forceinline__ void load_v(const uint16_t* p, float* v) {
+  if constexpr (V == 8) {
+    const u32x4_t r = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      v[2 * i] = __builtin_bit_cast(float, r[i] << 16);
+      v[2 * i + 1] = __builtin_bit_cast(float, r[i] & 0xffff0000u);
+    }
+  } else {
+    v[0] = bf16_to_f32(*p);
+  }
+}
+template <int V> __device__ __forceinline__ void load_v(const float* p, float* v) {
+  if constexpr (V == 4) {
+    const f32x4_t r = __builtin_nontemporal_load(reinterpret_cast<const f32x4_t*>(p));
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = r[i];
+  } else {
+    v[0] = *p;
+  }
+}
+template <int V> __device__ __forceinline__ void store_v(uint16_t* p, const float* v) {
+  if constexpr (V == 8) {
+    u32x4_t r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = bf16x2_rne(v[2 * i], v[2 * i + 1]);
+    __builtin_nontemporal_store(r, reinterpret_cast<u32x4_t*>(p));
+  } else {
+    *p = bf16_rne(v[0]);
+  }
+}
+template <int V> __device__ __forceinline__ void store_v(float* p, const float* v) {
+  if constexpr (V == 4) {
+    f32x4_t r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = v[i];
+    __builtin_nontemporal_store(r, reinterpret_cast<f32x4_t*>(p));
+  } else {
+    *p = v[0];
+  }
+}
+
+template <int LPR> __device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+  for (int m = 1; m < LPR; m <<= 1) v += __shfl_xor(v, m);
+  return v;
+}
+
+// V elements per access, NCH accesses per lane: a row has at most LPR * V * NCH columns.
+template <typename T, int V, int NCH, int LPR>
+__global__ void __launch_bounds__(64 * kWaves) k_norm_fwd(const T* __restrict__ x, long ldx, long M, int C,
+                                                          const float* __restrict__ w, const float* __restrict__ b,
+                                                          float eps, T* __restrict__ y, long ldy,
+                                                          float* __restrict__ mean, float* __restrict__ rstd) {
+  const int lr = threadIdx.x % LPR;
+  const long row = (long)blockIdx.x * (64 * kWaves / LPR) + threadIdx.x / LPR;
+  if (row >= M) return;  // whole groups of LPR lanes leave together; the shuffles below stay inside a group
+  float v[NCH * V];
+  float s = 0.f;
+#pragma unroll
+  for (int q = 0; q < NCH; q++) {
+    const int c = (q * LPR + lr) * V;
+#pragma unroll
+    for (int i = 0; i < V; i++) v[q * V + i] = 0.f;
+    if (c < C) load_v<V>(x + row * ldx + c, v + q * V);
+  }
+#pragma unroll
+  for (int i = 0; i < NCH * V; i++) s += v[i];
+  const float mu = row_sum<LPR>(s) / (float)C;
+  float s2 = 0.f;
+#pragma unroll
+  for (int q = 0; q < NCH; q++) {
+    const bool in = (q * LPR + lr) * V < C;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      v[q * V + i] -= mu;
+      s2 += in ? v[q * V + i] * v[q * V + i] : 0.f;
+    }
+  }
+  const float r = 1.f / sqrtf(row_sum<LPR>(s2) / (float)C + eps);
+  if (lr == 0) {
+    if (mean) mean[row] = mu;
+    if (rstd) rstd[row] = r;
+  }
+#pragma unroll
+  for (int q = 0; q < NCH; q++) {
+    const int c = (q * LPR + lr) * V;
+    if (c >= C) continue;
+    float o[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) o[i] = v[q * V + i] * r * (w ? w[c + i] : 1.f) + (b ? b[c + i] : 0.f);
+    store_v<V>(y + row * ldy + c, o);
+  }
+}
+
+// Rows wider than the registers: one block per row, three passes over it.
+template <typename T>
+__global__ void __launch_bounds__(256) k_norm_fwd_wide(const T* __restrict__ x, long ldx, int C,
+                                                       const float* __restrict__ w, const float* __restrict__ b,
+                                                       float eps, T* __restrict__ y, long ldy,
+                                                       float* __restrict__ mean, float* __restrict__ rstd) {
+  __shared__ float sh[2][4];
+  const long row = blockIdx.x;
+  const T* xr = x + row * ldx;
+  auto total = [&](float v, int k) {
+    v = row_sum<64>(v);
+    if ((threadIdx.x & 63) == 0) sh[k][threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (sh[k][0] + sh[k][1]) + (sh[k][2] + sh[k][3]);
+  };
+  float v, s = 0.f;
+  for (int c = threadIdx.x; c < C; c += 256) {
+    load_v<1>(xr + c, &v);
+    s += v;
+  }
+  const float mu = total(s, 0) / (float)C;
+  s = 0.f;
+  for (int c = threadIdx.x; c < C; c += 256) {
+    load_v<1>(xr + c, &v);
+    s += (v - mu) * (v - mu);
+  }
+  const float r = 1.f / sqrtf(total(s, 1) / (float)C + eps);
+  if (threadIdx.x == 0) {
+    if (mean) mean[row] = mu;
+    if (rstd) rstd[row] = r;
+  }
+  for (int c = threadIdx.x; c < C; c += 256) {
+    load_v<1>(xr + c, &v);
+    v = (v - mu) * r * (w ? w[c] : 1.f) + (b ? b[c] : 0.f);
+    store_v<1>(y + row * ldy + c, &v);
+  }
+}
+
+// Backward: a group of LPR lanes walks the rows group, group + groups, ...; dw and db of its columns stay in its
+// registers and are added over the block's groups through LDS. part: [blocks][2][C] (or dw, db themselves for one block).
+template <typename T, int V, int NCH, int LPR>
+__global__ void __launch_bounds__(64 * kWaves) k_norm_bwd(const T* __restrict__ x, long ldx, const T* __restrict__ dy,
+                                                          long lddy, long M, int C, const float* __restrict__ w,
+                                                          const float* __restrict__ mean,
+                                                          const float* __restrict__ rstd, T* __restrict__ dx,
+                                                          long lddx, float* __restrict__ dw, float* __restrict__ db,
+                                                          float* __restrict__ part) {
+  constexpr int E = NCH * V, GPB = 64 * kWaves / LPR;
+  static_assert(E <= kNormRegs, "registers of a row");
+  const int lr = threadIdx.x % LPR, grp = threadIdx.x / LPR;
+  float aw[E], ab[E], wv[E];
+#pragma unroll
+  for (int q = 0; q < NCH; q++)
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const int c = (q * LPR + lr) * V + i;
+      aw[q * V + i] = ab[q * V + i] = 0.f;
+      wv[q * V + i] = c < C ? (w ? w[c] : 1.f) : 0.f;
+    }
+  const float inv = 1.f / (float)C;
+  for (long row = (long)blockIdx.x * GPB + grp; row < M; row += (long)gridDim.x * GPB) {
+    float n[E], g[E];
+#pragma unroll
+    for (int q = 0; q < NCH; q++) {
+      const int c = (q * LPR + lr) * V;
+#pragma unroll
+      for (int i = 0; i < V; i++) n[q * V + i] = g[q * V + i] = 0.f;
+      if (c < C) {
+        load_v<V>(x + row * ldx + c, n + q * V);
+        load_v<V>(dy + row * lddy + c, g + q * V);
+      }
+    }
+    const float mu = mean[row], r = rstd[row];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+      n[i] = (n[i] - mu) * r;
+      aw[i] += g[i] * n[i];  // lanes past C add to columns that are never written
+      ab[i] += g[i];
+      g[i] *= wv[i];
+      s1 += g[i];
+      s2 += g[i] * n[i];
+    }
+    s1 = row_sum<LPR>(s1) * inv;
+    s2 = row_sum<LPR>(s2) * inv;
+#pragma unroll
+    for (int q = 0; q < NCH; q++) {
+      const int c = (q * LPR + lr) * V;
+      if (c >= C) continue;
+      float o[V];
+#pragma unroll
+      for (int i = 0; i < V; i++) o[i] = r * (g[q * V + i] - s1 - n[q * V + i] * s2);
+      store_v<V>(dx + row * lddx + c, o);
+    }
+  }
+  if (!part && !dw && !db) return;
+  // the block's groups, added in group order: one value of every column at a time
+  __shared__ float sh[2][GPB][LPR * V];
+#pragma unroll
+  for (int q = 0; q < NCH; q++) {
+    if (q) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      sh[0][grp][lr * V + i] = aw[q * V + i];
+      sh[1][grp][lr * V + i] = ab[q * V + i];
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 2 * LPR * V; e += 64 * kWaves) {
+      const int k = e / (LPR * V), c = e % (LPR * V), col = q * LPR * V + c;
+      if (col >= C) continue;
+      float s = 0.f;
+      for (int i = 0; i < GPB; i++) s += sh[k][i][c];
+      if (part) part[((long)blockIdx.x * 2 + k) * C + col] = s;
+      else if (k == 0 && dw) dw[col] = s;
+      else if (k == 1 && db) db[col] = s;
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_norm_bwd_wide(const T* __restrict__ x, long ldx, const T* __restrict__ dy,
+                                                       long lddy, int C, const float* __restrict__ w,
+                                                       const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                       T* __restrict__ dx, long lddx) {
+  __shared__ float sh[2][4];
+  const long row = blockIdx.x;
+  const float mu = mean[row], r = rstd[row];
+  float s1 = 0.f, s2 = 0.f, a, g;
+  for (int c = threadIdx.x; c < C; c += 256) {
+    load_v<1>(x + row * ldx + c, &a);
+    load_v<1>(dy + row * lddy + c, &g);
+    g *= w ? w[c] : 1.f;
+    s1 += g;
+    s2 += g * (a - mu) * r;
+  }
+  s1 = row_sum<64>(s1);
+  s2 = row_sum<64>(s2);
+  if ((threadIdx.x & 63) == 0) {
+    sh[0][threadIdx.x >> 6] = s1;
+    sh[1][threadIdx.x >> 6] = s2;
+  }
+  __syncthreads();
+  s1 = ((sh[0][0] + sh[0][1]) + (sh[0][2] + sh[0][3])) / (float)C;
+  s2 = ((sh[1][0] + sh[1][1]) + (sh[1][2] + sh[1][3])) / (float)C;
+  for (int c = threadIdx.x; c < C; c += 256) {
+    load_v<1>(x + row * ldx + c, &a);
+    load_v<1>(dy + row * lddy + c, &g);
+    a = r * (g * (w ? w[c] : 1.f) - s1 - (a - mu) * r * s2);
+    store_v<1>(dx + row * lddx + c, &a);
+  }
+}
+// dw and db partials of wide rows: 64 columns x a range of rows per block of four wavefronts.
+template <typename T>
+__global__ void __launch_bounds__(256) k_norm_cols_wide(const T* __restrict__ x, long ldx, const T* __restrict__ dy,
+                                                        long lddy, long M, int C, const float* __restrict__ mean,
+                                                        const float* __restrict__ rstd, float* __restrict__ part) {
+  __shared__ float sh[2][4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+  float sw = 0.f, sb = 0.f, a, g;
+  if (c < C)
+    for (long row = (long)blockIdx.y * 4 + wave; row < M; row += (long)gridDim.y * 4) {
+      load_v<1>(x + row * ldx + c, &a);
+      load_v<1>(dy + row * lddy + c, &g);
+      sw += g * (a - mean[row]) * rstd[row];
+      sb += g;
+    }
+  sh[0][wave][lane] = sw;
+  sh[1][wave][lane] = sb;
+  __syncthreads();
+  if (wave < 2 && c < C)
+    part[((long)blockIdx.y * 2 + wave) * C + c] = (sh[wave][0][lane] + sh[wave][1][lane]) + (sh[wave][2][lane] + sh[wave][3][lane]);
+}
+
+// dw, db = the partials' sums in a fixed order: 16 ranges of blocks per column, eight loads in flight each.
+__global__ void __launch_bounds__(256) k_norm_fold(const float* __restrict__ part, int blocks, int C,
+                                                   float* __restrict__ dw, float* __restrict__ db) {
+  __shared__ float sh[16][16];
+  const int e = threadIdx.x & 15, z = threadIdx.x >> 4, col = blockIdx.x * 16 + e;
+  const int per = (blocks + 15) / 16, end = min(blocks, (z + 1) * per);
+  float s = 0.f;
+  if (col < 2 * C) {
+    int i = z * per;
+    for (; i + 8 <= end; i += 8) {
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; q++) v[q] = part[(long)(i + q) * 2 * C + col];
+#pragma unroll
+      for (int q = 0; q < 8; q++) s += v[q];
+    }
+    for (; i < end; i++) s += part[(long)i * 2 * C + col];
+  }
+  sh[z][e] = s;
+  __syncthreads();
+  if (z || col >= 2 * C) return;
+  for (int q = 1; q < 16; q++) s += sh[q][e];
+  if (col < C) {
+    if (dw) dw[col] = s;
+  } else if (db) {
+    db[col - C] = s;
+  }
+}
+
+__global__ void k_norm_zero(float* dw, float* db, int C) {
+  for (int c = blockIdx.x * blockDim.x + threadIdx.x; c < C; c += gridDim.x * blockDim.x) {
+    if (dw) dw[c] = 0.f;
+    if (db) db[c] = 0.f;
+  }
+}
+
+// One call's arguments, and its dispatch over (V, NCH, LPR).
+template <typename T> struct NormCall {
+  const T *x, *dy;
+  T *y, *dx;
+  long ldx, lddy, ldy, lddx, M;
+  int C;
+  const float *w, *b;
+  float eps;
+  float *mean, *rstd;
+  const float *cmean, *crstd;
+  float *dw, *db;
+  hipStream_t st;
+
+  template <int V, int NCH, int LPR> int forward() const {
+    const long rows = 64 * kWaves / LPR;
+    k_norm_fwd<T, V, NCH, LPR><<<(unsigned)((M + rows - 1) / rows), 64 * kWaves, 0, st>>>(x, ldx, M, C, w, b, eps, y,
+                                                                                         ldy, mean, rstd);
+    PH_LAUNCH_CHECK();
+    return PH_OK;
+  }
+  template <int V, int NCH, int LPR> int backward() const {
+    const long rows = 64 * kWaves / LPR;
+    long blocks = (M + rows - 1) / rows;
+    if (blocks > 1024) blocks = 1024;
+    float* part = nullptr;
+    if (blocks > 1 && (dw || db)) {
+      part = (float*)scratch(kSlotNormPart, (size_t)blocks * 2 * C * 4);
+      if (!part) return PH_ERR_NOMEM;
+    }
+    k_norm_bwd<T, V, NCH, LPR><<<(unsigned)blocks, 64 * kWaves, 0, st>>>(x, ldx, dy, lddy, M, C, w, cmean, crstd, dx,
+                                                                         lddx, dw, db, part);
+    PH_LAUNCH_CHECK();
+    if (part) {
+      k_norm_fold<<<(unsigned)((2 * C + 15) / 16), 256, 0, st>>>(part, (int)blocks, C, dw, db);
+      PH_LAUNCH_CHECK();
+    }
+    return PH_OK;
+  }
+  template <int V, int NCH, int LPR> int go() const { return dy ? backward<V, NCH, LPR>() : forward<V, NCH, LPR>(); }
+  int wide() const {
+    if (!dy) {
+      k_norm_fwd_wide<T><<<(unsigned)M, 256, 0, st>>>(x, ldx, C, w, b, eps, y, ldy, mean, rstd);
+      PH_LAUNCH_CHECK();
+      return PH_OK;
+    }
+    k_norm_bwd_wide<T><<<(unsigned)M, 256, 0, st>>>(x, ldx, dy, lddy, C, w, cmean, crstd, dx, lddx);
+    PH_LAUNCH_CHECK();
+    if (!dw && !db) return PH_OK;
+    long ry = (M + 31) / 32;
+    if (ry > 128) ry = 128;
+    float* part = (float*)scratch(kSlotNormPart, (size_t)ry * 2 * C * 4);
+    if (!part) return PH_ERR_NOMEM;
+    k_norm_cols_wide<T><<<dim3((C + 63) / 64, (unsigned)ry), 256, 0, st>>>(x, ldx, dy, lddy, M, C, cmean, crstd, part);
+    PH_LAUNCH_CHECK();
+    k_norm_fold<<<(unsigned)((2 * C + 15) / 16), 256, 0, st>>>(part, (int)ry, C, dw, db);
+    PH_LAUNCH_CHECK();
+    return PH_OK;
+  }
+  template <int V> int by_width() const {
+    const int chunks = (C + V - 1) / V;  // accesses of a row
+    if (chunks <= 8) return go<V, 1, 8>();
+    if (chunks <= 16) return go<V, 1, 16>();
+    if (chunks <= 32) return go<V, 1, 32>();
+    if (chunks <= 64) return go<V, 1, 64>();
+    if (chunks <= 128) return go<V, 2, 64>();
+    if (chunks <= 256) return go<V, 4, 64>();
+    if constexpr (8 * V <= kNormRegs) {
+      if (chunks <= 512) return go<V, 8, 64>();
+    }
+    if constexpr (32 * V <= kNormRegs) {
+      if (chunks <= 1024) return go<V, 16, 64>();
+      if (chunks <= 2048) return go<V, 32, 64>();
+    }
+    return wide();
+  }
+  int run() const {
+    constexpr int V = sizeof(T) == 2 ? 8 : 4;
+    auto ok = [&](const void* p, long ld) { return !p || (((uintptr_t)p % 16) == 0 && ld % V == 0); };
+    const bool vec = C % V == 0 && ok(x, ldx) && ok(y, ldy) && ok(dy, lddy) && ok(dx, lddx);
+    return vec ? by_width<V>() : by_width<1>();
+  }
+};
+
+template <typename T> int norm_fwd_t(const void* x, size_t ldx, size_t M, size_t C, const float* w, const float* b,
+                                     float eps, void* y, size_t ldy, float* mean, float* rstd, hipStream_t st) {
+  NormCall<T> c{};
+  c.x = (const T*)x; c.y = (T*)y; c.ldx = (long)ldx; c.ldy = (long)ldy; c.M = (long)M; c.C = (int)C;
+  c.w = w; c.b = b; c.eps = eps; c.mean = mean; c.rstd = rstd; c.st = st;
+  return c.run();
+}
+template <typename T> int norm_bwd_t(const void* x, size_t ldx, const void* dy, size_t lddy, size_t M, size_t C,
+                                     const float* w, const float* mean, const float* rstd, void* dx, size_t lddx,
+                                     float* dw, float* db, hipStream_t st) {
+  NormCall<T> c{};
+  c.x = (const T*)x; c.dy = (const T*)dy; c.dx = (T*)dx; c.ldx = (long)ldx; c.lddy = (long)lddy; c.lddx = (long)lddx;
+  c.M = (long)M; c.C = (int)C; c.w = w; c.cmean = mean; c.crstd = rstd; c.dw = dw; c.db = db; c.st = st;
+  return c.run();
+}
+
+constexpr size_t kNormMaxCols = 1u << 20;
+constexpr size_t kNormMaxRows = 1u << 30;
+
+}  // namespace
+}  // namespace ph
+
+using namespace ph;
+
+extern "C" int ph_layer_norm(int dtype, const void* x, size_t ldx, size_t M, size_t C, const float* w, const float* b,
+                             float eps, void* y, size_t ldy, float* mean, float* rstd, void* stream) {
+  PH_REQUIRE(dtype == PH_F32 || dtype == PH_BF16, "layer_norm: dtype must be F32 or BF16");
+  PH_REQUIRE(C >= 1 && C <= kNormMaxCols && M <= kNormMaxRows, "layer_norm: %zu rows of %zu columns", M, C);
+  PH_REQUIRE(ldx >= C && ldy >= C, "layer_norm: row strides %zu, %zu below %zu columns", ldx, ldy, C);
+  PH_REQUIRE(eps >= 0.f, "layer_norm: eps %g", (double)eps);
+  if (M == 0) return PH_OK;
+  PH_REQUIRE(x && y, "layer_norm: x or y missing");
+  return dtype == PH_BF16 ? norm_fwd_t<uint16_t>(x, ldx, M, C, w, b, eps, y, ldy, mean, rstd, as_stream(stream))
+                          : norm_fwd_t<float>(x, ldx, M, C, w, b, eps, y, ldy, mean, rstd, as_stream(stream));
+}
+
+extern "C" int ph_layer_norm_grad(int dtype, const void* x, size_t ldx, const void* dy, size_t lddy, size_t M, size_t C,
+                                  const float* w, const float* mean, const float* rstd, void* dx, size_t lddx,
+                                  float* dw, float* db, void* stream) {
+  PH_REQUIRE(dtype == PH_F32 || dtype == PH_BF16, "layer_norm_grad: dtype must be F32 or BF16");
+  PH_REQUIRE(C >= 1 && C <= kNormMaxCols && M <= kNormMaxRows, "layer_norm_grad: %zu rows of %zu columns", M, C);
+  PH_REQUIRE(ldx >= C && lddy >= C && lddx >= C, "layer_norm_grad: a row stride is below %zu columns", C);
+  if (M == 0) {  // no rows: the columns' sums are zero
+    if (!dw && !db) return PH_OK;
+    k_norm_zero<<<ceil_div(C, 256), 256, 0, as_stream(stream)>>>(dw, db, (int)C);
+    PH_LAUNCH_CHECK();
+    return PH_OK;
+  }
+  PH_REQUIRE(x && dy && dx && mean && rstd, "layer_norm_grad: x, dy, dx, mean or rstd missing");
+  return dtype == PH_BF16 ? norm_bwd_t<uint16_t>(x, ldx, dy, lddy, M, C, w, mean, rstd, dx, lddx, dw, db, as_stream(stream))
+                          : norm_bwd_t<float>(x, ldx, dy, lddy, M, C, w, mean, rstd, dx, lddx, dw, db, as_stream(stream));
+}

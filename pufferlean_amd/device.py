@@ -476,3 +476,202 @@ def sample_actions_cont(y, dim, *, rng_state, ls_lo=-20.0, ls_hi=2.0, out=None):
     L.call("ph_sample_actions_cont", _DT[y.dtype], _p(y), y.stride(0), N, dim, rng_state & 0xFFFFFFFFFFFFFFFF,
            ls_lo, ls_hi, _p(out), _stream())
     return out
+
+
+# ---- state-space policy layer: normalisation, scan, gated feed-forward ---------------------------------
+def _act_dtype(x, what):
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{what} takes float32 or bfloat16, not {x.dtype}")
+    return _DT[x.dtype]
+
+
+def _like(t, x, shape, what):
+    """t has x's dtype, the given shape and a contiguous last dimension."""
+    if t.dtype != x.dtype or t.shape != shape or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{what} must be {x.dtype} {tuple(shape)} with a contiguous last dimension, "
+                         f"not {t.dtype} {tuple(t.shape)}")
+    return t
+
+
+def _f32(t, shape, what):
+    """t (may be None) is a contiguous float32 tensor of the given shape."""
+    if t is not None and (t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous()):
+        raise ValueError(f"{what} must be contiguous float32 {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+    return t
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _rows(t):
+    """Row stride of a matrix whose rows are contiguous (one row: its length)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def layer_norm(x, w=None, b=None, *, eps=1e-5, out=None, mean=None, rstd=None):
+    """Layer normalisation of the rows of x [M, C] (float32 or bfloat16, row stride honoured), w and b float32 [C].
+    Returns (y, mean, rstd), the statistics float32 [M] for layer_norm_grad."""
+    _dev(x, w, b)
+    dt = _act_dtype(x, "layer_norm")
+    M, C_ = x.shape
+    _like(x, x, x.shape, "x")
+    _f32(w, (C_,), "w"), _f32(b, (C_,), "b")
+    y = torch.empty((M, C_), device=x.device, dtype=x.dtype) if out is None else _like(out, x, x.shape, "out")
+    mean = torch.empty(M, device=x.device) if mean is None else _f32(mean, (M,), "mean")
+    rstd = torch.empty(M, device=x.device) if rstd is None else _f32(rstd, (M,), "rstd")
+    L.call("ph_layer_norm", dt, x.data_ptr(), _rows(x), M, C_, _ptr(w), _ptr(b), eps, y.data_ptr(), _rows(y),
+           mean.data_ptr(), rstd.data_ptr(), _stream())
+    return y, mean, rstd
+
+
+def layer_norm_grad(x, w, mean, rstd, dy, *, dx=None, dw=None, db=None):
+    """Gradient of layer_norm from its input and statistics: (dx, dw, db), dw and db float32 [C]."""
+    _dev(x, w, mean, rstd, dy)
+    dt = _act_dtype(x, "layer_norm_grad")
+    M, C_ = x.shape
+    _like(x, x, x.shape, "x"), _like(dy, x, x.shape, "dy")
+    _f32(w, (C_,), "w"), _f32(mean, (M,), "mean"), _f32(rstd, (M,), "rstd")
+    dx = torch.empty((M, C_), device=x.device, dtype=x.dtype) if dx is None else _like(dx, x, x.shape, "dx")
+    dw = torch.empty(C_, device=x.device) if dw is None else _f32(dw, (C_,), "dw")
+    db = torch.empty(C_, device=x.device) if db is None else _f32(db, (C_,), "db")
+    L.call("ph_layer_norm_grad", dt, x.data_ptr(), _rows(x), dy.data_ptr(), _rows(dy), M, C_, _ptr(w),
+           mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), _rows(dx), dw.data_ptr(), db.data_ptr(), _stream())
+    return dx, dw, db
+
+
+def _ssm_args(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, done, first, h0, win0):
+    """The checked ph_ssm_args of [T, B, C] (or single-step [B, C]) inputs."""
+    _dev(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, done, first, h0, win0)
+    dt = _act_dtype(x, "ssm")
+    lead, C_ = x.shape[:-1], x.shape[-1]
+    T, B = lead if len(lead) == 2 else (1, lead[0])
+    if A.dim() != 2:
+        raise ValueError("A must be [C, N]")
+    N, K = A.shape[1], 0 if conv_w is None else conv_w.shape[-1]
+    _like(x, x, x.shape, "x"), _like(delta, x, x.shape, "delta")
+    bc = torch.Size((*lead, groups * N))
+    _like(Bm, x, bc, "Bm"), _like(Cm, x, bc, "Cm")
+    if z is not None:
+        _like(z, x, x.shape, "z")
+    _f32(A, (C_, N), "A"), _f32(D, (C_,), "D"), _f32(dt_bias, (C_,), "dt_bias")
+    _f32(conv_w, (C_, K), "conv_w"), _f32(conv_b, (C_,), "conv_b")
+    _f32(done, (T, B), "done"), _f32(first, (B,), "first"), _f32(h0, (B, C_, N), "h0")
+    if K < 2:
+        win0 = None
+    _f32(win0, (B, K - 1, C_), "win0")
+    strides = []
+    for t in (x, z, delta, Bm, Cm):
+        strides += (0, 0) if t is None else t.stride()[:2] if len(lead) == 2 else (0, t.stride(0))
+    return L.SsmArgs(dt, T, B, C_, N, groups, K, _ptr(x), _ptr(z), _ptr(delta), _ptr(Bm), _ptr(Cm), *strides, _ptr(A),
+                     _ptr(D), _ptr(dt_bias), _ptr(conv_w), _ptr(conv_b), _ptr(done), _ptr(first), _ptr(h0), _ptr(win0))
+
+
+def ssm_scan(x, delta, A, Bm, Cm, *, D=None, z=None, dt_bias=None, conv_w=None, conv_b=None, groups=1, done=None,
+             first=None, h0=None, win0=None, out=None, h_out=None, win_out=None, save=False):
+    """Selective state-space scan with its short causal convolution over [T, B] steps (ph_ssm_scan): x, delta, z
+    [T, B, C] and Bm, Cm [T, B, groups*N] in float32 or bfloat16, any strides with a contiguous last dimension;
+    A [C, N], D, dt_bias, conv_b [C], conv_w [C, K], done [T, B], first [B], h0 [B, C, N], win0 [B, K-1, C] float32.
+    h_out and win_out receive the carried state (they may be h0 and win0). Returns y, or (y, saved) with save=True, saved
+    being what ssm_scan_grad needs."""
+    a = _ssm_args(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, done, first, h0, win0)
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype) if out is None else _like(out, x, x.shape, "out")
+    _f32(h_out, (a.B, a.C, a.N), "h_out")
+    if a.K < 2:
+        win_out = None
+    _f32(win_out, (a.B, a.K - 1, a.C), "win_out")
+    ref = C.byref(a)
+    keep = torch.empty(L.lib().ph_ssm_keep_floats(ref), device=x.device) if save else None
+    L.call("ph_ssm_scan", ref, y.data_ptr(), y.stride(0), y.stride(1), _ptr(h_out), _ptr(win_out), _ptr(keep), _stream())
+    return (y, keep) if save else y
+
+
+def ssm_scan_grad(x, delta, A, Bm, Cm, saved, dy, *, D=None, z=None, dt_bias=None, conv_w=None, conv_b=None, groups=1,
+                  done=None, first=None, win0=None, dx=None, ddelta=None, dBm=None, dCm=None, dz=None):
+    """Gradient of ssm_scan from its arguments and what it saved. Returns a dict: dx, ddelta, dBm, dCm (and dz) in the
+    activations' dtype, written into the given tensors where there are any, and dA (and dD, ddt_bias, dconv_w, dconv_b)
+    in float32. The carried-in state and window are constants."""
+    a = _ssm_args(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, done, first, None, win0)
+    _like(dy, x, x.shape, "dy")
+    ref = C.byref(a)
+    _f32(saved, (L.lib().ph_ssm_keep_floats(ref),), "saved")
+    g = {}
+    for name, t, like in (("dx", dx, x), ("dz", dz, z), ("ddelta", ddelta, delta), ("dBm", dBm, Bm), ("dCm", dCm, Cm)):
+        if like is not None:
+            g[name] = torch.empty(like.shape, device=x.device, dtype=x.dtype) if t is None else _like(t, x, like.shape, name)
+    strides = []
+    for name in ("dx", "dz", "ddelta", "dBm", "dCm"):
+        strides += g[name].stride()[:2] if name in g else (0, 0)
+    for name, p in (("dA", A), ("dD", D), ("ddt_bias", dt_bias), ("dconv_w", conv_w), ("dconv_b", conv_b)):
+        if p is not None:
+            g[name] = torch.empty_like(p)
+    c = L.SsmGrads(*(_ptr(g.get(n)) for n in ("dx", "dz", "ddelta", "dBm", "dCm")), *strides,
+                   *(_ptr(g.get(n)) for n in ("dA", "dD", "ddt_bias", "dconv_w", "dconv_b")))
+    L.call("ph_ssm_scan_grad", ref, saved.data_ptr(), dy.data_ptr(), dy.stride(0), dy.stride(1), C.byref(c), _stream())
+    return g
+
+
+def ssm_step(x, delta, A, Bm, Cm, h, win=None, *, D=None, z=None, dt_bias=None, conv_w=None, conv_b=None, groups=1,
+             first=None, out=None):
+    """One step of ssm_scan for B sequences: x, delta, z [B, C], Bm, Cm [B, groups*N]; the state h [B, C, N] and the
+    convolution's window win [B, K-1, C] (float32) are updated in place, cleared first where first[b] is set."""
+    a = _ssm_args(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, None, first, h, win)
+    if a.K > 1 and win is None:
+        raise ValueError("win is needed for a convolution of two taps or more")
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype) if out is None else _like(out, x, x.shape, "out")
+    L.call("ph_ssm_step", C.byref(a), y.data_ptr(), y.stride(0), h.data_ptr(), _ptr(win) if a.K > 1 else 0, _stream())
+    return y
+
+
+_ACT = {"silu": L.PH_ACT_SILU, "gelu": L.PH_ACT_GELU}
+
+
+def _ffn_shapes(x, w_in, w_out, act):
+    _dev(x, w_in, w_out)
+    dt = _act_dtype(x, "gated_ffn")
+    if act not in _ACT:
+        raise ValueError(f"gated_ffn: activation {act!r} is not one of {sorted(_ACT)}")
+    M, D = x.shape
+    F = w_out.shape[1]
+    _like(x, x, x.shape, "x"), _like(w_in, x, (2 * F, D), "w_in"), _like(w_out, x, (D, F), "w_out")
+    if not (w_in.is_contiguous() and w_out.is_contiguous()):
+        raise ValueError("gated_ffn: the weights must be contiguous")
+    return dt, M, D, F
+
+
+def _pitch(n):
+    return (n + 7) // 8 * 8
+
+
+def gated_ffn(x, w_in, w_out, *, act="silu", out=None, save=False):
+    """Gated feed-forward block (act(x Wg^T) * (x Wv^T)) Wo^T: x [M, D], w_in [2F, D] with the gate and value rows of unit
+    j at 2j and 2j + 1, w_out [D, F], float32 or bfloat16. Returns y, or (y, saved) with save=True, saved being what
+    gated_ffn_grad needs."""
+    dt, M, D, F = _ffn_shapes(x, w_in, w_out, act)
+    y = torch.empty((M, D), device=x.device, dtype=x.dtype) if out is None else _like(out, x, x.shape, "out")
+    ab = h = None
+    if save:
+        ab = torch.empty((M, _pitch(2 * F)), device=x.device, dtype=x.dtype)
+        h = torch.empty((M, _pitch(F)), device=x.device, dtype=x.dtype)
+    L.call("ph_ffn", dt, _ACT[act], M, D, F, x.data_ptr(), _rows(x), w_in.data_ptr(), w_out.data_ptr(), _ptr(ab), _ptr(h),
+           y.data_ptr(), _rows(y), _stream())
+    return (y, (ab, h)) if save else y
+
+
+def gated_ffn_grad(x, w_in, w_out, saved, dy, *, act="silu", dx=None, dw_in=None, dw_out=None, dw_dtype=None):
+    """Gradient of gated_ffn: (dx, dw_in, dw_out), the weights' in dw_dtype (x's dtype, or float32)."""
+    dt, M, D, F = _ffn_shapes(x, w_in, w_out, act)
+    _like(dy, x, x.shape, "dy")
+    ab, h = saved
+    _like(ab, x, (M, _pitch(2 * F)), "saved"), _like(h, x, (M, _pitch(F)), "saved")
+    dwt = dw_dtype or (x.dtype if dw_in is None else dw_in.dtype)
+    dx = torch.empty((M, D), device=x.device, dtype=x.dtype) if dx is None else _like(dx, x, x.shape, "dx")
+    dw_in = torch.empty((2 * F, D), device=x.device, dtype=dwt) if dw_in is None else dw_in
+    dw_out = torch.empty((D, F), device=x.device, dtype=dwt) if dw_out is None else dw_out
+    for t, shape, what in ((dw_in, (2 * F, D), "dw_in"), (dw_out, (D, F), "dw_out")):
+        if t.dtype != dwt or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous {dwt} {shape}")
+    L.call("ph_ffn_grad", dt, _ACT[act], M, D, F, x.data_ptr(), _rows(x), w_in.data_ptr(), w_out.data_ptr(), ab.data_ptr(),
+           h.data_ptr(), dy.data_ptr(), _rows(dy), dx.data_ptr(), _rows(dx), _DT[dwt], dw_in.data_ptr(), dw_out.data_ptr(),
+           _stream())
+    return dx, dw_in, dw_out

@@ -1,0 +1,191 @@
+"""The gated feed-forward block and its gradient against the definition in 64 bits.
+
+Bars, relative 2-norm. fp32: sums of up to K products round K^0.5 times 2^-24 of their size, under 1e-5 for the sizes here.
+bf16: the operands are exact and the sums fp32, so what is lost are the roundings of stored values (h, the projections, the
+projections' gradients, the result), at most 2^-8 each; up to three of them meet in a result. Each rounds one term of a sum
+by itself, so errors are measured against the root of the sum of the terms' squares, which a sum that cancels falls below."""
+import numpy as np
+import pytest
+import torch
+
+import policy_layer_ref as R
+from pufferlean_amd import _lib as L
+from pufferlean_amd import device as D
+from pufferlean_amd import rng
+
+pytestmark = pytest.mark.gpu
+BARS = {torch.float32: 1e-5, torch.bfloat16: 3 * R.BF16}
+
+
+def cu(seed, *shape, scale=1.0, dtype=torch.float32):
+    return torch.from_numpy(rng.normal(seed, int(np.prod(shape))).reshape(shape) * scale).float().to("cuda", dtype)
+
+
+def case(M, Dm, F, dt):
+    return (cu(1, M, Dm, dtype=dt), cu(2, 2 * F, Dm, scale=Dm ** -0.5, dtype=dt), cu(3, Dm, F, scale=F ** -0.5, dtype=dt),
+            cu(4, M, Dm, dtype=dt))
+
+
+def check(x, wi, wo, dy, act="silu", dw_dtype=None):
+    bar = BARS[x.dtype]
+    y, saved = D.gated_ffn(x, wi, wo, act=act, save=True)
+    assert R.rel(D.gated_ffn(x, wi, wo, act=act), y) <= bar
+    dx, dwi, dwo = D.gated_ffn_grad(x, wi, wo, saved, dy, act=act, dw_dtype=dw_dtype)
+    xr, ir, outr = R.leaf(x), R.leaf(wi), R.leaf(wo)
+    yr = R.ffn(xr, ir, outr, act)
+    gx, gi, go = torch.autograd.grad(yr, (xr, ir, outr), dy.double().cpu())
+    with torch.no_grad():
+        a = (xr @ ir[0::2].T).requires_grad_(True)
+        v = (xr @ ir[1::2].T).requires_grad_(True)
+        with torch.enable_grad():
+            h = R.glu(a, v, act)
+        da, dv = torch.autograd.grad(h, (a, v), dy.double().cpu() @ outr)
+        dab2 = torch.stack([da, dv], -1).reshape(len(x), -1) ** 2
+    for got, ref, terms in ((y, yr, (h ** 2) @ (outr ** 2).T), (dx, gx, dab2 @ ir ** 2), (dwi, gi, dab2.T @ xr ** 2),
+                            (dwo, go, (dy.double().cpu() ** 2).T @ h ** 2)):
+        size = max(float(terms.detach().sum().sqrt()), float(ref.norm()))
+        assert float((got.double().cpu() - ref).norm()) <= bar * size
+    return y, dx, dwi, dwo
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("M,Dm,F", [(1, 64, 96), (2, 8, 8), (3, 7, 5), (8, 512, 344), (16, 128, 128), (17, 96, 203), (33, 203, 64),
+                                    (64, 64, 1), (65, 1, 33), (130, 264, 520), (300, 128, 688)])
+def test_sizes(gpu, M, Dm, F, act, dt):
+    check(*case(M, Dm, F, dt), act)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,Dm,F", [(4096, 128, 344), (3001, 200, 333), (2048, 512, 1024)])
+def test_many_rows(gpu, M, Dm, F, dt):
+    check(*case(M, Dm, F, dt))
+
+
+def test_fp32_weight_gradients_of_bf16(gpu):
+    x, wi, wo, dy = case(700, 128, 264, torch.bfloat16)
+    _, _, dwi, dwo = check(x, wi, wo, dy, dw_dtype=torch.float32)
+    assert dwi.dtype == dwo.dtype == torch.float32
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("off", [0, 1, 8])
+def test_strided_rows(gpu, dt, off):
+    x, wi, wo, dy = case(200, 128, 96, dt)
+    ref = check(x, wi, wo, dy)
+
+    def wide(t):
+        buf = torch.full((200, 128 + 16), 5.0, device="cuda", dtype=dt)
+        buf[:, off:off + 128] = t
+        return buf[:, off:off + 128]
+    got = check(wide(x), wi, wo, wide(dy))
+    for a, b in zip(ref, got):
+        assert R.rel(a, b) <= BARS[dt]
+    out = torch.full((200, 144), 5.0, device="cuda", dtype=dt)
+    D.gated_ffn(x, wi, wo, out=out[:, off:off + 128])
+    assert R.rel(out[:, off:off + 128], ref[0]) <= BARS[dt]
+    assert torch.all(out[:, :off] == 5) and torch.all(out[:, off + 128:] == 5)
+
+
+def test_saturated_gates(gpu):
+    """Gates far on both sides: the activation is the identity or zero, and its gradient finite."""
+    x, wi, wo, dy = case(40, 64, 48, torch.float32)
+    wi[0::4] *= 60.0
+    wi[0::8] *= -1.0
+    for act in ("silu", "gelu"):
+        check(x, wi, wo, dy, act)
+
+
+def test_non_finite_rows_stay_theirs(gpu):
+    x, wi, wo, dy = case(70, 64, 96, torch.bfloat16)
+    ref = D.gated_ffn(x, wi, wo)
+    x[13] = float("nan")
+    x[40, 3] = float("inf")
+    y = D.gated_ffn(x, wi, wo)
+    ok = [i for i in range(70) if i not in (13, 40)]
+    assert torch.equal(y[ok], ref[ok]) and not torch.isfinite(y[13]).any()
+
+
+def test_no_rows(gpu):
+    x, wi, wo, dy = case(1, 16, 24, torch.bfloat16)
+    x = dy = x[:0]
+    y, saved = D.gated_ffn(x, wi, wo, save=True)
+    dx, dwi, dwo = D.gated_ffn_grad(x, wi, wo, saved, dy)
+    assert y.shape == (0, 16) and dx.shape == (0, 16) and not dwi.any() and not dwo.any()
+
+
+def test_gradient_against_differences(gpu):
+    x, wi, wo, dy = case(50, 32, 40, torch.float32)
+    y, saved = D.gated_ffn(x, wi, wo, save=True)
+    grads = D.gated_ffn_grad(x, wi, wo, saved, dy)
+    f = lambda *a: float((D.gated_ffn(*a).double() * dy.double()).sum())
+    e = 2.0 ** -7
+    for i, g in enumerate(grads):
+        base = [x, wi, wo]
+        v = cu(20 + i, *base[i].shape, scale=float(base[i].abs().mean()))
+        up, dn = list(base), list(base)
+        up[i], dn[i] = base[i] + e * v, base[i] - e * v
+        want, size = float((g * v).sum()), float(g.norm() * v.norm())
+        assert abs((f(*up) - f(*dn)) / (2 * e) - want) <= 2e-3 * (abs(want) + 0.1 * size)
+
+
+def test_same_twice_and_on_another_stream(gpu):
+    x, wi, wo, dy = case(1500, 136, 344, torch.bfloat16)
+    a = check(x, wi, wo, dy)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y, saved = D.gated_ffn(x, wi, wo, save=True)
+        b = (y, *D.gated_ffn_grad(x, wi, wo, saved, dy))
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("M", [8, 2000])
+def test_graph_replays(gpu, M):
+    x, wi, wo, dy = case(M, 128, 344, torch.bfloat16)
+    check(x, wi, wo, dy)
+
+    def both():
+        y, saved = D.gated_ffn(x, wi, wo, save=True)
+        return [y, D.gated_ffn(x, wi, wo), *D.gated_ffn_grad(x, wi, wo, saved, dy)]
+    ref = [t.clone() for t in both()]
+    g, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st), torch.cuda.graph(g, stream=st):
+        out = both()
+    torch.cuda.current_stream().wait_stream(st)
+    for _ in range(3):
+        for t in out:
+            t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ref, out))
+        (torch.ones(1000, device="cuda") * 2).sum().item()
+
+
+def test_refusals(gpu):
+    x, wi, wo, dy = case(4, 16, 24, torch.float32)
+    with pytest.raises(TypeError):
+        D.gated_ffn(x.half(), wi, wo)
+    with pytest.raises(ValueError):
+        D.gated_ffn(x, wi[:-2], wo)
+    with pytest.raises(ValueError):
+        D.gated_ffn(x, wi.bfloat16(), wo)
+    with pytest.raises(ValueError):
+        D.gated_ffn(x, wi, wo, act="relu")
+    with pytest.raises(ValueError):
+        D.gated_ffn(x, wi, wo.t().contiguous().t())
+    y, saved = D.gated_ffn(x, wi, wo, save=True)
+    with pytest.raises(ValueError):
+        D.gated_ffn_grad(x, wi, wo, saved, dy[:2])
+    with pytest.raises(L.PufferHipError):
+        D.gated_ffn_grad(x, wi, wo, saved, dy, dw_dtype=torch.bfloat16)
+    lib = L.lib()
+    p = x.data_ptr()
+    assert lib.ph_ffn(L.PH_F64, 0, 4, 16, 24, p, 16, p, p, None, None, p, 16, None) == L.PH_ERR_ARG
+    assert lib.ph_ffn(L.PH_F32, 2, 4, 16, 24, p, 16, p, p, None, None, p, 16, None) == L.PH_ERR_ARG
+    assert lib.ph_ffn(L.PH_F32, 0, 4, 16, 24, p, 15, p, p, None, None, p, 16, None) == L.PH_ERR_ARG
+    assert lib.ph_ffn(L.PH_F32, 0, 4, 16, 24, p, 16, p, p, p, None, p, 16, None) == L.PH_ERR_ARG
+    assert lib.ph_ffn(L.PH_F32, 0, 4, 0, 24, p, 16, p, p, None, None, p, 16, None) == L.PH_ERR_ARG

@@ -1,0 +1,201 @@
+"""Layer normalisation and its gradient against the definition in 64 bits.
+
+Bars: fp32 sums of at most 32 values per lane and 6 folds keep a row's statistics within 38 rounding errors of 2^-24
+(2.3e-6); the columns' sums add rows in runs of up to a few hundred, 1e-5. bf16 results add their one rounding. dx is the
+difference of three terms that may cancel (two columns: to the last digit), so its error is measured against them."""
+import numpy as np
+import pytest
+import torch
+
+import policy_layer_ref as R
+from pufferlean_amd import _lib as L
+from pufferlean_amd import device as D
+from pufferlean_amd import rng
+
+pytestmark = pytest.mark.gpu
+ROW, COL = 3e-6, 1e-5
+
+
+def cu(seed, *shape, scale=1.0, dtype=torch.float32):
+    return torch.from_numpy(rng.normal(seed, int(np.prod(shape))).reshape(shape) * scale).float().to("cuda", dtype)
+
+
+def laid(x, layout):
+    if layout == "packed":
+        return x.clone()
+    M, C = x.shape
+    buf = torch.full((M, C + 3), 7.0, device="cuda", dtype=x.dtype)
+    buf[:, 1:C + 1] = x
+    return buf[:, 1:C + 1]
+
+
+def case(M, C, dt, layout="packed", affine=True, offset=0.0):
+    x = laid((cu(1, M, C) + offset).to(dt), layout)
+    dy = laid(cu(2, M, C, dtype=dt), layout)
+    w = 1 + cu(3, C, scale=0.2) if affine else None
+    b = cu(4, C, scale=0.2) if affine else None
+    return x, dy, w, b
+
+
+def check(x, dy, w, b, row=ROW, col=COL):
+    out = R.BF16 if x.dtype == torch.bfloat16 else 0.0
+    y, mean, rstd = D.layer_norm(x, w, b)
+    dx, dw, db = D.layer_norm_grad(x, w, mean, rstd, dy)
+    xr, wr, br = R.leaf(x), R.leaf(w), R.leaf(b)
+    one = torch.ones(x.shape[1], dtype=torch.float64, requires_grad=True)
+    zero = torch.zeros(x.shape[1], dtype=torch.float64, requires_grad=True)
+    wr, br = one if wr is None else wr, zero if br is None else br
+    yr = R.layer_norm(xr, wr, br)
+    gx, gw, gb = torch.autograd.grad(yr, (xr, wr, br), dy.double().cpu())
+    assert R.rel(y, yr) <= row + out
+    with torch.no_grad():
+        n, g, r = R.layer_norm(xr, None, None), dy.double().cpu() * wr, rstd.double().cpu()[:, None]
+        terms = (r * (g.abs() + g.mean(1, keepdim=True).abs() + (n * (g * n).mean(1, keepdim=True)).abs())).norm()
+    assert float((dx.double().cpu() - gx).norm()) <= 3 * row * float(terms) + out * float(gx.norm())
+    if x.shape[1] > 1:  # of a row of one column n is zero, and so is dw
+        assert R.rel(dw, gw) <= col
+    assert R.rel(db, gb) <= col
+    return y, dx, dw, db
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("C", [1, 2, 7, 8, 9, 31, 64, 96, 128, 203, 255, 256, 512, 640, 1000, 1024, 2040, 2048])
+@pytest.mark.parametrize("M", [1, 3, 33, 130])
+def test_widths(gpu, M, C, dt):
+    check(*case(M, C, dt))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,C", [(5, 2049), (70, 4096), (3, 5001)])
+def test_wide_rows(gpu, M, C, dt):
+    # three passes over the row, 256 threads adding up to 20 values each: 20 + 8 folds
+    check(*case(M, C, dt))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,C", [(9000, 128), (4097, 203), (20011, 64), (1500, 1024)])
+def test_many_rows(gpu, M, C, dt):
+    check(*case(M, C, dt))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("affine", [True, False])
+def test_strided_rows_and_no_affine(gpu, dt, affine):
+    x, dy, w, b = case(300, 96, dt, "strided", affine)
+    got = check(x, dy, w, b)
+    again = check(x.clone(), dy.clone(), w, b)
+    for a, c in zip(got, again):  # the layout changes no value of a row; column sums keep their order
+        assert R.rel(a, c) <= COL
+    out = torch.full((300, 99), 7.0, device="cuda", dtype=dt)
+    D.layer_norm(x, w, b, out=out[:, 1:97])
+    assert torch.all(out[:, 0] == 7) and torch.all(out[:, 97:] == 7)
+
+
+def test_large_offset_keeps_its_digits(gpu):
+    # the mean is 1000 times the deviation: x itself holds 2^-24 * 1000 of a deviation, and so does the mean
+    x, dy, w, b = case(64, 512, torch.float32, offset=1000.0)
+    check(x, dy, w, b, row=3e-4, col=3e-4)
+
+
+def test_constant_and_non_finite_rows(gpu):
+    x, dy, w, b = case(8, 64, torch.float32)
+    x[1] = 2.5
+    x[3, 5] = float("nan")
+    x[5, 7] = float("inf")
+    y, mean, rstd = D.layer_norm(x, w, b)
+    assert torch.equal(y[1], b) and torch.isnan(y[3]).all() and torch.isnan(y[5]).all()
+    good = [0, 1, 2, 4, 6, 7]
+    assert torch.isfinite(y[good]).all()
+    dx, _, _ = D.layer_norm_grad(x, w, mean, rstd, dy)
+    assert torch.isfinite(dx[good]).all() and torch.isnan(dx[3]).all()
+
+
+def test_no_rows(gpu):
+    x = torch.empty(0, 16, device="cuda")
+    w = torch.ones(16, device="cuda")
+    y, mean, rstd = D.layer_norm(x, w)
+    dx, dw, db = D.layer_norm_grad(x, w, mean, rstd, x, dw=torch.ones(16, device="cuda"))
+    assert y.shape == (0, 16) and dx.shape == (0, 16) and not dw.any() and not db.any()
+
+
+def test_in_place(gpu):
+    x, dy, w, b = case(100, 96, torch.bfloat16)
+    y, mean, rstd = D.layer_norm(x, w, b)
+    dx, _, _ = D.layer_norm_grad(x, w, mean, rstd, dy)
+    g = dy.clone()
+    D.layer_norm_grad(x, w, mean, rstd, g, dx=g)
+    assert torch.equal(g, dx)
+    D.layer_norm(x, w, b, out=x)
+    assert torch.equal(x, y)
+
+
+def test_gradient_against_differences(gpu):
+    x, dy, w, b = case(40, 96, torch.float32)
+    y, mean, rstd = D.layer_norm(x, w, b)
+    dx, dw, db = D.layer_norm_grad(x, w, mean, rstd, dy)
+    f = lambda x, w, b: float((D.layer_norm(x, w, b)[0].double() * dy.double()).sum())
+    vx, vw, vb = cu(11, 40, 96), cu(12, 96), cu(13, 96)
+    e = 2.0 ** -7  # difference error e^2, rounding 2^-24 / e of |y| |dy|
+    for args, want in (((vx, 0, 0), (dx * vx).sum()), ((0, vw, 0), (dw * vw).sum()), ((0, 0, vb), (db * vb).sum())):
+        d = (f(x + e * args[0], w + e * args[1], b + e * args[2]) - f(x - e * args[0], w - e * args[1], b - e * args[2])) / (2 * e)
+        scale = float(vx.norm() * dx.norm()) * 0.05 + abs(float(want))
+        assert abs(d - float(want)) <= 2e-3 * scale
+
+
+def test_same_twice_and_on_another_stream(gpu):
+    x, dy, w, b = case(5000, 203, torch.float32)
+    a = check(x, dy, w, b)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y, mean, rstd = D.layer_norm(x, w, b)
+        c = (y, *D.layer_norm_grad(x, w, mean, rstd, dy))
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(a, c))
+
+
+def test_graph_replays(gpu):
+    x, dy, w, b = case(3000, 128, torch.bfloat16)
+    ref = check(x, dy, w, b)
+    y, mean, rstd = torch.empty_like(x), torch.empty(3000, device="cuda"), torch.empty(3000, device="cuda")
+    dx, dw, db = torch.empty_like(x), torch.empty(128, device="cuda"), torch.empty(128, device="cuda")
+    g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s), torch.cuda.graph(g, stream=s):
+        D.layer_norm(x, w, b, out=y, mean=mean, rstd=rstd)
+        D.layer_norm_grad(x, w, mean, rstd, dy, dx=dx, dw=dw, db=db)
+    torch.cuda.current_stream().wait_stream(s)
+    for _ in range(3):
+        for t in (y, dx, dw, db):
+            t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ref, (y, dx, dw, db)))
+        (torch.ones(1000, device="cuda") * 2).sum().item()
+
+
+def test_refusals(gpu):
+    x = torch.ones(4, 8, device="cuda")
+    w = torch.ones(8, device="cuda")
+    with pytest.raises(TypeError):
+        D.layer_norm(x.double(), w)
+    with pytest.raises(ValueError):
+        D.layer_norm(x, w[:4])
+    with pytest.raises(ValueError):
+        D.layer_norm(x, w.bfloat16())
+    with pytest.raises(ValueError):
+        D.layer_norm(x.t(), None)  # rows are not contiguous
+    with pytest.raises(ValueError):
+        D.layer_norm(x, w, out=torch.ones(4, 8, device="cuda", dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        D.layer_norm(x.cpu(), None)
+    lib = L.lib()
+    p = x.data_ptr()
+    assert lib.ph_layer_norm(L.PH_F64, p, 8, 4, 8, None, None, 1e-5, p, 8, None, None, None) == L.PH_ERR_ARG
+    assert lib.ph_layer_norm(L.PH_F32, p, 7, 4, 8, None, None, 1e-5, p, 8, None, None, None) == L.PH_ERR_ARG
+    assert lib.ph_layer_norm(L.PH_F32, p, 8, 4, 0, None, None, 1e-5, p, 8, None, None, None) == L.PH_ERR_ARG
+    assert lib.ph_layer_norm(L.PH_F32, None, 8, 4, 8, None, None, 1e-5, p, 8, None, None, None) == L.PH_ERR_ARG
+    assert lib.ph_layer_norm(L.PH_F32, p, 8, 4, 8, None, None, -1.0, p, 8, None, None, None) == L.PH_ERR_ARG
+    assert lib.ph_layer_norm_grad(L.PH_F32, p, 8, p, 8, 4, 8, None, None, None, p, 8, None, None, None) == L.PH_ERR_ARG
+    assert lib.ph_layer_norm_grad(L.PH_F32, p, 8, p, 8, 4, 8, None, p, p, p, 4, None, None, None) == L.PH_ERR_ARG
