@@ -8,12 +8,13 @@
 //
 // A step after the end of an episode starts from a cleared state and an empty convolution window.
 //
-// Layout. A lane owns one channel and all its N states in registers, a wavefront 64 channels of one sequence,
-// so the only values that cross lanes are B_t and C_t, which every lane of the block reads from LDS as broadcasts
-// (staged there kSteps steps at a time, converted once). The state stays in fp32 throughout and is never
-// written per step; what a step costs is vector arithmetic: per state one exponential (a quarter-rate
-// instruction, 16 cycles of a wavefront), the decay's argument, the input, the update and the output (4 cycles
-// each), 32 cycles in all against 8 bytes of memory per channel and step.
+// Layout. A lane owns one channel, a wavefront 64 channels of one sequence, so the only values that cross lanes are
+// B_t and C_t, which every lane of the block reads from LDS as broadcasts (staged there kSteps steps at a time,
+// converted once). Within those steps the states are taken four at a time: a lane's four states and decays rest in
+// LDS slots of its own and are in registers for the kSteps steps. So any N runs in the same few registers and short
+// code, and the state is fp32 throughout and never written per step. What a step costs is vector arithmetic: per state
+// one exponential (a quarter-rate instruction, 16 cycles of a wavefront), the decay's argument, the input, the update
+// and the output (4 cycles each), 32 cycles in all against 8 bytes of memory per channel and step.
 //
 // Long sequences of few channels do not fill the chip with one wavefront per 64 channels, so time is cut into
 // chunks: a first launch runs every chunk from a zero state and keeps its end state and the sum of d_t (the
@@ -22,26 +23,19 @@
 #include "common.hpp"
 #include "kernels.hpp"
 
-#include <cmath>
+#include <type_traits>
 
 namespace ph {
 namespace {
 
-constexpr int kSteps = 8;  // steps of a batch: staged, prefetched and (N <= 16) kept together
+constexpr int kSteps = 8;  // steps of a batch: staged and loaded together, and between two kept states of the training forward
 constexpr int kTaps = 4;   // most taps of the convolution; fewer are padded with zero taps in front
 constexpr int kMaxStates = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Steps between two kept states of the training forward: the backward holds that many steps' states in registers.
-constexpr int keep_steps(int ns) { return ns <= 16 ? 8 : (ns <= 32 ? 4 : 2); }
-// States of a lane's registers: the least of these that holds N.
-constexpr int states_of(long N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
-
-// Wavefronts of a block of the gradient: two to a SIMD where the states fit 256 registers, else one.
-constexpr int bwd_waves(int ns) { return ns <= 16 ? 8 : 4; }
-
 struct Args {
   long T, B, C, N, per, K;  // per: channels of a group
+  int Q;                    // states in fours, N rounded up
   const void *x, *z, *delta, *Bm, *Cm;
   long x_t, x_b, z_t, z_b, d_t, d_b, bm_t, bm_b, cm_t, cm_b;
   const float *A, *D, *dt_bias, *conv_w, *conv_b;
@@ -50,9 +44,11 @@ struct Args {
   long y_t, y_b;
   float *h_out, *keep;
   long chunk, chunks;   // steps of a chunk (a multiple of kSteps), their number
-  float *hloc, *dsum;   // [chunks][B][C][N] end (then start) states, [chunks][B][C] sums of d (-1: cleared inside)
-  int blocks_c;         // channel blocks of a group
+  float *hloc, *dsum;   // [chunks] end (then start) states, [chunks][B][C] sums of d (-1: cleared inside)
+  unsigned blocks_c, G; // channel blocks of a group, groups
 };
+// The library's own states are [..][B][Q][C][4]: a wavefront moves four states of 64 channels as 1 KB. The caller's are
+// [B][C][N].
 
 __device__ __forceinline__ float ldf(const uint16_t* p) { return bf16_to_f32(*p); }
 __device__ __forceinline__ float ldf(const float* p) { return *p; }
@@ -63,192 +59,323 @@ __device__ __forceinline__ float ex2(float v) { return __builtin_amdgcn_exp2f(v)
 // softplus without cancellation: with w = 1 + e rounded, log(w) e / (w - 1) is log(1 + e) to a few ulp for every e.
 __device__ __forceinline__ float softplus(float v) {
   const float e = __expf(-fabsf(v)), w = 1.f + e;
-  const float l = w == 1.f ? e : __logf(w) * (e / (w - 1.f));
+  const float l = w == 1.f ? e : __logf(w) * (e * __builtin_amdgcn_rcpf(w - 1.f));
   return fmaxf(v, 0.f) + l;
 }
-
-// The convolution's rolling window: the three inputs before the current one (those past K - 1 steps back stay 0).
-struct Conv {
-  float w[kTaps], bias;
-  float p[kTaps - 1];
-  int K;
-  __device__ __forceinline__ void init(const Args& a, long c) {
-    K = (int)a.K;
-#pragma unroll
-    for (int i = 0; i < kTaps; i++) {
-      const int k = i - (kTaps - K);
-      w[i] = K > 0 && k >= 0 ? a.conv_w[c * K + k] : 0.f;
-    }
-    bias = K > 0 && a.conv_b ? a.conv_b[c] : 0.f;
-    clear();
-  }
-  __device__ __forceinline__ void clear() { p[0] = p[1] = p[2] = 0.f; }
-  __device__ __forceinline__ float pre(float x) const {
-    return fmaf(w[3], x, fmaf(w[2], p[2], fmaf(w[1], p[1], fmaf(w[0], p[0], bias))));
-  }
-  __device__ __forceinline__ void push(float x) {
-    p[0] = K >= 4 ? p[1] : 0.f;
-    p[1] = K >= 3 ? p[2] : 0.f;
-    p[2] = K >= 2 ? x : 0.f;
-  }
-};
 __device__ __forceinline__ float silu(float v) { return v * sigm(v); }
+// d/dv of v sigma(v), s = sigma(v)
+__device__ __forceinline__ float dsilu(float v, float s) { return s * fmaf(v, 1.f - s, 1.f); }
 
 // Whether step t of sequence b starts an episode.
 __device__ __forceinline__ bool starts(const Args& a, long t, long b) {
   if (t > 0) return a.done && a.done[(t - 1) * a.B + b] != 0.f;
-  return a.first && a.first[b] != 0.f;
+  return t == 0 && a.first && a.first[b] != 0.f;
 }
+// Bit j of flag_bits(flag_load(..)): step t0 - 3 + j starts an episode (j < 11: a batch and the three steps that its
+// convolutions look back to). One load per lane, one ballot, apart so that the load can be issued a batch ahead.
+__device__ __forceinline__ float flag_load(const Args& a, long t0, long tend, long b) {
+  const int j = threadIdx.x & 63;
+  const long t = t0 - (kTaps - 1) + j;
+  float f = 0.f;
+  if (j < kSteps + kTaps - 1 && t < tend && t >= 0) {
+    if (t > 0) f = a.done ? a.done[(t - 1) * a.B + b] : 0.f;
+    else f = a.first ? a.first[b] : 0.f;
+  }
+  return f;
+}
+__device__ __forceinline__ unsigned flag_bits(float f) { return (unsigned)__ballot(f != 0.f); }
 
-// The window as it stands before step t0: the last K - 1 inputs, of the sequence or of the carried window.
-template <typename T>
-__device__ __forceinline__ void conv_seek(Conv& cv, const Args& a, long t0, long b, long c) {
-  if (cv.K < 2) return;
-  for (long t = t0 - (cv.K - 1); t < t0; t++) {
-    float v;
-    if (t < 0) v = a.win0 ? a.win0[(b * (cv.K - 1) + cv.K - 1 + t) * a.C + c] : 0.f;
-    else {
-      if (starts(a, t, b)) cv.clear();
-      v = ldf((const T*)a.x + t * a.x_t + b * a.x_b + c);
+// The convolution of one channel, padded to four taps. Inputs that a step does not see (past its taps, or of the
+// episode before) are selected away and not multiplied by zero: they may be infinite.
+struct Conv {
+  float w[kTaps], bias;
+  int K;
+  __device__ __forceinline__ void init(const Args& a, unsigned c) {
+    K = (int)a.K;
+#pragma unroll
+    for (int i = 0; i < kTaps; i++) {
+      const int k = i - (kTaps - K);
+      w[i] = K > 0 && k >= 0 ? a.conv_w[(long)c * K + k] : 0.f;
     }
-    cv.push(v);
+    bias = K > 0 && a.conv_b ? a.conv_b[c] : 0.f;
+  }
+  // How many steps back step i of a batch sees (0..3), uniform.
+  __device__ __forceinline__ int reach(unsigned bits, int i) const {
+    const int n = K < 1 ? 0 : K - 1;
+    if (bits >> i & 8u) return 0;
+    if (bits >> i & 4u) return min(n, 1);
+    if (bits >> i & 2u) return min(n, 2);
+    return n;
+  }
+  __device__ __forceinline__ float pre(float x, float x1, float x2, float x3) const {
+    return fmaf(w[3], x, fmaf(w[2], x1, fmaf(w[1], x2, fmaf(w[0], x3, bias))));
+  }
+};
+
+// The three inputs before step t0 as bits of T (of the sequence, or as fp32 values of the carried window).
+template <typename T>
+__device__ __forceinline__ void look_back(float (&x)[kTaps - 1], const Args& a, long t0, long b, unsigned c) {
+  const T* p = (const T*)a.x + b * a.x_b;
+  const int K1 = (int)a.K - 1;
+#pragma unroll
+  for (int j = 0; j < kTaps - 1; j++) {
+    const long t = t0 - (kTaps - 1) + j;
+    x[j] = 0.f;
+    if (t >= 0) x[j] = ldf(p + t * a.x_t + c);
+    else if (K1 + t >= 0 && a.win0) x[j] = a.win0[(b * K1 + K1 + t) * a.C + c];
   }
 }
 
+// A uniform row pointer that walks over steps. The empty asm keeps the walk a chain of scalar additions: without it the
+// compiler forms the addresses of all of a batch's rows at once, hundreds of scalar registers that it then spills.
+template <typename P>
+__device__ __forceinline__ void walk(P*& p, long d) {
+  p += d;
+  asm("" : "+s"(p));
+}
+
+// A value that every lane holds, in a scalar register (a division leaves its result in vector ones).
+__device__ __forceinline__ unsigned uniform(unsigned v) { return __builtin_amdgcn_readfirstlane(v); }
+
 struct Place {
-  long b, s, c, c0;  // sequence, chunk, this lane's channel (clamped into the group), the group's first channel
-  int g;
-  bool in;           // whether the lane has a channel
+  unsigned b, s, c, g;  // sequence, chunk, this lane's channel (clamped into the group), the group
+  bool in;              // whether the lane has a channel
 };
-__device__ __forceinline__ Place place(const Args& a, long id) {
+__device__ __forceinline__ Place place(const Args& a, unsigned id) {
   Place p;
-  const int cb = (int)(id % a.blocks_c);
+  const unsigned cb = id % a.blocks_c;
   id /= a.blocks_c;
-  const long G = a.C / a.per;
-  p.g = (int)(id % G);
-  id /= G;
-  p.b = id % a.B;
-  p.s = id / a.B;
-  const long lc = (long)cb * blockDim.x + threadIdx.x;
-  p.in = lc < a.per;
-  p.c0 = (long)p.g * a.per;
-  p.c = p.c0 + (p.in ? lc : a.per - 1);
+  p.g = id % a.G;
+  id /= a.G;
+  p.b = uniform(id % (unsigned)a.B);
+  p.s = uniform(id / (unsigned)a.B);
+  p.g = uniform(p.g);
+  const unsigned lc = cb * blockDim.x + threadIdx.x, per = (unsigned)a.per;
+  p.in = lc < per;
+  p.c = p.g * per + (p.in ? lc : per - 1);
   return p;
 }
 
-// B and C of kSteps steps from t0 as fp32 in LDS, [step][2][NS], zero past N and past the sequence's end.
-template <typename T, int NS>
-__device__ __forceinline__ void stage_bc(float* s, const Args& a, long t0, long tend, long b, int g) {
-  const int tot = kSteps * 2 * NS;
-  for (int e = threadIdx.x; e < tot; e += blockDim.x) {
-    const int n = e % NS, which = (e / NS) & 1;
-    const long t = t0 + e / (2 * NS);
-    float v = 0.f;
-    if (n < a.N && t < tend) {
-      const long col = g * a.N + n;
-      v = which ? ldf((const T*)a.Cm + t * a.cm_t + b * a.cm_b + col)
-                : ldf((const T*)a.Bm + t * a.bm_t + b * a.bm_b + col);
+// B and C of kSteps steps as fp32 in LDS, [Q][step][B, C][4], zero past N and past the sequence's end: loaded to registers
+// (get) and later written (put), each thread the values threadIdx.x, + blockDim.x, ... (kMost of them at most). A
+// value's place e gives its step (e / 8) % 8, its row (e / 4) % 2 and its state 4 (e / 64) + e % 4.
+__device__ __forceinline__ int place_step(int e) { return (e >> 3) & 7; }
+__device__ __forceinline__ int place_row(int e) { return (e >> 2) & 1; }
+__device__ __forceinline__ int place_state(int e) { return 4 * (e >> 6) + (e & 3); }
+static_assert(kSteps == 8, "places of the staged values");
+template <typename T, int kMost>
+struct StageBC {
+  const T* p[kMost];   // of step 0
+  long stride[kMost];
+  int step[kMost];     // of the batch; past it for no value
+  float v[kMost];
+  __device__ __forceinline__ void init(const Args& a, long b, unsigned g) {
+#pragma unroll
+    for (int k = 0; k < kMost; k++) {
+      const int e = threadIdx.x + k * blockDim.x, n = place_state(e);
+      const bool is_c = place_row(e);
+      p[k] = is_c ? (const T*)a.Cm + b * a.cm_b : (const T*)a.Bm + b * a.bm_b;
+      p[k] += g * a.N + n;
+      stride[k] = is_c ? a.cm_t : a.bm_t;
+      step[k] = n < a.N ? place_step(e) : kSteps;
     }
-    s[e] = v;
   }
+  __device__ __forceinline__ void get(long t0, int steps) {
+#pragma unroll
+    for (int k = 0; k < kMost; k++) v[k] = step[k] < steps ? ldf(p[k] + (t0 + step[k]) * stride[k]) : 0.f;
+  }
+  __device__ __forceinline__ void put(const Args& a, float* s) const {
+    const int tot = kSteps * 8 * a.Q;
+#pragma unroll
+    for (int k = 0; k < kMost; k++) {
+      const int e = threadIdx.x + k * blockDim.x;
+      if (e < tot) s[e] = v[k];
+    }
+  }
+};
+
+// States n0.. n0 + 3 of a row of N, zero past N.
+__device__ __forceinline__ float4 row4(const float* p, int n0, long N) {
+  return make_float4(p[n0], n0 + 1 < N ? p[n0 + 1] : 0.f, n0 + 2 < N ? p[n0 + 2] : 0.f, n0 + 3 < N ? p[n0 + 3] : 0.f);
+}
+__device__ __forceinline__ void set_row4(float* p, int n0, long N, const float4& v) {
+  p[n0] = v.x;
+  if (n0 + 1 < N) p[n0 + 1] = v.y;
+  if (n0 + 2 < N) p[n0 + 2] = v.z;
+  if (n0 + 3 < N) p[n0 + 3] = v.w;
+}
+// A in units of the base-2 exponential.
+__device__ __forceinline__ float4 decay4(const Args& a, unsigned c, int q) {
+  const float4 v = row4(a.A + (long)c * a.N, 4 * q, a.N);
+  return make_float4(v.x * kLog2e, v.y * kLog2e, v.z * kLog2e, v.w * kLog2e);
 }
 
-template <int NS>
-__device__ __forceinline__ void load_state(float (&h)[NS], const float* p, long N) {
+// Raw rows of a batch, loaded a batch ahead; steps past the end repeat the last one.
+template <typename T>
+struct Rows {
+  uint32_t v[kSteps];  // the bits: a bf16 value's, or an fp32's
+  __device__ __forceinline__ void get(const T* p, long stride, int steps, unsigned c) {
 #pragma unroll
-  for (int n = 0; n < NS; n++) h[n] = n < N ? p[n] : 0.f;
-}
-template <int NS>
-__device__ __forceinline__ void store_state(float* p, const float (&h)[NS], long N) {
+    for (int i = 0; i < kSteps; i++) {
+      if constexpr (sizeof(T) == 2) v[i] = p[c];
+      else v[i] = __builtin_bit_cast(uint32_t, p[c]);
+      walk(p, i + 1 < steps ? stride : 0);
+    }
+  }
+  __device__ __forceinline__ float operator[](int i) const {
+    return __builtin_bit_cast(float, sizeof(T) == 2 ? v[i] << 16 : v[i]);
+  }
+  // From here on the compiler takes the values as new: what is computed from them again is not kept from before.
+  __device__ __forceinline__ void renew() {
 #pragma unroll
-  for (int n = 0; n < NS; n++)
-    if (n < N) p[n] = h[n];
-}
+    for (int i = 0; i < kSteps; i++) asm("" : "+v"(v[i]));
+  }
+};
 
 // One chunk of one sequence. LOCAL: from a zero state, keeping only the end state and the decay's exponent.
-template <typename T, int NS, bool LOCAL>
+template <typename T, bool LOCAL, int MOST>
 __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
-  __shared__ __attribute__((aligned(16))) float sbc[kSteps * 2 * NS];
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  const int Q = a.Q, nt = blockDim.x, tid = threadIdx.x;
+  float4* sA = reinterpret_cast<float4*>(lds);  // [Q][nt]
+  float4* sH = sA + Q * nt;                     // [Q][nt]
+  float* sbc = lds + 8 * Q * nt;                // [2][Q][kSteps][2][4]
   const Place pl = place(a, blockIdx.x);
-  const long b = pl.b, c = pl.c;
+  const long b = pl.b;
+  const unsigned c = pl.c;
   const long tbeg = pl.s * a.chunk, tend = min(a.T, tbeg + a.chunk);
+  const T* xp = (const T*)a.x + b * a.x_b + tbeg * a.x_t;
+  const T* dp = (const T*)a.delta + b * a.d_b + tbeg * a.d_t;
+  const T* zp = (const T*)a.z + (a.z ? b * a.z_b + tbeg * a.z_t : 0);
+  T* yp = (T*)a.y + b * a.y_b + tbeg * a.y_t;
+  const long quads = a.B * Q * a.C;  // quads of the library's states of one chunk (or kept batch)
+  float4* keep = LOCAL || !a.keep ? nullptr : reinterpret_cast<float4*>(a.keep) + tbeg / kSteps * quads + b * Q * a.C;
+  Rows<T> rx, rd, rz;
+  StageBC<T, MOST> bc;
+  bc.init(a, b, pl.g);
+  float fl, back[kTaps - 1];
+  auto fetch = [&](long t0) __attribute__((always_inline)) {
+    const int n = (int)min((long)kSteps, tend - t0);
+    bc.get(t0, n);
+    rx.get(xp, a.x_t, n, c);
+    rd.get(dp, a.d_t, n, c);
+    if (!LOCAL && a.z) rz.get(zp, a.z_t, n, c);
+    fl = flag_load(a, t0, tend, b);
+    walk(xp, kSteps * a.x_t);
+    walk(dp, kSteps * a.d_t);
+    if (!LOCAL) walk(zp, kSteps * a.z_t);
+  };
+  fetch(tbeg);
+  look_back<T>(back, a, tbeg, b, c);
   Conv cv;
   cv.init(a, c);
-  conv_seek<T>(cv, a, tbeg, b, c);
-  float A2[NS], h[NS];
-#pragma unroll
-  for (int n = 0; n < NS; n++) A2[n] = n < a.N ? a.A[c * a.N + n] * kLog2e : 0.f;
   const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, Dc = a.D ? a.D[c] : 0.f;
-  const long hoff = (b * a.C + c) * a.N;
-  if (LOCAL || (a.chunks == 1 && !a.h0)) {
-#pragma unroll
-    for (int n = 0; n < NS; n++) h[n] = 0.f;
-  } else {
-    load_state<NS>(h, a.chunks > 1 ? a.hloc + pl.s * a.B * a.C * a.N + hoff : a.h0 + hoff, a.N);
+  for (int q = 0; q < Q; q++) {
+    sA[q * nt + tid] = decay4(a, c, q);
+    float4 h = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!LOCAL) {
+      if (a.chunks > 1) h = reinterpret_cast<const float4*>(a.hloc)[pl.s * quads + (b * Q + q) * a.C + c];
+      else if (a.h0) h = row4(a.h0 + (b * a.C + c) * a.N, 4 * q, a.N);
+    }
+    sH[q * nt + tid] = h;
   }
   float dsum = 0.f;
-  bool cleared = false;
-  const T* xp = (const T*)a.x + b * a.x_b + c;
-  const T* dp = (const T*)a.delta + b * a.d_b + c;
-  const T* zp = (const T*)a.z + (a.z ? b * a.z_b + c : 0);
-  T* yp = (T*)a.y + b * a.y_b + c;
-  for (long t0 = tbeg; t0 < tend; t0 += kSteps) {
-    float rx[kSteps], rd[kSteps], rz[kSteps];
+  unsigned cleared = 0;
+  int buf = 0;
+  for (long t0 = tbeg; t0 < tend; t0 += kSteps, buf ^= 1) {
+    // two buffers and one barrier: a wavefront writes this one again only after every wavefront has passed the
+    // barrier of the batch between, and so has read it
+    float* s = sbc + buf * 64 * Q;
+    bc.put(a, s);
+    const Rows<T> cx = rx, cd = rd, cz = rz;
+    const unsigned bits = flag_bits(fl), st = bits >> (kTaps - 1);
+    const int steps = (int)min((long)kSteps, tend - t0);
+    __syncthreads();
+    if (t0 + kSteps < tend) fetch(t0 + kSteps);
+    cleared |= st;
+    float d[kSteps], du[kSteps], o[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
-      const long t = min(t0 + i, tend - 1);
-      rx[i] = ldf(xp + t * a.x_t);
-      rd[i] = ldf(dp + t * a.d_t);
-      rz[i] = !LOCAL && a.z ? ldf(zp + t * a.z_t) : 0.f;
+      float u = cx[i];
+      if (cv.K) {
+        const int n = cv.reach(bits, i);
+        const float x1 = i > 0 ? cx[i > 0 ? i - 1 : 0] : back[2], x2 = i > 1 ? cx[i > 1 ? i - 2 : 0] : back[i + 1],
+                    x3 = i > 2 ? cx[i > 2 ? i - 3 : 0] : back[i];
+        u = silu(cv.pre(u, n > 0 ? x1 : 0.f, n > 1 ? x2 : 0.f, n > 2 ? x3 : 0.f));
+      }
+      // a step past the end leaves the state as it is: a decay of one and no input
+      d[i] = softplus(cd[i] + bias);
+      d[i] = i < steps ? d[i] : 0.f;
+      du[i] = i < steps ? d[i] * u : 0.f;
+      if (LOCAL) dsum += d[i];
+      o[i] = Dc * u;
     }
-    __syncthreads();
-    stage_bc<T, NS>(sbc, a, t0, tend, b, pl.g);
-    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kSteps; i++) {
-      const long t = t0 + i;
-      if (t >= tend) break;
-      if (!LOCAL && a.keep && i % keep_steps(NS) == 0 && pl.in)
-        store_state<NS>(a.keep + (t / keep_steps(NS)) * a.B * a.C * a.N + hoff, h, a.N);
-      if (starts(a, t, b)) {
-        cv.clear();
-        cleared = true;
+    for (int j = 0; j < kTaps - 1; j++) back[j] = cx[kSteps - (kTaps - 1) + j];
+    auto scan = [&](auto ANY) __attribute__((always_inline)) {  // ANY: an episode starts in this batch
+      for (int q = 0; q < Q; q++) {
+        const float4 A = sA[q * nt + tid];
+        float4 h = sH[q * nt + tid];
+        if (!LOCAL && keep && pl.in) (keep + q * a.C)[c] = h;
 #pragma unroll
-        for (int n = 0; n < NS; n++) h[n] = 0.f;
+        for (int i = 0; i < kSteps; i++) {
+          if constexpr (decltype(ANY)::value) {
+            const bool cut = st & (1u << i);
+            h = make_float4(cut ? 0.f : h.x, cut ? 0.f : h.y, cut ? 0.f : h.z, cut ? 0.f : h.w);
+          }
+          const float4 Bv = *reinterpret_cast<const float4*>(&s[64 * q + 8 * i]);
+          h.x = fmaf(ex2(d[i] * A.x), h.x, du[i] * Bv.x);
+          h.y = fmaf(ex2(d[i] * A.y), h.y, du[i] * Bv.y);
+          h.z = fmaf(ex2(d[i] * A.z), h.z, du[i] * Bv.z);
+          h.w = fmaf(ex2(d[i] * A.w), h.w, du[i] * Bv.w);
+          if (!LOCAL) {
+            const float4 Cv = *reinterpret_cast<const float4*>(&s[64 * q + 8 * i + 4]);
+            o[i] = fmaf(h.x, Cv.x, fmaf(h.y, Cv.y, fmaf(h.z, Cv.z, fmaf(h.w, Cv.w, o[i]))));
+          }
+          if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // bounds the values of later steps that are fetched early
+        }
+        sH[q * nt + tid] = h;
       }
-      const float x = rx[i];
-      const float u = cv.K ? silu(cv.pre(x)) : x;
-      cv.push(x);
-      const float d = softplus(rd[i] + bias), du = d * u;
-      dsum += d;
-      float o = Dc * u;
+    };
+    if (st) scan(std::true_type{});
+    else scan(std::false_type{});
+    if (!LOCAL) {
+      if (keep) walk(keep, quads);
 #pragma unroll
-      for (int n = 0; n < NS; n++) {
-        h[n] = fmaf(ex2(d * A2[n]), h[n], du * sbc[i * 2 * NS + n]);
-        if (!LOCAL) o = fmaf(h[n], sbc[(i * 2 + 1) * NS + n], o);
+      for (int i = 0; i < kSteps; i++) {
+        if (i < steps && pl.in) stf(yp + c, a.z ? o[i] * silu(cz[i]) : o[i]);
+        walk(yp, a.y_t);
       }
-      if (!LOCAL && pl.in) stf(yp + t * a.y_t, a.z ? o * silu(rz[i]) : o);
     }
   }
   if (!pl.in) return;
-  if (LOCAL) {
-    store_state<NS>(a.hloc + pl.s * a.B * a.C * a.N + hoff, h, a.N);
-    a.dsum[(pl.s * a.B + b) * a.C + c] = cleared ? -1.f : dsum;
-  } else if (tend == a.T && a.h_out) {
-    store_state<NS>(a.h_out + hoff, h, a.N);
+  for (int q = 0; q < Q; q++) {
+    const float4 h = sH[q * nt + tid];
+    if (LOCAL) reinterpret_cast<float4*>(a.hloc)[pl.s * quads + (b * Q + q) * a.C + c] = h;
+    else if (tend == a.T && a.h_out) set_row4(a.h_out + (b * a.C + c) * a.N, 4 * q, a.N, h);
   }
+  if (LOCAL) a.dsum[(pl.s * a.B + b) * a.C + c] = cleared ? -1.f : dsum;
 }
 
+// A thread's state in the library's layout, [B][Q][C][4].
+struct StateAt {
+  long bc, c, n;
+  bool in;
+};
+__device__ __forceinline__ StateAt state_at(const Args& a, long i) {
+  const long c = i / 4 % a.C, q = i / (4 * a.C) % a.Q, b = i / (4 * a.C * a.Q), n = 4 * q + i % 4;
+  return {b * a.C + c, c, n, n < a.N};
+}
 // Joins the chunks in order: hloc[s] becomes the state before chunk s. One thread per state.
 __global__ void __launch_bounds__(256) k_ssm_join(Args a) {
-  const long BCN = a.B * a.C * a.N, i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= BCN) return;
-  const long bc = i / a.N, c = bc % a.C, n = i % a.N;
-  const float A2 = a.A[c * a.N + n] * kLog2e;
-  float run = a.h0 ? a.h0[i] : 0.f;
+  const long row = a.B * a.C * 4 * a.Q, i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= row) return;
+  const StateAt at = state_at(a, i);
+  const float A2 = at.in ? a.A[at.c * a.N + at.n] * kLog2e : 0.f;
+  float run = at.in && a.h0 ? a.h0[at.bc * a.N + at.n] : 0.f;
   for (long s = 0; s < a.chunks; s++) {
-    const float loc = a.hloc[s * BCN + i], d = a.dsum[s * a.B * a.C + bc];
-    a.hloc[s * BCN + i] = run;
+    const float loc = a.hloc[s * row + i], d = a.dsum[s * a.B * a.C + at.bc];
+    a.hloc[s * row + i] = run;
     run = d < 0.f ? loc : fmaf(ex2(A2 * d), run, loc);
   }
 }
@@ -259,11 +386,17 @@ template <typename T>
 __global__ void __launch_bounds__(256) k_ssm_window(Args a, float* win) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= a.B * a.C) return;
-  const long b = i / a.C, c = i % a.C;
-  Conv cv;
-  cv.init(a, c);
-  conv_seek<T>(cv, a, a.T, b, c);
-  for (int k = 0; k < cv.K - 1; k++) win[(b * (cv.K - 1) + k) * a.C + c] = cv.p[kTaps - cv.K + k];
+  const long b = i / a.C, c = i % a.C, K1 = a.K - 1;
+  float x[kTaps - 1];
+  look_back<T>(x, a, a.T, b, (unsigned)c);
+  bool same = true;  // no episode has started after the input
+#pragma unroll
+  for (int j = kTaps - 2; j >= 0; j--) {
+    const long k = j - (kTaps - 1 - K1), t = a.T - (kTaps - 1) + j;
+    if (k < 0) break;
+    win[(b * K1 + k) * a.C + c] = same ? x[j] : 0.f;
+    same = same && !starts(a, t, b);
+  }
 }
 
 // ---- single tokens -------------------------------------------------------------------------------------
@@ -346,7 +479,7 @@ struct GradArgs {
   void *dx, *dz, *ddelta, *dB, *dC;
   long dx_t, dx_b, dz_t, dz_b, dd_t, dd_b, db_t, db_b, dc_t, dc_b;
   const float* keep;
-  float* carry;   // [chunks][B][C][N]: each chunk's own adjoint at its start, then the one coming in at its end
+  float* carry;   // [chunks] states: each chunk's own adjoint at its start, then the one coming in at its end
   float* bc;      // [blocks_c][T][B][G][2][N] sums of dB, dC over a block's channels
   float* par;     // [rows][C][P] sums of the parameters' gradients over a block's work, P = N + K + 3
   float* halo;    // [chunks][B][K-1][C]: what a chunk adds to dx of the K - 1 steps before it
@@ -354,12 +487,11 @@ struct GradArgs {
   int P;
 };
 
-// Sum of NV values over the 64 lanes, each value's result left in lanes of its own. Two values at a time are folded
-// by swapping wavefront halves, then rows of 16 lanes, then by lane permutations inside a row, so NV values take
-// about 2 NV instructions instead of 6 NV.
-template <int CTL> __device__ __forceinline__ float dpp_mov(float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTL, 0xF, 0xF, true));
-}
+// Sums over the 64 lanes of eight values at each of eight steps, in two halves. lane_sums takes a step's eight values and
+// leaves in lane l a partial of value l / 8, over the lanes of the same l % 8: two values at a time are folded by swapping
+// wavefront halves, then rows of 16 lanes, then lanes eight apart. step_sums takes the eight steps' partials and
+// leaves in lane l the total of value l / 8 at step l % 8. Together under 20 instructions a step, where eight
+// separate sums would take 48.
 // Two registers with one's upper and the other's lower wavefront half (or odd and even rows of 16 lanes) exchanged, two pairs
 // at a time: their sum then holds the first value's total in one half and the second's in the other. As asm: the
 // compiler's builtins return the first register for both. The exchange may not read a register in the two wait
@@ -370,291 +502,341 @@ __device__ __forceinline__ void swap32(float& a0, float& b0, float& a1, float& b
 __device__ __forceinline__ void swap16(float& a0, float& b0, float& a1, float& b1) {
   asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\tv_permlane16_swap_b32 %2, %3" : "+v"(a0), "+v"(b0), "+v"(a1), "+v"(b1));
 }
+template <int CTL> __device__ __forceinline__ float dpp_mov(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTL, 0xF, 0xF, true));
+}
 template <int CTL> __device__ __forceinline__ float fold_dpp(float lo, float hi, bool up) {
   return (up ? hi : lo) + dpp_mov<CTL>(up ? lo : hi);
 }
-// v[0..NV) (NV a power of two, 8..128) -> NV / 32 (at least 1) values per lane; lane_value gives their indexes.
-template <int NV>
-__device__ __forceinline__ void lane_sums(float (&v)[NV], int lane) {
-#pragma unroll
-  for (int i = 0; i < NV / 2; i += 2) {
-    swap32(v[i], v[i + NV / 2], v[i + 1], v[i + 1 + NV / 2]);
-    v[i] += v[i + NV / 2];
-    v[i + 1] += v[i + 1 + NV / 2];
-  }
-#pragma unroll
-  for (int i = 0; i < NV / 4; i += 2) {
-    swap16(v[i], v[i + NV / 4], v[i + 1], v[i + 1 + NV / 4]);
-    v[i] += v[i + NV / 4];
-    v[i + 1] += v[i + 1 + NV / 4];
-  }
-  const bool b3 = lane & 8, b2 = lane & 4, b1 = lane & 2;
-#pragma unroll
-  for (int i = 0; i < NV / 8; i++) v[i] = fold_dpp<0x128>(v[i], v[i + NV / 8], b3);  // lane ^ 8
-  if constexpr (NV >= 16) {
-#pragma unroll
-    for (int i = 0; i < NV / 16; i++) v[i] = fold_dpp<0x141>(v[i], v[i + NV / 16], b2);  // lane ^ 7
-  } else {
-    v[0] += dpp_mov<0x141>(v[0]);
-  }
-  if constexpr (NV >= 32) {
-#pragma unroll
-    for (int i = 0; i < NV / 32; i++) v[i] = fold_dpp<0x4E>(v[i], v[i + NV / 32], b1);  // lane ^ 2
-  } else {
-    v[0] += dpp_mov<0x4E>(v[0]);
-  }
-#pragma unroll
-  for (int i = 0; i < (NV >= 32 ? NV / 32 : 1); i++) v[i] += dpp_mov<0xB1>(v[i]);  // lane ^ 1
+__device__ __forceinline__ float lane_sums(float (&v)[8], int lane) {
+  swap32(v[0], v[4], v[1], v[5]);
+  swap32(v[2], v[6], v[3], v[7]);
+  float a = v[0] + v[4], b = v[1] + v[5], c = v[2] + v[6], d = v[3] + v[7];  // values k (lower half) and k + 4
+  swap16(a, c, b, d);
+  a += c;  // value 4 bit5 + 2 bit4
+  b += d;  // the one after it
+  return fold_dpp<0x128>(a, b, lane & 8);  // lane ^ 8
 }
-// Index of the value that register i of a lane holds after lane_sums, and whether the lane is the one to write it.
-template <int NV>
-__device__ __forceinline__ int lane_value(int i, int lane, bool& mine) {
-  int k = i;
-  k += ((lane >> 5) & 1) * (NV / 2) + ((lane >> 4) & 1) * (NV / 4) + ((lane >> 3) & 1) * (NV / 8);
-  mine = (lane & 1) == 0;
-  if (NV >= 16) k += ((lane >> 2) & 1) * (NV / 16);
-  else mine = mine && !(lane & 4);
-  if (NV >= 32) k += ((lane >> 1) & 1) * (NV / 32);
-  else mine = mine && !(lane & 2);
-  return k;
+__device__ __forceinline__ float step_sums(const float (&p)[8], int lane) {
+  float r[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) r[i] = fold_dpp<0x141>(p[i], p[i + 4], lane & 4);  // lane ^ 7
+  const float a = fold_dpp<0x4E>(r[0], r[2], lane & 2), b = fold_dpp<0x4E>(r[1], r[3], lane & 2);  // lane ^ 2
+  return fold_dpp<0xB1>(a, b, lane & 1);  // lane ^ 1
 }
-
-// d/dv of v sigma(v)
-__device__ __forceinline__ float dsilu(float v, float s) { return s * fmaf(v, 1.f - s, 1.f); }
 
 // The adjoint that a chunk alone sends back past its first step (its own outputs only).
-template <typename T, int NS>
+template <typename T, int MOST>
 __global__ void __launch_bounds__(256) k_ssm_bwd_local(Args a, GradArgs ga) {
-  __shared__ __attribute__((aligned(16))) float sbc[kSteps * 2 * NS];
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  const int Q = a.Q, nt = blockDim.x, tid = threadIdx.x;
+  float4* sA = reinterpret_cast<float4*>(lds);  // [Q][nt]
+  float4* sG = sA + Q * nt;                     // [Q][nt]
+  float* sbc = lds + 8 * Q * nt;                // [2][Q][kSteps][2][4]
   const Place pl = place(a, blockIdx.x);
-  const long b = pl.b, c = pl.c;
+  const long b = pl.b;
+  const unsigned c = pl.c;
   const long tbeg = pl.s * a.chunk, tend = min(a.T, tbeg + a.chunk);
-  float A2[NS], g[NS];
-#pragma unroll
-  for (int n = 0; n < NS; n++) {
-    A2[n] = n < a.N ? a.A[c * a.N + n] * kLog2e : 0.f;
-    g[n] = 0.f;
+  const long tlast = tbeg + (tend - tbeg - 1) / kSteps * kSteps;
+  for (int q = 0; q < Q; q++) {
+    sA[q * nt + tid] = decay4(a, c, q);
+    sG[q * nt + tid] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   const float bias = a.dt_bias ? a.dt_bias[c] : 0.f;
   float dsum = 0.f;
-  bool cleared = false;
-  const T* dp = (const T*)a.delta + b * a.d_b + c;
-  const T* zp = (const T*)a.z + (a.z ? b * a.z_b + c : 0);
-  const T* gp = (const T*)ga.dy + b * ga.dy_b + c;
-  for (long t0 = tbeg + (tend - tbeg - 1) / kSteps * kSteps; t0 >= tbeg; t0 -= kSteps) {
-    float rd[kSteps], rz[kSteps], rg[kSteps];
+  unsigned cleared = 0;
+  Rows<T> rd, rz, rg;
+  StageBC<T, MOST> bc;
+  bc.init(a, b, pl.g);
+  float fl;
+  auto fetch = [&](long t0) __attribute__((always_inline)) {
+    const int n = (int)min((long)kSteps, tend - t0);
+    bc.get(t0, n);
+    rd.get((const T*)a.delta + b * a.d_b + t0 * a.d_t, a.d_t, n, c);
+    if (a.z) rz.get((const T*)a.z + b * a.z_b + t0 * a.z_t, a.z_t, n, c);
+    rg.get((const T*)ga.dy + b * ga.dy_b + t0 * ga.dy_t, ga.dy_t, n, c);
+    fl = flag_load(a, t0, tend, b);
+  };
+  fetch(tlast);
+  int buf = 0;
+  for (long t0 = tlast; t0 >= tbeg; t0 -= kSteps, buf ^= 1) {
+    float* s = sbc + buf * 64 * Q;
+    bc.put(a, s);
+    const Rows<T> cd = rd, cz = rz, cg = rg;
+    const unsigned st = flag_bits(fl) >> (kTaps - 1);
+    const int steps = (int)min((long)kSteps, tend - t0);
+    __syncthreads();
+    if (t0 > tbeg) fetch(t0 - kSteps);
+    cleared |= st;
+    float d[kSteps], dout[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
-      const long t = min(t0 + i, tend - 1);
-      rd[i] = ldf(dp + t * a.d_t);
-      rz[i] = a.z ? ldf(zp + t * a.z_t) : 0.f;
-      rg[i] = ldf(gp + t * ga.dy_t);
+      d[i] = i < steps ? softplus(cd[i] + bias) : 0.f;
+      dout[i] = i < steps ? (a.z ? cg[i] * silu(cz[i]) : cg[i]) : 0.f;
+      dsum += d[i];
     }
-    __syncthreads();
-    stage_bc<T, NS>(sbc, a, t0, tend, b, pl.g);
-    __syncthreads();
+    for (int q = 0; q < Q; q++) {
+      const float4 A = sA[q * nt + tid];
+      float4 g = sG[q * nt + tid];
 #pragma unroll
-    for (int i = kSteps - 1; i >= 0; i--) {
-      const long t = t0 + i;
-      if (t >= tend) continue;
-      const float d = softplus(rd[i] + bias), dout = a.z ? rg[i] * silu(rz[i]) : rg[i];
-      dsum += d;
-      const bool st = starts(a, t, b);
-      cleared |= st;
-#pragma unroll
-      for (int n = 0; n < NS; n++) {
-        const float gn = fmaf(dout, sbc[(i * 2 + 1) * NS + n], g[n]);
-        g[n] = st ? 0.f : ex2(d * A2[n]) * gn;
+      for (int i = kSteps - 1; i >= 0; i--) {
+        const float4 Cv = *reinterpret_cast<const float4*>(&s[64 * q + 8 * i + 4]);
+        g.x = ex2(d[i] * A.x) * fmaf(dout[i], Cv.x, g.x);
+        g.y = ex2(d[i] * A.y) * fmaf(dout[i], Cv.y, g.y);
+        g.z = ex2(d[i] * A.z) * fmaf(dout[i], Cv.z, g.z);
+        g.w = ex2(d[i] * A.w) * fmaf(dout[i], Cv.w, g.w);
+        if (st & (1u << i)) g = make_float4(0.f, 0.f, 0.f, 0.f);
       }
+      sG[q * nt + tid] = g;
     }
   }
   if (!pl.in) return;
-  store_state<NS>(ga.carry + (pl.s * a.B * a.C + b * a.C + c) * a.N, g, a.N);
+  float4* out = reinterpret_cast<float4*>(ga.carry) + (pl.s * a.B + b) * Q * a.C + c;
+  for (int q = 0; q < Q; q++) out[q * a.C] = sG[q * nt + tid];
   a.dsum[(pl.s * a.B + b) * a.C + c] = cleared ? -1.f : dsum;
 }
 
 // Joins them from the end: carry[s] becomes the adjoint that comes in at chunk s's last step.
 __global__ void __launch_bounds__(256) k_ssm_bwd_join(Args a, GradArgs ga) {
-  const long BCN = a.B * a.C * a.N, i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= BCN) return;
-  const long bc = i / a.N, c = bc % a.C, n = i % a.N;
-  const float A2 = a.A[c * a.N + n] * kLog2e;
+  const long row = a.B * a.C * 4 * a.Q, i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= row) return;
+  const StateAt at = state_at(a, i);
+  const float A2 = at.in ? a.A[at.c * a.N + at.n] * kLog2e : 0.f;
   float run = 0.f;
   for (long s = a.chunks - 1; s >= 0; s--) {
-    const float loc = ga.carry[s * BCN + i], d = a.dsum[s * a.B * a.C + bc];
-    ga.carry[s * BCN + i] = run;
+    const float loc = ga.carry[s * row + i], d = a.dsum[s * a.B * a.C + at.bc];
+    ga.carry[s * row + i] = run;
     run = d < 0.f ? loc : fmaf(ex2(A2 * d), run, loc);
   }
 }
 
-// The gradient of one chunk after another. Batches of kS = keep_steps(NS) steps run backwards in time; each restores the
-// kept state before it, runs its steps forward again keeping a_t h_{t-1} of every step in registers, then runs them
-// backwards: g_t = C_t dout_t + a_{t+1} g_{t+1}. The sums over channels (dB, dC) are folded over the wavefront's lanes
-// and added over the block's wavefronts in LDS; the parameters' gradients stay in registers over all chunks of
-// the block. A block takes the items row, row + rows, ... of its channel block, an item being a chunk of a sequence.
-template <typename T, int NS>
-__global__ void __launch_bounds__(64 * bwd_waves(NS)) k_ssm_bwd(Args a, GradArgs ga) {
-  constexpr int kS = keep_steps(NS), NV = 2 * NS;
+// The gradient of one chunk after another. Batches of kSteps steps run backwards in time. Each takes the states four at
+// a time: from the kept states it runs its steps forward again, keeping the decay a_t and a_t h_{t-1} of every step
+// in registers (64 of them), then runs them backwards, g_t = C_t dout_t + a_{t+1} g_{t+1}. So the decays are computed once
+// per batch and two wavefronts share a SIMD; the other states' A, g and dA rest in the lane's LDS slots.
+//
+// With q = g a_t h_{t-1} per state: dA += d q, d(d) = sum A q + u sum g B, du = d sum g B, dB = sum_c g d u, dC = sum_c
+// h dout. The two sums over channels take g and a_t h_{t-1} as they are and add the step's own share, C_n or B_n times
+// S = sum_c dout d u, where they are joined; the sums over states likewise add dout (or d u) times <B, C>, which
+// the staging computes once per step. Sums over channels are folded over the wavefront's lanes, then over the
+// block's wavefronts in LDS; the parameters' gradients stay in LDS and registers over all the block's work. A block
+// takes the items row, row + rows, ... of its channel block, an item being a chunk of a sequence.
+template <typename T>
+__global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
-  float* sbc = lds;                  // [kS][2][NS]
-  float* red = lds + kS * NV;        // [waves][kS][2][NS]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  const long G = a.C / a.per;
-  const int cb = (int)(blockIdx.x % a.blocks_c);
-  const int grp = (int)((blockIdx.x / a.blocks_c) % G);
-  const long row = blockIdx.x / (a.blocks_c * G);
-  const long lc = (long)cb * blockDim.x + threadIdx.x;
-  const bool in = lc < a.per;
-  const long c = grp * a.per + (in ? lc : a.per - 1);
+  const int Q = a.Q, nt = blockDim.x, tid = threadIdx.x;
+  const int lane = tid & 63, wave = tid >> 6, waves = nt >> 6;
+  float4* sA = reinterpret_cast<float4*>(lds);  // [Q][nt]
+  float4* sG = sA + Q * nt;                     // [Q][nt]
+  float4* sdA = sG + Q * nt;                    // [Q][nt]
+  float* sbc = lds + 12 * Q * nt;               // [2][Q][kSteps][B, C][4]
+  float* red = sbc + 2 * 64 * Q;                // [waves][Q][kSteps][dB, dC][4]
+  float* reds = red + waves * 64 * Q;           // [waves][kSteps] of S
+  float* scb = reds + waves * kSteps;           // [2][kSteps] of <B, C>
+  const unsigned cb = uniform(blockIdx.x % a.blocks_c), grp = uniform((blockIdx.x / a.blocks_c) % a.G);
+  const unsigned row = uniform(blockIdx.x / (a.blocks_c * a.G)), items = (unsigned)(a.B * a.chunks);
+  const unsigned lc = cb * nt + tid;
+  const bool in = lc < (unsigned)a.per;
+  const unsigned c = grp * (unsigned)a.per + (in ? lc : (unsigned)a.per - 1);
+  const int out = 8 * (lane & 7) + (lane >> 3);  // place of the total that step_sums leaves in this lane
   Conv cv;
   cv.init(a, c);
-  float A2[NS], dA[NS], g[NS];
-#pragma unroll
-  for (int n = 0; n < NS; n++) {
-    A2[n] = n < a.N ? a.A[c * a.N + n] * kLog2e : 0.f;
-    dA[n] = 0.f;
+  for (int q = 0; q < Q; q++) {
+    sA[q * nt + tid] = decay4(a, c, q);
+    sdA[q * nt + tid] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, Dc = a.D ? a.D[c] : 0.f;
   float dD = 0.f, dbias = 0.f, dcb = 0.f, dw[kTaps] = {};
   const int K = cv.K;
-  for (long item = row; item < a.B * a.chunks; item += ga.rows) {
-    const long b = item % a.B, s = item / a.B;
+  const long quads = a.B * Q * a.C;
+  int buf = 0;
+  for (unsigned item = row; item < items; item += (unsigned)ga.rows) {
+    const long b = uniform(item % (unsigned)a.B), s = uniform(item / (unsigned)a.B);
     const long tbeg = s * a.chunk, tend = min(a.T, tbeg + a.chunk);
-    const long hoff = (b * a.C + c) * a.N;
-    if (a.chunks > 1) load_state<NS>(g, ga.carry + s * a.B * a.C * a.N + hoff, a.N);
-    else {
-#pragma unroll
-      for (int n = 0; n < NS; n++) g[n] = 0.f;
+    {
+      const float4* carry = reinterpret_cast<const float4*>(ga.carry) + s * quads + b * Q * a.C;
+      for (int q = 0; q < Q; q++)  // a lane without a channel sends nothing back, and so adds nothing to a sum
+        sG[q * nt + tid] = a.chunks > 1 && in ? (carry + q * a.C)[c] : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     // ds of the three steps after the current one, of the same episode (zero past the chunk: its successor's
     // share of this chunk's last steps comes through the halo)
     float q1 = 0.f, q2 = 0.f, q3 = 0.f;
-    const T* xp = (const T*)a.x + b * a.x_b + c;
-    const T* dp = (const T*)a.delta + b * a.d_b + c;
-    const T* zp = (const T*)a.z + (a.z ? b * a.z_b + c : 0);
-    const T* gp = (const T*)ga.dy + b * ga.dy_b + c;
-    for (long t0 = tbeg + (tend - tbeg - 1) / kS * kS; t0 >= tbeg; t0 -= kS) {
-      float rx[kS], rd[kS], rz[kS], rg[kS];
-#pragma unroll
-      for (int i = 0; i < kS; i++) {
-        const long t = min(t0 + i, tend - 1);
-        rx[i] = ldf(xp + t * a.x_t);
-        rd[i] = ldf(dp + t * a.d_t) + bias;
-        rz[i] = a.z ? ldf(zp + t * a.z_t) : 0.f;
-        rg[i] = ldf(gp + t * ga.dy_t);
-      }
-      float h[NS], ah[kS][NS];
-      load_state<NS>(h, ga.keep + (t0 / kS) * a.B * a.C * a.N + hoff, a.N);
-      cv.clear();
-      conv_seek<T>(cv, a, t0, b, c);
-      __syncthreads();  // the last batch's sums have been read
-      for (int e = threadIdx.x; e < kS * NV; e += blockDim.x) {
-        const int n = e % NS, which = (e / NS) & 1;
-        const long t = t0 + e / NV;
+    for (long t0 = tbeg + (tend - tbeg - 1) / kSteps * kSteps; t0 >= tbeg; t0 -= kSteps, buf ^= 1) {
+      const int steps = (int)min((long)kSteps, tend - t0);
+      Rows<T> rx, rd, rz, rg;
+      float back[kTaps - 1];
+      rx.get((const T*)a.x + b * a.x_b + t0 * a.x_t, a.x_t, steps, c);
+      rd.get((const T*)a.delta + b * a.d_b + t0 * a.d_t, a.d_t, steps, c);
+      if (a.z) rz.get((const T*)a.z + b * a.z_b + t0 * a.z_t, a.z_t, steps, c);
+      else rz = rx;  // not looked at
+      rg.get((const T*)ga.dy + b * ga.dy_b + t0 * ga.dy_t, ga.dy_t, steps, c);
+      look_back<T>(back, a, t0, b, c);
+      const float4* keep = reinterpret_cast<const float4*>(ga.keep) + t0 / kSteps * quads + b * Q * a.C;
+      float4 next = keep[c];
+      const unsigned bits = flag_bits(flag_load(a, t0, tend, b)), st = bits >> (kTaps - 1);
+      // stage B and C
+      float* sb = sbc + buf * 64 * Q;
+      for (int e = tid; e < 64 * Q; e += nt) {
+        const int n = place_state(e), i = place_step(e);
         float v = 0.f;
-        if (n < a.N && t < tend) {
-          const long col = grp * a.N + n;
-          v = which ? ldf((const T*)a.Cm + t * a.cm_t + b * a.cm_b + col)
-                    : ldf((const T*)a.Bm + t * a.bm_t + b * a.bm_b + col);
-        }
-        sbc[e] = v;
+        if (n < a.N && i < steps)
+          v = place_row(e) ? ldf((const T*)a.Cm + (t0 + i) * a.cm_t + b * a.cm_b + grp * a.N + n)
+                           : ldf((const T*)a.Bm + (t0 + i) * a.bm_t + b * a.bm_b + grp * a.N + n);
+        sb[e] = v;
+      }
+      // Input j (0..10) of the batch and of the three steps before it, and a step's own convolution.
+      auto input = [&](int j) __attribute__((always_inline)) { return j < kTaps - 1 ? back[j < kTaps - 1 ? j : 0] : rx[j < kTaps - 1 ? 0 : j - (kTaps - 1)]; };
+      auto conv = [&](int i, float& x1, float& x2, float& x3) __attribute__((always_inline)) {
+        const int n = cv.reach(bits, i);
+        x1 = n > 0 ? input(i + 2) : 0.f;
+        x2 = n > 1 ? input(i + 1) : 0.f;
+        x3 = n > 2 ? input(i) : 0.f;
+        return cv.pre(rx[i], x1, x2, x3);
+      };
+      float d[kSteps], du[kSteps], dout[kSteps], o[kSteps], gB[kSteps], Aq[kSteps];
+#pragma unroll
+      for (int i = 0; i < kSteps; i++) {
+        float x1, x2, x3;
+        const float u = K ? silu(conv(i, x1, x2, x3)) : rx[i];
+        // a step past the end neither decays, nor takes nor gives
+        d[i] = softplus(rd[i] + bias);
+        d[i] = i < steps ? d[i] : 0.f;
+        du[i] = i < steps ? d[i] * u : 0.f;
+        dout[i] = a.z ? rg[i] * silu(rz[i]) : rg[i];
+        dout[i] = i < steps && in ? dout[i] : 0.f;
+        o[i] = gB[i] = Aq[i] = 0.f;
       }
       __syncthreads();
-      // forward again
-      float pre[kS], u[kS], d[kS], p1[kS], p2[kS], p3[kS];
-      bool st[kS];
-#pragma unroll
-      for (int i = 0; i < kS; i++) {
-        const long t = t0 + i;
-        st[i] = t < tend && starts(a, t, b);
-        if (st[i]) cv.clear();
-        pre[i] = K ? cv.pre(rx[i]) : rx[i];
-        u[i] = K ? silu(pre[i]) : rx[i];
-        p1[i] = cv.p[2];
-        p2[i] = cv.p[1];
-        p3[i] = cv.p[0];
-        cv.push(rx[i]);
-        d[i] = softplus(rd[i]);
-        const float du = d[i] * u[i];
-#pragma unroll
-        for (int n = 0; n < NS; n++) {
-          ah[i][n] = st[i] ? 0.f : ex2(d[i] * A2[n]) * h[n];
-          h[n] = fmaf(du, sbc[i * NV + n], ah[i][n]);
-        }
+      if (tid < kSteps) {  // read after the barrier below
+        float p = 0.f;
+        for (int q = 0; q < Q; q++)
+          for (int n = 0; n < 4; n++) p = fmaf(sb[64 * q + 8 * tid + n], sb[64 * q + 8 * tid + 4 + n], p);
+        scb[buf * kSteps + tid] = p;
       }
-      // and back
+      auto scan = [&](auto ANY) __attribute__((always_inline)) {  // ANY: an episode starts in this batch
+        for (int q = 0; q < Q; q++) {
+          const float4 A = sA[q * nt + tid], kh = next;
+          next = (keep + (q + 1 < Q ? q + 1 : q) * a.C)[c];
+          const float4 g4 = sG[q * nt + tid];
+          const float Av[4] = {A.x, A.y, A.z, A.w};
+          float h[4] = {kh.x, kh.y, kh.z, kh.w}, g[4] = {g4.x, g4.y, g4.z, g4.w}, dA[4] = {};
+          float dec[kSteps][4], ah[kSteps][4], part[kSteps];
 #pragma unroll
-      for (int i = kS - 1; i >= 0; i--) {
-        const long t = t0 + i;
-        if (t >= tend) {
-          if (lane < NV) red[(wave * kS + i) * NV + lane] = 0.f;
-          continue;
-        }
-        const float sz = a.z ? sigm(rz[i]) : 0.f;
-        const float dout = a.z ? rg[i] * (rz[i] * sz) : rg[i];
-        const float du = d[i] * u[i];
-        float o = Dc * u[i], gB = 0.f, Aq = 0.f;
-        float v[NV];
+          for (int i = 0; i < kSteps; i++) {
+            const bool cut = decltype(ANY)::value && (st & (1u << i));
+            const float4 Bv = *reinterpret_cast<const float4*>(&sb[64 * q + 8 * i]);
+            const float Bn[4] = {Bv.x, Bv.y, Bv.z, Bv.w};
 #pragma unroll
-        for (int n = 0; n < NS; n++) {
-          const float Bn = sbc[i * NV + n], Cn = sbc[i * NV + NS + n];
-          const float hn = fmaf(du, Bn, ah[i][n]);
-          const float gn = fmaf(dout, Cn, g[n]);
-          o = fmaf(hn, Cn, o);
-          gB = fmaf(gn, Bn, gB);
-          const float q = gn * ah[i][n];
-          Aq = fmaf(A2[n], q, Aq);
-          dA[n] = fmaf(d[i], q, dA[n]);
-          v[n] = in ? gn * du : 0.f;
-          v[NS + n] = in ? hn * dout : 0.f;
-          g[n] = st[i] ? 0.f : ex2(d[i] * A2[n]) * gn;
-        }
-        lane_sums<NV>(v, lane);
-#pragma unroll
-        for (int k = 0; k < (NV >= 32 ? NV / 32 : 1); k++) {
-          bool mine;
-          const int idx = lane_value<NV>(k, lane, mine);
-          if (mine) red[(wave * kS + i) * NV + idx] = v[k];
-        }
-        const float ddt = fmaf(u[i], gB, Aq * (1.f / kLog2e)) * sigm(rd[i]);
-        float ds = fmaf(d[i], gB, Dc * dout);
-        dD = fmaf(dout, u[i], dD);
-        dbias += ddt;
-        float dxv = ds;
-        if (K) {
-          const float sg = sigm(pre[i]);
-          ds *= dsilu(pre[i], sg);
-          dcb += ds;
-          dw[3] = fmaf(ds, rx[i], dw[3]);
-          dw[2] = fmaf(ds, p1[i], dw[2]);
-          dw[1] = fmaf(ds, p2[i], dw[1]);
-          dw[0] = fmaf(ds, p3[i], dw[0]);
-          dxv = fmaf(cv.w[3], ds, fmaf(cv.w[2], q1, fmaf(cv.w[1], q2, cv.w[0] * q3)));
-          q3 = st[i] || K < 4 ? 0.f : q2;
-          q2 = st[i] || K < 3 ? 0.f : q1;
-          q1 = st[i] || K < 2 ? 0.f : ds;
-        }
-        if (in) {
-          if (ga.ddelta) stf((T*)ga.ddelta + t * ga.dd_t + b * ga.dd_b + c, ddt);
-          if (a.z && ga.dz) stf((T*)ga.dz + t * ga.dz_t + b * ga.dz_b + c, rg[i] * o * dsilu(rz[i], sz));
-          // the last K - 1 steps of a chunk that has a successor are finished by the halo's launch
-          if (ga.dx) {
-            if (t >= tend - (K - 1) && tend < a.T) ga.halo[(((s * 2) * a.B + b) * (kTaps - 1) + (tend - 1 - t)) * a.C + c] = dxv;
-            else stf((T*)ga.dx + t * ga.dx_t + b * ga.dx_b + c, dxv);
+            for (int n = 0; n < 4; n++) {
+              dec[i][n] = ex2(d[i] * Av[n]);
+              ah[i][n] = dec[i][n] * (cut ? 0.f : h[n]);
+              h[n] = fmaf(du[i], Bn[n], ah[i][n]);
+            }
+            if (i % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // bounds the values of later steps that are fetched early
           }
+#pragma unroll
+          for (int i = kSteps - 1; i >= 0; i--) {
+            const bool cut = decltype(ANY)::value && (st & (1u << i));
+            const float4 Bv = *reinterpret_cast<const float4*>(&sb[64 * q + 8 * i]);
+            const float4 Cv = *reinterpret_cast<const float4*>(&sb[64 * q + 8 * i + 4]);
+            const float Bn[4] = {Bv.x, Bv.y, Bv.z, Bv.w}, Cn[4] = {Cv.x, Cv.y, Cv.z, Cv.w};
+            float v[8];
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+              v[n] = g[n] * du[i];
+              v[4 + n] = ah[i][n] * dout[i];
+              gB[i] = fmaf(g[n], Bn[n], gB[i]);
+              o[i] = fmaf(ah[i][n], Cn[n], o[i]);
+              const float gn = fmaf(dout[i], Cn[n], g[n]), qn = gn * ah[i][n];
+              Aq[i] = fmaf(Av[n], qn, Aq[i]);
+              dA[n] = fmaf(d[i], qn, dA[n]);
+              g[n] = cut ? 0.f : dec[i][n] * gn;
+            }
+            part[i] = lane_sums(v, lane);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          red[(wave * Q + q) * 64 + out] = step_sums(part, lane);
+          sG[q * nt + tid] = make_float4(g[0], g[1], g[2], g[3]);
+          const float4 acc = sdA[q * nt + tid];
+          sdA[q * nt + tid] = make_float4(acc.x + dA[0], acc.y + dA[1], acc.z + dA[2], acc.w + dA[3]);
         }
+      };
+      if (st) scan(std::true_type{});
+      else scan(std::false_type{});
+      {
+        float v[kSteps];
+#pragma unroll
+        for (int i = 0; i < kSteps; i++) v[i] = dout[i] * du[i];
+        float S = lane_sums(v, lane);  // of step lane / 8, over lanes of the same lane % 8
+        S += dpp_mov<0x141>(S);
+        S += dpp_mov<0x4E>(S);
+        S += dpp_mov<0xB1>(S);
+        if ((lane & 7) == 0) reds[wave * kSteps + (lane >> 3)] = S;
       }
       __syncthreads();
       // the block's sums over its wavefronts, in order
-      for (int e = threadIdx.x; e < kS * NV; e += blockDim.x) {
-        const int n = e % NS, which = (e / NS) & 1;
-        const long t = t0 + e / NV;
-        if (n >= a.N || t >= tend) continue;
-        float sum = 0.f;
-        for (int w = 0; w < waves; w++) sum += red[w * kS * NV + e];
-        if (ga.bc) ga.bc[((((long)cb * a.T + t) * a.B + b) * G + grp) * 2 * a.N + which * a.N + n] = sum;
+      for (int e = tid; e < 64 * Q; e += nt) {
+        const int i = place_step(e), which = place_row(e), n = place_state(e);
+        if (n >= a.N || i >= steps) continue;
+        float sum = 0.f, S = 0.f;
+        for (int w = 0; w < waves; w++) {
+          sum += red[w * 64 * Q + e];
+          S += reds[w * kSteps + i];
+        }
+        sum = fmaf(sb[e ^ 4], S, sum);
+        const long t = t0 + i;
+        if (ga.bc) ga.bc[(((cb * a.T + t) * a.B + b) * a.G + grp) * 2 * a.N + which * a.N + n] = sum;
         else if (which && ga.dC) stf((T*)ga.dC + t * ga.dc_t + b * ga.dc_b + grp * a.N + n, sum);
         else if (!which && ga.dB) stf((T*)ga.dB + t * ga.db_t + b * ga.db_b + grp * a.N + n, sum);
+      }
+      // the channel's own gradients
+      rx.renew();
+      rd.renew();
+      rz.renew();
+      const long last = t0 + steps - 1;
+      T* pdd = (T*)ga.ddelta + b * ga.dd_b + last * ga.dd_t;
+      T* pdz = (T*)ga.dz + b * ga.dz_b + last * ga.dz_t;
+      T* pdx = (T*)ga.dx + b * ga.dx_b + last * ga.dx_t;
+      const int own = tend < a.T && t0 + kSteps >= tend ? steps - (K - 1) : kSteps;  // steps from here on are finished by the halo's launch
+#pragma unroll
+      for (int i = kSteps - 1; i >= 0; i--) {
+        if (i >= steps) continue;
+        float x1, x2, x3, u = rx[i], pre = 0.f, sg = 0.f;
+        if (K) {
+          pre = conv(i, x1, x2, x3);
+          sg = sigm(pre);
+          u = pre * sg;
+        }
+        const float cb2 = scb[buf * kSteps + i], gb = fmaf(dout[i], cb2, gB[i]);
+        const float ddt = fmaf(u, gb, Aq[i] * (1.f / kLog2e)) * sigm(rd[i] + bias);
+        float ds = fmaf(d[i], gb, Dc * dout[i]);
+        dD = fmaf(dout[i], u, dD);
+        dbias += ddt;
+        float dxv = ds;
+        if (K) {
+          ds *= dsilu(pre, sg);
+          dcb += ds;
+          dw[3] = fmaf(ds, rx[i], dw[3]);
+          dw[2] = fmaf(ds, x1, dw[2]);
+          dw[1] = fmaf(ds, x2, dw[1]);
+          dw[0] = fmaf(ds, x3, dw[0]);
+          dxv = fmaf(cv.w[3], ds, fmaf(cv.w[2], q1, fmaf(cv.w[1], q2, cv.w[0] * q3)));
+          const bool cut = st & (1u << i);
+          q3 = cut || K < 4 ? 0.f : q2;
+          q2 = cut || K < 3 ? 0.f : q1;
+          q1 = cut || K < 2 ? 0.f : ds;
+        }
+        if (in) {
+          if (ga.ddelta) stf(pdd + c, ddt);
+          if (a.z && ga.dz) stf(pdz + c, rg[i] * fmaf(du[i], cb2, fmaf(Dc, u, o[i])) * dsilu(rz[i], sigm(rz[i])));
+          if (ga.dx) {
+            if (i < own) stf(pdx + c, dxv);
+            else (ga.halo + ((s * 2 * a.B + b) * (kTaps - 1) + (steps - 1 - i)) * a.C)[c] = dxv;
+          }
+        }
+        walk(pdd, -ga.dd_t);
+        walk(pdz, -ga.dz_t);
+        walk(pdx, -ga.dx_t);
       }
     }
     // what this chunk adds to dx of the K - 1 steps before it: step tbeg - 1 - j takes ds of up to K - 1 - j steps on
@@ -667,10 +849,8 @@ __global__ void __launch_bounds__(64 * bwd_waves(NS)) k_ssm_bwd(Args a, GradArgs
     }
   }
   if (in && ga.par) {
-    float* p = ga.par + (row * a.C + c) * ga.P;
-#pragma unroll
-    for (int n = 0; n < NS; n++)
-      if (n < a.N) p[n] = dA[n];
+    float* p = ga.par + ((long)row * a.C + c) * ga.P;
+    for (int q = 0; q < Q; q++) set_row4(p, 4 * q, a.N, sdA[q * nt + tid]);
     p += a.N;
     p[0] = dD;
     p[1] = dbias;
@@ -700,7 +880,7 @@ __global__ void __launch_bounds__(256) k_ssm_halo(Args a, GradArgs ga) {
 // dB, dC = the channel blocks' sums in order.
 template <typename T>
 __global__ void __launch_bounds__(256) k_ssm_fold_bc(Args a, GradArgs ga) {
-  const long G = a.C / a.per, W = G * 2 * a.N, tot = a.T * a.B * W;
+  const long G = a.G, W = G * 2 * a.N, tot = a.T * a.B * W;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < tot; i += (long)gridDim.x * 256) {
     const long tb = i / W, b = tb % a.B, t = tb / a.B;
     const long e = i % W, g = e / (2 * a.N), r = e % (2 * a.N), which = r / a.N, n = r % a.N;
@@ -773,6 +953,8 @@ int check(const ph_ssm_args& p, const char* who) {
 Args args_of(const ph_ssm_args& p) {
   Args a{};
   a.T = (long)p.T; a.B = (long)p.B; a.C = (long)p.C; a.N = (long)p.N; a.per = (long)(p.C / p.G); a.K = (long)p.K;
+  a.G = (unsigned)p.G;
+  a.Q = (int)((p.N + 3) / 4);
   a.x = p.x; a.z = p.z; a.delta = p.delta; a.Bm = p.Bm; a.Cm = p.Cm;
   a.x_t = p.x_t; a.x_b = p.x_b; a.z_t = p.z_t; a.z_b = p.z_b; a.d_t = p.delta_t; a.d_b = p.delta_b;
   a.bm_t = p.Bm_t; a.bm_b = p.Bm_b; a.cm_t = p.Cm_t; a.cm_b = p.Cm_b;
@@ -781,15 +963,25 @@ Args args_of(const ph_ssm_args& p) {
   return a;
 }
 
-// Threads of a block: whole wavefronts over a group's channels, `most` at most.
-int block_threads(const Args& a, int most) {
-  const long w = (a.per + 63) / 64;
-  return 64 * (int)(w < most ? w : most);
+// LDS of a block of nt threads: the lanes' slots, the staged rows and (gradient) the wavefronts' sums.
+size_t fwd_lds(int Q, int nt) { return (size_t)4 * (8 * Q * nt + 2 * 64 * Q); }
+size_t bwd_lds(int Q, int nt) {
+  const int waves = nt / 64;
+  return (size_t)4 * (12 * Q * nt + (2 + waves) * 64 * Q + waves * kSteps + 2 * kSteps);
 }
 
+// Threads of a block: whole wavefronts over a group's channels, at most four and as LDS holds (N = 64: one in the gradient).
+int block_threads(const Args& a, bool grad) {
+  const long w = (a.per + 63) / 64;
+  int nt = 64 * (int)(w < 4 ? w : 4);
+  while (nt > 64 && (grad ? bwd_lds(a.Q, nt) : fwd_lds(a.Q, nt)) > 64 * 1024) nt -= 64;
+  return nt;
+}
+static_assert(4 * (12 * 16 * 64 + 3 * 64 * 16 + 3 * kSteps) <= 64 * 1024, "one wavefront at N = 64");
+
 // Chunks of time: enough wavefronts for every SIMD to hold two, in chunks of at least 32 steps.
-void set_chunks(Args& a) {
-  const long waves = a.B * (a.C / a.per) * ((a.per + 63) / 64);
+int set_chunks(Args& a) {
+  const long waves = a.B * a.G * ((a.per + 63) / 64);
   long want = (2048 + waves - 1) / waves;
   const long most = (a.T + 31) / 32;
   if (want > most) want = most;
@@ -797,20 +989,28 @@ void set_chunks(Args& a) {
   a.chunk = (a.T + want - 1) / want;
   a.chunk = (a.chunk + kSteps - 1) / kSteps * kSteps;
   a.chunks = (a.T + a.chunk - 1) / a.chunk;
+  PH_REQUIRE(a.chunks * waves < (1L << 31), "ssm: %ld sequences of %ld channels in %ld chunks of time", a.B, a.C, a.chunks);
+  return PH_OK;
 }
 
-template <typename T, int NS>
-int fwd_n(Args& a, float* win_out, hipStream_t st) {
-  const int nt = block_threads(a, 4);
-  a.blocks_c = (int)((a.per + nt - 1) / nt);
-  const long blocks = a.chunks * a.B * (a.C / a.per) * a.blocks_c;
+template <typename T>
+int fwd_t(Args& a, float* win_out, hipStream_t st) {
+  const int nt = block_threads(a, false);
+  const size_t lds = fwd_lds(a.Q, nt);
+  a.blocks_c = (unsigned)((a.per + nt - 1) / nt);
+  const unsigned blocks = (unsigned)(a.chunks * a.B * a.G * a.blocks_c);
+  const int most = (kSteps * 8 * a.Q + nt - 1) / nt;
   if (a.chunks > 1) {
-    k_ssm_fwd<T, NS, true><<<(unsigned)blocks, nt, 0, st>>>(a);
+    if (most <= 1) k_ssm_fwd<T, true, 1><<<blocks, nt, lds, st>>>(a);
+    else if (most <= 4) k_ssm_fwd<T, true, 4><<<blocks, nt, lds, st>>>(a);
+    else k_ssm_fwd<T, true, 16><<<blocks, nt, lds, st>>>(a);
     PH_LAUNCH_CHECK();
-    k_ssm_join<<<ceil_div((size_t)(a.B * a.C * a.N), 256), 256, 0, st>>>(a);
+    k_ssm_join<<<ceil_div((size_t)(a.B * a.C * 4 * a.Q), 256), 256, 0, st>>>(a);
     PH_LAUNCH_CHECK();
   }
-  k_ssm_fwd<T, NS, false><<<(unsigned)blocks, nt, 0, st>>>(a);
+  if (most <= 1) k_ssm_fwd<T, false, 1><<<blocks, nt, lds, st>>>(a);
+  else if (most <= 4) k_ssm_fwd<T, false, 4><<<blocks, nt, lds, st>>>(a);
+  else k_ssm_fwd<T, false, 16><<<blocks, nt, lds, st>>>(a);
   PH_LAUNCH_CHECK();
   if (win_out && a.K > 1) {
     k_ssm_window<T><<<ceil_div((size_t)(a.B * a.C), 256), 256, 0, st>>>(a, win_out);
@@ -820,40 +1020,25 @@ int fwd_n(Args& a, float* win_out, hipStream_t st) {
 }
 
 template <typename T>
-int fwd_t(Args& a, float* win_out, hipStream_t st) {
-  switch (states_of(a.N)) {
-    case 4: return fwd_n<T, 4>(a, win_out, st);
-    case 8: return fwd_n<T, 8>(a, win_out, st);
-    case 16: return fwd_n<T, 16>(a, win_out, st);
-    case 32: return fwd_n<T, 32>(a, win_out, st);
-    default: return fwd_n<T, 64>(a, win_out, st);
-  }
-}
-
-template <typename T, int NS>
-int bwd_n(Args& a, GradArgs& ga, const ParOut& po, hipStream_t st) {
-  constexpr int kS = keep_steps(NS);
-  const int nl = block_threads(a, 4), nt = block_threads(a, bwd_waves(NS));
-  const long G = a.C / a.per;
+int bwd_t(Args& a, GradArgs& ga, int nt, const ParOut& po, hipStream_t st) {
   if (a.chunks > 1) {
-    a.blocks_c = (int)((a.per + nl - 1) / nl);
-    k_ssm_bwd_local<T, NS><<<(unsigned)(a.chunks * a.B * G * a.blocks_c), nl, 0, st>>>(a, ga);
+    const unsigned blocks = (unsigned)(a.chunks * a.B * a.G * a.blocks_c);
+    const int most = (kSteps * 8 * a.Q + nt - 1) / nt;
+    if (most <= 1) k_ssm_bwd_local<T, 1><<<blocks, nt, fwd_lds(a.Q, nt), st>>>(a, ga);
+    else if (most <= 4) k_ssm_bwd_local<T, 4><<<blocks, nt, fwd_lds(a.Q, nt), st>>>(a, ga);
+    else k_ssm_bwd_local<T, 16><<<blocks, nt, fwd_lds(a.Q, nt), st>>>(a, ga);
     PH_LAUNCH_CHECK();
-    k_ssm_bwd_join<<<ceil_div((size_t)(a.B * a.C * a.N), 256), 256, 0, st>>>(a, ga);
+    k_ssm_bwd_join<<<ceil_div((size_t)(a.B * a.C * 4 * a.Q), 256), 256, 0, st>>>(a, ga);
     PH_LAUNCH_CHECK();
   }
-  a.blocks_c = (int)((a.per + nt - 1) / nt);
-  const size_t lds = (size_t)(1 + nt / 64) * kS * 2 * NS * 4;
-  static_assert((1 + bwd_waves(NS)) * kS * 2 * NS * 4 <= kMaxLdsBytes, "LDS budget");
-  k_ssm_bwd<T, NS><<<(unsigned)(ga.rows * G * a.blocks_c), nt, lds, st>>>(a, ga);
+  k_ssm_bwd<T><<<(unsigned)(ga.rows * a.G * a.blocks_c), nt, bwd_lds(a.Q, nt), st>>>(a, ga);
   PH_LAUNCH_CHECK();
   if (a.chunks > 1 && a.K > 1 && ga.dx) {
     k_ssm_halo<T><<<ceil_div((size_t)((a.chunks - 1) * a.B * (a.K - 1) * a.C), 256), 256, 0, st>>>(a, ga);
     PH_LAUNCH_CHECK();
   }
   if (ga.bc) {
-    const size_t n = (size_t)a.T * a.B * G * 2 * a.N;
-    const unsigned blocks = ceil_div(n, 256);
+    const unsigned blocks = ceil_div((size_t)a.T * a.B * a.G * 2 * a.N, 256);
     k_ssm_fold_bc<T><<<blocks < 8192 ? blocks : 8192, 256, 0, st>>>(a, ga);
     PH_LAUNCH_CHECK();
   }
@@ -863,20 +1048,10 @@ int bwd_n(Args& a, GradArgs& ga, const ParOut& po, hipStream_t st) {
   return PH_OK;
 }
 
-template <typename T>
-int bwd_t(Args& a, GradArgs& ga, const ParOut& po, hipStream_t st) {
-  switch (states_of(a.N)) {
-    case 4: return bwd_n<T, 4>(a, ga, po, st);
-    case 8: return bwd_n<T, 8>(a, ga, po, st);
-    case 16: return bwd_n<T, 16>(a, ga, po, st);
-    case 32: return bwd_n<T, 32>(a, ga, po, st);
-    default: return bwd_n<T, 64>(a, ga, po, st);
-  }
-}
-
 template <typename T, bool VEC>
 int step_t(const Args& a, float* h, float* win, hipStream_t st) {
-  const int lpc = states_of(a.N) / 4;
+  int lpc = 1;  // lanes of a channel: a power of two, as the shuffles need
+  while (lpc < a.Q) lpc *= 2;
   const unsigned grid = (unsigned)((a.C + 256 / lpc - 1) / (256 / lpc) * a.B);
   switch (lpc) {
     case 1: k_ssm_step<T, 1, VEC><<<grid, 256, 0, st>>>(a, h, win); break;
@@ -909,8 +1084,7 @@ using namespace ph;
 
 extern "C" size_t ph_ssm_keep_floats(const ph_ssm_args* p) {
   if (!p || p->N < 1 || p->N > (size_t)kMaxStates) return 0;
-  const size_t ks = (size_t)keep_steps(states_of((long)p->N));
-  return (p->T + ks - 1) / ks * p->B * p->C * p->N;
+  return (p->T + kSteps - 1) / kSteps * p->B * p->C * ((p->N + 3) / 4 * 4);
 }
 
 extern "C" int ph_ssm_scan(const ph_ssm_args* p, void* y, long y_t, long y_b, float* h_out, float* win_out, float* keep,
@@ -923,9 +1097,9 @@ extern "C" int ph_ssm_scan(const ph_ssm_args* p, void* y, long y_t, long y_b, fl
   hipStream_t st = as_stream(stream);
   Args a = args_of(*p);
   a.y = y; a.y_t = y_t; a.y_b = y_b; a.h_out = h_out; a.keep = keep;
-  set_chunks(a);
+  PH_TRY(set_chunks(a));
   if (a.chunks > 1) {
-    const size_t nh = (size_t)a.chunks * a.B * a.C * a.N, nd = (size_t)a.chunks * a.B * a.C;
+    const size_t nh = (size_t)a.chunks * a.B * a.C * 4 * a.Q, nd = (size_t)a.chunks * a.B * a.C;
     float* ws = (float*)scratch(kSlotSsm, (nh + nd) * 4);
     if (!ws) return PH_ERR_NOMEM;
     a.hloc = ws;
@@ -948,7 +1122,7 @@ extern "C" int ph_ssm_scan_grad(const ph_ssm_args* p, const float* keep, const v
   PH_REQUIRE(p->T >= 1, "ssm_scan_grad: no steps");
   PH_REQUIRE(dy && keep, "ssm_scan_grad: dy or the kept states missing");
   Args a = args_of(*p);
-  set_chunks(a);
+  PH_TRY(set_chunks(a));
   GradArgs ga{};
   ga.dy = dy; ga.dy_t = dy_t; ga.dy_b = dy_b; ga.keep = keep;
   ga.dx = g->dx; ga.dx_t = g->dx_t; ga.dx_b = g->dx_b;
@@ -957,13 +1131,15 @@ extern "C" int ph_ssm_scan_grad(const ph_ssm_args* p, const float* keep, const v
   ga.dB = g->dBm; ga.db_t = g->dBm_t; ga.db_b = g->dBm_b;
   ga.dC = g->dCm; ga.dc_t = g->dCm_t; ga.dc_b = g->dCm_b;
   ga.P = (int)(a.N + a.K + 3);
-  const long G = a.C / a.per, nt = block_threads(a, bwd_waves(states_of(a.N))), bc = (a.per + nt - 1) / nt;
+  const int nt = block_threads(a, true);
+  const long G = a.G, bc = (a.per + nt - 1) / nt;
+  a.blocks_c = (unsigned)bc;
   // blocks of a channel block: a few for every CU, each with many items of its own
   const long items = a.B * a.chunks;
-  ga.rows = 1024 / (G * bc);
+  ga.rows = 512 / (G * bc);
   if (ga.rows > items) ga.rows = items;
   if (ga.rows < 1) ga.rows = 1;
-  const size_t nh = a.chunks > 1 ? (size_t)a.chunks * a.B * a.C * a.N : 0, nd = a.chunks > 1 ? (size_t)a.chunks * a.B * a.C : 0;
+  const size_t nh = a.chunks > 1 ? (size_t)a.chunks * a.B * a.C * 4 * a.Q : 0, nd = a.chunks > 1 ? (size_t)a.chunks * a.B * a.C : 0;
   const size_t nhalo = a.chunks > 1 ? (size_t)(2 * a.chunks) * a.B * (kTaps - 1) * a.C : 0;
   const size_t nbc = bc > 1 && (ga.dB || ga.dC) ? (size_t)bc * a.T * a.B * G * 2 * a.N : 0;
   const size_t npar = (size_t)ga.rows * a.C * ga.P;
@@ -974,7 +1150,7 @@ extern "C" int ph_ssm_scan_grad(const ph_ssm_args* p, const float* keep, const v
   ga.halo = ws + nh + nd;
   ga.bc = nbc ? ws + nh + nd + nhalo : nullptr;
   ga.par = ws + nh + nd + nhalo + nbc;
-  return p->dtype == PH_BF16 ? bwd_t<uint16_t>(a, ga, po, st) : bwd_t<float>(a, ga, po, st);
+  return p->dtype == PH_BF16 ? bwd_t<uint16_t>(a, ga, nt, po, st) : bwd_t<float>(a, ga, nt, po, st);
 }
 
 extern "C" int ph_ssm_step(const ph_ssm_args* p, void* y, long y_b, float* h, float* win, void* stream) {
@@ -986,8 +1162,7 @@ extern "C" int ph_ssm_step(const ph_ssm_args* p, void* y, long y_b, float* h, fl
   PH_REQUIRE(p->K < 2 || win, "ssm_step: the convolution's window missing");
   Args a = args_of(*p);
   a.y = y; a.y_b = y_b;
-  const bool vec = p->N % 4 == 0 && ((uintptr_t)h % 16) == 0 && ((uintptr_t)p->A % 16) == 0 &&
-                   (states_of((long)p->N) == (long)p->N);
+  const bool vec = p->N >= 4 && (p->N & (p->N - 1)) == 0 && ((uintptr_t)h % 16) == 0 && ((uintptr_t)p->A % 16) == 0;
   hipStream_t st = as_stream(stream);
   if (p->dtype == PH_BF16) return vec ? step_t<uint16_t, true>(a, h, win, st) : step_t<uint16_t, false>(a, h, win, st);
   return vec ? step_t<float, true>(a, h, win, st) : step_t<float, false>(a, h, win, st);
