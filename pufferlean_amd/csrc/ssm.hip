@@ -400,75 +400,116 @@ __global__ void __launch_bounds__(256) k_ssm_window(Args a, float* win) {
 }
 
 // ---- single tokens -------------------------------------------------------------------------------------
-// One step of every sequence, the state updated in place: bound by the state's 8 bytes per element. Four lanes'
-// worth of a channel: each lane holds four consecutive states (one 16-byte access each way), LPC lanes a channel.
-template <typename T, int LPC, bool VEC>
-__global__ void __launch_bounds__(256) k_ssm_step(Args a, float* __restrict__ hs, float* __restrict__ win) {
-  const long nb = (a.C + 256 / LPC - 1) / (256 / LPC), b = blockIdx.x / nb;
-  const long cc = (blockIdx.x % nb) * (256 / LPC) + threadIdx.x / LPC;
-  const bool in = cc < a.C;  // the lanes of a channel agree; the shuffles stay inside them
-  const long c = in ? cc : a.C - 1;
-  const int n0 = (threadIdx.x % LPC) * 4, N = (int)a.N;
-  const bool clear = a.first && a.first[b] != 0.f;
-  float* hp = hs + (b * a.C + c) * N + n0;
-  float h[4], Av[4], Bv[4], Cv[4];
-  if constexpr (VEC) {
-    const float4 hv = *reinterpret_cast<const float4*>(hp), av = *reinterpret_cast<const float4*>(a.A + c * N + n0);
-    h[0] = hv.x; h[1] = hv.y; h[2] = hv.z; h[3] = hv.w;
-    Av[0] = av.x; Av[1] = av.y; Av[2] = av.z; Av[3] = av.w;
-  } else {
+// Four consecutive elements of a row of B or C.
+__device__ __forceinline__ float4 quad_of(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 quad_of(const uint16_t* p) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  return make_float4(__builtin_bit_cast(float, v.x << 16), __builtin_bit_cast(float, v.x & 0xffff0000u),
+                     __builtin_bit_cast(float, v.y << 16), __builtin_bit_cast(float, v.y & 0xffff0000u));
+}
+
+// One step of every sequence, the state updated in place: bound by the state's 8 bytes per element, so what a channel
+// needs once (convolution, time step, gate) is computed once, by the lane of that channel, and handed over through LDS to
+// the lanes that move the state, each four states of it as one 16-byte access (consecutive lanes, consecutive
+// addresses). QT: Q where it is 1, 2 or 4 and every access may be a vector one (VEC), with the decays in registers over
+// the block's sequences; 0: any Q.
+template <typename T, int QT>
+__global__ void __launch_bounds__(256) k_ssm_step(Args a, float* __restrict__ hs, float* __restrict__ win, int per_block) {
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  const int nt = blockDim.x, tid = threadIdx.x, Q = QT ? QT : a.Q, N = (int)a.N;
+  float* sd = lds;           // [nt] d
+  float* sdu = lds + nt;     // [nt] d u
+  float* so = lds + 2 * nt;  // [nt][Q] shares of <h, C>
+  const unsigned nblk = (unsigned)((a.C + nt - 1) / nt), cb = uniform(blockIdx.x % nblk);
+  const long b0 = (long)uniform(blockIdx.x / nblk) * per_block, b1 = min(a.B, b0 + per_block);
+  const long c0 = (long)cb * nt;
+  const bool in = c0 + tid < a.C;
+  const unsigned c = (unsigned)(in ? c0 + tid : a.C - 1);
+  const int K = (int)a.K, chans = (int)min((long)nt, a.C - c0);
+  Conv cv;
+  cv.init(a, c);
+  const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, Dc = a.D ? a.D[c] : 0.f;
+  float4 Av[QT ? QT : 1];
+  int lcs[QT ? QT : 1], goff[QT ? QT : 1];
+  if constexpr (QT > 0) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const bool ok = n0 + i < N;
-      h[i] = ok ? hp[i] : 0.f;
-      Av[i] = ok ? a.A[c * N + n0 + i] : 0.f;
+    for (int j = 0; j < QT; j++) {
+      const int idx = j * nt + tid, lc = idx / QT;
+      lcs[j] = lc;
+      const long ch = c0 + (lc < chans ? lc : 0);
+      goff[j] = (int)(ch / a.per) * N + 4 * (idx % QT);
+      const float4 v = lc < chans ? *reinterpret_cast<const float4*>(a.A + c0 * N + 4 * idx) : make_float4(0.f, 0.f, 0.f, 0.f);
+      Av[j] = make_float4(v.x * kLog2e, v.y * kLog2e, v.z * kLog2e, v.w * kLog2e);
     }
   }
-  const long g = c / a.per;
+  for (long b = b0; b < b1; b++) {
+    const bool clear = a.first && a.first[b] != 0.f;
+    float* hb = hs + (b * a.C + c0) * N;
+    const T* Bp = (const T*)a.Bm + b * a.bm_b;
+    const T* Cp = (const T*)a.Cm + b * a.cm_b;
+    float4 hv[QT ? QT : 1];
+    if constexpr (QT > 0) {  // the state's loads first
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const bool ok = n0 + i < N;
-    Bv[i] = ok ? ldf((const T*)a.Bm + b * a.bm_b + g * N + n0 + i) : 0.f;
-    Cv[i] = ok ? ldf((const T*)a.Cm + b * a.cm_b + g * N + n0 + i) : 0.f;
-  }
-  const float x = ldf((const T*)a.x + b * a.x_b + c);
-  const int K = (int)a.K;
-  float u = x;
-  if (K) {
-    float s = a.conv_b ? a.conv_b[c] : 0.f;
-    float p[kTaps - 1] = {};
-    for (int k = 0; k < K - 1; k++) {
-      p[k] = clear ? 0.f : win[(b * (K - 1) + k) * a.C + c];
-      s = fmaf(a.conv_w[c * K + k], p[k], s);
+      for (int j = 0; j < QT; j++)
+        hv[j] = lcs[j] < chans && !clear ? *reinterpret_cast<const float4*>(hb + 4 * (j * nt + tid)) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    s = fmaf(a.conv_w[c * K + K - 1], x, s);
-    u = silu(s);
-    // one lane of the channel moves the window on; its wavefront's loads of it are done (they fed s)
-    if (in && n0 == 0)
-      for (int k = 0; k < K - 1; k++) win[(b * (K - 1) + k) * a.C + c] = k + 1 < K - 1 ? p[k + 1] : x;
-  }
-  const float d = softplus(ldf((const T*)a.delta + b * a.d_b + c) + (a.dt_bias ? a.dt_bias[c] : 0.f)), du = d * u;
-  float o = 0.f;
+    const float x = ldf((const T*)a.x + b * a.x_b + c);
+    float u = x;
+    if (K) {
+      float* wp = win + b * (K - 1) * a.C;
+      const float x1 = K > 1 && !clear ? wp[(K - 2) * a.C + c] : 0.f, x2 = K > 2 && !clear ? wp[(K - 3) * a.C + c] : 0.f,
+                  x3 = K > 3 && !clear ? wp[c] : 0.f;
+      u = silu(cv.pre(x, x1, x2, x3));
+      if (in) {  // the window moves on
+        if (K > 1) wp[(K - 2) * a.C + c] = x;
+        if (K > 2) wp[(K - 3) * a.C + c] = x1;
+        if (K > 3) wp[c] = x2;
+      }
+    }
+    const float d = softplus(ldf((const T*)a.delta + b * a.d_b + c) + bias);
+    sd[tid] = d;
+    sdu[tid] = d * u;
+    __syncthreads();
+    if constexpr (QT > 0) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    h[i] = fmaf(ex2(d * (Av[i] * kLog2e)), clear ? 0.f : h[i], du * Bv[i]);
-    o = fmaf(h[i], Cv[i], o);
-  }
-  if (in) {
-    if constexpr (VEC) {
-      *reinterpret_cast<float4*>(hp) = make_float4(h[0], h[1], h[2], h[3]);
+      for (int j = 0; j < QT; j++) {
+        if (lcs[j] >= chans) continue;
+        const float dd = sd[lcs[j]], du = sdu[lcs[j]];
+        const float4 Bv = quad_of(Bp + goff[j]), Cv = quad_of(Cp + goff[j]), A = Av[j];
+        float4 h = hv[j];
+        h.x = fmaf(ex2(dd * A.x), h.x, du * Bv.x);
+        h.y = fmaf(ex2(dd * A.y), h.y, du * Bv.y);
+        h.z = fmaf(ex2(dd * A.z), h.z, du * Bv.z);
+        h.w = fmaf(ex2(dd * A.w), h.w, du * Bv.w);
+        *reinterpret_cast<float4*>(hb + 4 * (j * nt + tid)) = h;
+        so[j * nt + tid] = fmaf(h.x, Cv.x, fmaf(h.y, Cv.y, fmaf(h.z, Cv.z, h.w * Cv.w)));
+      }
     } else {
+      for (int idx = tid; idx < chans * Q; idx += nt) {
+        const int lc = idx / Q, n0 = 4 * (idx - lc * Q);
+        const long ch = c0 + lc, g = ch / a.per;
+        const float dd = sd[lc], du = sdu[lc];
+        float o = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (n0 + i < N) hp[i] = h[i];
+        for (int i = 0; i < 4; i++) {
+          const int n = n0 + i;
+          if (n >= N) break;
+          float h = clear ? 0.f : hb[lc * N + n];
+          h = fmaf(ex2(dd * (a.A[ch * N + n] * kLog2e)), h, du * ldf(Bp + g * N + n));
+          hb[lc * N + n] = h;
+          o = fmaf(h, ldf(Cp + g * N + n), o);
+        }
+        so[idx] = o;
+      }
     }
-  }
-#pragma unroll
-  for (int m = 1; m < LPC; m <<= 1) o += __shfl_xor(o, m);
-  if (in && n0 == 0) {
-    o = fmaf(a.D ? a.D[c] : 0.f, u, o);
-    if (a.z) o *= silu(ldf((const T*)a.z + b * a.z_b + c));
-    stf((T*)a.y + b * a.y_b + c, o);
+    __syncthreads();
+    if (in) {
+      float o = Dc * u;
+      for (int q = 0; q < Q; q++) o += so[tid * Q + q];
+      if (a.z) o *= silu(ldf((const T*)a.z + b * a.z_b + c));
+      stf((T*)a.y + b * a.y_b + c, o);
+    }
+    // the next sequence writes sd and sdu, which nobody reads any more, and so only after its own barrier
   }
 }
 
@@ -1048,18 +1089,25 @@ int bwd_t(Args& a, GradArgs& ga, int nt, const ParOut& po, hipStream_t st) {
   return PH_OK;
 }
 
-template <typename T, bool VEC>
+template <typename T>
 int step_t(const Args& a, float* h, float* win, hipStream_t st) {
-  int lpc = 1;  // lanes of a channel: a power of two, as the shuffles need
-  while (lpc < a.Q) lpc *= 2;
-  const unsigned grid = (unsigned)((a.C + 256 / lpc - 1) / (256 / lpc) * a.B);
-  switch (lpc) {
-    case 1: k_ssm_step<T, 1, VEC><<<grid, 256, 0, st>>>(a, h, win); break;
-    case 2: k_ssm_step<T, 2, VEC><<<grid, 256, 0, st>>>(a, h, win); break;
-    case 4: k_ssm_step<T, 4, VEC><<<grid, 256, 0, st>>>(a, h, win); break;
-    case 8: k_ssm_step<T, 8, VEC><<<grid, 256, 0, st>>>(a, h, win); break;
-    default: k_ssm_step<T, 16, VEC><<<grid, 256, 0, st>>>(a, h, win); break;
-  }
+  const long w = (a.C + 63) / 64;
+  const int nt = 64 * (int)(w < 4 ? w : 4);
+  const long nblk = (a.C + nt - 1) / nt;
+  // sequences of a block: what it loads once (decays, taps) is worth a few, as long as eight blocks are left for a CU
+  long per_block = a.B * nblk / 2048;
+  per_block = per_block < 1 ? 1 : per_block > 8 ? 8 : per_block;
+  const long blocks = nblk * ((a.B + per_block - 1) / per_block);
+  PH_REQUIRE(blocks < (1L << 31), "ssm_step: %ld sequences of %ld channels", a.B, a.C);
+  const size_t lds = (size_t)(2 + a.Q) * nt * 4;
+  const size_t ea = 4 * sizeof(T);  // a quad of B or C
+  const bool vec = a.N % 4 == 0 && ((uintptr_t)h % 16) == 0 && ((uintptr_t)a.A % 16) == 0 && ((uintptr_t)a.Bm % ea) == 0 &&
+                   ((uintptr_t)a.Cm % ea) == 0 && a.bm_b % 4 == 0 && a.cm_b % 4 == 0;
+  const int qt = vec && (a.Q == 1 || a.Q == 2 || a.Q == 4) ? a.Q : 0;
+  if (qt == 1) k_ssm_step<T, 1><<<(unsigned)blocks, nt, lds, st>>>(a, h, win, (int)per_block);
+  else if (qt == 2) k_ssm_step<T, 2><<<(unsigned)blocks, nt, lds, st>>>(a, h, win, (int)per_block);
+  else if (qt == 4) k_ssm_step<T, 4><<<(unsigned)blocks, nt, lds, st>>>(a, h, win, (int)per_block);
+  else k_ssm_step<T, 0><<<(unsigned)blocks, nt, lds, st>>>(a, h, win, (int)per_block);
   PH_LAUNCH_CHECK();
   return PH_OK;
 }
@@ -1162,8 +1210,6 @@ extern "C" int ph_ssm_step(const ph_ssm_args* p, void* y, long y_b, float* h, fl
   PH_REQUIRE(p->K < 2 || win, "ssm_step: the convolution's window missing");
   Args a = args_of(*p);
   a.y = y; a.y_b = y_b;
-  const bool vec = p->N >= 4 && (p->N & (p->N - 1)) == 0 && ((uintptr_t)h % 16) == 0 && ((uintptr_t)p->A % 16) == 0;
   hipStream_t st = as_stream(stream);
-  if (p->dtype == PH_BF16) return vec ? step_t<uint16_t, true>(a, h, win, st) : step_t<uint16_t, false>(a, h, win, st);
-  return vec ? step_t<float, true>(a, h, win, st) : step_t<float, false>(a, h, win, st);
+  return p->dtype == PH_BF16 ? step_t<uint16_t>(a, h, win, st) : step_t<float>(a, h, win, st);
 }
