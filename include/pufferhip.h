@@ -438,16 +438,16 @@ int ph_ssm_step(const ph_ssm_args* a, void* y, long y_b, float* h, float* win, v
  * are part of that product's epilogue; w_out [D][F]. Both in dtype; PH_BF16 runs bf16 MFMA with fp32 accumulation,
  * PH_F32 fp32 MFMA. */
 typedef enum { PH_ACT_SILU = 0, PH_ACT_GELU = 1 } ph_act;
-/* ab [M][ph_ffn_pitch(2F)] and h [M][ph_ffn_pitch(F)] (dtype): the projections and the units for the gradient; both
- * NULL where no gradient follows. */
+/* pf [M][2 ph_ffn_pitch(F)] and h [M][ph_ffn_pitch(F)] (dtype, 16-byte aligned) receive what the gradient needs: the units
+ * h_j = act(a_j) v_j, and the pairs v_j act'(a_j), act(a_j). Both NULL where no gradient follows. */
 int ph_ffn(int dtype, int act, size_t M, size_t D, size_t F, const void* x, size_t ldx, const void* w_in,
-           const void* w_out, void* ab, void* h, void* y, size_t ldy, void* stream);
-/* Row pitch of ab and h: their columns rounded up to whole 16-byte accesses. */
+           const void* w_out, void* pf, void* h, void* y, size_t ldy, void* stream);
+/* Row pitch of `columns` values in whole 16-byte accesses. */
 size_t ph_ffn_pitch(size_t columns);
 /* dx [M][D], dw_in [2F][D] and dw_out [D][F], each written where not NULL; the weights' gradients in dw_dtype (dtype or
  * PH_F32), overwritten. */
 int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, const void* x, size_t ldx, const void* w_in,
-                const void* w_out, const void* ab, const void* h, const void* dy, size_t lddy, void* dx, size_t lddx,
+                const void* w_out, const void* pf, const void* h, const void* dy, size_t lddy, void* dx, size_t lddx,
                 int dw_dtype, void* dw_in, void* dw_out, void* stream);
 
 /* ============================================================================================== */

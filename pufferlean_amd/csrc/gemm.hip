@@ -18,6 +18,7 @@
 // optional second bf16 output (plain or transposed). Split-K writes fp32 partials per split and a
 // second kernel adds them in split order (deterministic).
 #include "common.hpp"
+#include "glu.hpp"
 #include "kernels.hpp"
 #include "routes.hpp"
 
@@ -806,12 +807,107 @@ __device__ __forceinline__ void flush_bf16(const GemmArgs& g, const uint32_t* sT
   }
 }
 
+// Eight consecutive values of a row.
+__device__ __forceinline__ void load8_of(const float* p, float (&v)[8]) {
+  const float4 a = load4_f32(p), b = load4_f32(p + 4);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void store8_of(uint16_t* p, const float* v) {
+  store8(p, make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]));
+}
+__device__ __forceinline__ void store8_of(float* p, const float* v) {
+  store4(p, make_float4(v[0], v[1], v[2], v[3]));
+  store4(p + 4, make_float4(v[4], v[5], v[6], v[7]));
+}
+
+// Epilogue of the gated feed-forward products (glu.hpp) on a staged tile: kGluUnits turns each pair of columns into a unit,
+// so neither projection is written and read again; kGluGrad turns a unit's gradient into its pair. Here C is h (or
+// dab), C2 and aux are pf, and epi is the activation. Rows as in flush_tile.
+enum : int { kGluNone = 0, kGluUnits = 1, kGluGrad = 2 };
+// Four bf16 (fp32) values as one 8-byte (16-byte) store.
+__device__ __forceinline__ void store4_once(uint16_t* p, const float* v) {
+  typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+  const u32x2_t w = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+  __builtin_nontemporal_store(w, reinterpret_cast<u32x2_t*>(p));
+}
+__device__ __forceinline__ void store4_once(float* p, const float* v) { store4(p, make_float4(v[0], v[1], v[2], v[3])); }
+
+// kGluGrad's factors of a pass, loaded before the pass is staged and all waited for before its first store: loads and
+// stores share one counter, so a load behind a store would wait for that store's round trip.
+template <int GLU, typename TC, int BM, int BN, int NT>
+struct GluFactors {
+  static constexpr int CPR = BN / 8, NCH = GLU == kGluGrad ? BM * CPR / NT : 1;
+  Raw8<TC> v[NCH][2];
+  __device__ __forceinline__ void load(const GemmArgs& g, int m0, int n0, int mhi = -1) {
+    if constexpr (GLU == kGluGrad) {
+      if (mhi < 0) mhi = m0 + BM / 2;
+#pragma unroll
+      for (int q = 0; q < NCH; q++) {
+        const int c = threadIdx.x + q * NT, lr = c / CPR, lc = (c % CPR) * 8;
+        const int row = lr < BM / 2 ? m0 + lr : mhi + (lr - BM / 2), col = n0 + lc;
+        const bool in = row < g.M && col < g.N;
+        const gptr<TC> p = (gptr<TC>)g.aux + (long)row * g.ldaux + 2 * col;
+        v[q][0] = load_raw8(in ? p : zero_page<TC>());
+        v[q][1] = load_raw8(in ? p + 8 : zero_page<TC>());
+      }
+    }
+  }
+};
+__device__ __forceinline__ void cvt8(const Raw8<uint16_t>& r, float (&v)[8]) {
+  const float4 a = cvt4(EpiRaw4<uint16_t>{make_uint2(r.v.x, r.v.y)}), b = cvt4(EpiRaw4<uint16_t>{make_uint2(r.v.z, r.v.w)});
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void cvt8(const Raw8<float>& r, float (&v)[8]) {
+  v[0] = r.a.x; v[1] = r.a.y; v[2] = r.a.z; v[3] = r.a.w; v[4] = r.b.x; v[5] = r.b.y; v[6] = r.b.z; v[7] = r.b.w;
+}
+
+template <int GLU, typename TC, int BM, int BN, int NT, int LDC>
+__device__ __forceinline__ void flush_glu(const GemmArgs& g, const float* sC, const GluFactors<GLU, TC, BM, BN, NT>& fac, int m0,
+                                          int n0, int mhi = -1) {
+  constexpr int CPR = BN / 8, NCH = BM * CPR / NT;
+  static_assert(NCH * NT == BM * CPR, "C tile / threads");
+  if (mhi < 0) mhi = m0 + BM / 2;
+  const int tid = threadIdx.x;
+  if constexpr (GLU == kGluGrad) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+#pragma unroll
+  for (int q = 0; q < NCH; q++) {
+    const int c = tid + q * NT, lr = c / CPR, lc = (c % CPR) * 8;
+    const int row = lr < BM / 2 ? m0 + lr : mhi + (lr - BM / 2), col = n0 + lc;
+    if (row >= g.M || col >= g.N) continue;
+    float v[8];
+    load8_of(&sC[lr * LDC + lc], v);
+    TC* out = reinterpret_cast<TC*>(g.C) + (long)row * g.ldc;
+    if constexpr (GLU == kGluUnits) {
+      float h[4], pf[8];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        float f, df;
+        glu_act(g.epi, v[2 * j], f, df);
+        h[j] = f * v[2 * j + 1];
+        pf[2 * j] = v[2 * j + 1] * df;
+        pf[2 * j + 1] = f;
+      }
+      store4_once(out + col / 2, h);
+      if (g.C2) store8_of(reinterpret_cast<TC*>(g.C2) + (long)row * g.ldc2 + col, pf);
+    } else {
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        float m[8], d[8];
+        cvt8(fac.v[q][half], m);
+#pragma unroll
+        for (int j = 0; j < 8; j++) d[j] = v[4 * half + j / 2] * m[j];
+        store8_of(out + 2 * col + 8 * half, d);
+      }
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------
 // bf16-math kernel. WGM x WGN wavefronts; prefetch distance 2: while k-tile kt is multiplied out of
 // LDS, tile kt+1 sits in registers and tile kt+2 is in flight from memory. The two register sets
 // alternate, so the k loop is unrolled by two to keep every register index static.
 template <int BM, int BN, int BK, int WGM, int WGN, bool TA, bool TB, typename TIA, typename TIB,
-          typename TC, bool X3 = false>
+          typename TC, bool X3 = false, int GLU = kGluNone>
 __global__ void __launch_bounds__(WGM * WGN * 64) k_gemm_bf16(GemmArgs g) {
   // X3: fp32 operands split as x = hi + lo (both bf16); acc += hi*hi + hi*lo + lo*hi
   static_assert(!X3 || (sizeof(TIA) == 4 && sizeof(TIB) == 4), "split-bf16 needs fp32 operands");
@@ -1097,16 +1193,22 @@ __global__ void __launch_bounds__(WGM * WGN * 64) k_gemm_bf16(GemmArgs g) {
 
   // the last loop iteration ended with a barrier: the pipeline buffers are free for the C tile
   if constexpr (EPR == BM) {
+    GluFactors<GLU, TC, BM, BN, NT> fac;
+    if constexpr (GLU == kGluGrad) fac.load(g, m0, n0);
     stage_acc<SM, SN, LDC>(sC, acc, wm0, wn0, lane);
     lds_barrier();
-    flush_tile<TC, BM, BN, NT, LDC>(g, sC, m0, n0);
+    if constexpr (GLU != kGluNone) flush_glu<GLU, TC, BM, BN, NT, LDC>(g, sC, fac, m0, n0);
+    else flush_tile<TC, BM, BN, NT, LDC>(g, sC, m0, n0);
   } else {
 #pragma unroll 1
     for (int p = 0; p < BM / EPR; p++) {
+      GluFactors<GLU, TC, EPR, BN, NT> fac;
+      if constexpr (GLU == kGluGrad) fac.load(g, m0 + p * EPR, n0);
       if (p > 0) lds_barrier();  // the previous pass's flush has read the staging area
       stage_acc_rows<SM, SN, LDC>(sC, acc, wm0 - p * EPR, wn0, lane, EPR);
       lds_barrier();
-      flush_tile<TC, EPR, BN, NT, LDC>(g, sC, m0 + p * EPR, n0);
+      if constexpr (GLU != kGluNone) flush_glu<GLU, TC, EPR, BN, NT, LDC>(g, sC, fac, m0 + p * EPR, n0);
+      else flush_tile<TC, EPR, BN, NT, LDC>(g, sC, m0 + p * EPR, n0);
     }
   }
 }
@@ -1174,7 +1276,8 @@ __device__ __forceinline__ uint4 rd_tr(const uint16_t* s, int c0, int koff, int 
 // TN: A stored [K][M] and B stored [K][N] (the weight-gradient form): each stage holds BK k-rows of the
 // BM (BN) columns, the 16-byte chunks of a row XOR-permuted by the row's low two bits, and fragments are
 // read with the LDS transpose read (ds_read_b64_tr_b16, two per fragment).
-template <int BM, int BN, typename TC, bool S16 = false, int WGM = 2, int WGN = 2, int NSTG = 3, bool TN = false>
+template <int BM, int BN, typename TC, bool S16 = false, int WGM = 2, int WGN = 2, int NSTG = 3, bool TN = false,
+          int GLU = kGluNone>
 __global__ void __launch_bounds__(64 * WGM * WGN, WGM * WGN == 4 ? 2 : 1) k_gemm_nt_dma(GemmArgs g) {
   constexpr int BK = 32, NT = 64 * WGM * WGN;
   static_assert(!TN || (BM >= 128 && BN >= 128 && !S16), "transposed stages: 16+ chunks per row");
@@ -1378,16 +1481,22 @@ __global__ void __launch_bounds__(64 * WGM * WGN, WGM * WGN == 4 ? 2 : 1) k_gemm
     static_assert(WM * LDC * 4 <= SMEM && WM % 8 == 0, "epilogue staging rows");
     auto pass = [&](auto P) {
       constexpr int p = decltype(P)::value;
+      GluFactors<GLU, TC, WM, BN, NT> fac;
+      if constexpr (GLU == kGluGrad) fac.load(g, m0 + p * WM, n0);
       if (p > 0) lds_barrier();  // the previous pass's flush has read the staging area
       if (wave / WGN == p) stage_acc<SM, SN, LDC>(sC, acc, 0, wn0, lane);
       lds_barrier();
-      flush_tile<TC, WM, BN, NT, LDC>(g, sC, m0 + p * WM, n0);
+      if constexpr (GLU != kGluNone) flush_glu<GLU, TC, WM, BN, NT, LDC>(g, sC, fac, m0 + p * WM, n0);
+      else flush_tile<TC, WM, BN, NT, LDC>(g, sC, m0 + p * WM, n0);
     };
     static_for(pass, std::make_integer_sequence<int, WGM>{});
   } else if constexpr (EPR == BM) {
+    GluFactors<GLU, TC, BM, BN, NT> fac;
+    if constexpr (GLU == kGluGrad) fac.load(g, m0, n0);
     stage_acc<SM, SN, LDC>(sC, acc, wm0, wn0, lane);
     lds_barrier();
-    flush_tile<TC, BM, BN, NT, LDC>(g, sC, m0, n0);
+    if constexpr (GLU != kGluNone) flush_glu<GLU, TC, BM, BN, NT, LDC>(g, sC, fac, m0, n0);
+    else flush_tile<TC, BM, BN, NT, LDC>(g, sC, m0, n0);
   } else {
     // Pass p stages sub-tiles [p SMP, (p + 1) SMP) of EVERY wave (staged rows [0, EPR/2) from the
     // upper wave row, [EPR/2, EPR) from the lower), so each pass retires part of every wave's
@@ -1396,10 +1505,13 @@ __global__ void __launch_bounds__(64 * WGM * WGN, WGM * WGN == 4 ? 2 : 1) k_gemm
     static_assert(SMP * BM == SM * EPR && EPR == 2 * SMP * 32, "epilogue pass split");
     auto pass = [&](auto P) {
       constexpr int p = decltype(P)::value;
+      GluFactors<GLU, TC, EPR, BN, NT> fac;
+      if constexpr (GLU == kGluGrad) fac.load(g, m0 + p * SMP * 32, n0, m0 + WM + p * SMP * 32);
       if (p > 0) lds_barrier();  // the previous pass's flush has read the staging area
       stage_acc_part<p * SMP, SMP, SM, SN, LDC>(sC, acc, (wave / 2) * SMP * 32, wn0, lane);
       lds_barrier();
-      flush_tile<TC, EPR, BN, NT, LDC>(g, sC, m0 + p * SMP * 32, n0, m0 + WM + p * SMP * 32);
+      if constexpr (GLU != kGluNone) flush_glu<GLU, TC, EPR, BN, NT, LDC>(g, sC, fac, m0 + p * SMP * 32, n0, m0 + WM + p * SMP * 32);
+      else flush_tile<TC, EPR, BN, NT, LDC>(g, sC, m0 + p * SMP * 32, n0, m0 + WM + p * SMP * 32);
     };
     static_for(pass, std::make_integer_sequence<int, BM / EPR>{});
   }
@@ -1407,7 +1519,7 @@ __global__ void __launch_bounds__(64 * WGM * WGN, WGM * WGN == 4 ? 2 : 1) k_gemm
 
 // ------------------------------------------------------------------------------------------------
 // fp32-math kernel (fp32 inputs only).
-template <int BM, int BN, int BK, bool TA, bool TB, typename TC>
+template <int BM, int BN, int BK, bool TA, bool TB, typename TC, int GLU = kGluNone>
 __global__ void __launch_bounds__(256) k_gemm_f32(GemmArgs g) {
   constexpr int PAD = 4;
   constexpr int LDK = BK + PAD;
@@ -1539,9 +1651,12 @@ __global__ void __launch_bounds__(256) k_gemm_f32(GemmArgs g) {
     if (kt + 1 < nk) sstore(s ^ 1);
     lds_barrier();
   }
+  GluFactors<GLU, TC, BM, BN, 256> fac;
+  if constexpr (GLU == kGluGrad) fac.load(g, m0, n0);
   stage_acc<SM, SN, LDC>(sC, acc, wm0, wn0, lane);
   lds_barrier();
-  flush_tile<TC, BM, BN, 256, LDC>(g, sC, m0, n0);
+  if constexpr (GLU != kGluNone) flush_glu<GLU, TC, BM, BN, 256, LDC>(g, sC, fac, m0, n0);
+  else flush_tile<TC, BM, BN, 256, LDC>(g, sC, m0, n0);
 }
 
 // Split-K fold: C = epilogue(sum over splits). Bound by load latency for the small outputs that take many
@@ -1765,7 +1880,51 @@ int pad_operands(PhGemmDesc& d, int vec, hipStream_t st) {
   return PH_OK;
 }
 
+template <int GLU>
+int launch_glu(const GemmArgs& g, int dtype, hipStream_t st) {
+  auto tiles = [&](long bm, long bn) { return (unsigned)((g.M + bm - 1) / bm * ((g.N + bn - 1) / bn)); };
+  if (dtype == PH_BF16) {
+    // tiles as for a plain NT product: 256x256 or 256x128 from 512 of 256x128 on, whichever pads the columns less
+    if (tiles(256, 128) >= 512) {
+      const long n256 = (g.N + 255) / 256 * 256, n128 = (g.N + 127) / 128 * 128;
+      if (n256 <= n128 + n128 / 16)
+        k_gemm_nt_dma<256, 256, uint16_t, false, 4, 4, 4, false, GLU><<<tiles(256, 256), 1024, 0, st>>>(g);
+      else k_gemm_nt_dma<256, 128, uint16_t, false, 2, 2, 3, false, GLU><<<tiles(256, 128), 256, 0, st>>>(g);
+    } else if (tiles(128, 128) >= 128) {
+      k_gemm_bf16<128, 128, 64, 2, 2, false, true, uint16_t, uint16_t, uint16_t, false, GLU><<<tiles(128, 128), 256, 0, st>>>(g);
+    } else {
+      k_gemm_bf16<64, 64, 64, 2, 2, false, true, uint16_t, uint16_t, uint16_t, false, GLU><<<tiles(64, 64), 256, 0, st>>>(g);
+    }
+  } else if (tiles(128, 128) >= 128) {
+    k_gemm_f32<128, 128, 32, false, true, float, GLU><<<tiles(128, 128), 256, 0, st>>>(g);
+  } else {
+    k_gemm_f32<64, 64, 32, false, true, float, GLU><<<tiles(64, 64), 256, 0, st>>>(g);
+  }
+  PH_LAUNCH_CHECK();
+  return PH_OK;
+}
+
 }  // namespace
+
+int glu_product(const GluProduct& p, hipStream_t st) {
+  auto ok = [](const void* q, long ld) { return ((uintptr_t)q % 16) == 0 && ld % 8 == 0; };
+  PH_REQUIRE(p.N % 8 == 0 && p.K % 8 == 0 && ok(p.A, p.lda) && ok(p.B, p.ldb) && ok(p.h, p.ldh) && ok(p.pf, p.ldpf) &&
+                 ok(p.dab, p.lddab),
+             "glu_product: operands of %d x %d x %d off their alignment", p.M, p.N, p.K);
+  if (p.M == 0) return PH_OK;
+  GemmArgs g{};
+  g.M = p.M; g.N = p.N; g.K = p.K; g.kps = p.K;
+  g.A = p.A; g.lda = p.lda; g.B = p.B; g.ldb = p.ldb;
+  g.c_bf16 = p.dtype == PH_BF16;
+  g.epi = p.act;
+  g.remap = 1;
+  if (p.grad) {
+    g.C = p.dab; g.ldc = p.lddab; g.aux = p.pf; g.ldaux = p.ldpf;
+    return launch_glu<kGluGrad>(g, p.dtype, st);
+  }
+  g.C = p.h; g.ldc = p.ldh; g.C2 = (uint16_t*)p.pf; g.ldc2 = p.ldpf;
+  return launch_glu<kGluUnits>(g, p.dtype, st);
+}
 
 int gemm(const PhGemmDesc& d_in, hipStream_t st) {
   PhGemmDesc d = d_in;

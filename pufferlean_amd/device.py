@@ -649,21 +649,21 @@ def gated_ffn(x, w_in, w_out, *, act="silu", out=None, save=False):
     gated_ffn_grad needs."""
     dt, M, D, F = _ffn_shapes(x, w_in, w_out, act)
     y = torch.empty((M, D), device=x.device, dtype=x.dtype) if out is None else _like(out, x, x.shape, "out")
-    ab = h = None
+    pf = h = None
     if save:
-        ab = torch.empty((M, _pitch(2 * F)), device=x.device, dtype=x.dtype)
+        pf = torch.empty((M, 2 * _pitch(F)), device=x.device, dtype=x.dtype)
         h = torch.empty((M, _pitch(F)), device=x.device, dtype=x.dtype)
-    L.call("ph_ffn", dt, _ACT[act], M, D, F, x.data_ptr(), _rows(x), w_in.data_ptr(), w_out.data_ptr(), _ptr(ab), _ptr(h),
+    L.call("ph_ffn", dt, _ACT[act], M, D, F, x.data_ptr(), _rows(x), w_in.data_ptr(), w_out.data_ptr(), _ptr(pf), _ptr(h),
            y.data_ptr(), _rows(y), _stream())
-    return (y, (ab, h)) if save else y
+    return (y, (pf, h)) if save else y
 
 
 def gated_ffn_grad(x, w_in, w_out, saved, dy, *, act="silu", dx=None, dw_in=None, dw_out=None, dw_dtype=None):
     """Gradient of gated_ffn: (dx, dw_in, dw_out), the weights' in dw_dtype (x's dtype, or float32)."""
     dt, M, D, F = _ffn_shapes(x, w_in, w_out, act)
     _like(dy, x, x.shape, "dy")
-    ab, h = saved
-    _like(ab, x, (M, _pitch(2 * F)), "saved"), _like(h, x, (M, _pitch(F)), "saved")
+    pf, h = saved
+    _like(pf, x, (M, 2 * _pitch(F)), "saved"), _like(h, x, (M, _pitch(F)), "saved")
     dwt = dw_dtype or (x.dtype if dw_in is None else dw_in.dtype)
     dx = torch.empty((M, D), device=x.device, dtype=x.dtype) if dx is None else _like(dx, x, x.shape, "dx")
     dw_in = torch.empty((2 * F, D), device=x.device, dtype=dwt) if dw_in is None else dw_in
@@ -671,7 +671,7 @@ def gated_ffn_grad(x, w_in, w_out, saved, dy, *, act="silu", dx=None, dw_in=None
     for t, shape, what in ((dw_in, (2 * F, D), "dw_in"), (dw_out, (D, F), "dw_out")):
         if t.dtype != dwt or t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{what} must be contiguous {dwt} {shape}")
-    L.call("ph_ffn_grad", dt, _ACT[act], M, D, F, x.data_ptr(), _rows(x), w_in.data_ptr(), w_out.data_ptr(), ab.data_ptr(),
+    L.call("ph_ffn_grad", dt, _ACT[act], M, D, F, x.data_ptr(), _rows(x), w_in.data_ptr(), w_out.data_ptr(), pf.data_ptr(),
            h.data_ptr(), dy.data_ptr(), _rows(dy), dx.data_ptr(), _rows(dx), _DT[dwt], dw_in.data_ptr(), dw_out.data_ptr(),
            _stream())
     return dx, dw_in, dw_out
