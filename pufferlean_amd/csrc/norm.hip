@@ -362,7 +362,9 @@ template <typename T> struct NormCall {
   }
   template <int V, int NCH, int LPR> int backward() const {
     const long rows = 64 * kWaves / LPR;
-    long blocks = (M + rows - 1) / rows;
+    // eight rows to a group before there are more blocks: each block's partial row is written, read and added
+    long blocks = (M + 8 * rows - 1) / (8 * rows);
+    if (blocks < 256) blocks = (M + rows - 1) / rows < 256 ? (M + rows - 1) / rows : 256;
     if (blocks > 1024) blocks = 1024;
     float* part = nullptr;
     if (blocks > 1 && (dw || db)) {

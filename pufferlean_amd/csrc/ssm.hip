@@ -42,7 +42,8 @@ struct Args {
   const float *done, *first, *h0, *win0;
   void* y;
   long y_t, y_b;
-  float *h_out, *keep;
+  float *h_out, *keep, *win_out;
+  int win_here;         // the scan's last chunk writes win_out
   long chunk, chunks;   // steps of a chunk (a multiple of kSteps), their number
   float *hloc, *dsum;   // [chunks] end (then start) states, [chunks][B][C] sums of d (-1: cleared inside)
   unsigned blocks_c, G; // channel blocks of a group, groups
@@ -232,6 +233,27 @@ struct Rows {
   }
 };
 
+// The window after the last step: its K - 1 inputs, zero where an episode started after them.
+template <typename T>
+__device__ __forceinline__ void store_window(const Args& a, float* win, long b, unsigned c) {
+  const long K1 = a.K - 1;
+  float x[kTaps - 1];
+  look_back<T>(x, a, a.T, b, c);
+  bool same = true;  // no episode has started after the input
+#pragma unroll
+  for (int j = kTaps - 2; j >= 0; j--) {
+    const long k = j - (kTaps - 1 - K1), t = a.T - (kTaps - 1) + j;
+    if (k < 0) break;
+    win[(b * K1 + k) * a.C + c] = same ? x[j] : 0.f;
+    same = same && !starts(a, t, b);
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) k_ssm_window(Args a) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i < a.B * a.C) store_window<T>(a, a.win_out, i / a.C, (unsigned)(i % a.C));
+}
+
 // One chunk of one sequence. LOCAL: from a zero state, keeping only the end state and the decay's exponent.
 template <typename T, bool LOCAL, int MOST>
 __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
@@ -355,6 +377,7 @@ __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
     else if (tend == a.T && a.h_out) set_row4(a.h_out + (b * a.C + c) * a.N, 4 * q, a.N, h);
   }
   if (LOCAL) a.dsum[(pl.s * a.B + b) * a.C + c] = cleared ? -1.f : dsum;
+  else if (tend == a.T && a.win_here) store_window<T>(a, a.win_out, b, c);
 }
 
 // A thread's state in the library's layout, [B][Q][C][4].
@@ -366,37 +389,34 @@ __device__ __forceinline__ StateAt state_at(const Args& a, long i) {
   const long c = i / 4 % a.C, q = i / (4 * a.C) % a.Q, b = i / (4 * a.C * a.Q), n = 4 * q + i % 4;
   return {b * a.C + c, c, n, n < a.N};
 }
+// run -> decay run + local over the chunks in order, each chunk's entry replaced by the run before it. A chain of short
+// steps, so the loads of eight of them go ahead of it.
+template <int DIR>
+__device__ __forceinline__ void join(float* loc, long row, const float* dsum, long drow, int chunks, float A2, float run) {
+  for (int s0 = 0; s0 < chunks; s0 += 8) {
+    float l[8], d[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const long s = min(s0 + k, chunks - 1);
+      l[k] = loc[DIR * s * row];
+      d[k] = dsum[DIR * s * drow];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      if (s0 + k >= chunks) break;
+      loc[DIR * (long)(s0 + k) * row] = run;
+      run = d[k] < 0.f ? l[k] : fmaf(ex2(A2 * d[k]), run, l[k]);
+    }
+  }
+}
+
 // Joins the chunks in order: hloc[s] becomes the state before chunk s. One thread per state.
 __global__ void __launch_bounds__(256) k_ssm_join(Args a) {
   const long row = a.B * a.C * 4 * a.Q, i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= row) return;
   const StateAt at = state_at(a, i);
   const float A2 = at.in ? a.A[at.c * a.N + at.n] * kLog2e : 0.f;
-  float run = at.in && a.h0 ? a.h0[at.bc * a.N + at.n] : 0.f;
-  for (long s = 0; s < a.chunks; s++) {
-    const float loc = a.hloc[s * row + i], d = a.dsum[s * a.B * a.C + at.bc];
-    a.hloc[s * row + i] = run;
-    run = d < 0.f ? loc : fmaf(ex2(A2 * d), run, loc);
-  }
-}
-
-// The window after the last step: its K - 1 inputs, zero where an episode started after them. A launch of its own, so
-// that it may overwrite the window that the scan read.
-template <typename T>
-__global__ void __launch_bounds__(256) k_ssm_window(Args a, float* win) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.B * a.C) return;
-  const long b = i / a.C, c = i % a.C, K1 = a.K - 1;
-  float x[kTaps - 1];
-  look_back<T>(x, a, a.T, b, (unsigned)c);
-  bool same = true;  // no episode has started after the input
-#pragma unroll
-  for (int j = kTaps - 2; j >= 0; j--) {
-    const long k = j - (kTaps - 1 - K1), t = a.T - (kTaps - 1) + j;
-    if (k < 0) break;
-    win[(b * K1 + k) * a.C + c] = same ? x[j] : 0.f;
-    same = same && !starts(a, t, b);
-  }
+  join<1>(a.hloc + i, row, a.dsum + at.bc, a.B * a.C, (int)a.chunks, A2, at.in && a.h0 ? a.h0[at.bc * a.N + at.n] : 0.f);
 }
 
 // ---- single tokens -------------------------------------------------------------------------------------
@@ -643,12 +663,8 @@ __global__ void __launch_bounds__(256) k_ssm_bwd_join(Args a, GradArgs ga) {
   if (i >= row) return;
   const StateAt at = state_at(a, i);
   const float A2 = at.in ? a.A[at.c * a.N + at.n] * kLog2e : 0.f;
-  float run = 0.f;
-  for (long s = a.chunks - 1; s >= 0; s--) {
-    const float loc = ga.carry[s * row + i], d = a.dsum[s * a.B * a.C + at.bc];
-    ga.carry[s * row + i] = run;
-    run = d < 0.f ? loc : fmaf(ex2(A2 * d), run, loc);
-  }
+  const long last = a.chunks - 1;
+  join<-1>(ga.carry + last * row + i, row, a.dsum + last * a.B * a.C + at.bc, a.B * a.C, (int)a.chunks, A2, 0.f);
 }
 
 // The gradient of one chunk after another. Batches of kSteps steps run backwards in time. Each takes the states four at
@@ -1035,7 +1051,7 @@ int set_chunks(Args& a) {
 }
 
 template <typename T>
-int fwd_t(Args& a, float* win_out, hipStream_t st) {
+int fwd_t(Args& a, hipStream_t st) {
   const int nt = block_threads(a, false);
   const size_t lds = fwd_lds(a.Q, nt);
   a.blocks_c = (unsigned)((a.per + nt - 1) / nt);
@@ -1053,8 +1069,8 @@ int fwd_t(Args& a, float* win_out, hipStream_t st) {
   else if (most <= 4) k_ssm_fwd<T, false, 4><<<blocks, nt, lds, st>>>(a);
   else k_ssm_fwd<T, false, 16><<<blocks, nt, lds, st>>>(a);
   PH_LAUNCH_CHECK();
-  if (win_out && a.K > 1) {
-    k_ssm_window<T><<<ceil_div((size_t)(a.B * a.C), 256), 256, 0, st>>>(a, win_out);
+  if (a.win_out && !a.win_here) {
+    k_ssm_window<T><<<ceil_div((size_t)(a.B * a.C), 256), 256, 0, st>>>(a);
     PH_LAUNCH_CHECK();
   }
   return PH_OK;
@@ -1146,6 +1162,9 @@ extern "C" int ph_ssm_scan(const ph_ssm_args* p, void* y, long y_t, long y_b, fl
   Args a = args_of(*p);
   a.y = y; a.y_t = y_t; a.y_b = y_b; a.h_out = h_out; a.keep = keep;
   PH_TRY(set_chunks(a));
+  a.win_out = a.K > 1 ? win_out : nullptr;
+  // with several chunks the first one may still read the window that the last would overwrite
+  a.win_here = a.win_out && (a.chunks == 1 || a.win_out != a.win0);
   if (a.chunks > 1) {
     const size_t nh = (size_t)a.chunks * a.B * a.C * 4 * a.Q, nd = (size_t)a.chunks * a.B * a.C;
     float* ws = (float*)scratch(kSlotSsm, (nh + nd) * 4);
@@ -1153,7 +1172,7 @@ extern "C" int ph_ssm_scan(const ph_ssm_args* p, void* y, long y_t, long y_b, fl
     a.hloc = ws;
     a.dsum = ws + nh;
   }
-  return p->dtype == PH_BF16 ? fwd_t<uint16_t>(a, win_out, st) : fwd_t<float>(a, win_out, st);
+  return p->dtype == PH_BF16 ? fwd_t<uint16_t>(a, st) : fwd_t<float>(a, st);
 }
 
 extern "C" int ph_ssm_scan_grad(const ph_ssm_args* p, const float* keep, const void* dy, long dy_t, long dy_b,

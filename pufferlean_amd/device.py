@@ -5,6 +5,7 @@ torch only supplies allocation and the current stream; every computation runs in
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -20,7 +21,9 @@ def _p(t):
 
 
 def _stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    """The current stream of the current device. torch's raw form of it: the Stream object that torch.cuda.current_stream()
+    makes costs 2.7 us, half of a small call."""
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
 def _dev(*ts):
@@ -479,24 +482,30 @@ def sample_actions_cont(y, dim, *, rng_state, ls_lo=-20.0, ls_hi=2.0, out=None):
 
 
 # ---- state-space policy layer: normalisation, scan, gated feed-forward ---------------------------------
+# These calls are short enough for the time spent here to show, so what is checked is checked in few steps.
+_ACT_DT = {torch.float32: L.PH_F32, torch.bfloat16: L.PH_BF16}
+_F32 = torch.float32
+
+
 def _act_dtype(x, what):
-    if x.dtype not in (torch.float32, torch.bfloat16):
+    dt = _ACT_DT.get(x.dtype)
+    if dt is None:
         raise TypeError(f"{what} takes float32 or bfloat16, not {x.dtype}")
-    return _DT[x.dtype]
+    return dt
 
 
 def _like(t, x, shape, what):
-    """t has x's dtype, the given shape and a contiguous last dimension."""
-    if t.dtype != x.dtype or t.shape != shape or (t.shape[-1] > 1 and t.stride(-1) != 1):
-        raise ValueError(f"{what} must be {x.dtype} {tuple(shape)} with a contiguous last dimension, "
+    """t has x's dtype, the given shape and a contiguous last dimension, on a GPU."""
+    if t.dtype is not x.dtype or t.shape != shape or not t.is_cuda or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise ValueError(f"{what} must be {x.dtype} {tuple(shape)} on a GPU with a contiguous last dimension, "
                          f"not {t.dtype} {tuple(t.shape)}")
     return t
 
 
 def _f32(t, shape, what):
-    """t (may be None) is a contiguous float32 tensor of the given shape."""
-    if t is not None and (t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous()):
-        raise ValueError(f"{what} must be contiguous float32 {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+    """t is a contiguous float32 tensor of the given shape on a GPU."""
+    if t.dtype is not _F32 or t.shape != shape or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous float32 {tuple(shape)} on a GPU, not {t.dtype} {tuple(t.shape)}")
     return t
 
 
@@ -512,14 +521,17 @@ def _rows(t):
 def layer_norm(x, w=None, b=None, *, eps=1e-5, out=None, mean=None, rstd=None):
     """Layer normalisation of the rows of x [M, C] (float32 or bfloat16, row stride honoured), w and b float32 [C].
     Returns (y, mean, rstd), the statistics float32 [M] for layer_norm_grad."""
-    _dev(x, w, b)
     dt = _act_dtype(x, "layer_norm")
-    M, C_ = x.shape
-    _like(x, x, x.shape, "x")
-    _f32(w, (C_,), "w"), _f32(b, (C_,), "b")
-    y = torch.empty((M, C_), device=x.device, dtype=x.dtype) if out is None else _like(out, x, x.shape, "out")
-    mean = torch.empty(M, device=x.device) if mean is None else _f32(mean, (M,), "mean")
-    rstd = torch.empty(M, device=x.device) if rstd is None else _f32(rstd, (M,), "rstd")
+    shape = x.shape
+    M, C_ = shape
+    _like(x, x, shape, "x")
+    if w is not None:
+        _f32(w, (C_,), "w")
+    if b is not None:
+        _f32(b, (C_,), "b")
+    y = x.new_empty(shape) if out is None else _like(out, x, shape, "out")
+    mean = x.new_empty(M, dtype=_F32) if mean is None else _f32(mean, (M,), "mean")
+    rstd = x.new_empty(M, dtype=_F32) if rstd is None else _f32(rstd, (M,), "rstd")
     L.call("ph_layer_norm", dt, x.data_ptr(), _rows(x), M, C_, _ptr(w), _ptr(b), eps, y.data_ptr(), _rows(y),
            mean.data_ptr(), rstd.data_ptr(), _stream())
     return y, mean, rstd
@@ -527,44 +539,70 @@ def layer_norm(x, w=None, b=None, *, eps=1e-5, out=None, mean=None, rstd=None):
 
 def layer_norm_grad(x, w, mean, rstd, dy, *, dx=None, dw=None, db=None):
     """Gradient of layer_norm from its input and statistics: (dx, dw, db), dw and db float32 [C]."""
-    _dev(x, w, mean, rstd, dy)
     dt = _act_dtype(x, "layer_norm_grad")
-    M, C_ = x.shape
-    _like(x, x, x.shape, "x"), _like(dy, x, x.shape, "dy")
-    _f32(w, (C_,), "w"), _f32(mean, (M,), "mean"), _f32(rstd, (M,), "rstd")
-    dx = torch.empty((M, C_), device=x.device, dtype=x.dtype) if dx is None else _like(dx, x, x.shape, "dx")
-    dw = torch.empty(C_, device=x.device) if dw is None else _f32(dw, (C_,), "dw")
-    db = torch.empty(C_, device=x.device) if db is None else _f32(db, (C_,), "db")
+    shape = x.shape
+    M, C_ = shape
+    _like(x, x, shape, "x"), _like(dy, x, shape, "dy")
+    if w is not None:
+        _f32(w, (C_,), "w")
+    _f32(mean, (M,), "mean"), _f32(rstd, (M,), "rstd")
+    dx = x.new_empty(shape) if dx is None else _like(dx, x, shape, "dx")
+    dw = x.new_empty(C_, dtype=_F32) if dw is None else _f32(dw, (C_,), "dw")
+    db = x.new_empty(C_, dtype=_F32) if db is None else _f32(db, (C_,), "db")
     L.call("ph_layer_norm_grad", dt, x.data_ptr(), _rows(x), dy.data_ptr(), _rows(dy), M, C_, _ptr(w),
            mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), _rows(dx), dw.data_ptr(), db.data_ptr(), _stream())
     return dx, dw, db
 
 
+# ph_ssm_args and ph_ssm_grads as bytes: a third of the time that a ctypes.Structure of as many fields takes
+_SSM_ARGS = struct.Struct("@i6N5P10l9P")
+_SSM_GRADS = struct.Struct("@5P10l5P")
+assert _SSM_ARGS.size == C.sizeof(L.SsmArgs) and _SSM_GRADS.size == C.sizeof(L.SsmGrads)
+
+
 def _ssm_args(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, done, first, h0, win0):
-    """The checked ph_ssm_args of [T, B, C] (or single-step [B, C]) inputs."""
-    _dev(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, done, first, h0, win0)
+    """The checked ph_ssm_args of [T, B, C] (or single-step [B, C]) inputs, and (T, B, C, N, K)."""
     dt = _act_dtype(x, "ssm")
-    lead, C_ = x.shape[:-1], x.shape[-1]
-    T, B = lead if len(lead) == 2 else (1, lead[0])
-    if A.dim() != 2:
-        raise ValueError("A must be [C, N]")
+    shape = x.shape
+    seq = len(shape) == 3
+    if not seq and len(shape) != 2 or A.dim() != 2:
+        raise ValueError("x must be [T, B, C] or [B, C], and A [C, N]")
+    T, B, C_ = shape if seq else (1, *shape)
     N, K = A.shape[1], 0 if conv_w is None else conv_w.shape[-1]
-    _like(x, x, x.shape, "x"), _like(delta, x, x.shape, "delta")
-    bc = torch.Size((*lead, groups * N))
-    _like(Bm, x, bc, "Bm"), _like(Cm, x, bc, "Cm")
+    bc = (T, B, groups * N) if seq else (B, groups * N)
+    _like(x, x, shape, "x"), _like(delta, x, shape, "delta"), _like(Bm, x, bc, "Bm"), _like(Cm, x, bc, "Cm")
     if z is not None:
-        _like(z, x, x.shape, "z")
-    _f32(A, (C_, N), "A"), _f32(D, (C_,), "D"), _f32(dt_bias, (C_,), "dt_bias")
-    _f32(conv_w, (C_, K), "conv_w"), _f32(conv_b, (C_,), "conv_b")
-    _f32(done, (T, B), "done"), _f32(first, (B,), "first"), _f32(h0, (B, C_, N), "h0")
+        _like(z, x, shape, "z")
+    _f32(A, (C_, N), "A")
+    c = (C_,)
+    if D is not None:
+        _f32(D, c, "D")
+    if dt_bias is not None:
+        _f32(dt_bias, c, "dt_bias")
+    if conv_w is not None:
+        _f32(conv_w, (C_, K), "conv_w")
+    if conv_b is not None:
+        _f32(conv_b, c, "conv_b")
+    if done is not None:
+        _f32(done, (T, B), "done")
+    if first is not None:
+        _f32(first, (B,), "first")
+    if h0 is not None:
+        _f32(h0, (B, C_, N), "h0")
     if K < 2:
         win0 = None
-    _f32(win0, (B, K - 1, C_), "win0")
-    strides = []
-    for t in (x, z, delta, Bm, Cm):
-        strides += (0, 0) if t is None else t.stride()[:2] if len(lead) == 2 else (0, t.stride(0))
-    return L.SsmArgs(dt, T, B, C_, N, groups, K, _ptr(x), _ptr(z), _ptr(delta), _ptr(Bm), _ptr(Cm), *strides, _ptr(A),
-                     _ptr(D), _ptr(dt_bias), _ptr(conv_w), _ptr(conv_b), _ptr(done), _ptr(first), _ptr(h0), _ptr(win0))
+    elif win0 is not None:
+        _f32(win0, (B, K - 1, C_), "win0")
+    xs, ds, bs, cs = x.stride(), delta.stride(), Bm.stride(), Cm.stride()
+    zs = (0, 0) if z is None else z.stride()
+    if seq:
+        st = (xs[0], xs[1], zs[0], zs[1], ds[0], ds[1], bs[0], bs[1], cs[0], cs[1])
+    else:
+        st = (0, xs[0], 0, zs[0], 0, ds[0], 0, bs[0], 0, cs[0])
+    a = _SSM_ARGS.pack(dt, T, B, C_, N, groups, K, x.data_ptr(), _ptr(z), delta.data_ptr(), Bm.data_ptr(), Cm.data_ptr(), *st,
+                       A.data_ptr(), _ptr(D), _ptr(dt_bias), _ptr(conv_w), _ptr(conv_b), _ptr(done), _ptr(first), _ptr(h0),
+                       _ptr(win0))
+    return a, T, B, C_, N, K
 
 
 def ssm_scan(x, delta, A, Bm, Cm, *, D=None, z=None, dt_bias=None, conv_w=None, conv_b=None, groups=1, done=None,
@@ -574,15 +612,16 @@ def ssm_scan(x, delta, A, Bm, Cm, *, D=None, z=None, dt_bias=None, conv_w=None, 
     A [C, N], D, dt_bias, conv_b [C], conv_w [C, K], done [T, B], first [B], h0 [B, C, N], win0 [B, K-1, C] float32.
     h_out and win_out receive the carried state (they may be h0 and win0). Returns y, or (y, saved) with save=True, saved
     being what ssm_scan_grad needs."""
-    a = _ssm_args(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, done, first, h0, win0)
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype) if out is None else _like(out, x, x.shape, "out")
-    _f32(h_out, (a.B, a.C, a.N), "h_out")
-    if a.K < 2:
+    a, T, B, C_, N, K = _ssm_args(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, done, first, h0, win0)
+    y = x.new_empty(x.shape) if out is None else _like(out, x, x.shape, "out")
+    if h_out is not None:
+        _f32(h_out, (B, C_, N), "h_out")
+    if K < 2:
         win_out = None
-    _f32(win_out, (a.B, a.K - 1, a.C), "win_out")
-    ref = C.byref(a)
-    keep = torch.empty(L.lib().ph_ssm_keep_floats(ref), device=x.device) if save else None
-    L.call("ph_ssm_scan", ref, y.data_ptr(), y.stride(0), y.stride(1), _ptr(h_out), _ptr(win_out), _ptr(keep), _stream())
+    elif win_out is not None:
+        _f32(win_out, (B, K - 1, C_), "win_out")
+    keep = x.new_empty(L.lib().ph_ssm_keep_floats(a), dtype=_F32) if save else None
+    L.call("ph_ssm_scan", a, y.data_ptr(), y.stride(0), y.stride(1), _ptr(h_out), _ptr(win_out), _ptr(keep), _stream())
     return (y, keep) if save else y
 
 
@@ -591,23 +630,27 @@ def ssm_scan_grad(x, delta, A, Bm, Cm, saved, dy, *, D=None, z=None, dt_bias=Non
     """Gradient of ssm_scan from its arguments and what it saved. Returns a dict: dx, ddelta, dBm, dCm (and dz) in the
     activations' dtype, written into the given tensors where there are any, and dA (and dD, ddt_bias, dconv_w, dconv_b)
     in float32. The carried-in state and window are constants."""
-    a = _ssm_args(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, done, first, None, win0)
+    a, T, B, C_, N, K = _ssm_args(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, done, first, None, win0)
     _like(dy, x, x.shape, "dy")
-    ref = C.byref(a)
-    _f32(saved, (L.lib().ph_ssm_keep_floats(ref),), "saved")
-    g = {}
+    _f32(saved, (L.lib().ph_ssm_keep_floats(a),), "saved")
+    g, ptrs, strides = {}, [], []
     for name, t, like in (("dx", dx, x), ("dz", dz, z), ("ddelta", ddelta, delta), ("dBm", dBm, Bm), ("dCm", dCm, Cm)):
-        if like is not None:
-            g[name] = torch.empty(like.shape, device=x.device, dtype=x.dtype) if t is None else _like(t, x, like.shape, name)
-    strides = []
-    for name in ("dx", "dz", "ddelta", "dBm", "dCm"):
-        strides += g[name].stride()[:2] if name in g else (0, 0)
+        if like is None:
+            ptrs.append(0)
+            strides += (0, 0)
+            continue
+        g[name] = t = x.new_empty(like.shape) if t is None else _like(t, x, like.shape, name)
+        ptrs.append(t.data_ptr())
+        strides += t.stride()[:2]
+    outs = []
     for name, p in (("dA", A), ("dD", D), ("ddt_bias", dt_bias), ("dconv_w", conv_w), ("dconv_b", conv_b)):
-        if p is not None:
-            g[name] = torch.empty_like(p)
-    c = L.SsmGrads(*(_ptr(g.get(n)) for n in ("dx", "dz", "ddelta", "dBm", "dCm")), *strides,
-                   *(_ptr(g.get(n)) for n in ("dA", "dD", "ddt_bias", "dconv_w", "dconv_b")))
-    L.call("ph_ssm_scan_grad", ref, saved.data_ptr(), dy.data_ptr(), dy.stride(0), dy.stride(1), C.byref(c), _stream())
+        if p is None:
+            outs.append(0)
+        else:
+            g[name] = p = torch.empty_like(p)
+            outs.append(p.data_ptr())
+    L.call("ph_ssm_scan_grad", a, saved.data_ptr(), dy.data_ptr(), dy.stride(0), dy.stride(1),
+           _SSM_GRADS.pack(*ptrs, *strides, *outs), _stream())
     return g
 
 
@@ -615,11 +658,11 @@ def ssm_step(x, delta, A, Bm, Cm, h, win=None, *, D=None, z=None, dt_bias=None, 
              first=None, out=None):
     """One step of ssm_scan for B sequences: x, delta, z [B, C], Bm, Cm [B, groups*N]; the state h [B, C, N] and the
     convolution's window win [B, K-1, C] (float32) are updated in place, cleared first where first[b] is set."""
-    a = _ssm_args(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, None, first, h, win)
-    if a.K > 1 and win is None:
+    a, _, _, _, _, K = _ssm_args(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, None, first, h, win)
+    if K > 1 and win is None:
         raise ValueError("win is needed for a convolution of two taps or more")
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype) if out is None else _like(out, x, x.shape, "out")
-    L.call("ph_ssm_step", C.byref(a), y.data_ptr(), y.stride(0), h.data_ptr(), _ptr(win) if a.K > 1 else 0, _stream())
+    y = x.new_empty(x.shape) if out is None else _like(out, x, x.shape, "out")
+    L.call("ph_ssm_step", a, y.data_ptr(), y.stride(0), h.data_ptr(), win.data_ptr() if K > 1 else 0, _stream())
     return y
 
 
@@ -627,7 +670,6 @@ _ACT = {"silu": L.PH_ACT_SILU, "gelu": L.PH_ACT_GELU}
 
 
 def _ffn_shapes(x, w_in, w_out, act):
-    _dev(x, w_in, w_out)
     dt = _act_dtype(x, "gated_ffn")
     if act not in _ACT:
         raise ValueError(f"gated_ffn: activation {act!r} is not one of {sorted(_ACT)}")
@@ -648,11 +690,10 @@ def gated_ffn(x, w_in, w_out, *, act="silu", out=None, save=False):
     j at 2j and 2j + 1, w_out [D, F], float32 or bfloat16. Returns y, or (y, saved) with save=True, saved being what
     gated_ffn_grad needs."""
     dt, M, D, F = _ffn_shapes(x, w_in, w_out, act)
-    y = torch.empty((M, D), device=x.device, dtype=x.dtype) if out is None else _like(out, x, x.shape, "out")
+    y = x.new_empty((M, D)) if out is None else _like(out, x, x.shape, "out")
     pf = h = None
     if save:
-        pf = torch.empty((M, 2 * _pitch(F)), device=x.device, dtype=x.dtype)
-        h = torch.empty((M, _pitch(F)), device=x.device, dtype=x.dtype)
+        pf, h = x.new_empty((M, 2 * _pitch(F))), x.new_empty((M, _pitch(F)))
     L.call("ph_ffn", dt, _ACT[act], M, D, F, x.data_ptr(), _rows(x), w_in.data_ptr(), w_out.data_ptr(), _ptr(pf), _ptr(h),
            y.data_ptr(), _rows(y), _stream())
     return (y, (pf, h)) if save else y
@@ -663,14 +704,16 @@ def gated_ffn_grad(x, w_in, w_out, saved, dy, *, act="silu", dx=None, dw_in=None
     dt, M, D, F = _ffn_shapes(x, w_in, w_out, act)
     _like(dy, x, x.shape, "dy")
     pf, h = saved
-    _like(pf, x, (M, 2 * _pitch(F)), "saved"), _like(h, x, (M, _pitch(F)), "saved")
+    for t, cols in ((pf, 2 * _pitch(F)), (h, _pitch(F))):
+        if not _like(t, x, (M, cols), "saved").is_contiguous():
+            raise ValueError("saved must be as gated_ffn returned it")
     dwt = dw_dtype or (x.dtype if dw_in is None else dw_in.dtype)
-    dx = torch.empty((M, D), device=x.device, dtype=x.dtype) if dx is None else _like(dx, x, x.shape, "dx")
-    dw_in = torch.empty((2 * F, D), device=x.device, dtype=dwt) if dw_in is None else dw_in
-    dw_out = torch.empty((D, F), device=x.device, dtype=dwt) if dw_out is None else dw_out
+    dx = x.new_empty((M, D)) if dx is None else _like(dx, x, x.shape, "dx")
+    dw_in = x.new_empty((2 * F, D), dtype=dwt) if dw_in is None else dw_in
+    dw_out = x.new_empty((D, F), dtype=dwt) if dw_out is None else dw_out
     for t, shape, what in ((dw_in, (2 * F, D), "dw_in"), (dw_out, (D, F), "dw_out")):
-        if t.dtype != dwt or t.shape != shape or not t.is_contiguous():
-            raise ValueError(f"{what} must be contiguous {dwt} {shape}")
+        if t.dtype is not dwt or t.shape != shape or not t.is_cuda or not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous {dwt} {shape} on a GPU")
     L.call("ph_ffn_grad", dt, _ACT[act], M, D, F, x.data_ptr(), _rows(x), w_in.data_ptr(), w_out.data_ptr(), pf.data_ptr(),
            h.data_ptr(), dy.data_ptr(), _rows(dy), dx.data_ptr(), _rows(dx), _DT[dwt], dw_in.data_ptr(), dw_out.data_ptr(),
            _stream())
