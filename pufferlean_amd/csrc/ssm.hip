@@ -33,9 +33,18 @@ constexpr int kTaps = 4;   // most taps of the convolution; fewer are padded wit
 constexpr int kMaxStates = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Global pointers as such: the compiler loses track of a pointer that an asm has touched (walk, below) and would access it
+// as one that may also point to LDS.
+#define PH_GLOBAL __attribute__((address_space(1)))
+template <typename T> using gin = const PH_GLOBAL T*;
+template <typename T> using gout = PH_GLOBAL T*;
+typedef float f4t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f4t f4(float x, float y, float z, float w) { return f4t{x, y, z, w}; }
+
 struct Args {
-  long T, B, C, N, per, K;  // per: channels of a group
-  int Q;                    // states in fours, N rounded up
+  int T, C, N, per, K;  // per: channels of a group
+  int Q;                // states in fours, N rounded up
+  long B;
   const void *x, *z, *delta, *Bm, *Cm;
   long x_t, x_b, z_t, z_b, d_t, d_b, bm_t, bm_b, cm_t, cm_b;
   const float *A, *D, *dt_bias, *conv_w, *conv_b;
@@ -44,17 +53,19 @@ struct Args {
   long y_t, y_b;
   float *h_out, *keep, *win_out;
   int win_here;         // the scan's last chunk writes win_out
-  long chunk, chunks;   // steps of a chunk (a multiple of kSteps), their number
+  int chunk, chunks;    // steps of a chunk (a multiple of kSteps), their number
   float *hloc, *dsum;   // [chunks] end (then start) states, [chunks][B][C] sums of d (-1: cleared inside)
   unsigned blocks_c, G; // channel blocks of a group, groups
 };
 // The library's own states are [..][B][Q][C][4]: a wavefront moves four states of 64 channels as 1 KB. The caller's are
 // [B][C][N].
 
-__device__ __forceinline__ float ldf(const uint16_t* p) { return bf16_to_f32(*p); }
-__device__ __forceinline__ float ldf(const float* p) { return *p; }
-__device__ __forceinline__ void stf(uint16_t* p, float v) { *p = bf16_rne(v); }
-__device__ __forceinline__ void stf(float* p, float v) { *p = v; }
+__device__ __forceinline__ float ldf(gin<uint16_t> p) { return bf16_to_f32(*p); }
+__device__ __forceinline__ float ldf(gin<float> p) { return *p; }
+__device__ __forceinline__ float ldf(const uint16_t* p) { return ldf((gin<uint16_t>)p); }
+__device__ __forceinline__ float ldf(const float* p) { return ldf((gin<float>)p); }
+__device__ __forceinline__ void stf(gout<uint16_t> p, float v) { *p = bf16_rne(v); }
+__device__ __forceinline__ void stf(gout<float> p, float v) { *p = v; }
 
 __device__ __forceinline__ float ex2(float v) { return __builtin_amdgcn_exp2f(v); }
 // softplus without cancellation: with w = 1 + e rounded, log(w) e / (w - 1) is log(1 + e) to a few ulp for every e.
@@ -68,18 +79,17 @@ __device__ __forceinline__ float silu(float v) { return v * sigm(v); }
 __device__ __forceinline__ float dsilu(float v, float s) { return s * fmaf(v, 1.f - s, 1.f); }
 
 // Whether step t of sequence b starts an episode.
-__device__ __forceinline__ bool starts(const Args& a, long t, long b) {
-  if (t > 0) return a.done && a.done[(t - 1) * a.B + b] != 0.f;
+__device__ __forceinline__ bool starts(const Args& a, int t, long b) {
+  if (t > 0) return a.done && a.done[(long)(t - 1) * a.B + b] != 0.f;
   return t == 0 && a.first && a.first[b] != 0.f;
 }
 // Bit j of flag_bits(flag_load(..)): step t0 - 3 + j starts an episode (j < 11: a batch and the three steps that its
 // convolutions look back to). One load per lane, one ballot, apart so that the load can be issued a batch ahead.
-__device__ __forceinline__ float flag_load(const Args& a, long t0, long tend, long b) {
-  const int j = threadIdx.x & 63;
-  const long t = t0 - (kTaps - 1) + j;
+__device__ __forceinline__ float flag_load(const Args& a, int t0, int tend, long b) {
+  const int j = threadIdx.x & 63, t = t0 - (kTaps - 1) + j;
   float f = 0.f;
   if (j < kSteps + kTaps - 1 && t < tend && t >= 0) {
-    if (t > 0) f = a.done ? a.done[(t - 1) * a.B + b] : 0.f;
+    if (t > 0) f = a.done ? a.done[(long)(t - 1) * a.B + b] : 0.f;
     else f = a.first ? a.first[b] : 0.f;
   }
   return f;
@@ -92,7 +102,7 @@ struct Conv {
   float w[kTaps], bias;
   int K;
   __device__ __forceinline__ void init(const Args& a, unsigned c) {
-    K = (int)a.K;
+    K = a.K;
 #pragma unroll
     for (int i = 0; i < kTaps; i++) {
       const int k = i - (kTaps - K);
@@ -115,12 +125,12 @@ struct Conv {
 
 // The three inputs before step t0 as bits of T (of the sequence, or as fp32 values of the carried window).
 template <typename T>
-__device__ __forceinline__ void look_back(float (&x)[kTaps - 1], const Args& a, long t0, long b, unsigned c) {
-  const T* p = (const T*)a.x + b * a.x_b;
-  const int K1 = (int)a.K - 1;
+__device__ __forceinline__ void look_back(float (&x)[kTaps - 1], const Args& a, int t0, long b, unsigned c) {
+  const gin<T> p = (gin<T>)a.x + b * a.x_b;
+  const int K1 = a.K - 1;
 #pragma unroll
   for (int j = 0; j < kTaps - 1; j++) {
-    const long t = t0 - (kTaps - 1) + j;
+    const int t = t0 - (kTaps - 1) + j;
     x[j] = 0.f;
     if (t >= 0) x[j] = ldf(p + t * a.x_t + c);
     else if (K1 + t >= 0 && a.win0) x[j] = a.win0[(b * K1 + K1 + t) * a.C + c];
@@ -130,7 +140,7 @@ __device__ __forceinline__ void look_back(float (&x)[kTaps - 1], const Args& a, 
 // A uniform row pointer that walks over steps. The empty asm keeps the walk a chain of scalar additions: without it the
 // compiler forms the addresses of all of a batch's rows at once, hundreds of scalar registers that it then spills.
 template <typename P>
-__device__ __forceinline__ void walk(P*& p, long d) {
+__device__ __forceinline__ void walk(P& p, long d) {
   p += d;
   asm("" : "+s"(p));
 }
@@ -166,7 +176,7 @@ __device__ __forceinline__ int place_state(int e) { return 4 * (e >> 6) + (e & 3
 static_assert(kSteps == 8, "places of the staged values");
 template <typename T, int kMost>
 struct StageBC {
-  const T* p[kMost];   // of step 0
+  gin<T> p[kMost];     // of step 0
   long stride[kMost];
   int step[kMost];     // of the batch; past it for no value
   float v[kMost];
@@ -175,15 +185,15 @@ struct StageBC {
     for (int k = 0; k < kMost; k++) {
       const int e = threadIdx.x + k * blockDim.x, n = place_state(e);
       const bool is_c = place_row(e);
-      p[k] = is_c ? (const T*)a.Cm + b * a.cm_b : (const T*)a.Bm + b * a.bm_b;
+      p[k] = is_c ? (gin<T>)a.Cm + b * a.cm_b : (gin<T>)a.Bm + b * a.bm_b;
       p[k] += g * a.N + n;
       stride[k] = is_c ? a.cm_t : a.bm_t;
       step[k] = n < a.N ? place_step(e) : kSteps;
     }
   }
-  __device__ __forceinline__ void get(long t0, int steps) {
+  __device__ __forceinline__ void get(int t0, int steps) {
 #pragma unroll
-    for (int k = 0; k < kMost; k++) v[k] = step[k] < steps ? ldf(p[k] + (t0 + step[k]) * stride[k]) : 0.f;
+    for (int k = 0; k < kMost; k++) v[k] = step[k] < steps ? ldf(p[k] + (long)(t0 + step[k]) * stride[k]) : 0.f;
   }
   __device__ __forceinline__ void put(const Args& a, float* s) const {
     const int tot = kSteps * 8 * a.Q;
@@ -196,26 +206,26 @@ struct StageBC {
 };
 
 // States n0.. n0 + 3 of a row of N, zero past N.
-__device__ __forceinline__ float4 row4(const float* p, int n0, long N) {
-  return make_float4(p[n0], n0 + 1 < N ? p[n0 + 1] : 0.f, n0 + 2 < N ? p[n0 + 2] : 0.f, n0 + 3 < N ? p[n0 + 3] : 0.f);
+__device__ __forceinline__ f4t row4(const float* p, int n0, int N) {
+  return f4(p[n0], n0 + 1 < N ? p[n0 + 1] : 0.f, n0 + 2 < N ? p[n0 + 2] : 0.f, n0 + 3 < N ? p[n0 + 3] : 0.f);
 }
-__device__ __forceinline__ void set_row4(float* p, int n0, long N, const float4& v) {
+__device__ __forceinline__ void set_row4(float* p, int n0, int N, const f4t& v) {
   p[n0] = v.x;
   if (n0 + 1 < N) p[n0 + 1] = v.y;
   if (n0 + 2 < N) p[n0 + 2] = v.z;
   if (n0 + 3 < N) p[n0 + 3] = v.w;
 }
 // A in units of the base-2 exponential.
-__device__ __forceinline__ float4 decay4(const Args& a, unsigned c, int q) {
-  const float4 v = row4(a.A + (long)c * a.N, 4 * q, a.N);
-  return make_float4(v.x * kLog2e, v.y * kLog2e, v.z * kLog2e, v.w * kLog2e);
+__device__ __forceinline__ f4t decay4(const Args& a, unsigned c, int q) {
+  const f4t v = row4(a.A + (long)c * a.N, 4 * q, a.N);
+  return f4(v.x * kLog2e, v.y * kLog2e, v.z * kLog2e, v.w * kLog2e);
 }
 
 // Raw rows of a batch, loaded a batch ahead; steps past the end repeat the last one.
 template <typename T>
 struct Rows {
   uint32_t v[kSteps];  // the bits: a bf16 value's, or an fp32's
-  __device__ __forceinline__ void get(const T* p, long stride, int steps, unsigned c) {
+  __device__ __forceinline__ void get(gin<T> p, long stride, int steps, unsigned c) {
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
       if constexpr (sizeof(T) == 2) v[i] = p[c];
@@ -259,25 +269,25 @@ template <typename T, bool LOCAL, int MOST>
 __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int Q = a.Q, nt = blockDim.x, tid = threadIdx.x;
-  float4* sA = reinterpret_cast<float4*>(lds);  // [Q][nt]
-  float4* sH = sA + Q * nt;                     // [Q][nt]
+  f4t* sA = reinterpret_cast<f4t*>(lds);  // [Q][nt]
+  f4t* sH = sA + Q * nt;                     // [Q][nt]
   float* sbc = lds + 8 * Q * nt;                // [2][Q][kSteps][2][4]
   const Place pl = place(a, blockIdx.x);
   const long b = pl.b;
   const unsigned c = pl.c;
-  const long tbeg = pl.s * a.chunk, tend = min(a.T, tbeg + a.chunk);
-  const T* xp = (const T*)a.x + b * a.x_b + tbeg * a.x_t;
-  const T* dp = (const T*)a.delta + b * a.d_b + tbeg * a.d_t;
-  const T* zp = (const T*)a.z + (a.z ? b * a.z_b + tbeg * a.z_t : 0);
-  T* yp = (T*)a.y + b * a.y_b + tbeg * a.y_t;
+  const int tbeg = (int)pl.s * a.chunk, tend = min(a.T, tbeg + a.chunk);
+  gin<T> xp = (gin<T>)a.x + b * a.x_b + tbeg * a.x_t;
+  gin<T> dp = (gin<T>)a.delta + b * a.d_b + tbeg * a.d_t;
+  gin<T> zp = (gin<T>)a.z + (a.z ? b * a.z_b + tbeg * a.z_t : 0);
+  gout<T> yp = (gout<T>)a.y + b * a.y_b + tbeg * a.y_t;
   const long quads = a.B * Q * a.C;  // quads of the library's states of one chunk (or kept batch)
-  float4* keep = LOCAL || !a.keep ? nullptr : reinterpret_cast<float4*>(a.keep) + tbeg / kSteps * quads + b * Q * a.C;
+  gout<f4t> keep = LOCAL || !a.keep ? nullptr : (gout<f4t>)a.keep + tbeg / kSteps * quads + b * Q * a.C;
   Rows<T> rx, rd, rz;
   StageBC<T, MOST> bc;
   bc.init(a, b, pl.g);
   float fl, back[kTaps - 1];
-  auto fetch = [&](long t0) __attribute__((always_inline)) {
-    const int n = (int)min((long)kSteps, tend - t0);
+  auto fetch = [&](int t0) __attribute__((always_inline)) {
+    const int n = min(kSteps, tend - t0);
     bc.get(t0, n);
     rx.get(xp, a.x_t, n, c);
     rd.get(dp, a.d_t, n, c);
@@ -294,9 +304,9 @@ __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
   const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, Dc = a.D ? a.D[c] : 0.f;
   for (int q = 0; q < Q; q++) {
     sA[q * nt + tid] = decay4(a, c, q);
-    float4 h = make_float4(0.f, 0.f, 0.f, 0.f);
+    f4t h = f4(0.f, 0.f, 0.f, 0.f);
     if (!LOCAL) {
-      if (a.chunks > 1) h = reinterpret_cast<const float4*>(a.hloc)[pl.s * quads + (b * Q + q) * a.C + c];
+      if (a.chunks > 1) h = reinterpret_cast<const f4t*>(a.hloc)[pl.s * quads + (b * Q + q) * a.C + c];
       else if (a.h0) h = row4(a.h0 + (b * a.C + c) * a.N, 4 * q, a.N);
     }
     sH[q * nt + tid] = h;
@@ -304,14 +314,14 @@ __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
   float dsum = 0.f;
   unsigned cleared = 0;
   int buf = 0;
-  for (long t0 = tbeg; t0 < tend; t0 += kSteps, buf ^= 1) {
+  for (int t0 = tbeg; t0 < tend; t0 += kSteps, buf ^= 1) {
     // two buffers and one barrier: a wavefront writes this one again only after every wavefront has passed the
     // barrier of the batch between, and so has read it
     float* s = sbc + buf * 64 * Q;
     bc.put(a, s);
     const Rows<T> cx = rx, cd = rd, cz = rz;
     const unsigned bits = flag_bits(fl), st = bits >> (kTaps - 1);
-    const int steps = (int)min((long)kSteps, tend - t0);
+    const int steps = min(kSteps, tend - t0);
     __syncthreads();
     if (t0 + kSteps < tend) fetch(t0 + kSteps);
     cleared |= st;
@@ -336,22 +346,22 @@ __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
     for (int j = 0; j < kTaps - 1; j++) back[j] = cx[kSteps - (kTaps - 1) + j];
     auto scan = [&](auto ANY) __attribute__((always_inline)) {  // ANY: an episode starts in this batch
       for (int q = 0; q < Q; q++) {
-        const float4 A = sA[q * nt + tid];
-        float4 h = sH[q * nt + tid];
+        const f4t A = sA[q * nt + tid];
+        f4t h = sH[q * nt + tid];
         if (!LOCAL && keep && pl.in) (keep + q * a.C)[c] = h;
 #pragma unroll
         for (int i = 0; i < kSteps; i++) {
           if constexpr (decltype(ANY)::value) {
             const bool cut = st & (1u << i);
-            h = make_float4(cut ? 0.f : h.x, cut ? 0.f : h.y, cut ? 0.f : h.z, cut ? 0.f : h.w);
+            h = f4(cut ? 0.f : h.x, cut ? 0.f : h.y, cut ? 0.f : h.z, cut ? 0.f : h.w);
           }
-          const float4 Bv = *reinterpret_cast<const float4*>(&s[64 * q + 8 * i]);
+          const f4t Bv = *reinterpret_cast<const f4t*>(&s[64 * q + 8 * i]);
           h.x = fmaf(ex2(d[i] * A.x), h.x, du[i] * Bv.x);
           h.y = fmaf(ex2(d[i] * A.y), h.y, du[i] * Bv.y);
           h.z = fmaf(ex2(d[i] * A.z), h.z, du[i] * Bv.z);
           h.w = fmaf(ex2(d[i] * A.w), h.w, du[i] * Bv.w);
           if (!LOCAL) {
-            const float4 Cv = *reinterpret_cast<const float4*>(&s[64 * q + 8 * i + 4]);
+            const f4t Cv = *reinterpret_cast<const f4t*>(&s[64 * q + 8 * i + 4]);
             o[i] = fmaf(h.x, Cv.x, fmaf(h.y, Cv.y, fmaf(h.z, Cv.z, fmaf(h.w, Cv.w, o[i]))));
           }
           if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // bounds the values of later steps that are fetched early
@@ -372,8 +382,8 @@ __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
   }
   if (!pl.in) return;
   for (int q = 0; q < Q; q++) {
-    const float4 h = sH[q * nt + tid];
-    if (LOCAL) reinterpret_cast<float4*>(a.hloc)[pl.s * quads + (b * Q + q) * a.C + c] = h;
+    const f4t h = sH[q * nt + tid];
+    if (LOCAL) reinterpret_cast<f4t*>(a.hloc)[pl.s * quads + (b * Q + q) * a.C + c] = h;
     else if (tend == a.T && a.h_out) set_row4(a.h_out + (b * a.C + c) * a.N, 4 * q, a.N, h);
   }
   if (LOCAL) a.dsum[(pl.s * a.B + b) * a.C + c] = cleared ? -1.f : dsum;
@@ -416,15 +426,15 @@ __global__ void __launch_bounds__(256) k_ssm_join(Args a) {
   if (i >= row) return;
   const StateAt at = state_at(a, i);
   const float A2 = at.in ? a.A[at.c * a.N + at.n] * kLog2e : 0.f;
-  join<1>(a.hloc + i, row, a.dsum + at.bc, a.B * a.C, (int)a.chunks, A2, at.in && a.h0 ? a.h0[at.bc * a.N + at.n] : 0.f);
+  join<1>(a.hloc + i, row, a.dsum + at.bc, a.B * a.C, a.chunks, A2, at.in && a.h0 ? a.h0[at.bc * a.N + at.n] : 0.f);
 }
 
 // ---- single tokens -------------------------------------------------------------------------------------
 // Four consecutive elements of a row of B or C.
-__device__ __forceinline__ float4 quad_of(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 quad_of(const uint16_t* p) {
+__device__ __forceinline__ f4t quad_of(const float* p) { return *reinterpret_cast<const f4t*>(p); }
+__device__ __forceinline__ f4t quad_of(const uint16_t* p) {
   const uint2 v = *reinterpret_cast<const uint2*>(p);
-  return make_float4(__builtin_bit_cast(float, v.x << 16), __builtin_bit_cast(float, v.x & 0xffff0000u),
+  return f4(__builtin_bit_cast(float, v.x << 16), __builtin_bit_cast(float, v.x & 0xffff0000u),
                      __builtin_bit_cast(float, v.y << 16), __builtin_bit_cast(float, v.y & 0xffff0000u));
 }
 
@@ -436,7 +446,7 @@ __device__ __forceinline__ float4 quad_of(const uint16_t* p) {
 template <typename T, int QT>
 __global__ void __launch_bounds__(256) k_ssm_step(Args a, float* __restrict__ hs, float* __restrict__ win, int per_block) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
-  const int nt = blockDim.x, tid = threadIdx.x, Q = QT ? QT : a.Q, N = (int)a.N;
+  const int nt = blockDim.x, tid = threadIdx.x, Q = QT ? QT : a.Q, N = a.N;
   float* sd = lds;           // [nt] d
   float* sdu = lds + nt;     // [nt] d u
   float* so = lds + 2 * nt;  // [nt][Q] shares of <h, C>
@@ -445,11 +455,11 @@ __global__ void __launch_bounds__(256) k_ssm_step(Args a, float* __restrict__ hs
   const long c0 = (long)cb * nt;
   const bool in = c0 + tid < a.C;
   const unsigned c = (unsigned)(in ? c0 + tid : a.C - 1);
-  const int K = (int)a.K, chans = (int)min((long)nt, a.C - c0);
+  const int K = a.K, chans = (int)min((long)nt, a.C - c0);
   Conv cv;
   cv.init(a, c);
   const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, Dc = a.D ? a.D[c] : 0.f;
-  float4 Av[QT ? QT : 1];
+  f4t Av[QT ? QT : 1];
   int lcs[QT ? QT : 1], goff[QT ? QT : 1];
   if constexpr (QT > 0) {
 #pragma unroll
@@ -458,8 +468,8 @@ __global__ void __launch_bounds__(256) k_ssm_step(Args a, float* __restrict__ hs
       lcs[j] = lc;
       const long ch = c0 + (lc < chans ? lc : 0);
       goff[j] = (int)(ch / a.per) * N + 4 * (idx % QT);
-      const float4 v = lc < chans ? *reinterpret_cast<const float4*>(a.A + c0 * N + 4 * idx) : make_float4(0.f, 0.f, 0.f, 0.f);
-      Av[j] = make_float4(v.x * kLog2e, v.y * kLog2e, v.z * kLog2e, v.w * kLog2e);
+      const f4t v = lc < chans ? *reinterpret_cast<const f4t*>(a.A + c0 * N + 4 * idx) : f4(0.f, 0.f, 0.f, 0.f);
+      Av[j] = f4(v.x * kLog2e, v.y * kLog2e, v.z * kLog2e, v.w * kLog2e);
     }
   }
   for (long b = b0; b < b1; b++) {
@@ -467,13 +477,13 @@ __global__ void __launch_bounds__(256) k_ssm_step(Args a, float* __restrict__ hs
     float* hb = hs + (b * a.C + c0) * N;
     const T* Bp = (const T*)a.Bm + b * a.bm_b;
     const T* Cp = (const T*)a.Cm + b * a.cm_b;
-    float4 hv[QT ? QT : 1];
+    f4t hv[QT ? QT : 1];
     if constexpr (QT > 0) {  // the state's loads first
 #pragma unroll
       for (int j = 0; j < QT; j++)
-        hv[j] = lcs[j] < chans && !clear ? *reinterpret_cast<const float4*>(hb + 4 * (j * nt + tid)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        hv[j] = lcs[j] < chans && !clear ? *reinterpret_cast<const f4t*>(hb + 4 * (j * nt + tid)) : f4(0.f, 0.f, 0.f, 0.f);
     }
-    const float x = ldf((const T*)a.x + b * a.x_b + c);
+    const float x = ldf((gin<T>)a.x + b * a.x_b + c);
     float u = x;
     if (K) {
       float* wp = win + b * (K - 1) * a.C;
@@ -486,7 +496,7 @@ __global__ void __launch_bounds__(256) k_ssm_step(Args a, float* __restrict__ hs
         if (K > 3) wp[c] = x2;
       }
     }
-    const float d = softplus(ldf((const T*)a.delta + b * a.d_b + c) + bias);
+    const float d = softplus(ldf((gin<T>)a.delta + b * a.d_b + c) + bias);
     sd[tid] = d;
     sdu[tid] = d * u;
     __syncthreads();
@@ -495,13 +505,13 @@ __global__ void __launch_bounds__(256) k_ssm_step(Args a, float* __restrict__ hs
       for (int j = 0; j < QT; j++) {
         if (lcs[j] >= chans) continue;
         const float dd = sd[lcs[j]], du = sdu[lcs[j]];
-        const float4 Bv = quad_of(Bp + goff[j]), Cv = quad_of(Cp + goff[j]), A = Av[j];
-        float4 h = hv[j];
+        const f4t Bv = quad_of(Bp + goff[j]), Cv = quad_of(Cp + goff[j]), A = Av[j];
+        f4t h = hv[j];
         h.x = fmaf(ex2(dd * A.x), h.x, du * Bv.x);
         h.y = fmaf(ex2(dd * A.y), h.y, du * Bv.y);
         h.z = fmaf(ex2(dd * A.z), h.z, du * Bv.z);
         h.w = fmaf(ex2(dd * A.w), h.w, du * Bv.w);
-        *reinterpret_cast<float4*>(hb + 4 * (j * nt + tid)) = h;
+        *reinterpret_cast<f4t*>(hb + 4 * (j * nt + tid)) = h;
         so[j * nt + tid] = fmaf(h.x, Cv.x, fmaf(h.y, Cv.y, fmaf(h.z, Cv.z, h.w * Cv.w)));
       }
     } else {
@@ -526,8 +536,8 @@ __global__ void __launch_bounds__(256) k_ssm_step(Args a, float* __restrict__ hs
     if (in) {
       float o = Dc * u;
       for (int q = 0; q < Q; q++) o += so[tid * Q + q];
-      if (a.z) o *= silu(ldf((const T*)a.z + b * a.z_b + c));
-      stf((T*)a.y + b * a.y_b + c, o);
+      if (a.z) o *= silu(ldf((gin<T>)a.z + b * a.z_b + c));
+      stf((gout<T>)a.y + b * a.y_b + c, o);
     }
     // the next sequence writes sd and sdu, which nobody reads any more, and so only after its own barrier
   }
@@ -591,17 +601,17 @@ template <typename T, int MOST>
 __global__ void __launch_bounds__(256) k_ssm_bwd_local(Args a, GradArgs ga) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int Q = a.Q, nt = blockDim.x, tid = threadIdx.x;
-  float4* sA = reinterpret_cast<float4*>(lds);  // [Q][nt]
-  float4* sG = sA + Q * nt;                     // [Q][nt]
+  f4t* sA = reinterpret_cast<f4t*>(lds);  // [Q][nt]
+  f4t* sG = sA + Q * nt;                     // [Q][nt]
   float* sbc = lds + 8 * Q * nt;                // [2][Q][kSteps][2][4]
   const Place pl = place(a, blockIdx.x);
   const long b = pl.b;
   const unsigned c = pl.c;
-  const long tbeg = pl.s * a.chunk, tend = min(a.T, tbeg + a.chunk);
-  const long tlast = tbeg + (tend - tbeg - 1) / kSteps * kSteps;
+  const int tbeg = (int)pl.s * a.chunk, tend = min(a.T, tbeg + a.chunk);
+  const int tlast = tbeg + (tend - tbeg - 1) / kSteps * kSteps;
   for (int q = 0; q < Q; q++) {
     sA[q * nt + tid] = decay4(a, c, q);
-    sG[q * nt + tid] = make_float4(0.f, 0.f, 0.f, 0.f);
+    sG[q * nt + tid] = f4(0.f, 0.f, 0.f, 0.f);
   }
   const float bias = a.dt_bias ? a.dt_bias[c] : 0.f;
   float dsum = 0.f;
@@ -610,22 +620,22 @@ __global__ void __launch_bounds__(256) k_ssm_bwd_local(Args a, GradArgs ga) {
   StageBC<T, MOST> bc;
   bc.init(a, b, pl.g);
   float fl;
-  auto fetch = [&](long t0) __attribute__((always_inline)) {
-    const int n = (int)min((long)kSteps, tend - t0);
+  auto fetch = [&](int t0) __attribute__((always_inline)) {
+    const int n = min(kSteps, tend - t0);
     bc.get(t0, n);
-    rd.get((const T*)a.delta + b * a.d_b + t0 * a.d_t, a.d_t, n, c);
-    if (a.z) rz.get((const T*)a.z + b * a.z_b + t0 * a.z_t, a.z_t, n, c);
-    rg.get((const T*)ga.dy + b * ga.dy_b + t0 * ga.dy_t, ga.dy_t, n, c);
+    rd.get((gin<T>)a.delta + b * a.d_b + t0 * a.d_t, a.d_t, n, c);
+    if (a.z) rz.get((gin<T>)a.z + b * a.z_b + t0 * a.z_t, a.z_t, n, c);
+    rg.get((gin<T>)ga.dy + b * ga.dy_b + t0 * ga.dy_t, ga.dy_t, n, c);
     fl = flag_load(a, t0, tend, b);
   };
   fetch(tlast);
   int buf = 0;
-  for (long t0 = tlast; t0 >= tbeg; t0 -= kSteps, buf ^= 1) {
+  for (int t0 = tlast; t0 >= tbeg; t0 -= kSteps, buf ^= 1) {
     float* s = sbc + buf * 64 * Q;
     bc.put(a, s);
     const Rows<T> cd = rd, cz = rz, cg = rg;
     const unsigned st = flag_bits(fl) >> (kTaps - 1);
-    const int steps = (int)min((long)kSteps, tend - t0);
+    const int steps = min(kSteps, tend - t0);
     __syncthreads();
     if (t0 > tbeg) fetch(t0 - kSteps);
     cleared |= st;
@@ -637,22 +647,22 @@ __global__ void __launch_bounds__(256) k_ssm_bwd_local(Args a, GradArgs ga) {
       dsum += d[i];
     }
     for (int q = 0; q < Q; q++) {
-      const float4 A = sA[q * nt + tid];
-      float4 g = sG[q * nt + tid];
+      const f4t A = sA[q * nt + tid];
+      f4t g = sG[q * nt + tid];
 #pragma unroll
       for (int i = kSteps - 1; i >= 0; i--) {
-        const float4 Cv = *reinterpret_cast<const float4*>(&s[64 * q + 8 * i + 4]);
+        const f4t Cv = *reinterpret_cast<const f4t*>(&s[64 * q + 8 * i + 4]);
         g.x = ex2(d[i] * A.x) * fmaf(dout[i], Cv.x, g.x);
         g.y = ex2(d[i] * A.y) * fmaf(dout[i], Cv.y, g.y);
         g.z = ex2(d[i] * A.z) * fmaf(dout[i], Cv.z, g.z);
         g.w = ex2(d[i] * A.w) * fmaf(dout[i], Cv.w, g.w);
-        if (st & (1u << i)) g = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (st & (1u << i)) g = f4(0.f, 0.f, 0.f, 0.f);
       }
       sG[q * nt + tid] = g;
     }
   }
   if (!pl.in) return;
-  float4* out = reinterpret_cast<float4*>(ga.carry) + (pl.s * a.B + b) * Q * a.C + c;
+  gout<f4t> out = (gout<f4t>)ga.carry + (pl.s * a.B + b) * Q * a.C + c;
   for (int q = 0; q < Q; q++) out[q * a.C] = sG[q * nt + tid];
   a.dsum[(pl.s * a.B + b) * a.C + c] = cleared ? -1.f : dsum;
 }
@@ -664,7 +674,7 @@ __global__ void __launch_bounds__(256) k_ssm_bwd_join(Args a, GradArgs ga) {
   const StateAt at = state_at(a, i);
   const float A2 = at.in ? a.A[at.c * a.N + at.n] * kLog2e : 0.f;
   const long last = a.chunks - 1;
-  join<-1>(ga.carry + last * row + i, row, a.dsum + last * a.B * a.C + at.bc, a.B * a.C, (int)a.chunks, A2, 0.f);
+  join<-1>(ga.carry + last * row + i, row, a.dsum + last * a.B * a.C + at.bc, a.B * a.C, a.chunks, A2, 0.f);
 }
 
 // The gradient of one chunk after another. Batches of kSteps steps run backwards in time. Each takes the states four at
@@ -683,9 +693,9 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int Q = a.Q, nt = blockDim.x, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6, waves = nt >> 6;
-  float4* sA = reinterpret_cast<float4*>(lds);  // [Q][nt]
-  float4* sG = sA + Q * nt;                     // [Q][nt]
-  float4* sdA = sG + Q * nt;                    // [Q][nt]
+  f4t* sA = reinterpret_cast<f4t*>(lds);  // [Q][nt]
+  f4t* sG = sA + Q * nt;                     // [Q][nt]
+  f4t* sdA = sG + Q * nt;                    // [Q][nt]
   float* sbc = lds + 12 * Q * nt;               // [2][Q][kSteps][B, C][4]
   float* red = sbc + 2 * 64 * Q;                // [waves][Q][kSteps][dB, dC][4]
   float* reds = red + waves * 64 * Q;           // [waves][kSteps] of S
@@ -700,7 +710,7 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
   cv.init(a, c);
   for (int q = 0; q < Q; q++) {
     sA[q * nt + tid] = decay4(a, c, q);
-    sdA[q * nt + tid] = make_float4(0.f, 0.f, 0.f, 0.f);
+    sdA[q * nt + tid] = f4(0.f, 0.f, 0.f, 0.f);
   }
   const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, Dc = a.D ? a.D[c] : 0.f;
   float dD = 0.f, dbias = 0.f, dcb = 0.f, dw[kTaps] = {};
@@ -709,27 +719,27 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
   int buf = 0;
   for (unsigned item = row; item < items; item += (unsigned)ga.rows) {
     const long b = uniform(item % (unsigned)a.B), s = uniform(item / (unsigned)a.B);
-    const long tbeg = s * a.chunk, tend = min(a.T, tbeg + a.chunk);
+    const int tbeg = (int)s * a.chunk, tend = min(a.T, tbeg + a.chunk);
     {
-      const float4* carry = reinterpret_cast<const float4*>(ga.carry) + s * quads + b * Q * a.C;
+      gin<f4t> carry = (gin<f4t>)ga.carry + s * quads + b * Q * a.C;
       for (int q = 0; q < Q; q++)  // a lane without a channel sends nothing back, and so adds nothing to a sum
-        sG[q * nt + tid] = a.chunks > 1 && in ? (carry + q * a.C)[c] : make_float4(0.f, 0.f, 0.f, 0.f);
+        sG[q * nt + tid] = a.chunks > 1 && in ? (carry + q * a.C)[c] : f4(0.f, 0.f, 0.f, 0.f);
     }
     // ds of the three steps after the current one, of the same episode (zero past the chunk: its successor's
     // share of this chunk's last steps comes through the halo)
     float q1 = 0.f, q2 = 0.f, q3 = 0.f;
-    for (long t0 = tbeg + (tend - tbeg - 1) / kSteps * kSteps; t0 >= tbeg; t0 -= kSteps, buf ^= 1) {
-      const int steps = (int)min((long)kSteps, tend - t0);
+    for (int t0 = tbeg + (tend - tbeg - 1) / kSteps * kSteps; t0 >= tbeg; t0 -= kSteps, buf ^= 1) {
+      const int steps = min(kSteps, tend - t0);
       Rows<T> rx, rd, rz, rg;
       float back[kTaps - 1];
-      rx.get((const T*)a.x + b * a.x_b + t0 * a.x_t, a.x_t, steps, c);
-      rd.get((const T*)a.delta + b * a.d_b + t0 * a.d_t, a.d_t, steps, c);
-      if (a.z) rz.get((const T*)a.z + b * a.z_b + t0 * a.z_t, a.z_t, steps, c);
+      rx.get((gin<T>)a.x + b * a.x_b + t0 * a.x_t, a.x_t, steps, c);
+      rd.get((gin<T>)a.delta + b * a.d_b + t0 * a.d_t, a.d_t, steps, c);
+      if (a.z) rz.get((gin<T>)a.z + b * a.z_b + t0 * a.z_t, a.z_t, steps, c);
       else rz = rx;  // not looked at
-      rg.get((const T*)ga.dy + b * ga.dy_b + t0 * ga.dy_t, ga.dy_t, steps, c);
+      rg.get((gin<T>)ga.dy + b * ga.dy_b + t0 * ga.dy_t, ga.dy_t, steps, c);
       look_back<T>(back, a, t0, b, c);
-      const float4* keep = reinterpret_cast<const float4*>(ga.keep) + t0 / kSteps * quads + b * Q * a.C;
-      float4 next = keep[c];
+      gin<f4t> keep = (gin<f4t>)ga.keep + t0 / kSteps * quads + b * Q * a.C;
+      f4t next = keep[c];
       const unsigned bits = flag_bits(flag_load(a, t0, tend, b)), st = bits >> (kTaps - 1);
       // stage B and C
       float* sb = sbc + buf * 64 * Q;
@@ -737,8 +747,8 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
         const int n = place_state(e), i = place_step(e);
         float v = 0.f;
         if (n < a.N && i < steps)
-          v = place_row(e) ? ldf((const T*)a.Cm + (t0 + i) * a.cm_t + b * a.cm_b + grp * a.N + n)
-                           : ldf((const T*)a.Bm + (t0 + i) * a.bm_t + b * a.bm_b + grp * a.N + n);
+          v = place_row(e) ? ldf((gin<T>)a.Cm + (t0 + i) * a.cm_t + b * a.cm_b + grp * a.N + n)
+                           : ldf((gin<T>)a.Bm + (t0 + i) * a.bm_t + b * a.bm_b + grp * a.N + n);
         sb[e] = v;
       }
       // Input j (0..10) of the batch and of the three steps before it, and a step's own convolution.
@@ -772,16 +782,16 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
       }
       auto scan = [&](auto ANY) __attribute__((always_inline)) {  // ANY: an episode starts in this batch
         for (int q = 0; q < Q; q++) {
-          const float4 A = sA[q * nt + tid], kh = next;
+          const f4t A = sA[q * nt + tid], kh = next;
           next = (keep + (q + 1 < Q ? q + 1 : q) * a.C)[c];
-          const float4 g4 = sG[q * nt + tid];
+          const f4t g4 = sG[q * nt + tid];
           const float Av[4] = {A.x, A.y, A.z, A.w};
           float h[4] = {kh.x, kh.y, kh.z, kh.w}, g[4] = {g4.x, g4.y, g4.z, g4.w}, dA[4] = {};
           float dec[kSteps][4], ah[kSteps][4], part[kSteps];
 #pragma unroll
           for (int i = 0; i < kSteps; i++) {
             const bool cut = decltype(ANY)::value && (st & (1u << i));
-            const float4 Bv = *reinterpret_cast<const float4*>(&sb[64 * q + 8 * i]);
+            const f4t Bv = *reinterpret_cast<const f4t*>(&sb[64 * q + 8 * i]);
             const float Bn[4] = {Bv.x, Bv.y, Bv.z, Bv.w};
 #pragma unroll
             for (int n = 0; n < 4; n++) {
@@ -794,8 +804,8 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
 #pragma unroll
           for (int i = kSteps - 1; i >= 0; i--) {
             const bool cut = decltype(ANY)::value && (st & (1u << i));
-            const float4 Bv = *reinterpret_cast<const float4*>(&sb[64 * q + 8 * i]);
-            const float4 Cv = *reinterpret_cast<const float4*>(&sb[64 * q + 8 * i + 4]);
+            const f4t Bv = *reinterpret_cast<const f4t*>(&sb[64 * q + 8 * i]);
+            const f4t Cv = *reinterpret_cast<const f4t*>(&sb[64 * q + 8 * i + 4]);
             const float Bn[4] = {Bv.x, Bv.y, Bv.z, Bv.w}, Cn[4] = {Cv.x, Cv.y, Cv.z, Cv.w};
             float v[8];
 #pragma unroll
@@ -813,9 +823,9 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
             __builtin_amdgcn_sched_barrier(0);
           }
           red[(wave * Q + q) * 64 + out] = step_sums(part, lane);
-          sG[q * nt + tid] = make_float4(g[0], g[1], g[2], g[3]);
-          const float4 acc = sdA[q * nt + tid];
-          sdA[q * nt + tid] = make_float4(acc.x + dA[0], acc.y + dA[1], acc.z + dA[2], acc.w + dA[3]);
+          sG[q * nt + tid] = f4(g[0], g[1], g[2], g[3]);
+          const f4t acc = sdA[q * nt + tid];
+          sdA[q * nt + tid] = f4(acc.x + dA[0], acc.y + dA[1], acc.z + dA[2], acc.w + dA[3]);
         }
       };
       if (st) scan(std::true_type{});
@@ -842,18 +852,18 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
         }
         sum = fmaf(sb[e ^ 4], S, sum);
         const long t = t0 + i;
-        if (ga.bc) ga.bc[(((cb * a.T + t) * a.B + b) * a.G + grp) * 2 * a.N + which * a.N + n] = sum;
-        else if (which && ga.dC) stf((T*)ga.dC + t * ga.dc_t + b * ga.dc_b + grp * a.N + n, sum);
-        else if (!which && ga.dB) stf((T*)ga.dB + t * ga.db_t + b * ga.db_b + grp * a.N + n, sum);
+        if (ga.bc) ga.bc[((((long)cb * a.T + t) * a.B + b) * a.G + grp) * 2 * a.N + which * a.N + n] = sum;
+        else if (which && ga.dC) stf((gout<T>)ga.dC + t * ga.dc_t + b * ga.dc_b + grp * a.N + n, sum);
+        else if (!which && ga.dB) stf((gout<T>)ga.dB + t * ga.db_t + b * ga.db_b + grp * a.N + n, sum);
       }
       // the channel's own gradients
       rx.renew();
       rd.renew();
       rz.renew();
-      const long last = t0 + steps - 1;
-      T* pdd = (T*)ga.ddelta + b * ga.dd_b + last * ga.dd_t;
-      T* pdz = (T*)ga.dz + b * ga.dz_b + last * ga.dz_t;
-      T* pdx = (T*)ga.dx + b * ga.dx_b + last * ga.dx_t;
+      const int last = t0 + steps - 1;
+      gout<T> pdd = (gout<T>)ga.ddelta + b * ga.dd_b + last * ga.dd_t;
+      gout<T> pdz = (gout<T>)ga.dz + b * ga.dz_b + last * ga.dz_t;
+      gout<T> pdx = (gout<T>)ga.dx + b * ga.dx_b + last * ga.dx_t;
       const int own = tend < a.T && t0 + kSteps >= tend ? steps - (K - 1) : kSteps;  // steps from here on are finished by the halo's launch
 #pragma unroll
       for (int i = kSteps - 1; i >= 0; i--) {
@@ -888,7 +898,7 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
           if (a.z && ga.dz) stf(pdz + c, rg[i] * fmaf(du[i], cb2, fmaf(Dc, u, o[i])) * dsilu(rz[i], sigm(rz[i])));
           if (ga.dx) {
             if (i < own) stf(pdx + c, dxv);
-            else (ga.halo + ((s * 2 * a.B + b) * (kTaps - 1) + (steps - 1 - i)) * a.C)[c] = dxv;
+            else ((gout<float>)ga.halo + ((s * 2 * a.B + b) * (kTaps - 1) + (steps - 1 - i)) * a.C)[c] = dxv;
           }
         }
         walk(pdd, -ga.dd_t);
@@ -931,7 +941,7 @@ __global__ void __launch_bounds__(256) k_ssm_halo(Args a, GradArgs ga) {
   bool cut = false;
   for (long q = t + 1; q < tend; q++) cut |= starts(a, q, b);
   if (!cut) v += ga.halo[(((s * 2 + 1) * a.B + b) * (kTaps - 1) + j) * a.C + c];
-  stf((T*)ga.dx + t * ga.dx_t + b * ga.dx_b + c, v);
+  stf((gout<T>)ga.dx + t * ga.dx_t + b * ga.dx_b + c, v);
 }
 
 // dB, dC = the channel blocks' sums in order.
@@ -944,9 +954,9 @@ __global__ void __launch_bounds__(256) k_ssm_fold_bc(Args a, GradArgs ga) {
     float s = 0.f;
     for (int cb = 0; cb < a.blocks_c; cb++) s += ga.bc[cb * tot + i];
     if (which) {
-      if (ga.dC) stf((T*)ga.dC + t * ga.dc_t + b * ga.dc_b + g * a.N + n, s);
+      if (ga.dC) stf((gout<T>)ga.dC + t * ga.dc_t + b * ga.dc_b + g * a.N + n, s);
     } else if (ga.dB) {
-      stf((T*)ga.dB + t * ga.db_t + b * ga.db_b + g * a.N + n, s);
+      stf((gout<T>)ga.dB + t * ga.db_t + b * ga.db_b + g * a.N + n, s);
     }
   }
 }
@@ -1009,7 +1019,7 @@ int check(const ph_ssm_args& p, const char* who) {
 
 Args args_of(const ph_ssm_args& p) {
   Args a{};
-  a.T = (long)p.T; a.B = (long)p.B; a.C = (long)p.C; a.N = (long)p.N; a.per = (long)(p.C / p.G); a.K = (long)p.K;
+  a.T = (int)p.T; a.B = (long)p.B; a.C = (int)p.C; a.N = (int)p.N; a.per = (int)(p.C / p.G); a.K = (int)p.K;
   a.G = (unsigned)p.G;
   a.Q = (int)((p.N + 3) / 4);
   a.x = p.x; a.z = p.z; a.delta = p.delta; a.Bm = p.Bm; a.Cm = p.Cm;
@@ -1036,13 +1046,15 @@ int block_threads(const Args& a, bool grad) {
 }
 static_assert(4 * (12 * 16 * 64 + 3 * 64 * 16 + 3 * kSteps) <= 64 * 1024, "one wavefront at N = 64");
 
-// Chunks of time: enough wavefronts for every SIMD to hold two, in chunks of at least 32 steps.
+// Chunks of time: enough wavefronts for every SIMD to hold two, in chunks of at least 32 steps. Chunks cost a second pass
+// over their steps and three launches (about 20 us each way), so sequences stay whole while one pass over all their
+// steps is not longer than that: up to 128 steps of 16 states, the more the fewer the states.
 int set_chunks(Args& a) {
   const long waves = a.B * a.G * ((a.per + 63) / 64);
   long want = (2048 + waves - 1) / waves;
   const long most = (a.T + 31) / 32;
   if (want > most) want = most;
-  if (want < 1) want = 1;
+  if (want < 1 || (long)a.T * (8 + a.N) <= 128 * (8 + 16)) want = 1;
   a.chunk = (a.T + want - 1) / want;
   a.chunk = (a.chunk + kSteps - 1) / kSteps * kSteps;
   a.chunks = (a.T + a.chunk - 1) / a.chunk;
@@ -1100,7 +1112,7 @@ int bwd_t(Args& a, GradArgs& ga, int nt, const ParOut& po, hipStream_t st) {
     PH_LAUNCH_CHECK();
   }
   const long CP = a.C * ga.P;
-  k_ssm_fold_par<<<ceil_div((size_t)CP, 64), 256, 0, st>>>(ga.par, ga.rows, CP, (int)a.N, (int)a.K, ga.P, po);
+  k_ssm_fold_par<<<ceil_div((size_t)CP, 64), 256, 0, st>>>(ga.par, ga.rows, CP, a.N, a.K, ga.P, po);
   PH_LAUNCH_CHECK();
   return PH_OK;
 }
