@@ -291,7 +291,10 @@ __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
     bc.get(t0, n);
     rx.get(xp, a.x_t, n, c);
     rd.get(dp, a.d_t, n, c);
-    if (!LOCAL && a.z) rz.get(zp, a.z_t, n, c);
+    if (!LOCAL) {
+      if (a.z) rz.get(zp, a.z_t, n, c);
+      else rz = rx;  // not looked at
+    }
     fl = flag_load(a, t0, tend, b);
     walk(xp, kSteps * a.x_t);
     walk(dp, kSteps * a.d_t);
@@ -326,22 +329,29 @@ __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
     if (t0 + kSteps < tend) fetch(t0 + kSteps);
     cleared |= st;
     float d[kSteps], du[kSteps], o[kSteps];
+    // CLEAN: a whole batch that no episode's start cuts; the other form selects what each step sees. Without a convolution or
+    // gate theirs are computed all the same and not taken: a choice per step would split the batch into many short blocks.
+    auto prepare = [&](auto CLEAN) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kSteps; i++) {
-      float u = cx[i];
-      if (cv.K) {
-        const int n = cv.reach(bits, i);
+      for (int i = 0; i < kSteps; i++) {
+        const int n = decltype(CLEAN)::value ? cv.K - 1 : cv.reach(bits, i);
         const float x1 = i > 0 ? cx[i > 0 ? i - 1 : 0] : back[2], x2 = i > 1 ? cx[i > 1 ? i - 2 : 0] : back[i + 1],
                     x3 = i > 2 ? cx[i > 2 ? i - 3 : 0] : back[i];
-        u = silu(cv.pre(u, n > 0 ? x1 : 0.f, n > 1 ? x2 : 0.f, n > 2 ? x3 : 0.f));
+        const float w = silu(cv.pre(cx[i], n > 0 ? x1 : 0.f, n > 1 ? x2 : 0.f, n > 2 ? x3 : 0.f));
+        const float u = cv.K ? w : cx[i];
+        d[i] = softplus(cd[i] + bias);
+        du[i] = d[i] * u;
+        if (!decltype(CLEAN)::value) {
+          // a step past the end leaves the state as it is: a decay of one and no input
+          d[i] = i < steps ? d[i] : 0.f;
+          du[i] = i < steps ? du[i] : 0.f;
+        }
+        if (LOCAL) dsum += d[i];
+        o[i] = Dc * u;
       }
-      // a step past the end leaves the state as it is: a decay of one and no input
-      d[i] = softplus(cd[i] + bias);
-      d[i] = i < steps ? d[i] : 0.f;
-      du[i] = i < steps ? d[i] * u : 0.f;
-      if (LOCAL) dsum += d[i];
-      o[i] = Dc * u;
-    }
+    };
+    if (bits == 0 && steps == kSteps) prepare(std::true_type{});
+    else prepare(std::false_type{});
 #pragma unroll
     for (int j = 0; j < kTaps - 1; j++) back[j] = cx[kSteps - (kTaps - 1) + j];
     auto scan = [&](auto ANY) __attribute__((always_inline)) {  // ANY: an episode starts in this batch
@@ -375,9 +385,23 @@ __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
       if (keep) walk(keep, quads);
 #pragma unroll
       for (int i = 0; i < kSteps; i++) {
-        if (i < steps && pl.in) stf(yp + c, a.z ? o[i] * silu(cz[i]) : o[i]);
-        walk(yp, a.y_t);
+        const float w = o[i] * silu(cz[i]);
+        o[i] = a.z ? w : o[i];
       }
+      if (pl.in) {
+        if (steps == kSteps) {
+          gout<T> p = yp;
+#pragma unroll
+          for (int i = 0; i < kSteps; i++) {
+            stf(p + c, o[i]);
+            walk(p, a.y_t);
+          }
+        } else {
+          for (int i = 0; i < kSteps; i++)
+            if (i < steps) stf(yp + i * a.y_t + c, o[i]);
+        }
+      }
+      walk(yp, kSteps * a.y_t);
     }
   }
   if (!pl.in) return;
@@ -400,19 +424,20 @@ __device__ __forceinline__ StateAt state_at(const Args& a, long i) {
   return {b * a.C + c, c, n, n < a.N};
 }
 // run -> decay run + local over the chunks in order, each chunk's entry replaced by the run before it. A chain of short
-// steps, so the loads of eight of them go ahead of it.
+// steps, so the loads of sixteen of them go ahead of it.
 template <int DIR>
 __device__ __forceinline__ void join(float* loc, long row, const float* dsum, long drow, int chunks, float A2, float run) {
-  for (int s0 = 0; s0 < chunks; s0 += 8) {
-    float l[8], d[8];
+  constexpr int kAhead = 16;
+  for (int s0 = 0; s0 < chunks; s0 += kAhead) {
+    float l[kAhead], d[kAhead];
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
+    for (int k = 0; k < kAhead; k++) {
       const long s = min(s0 + k, chunks - 1);
       l[k] = loc[DIR * s * row];
       d[k] = dsum[DIR * s * drow];
     }
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
+    for (int k = 0; k < kAhead; k++) {
       if (s0 + k >= chunks) break;
       loc[DIR * (long)(s0 + k) * row] = run;
       run = d[k] < 0.f ? l[k] : fmaf(ex2(A2 * d[k]), run, l[k]);
@@ -751,28 +776,37 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
                            : ldf((gin<T>)a.Bm + (t0 + i) * a.bm_t + b * a.bm_b + grp * a.N + n);
         sb[e] = v;
       }
-      // Input j (0..10) of the batch and of the three steps before it, and a step's own convolution.
+      // Input j (0..10) of the batch and of the three steps before it, and a step's own convolution. CLEAN as in the forward.
       auto input = [&](int j) __attribute__((always_inline)) { return j < kTaps - 1 ? back[j < kTaps - 1 ? j : 0] : rx[j < kTaps - 1 ? 0 : j - (kTaps - 1)]; };
-      auto conv = [&](int i, float& x1, float& x2, float& x3) __attribute__((always_inline)) {
-        const int n = cv.reach(bits, i);
+      auto conv = [&](auto CLEAN, int i, float& x1, float& x2, float& x3) __attribute__((always_inline)) {
+        const int n = decltype(CLEAN)::value ? K - 1 : cv.reach(bits, i);
         x1 = n > 0 ? input(i + 2) : 0.f;
         x2 = n > 1 ? input(i + 1) : 0.f;
         x3 = n > 2 ? input(i) : 0.f;
         return cv.pre(rx[i], x1, x2, x3);
       };
+      const bool clean = bits == 0 && steps == kSteps;
       float d[kSteps], du[kSteps], dout[kSteps], o[kSteps], gB[kSteps], Aq[kSteps];
+      auto prepare = [&](auto CLEAN) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < kSteps; i++) {
-        float x1, x2, x3;
-        const float u = K ? silu(conv(i, x1, x2, x3)) : rx[i];
-        // a step past the end neither decays, nor takes nor gives
-        d[i] = softplus(rd[i] + bias);
-        d[i] = i < steps ? d[i] : 0.f;
-        du[i] = i < steps ? d[i] * u : 0.f;
-        dout[i] = a.z ? rg[i] * silu(rz[i]) : rg[i];
-        dout[i] = i < steps && in ? dout[i] : 0.f;
-        o[i] = gB[i] = Aq[i] = 0.f;
-      }
+        for (int i = 0; i < kSteps; i++) {
+          float x1, x2, x3;
+          const float w = silu(conv(CLEAN, i, x1, x2, x3)), u = K ? w : rx[i], gated = rg[i] * silu(rz[i]);
+          d[i] = softplus(rd[i] + bias);
+          du[i] = d[i] * u;
+          dout[i] = a.z ? gated : rg[i];
+          if (!decltype(CLEAN)::value) {
+            // a step past the end neither decays, nor takes nor gives
+            d[i] = i < steps ? d[i] : 0.f;
+            du[i] = i < steps ? du[i] : 0.f;
+            dout[i] = i < steps ? dout[i] : 0.f;
+          }
+          dout[i] = in ? dout[i] : 0.f;
+          o[i] = gB[i] = Aq[i] = 0.f;
+        }
+      };
+      if (clean) prepare(std::true_type{});
+      else prepare(std::false_type{});
       __syncthreads();
       if (tid < kSteps) {  // read after the barrier below
         float p = 0.f;
@@ -861,49 +895,71 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
       rd.renew();
       rz.renew();
       const int last = t0 + steps - 1;
-      gout<T> pdd = (gout<T>)ga.ddelta + b * ga.dd_b + last * ga.dd_t;
-      gout<T> pdz = (gout<T>)ga.dz + b * ga.dz_b + last * ga.dz_t;
-      gout<T> pdx = (gout<T>)ga.dx + b * ga.dx_b + last * ga.dx_t;
-      const int own = tend < a.T && t0 + kSteps >= tend ? steps - (K - 1) : kSteps;  // steps from here on are finished by the halo's launch
+      float cb2[kSteps];
 #pragma unroll
-      for (int i = kSteps - 1; i >= 0; i--) {
-        if (i >= steps) continue;
-        float x1, x2, x3, u = rx[i], pre = 0.f, sg = 0.f;
-        if (K) {
-          pre = conv(i, x1, x2, x3);
-          sg = sigm(pre);
-          u = pre * sg;
-        }
-        const float cb2 = scb[buf * kSteps + i], gb = fmaf(dout[i], cb2, gB[i]);
-        const float ddt = fmaf(u, gb, Aq[i] * (1.f / kLog2e)) * sigm(rd[i] + bias);
-        float ds = fmaf(d[i], gb, Dc * dout[i]);
-        dD = fmaf(dout[i], u, dD);
-        dbias += ddt;
-        float dxv = ds;
-        if (K) {
-          ds *= dsilu(pre, sg);
+      for (int i = 0; i < kSteps; i++) cb2[i] = scb[buf * kSteps + i];
+      float dxv[kSteps], ddt[kSteps], dzv[kSteps];
+      auto finish = [&](auto CLEAN) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = kSteps - 1; i >= 0; i--) {
+          if (!decltype(CLEAN)::value && i >= steps) continue;
+          float x1, x2, x3;
+          const float pre = conv(CLEAN, i, x1, x2, x3), sg = sigm(pre), w = pre * sg, u = K ? w : rx[i];
+          const float gb = fmaf(dout[i], cb2[i], gB[i]);
+          ddt[i] = fmaf(u, gb, Aq[i] * (1.f / kLog2e)) * sigm(rd[i] + bias);
+          dzv[i] = rg[i] * fmaf(du[i], cb2[i], fmaf(Dc, u, o[i])) * dsilu(rz[i], sigm(rz[i]));
+          const float dus = fmaf(d[i], gb, Dc * dout[i]), ds = dus * dsilu(pre, sg);
+          dD = fmaf(dout[i], u, dD);
+          dbias += ddt[i];
           dcb += ds;
           dw[3] = fmaf(ds, rx[i], dw[3]);
           dw[2] = fmaf(ds, x1, dw[2]);
           dw[1] = fmaf(ds, x2, dw[1]);
           dw[0] = fmaf(ds, x3, dw[0]);
-          dxv = fmaf(cv.w[3], ds, fmaf(cv.w[2], q1, fmaf(cv.w[1], q2, cv.w[0] * q3)));
-          const bool cut = st & (1u << i);
+          const float dc = fmaf(cv.w[3], ds, fmaf(cv.w[2], q1, fmaf(cv.w[1], q2, cv.w[0] * q3)));
+          dxv[i] = K ? dc : dus;
+          const bool cut = !decltype(CLEAN)::value && (st & (1u << i));
           q3 = cut || K < 4 ? 0.f : q2;
           q2 = cut || K < 3 ? 0.f : q1;
           q1 = cut || K < 2 ? 0.f : ds;
         }
-        if (in) {
-          if (ga.ddelta) stf(pdd + c, ddt);
-          if (a.z && ga.dz) stf(pdz + c, rg[i] * fmaf(du[i], cb2, fmaf(Dc, u, o[i])) * dsilu(rz[i], sigm(rz[i])));
-          if (ga.dx) {
-            if (i < own) stf(pdx + c, dxv);
-            else ((gout<float>)ga.halo + ((s * 2 * a.B + b) * (kTaps - 1) + (steps - 1 - i)) * a.C)[c] = dxv;
+      };
+      if (clean) finish(std::true_type{});
+      else finish(std::false_type{});
+      if (in) {
+        // the last K - 1 steps of a chunk that has a successor are finished by the halo's launch
+        const bool halo = tend < a.T && t0 + kSteps >= tend && K > 1;
+        if (steps == kSteps && !halo && ga.ddelta && ga.dx) {
+          gout<T> pd = (gout<T>)ga.ddelta + b * ga.dd_b + t0 * ga.dd_t;
+          gout<T> px = (gout<T>)ga.dx + b * ga.dx_b + t0 * ga.dx_t;
+#pragma unroll
+          for (int i = 0; i < kSteps; i++) {
+            stf(pd + c, ddt[i]);
+            stf(px + c, dxv[i]);
+            walk(pd, ga.dd_t);
+            walk(px, ga.dx_t);
+          }
+          if (ga.dz) {
+            gout<T> pz = (gout<T>)ga.dz + b * ga.dz_b + t0 * ga.dz_t;
+#pragma unroll
+            for (int i = 0; i < kSteps; i++) {
+              stf(pz + c, dzv[i]);
+              walk(pz, ga.dz_t);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kSteps; i++) {
+            if (i >= steps) break;
+            const int t = t0 + i;
+            if (ga.ddelta) stf((gout<T>)ga.ddelta + b * ga.dd_b + t * ga.dd_t + c, ddt[i]);
+            if (ga.dz) stf((gout<T>)ga.dz + b * ga.dz_b + t * ga.dz_t + c, dzv[i]);
+            if (ga.dx) {
+              if (!halo || last - t >= K - 1) stf((gout<T>)ga.dx + b * ga.dx_b + t * ga.dx_t + c, dxv[i]);
+              else ((gout<float>)ga.halo + ((s * 2 * a.B + b) * (kTaps - 1) + (last - t)) * a.C)[c] = dxv[i];
+            }
           }
         }
-        walk(pdd, -ga.dd_t);
-        walk(pdz, -ga.dz_t);
-        walk(pdx, -ga.dx_t);
       }
     }
     // what this chunk adds to dx of the K - 1 steps before it: step tbeg - 1 - j takes ds of up to K - 1 - j steps on
@@ -1205,7 +1261,7 @@ extern "C" int ph_ssm_scan_grad(const ph_ssm_args* p, const float* keep, const v
   GradArgs ga{};
   ga.dy = dy; ga.dy_t = dy_t; ga.dy_b = dy_b; ga.keep = keep;
   ga.dx = g->dx; ga.dx_t = g->dx_t; ga.dx_b = g->dx_b;
-  ga.dz = g->dz; ga.dz_t = g->dz_t; ga.dz_b = g->dz_b;
+  ga.dz = p->z ? g->dz : nullptr; ga.dz_t = g->dz_t; ga.dz_b = g->dz_b;
   ga.ddelta = g->ddelta; ga.dd_t = g->ddelta_t; ga.dd_b = g->ddelta_b;
   ga.dB = g->dBm; ga.db_t = g->dBm_t; ga.db_b = g->dBm_b;
   ga.dC = g->dCm; ga.dc_t = g->dCm_t; ga.dc_b = g->dCm_b;
