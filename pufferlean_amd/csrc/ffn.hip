@@ -22,43 +22,68 @@ namespace {
 
 size_t up8(size_t n) { return (n + 7) / 8 * 8; }
 
-// dst [rows_p][cols_p] = src [rows][cols] (row stride ld) with zeros beyond, or its transpose, [cols_p][rows_p].
+// One copy: dst [rows_p][cols_p] = src [rows][cols] (row stride ld) with zeros beyond, or its transpose, [cols_p][rows_p].
+struct Lay {
+  const void* src;
+  void* dst;
+  long rows, cols, ld, rows_p, cols_p;
+  int trans;
+  unsigned first;  // block of its first 32 x 32 tile
+};
+constexpr int kMostLays = 4;
+struct Lays {
+  Lay l[kMostLays];
+  int n;
+  unsigned blocks;
+};
+// All copies of a call in one launch, a 32 x 32 tile per block.
 template <typename T>
-__global__ void __launch_bounds__(256) k_lay(const T* __restrict__ src, long rows, long cols, long ld, T* __restrict__ dst,
-                                             long rows_p, long cols_p, int trans) {
+__global__ void __launch_bounds__(256) k_lay(Lays ls) {
   __shared__ T tile[32][33];
-  const long nc = (cols_p + 31) / 32, r0 = blockIdx.x / nc * 32, c0 = blockIdx.x % nc * 32;
+  int w = 0;
+  while (w + 1 < ls.n && blockIdx.x >= ls.l[w + 1].first) w++;
+  const Lay& j = ls.l[w];
+  const T* src = (const T*)j.src;
+  T* dst = (T*)j.dst;
+  const long nc = (j.cols_p + 31) / 32, id = blockIdx.x - j.first, r0 = id / nc * 32, c0 = id % nc * 32;
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
 #pragma unroll
   for (int i = 0; i < 32; i += 8) {
     const long r = r0 + y + i, c = c0 + x;
-    const T v = r < rows && c < cols ? src[r * ld + c] : T(0);
-    if (!trans) {
-      if (r < rows_p && c < cols_p) dst[r * cols_p + c] = v;
+    const T v = r < j.rows && c < j.cols ? src[r * j.ld + c] : T(0);
+    if (!j.trans) {
+      if (r < j.rows_p && c < j.cols_p) dst[r * j.cols_p + c] = v;
     } else {
       tile[y + i][x] = v;
     }
   }
-  if (!trans) return;
+  if (!j.trans) return;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 32; i += 8) {
     const long c = c0 + y + i, r = r0 + x;
-    if (r < rows_p && c < cols_p) dst[c * rows_p + r] = tile[x][y + i];
+    if (r < j.rows_p && c < j.cols_p) dst[c * j.rows_p + r] = tile[x][y + i];
   }
 }
 
-int lay(int dtype, const void* src, size_t rows, size_t cols, size_t ld, void* dst, size_t rows_p, size_t cols_p, bool trans,
-        hipStream_t st) {
-  const size_t blocks = (rows_p + 31) / 32 * ((cols_p + 31) / 32);
-  PH_REQUIRE(blocks < (1u << 31), "ffn: %zu x %zu values to lay out", rows_p, cols_p);
-  if (dtype == PH_BF16)
-    k_lay<uint16_t><<<(unsigned)blocks, 256, 0, st>>>((const uint16_t*)src, rows, cols, ld, (uint16_t*)dst, rows_p, cols_p, trans);
-  else
-    k_lay<float><<<(unsigned)blocks, 256, 0, st>>>((const float*)src, rows, cols, ld, (float*)dst, rows_p, cols_p, trans);
-  PH_LAUNCH_CHECK();
-  return PH_OK;
-}
+// Collects a call's copies.
+struct Layer {
+  Lays ls{};
+  int add(const void* src, size_t rows, size_t cols, size_t ld, void* dst, size_t rows_p, size_t cols_p, bool trans) {
+    const size_t blocks = ls.blocks + (rows_p + 31) / 32 * ((cols_p + 31) / 32);
+    PH_REQUIRE(blocks < (1u << 31) && ls.n < kMostLays, "ffn: %zu x %zu values to lay out", rows_p, cols_p);
+    ls.l[ls.n++] = Lay{src, dst, (long)rows, (long)cols, (long)ld, (long)rows_p, (long)cols_p, trans, ls.blocks};
+    ls.blocks = (unsigned)blocks;
+    return PH_OK;
+  }
+  int run(int dtype, hipStream_t st) {
+    if (!ls.n) return PH_OK;
+    if (dtype == PH_BF16) k_lay<uint16_t><<<ls.blocks, 256, 0, st>>>(ls);
+    else k_lay<float><<<ls.blocks, 256, 0, st>>>(ls);
+    PH_LAUNCH_CHECK();
+    return PH_OK;
+  }
+};
 
 // ---- few rows --------------------------------------------------------------------------------------------
 // Up to 64 rows are bound by the weights' bytes and by latency, so the weights go from memory straight into the operand
@@ -154,6 +179,9 @@ int product(int ta, int tb, size_t M, size_t N, size_t K, int dtype, const void*
   return gemm(d, st);
 }
 
+// Rows from which the backward's products take transposed weights.
+constexpr size_t kTransposeRows = 2048;
+
 // One call's sizes, and its scratch handed out in pieces of 256 bytes.
 struct Call {
   int dtype, act;
@@ -210,22 +238,20 @@ extern "C" int ph_ffn(int dtype, int act, size_t M, size_t D, size_t F, const vo
   if (!wo_ok) c.want(D * Fp, c.e);
   if (!h) c.want(M * Fp, c.e);
   PH_TRY(c.take_all());
+  Layer lay;
+  auto padded = [&](const void*& p, size_t rows, size_t cols, size_t ld, size_t rows_p, size_t cols_p) {
+    void* q = c.take(rows_p * cols_p, c.e);
+    const void* src = p;
+    p = q;
+    return lay.add(src, rows, cols, ld, q, rows_p, cols_p, false);
+  };
   if (!x_ok) {
-    void* p = c.take(M * Dp, c.e);
-    PH_TRY(lay(dtype, x, M, D, ldx, p, M, Dp, false, c.st));
-    x = p;
+    PH_TRY(padded(x, M, D, ldx, M, Dp));
     ldx = Dp;
   }
-  if (!wi_ok) {
-    void* p = c.take(2 * Fp * Dp, c.e);
-    PH_TRY(lay(dtype, w_in, 2 * F, D, D, p, 2 * Fp, Dp, false, c.st));
-    w_in = p;
-  }
-  if (!wo_ok) {
-    void* p = c.take(D * Fp, c.e);
-    PH_TRY(lay(dtype, w_out, D, F, F, p, D, Fp, false, c.st));
-    w_out = p;
-  }
+  if (!wi_ok) PH_TRY(padded(w_in, 2 * F, D, D, 2 * Fp, Dp));
+  if (!wo_ok) PH_TRY(padded(w_out, D, F, F, D, Fp));
+  PH_TRY(lay.run(dtype, c.st));
   if (!h) h = c.take(M * Fp, c.e);
   if (dtype == PH_BF16 && M <= (size_t)kFewRows && F == Fp) {
     auto run = [&](auto mt) {
@@ -260,49 +286,61 @@ extern "C" int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, con
   }
   const size_t Dp = c.Dp, Fp = c.Fp, we = dw_dtype == PH_BF16 ? 2 : 4;
   const bool x_ok = c.whole(x, ldx, D, Dp), dy_ok = c.whole(dy, lddy, D, Dp), w_ok = D == Dp && F == Fp;
+  // Transposed copies of the weights, so that both products read their operands along k: with many rows the products
+  // are faster by more than the copies take. With few rows the products take the weights as they are (or padded).
+  const bool trans = M >= kTransposeRows;
+  const bool wo_ok = !trans && c.whole(w_out, F, F, Fp) && D == Dp, wi_ok = !trans && c.whole(w_in, D, D, Dp) && F == Fp;
+  const bool need_dab = dx || dw_in;
   if (!x_ok && dw_in) c.want(M * Dp, c.e);
   if (!dy_ok) c.want(M * Dp, c.e);
-  c.want(Fp * Dp, c.e);          // w_out transposed
-  c.want(2 * Fp * Dp, c.e);      // w_in transposed
-  c.want(M * 2 * Fp, c.e);       // dab
-  if (!w_ok) c.want(2 * Fp * Dp, we);
+  if (need_dab) {
+    if (!wo_ok) c.want(Fp * Dp, c.e);
+    if (!wi_ok && dx) c.want(2 * Fp * Dp, c.e);
+    c.want(M * 2 * Fp, c.e);
+  }
+  if (!w_ok) c.want(2 * Fp * Dp, we), c.want(Fp * Dp, we);
   PH_TRY(c.take_all());
+  Layer lay;
+  auto laid = [&](const void*& p, size_t rows, size_t cols, size_t ld, size_t rows_p, size_t cols_p, bool tr) {
+    void* q = c.take(rows_p * cols_p, c.e);
+    const void* src = p;
+    p = q;
+    return lay.add(src, rows, cols, ld, q, rows_p, cols_p, tr);
+  };
   if (!x_ok && dw_in) {
-    void* p = c.take(M * Dp, c.e);
-    PH_TRY(lay(dtype, x, M, D, ldx, p, M, Dp, false, c.st));
-    x = p;
+    PH_TRY(laid(x, M, D, ldx, M, Dp, false));
     ldx = Dp;
   }
   if (!dy_ok) {
-    void* p = c.take(M * Dp, c.e);
-    PH_TRY(lay(dtype, dy, M, D, lddy, p, M, Dp, false, c.st));
-    dy = p;
+    PH_TRY(laid(dy, M, D, lddy, M, Dp, false));
     lddy = Dp;
   }
-  void* wot = c.take(Fp * Dp, c.e);
-  void* wit = c.take(2 * Fp * Dp, c.e);
-  void* dab = c.take(M * 2 * Fp, c.e);
-  void* dwp = w_ok ? nullptr : c.take(2 * Fp * Dp, we);
-  if (dx || dw_in) {
-    PH_TRY(lay(dtype, w_out, D, F, F, wot, Dp, Fp, true, c.st));
+  void* dab = nullptr;
+  if (need_dab) {
+    if (!wo_ok) PH_TRY(laid(w_out, D, F, F, Dp, Fp, trans));
+    if (!wi_ok && dx) PH_TRY(laid(w_in, 2 * F, D, D, 2 * Fp, Dp, trans));
+    dab = c.take(M * 2 * Fp, c.e);
+  }
+  PH_TRY(lay.run(dtype, c.st));
+  if (need_dab) {
     GluProduct g{};
-    g.grad = 1; g.dtype = dtype; g.act = act; g.M = (int)M; g.N = (int)Fp; g.K = (int)Dp;
-    g.A = dy; g.lda = (long)lddy; g.B = wot; g.ldb = (long)Dp;
+    g.grad = 1; g.dtype = dtype; g.act = act; g.M = (int)M; g.N = (int)Fp; g.K = (int)Dp; g.b_kn = !trans;
+    g.A = dy; g.lda = (long)lddy; g.B = w_out; g.ldb = (long)(trans ? Dp : Fp);
     g.pf = const_cast<void*>(pf); g.ldpf = (long)(2 * Fp); g.dab = dab; g.lddab = (long)(2 * Fp);
     PH_TRY(glu_product(g, c.st));
   }
-  if (dx) {
-    PH_TRY(lay(dtype, w_in, 2 * F, D, D, wit, 2 * Fp, Dp, true, c.st));
-    PH_TRY(product(0, 1, M, D, 2 * Fp, dtype, dab, 2 * Fp, wit, 2 * Fp, dtype, dx, lddx, c.st));
-  }
+  if (dx) PH_TRY(product(0, trans, M, D, 2 * Fp, dtype, dab, 2 * Fp, w_in, trans ? 2 * Fp : Dp, dtype, dx, lddx, c.st));
   // the weights' gradients; of padded operands through a padded copy
+  Layer out;
   if (dw_in) {
-    PH_TRY(product(1, 0, w_ok ? 2 * F : 2 * Fp, w_ok ? D : Dp, M, dtype, dab, 2 * Fp, x, ldx, dw_dtype, w_ok ? dw_in : dwp, Dp, c.st));
-    if (!w_ok) PH_TRY(lay(dw_dtype, dwp, 2 * F, D, Dp, dw_in, 2 * F, D, false, c.st));
+    void* q = w_ok ? dw_in : c.take(2 * Fp * Dp, we);
+    PH_TRY(product(1, 0, w_ok ? 2 * F : 2 * Fp, w_ok ? D : Dp, M, dtype, dab, 2 * Fp, x, ldx, dw_dtype, q, Dp, c.st));
+    if (!w_ok) PH_TRY(out.add(q, 2 * F, D, Dp, dw_in, 2 * F, D, false));
   }
   if (dw_out) {
-    PH_TRY(product(1, 0, w_ok ? D : Dp, w_ok ? F : Fp, M, dtype, dy, lddy, h, Fp, dw_dtype, w_ok ? dw_out : dwp, Fp, c.st));
-    if (!w_ok) PH_TRY(lay(dw_dtype, dwp, D, F, Fp, dw_out, D, F, false, c.st));
+    void* q = w_ok ? dw_out : c.take(Fp * Dp, we);
+    PH_TRY(product(1, 0, w_ok ? D : Dp, w_ok ? F : Fp, M, dtype, dy, lddy, h, Fp, dw_dtype, q, Fp, c.st));
+    if (!w_ok) PH_TRY(out.add(q, D, F, Fp, dw_out, D, F, false));
   }
-  return PH_OK;
+  return out.run(dw_dtype, c.st);
 }

@@ -1880,25 +1880,25 @@ int pad_operands(PhGemmDesc& d, int vec, hipStream_t st) {
   return PH_OK;
 }
 
-template <int GLU>
+template <int GLU, bool TB>
 int launch_glu(const GemmArgs& g, int dtype, hipStream_t st) {
   auto tiles = [&](long bm, long bn) { return (unsigned)((g.M + bm - 1) / bm * ((g.N + bn - 1) / bn)); };
   if (dtype == PH_BF16) {
     // tiles as for a plain NT product: 256x256 or 256x128 from 512 of 256x128 on, whichever pads the columns less
-    if (tiles(256, 128) >= 512) {
+    if (TB && tiles(256, 128) >= 512) {
       const long n256 = (g.N + 255) / 256 * 256, n128 = (g.N + 127) / 128 * 128;
       if (n256 <= n128 + n128 / 16)
         k_gemm_nt_dma<256, 256, uint16_t, false, 4, 4, 4, false, GLU><<<tiles(256, 256), 1024, 0, st>>>(g);
       else k_gemm_nt_dma<256, 128, uint16_t, false, 2, 2, 3, false, GLU><<<tiles(256, 128), 256, 0, st>>>(g);
     } else if (tiles(128, 128) >= 128) {
-      k_gemm_bf16<128, 128, 64, 2, 2, false, true, uint16_t, uint16_t, uint16_t, false, GLU><<<tiles(128, 128), 256, 0, st>>>(g);
+      k_gemm_bf16<128, 128, 64, 2, 2, false, TB, uint16_t, uint16_t, uint16_t, false, GLU><<<tiles(128, 128), 256, 0, st>>>(g);
     } else {
-      k_gemm_bf16<64, 64, 64, 2, 2, false, true, uint16_t, uint16_t, uint16_t, false, GLU><<<tiles(64, 64), 256, 0, st>>>(g);
+      k_gemm_bf16<64, 64, 64, 2, 2, false, TB, uint16_t, uint16_t, uint16_t, false, GLU><<<tiles(64, 64), 256, 0, st>>>(g);
     }
   } else if (tiles(128, 128) >= 128) {
-    k_gemm_f32<128, 128, 32, false, true, float, GLU><<<tiles(128, 128), 256, 0, st>>>(g);
+    k_gemm_f32<128, 128, 32, false, TB, float, GLU><<<tiles(128, 128), 256, 0, st>>>(g);
   } else {
-    k_gemm_f32<64, 64, 32, false, true, float, GLU><<<tiles(64, 64), 256, 0, st>>>(g);
+    k_gemm_f32<64, 64, 32, false, TB, float, GLU><<<tiles(64, 64), 256, 0, st>>>(g);
   }
   PH_LAUNCH_CHECK();
   return PH_OK;
@@ -1920,10 +1920,10 @@ int glu_product(const GluProduct& p, hipStream_t st) {
   g.remap = 1;
   if (p.grad) {
     g.C = p.dab; g.ldc = p.lddab; g.aux = p.pf; g.ldaux = p.ldpf;
-    return launch_glu<kGluGrad>(g, p.dtype, st);
+    return p.b_kn ? launch_glu<kGluGrad, false>(g, p.dtype, st) : launch_glu<kGluGrad, true>(g, p.dtype, st);
   }
   g.C = p.h; g.ldc = p.ldh; g.C2 = (uint16_t*)p.pf; g.ldc2 = p.ldpf;
-  return launch_glu<kGluUnits>(g, p.dtype, st);
+  return launch_glu<kGluUnits, true>(g, p.dtype, st);
 }
 
 int gemm(const PhGemmDesc& d_in, hipStream_t st) {

@@ -18,13 +18,13 @@ __device__ __forceinline__ void glu_act(int act, float a, float& f, float& df) {
   }
 }
 
-// Product with the gated unit in its epilogue, C[M x N] = A[M x K] B[N x K]^T, all of one type; N, K and the leading
+// Product with the gated unit in its epilogue, C[M x N] = A[M x K] B[N x K]^T (b_kn: B stored [K][N]), all of one type; N, K and the leading
 // dimensions are multiples of 8 and the pointers 16-byte aligned.
 //   grad 0: columns 2j, 2j+1 are unit j's gate and value projections a, v. h[row][j] = act(a) v, and (pf not NULL)
 //           pf[row][2j..] = v act'(a), act(a): what the gradient multiplies dh with, rounded once.
 //   grad 1: the columns are dh; dab[row][2j..] = dh pf[row][2j..], the projections' gradients.
 struct GluProduct {
-  int grad, dtype, act, M, N, K;
+  int grad, dtype, act, M, N, K, b_kn;
   const void* A;
   long lda;
   const void* B;

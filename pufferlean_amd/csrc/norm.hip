@@ -20,10 +20,22 @@ constexpr int kNormRegs = 32;    // values of a row that a lane holds at most: r
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-// V consecutive elements at p as fp32: one 16-byte access for V = 8 (bf16) and V = 4 (fp32), else one element.
-template <int V> __device__ __forceinline__ void load_v(const uint16_t* p, float* v) {
+// V consecutive elements at p as fp32: one 16-byte access for V = 8 (bf16) and V = 4 (fp32), else one element. AL: p is
+// 16-byte aligned, and the row streams past the caches; rows of odd width start anywhere, which the hardware takes at
+// element alignment, and share their lines with their neighbours.
+template <typename T, int V, bool AL> __device__ __forceinline__ u32x4_t load16(const T* p) {
+  u32x4_t r;
+  if constexpr (AL) r = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+  else __builtin_memcpy(&r, p, 16);
+  return r;
+}
+template <typename T, bool AL> __device__ __forceinline__ void store16(T* p, const u32x4_t& r) {
+  if constexpr (AL) __builtin_nontemporal_store(r, reinterpret_cast<u32x4_t*>(p));
+  else __builtin_memcpy(p, &r, 16);
+}
+template <int V, bool AL> __device__ __forceinline__ void load_v(const uint16_t* p, float* v) {
   if constexpr (V == 8) {
-    const u32x4_t r = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+    const u32x4_t r = load16<uint16_t, V, AL>(p);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       v[2 * i] = __builtin_bit_cast(float, r[i] << 16);
@@ -33,33 +45,71 @@ template <int V> __device__ __forceinline__ void load_v(const uint16_t* p, float
     v[0] = bf16_to_f32(*p);
   }
 }
-template <int V> __device__ __forceinline__ void load_v(const float* p, float* v) {
+template <int V, bool AL> __device__ __forceinline__ void load_v(const float* p, float* v) {
   if constexpr (V == 4) {
-    const f32x4_t r = __builtin_nontemporal_load(reinterpret_cast<const f32x4_t*>(p));
+    const u32x4_t r = load16<float, V, AL>(p);
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = r[i];
+    for (int i = 0; i < 4; i++) {
+      const uint32_t u = r[i];  // a bit cast of the vector's element itself takes element 0
+      v[i] = __builtin_bit_cast(float, u);
+    }
   } else {
     v[0] = *p;
   }
 }
-template <int V> __device__ __forceinline__ void store_v(uint16_t* p, const float* v) {
+template <int V, bool AL> __device__ __forceinline__ void store_v(uint16_t* p, const float* v) {
   if constexpr (V == 8) {
     u32x4_t r;
 #pragma unroll
     for (int i = 0; i < 4; i++) r[i] = bf16x2_rne(v[2 * i], v[2 * i + 1]);
-    __builtin_nontemporal_store(r, reinterpret_cast<u32x4_t*>(p));
+    store16<uint16_t, AL>(p, r);
   } else {
     *p = bf16_rne(v[0]);
   }
 }
-template <int V> __device__ __forceinline__ void store_v(float* p, const float* v) {
+template <int V, bool AL> __device__ __forceinline__ void store_v(float* p, const float* v) {
   if constexpr (V == 4) {
-    f32x4_t r;
+    u32x4_t r;
 #pragma unroll
-    for (int i = 0; i < 4; i++) r[i] = v[i];
-    __builtin_nontemporal_store(r, reinterpret_cast<f32x4_t*>(p));
+    for (int i = 0; i < 4; i++) r[i] = __builtin_bit_cast(uint32_t, v[i]);
+    store16<float, AL>(p, r);
   } else {
     *p = v[0];
+  }
+}
+
+// The V columns that a lane holds in its access at column c of a row of C >= V: the last access of a row whose width is no
+// multiple of V is moved back to the row's last V columns, of which it takes those from index `skip` on.
+template <int V> struct Cols {
+  int c, skip;
+  bool in;
+  __device__ __forceinline__ Cols(int at, int C) {
+    in = at < C;
+    c = V > 1 && at + V > C ? C - V : at;
+    skip = at - c;
+  }
+  __device__ __forceinline__ bool has(int i) const { return in && i >= skip; }
+};
+// The access at k of row p, zero where it has no columns; and its store.
+template <int V, bool AL, typename T>
+__device__ __forceinline__ void get_cols(const Cols<V>& k, const T* p, float* v) {
+#pragma unroll
+  for (int i = 0; i < V; i++) v[i] = 0.f;
+  if (k.in) load_v<V, AL>(p + k.c, v);
+  if constexpr (V > 1 && !AL) {
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = i >= k.skip ? v[i] : 0.f;
+  }
+}
+template <int V, bool AL, typename T>
+__device__ __forceinline__ void put_cols(const Cols<V>& k, T* p, const float* v) {
+  if (!k.in) return;
+  if (AL || k.skip == 0) {
+    store_v<V, AL>(p + k.c, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i++)
+      if (i >= k.skip) store_v<1, false>(p + k.c + i, v + i);
   }
 }
 
@@ -72,7 +122,7 @@ template <int LPR> __device__ __forceinline__ float row_sum(float v) {
 // V elements per access, NCH accesses per lane: a row has at most LPR * V * NCH columns. A group of LPR lanes walks the
 // rows group, group + groups, ... with its columns of w and b in registers: loaded again for every row they cost
 // more than the row (262144x512 bf16: 475 us, 115 this way, 4.7 TB/s).
-template <typename T, int V, int NCH, int LPR>
+template <typename T, int V, bool AL, int NCH, int LPR>
 __global__ void __launch_bounds__(64 * kWaves) k_norm_fwd(const T* __restrict__ x, long ldx, long M, int C,
                                                           const float* __restrict__ w, const float* __restrict__ b,
                                                           float eps, T* __restrict__ y, long ldy,
@@ -81,36 +131,32 @@ __global__ void __launch_bounds__(64 * kWaves) k_norm_fwd(const T* __restrict__ 
   const int lr = threadIdx.x % LPR;
   float wv[E], bv[E];
 #pragma unroll
-  for (int q = 0; q < NCH; q++)
+  for (int q = 0; q < NCH; q++) {
+    const Cols<V> k((q * LPR + lr) * V, C);
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      const int c = (q * LPR + lr) * V + i;
-      wv[q * V + i] = c < C && w ? w[c] : 1.f;
-      bv[q * V + i] = c < C && b ? b[c] : 0.f;
+      wv[q * V + i] = k.in && w ? w[k.c + i] : 1.f;
+      bv[q * V + i] = k.in && b ? b[k.c + i] : 0.f;
     }
+  }
   const float inv = 1.f / (float)C;
   // whole groups of LPR lanes leave the loop together; the shuffles stay inside a group
   for (long row = (long)blockIdx.x * GPB + threadIdx.x / LPR; row < M; row += (long)gridDim.x * GPB) {
     float v[E];
     float s = 0.f;
 #pragma unroll
-    for (int q = 0; q < NCH; q++) {
-      const int c = (q * LPR + lr) * V;
-#pragma unroll
-      for (int i = 0; i < V; i++) v[q * V + i] = 0.f;
-      if (c < C) load_v<V>(x + row * ldx + c, v + q * V);
-    }
+    for (int q = 0; q < NCH; q++) get_cols<V, AL>(Cols<V>((q * LPR + lr) * V, C), x + row * ldx, v + q * V);
 #pragma unroll
     for (int i = 0; i < E; i++) s += v[i];
     const float mu = row_sum<LPR>(s) * inv;
     float s2 = 0.f;
 #pragma unroll
     for (int q = 0; q < NCH; q++) {
-      const bool in = (q * LPR + lr) * V < C;
+      const Cols<V> k((q * LPR + lr) * V, C);
 #pragma unroll
       for (int i = 0; i < V; i++) {
         v[q * V + i] -= mu;
-        s2 += in ? v[q * V + i] * v[q * V + i] : 0.f;
+        s2 += (AL ? k.in : k.has(i)) ? v[q * V + i] * v[q * V + i] : 0.f;
       }
     }
     const float r = 1.f / sqrtf(row_sum<LPR>(s2) * inv + eps);
@@ -120,12 +166,10 @@ __global__ void __launch_bounds__(64 * kWaves) k_norm_fwd(const T* __restrict__ 
     }
 #pragma unroll
     for (int q = 0; q < NCH; q++) {
-      const int c = (q * LPR + lr) * V;
-      if (c >= C) continue;
       float o[V];
 #pragma unroll
       for (int i = 0; i < V; i++) o[i] = fmaf(v[q * V + i] * r, wv[q * V + i], bv[q * V + i]);
-      store_v<V>(y + row * ldy + c, o);
+      put_cols<V, AL>(Cols<V>((q * LPR + lr) * V, C), y + row * ldy, o);
     }
   }
 }
@@ -147,13 +191,13 @@ __global__ void __launch_bounds__(256) k_norm_fwd_wide(const T* __restrict__ x, 
   };
   float v, s = 0.f;
   for (int c = threadIdx.x; c < C; c += 256) {
-    load_v<1>(xr + c, &v);
+    load_v<1, false>(xr + c, &v);
     s += v;
   }
   const float mu = total(s, 0) / (float)C;
   s = 0.f;
   for (int c = threadIdx.x; c < C; c += 256) {
-    load_v<1>(xr + c, &v);
+    load_v<1, false>(xr + c, &v);
     s += (v - mu) * (v - mu);
   }
   const float r = 1.f / sqrtf(total(s, 1) / (float)C + eps);
@@ -162,15 +206,15 @@ __global__ void __launch_bounds__(256) k_norm_fwd_wide(const T* __restrict__ x, 
     if (rstd) rstd[row] = r;
   }
   for (int c = threadIdx.x; c < C; c += 256) {
-    load_v<1>(xr + c, &v);
+    load_v<1, false>(xr + c, &v);
     v = (v - mu) * r * (w ? w[c] : 1.f) + (b ? b[c] : 0.f);
-    store_v<1>(y + row * ldy + c, &v);
+    store_v<1, false>(y + row * ldy + c, &v);
   }
 }
 
 // Backward: a group of LPR lanes walks the rows group, group + groups, ...; dw and db of its columns stay in its
 // registers and are added over the block's groups through LDS. part: [blocks][2][C] (or dw, db themselves for one block).
-template <typename T, int V, int NCH, int LPR>
+template <typename T, int V, bool AL, int NCH, int LPR>
 __global__ void __launch_bounds__(64 * kWaves) k_norm_bwd(const T* __restrict__ x, long ldx, const T* __restrict__ dy,
                                                           long lddy, long M, int C, const float* __restrict__ w,
                                                           const float* __restrict__ mean,
@@ -182,32 +226,29 @@ __global__ void __launch_bounds__(64 * kWaves) k_norm_bwd(const T* __restrict__ 
   const int lr = threadIdx.x % LPR, grp = threadIdx.x / LPR;
   float aw[E], ab[E], wv[E];
 #pragma unroll
-  for (int q = 0; q < NCH; q++)
+  for (int q = 0; q < NCH; q++) {
+    const Cols<V> k((q * LPR + lr) * V, C);
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      const int c = (q * LPR + lr) * V + i;
       aw[q * V + i] = ab[q * V + i] = 0.f;
-      wv[q * V + i] = c < C ? (w ? w[c] : 1.f) : 0.f;
+      wv[q * V + i] = k.in ? (w ? w[k.c + i] : 1.f) : 0.f;
     }
+  }
   const float inv = 1.f / (float)C;
   for (long row = (long)blockIdx.x * GPB + grp; row < M; row += (long)gridDim.x * GPB) {
     float n[E], g[E];
 #pragma unroll
     for (int q = 0; q < NCH; q++) {
-      const int c = (q * LPR + lr) * V;
-#pragma unroll
-      for (int i = 0; i < V; i++) n[q * V + i] = g[q * V + i] = 0.f;
-      if (c < C) {
-        load_v<V>(x + row * ldx + c, n + q * V);
-        load_v<V>(dy + row * lddy + c, g + q * V);
-      }
+      const Cols<V> k((q * LPR + lr) * V, C);
+      get_cols<V, AL>(k, x + row * ldx, n + q * V);
+      get_cols<V, AL>(k, dy + row * lddy, g + q * V);
     }
     const float mu = mean[row], r = rstd[row];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < E; i++) {
       n[i] = (n[i] - mu) * r;
-      aw[i] += g[i] * n[i];  // lanes past C add to columns that are never written
+      aw[i] += g[i] * n[i];  // dy is zero where the lane has no column
       ab[i] += g[i];
       g[i] *= wv[i];
       s1 += g[i];
@@ -217,16 +258,14 @@ __global__ void __launch_bounds__(64 * kWaves) k_norm_bwd(const T* __restrict__ 
     s2 = row_sum<LPR>(s2) * inv;
 #pragma unroll
     for (int q = 0; q < NCH; q++) {
-      const int c = (q * LPR + lr) * V;
-      if (c >= C) continue;
       float o[V];
 #pragma unroll
       for (int i = 0; i < V; i++) o[i] = r * (g[q * V + i] - s1 - n[q * V + i] * s2);
-      store_v<V>(dx + row * lddx + c, o);
+      put_cols<V, AL>(Cols<V>((q * LPR + lr) * V, C), dx + row * lddx, o);
     }
   }
   if (!part && !dw && !db) return;
-  // the block's groups, added in group order: one value of every column at a time
+  // the block's groups, added in group order: one access of every lane at a time
   __shared__ float sh[2][GPB][LPR * V];
 #pragma unroll
   for (int q = 0; q < NCH; q++) {
@@ -238,13 +277,15 @@ __global__ void __launch_bounds__(64 * kWaves) k_norm_bwd(const T* __restrict__ 
     }
     __syncthreads();
     for (int e = threadIdx.x; e < 2 * LPR * V; e += 64 * kWaves) {
-      const int k = e / (LPR * V), c = e % (LPR * V), col = q * LPR * V + c;
-      if (col >= C) continue;
-      float s = 0.f;
-      for (int i = 0; i < GPB; i++) s += sh[k][i][c];
-      if (part) part[((long)blockIdx.x * 2 + k) * C + col] = s;
-      else if (k == 0 && dw) dw[col] = s;
-      else if (k == 1 && db) db[col] = s;
+      const int s = e / (LPR * V), l = e % (LPR * V);
+      const Cols<V> k((q * LPR + l / V) * V, C);
+      if (!k.has(l % V)) continue;
+      float sum = 0.f;
+      for (int i = 0; i < GPB; i++) sum += sh[s][i][l];
+      const int col = k.c + l % V;
+      if (part) part[((long)blockIdx.x * 2 + s) * C + col] = sum;
+      else if (s == 0 && dw) dw[col] = sum;
+      else if (s == 1 && db) db[col] = sum;
     }
   }
 }
@@ -259,8 +300,8 @@ __global__ void __launch_bounds__(256) k_norm_bwd_wide(const T* __restrict__ x, 
   const float mu = mean[row], r = rstd[row];
   float s1 = 0.f, s2 = 0.f, a, g;
   for (int c = threadIdx.x; c < C; c += 256) {
-    load_v<1>(x + row * ldx + c, &a);
-    load_v<1>(dy + row * lddy + c, &g);
+    load_v<1, false>(x + row * ldx + c, &a);
+    load_v<1, false>(dy + row * lddy + c, &g);
     g *= w ? w[c] : 1.f;
     s1 += g;
     s2 += g * (a - mu) * r;
@@ -275,10 +316,10 @@ __global__ void __launch_bounds__(256) k_norm_bwd_wide(const T* __restrict__ x, 
   s1 = ((sh[0][0] + sh[0][1]) + (sh[0][2] + sh[0][3])) / (float)C;
   s2 = ((sh[1][0] + sh[1][1]) + (sh[1][2] + sh[1][3])) / (float)C;
   for (int c = threadIdx.x; c < C; c += 256) {
-    load_v<1>(x + row * ldx + c, &a);
-    load_v<1>(dy + row * lddy + c, &g);
+    load_v<1, false>(x + row * ldx + c, &a);
+    load_v<1, false>(dy + row * lddy + c, &g);
     a = r * (g * (w ? w[c] : 1.f) - s1 - (a - mu) * r * s2);
-    store_v<1>(dx + row * lddx + c, &a);
+    store_v<1, false>(dx + row * lddx + c, &a);
   }
 }
 // dw and db partials of wide rows: 64 columns x a range of rows per block of four wavefronts.
@@ -291,8 +332,8 @@ __global__ void __launch_bounds__(256) k_norm_cols_wide(const T* __restrict__ x,
   float sw = 0.f, sb = 0.f, a, g;
   if (c < C)
     for (long row = (long)blockIdx.y * 4 + wave; row < M; row += (long)gridDim.y * 4) {
-      load_v<1>(x + row * ldx + c, &a);
-      load_v<1>(dy + row * lddy + c, &g);
+      load_v<1, false>(x + row * ldx + c, &a);
+      load_v<1, false>(dy + row * lddy + c, &g);
       sw += g * (a - mean[row]) * rstd[row];
       sb += g;
     }
@@ -352,18 +393,18 @@ template <typename T> struct NormCall {
   float *dw, *db;
   hipStream_t st;
 
-  template <int V, int NCH, int LPR> int forward() const {
+  template <int V, bool AL, int NCH, int LPR> int forward() const {
     const long rows = 64 * kWaves / LPR;
     long blocks = (M + rows - 1) / rows;
     if (blocks > 2048) blocks = 2048;  // eight to a CU
-    k_norm_fwd<T, V, NCH, LPR><<<(unsigned)blocks, 64 * kWaves, 0, st>>>(x, ldx, M, C, w, b, eps, y, ldy, mean, rstd);
+    k_norm_fwd<T, V, AL, NCH, LPR><<<(unsigned)blocks, 64 * kWaves, 0, st>>>(x, ldx, M, C, w, b, eps, y, ldy, mean, rstd);
     PH_LAUNCH_CHECK();
     return PH_OK;
   }
-  template <int V, int NCH, int LPR> int backward() const {
+  template <int V, bool AL, int NCH, int LPR> int backward() const {
     const long rows = 64 * kWaves / LPR;
-    // eight rows to a group before there are more blocks: each block's partial row is written, read and added
-    long blocks = (M + 8 * rows - 1) / (8 * rows);
+    // four rows to a group before there are more than 256 blocks: each block's partial row is written, read and added
+    long blocks = (M + 4 * rows - 1) / (4 * rows);
     if (blocks < 256) blocks = (M + rows - 1) / rows < 256 ? (M + rows - 1) / rows : 256;
     if (blocks > 1024) blocks = 1024;
     float* part = nullptr;
@@ -371,7 +412,7 @@ template <typename T> struct NormCall {
       part = (float*)scratch(kSlotNormPart, (size_t)blocks * 2 * C * 4);
       if (!part) return PH_ERR_NOMEM;
     }
-    k_norm_bwd<T, V, NCH, LPR><<<(unsigned)blocks, 64 * kWaves, 0, st>>>(x, ldx, dy, lddy, M, C, w, cmean, crstd, dx,
+    k_norm_bwd<T, V, AL, NCH, LPR><<<(unsigned)blocks, 64 * kWaves, 0, st>>>(x, ldx, dy, lddy, M, C, w, cmean, crstd, dx,
                                                                          lddx, dw, db, part);
     PH_LAUNCH_CHECK();
     if (part) {
@@ -380,7 +421,7 @@ template <typename T> struct NormCall {
     }
     return PH_OK;
   }
-  template <int V, int NCH, int LPR> int go() const { return dy ? backward<V, NCH, LPR>() : forward<V, NCH, LPR>(); }
+  template <int V, bool AL, int NCH, int LPR> int go() const { return dy ? backward<V, AL, NCH, LPR>() : forward<V, AL, NCH, LPR>(); }
   int wide() const {
     if (!dy) {
       k_norm_fwd_wide<T><<<(unsigned)M, 256, 0, st>>>(x, ldx, C, w, b, eps, y, ldy, mean, rstd);
@@ -400,28 +441,27 @@ template <typename T> struct NormCall {
     PH_LAUNCH_CHECK();
     return PH_OK;
   }
-  template <int V> int by_width() const {
-    const int chunks = (C + V - 1) / V;  // accesses of a row
-    if (chunks <= 8) return go<V, 1, 8>();
-    if (chunks <= 16) return go<V, 1, 16>();
-    if (chunks <= 32) return go<V, 1, 32>();
-    if (chunks <= 64) return go<V, 1, 64>();
-    if (chunks <= 128) return go<V, 2, 64>();
-    if (chunks <= 256) return go<V, 4, 64>();
-    if constexpr (8 * V <= kNormRegs) {
-      if (chunks <= 512) return go<V, 8, 64>();
-    }
-    if constexpr (32 * V <= kNormRegs) {
-      if (chunks <= 1024) return go<V, 16, 64>();
-      if (chunks <= 2048) return go<V, 32, 64>();
+  template <int V, bool AL> int by_width() const {
+    const int accesses = (C + V - 1) / V;  // of a row
+    if (accesses <= 8) return go<V, AL, 1, 8>();
+    if constexpr (V > 1) {  // fewer columns than a vector access has: one element per lane and access, 8 lanes
+      if (accesses <= 16) return go<V, AL, 1, 16>();
+      if (accesses <= 32) return go<V, AL, 1, 32>();
+      if (accesses <= 64) return go<V, AL, 1, 64>();
+      if (accesses <= 128) return go<V, AL, 2, 64>();
+      if (accesses <= 256) return go<V, AL, 4, 64>();
+      if constexpr (8 * V <= kNormRegs) {
+        if (accesses <= 512) return go<V, AL, 8, 64>();
+      }
     }
     return wide();
   }
   int run() const {
     constexpr int V = sizeof(T) == 2 ? 8 : 4;
+    if (C < V) return by_width<1, false>();
     auto ok = [&](const void* p, long ld) { return !p || (((uintptr_t)p % 16) == 0 && ld % V == 0); };
-    const bool vec = C % V == 0 && ok(x, ldx) && ok(y, ldy) && ok(dy, lddy) && ok(dx, lddx);
-    return vec ? by_width<V>() : by_width<1>();
+    const bool al = C % V == 0 && ok(x, ldx) && ok(y, ldy) && ok(dy, lddy) && ok(dx, lddx);
+    return al ? by_width<V, true>() : by_width<V, false>();
   }
 };
 
