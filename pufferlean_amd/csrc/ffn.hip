@@ -15,8 +15,6 @@
 #include "glu.hpp"
 #include "kernels.hpp"
 
-#include <type_traits>
-
 namespace ph {
 namespace {
 
@@ -87,86 +85,132 @@ struct Layer {
 
 // ---- few rows --------------------------------------------------------------------------------------------
 // Up to 64 rows are bound by the weights' bytes and by latency, so the weights go from memory straight into the operand
-// registers of 16x16x32 products (16 weight rows to a wavefront, a lane 8 consecutive values of one), with the
-// rows of x as the other operand; the block's wavefronts share the reduction and are added through LDS.
+// registers of 16-wide products (16 weight rows to a wavefront, 16 bytes of one to a lane), with the rows of x as the
+// other operand; the block's wavefronts share the reduction and are added through LDS. fp32 takes four products of
+// 16x16x4 for the four values of a lane: the same k of both operands, in an order of its own.
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 constexpr int kFewRows = 64;
 
-__device__ __forceinline__ bf16x8_t frag(const uint16_t* row, long k, long K) {
-  const uint4 v = k < K ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0u, 0u, 0u, 0u);
-  return __builtin_bit_cast(bf16x8_t, v);
+template <typename T> struct Few;
+template <> struct Few<uint16_t> {
+  static constexpr int kPer = 8;  // k values of a lane
+  typedef bf16x8_t Frag;
+  static __device__ __forceinline__ Frag load(const uint16_t* row, long k, long K) {
+    const uint4 v = k < K ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0u, 0u, 0u, 0u);
+    return __builtin_bit_cast(bf16x8_t, v);
+  }
+  static __device__ __forceinline__ f32x4_t mma(Frag a, Frag b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct Few<float> {
+  static constexpr int kPer = 4;
+  typedef f32x4_t Frag;
+  static __device__ __forceinline__ Frag load(const float* row, long k, long K) {
+    return k < K ? *reinterpret_cast<const f32x4_t*>(row + k) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  static __device__ __forceinline__ f32x4_t mma(Frag a, Frag b, f32x4_t c) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+__device__ __forceinline__ void put(uint16_t* p, float a, float b) { *reinterpret_cast<uint32_t*>(p) = bf16x2_rne(a, b); }
+__device__ __forceinline__ void put(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+__device__ __forceinline__ void get(const uint16_t* p, float& a, float& b) {
+  const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
+  a = __builtin_bit_cast(float, u << 16);
+  b = __builtin_bit_cast(float, u & 0xffff0000u);
 }
-// acc[m][r] = the products of weight rows w0 + 4 (lane / 16) + r and x rows 16 m + lane % 16 over this wavefront's share
-// of k, then summed over the block's WAVES wavefronts: wavefront m < MT returns with block m's in acc[0].
-template <int MT, int WAVES>
-__device__ __forceinline__ void few_rows(f32x4_t (&acc)[MT], const uint16_t* w, long ldw, int w0, int wrows, const uint16_t* x,
-                                         long ldx, int M, long K, float* red) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15;
-  const uint16_t* wr = w + (long)min(w0 + r, wrows - 1) * ldw;
-  const uint16_t* xr[MT];
+__device__ __forceinline__ void get(const float* p, float& a, float& b) {
+  const float2 u = *reinterpret_cast<const float2*>(p);
+  a = u.x;
+  b = u.y;
+}
+__device__ __forceinline__ void put1(uint16_t* p, float a) { *p = bf16_rne(a); }
+__device__ __forceinline__ void put1(float* p, float a) { *p = a; }
+
+// The product of few rows: out[m][n] = sum_k x[m][k] w[n][k]. kIn: n are the projections, out is h (and pf); kGrad: n are
+// units, out is dab, from pf; kPlain: out has N columns. K and the leading dimensions are multiples of 8.
+enum : int { kIn, kGrad, kPlain };
+struct FewArgs {
+  const void *x, *w;
+  long ldx, ldw, K;
+  int M, N, act;
+  void* out;
+  long ldo;
+  void* pf;
+  long ldpf;
+};
+template <typename T, int MODE, int MT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) k_few(FewArgs g) {
+  __shared__ f32x4_t red[WAVES][MT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, w0 = blockIdx.x * 16;
+  const T* wr = (const T*)g.w + (long)min(w0 + r, g.N - 1) * g.ldw;  // rows past N and M repeat the last: not stored
+  const T* xr[MT];
+  f32x4_t acc[MT];
 #pragma unroll
   for (int m = 0; m < MT; m++) {
-    xr[m] = x + (long)min(16 * m + r, M - 1) * ldx;  // rows past M repeat the last; they are not stored
+    xr[m] = (const T*)g.x + (long)min(16 * m + r, g.M - 1) * g.ldx;
     acc[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  const long steps = (K + 31) / 32, per = (steps + WAVES - 1) / WAVES, beg = wave * per, end = min(steps, beg + per);
-  const int ko = 8 * (lane >> 4);
+  constexpr int kPer = Few<T>::kPer, kStep = 4 * kPer;
+  const long steps = (g.K + kStep - 1) / kStep, per = (steps + WAVES - 1) / WAVES, beg = wave * per, end = min(steps, beg + per);
+  const int ko = kPer * (lane >> 4);
 #pragma unroll 4
   for (long s = beg; s < end; s++) {
-    const bf16x8_t a = frag(wr, 32 * s + ko, K);
+    const auto a = Few<T>::load(wr, kStep * s + ko, g.K);
 #pragma unroll
-    for (int m = 0; m < MT; m++)
-      acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, frag(xr[m], 32 * s + ko, K), acc[m], 0, 0, 0);
+    for (int m = 0; m < MT; m++) acc[m] = Few<T>::mma(a, Few<T>::load(xr[m], kStep * s + ko, g.K), acc[m]);
   }
-  f32x4_t* sh = reinterpret_cast<f32x4_t*>(red);  // [WAVES][MT][64]
 #pragma unroll
-  for (int m = 0; m < MT; m++) sh[(wave * MT + m) * 64 + lane] = acc[m];
+  for (int m = 0; m < MT; m++) red[wave][m][lane] = acc[m];
   __syncthreads();
   if (wave >= MT) return;
-  f32x4_t s = sh[wave * 64 + lane];
-  for (int v = 1; v < WAVES; v++) s += sh[(v * MT + wave) * 64 + lane];
-  acc[0] = s;
-}
-
-template <int MT>
-__global__ void __launch_bounds__(256) k_few_in(const uint16_t* __restrict__ x, long ldx, const uint16_t* __restrict__ w, long D,
-                                                int M, int F, int act, uint16_t* __restrict__ h, uint16_t* __restrict__ pf) {
-  __shared__ __attribute__((aligned(16))) float red[4 * MT * 64 * 4];
-  f32x4_t acc[MT];
-  few_rows<MT, 4>(acc, w, D, blockIdx.x * 16, 2 * F, x, ldx, M, D, red);
-  const int lane = threadIdx.x & 63, row = 16 * (threadIdx.x >> 6) + (lane & 15), u = blockIdx.x * 8 + 2 * (lane >> 4);
-  if ((threadIdx.x >> 6) >= MT || row >= M) return;
-  float f0, d0, f1, d1;
-  glu_act(act, acc[0][0], f0, d0);
-  glu_act(act, acc[0][2], f1, d1);
-  *reinterpret_cast<uint32_t*>(h + (long)row * F + u) = bf16x2_rne(f0 * acc[0][1], f1 * acc[0][3]);
-  if (pf)
-    *reinterpret_cast<uint2*>(pf + (long)row * 2 * F + 2 * u) =
-        make_uint2(bf16x2_rne(acc[0][1] * d0, f0), bf16x2_rne(acc[0][3] * d1, f1));
-}
-
-template <int MT>
-__global__ void __launch_bounds__(512) k_few_out(const uint16_t* __restrict__ h, const uint16_t* __restrict__ w, long F, int M, int D,
-                                                 uint16_t* __restrict__ y, long ldy) {
-  __shared__ __attribute__((aligned(16))) float red[8 * MT * 64 * 4];
-  f32x4_t acc[MT];
-  few_rows<MT, 8>(acc, w, F, blockIdx.x * 16, D, h, F, M, F, red);
-  const int lane = threadIdx.x & 63, row = 16 * (threadIdx.x >> 6) + (lane & 15), d = blockIdx.x * 16 + 4 * (lane >> 4);
-  if ((threadIdx.x >> 6) >= MT || row >= M) return;
+  f32x4_t s = red[0][wave][lane];
+  for (int v = 1; v < WAVES; v++) s += red[v][wave][lane];
+  // the lane has columns n..n+3 of one row
+  const int row = 16 * wave + r, n = w0 + 4 * (lane >> 4);
+  if (row >= g.M || n >= g.N) return;
+  T* out = (T*)g.out + (long)row * g.ldo;
+  T* pf = g.pf ? (T*)g.pf + (long)row * g.ldpf : nullptr;
+  if constexpr (MODE == kIn) {
+    float f0, d0, f1, d1;
+    glu_act(g.act, s[0], f0, d0);
+    glu_act(g.act, s[2], f1, d1);
+    put(out + n / 2, f0 * s[1], f1 * s[3]);
+    if (pf) {
+      put(pf + n, s[1] * d0, f0);
+      put(pf + n + 2, s[3] * d1, f1);
+    }
+  } else if constexpr (MODE == kGrad) {
 #pragma unroll
-  for (int r = 0; r < 4; r++)
-    if (d + r < D) y[(long)row * ldy + d + r] = bf16_rne(acc[0][r]);
+    for (int i = 0; i < 4; i++) {
+      float p, f;
+      get(pf + 2 * (n + i), p, f);
+      put(out + 2 * (n + i), s[i] * p, s[i] * f);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (n + i < g.N) put1(out + n + i, s[i]);
+  }
 }
 
-template <int MT>
-int few_rows_ffn(const uint16_t* x, long ldx, const uint16_t* w_in, const uint16_t* w_out, int M, int D, int F, int act,
-                 uint16_t* h, uint16_t* pf, uint16_t* y, long ldy, hipStream_t st) {
-  k_few_in<MT><<<(unsigned)(2 * F / 16), 256, 0, st>>>(x, ldx, w_in, D, M, F, act, h, pf);
-  PH_LAUNCH_CHECK();
-  k_few_out<MT><<<(unsigned)((D + 15) / 16), 512, 0, st>>>(h, w_out, F, M, D, y, ldy);
+template <typename T, int MODE>
+int few_t(const FewArgs& g, hipStream_t st) {
+  const unsigned blocks = (unsigned)((g.N + 15) / 16);
+  if (g.M <= 16) k_few<T, MODE, 1, 8><<<blocks, 512, 0, st>>>(g);
+  else if (g.M <= 32) k_few<T, MODE, 2, 8><<<blocks, 512, 0, st>>>(g);
+  else k_few<T, MODE, 4, 8><<<blocks, 512, 0, st>>>(g);
   PH_LAUNCH_CHECK();
   return PH_OK;
+}
+template <int MODE>
+int few(int dtype, const FewArgs& g, hipStream_t st) {
+  return dtype == PH_BF16 ? few_t<uint16_t, MODE>(g, st) : few_t<float, MODE>(g, st);
 }
 
 int product(int ta, int tb, size_t M, size_t N, size_t K, int dtype, const void* A, size_t lda, const void* B, size_t ldb,
@@ -253,16 +297,14 @@ extern "C" int ph_ffn(int dtype, int act, size_t M, size_t D, size_t F, const vo
   if (!wo_ok) PH_TRY(padded(w_out, D, F, F, D, Fp));
   PH_TRY(lay.run(dtype, c.st));
   if (!h) h = c.take(M * Fp, c.e);
-  if (dtype == PH_BF16 && M <= (size_t)kFewRows && F == Fp) {
-    auto run = [&](auto mt) {
-      return few_rows_ffn<decltype(mt)::value>((const uint16_t*)x, (long)ldx, (const uint16_t*)w_in, (const uint16_t*)w_out, (int)M,
-                                               (int)D, (int)F, act, (uint16_t*)h, (uint16_t*)pf, (uint16_t*)y, (long)ldy, c.st);
-    };
-    if (D == Dp) {
-      if (M <= 16) return run(std::integral_constant<int, 1>{});
-      if (M <= 32) return run(std::integral_constant<int, 2>{});
-      return run(std::integral_constant<int, 4>{});
-    }
+  if (M <= (size_t)kFewRows) {
+    FewArgs g{};
+    g.x = x; g.ldx = (long)ldx; g.w = w_in; g.ldw = g.K = (long)Dp; g.M = (int)M; g.N = (int)(2 * Fp); g.act = act;
+    g.out = h; g.ldo = (long)Fp; g.pf = pf; g.ldpf = (long)(2 * Fp);
+    PH_TRY(few<kIn>(dtype, g, c.st));
+    FewArgs o{};
+    o.x = h; o.ldx = (long)Fp; o.w = w_out; o.ldw = o.K = (long)Fp; o.M = (int)M; o.N = (int)D; o.out = y; o.ldo = (long)ldy;
+    return few<kPlain>(dtype, o, c.st);
   }
   GluProduct g{};
   g.dtype = dtype; g.act = act; g.M = (int)M; g.N = (int)(2 * Fp); g.K = (int)Dp;
@@ -287,8 +329,9 @@ extern "C" int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, con
   const size_t Dp = c.Dp, Fp = c.Fp, we = dw_dtype == PH_BF16 ? 2 : 4;
   const bool x_ok = c.whole(x, ldx, D, Dp), dy_ok = c.whole(dy, lddy, D, Dp), w_ok = D == Dp && F == Fp;
   // Transposed copies of the weights, so that both products read their operands along k: with many rows the products
-  // are faster by more than the copies take. With few rows the products take the weights as they are (or padded).
-  const bool trans = M >= kTransposeRows;
+  // are faster by more than the copies take, and the kernel of few rows has no other form. In between the products
+  // take the weights as they are (or padded).
+  const bool few_rows = M <= (size_t)kFewRows, trans = M >= kTransposeRows || few_rows;
   const bool wo_ok = !trans && c.whole(w_out, F, F, Fp) && D == Dp, wi_ok = !trans && c.whole(w_in, D, D, Dp) && F == Fp;
   const bool need_dab = dx || dw_in;
   if (!x_ok && dw_in) c.want(M * Dp, c.e);
@@ -322,14 +365,23 @@ extern "C" int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, con
     dab = c.take(M * 2 * Fp, c.e);
   }
   PH_TRY(lay.run(dtype, c.st));
-  if (need_dab) {
+  if (need_dab && few_rows) {
+    FewArgs g{};
+    g.x = dy; g.ldx = (long)lddy; g.w = w_out; g.ldw = g.K = (long)Dp; g.M = (int)M; g.N = (int)Fp; g.out = dab; g.ldo = (long)(2 * Fp);
+    g.pf = const_cast<void*>(pf); g.ldpf = (long)(2 * Fp);
+    PH_TRY(few<kGrad>(dtype, g, c.st));
+  } else if (need_dab) {
     GluProduct g{};
     g.grad = 1; g.dtype = dtype; g.act = act; g.M = (int)M; g.N = (int)Fp; g.K = (int)Dp; g.b_kn = !trans;
     g.A = dy; g.lda = (long)lddy; g.B = w_out; g.ldb = (long)(trans ? Dp : Fp);
     g.pf = const_cast<void*>(pf); g.ldpf = (long)(2 * Fp); g.dab = dab; g.lddab = (long)(2 * Fp);
     PH_TRY(glu_product(g, c.st));
   }
-  if (dx) PH_TRY(product(0, trans, M, D, 2 * Fp, dtype, dab, 2 * Fp, w_in, trans ? 2 * Fp : Dp, dtype, dx, lddx, c.st));
+  if (dx && few_rows) {
+    FewArgs g{};
+    g.x = dab; g.ldx = (long)(2 * Fp); g.w = w_in; g.ldw = g.K = (long)(2 * Fp); g.M = (int)M; g.N = (int)D; g.out = dx; g.ldo = (long)lddx;
+    PH_TRY(few<kPlain>(dtype, g, c.st));
+  } else if (dx) PH_TRY(product(0, trans, M, D, 2 * Fp, dtype, dab, 2 * Fp, w_in, trans ? 2 * Fp : Dp, dtype, dx, lddx, c.st));
   // the weights' gradients; of padded operands through a padded copy
   Layer out;
   if (dw_in) {

@@ -10,6 +10,7 @@
 // which leaves one partial row per block for a second, small launch to add in a fixed order.
 #include "common.hpp"
 #include "kernels.hpp"
+#include "lanes.hpp"
 
 namespace ph {
 namespace {
@@ -113,10 +114,18 @@ __device__ __forceinline__ void put_cols(const Cols<V>& k, T* p, const float* v)
   }
 }
 
-template <int LPR> __device__ __forceinline__ float row_sum(float v) {
+// The columns of w (or b) that a lane holds, 16 bytes at a time.
+template <int V>
+__device__ __forceinline__ void get_weights(const Cols<V>& k, const float* w, float none, float* v) {
 #pragma unroll
-  for (int m = 1; m < LPR; m <<= 1) v += __shfl_xor(v, m);
-  return v;
+  for (int i = 0; i < V; i++) v[i] = none;
+  if (!w || !k.in) return;
+  if constexpr (V >= 4) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) load_v<4, false>(w + k.c + i, v + i);
+  } else {
+    v[0] = w[k.c];
+  }
 }
 
 // V elements per access, NCH accesses per lane: a row has at most LPR * V * NCH columns. A group of LPR lanes walks the
@@ -133,11 +142,8 @@ __global__ void __launch_bounds__(64 * kWaves) k_norm_fwd(const T* __restrict__ 
 #pragma unroll
   for (int q = 0; q < NCH; q++) {
     const Cols<V> k((q * LPR + lr) * V, C);
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-      wv[q * V + i] = k.in && w ? w[k.c + i] : 1.f;
-      bv[q * V + i] = k.in && b ? b[k.c + i] : 0.f;
-    }
+    get_weights<V>(k, w, 1.f, wv + q * V);
+    get_weights<V>(k, b, 0.f, bv + q * V);
   }
   const float inv = 1.f / (float)C;
   // whole groups of LPR lanes leave the loop together; the shuffles stay inside a group
@@ -148,7 +154,7 @@ __global__ void __launch_bounds__(64 * kWaves) k_norm_fwd(const T* __restrict__ 
     for (int q = 0; q < NCH; q++) get_cols<V, AL>(Cols<V>((q * LPR + lr) * V, C), x + row * ldx, v + q * V);
 #pragma unroll
     for (int i = 0; i < E; i++) s += v[i];
-    const float mu = row_sum<LPR>(s) * inv;
+    const float mu = group_sum<LPR>(s) * inv;
     float s2 = 0.f;
 #pragma unroll
     for (int q = 0; q < NCH; q++) {
@@ -159,7 +165,7 @@ __global__ void __launch_bounds__(64 * kWaves) k_norm_fwd(const T* __restrict__ 
         s2 += (AL ? k.in : k.has(i)) ? v[q * V + i] * v[q * V + i] : 0.f;
       }
     }
-    const float r = 1.f / sqrtf(row_sum<LPR>(s2) * inv + eps);
+    const float r = 1.f / sqrtf(group_sum<LPR>(s2) * inv + eps);
     if (lr == 0) {
       if (mean) mean[row] = mu;
       if (rstd) rstd[row] = r;
@@ -184,7 +190,7 @@ __global__ void __launch_bounds__(256) k_norm_fwd_wide(const T* __restrict__ x, 
   const long row = blockIdx.x;
   const T* xr = x + row * ldx;
   auto total = [&](float v, int k) {
-    v = row_sum<64>(v);
+    v = group_sum<64>(v);
     if ((threadIdx.x & 63) == 0) sh[k][threadIdx.x >> 6] = v;
     __syncthreads();
     return (sh[k][0] + sh[k][1]) + (sh[k][2] + sh[k][3]);
@@ -227,12 +233,9 @@ __global__ void __launch_bounds__(64 * kWaves) k_norm_bwd(const T* __restrict__ 
   float aw[E], ab[E], wv[E];
 #pragma unroll
   for (int q = 0; q < NCH; q++) {
-    const Cols<V> k((q * LPR + lr) * V, C);
+    get_weights<V>(Cols<V>((q * LPR + lr) * V, C), w, 1.f, wv + q * V);
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-      aw[q * V + i] = ab[q * V + i] = 0.f;
-      wv[q * V + i] = k.in ? (w ? w[k.c + i] : 1.f) : 0.f;
-    }
+    for (int i = 0; i < V; i++) aw[q * V + i] = ab[q * V + i] = 0.f;
   }
   const float inv = 1.f / (float)C;
   for (long row = (long)blockIdx.x * GPB + grp; row < M; row += (long)gridDim.x * GPB) {
@@ -254,8 +257,9 @@ __global__ void __launch_bounds__(64 * kWaves) k_norm_bwd(const T* __restrict__ 
       s1 += g[i];
       s2 += g[i] * n[i];
     }
-    s1 = row_sum<LPR>(s1) * inv;
-    s2 = row_sum<LPR>(s2) * inv;
+    group_sum<LPR>(s1, s2);
+    s1 *= inv;
+    s2 *= inv;
 #pragma unroll
     for (int q = 0; q < NCH; q++) {
       float o[V];
@@ -306,8 +310,8 @@ __global__ void __launch_bounds__(256) k_norm_bwd_wide(const T* __restrict__ x, 
     s1 += g;
     s2 += g * (a - mu) * r;
   }
-  s1 = row_sum<64>(s1);
-  s2 = row_sum<64>(s2);
+  s1 = group_sum<64>(s1);
+  s2 = group_sum<64>(s2);
   if ((threadIdx.x & 63) == 0) {
     sh[0][threadIdx.x >> 6] = s1;
     sh[1][threadIdx.x >> 6] = s2;
@@ -396,7 +400,8 @@ template <typename T> struct NormCall {
   template <int V, bool AL, int NCH, int LPR> int forward() const {
     const long rows = 64 * kWaves / LPR;
     long blocks = (M + rows - 1) / rows;
-    if (blocks > 2048) blocks = 2048;  // eight to a CU
+    const long most = NCH * V > 8 ? 1024 : 2048;  // as many as run at a time: rows of 512 columns and more take more registers
+    if (blocks > most) blocks = most;
     k_norm_fwd<T, V, AL, NCH, LPR><<<(unsigned)blocks, 64 * kWaves, 0, st>>>(x, ldx, M, C, w, b, eps, y, ldy, mean, rstd);
     PH_LAUNCH_CHECK();
     return PH_OK;

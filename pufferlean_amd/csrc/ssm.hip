@@ -22,6 +22,7 @@
 // chunks again from those.
 #include "common.hpp"
 #include "kernels.hpp"
+#include "lanes.hpp"
 
 #include <type_traits>
 
@@ -588,19 +589,6 @@ struct GradArgs {
 // wavefront halves, then rows of 16 lanes, then lanes eight apart. step_sums takes the eight steps' partials and
 // leaves in lane l the total of value l / 8 at step l % 8. Together under 20 instructions a step, where eight
 // separate sums would take 48.
-// Two registers with one's upper and the other's lower wavefront half (or odd and even rows of 16 lanes) exchanged, two pairs
-// at a time: their sum then holds the first value's total in one half and the second's in the other. As asm: the
-// compiler's builtins return the first register for both. The exchange may not read a register in the two wait
-// states after vector arithmetic wrote it, hence the s_nop.
-__device__ __forceinline__ void swap32(float& a0, float& b0, float& a1, float& b1) {
-  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\tv_permlane32_swap_b32 %2, %3" : "+v"(a0), "+v"(b0), "+v"(a1), "+v"(b1));
-}
-__device__ __forceinline__ void swap16(float& a0, float& b0, float& a1, float& b1) {
-  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\tv_permlane16_swap_b32 %2, %3" : "+v"(a0), "+v"(b0), "+v"(a1), "+v"(b1));
-}
-template <int CTL> __device__ __forceinline__ float dpp_mov(float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTL, 0xF, 0xF, true));
-}
 template <int CTL> __device__ __forceinline__ float fold_dpp(float lo, float hi, bool up) {
   return (up ? hi : lo) + dpp_mov<CTL>(up ? lo : hi);
 }
@@ -1102,12 +1090,17 @@ int block_threads(const Args& a, bool grad) {
 }
 static_assert(4 * (12 * 16 * 64 + 3 * 64 * 16 + 3 * kSteps) <= 64 * 1024, "one wavefront at N = 64");
 
-// Chunks of time: enough wavefronts for every SIMD to hold two, in chunks of at least 32 steps. Chunks cost a second pass
-// over their steps and three launches (about 20 us each way), so sequences stay whole while one pass over all their
-// steps is not longer than that: up to 128 steps of 16 states, the more the fewer the states.
+// Blocks of nt threads that run at a time in the gradient: two wavefronts to a SIMD, whole blocks to a CU.
+long resident(int nt) { return 256L * (8 / (nt / 64)); }
+
+// Chunks of time: as many as make one round of blocks, in chunks of at least 32 steps (2048x8, two groups of 192 channels: a
+// chunk more and a second round gave 401 us both directions). Chunks cost a second pass over their steps and three
+// launches (about 20 us each way), so sequences stay whole while one pass over all their steps is not longer than that:
+// up to 128 steps of 16 states, the more the fewer the states.
 int set_chunks(Args& a) {
+  const int nt = block_threads(a, true);
   const long waves = a.B * a.G * ((a.per + 63) / 64);
-  long want = (2048 + waves - 1) / waves;
+  long want = resident(nt) / (a.B * a.G * ((a.per + nt - 1) / nt));
   const long most = (a.T + 31) / 32;
   if (want > most) want = most;
   if (want < 1 || (long)a.T * (8 + a.N) <= 128 * (8 + 16)) want = 1;
@@ -1269,10 +1262,10 @@ extern "C" int ph_ssm_scan_grad(const ph_ssm_args* p, const float* keep, const v
   const int nt = block_threads(a, true);
   const long G = a.G, bc = (a.per + nt - 1) / nt;
   a.blocks_c = (unsigned)bc;
-  // blocks of a channel block: a few for every CU, each with many items of its own
-  const long items = a.B * a.chunks;
-  ga.rows = 512 / (G * bc);
-  if (ga.rows > items) ga.rows = items;
+  // blocks of a channel block: as many as run at a time, with as equal shares of the items as there are
+  const long items = a.B * a.chunks, most = resident(nt) / (G * bc) > 0 ? resident(nt) / (G * bc) : 1;
+  const long rounds = (items + most - 1) / most;
+  ga.rows = (items + rounds - 1) / rounds;
   if (ga.rows < 1) ga.rows = 1;
   const size_t nh = a.chunks > 1 ? (size_t)a.chunks * a.B * a.C * 4 * a.Q : 0, nd = a.chunks > 1 ? (size_t)a.chunks * a.B * a.C : 0;
   const size_t nhalo = a.chunks > 1 ? (size_t)(2 * a.chunks) * a.B * (kTaps - 1) * a.C : 0;
