@@ -1094,16 +1094,17 @@ static_assert(4 * (12 * 16 * 64 + 3 * 64 * 16 + 3 * kSteps) <= 64 * 1024, "one w
 long resident(int nt) { return 256L * (8 / (nt / 64)); }
 
 // Chunks of time: as many as make one round of blocks, in chunks of at least 32 steps (2048x8, two groups of 192 channels: a
-// chunk more and a second round gave 401 us both directions). Chunks cost a second pass over their steps and three
-// launches (about 20 us each way), so sequences stay whole while one pass over all their steps is not longer than that:
-// up to 128 steps of 16 states, the more the fewer the states.
-int set_chunks(Args& a) {
+// chunk more and a second round gave 401 us both directions, 361 without). Chunks cost a second pass over their steps and
+// three launches (about 20 us), so sequences stay whole while one pass over all their steps is not longer than that: up
+// to 128 steps of 16 states forward, 64 in the gradient, whose steps take three times as long; the more the fewer the
+// states. (33 steps of 203x96x5 fp32 both directions: 104 us in two chunks, 84 whole.)
+int set_chunks(Args& a, bool grad) {
   const int nt = block_threads(a, true);
   const long waves = a.B * a.G * ((a.per + 63) / 64);
   long want = resident(nt) / (a.B * a.G * ((a.per + nt - 1) / nt));
   const long most = (a.T + 31) / 32;
   if (want > most) want = most;
-  if (want < 1 || (long)a.T * (8 + a.N) <= 128 * (8 + 16)) want = 1;
+  if (want < 1 || (long)a.T * (8 + a.N) <= (grad ? 64 : 128) * (8 + 16)) want = 1;
   a.chunk = (a.T + want - 1) / want;
   a.chunk = (a.chunk + kSteps - 1) / kSteps * kSteps;
   a.chunks = (a.T + a.chunk - 1) / a.chunk;
@@ -1222,7 +1223,7 @@ extern "C" int ph_ssm_scan(const ph_ssm_args* p, void* y, long y_t, long y_b, fl
   hipStream_t st = as_stream(stream);
   Args a = args_of(*p);
   a.y = y; a.y_t = y_t; a.y_b = y_b; a.h_out = h_out; a.keep = keep;
-  PH_TRY(set_chunks(a));
+  PH_TRY(set_chunks(a, false));
   a.win_out = a.K > 1 ? win_out : nullptr;
   // with several chunks the first one may still read the window that the last would overwrite
   a.win_here = a.win_out && (a.chunks == 1 || a.win_out != a.win0);
@@ -1250,7 +1251,7 @@ extern "C" int ph_ssm_scan_grad(const ph_ssm_args* p, const float* keep, const v
   PH_REQUIRE(p->T >= 1, "ssm_scan_grad: no steps");
   PH_REQUIRE(dy && keep, "ssm_scan_grad: dy or the kept states missing");
   Args a = args_of(*p);
-  PH_TRY(set_chunks(a));
+  PH_TRY(set_chunks(a, true));
   GradArgs ga{};
   ga.dy = dy; ga.dy_t = dy_t; ga.dy_b = dy_b; ga.keep = keep;
   ga.dx = g->dx; ga.dx_t = g->dx_t; ga.dx_b = g->dx_b;
