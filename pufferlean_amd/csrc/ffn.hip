@@ -226,6 +226,26 @@ int product(int ta, int tb, size_t M, size_t N, size_t K, int dtype, const void*
 // Rows from which the backward's products take transposed weights.
 constexpr size_t kTransposeRows = 2048;
 
+// A weight's gradient A^T B over the M rows. A few hundred tiles of 64x64 at most, each a long sum, leave the chip idle or its
+// blocks without company: enough splits for six blocks to a CU, of 256 rows at least (fp32 1072x208x6699 90 -> 57 us,
+// 208x536x6699 45 -> 35, 2752x512x4096 258 -> 157). bf16 keeps gemm()'s own choice (3592 rows, 2208x384 and 384x1104: 54 us, 66
+// this way).
+int weight_grad(size_t rows, size_t cols, size_t M, int dtype, const void* A, size_t lda, const void* B, size_t ldb, int c_dtype,
+                void* C, hipStream_t st) {
+  PhGemmDesc d{};
+  d.trans_a = 1; d.M = (int)rows; d.N = (int)cols; d.K = (int)M;
+  d.a_dtype = d.b_dtype = dtype; d.A = A; d.lda = (long)lda; d.B = B; d.ldb = (long)ldb;
+  d.c_dtype = c_dtype; d.C = C; d.ldc = (long)cols;
+  d.math = dtype == PH_BF16 ? PH_MATH_BF16 : PH_MATH_F32;
+  const long tiles = (long)((rows + 63) / 64) * (long)((cols + 63) / 64);
+  if (dtype == PH_F32 && M >= 512 && tiles < 768) {
+    const long want = (1536 + tiles - 1) / tiles, most = (long)M / 256;
+    d.splits = (int)(want < most ? want : most);
+    d.small_tiles = 1;
+  }
+  return gemm(d, st);
+}
+
 // One call's sizes, and its scratch handed out in pieces of 256 bytes.
 struct Call {
   int dtype, act;
@@ -386,12 +406,12 @@ extern "C" int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, con
   Layer out;
   if (dw_in) {
     void* q = w_ok ? dw_in : c.take(2 * Fp * Dp, we);
-    PH_TRY(product(1, 0, w_ok ? 2 * F : 2 * Fp, w_ok ? D : Dp, M, dtype, dab, 2 * Fp, x, ldx, dw_dtype, q, Dp, c.st));
+    PH_TRY(weight_grad(w_ok ? 2 * F : 2 * Fp, w_ok ? D : Dp, M, dtype, dab, 2 * Fp, x, ldx, dw_dtype, q, c.st));
     if (!w_ok) PH_TRY(out.add(q, 2 * F, D, Dp, dw_in, 2 * F, D, false));
   }
   if (dw_out) {
     void* q = w_ok ? dw_out : c.take(Fp * Dp, we);
-    PH_TRY(product(1, 0, w_ok ? D : Dp, w_ok ? F : Fp, M, dtype, dy, lddy, h, Fp, dw_dtype, q, Fp, c.st));
+    PH_TRY(weight_grad(w_ok ? D : Dp, w_ok ? F : Fp, M, dtype, dy, lddy, h, Fp, dw_dtype, q, c.st));
     if (!w_ok) PH_TRY(out.add(q, D, F, Fp, dw_out, D, F, false));
   }
   return out.run(dw_dtype, c.st);

@@ -1895,7 +1895,9 @@ int launch_glu(const GemmArgs& g, int dtype, hipStream_t st) {
     } else {
       k_gemm_bf16<64, 64, 64, 2, 2, false, TB, uint16_t, uint16_t, uint16_t, false, GLU><<<tiles(64, 64), 256, 0, st>>>(g);
     }
-  } else if (tiles(128, 128) >= 128) {
+  } else if (tiles(128, 128) >= 512) {
+    // two blocks of 128x128 to a CU; below that 64x64 tiles, four to a CU, keep more of the chip at work (6699x536x208: 49 us
+    // in 265 tiles of 128x128, 30 in 64x64; 6699x1072x208, 477 tiles: 48 either way)
     k_gemm_f32<128, 128, 32, false, TB, float, GLU><<<tiles(128, 128), 256, 0, st>>>(g);
   } else {
     k_gemm_f32<64, 64, 32, false, TB, float, GLU><<<tiles(64, 64), 256, 0, st>>>(g);
@@ -2023,6 +2025,7 @@ int gemm(const PhGemmDesc& d_in, hipStream_t st) {
       if (splits < 1) splits = 1;
     }
   }
+  if (d.small_tiles && d.splits > 0) small = true;
   const int BK = 64;  // split granularity: a multiple of every k-tile in use
   int kps = (d.K + splits - 1) / splits;
   kps = (kps + BK - 1) / BK * BK;

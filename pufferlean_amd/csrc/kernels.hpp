@@ -105,6 +105,7 @@ struct PhGemmDesc {
   long ldc2;
   int c2_trans;
   int splits;   // <= 0: chosen by shape
+  int small_tiles;  // with a given number of splits: 64x64 tiles instead of 128x128
   int ws_slot;  // scratch slot of the split-K partials (0: the shared default slot)
   const void* aux2;  // second epilogue operand (kEpiGateSkip)
   long ldaux2;

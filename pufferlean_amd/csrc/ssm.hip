@@ -69,13 +69,14 @@ __device__ __forceinline__ void stf(gout<uint16_t> p, float v) { *p = bf16_rne(v
 __device__ __forceinline__ void stf(gout<float> p, float v) { *p = v; }
 
 __device__ __forceinline__ float ex2(float v) { return __builtin_amdgcn_exp2f(v); }
-// softplus without cancellation: with w = 1 + e rounded, log(w) e / (w - 1) is log(1 + e) to a few ulp for every e.
+// softplus, max(v, 0) + log(1 + e) with e = exp(-|v|). What rounding 1 + e to w dropped, e - (w - 1), is added back as it is
+// (its share of the logarithm is that over w, and it is nothing but where w is near 1), so small e keep their digits.
 __device__ __forceinline__ float softplus(float v) {
-  const float e = __expf(-fabsf(v)), w = 1.f + e;
-  const float l = w == 1.f ? e : __logf(w) * (e * __builtin_amdgcn_rcpf(w - 1.f));
-  return fmaxf(v, 0.f) + l;
+  const float e = ex2(-fabsf(v) * kLog2e), w = 1.f + e;
+  return fmaxf(v, 0.f) + fmaf(__builtin_amdgcn_logf(w), 1.f / kLog2e, e - (w - 1.f));
 }
-__device__ __forceinline__ float silu(float v) { return v * sigm(v); }
+__device__ __forceinline__ float sigma(float v) { return __builtin_amdgcn_rcpf(1.f + ex2(v * -kLog2e)); }
+__device__ __forceinline__ float silu(float v) { return v * sigma(v); }
 // d/dv of v sigma(v), s = sigma(v)
 __device__ __forceinline__ float dsilu(float v, float s) { return s * fmaf(v, 1.f - s, 1.f); }
 
@@ -232,6 +233,7 @@ struct Rows {
       if constexpr (sizeof(T) == 2) v[i] = p[c];
       else v[i] = __builtin_bit_cast(uint32_t, p[c]);
       walk(p, i + 1 < steps ? stride : 0);
+      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // or the addresses of all rows of a batch are made first
     }
   }
   __device__ __forceinline__ float operator[](int i) const {
@@ -892,10 +894,10 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
         for (int i = kSteps - 1; i >= 0; i--) {
           if (!decltype(CLEAN)::value && i >= steps) continue;
           float x1, x2, x3;
-          const float pre = conv(CLEAN, i, x1, x2, x3), sg = sigm(pre), w = pre * sg, u = K ? w : rx[i];
+          const float pre = conv(CLEAN, i, x1, x2, x3), sg = sigma(pre), w = pre * sg, u = K ? w : rx[i];
           const float gb = fmaf(dout[i], cb2[i], gB[i]);
-          ddt[i] = fmaf(u, gb, Aq[i] * (1.f / kLog2e)) * sigm(rd[i] + bias);
-          dzv[i] = rg[i] * fmaf(du[i], cb2[i], fmaf(Dc, u, o[i])) * dsilu(rz[i], sigm(rz[i]));
+          ddt[i] = fmaf(u, gb, Aq[i] * (1.f / kLog2e)) * sigma(rd[i] + bias);
+          dzv[i] = rg[i] * fmaf(du[i], cb2[i], fmaf(Dc, u, o[i])) * dsilu(rz[i], sigma(rz[i]));
           const float dus = fmaf(d[i], gb, Dc * dout[i]), ds = dus * dsilu(pre, sg);
           dD = fmaf(dout[i], u, dD);
           dbias += ddt[i];
