@@ -65,6 +65,8 @@ __device__ __forceinline__ float ldf(gin<uint16_t> p) { return bf16_to_f32(*p); 
 __device__ __forceinline__ float ldf(gin<float> p) { return *p; }
 __device__ __forceinline__ float ldf(const uint16_t* p) { return ldf((gin<uint16_t>)p); }
 __device__ __forceinline__ float ldf(const float* p) { return ldf((gin<float>)p); }
+__device__ __forceinline__ float raw_f32(float v) { return v; }
+__device__ __forceinline__ float raw_f32(uint16_t v) { return bf16_to_f32(v); }
 __device__ __forceinline__ void stf(gout<uint16_t> p, float v) { *p = bf16_rne(v); }
 __device__ __forceinline__ void stf(gout<float> p, float v) { *p = v; }
 
@@ -181,7 +183,7 @@ struct StageBC {
   gin<T> p[kMost];     // of step 0
   long stride[kMost];
   int step[kMost];     // of the batch; past it for no value
-  float v[kMost];
+  T v[kMost];          // as loaded
   __device__ __forceinline__ void init(const Args& a, long b, unsigned g) {
 #pragma unroll
     for (int k = 0; k < kMost; k++) {
@@ -195,14 +197,14 @@ struct StageBC {
   }
   __device__ __forceinline__ void get(int t0, int steps) {
 #pragma unroll
-    for (int k = 0; k < kMost; k++) v[k] = step[k] < steps ? ldf(p[k] + (long)(t0 + step[k]) * stride[k]) : 0.f;
+    for (int k = 0; k < kMost; k++) v[k] = step[k] < steps ? p[k][(long)(t0 + step[k]) * stride[k]] : T(0);
   }
   __device__ __forceinline__ void put(const Args& a, float* s) const {
     const int tot = kSteps * 8 * a.Q;
 #pragma unroll
     for (int k = 0; k < kMost; k++) {
       const int e = threadIdx.x + k * blockDim.x;
-      if (e < tot) s[e] = v[k];
+      if (e < tot) s[e] = raw_f32(v[k]);
     }
   }
 };
@@ -223,21 +225,21 @@ __device__ __forceinline__ f4t decay4(const Args& a, unsigned c, int q) {
   return f4(v.x * kLog2e, v.y * kLog2e, v.z * kLog2e, v.w * kLog2e);
 }
 
-// Raw rows of a batch, loaded a batch ahead; steps past the end repeat the last one.
+// Raw rows of a batch, loaded a batch ahead; steps past the end repeat the last one. They stay what the load gives, in T:
+// anything done to a value where it is loaded, a widening too, would wait for it there.
 template <typename T>
 struct Rows {
-  uint32_t v[kSteps];  // the bits: a bf16 value's, or an fp32's
+  T v[kSteps];
   __device__ __forceinline__ void get(gin<T> p, long stride, int steps, unsigned c) {
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
-      if constexpr (sizeof(T) == 2) v[i] = p[c];
-      else v[i] = __builtin_bit_cast(uint32_t, p[c]);
+      v[i] = p[c];
       walk(p, i + 1 < steps ? stride : 0);
       if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // or the addresses of all rows of a batch are made first
     }
   }
   __device__ __forceinline__ float operator[](int i) const {
-    return __builtin_bit_cast(float, sizeof(T) == 2 ? v[i] << 16 : v[i]);
+    return raw_f32(v[i]);
   }
   // From here on the compiler takes the values as new: what is computed from them again is not kept from before.
   __device__ __forceinline__ void renew() {
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
   gout<T> yp = (gout<T>)a.y + b * a.y_b + tbeg * a.y_t;
   const long quads = a.B * Q * a.C;  // quads of the library's states of one chunk (or kept batch)
   gout<f4t> keep = LOCAL || !a.keep ? nullptr : (gout<f4t>)a.keep + tbeg / kSteps * quads + b * Q * a.C;
-  Rows<T> rx, rd, rz;
+  Rows<T> rx, rd, rz = {};
   StageBC<T, MOST> bc;
   bc.init(a, b, pl.g);
   float fl, back[kTaps - 1];
@@ -294,10 +296,7 @@ __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
     bc.get(t0, n);
     rx.get(xp, a.x_t, n, c);
     rd.get(dp, a.d_t, n, c);
-    if (!LOCAL) {
-      if (a.z) rz.get(zp, a.z_t, n, c);
-      else rz = rx;  // not looked at
-    }
+    if (!LOCAL && a.z) rz.get(zp, a.z_t, n, c);
     fl = flag_load(a, t0, tend, b);
     walk(xp, kSteps * a.x_t);
     walk(dp, kSteps * a.d_t);
@@ -332,16 +331,17 @@ __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
     if (t0 + kSteps < tend) fetch(t0 + kSteps);
     cleared |= st;
     float d[kSteps], du[kSteps], o[kSteps];
-    // CLEAN: a whole batch that no episode's start cuts; the other form selects what each step sees. Without a convolution or
-    // gate theirs are computed all the same and not taken: a choice per step would split the batch into many short blocks.
+    // CLEAN: a whole batch that no episode's start cuts, of a convolution of all taps; the other form selects what each step
+    // sees. Without a convolution or gate theirs are computed all the same and not taken: a choice per step would split
+    // the batch into many short blocks.
     auto prepare = [&](auto CLEAN) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < kSteps; i++) {
-        const int n = decltype(CLEAN)::value ? cv.K - 1 : cv.reach(bits, i);
+        const int n = decltype(CLEAN)::value ? kTaps - 1 : cv.reach(bits, i);
         const float x1 = i > 0 ? cx[i > 0 ? i - 1 : 0] : back[2], x2 = i > 1 ? cx[i > 1 ? i - 2 : 0] : back[i + 1],
                     x3 = i > 2 ? cx[i > 2 ? i - 3 : 0] : back[i];
         const float w = silu(cv.pre(cx[i], n > 0 ? x1 : 0.f, n > 1 ? x2 : 0.f, n > 2 ? x3 : 0.f));
-        const float u = cv.K ? w : cx[i];
+        const float u = decltype(CLEAN)::value || cv.K ? w : cx[i];
         d[i] = softplus(cd[i] + bias);
         du[i] = d[i] * u;
         if (!decltype(CLEAN)::value) {
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
         o[i] = Dc * u;
       }
     };
-    if (bits == 0 && steps == kSteps) prepare(std::true_type{});
+    if (bits == 0 && steps == kSteps && cv.K == kTaps) prepare(std::true_type{});
     else prepare(std::false_type{});
 #pragma unroll
     for (int j = 0; j < kTaps - 1; j++) back[j] = cx[kSteps - (kTaps - 1) + j];
@@ -631,7 +631,7 @@ __global__ void __launch_bounds__(256) k_ssm_bwd_local(Args a, GradArgs ga) {
   const float bias = a.dt_bias ? a.dt_bias[c] : 0.f;
   float dsum = 0.f;
   unsigned cleared = 0;
-  Rows<T> rd, rz, rg;
+  Rows<T> rd, rz = {}, rg;
   StageBC<T, MOST> bc;
   bc.init(a, b, pl.g);
   float fl;
@@ -703,7 +703,7 @@ __global__ void __launch_bounds__(256) k_ssm_bwd_join(Args a, GradArgs ga) {
 // the staging computes once per step. Sums over channels are folded over the wavefront's lanes, then over the
 // block's wavefronts in LDS; the parameters' gradients stay in LDS and registers over all the block's work. A block
 // takes the items row, row + rows, ... of its channel block, an item being a chunk of a sequence.
-template <typename T>
+template <typename T, int MOST>
 __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int Q = a.Q, nt = blockDim.x, tid = threadIdx.x;
@@ -731,60 +731,109 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
   float dD = 0.f, dbias = 0.f, dcb = 0.f, dw[kTaps] = {};
   const int K = cv.K;
   const long quads = a.B * Q * a.C;
+  // What a batch reads: the rows, the three inputs before them, the flags, the first kept states and this thread's share of B
+  // and C, as loaded. The next batch's are on their way while a batch computes its channels' own gradients, where the
+  // registers of the states' steps are free again.
+  struct Where {
+    unsigned b, s;
+    int tbeg, tend, t0;
+  };
+  auto enter = [&](unsigned item) __attribute__((always_inline)) {  // the last batch of an item
+    Where w;
+    w.b = uniform(item % (unsigned)a.B);
+    w.s = uniform(item / (unsigned)a.B);
+    w.tbeg = (int)w.s * a.chunk;
+    w.tend = min(a.T, w.tbeg + a.chunk);
+    w.t0 = w.tbeg + (w.tend - w.tbeg - 1) / kSteps * kSteps;
+    return w;
+  };
+  Rows<T> rx, rd, rz = {}, rg;
+  T before[kTaps - 1] = {}, vbc[MOST];
+  float fl;
+  f4t next;
+  auto fetch = [&](const Where& w) __attribute__((always_inline)) {
+    const long b = w.b;
+    const int t0 = w.t0, steps = min(kSteps, w.tend - t0);
+    int me = tid;
+    asm("" : "+v"(me));  // or the places of all MOST values wait in registers over the states' steps
+#pragma unroll
+    for (int k = 0; k < MOST; k++) {
+      const int e = me + k * nt, n = place_state(e), i = place_step(e);
+      const bool is_c = place_row(e);
+      gin<T> p = is_c ? (gin<T>)a.Cm + b * a.cm_b : (gin<T>)a.Bm + b * a.bm_b;
+      vbc[k] = n < a.N && i < steps ? p[(long)(t0 + i) * (is_c ? a.cm_t : a.bm_t) + grp * a.N + n] : T(0);
+    }
+    fl = flag_load(a, t0, w.tend, b);
+    rx.get((gin<T>)a.x + b * a.x_b + t0 * a.x_t, a.x_t, steps, c);
+    if (t0 > 0) {
+#pragma unroll
+      for (int j = 0; j < kTaps - 1; j++) before[j] = ((gin<T>)a.x + b * a.x_b + (t0 - (kTaps - 1) + j) * a.x_t)[c];
+    }
+    rd.get((gin<T>)a.delta + b * a.d_b + t0 * a.d_t, a.d_t, steps, c);
+    if (a.z) rz.get((gin<T>)a.z + b * a.z_b + t0 * a.z_t, a.z_t, steps, c);
+    rg.get((gin<T>)ga.dy + b * ga.dy_b + t0 * ga.dy_t, ga.dy_t, steps, c);
+    next = ((gin<f4t>)ga.keep + t0 / kSteps * quads + b * Q * a.C)[c];
+  };
   int buf = 0;
-  for (unsigned item = row; item < items; item += (unsigned)ga.rows) {
-    const long b = uniform(item % (unsigned)a.B), s = uniform(item / (unsigned)a.B);
-    const int tbeg = (int)s * a.chunk, tend = min(a.T, tbeg + a.chunk);
-    {
+  unsigned item = row;
+  if (item >= items) return;  // (a block without work: the launch has none)
+  Where at = enter(item);
+  fetch(at);
+  // ds of the three steps after the current one, of the same episode (zero past the chunk: its successor's
+  // share of this chunk's last steps comes through the halo)
+  float q1 = 0.f, q2 = 0.f, q3 = 0.f;
+  for (;; buf ^= 1) {
+    const long b = at.b, s = at.s;
+    const int tbeg = at.tbeg, tend = at.tend, t0 = at.t0;
+    if (t0 + kSteps >= tend) {
+      q1 = q2 = q3 = 0.f;
       gin<f4t> carry = (gin<f4t>)ga.carry + s * quads + b * Q * a.C;
       for (int q = 0; q < Q; q++)  // a lane without a channel sends nothing back, and so adds nothing to a sum
         sG[q * nt + tid] = a.chunks > 1 && in ? (carry + q * a.C)[c] : f4(0.f, 0.f, 0.f, 0.f);
     }
-    // ds of the three steps after the current one, of the same episode (zero past the chunk: its successor's
-    // share of this chunk's last steps comes through the halo)
-    float q1 = 0.f, q2 = 0.f, q3 = 0.f;
-    for (int t0 = tbeg + (tend - tbeg - 1) / kSteps * kSteps; t0 >= tbeg; t0 -= kSteps, buf ^= 1) {
+    Where to = at;  // the batch after this one
+    to.t0 = t0 - kSteps;
+    bool more = true;
+    if (t0 == tbeg) {
+      item += (unsigned)ga.rows;
+      more = item < items;
+      if (more) to = enter(item);
+    }
+    {
       const int steps = min(kSteps, tend - t0);
-      Rows<T> rx, rd, rz, rg;
-      float back[kTaps - 1];
-      rx.get((gin<T>)a.x + b * a.x_b + t0 * a.x_t, a.x_t, steps, c);
-      rd.get((gin<T>)a.delta + b * a.d_b + t0 * a.d_t, a.d_t, steps, c);
-      if (a.z) rz.get((gin<T>)a.z + b * a.z_b + t0 * a.z_t, a.z_t, steps, c);
-      else rz = rx;  // not looked at
-      rg.get((gin<T>)ga.dy + b * ga.dy_b + t0 * ga.dy_t, ga.dy_t, steps, c);
-      look_back<T>(back, a, t0, b, c);
       gin<f4t> keep = (gin<f4t>)ga.keep + t0 / kSteps * quads + b * Q * a.C;
-      f4t next = keep[c];
-      const unsigned bits = flag_bits(flag_load(a, t0, tend, b)), st = bits >> (kTaps - 1);
-      // stage B and C
-      float* sb = sbc + buf * 64 * Q;
-      for (int e = tid; e < 64 * Q; e += nt) {
-        const int n = place_state(e), i = place_step(e);
-        float v = 0.f;
-        if (n < a.N && i < steps)
-          v = place_row(e) ? ldf((gin<T>)a.Cm + (t0 + i) * a.cm_t + b * a.cm_b + grp * a.N + n)
-                           : ldf((gin<T>)a.Bm + (t0 + i) * a.bm_t + b * a.bm_b + grp * a.N + n);
-        sb[e] = v;
+      Rows<T> cx = rx, cd = rd, cz = rz, cg = rg;
+      float back[kTaps - 1];
+      if (t0 > 0) {
+#pragma unroll
+        for (int j = 0; j < kTaps - 1; j++) back[j] = raw_f32(before[j]);
+      } else {
+        look_back<T>(back, a, 0, b, c);
       }
+      const unsigned bits = flag_bits(fl), st = bits >> (kTaps - 1);
+      float* sb = sbc + buf * 64 * Q;
+#pragma unroll
+      for (int k = 0; k < MOST; k++)
+        if (tid + k * nt < 64 * Q) sb[tid + k * nt] = raw_f32(vbc[k]);
       // Input j (0..10) of the batch and of the three steps before it, and a step's own convolution. CLEAN as in the forward.
-      auto input = [&](int j) __attribute__((always_inline)) { return j < kTaps - 1 ? back[j < kTaps - 1 ? j : 0] : rx[j < kTaps - 1 ? 0 : j - (kTaps - 1)]; };
+      auto input = [&](int j) __attribute__((always_inline)) { return j < kTaps - 1 ? back[j < kTaps - 1 ? j : 0] : cx[j < kTaps - 1 ? 0 : j - (kTaps - 1)]; };
       auto conv = [&](auto CLEAN, int i, float& x1, float& x2, float& x3) __attribute__((always_inline)) {
-        const int n = decltype(CLEAN)::value ? K - 1 : cv.reach(bits, i);
+        const int n = decltype(CLEAN)::value ? kTaps - 1 : cv.reach(bits, i);
         x1 = n > 0 ? input(i + 2) : 0.f;
         x2 = n > 1 ? input(i + 1) : 0.f;
         x3 = n > 2 ? input(i) : 0.f;
-        return cv.pre(rx[i], x1, x2, x3);
+        return cv.pre(cx[i], x1, x2, x3);
       };
-      const bool clean = bits == 0 && steps == kSteps;
+      const bool clean = bits == 0 && steps == kSteps && K == kTaps;
       float d[kSteps], du[kSteps], dout[kSteps], o[kSteps], gB[kSteps], Aq[kSteps];
       auto prepare = [&](auto CLEAN) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < kSteps; i++) {
           float x1, x2, x3;
-          const float w = silu(conv(CLEAN, i, x1, x2, x3)), u = K ? w : rx[i], gated = rg[i] * silu(rz[i]);
-          d[i] = softplus(rd[i] + bias);
+          const float w = silu(conv(CLEAN, i, x1, x2, x3)), u = decltype(CLEAN)::value || K ? w : cx[i], gated = cg[i] * silu(cz[i]);
+          d[i] = softplus(cd[i] + bias);
           du[i] = d[i] * u;
-          dout[i] = a.z ? gated : rg[i];
+          dout[i] = a.z ? gated : cg[i];
           if (!decltype(CLEAN)::value) {
             // a step past the end neither decays, nor takes nor gives
             d[i] = i < steps ? d[i] : 0.f;
@@ -865,6 +914,7 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
         if ((lane & 7) == 0) reds[wave * kSteps + (lane >> 3)] = S;
       }
       __syncthreads();
+      if (more) fetch(to);
       // the block's sums over its wavefronts, in order
       for (int e = tid; e < 64 * Q; e += nt) {
         const int i = place_step(e), which = place_row(e), n = place_state(e);
@@ -881,9 +931,9 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
         else if (!which && ga.dB) stf((gout<T>)ga.dB + t * ga.db_t + b * ga.db_b + grp * a.N + n, sum);
       }
       // the channel's own gradients
-      rx.renew();
-      rd.renew();
-      rz.renew();
+      cx.renew();
+      cd.renew();
+      cz.renew();
       const int last = t0 + steps - 1;
       float cb2[kSteps];
 #pragma unroll
@@ -894,24 +944,24 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
         for (int i = kSteps - 1; i >= 0; i--) {
           if (!decltype(CLEAN)::value && i >= steps) continue;
           float x1, x2, x3;
-          const float pre = conv(CLEAN, i, x1, x2, x3), sg = sigma(pre), w = pre * sg, u = K ? w : rx[i];
+          const float pre = conv(CLEAN, i, x1, x2, x3), sg = sigma(pre), w = pre * sg, u = decltype(CLEAN)::value || K ? w : cx[i];
           const float gb = fmaf(dout[i], cb2[i], gB[i]);
-          ddt[i] = fmaf(u, gb, Aq[i] * (1.f / kLog2e)) * sigma(rd[i] + bias);
-          dzv[i] = rg[i] * fmaf(du[i], cb2[i], fmaf(Dc, u, o[i])) * dsilu(rz[i], sigma(rz[i]));
+          ddt[i] = fmaf(u, gb, Aq[i] * (1.f / kLog2e)) * sigma(cd[i] + bias);
+          dzv[i] = cg[i] * fmaf(du[i], cb2[i], fmaf(Dc, u, o[i])) * dsilu(cz[i], sigma(cz[i]));
           const float dus = fmaf(d[i], gb, Dc * dout[i]), ds = dus * dsilu(pre, sg);
           dD = fmaf(dout[i], u, dD);
           dbias += ddt[i];
           dcb += ds;
-          dw[3] = fmaf(ds, rx[i], dw[3]);
+          dw[3] = fmaf(ds, cx[i], dw[3]);
           dw[2] = fmaf(ds, x1, dw[2]);
           dw[1] = fmaf(ds, x2, dw[1]);
           dw[0] = fmaf(ds, x3, dw[0]);
           const float dc = fmaf(cv.w[3], ds, fmaf(cv.w[2], q1, fmaf(cv.w[1], q2, cv.w[0] * q3)));
-          dxv[i] = K ? dc : dus;
+          dxv[i] = decltype(CLEAN)::value || K ? dc : dus;
           const bool cut = !decltype(CLEAN)::value && (st & (1u << i));
-          q3 = cut || K < 4 ? 0.f : q2;
-          q2 = cut || K < 3 ? 0.f : q1;
-          q1 = cut || K < 2 ? 0.f : ds;
+          q3 = cut || (!decltype(CLEAN)::value && K < 4) ? 0.f : q2;
+          q2 = cut || (!decltype(CLEAN)::value && K < 3) ? 0.f : q1;
+          q1 = cut || (!decltype(CLEAN)::value && K < 2) ? 0.f : ds;
         }
       };
       if (clean) finish(std::true_type{});
@@ -953,13 +1003,15 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
       }
     }
     // what this chunk adds to dx of the K - 1 steps before it: step tbeg - 1 - j takes ds of up to K - 1 - j steps on
-    if (in && K > 1 && s > 0 && ga.dx) {
+    if (t0 == tbeg && in && K > 1 && s > 0 && ga.dx) {
       const float hq[kTaps - 1] = {fmaf(cv.w[2], q1, fmaf(cv.w[1], q2, cv.w[0] * q3)), fmaf(cv.w[1], q1, cv.w[0] * q2),
                                    cv.w[0] * q1};
 #pragma unroll
       for (int j = 0; j < kTaps - 1; j++)
         if (j < K - 1) ga.halo[(((s * 2 - 1) * a.B + b) * (kTaps - 1) + j) * a.C + c] = hq[j];
     }
+    if (!more) break;
+    at = to;
   }
   if (in && ga.par) {
     float* p = ga.par + ((long)row * a.C + c) * ga.P;
@@ -1142,9 +1194,9 @@ int fwd_t(Args& a, hipStream_t st) {
 
 template <typename T>
 int bwd_t(Args& a, GradArgs& ga, int nt, const ParOut& po, hipStream_t st) {
+  const int most = (kSteps * 8 * a.Q + nt - 1) / nt;
   if (a.chunks > 1) {
     const unsigned blocks = (unsigned)(a.chunks * a.B * a.G * a.blocks_c);
-    const int most = (kSteps * 8 * a.Q + nt - 1) / nt;
     if (most <= 1) k_ssm_bwd_local<T, 1><<<blocks, nt, fwd_lds(a.Q, nt), st>>>(a, ga);
     else if (most <= 4) k_ssm_bwd_local<T, 4><<<blocks, nt, fwd_lds(a.Q, nt), st>>>(a, ga);
     else k_ssm_bwd_local<T, 16><<<blocks, nt, fwd_lds(a.Q, nt), st>>>(a, ga);
@@ -1152,7 +1204,10 @@ int bwd_t(Args& a, GradArgs& ga, int nt, const ParOut& po, hipStream_t st) {
     k_ssm_bwd_join<<<ceil_div((size_t)(a.B * a.C * 4 * a.Q), 256), 256, 0, st>>>(a, ga);
     PH_LAUNCH_CHECK();
   }
-  k_ssm_bwd<T><<<(unsigned)(ga.rows * a.G * a.blocks_c), nt, bwd_lds(a.Q, nt), st>>>(a, ga);
+  const unsigned blocks = (unsigned)(ga.rows * a.G * a.blocks_c);
+  if (most <= 1) k_ssm_bwd<T, 1><<<blocks, nt, bwd_lds(a.Q, nt), st>>>(a, ga);
+  else if (most <= 4) k_ssm_bwd<T, 4><<<blocks, nt, bwd_lds(a.Q, nt), st>>>(a, ga);
+  else k_ssm_bwd<T, 16><<<blocks, nt, bwd_lds(a.Q, nt), st>>>(a, ga);
   PH_LAUNCH_CHECK();
   if (a.chunks > 1 && a.K > 1 && ga.dx) {
     k_ssm_halo<T><<<ceil_div((size_t)((a.chunks - 1) * a.B * (a.K - 1) * a.C), 256), 256, 0, st>>>(a, ga);
