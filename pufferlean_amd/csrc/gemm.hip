@@ -1582,6 +1582,9 @@ __global__ void __launch_bounds__(256) k_gemm_f32(GemmArgs g) {
       rb[c] = v;
     }
   };
+  // An operand that is transposed into LDS is written in 4-byte stores of 16 rows apart by 4 (a bank apart by 16 each) and four
+  // k: its groups of four k change places by the row's bits 4 and 5, so that a wavefront's store meets every bank once.
+  auto swz = [](int r, int k) { return k ^ ((r >> 4 & 3) << 2); };
   auto sstore = [&](int s) {
 #pragma unroll
     for (int c = 0; c < CA; c++) {
@@ -1590,11 +1593,11 @@ __global__ void __launch_bounds__(256) k_gemm_f32(GemmArgs g) {
         const int r = id / (BK / 4), k = (id % (BK / 4)) * 4;
         *reinterpret_cast<float4*>(&sA[s][r * LDK + k]) = ra[c];
       } else {
-        const int k = id / (BM / 4), r = (id % (BM / 4)) * 4;
-        sA[s][(r + 0) * LDK + k] = ra[c].x;
-        sA[s][(r + 1) * LDK + k] = ra[c].y;
-        sA[s][(r + 2) * LDK + k] = ra[c].z;
-        sA[s][(r + 3) * LDK + k] = ra[c].w;
+        const int k = id / (BM / 4), r = (id % (BM / 4)) * 4, at = swz(r, k);
+        sA[s][(r + 0) * LDK + at] = ra[c].x;
+        sA[s][(r + 1) * LDK + at] = ra[c].y;
+        sA[s][(r + 2) * LDK + at] = ra[c].z;
+        sA[s][(r + 3) * LDK + at] = ra[c].w;
       }
     }
 #pragma unroll
@@ -1604,11 +1607,11 @@ __global__ void __launch_bounds__(256) k_gemm_f32(GemmArgs g) {
         const int r = id / (BK / 4), k = (id % (BK / 4)) * 4;
         *reinterpret_cast<float4*>(&sB[s][r * LDK + k]) = rb[c];
       } else {
-        const int k = id / (BN / 4), r = (id % (BN / 4)) * 4;
-        sB[s][(r + 0) * LDK + k] = rb[c].x;
-        sB[s][(r + 1) * LDK + k] = rb[c].y;
-        sB[s][(r + 2) * LDK + k] = rb[c].z;
-        sB[s][(r + 3) * LDK + k] = rb[c].w;
+        const int k = id / (BN / 4), r = (id % (BN / 4)) * 4, at = swz(r, k);
+        sB[s][(r + 0) * LDK + at] = rb[c].x;
+        sB[s][(r + 1) * LDK + at] = rb[c].y;
+        sB[s][(r + 2) * LDK + at] = rb[c].z;
+        sB[s][(r + 3) * LDK + at] = rb[c].w;
       }
     }
   };
@@ -1635,9 +1638,9 @@ __global__ void __launch_bounds__(256) k_gemm_f32(GemmArgs g) {
     for (int kb = 0; kb < BK; kb += 8) {
       float4 a[SM], b[SN];
 #pragma unroll
-      for (int i = 0; i < SM; i++) a[i] = *reinterpret_cast<const float4*>(&sA[s][(wm0 + i * 32 + lr) * LDK + kb + lk]);
+      for (int i = 0; i < SM; i++) a[i] = *reinterpret_cast<const float4*>(&sA[s][(wm0 + i * 32 + lr) * LDK + (TA ? swz(lr + i * 32 + wm0, kb + lk) : kb + lk)]);
 #pragma unroll
-      for (int j = 0; j < SN; j++) b[j] = *reinterpret_cast<const float4*>(&sB[s][(wn0 + j * 32 + lr) * LDK + kb + lk]);
+      for (int j = 0; j < SN; j++) b[j] = *reinterpret_cast<const float4*>(&sB[s][(wn0 + j * 32 + lr) * LDK + (!TB ? swz(lr + j * 32 + wn0, kb + lk) : kb + lk)]);
 #pragma unroll
       for (int i = 0; i < SM; i++)
 #pragma unroll
@@ -1896,11 +1899,12 @@ int launch_glu(const GemmArgs& g, int dtype, hipStream_t st) {
       k_gemm_bf16<64, 64, 64, 2, 2, false, TB, uint16_t, uint16_t, uint16_t, false, GLU><<<tiles(64, 64), 256, 0, st>>>(g);
     }
   } else if (tiles(128, 128) >= 512) {
-    // two blocks of 128x128 to a CU; below that 64x64 tiles, four to a CU, keep more of the chip at work (6699x536x208: 49 us
-    // in 265 tiles of 128x128, 30 in 64x64; 6699x1072x208, 477 tiles: 48 either way)
+    // two blocks of 128x128 to a CU; below that 64x64 tiles keep more of the chip at work (6699x536x208: 49 us in 265 tiles of
+    // 128x128, 31 in 64x64; 6699x1072x208, 477 tiles: 48, 45 in 64x64). Their k tiles of 16 let eight blocks share a CU's
+    // LDS and waste less of a short K (6699x1072x208 at k tiles of 32: 50 us).
     k_gemm_f32<128, 128, 32, false, TB, float, GLU><<<tiles(128, 128), 256, 0, st>>>(g);
   } else {
-    k_gemm_f32<64, 64, 32, false, TB, float, GLU><<<tiles(64, 64), 256, 0, st>>>(g);
+    k_gemm_f32<64, 64, 16, false, TB, float, GLU><<<tiles(64, 64), 256, 0, st>>>(g);
   }
   PH_LAUNCH_CHECK();
   return PH_OK;
