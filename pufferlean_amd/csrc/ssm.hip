@@ -141,12 +141,37 @@ __device__ __forceinline__ void look_back(float (&x)[kTaps - 1], const Args& a, 
   }
 }
 
+// A lane's place in uniform rows of T. A 32-bit byte offset beside a scalar base is an address that loads and stores take as
+// it is; but the compiler widens the offset once, outside the loops, and then adds in 64 bits for every row. What comes out of
+// the empty asm it has to widen where it is used.
+template <typename T>
+struct Lane {
+  unsigned o;
+  __device__ __forceinline__ explicit Lane(unsigned c) : o(c * (unsigned)sizeof(T)) { asm("" : "+v"(o)); }
+  __device__ __forceinline__ gin<T> operator()(gin<T> row) const { return (gin<T>)((gin<char>)row + o); }
+  __device__ __forceinline__ gout<T> operator()(gout<T> row) const { return (gout<T>)((gout<char>)row + o); }
+};
+
 // A uniform row pointer that walks over steps. The empty asm keeps the walk a chain of scalar additions: without it the
 // compiler forms the addresses of all of a batch's rows at once, hundreds of scalar registers that it then spills.
 template <typename P>
 __device__ __forceinline__ void walk(P& p, long d) {
   p += d;
   asm("" : "+s"(p));
+}
+
+// The kernel's own arguments, read again from where the launch put them: Args first, GradArgs behind. The compiler reads
+// arguments once, at the kernel's start, and what the scalar registers cannot hold over the loops it keeps in lanes of
+// vector registers, an instruction of each wavefront for every word it takes back.
+template <typename A>
+__device__ __forceinline__ A again(unsigned at) {
+  static_assert(sizeof(A) % 8 == 0 && alignof(A) == 8, "read in words of eight bytes");
+  auto p = (const __attribute__((address_space(4))) uint64_t*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm("" : "+s"(p));
+  uint64_t w[sizeof(A) / 8];
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(A) / 8; i++) w[i] = p[at / 8 + i];
+  return __builtin_bit_cast(A, w);
 }
 
 // A value that every lane holds, in a scalar register (a division leaves its result in vector ones).
@@ -231,11 +256,20 @@ template <typename T>
 struct Rows {
   T v[kSteps];
   __device__ __forceinline__ void get(gin<T> p, long stride, int steps, unsigned c) {
+    const Lane<T> at(c);
+    if (steps == kSteps) {
 #pragma unroll
-    for (int i = 0; i < kSteps; i++) {
-      v[i] = p[c];
-      walk(p, i + 1 < steps ? stride : 0);
-      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // or the addresses of all rows of a batch are made first
+      for (int i = 0; i < kSteps; i++) {
+        v[i] = *at(p);
+        walk(p, stride);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSteps; i++) {
+        v[i] = *at(p);
+        walk(p, i + 1 < steps ? stride : 0);
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // or the addresses of all rows of a batch are made first
+      }
     }
   }
   __device__ __forceinline__ float operator[](int i) const {
@@ -361,7 +395,7 @@ __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
       for (int q = 0; q < Q; q++) {
         const f4t A = sA[q * nt + tid];
         f4t h = sH[q * nt + tid];
-        if (!LOCAL && keep && pl.in) (keep + q * a.C)[c] = h;
+        if (!LOCAL && keep && pl.in) *Lane<f4t>(c)(keep + q * a.C) = h;
 #pragma unroll
         for (int i = 0; i < kSteps; i++) {
           if constexpr (decltype(ANY)::value) {
@@ -394,9 +428,10 @@ __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
       if (pl.in) {
         if (steps == kSteps) {
           gout<T> p = yp;
+          const Lane<T> at(c);
 #pragma unroll
           for (int i = 0; i < kSteps; i++) {
-            stf(p + c, o[i]);
+            stf(at(p), o[i]);
             walk(p, a.y_t);
           }
         } else {
@@ -752,6 +787,8 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
   float fl;
   f4t next;
   auto fetch = [&](const Where& w) __attribute__((always_inline)) {
+    const Args a = again<Args>(0);
+    const GradArgs ga = again<GradArgs>(sizeof(Args));
     const long b = w.b;
     const int t0 = w.t0, steps = min(kSteps, w.tend - t0);
     int me = tid;
@@ -766,13 +803,18 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
     fl = flag_load(a, t0, w.tend, b);
     rx.get((gin<T>)a.x + b * a.x_b + t0 * a.x_t, a.x_t, steps, c);
     if (t0 > 0) {
+      gin<T> p = (gin<T>)a.x + b * a.x_b + (t0 - (kTaps - 1)) * a.x_t;
+      const Lane<T> at(c);
 #pragma unroll
-      for (int j = 0; j < kTaps - 1; j++) before[j] = ((gin<T>)a.x + b * a.x_b + (t0 - (kTaps - 1) + j) * a.x_t)[c];
+      for (int j = 0; j < kTaps - 1; j++) {
+        before[j] = *at(p);
+        walk(p, a.x_t);
+      }
     }
     rd.get((gin<T>)a.delta + b * a.d_b + t0 * a.d_t, a.d_t, steps, c);
     if (a.z) rz.get((gin<T>)a.z + b * a.z_b + t0 * a.z_t, a.z_t, steps, c);
     rg.get((gin<T>)ga.dy + b * ga.dy_b + t0 * ga.dy_t, ga.dy_t, steps, c);
-    next = ((gin<f4t>)ga.keep + t0 / kSteps * quads + b * Q * a.C)[c];
+    next = *Lane<f4t>(c)((gin<f4t>)ga.keep + t0 / kSteps * quads + b * Q * a.C);
   };
   int buf = 0;
   unsigned item = row;
@@ -856,7 +898,7 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
       auto scan = [&](auto ANY) __attribute__((always_inline)) {  // ANY: an episode starts in this batch
         for (int q = 0; q < Q; q++) {
           const f4t A = sA[q * nt + tid], kh = next;
-          next = (keep + (q + 1 < Q ? q + 1 : q) * a.C)[c];
+          next = *Lane<f4t>(c)(keep + (q + 1 < Q ? q + 1 : q) * a.C);
           const f4t g4 = sG[q * nt + tid];
           const float Av[4] = {A.x, A.y, A.z, A.w};
           float h[4] = {kh.x, kh.y, kh.z, kh.w}, g[4] = {g4.x, g4.y, g4.z, g4.w}, dA[4] = {};
@@ -915,10 +957,12 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
       }
       __syncthreads();
       if (more) fetch(to);
+      const Args aa = again<Args>(0);
+      const GradArgs gg = again<GradArgs>(sizeof(Args));
       // the block's sums over its wavefronts, in order
       for (int e = tid; e < 64 * Q; e += nt) {
         const int i = place_step(e), which = place_row(e), n = place_state(e);
-        if (n >= a.N || i >= steps) continue;
+        if (n >= aa.N || i >= steps) continue;
         float sum = 0.f, S = 0.f;
         for (int w = 0; w < waves; w++) {
           sum += red[w * 64 * Q + e];
@@ -926,9 +970,9 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
         }
         sum = fmaf(sb[e ^ 4], S, sum);
         const long t = t0 + i;
-        if (ga.bc) ga.bc[((((long)cb * a.T + t) * a.B + b) * a.G + grp) * 2 * a.N + which * a.N + n] = sum;
-        else if (which && ga.dC) stf((gout<T>)ga.dC + t * ga.dc_t + b * ga.dc_b + grp * a.N + n, sum);
-        else if (!which && ga.dB) stf((gout<T>)ga.dB + t * ga.db_t + b * ga.db_b + grp * a.N + n, sum);
+        if (gg.bc) gg.bc[((((long)cb * aa.T + t) * aa.B + b) * aa.G + grp) * 2 * aa.N + which * aa.N + n] = sum;
+        else if (which && gg.dC) stf((gout<T>)gg.dC + t * gg.dc_t + b * gg.dc_b + grp * aa.N + n, sum);
+        else if (!which && gg.dB) stf((gout<T>)gg.dB + t * gg.db_t + b * gg.db_b + grp * aa.N + n, sum);
       }
       // the channel's own gradients
       cx.renew();
@@ -939,10 +983,10 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
 #pragma unroll
       for (int i = 0; i < kSteps; i++) cb2[i] = scb[buf * kSteps + i];
       float dxv[kSteps], ddt[kSteps], dzv[kSteps];
-      auto finish = [&](auto CLEAN) __attribute__((always_inline)) {
+      auto finish = [&](auto CLEAN, auto WHOLE) __attribute__((always_inline)) {  // WHOLE: no step is past the end
 #pragma unroll
         for (int i = kSteps - 1; i >= 0; i--) {
-          if (!decltype(CLEAN)::value && i >= steps) continue;
+          if (!decltype(WHOLE)::value && i >= steps) continue;
           float x1, x2, x3;
           const float pre = conv(CLEAN, i, x1, x2, x3), sg = sigma(pre), w = pre * sg, u = decltype(CLEAN)::value || K ? w : cx[i];
           const float gb = fmaf(dout[i], cb2[i], gB[i]);
@@ -964,27 +1008,29 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
           q1 = cut || (!decltype(CLEAN)::value && K < 2) ? 0.f : ds;
         }
       };
-      if (clean) finish(std::true_type{});
-      else finish(std::false_type{});
+      if (clean) finish(std::true_type{}, std::true_type{});
+      else if (steps == kSteps) finish(std::false_type{}, std::true_type{});
+      else finish(std::false_type{}, std::false_type{});
       if (in) {
         // the last K - 1 steps of a chunk that has a successor are finished by the halo's launch
-        const bool halo = tend < a.T && t0 + kSteps >= tend && K > 1;
-        if (steps == kSteps && !halo && ga.ddelta && ga.dx) {
-          gout<T> pd = (gout<T>)ga.ddelta + b * ga.dd_b + t0 * ga.dd_t;
-          gout<T> px = (gout<T>)ga.dx + b * ga.dx_b + t0 * ga.dx_t;
+        const bool halo = tend < aa.T && t0 + kSteps >= tend && K > 1;
+        if (steps == kSteps && !halo && gg.ddelta && gg.dx) {
+          gout<T> pd = (gout<T>)gg.ddelta + b * gg.dd_b + t0 * gg.dd_t;
+          gout<T> px = (gout<T>)gg.dx + b * gg.dx_b + t0 * gg.dx_t;
+          const Lane<T> at(c);
 #pragma unroll
           for (int i = 0; i < kSteps; i++) {
-            stf(pd + c, ddt[i]);
-            stf(px + c, dxv[i]);
-            walk(pd, ga.dd_t);
-            walk(px, ga.dx_t);
+            stf(at(pd), ddt[i]);
+            stf(at(px), dxv[i]);
+            walk(pd, gg.dd_t);
+            walk(px, gg.dx_t);
           }
-          if (ga.dz) {
-            gout<T> pz = (gout<T>)ga.dz + b * ga.dz_b + t0 * ga.dz_t;
+          if (gg.dz) {
+            gout<T> pz = (gout<T>)gg.dz + b * gg.dz_b + t0 * gg.dz_t;
 #pragma unroll
             for (int i = 0; i < kSteps; i++) {
-              stf(pz + c, dzv[i]);
-              walk(pz, ga.dz_t);
+              stf(at(pz), dzv[i]);
+              walk(pz, gg.dz_t);
             }
           }
         } else {
@@ -992,11 +1038,11 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
           for (int i = 0; i < kSteps; i++) {
             if (i >= steps) break;
             const int t = t0 + i;
-            if (ga.ddelta) stf((gout<T>)ga.ddelta + b * ga.dd_b + t * ga.dd_t + c, ddt[i]);
-            if (ga.dz) stf((gout<T>)ga.dz + b * ga.dz_b + t * ga.dz_t + c, dzv[i]);
-            if (ga.dx) {
-              if (!halo || last - t >= K - 1) stf((gout<T>)ga.dx + b * ga.dx_b + t * ga.dx_t + c, dxv[i]);
-              else ((gout<float>)ga.halo + ((s * 2 * a.B + b) * (kTaps - 1) + (last - t)) * a.C)[c] = dxv[i];
+            if (gg.ddelta) stf((gout<T>)gg.ddelta + b * gg.dd_b + t * gg.dd_t + c, ddt[i]);
+            if (gg.dz) stf((gout<T>)gg.dz + b * gg.dz_b + t * gg.dz_t + c, dzv[i]);
+            if (gg.dx) {
+              if (!halo || last - t >= K - 1) stf((gout<T>)gg.dx + b * gg.dx_b + t * gg.dx_t + c, dxv[i]);
+              else ((gout<float>)gg.halo + ((s * 2 * aa.B + b) * (kTaps - 1) + (last - t)) * aa.C)[c] = dxv[i];
             }
           }
         }
