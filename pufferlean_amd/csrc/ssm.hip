@@ -90,7 +90,9 @@ __device__ __forceinline__ bool starts(const Args& a, int t, long b) {
 // Bit j of flag_bits(flag_load(..)): step t0 - 3 + j starts an episode (j < 11: a batch and the three steps that its
 // convolutions look back to). One load per lane, one ballot, apart so that the load can be issued a batch ahead.
 __device__ __forceinline__ float flag_load(const Args& a, int t0, int tend, long b) {
-  const int j = threadIdx.x & 63, t = t0 - (kTaps - 1) + j;
+  int me = threadIdx.x;
+  asm("" : "+v"(me));  // computed here, not once for all batches
+  const int j = me & 63, t = t0 - (kTaps - 1) + j;
   float f = 0.f;
   if (j < kSteps + kTaps - 1 && t < tend && t >= 0) {
     if (t > 0) f = a.done ? a.done[(long)(t - 1) * a.B + b] : 0.f;
@@ -738,6 +740,7 @@ __global__ void __launch_bounds__(256) k_ssm_bwd_join(Args a, GradArgs ga) {
 // the staging computes once per step. Sums over channels are folded over the wavefront's lanes, then over the
 // block's wavefronts in LDS; the parameters' gradients stay in LDS and registers over all the block's work. A block
 // takes the items row, row + rows, ... of its channel block, an item being a chunk of a sequence.
+constexpr int kOwn = 3 + kTaps;  // a channel's own sums in the gradient
 template <typename T, int MOST>
 __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -750,6 +753,7 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
   float* red = sbc + 2 * 64 * Q;                // [waves][Q][kSteps][dB, dC][4]
   float* reds = red + waves * 64 * Q;           // [waves][kSteps] of S
   float* scb = reds + waves * kSteps;           // [2][kSteps] of <B, C>
+  float* own = scb + 2 * kSteps;                // [kOwn][nt]: dD, d(dt_bias), d(conv_b), d(conv_w)
   const unsigned cb = uniform(blockIdx.x % a.blocks_c), grp = uniform((blockIdx.x / a.blocks_c) % a.G);
   const unsigned row = uniform(blockIdx.x / (a.blocks_c * a.G)), items = (unsigned)(a.B * a.chunks);
   const unsigned lc = cb * nt + tid;
@@ -763,7 +767,8 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
     sdA[q * nt + tid] = f4(0.f, 0.f, 0.f, 0.f);
   }
   const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, Dc = a.D ? a.D[c] : 0.f;
-  float dD = 0.f, dbias = 0.f, dcb = 0.f, dw[kTaps] = {};
+#pragma unroll
+  for (int k = 0; k < kOwn; k++) own[k * nt + tid] = 0.f;
   const int K = cv.K;
   const long quads = a.B * Q * a.C;
   // What a batch reads: the rows, the three inputs before them, the flags, the first kept states and this thread's share of B
@@ -791,16 +796,6 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
     const GradArgs ga = again<GradArgs>(sizeof(Args));
     const long b = w.b;
     const int t0 = w.t0, steps = min(kSteps, w.tend - t0);
-    int me = tid;
-    asm("" : "+v"(me));  // or the places of all MOST values wait in registers over the states' steps
-#pragma unroll
-    for (int k = 0; k < MOST; k++) {
-      const int e = me + k * nt, n = place_state(e), i = place_step(e);
-      const bool is_c = place_row(e);
-      gin<T> p = is_c ? (gin<T>)a.Cm + b * a.cm_b : (gin<T>)a.Bm + b * a.bm_b;
-      vbc[k] = n < a.N && i < steps ? p[(long)(t0 + i) * (is_c ? a.cm_t : a.bm_t) + grp * a.N + n] : T(0);
-    }
-    fl = flag_load(a, t0, w.tend, b);
     rx.get((gin<T>)a.x + b * a.x_b + t0 * a.x_t, a.x_t, steps, c);
     if (t0 > 0) {
       gin<T> p = (gin<T>)a.x + b * a.x_b + (t0 - (kTaps - 1)) * a.x_t;
@@ -815,6 +810,16 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
     if (a.z) rz.get((gin<T>)a.z + b * a.z_b + t0 * a.z_t, a.z_t, steps, c);
     rg.get((gin<T>)ga.dy + b * ga.dy_b + t0 * ga.dy_t, ga.dy_t, steps, c);
     next = *Lane<f4t>(c)((gin<f4t>)ga.keep + t0 / kSteps * quads + b * Q * a.C);
+    int me = tid;
+    asm("" : "+v"(me));  // or the places of all MOST values wait in registers over the states' steps
+#pragma unroll
+    for (int k = 0; k < MOST; k++) {
+      const int e = me + k * nt, n = place_state(e), i = place_step(e);
+      const bool is_c = place_row(e);
+      gin<T> p = is_c ? (gin<T>)a.Cm + b * a.cm_b : (gin<T>)a.Bm + b * a.bm_b;
+      vbc[k] = n < a.N && i < steps ? p[(long)(t0 + i) * (is_c ? a.cm_t : a.bm_t) + grp * a.N + n] : T(0);
+    }
+    fl = flag_load(a, t0, w.tend, b);
   };
   int buf = 0;
   unsigned item = row;
@@ -983,6 +988,9 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
 #pragma unroll
       for (int i = 0; i < kSteps; i++) cb2[i] = scb[buf * kSteps + i];
       float dxv[kSteps], ddt[kSteps], dzv[kSteps];
+      float dD = own[tid], dbias = own[nt + tid], dcb = own[2 * nt + tid], dw[kTaps];
+#pragma unroll
+      for (int k = 0; k < kTaps; k++) dw[k] = own[(3 + k) * nt + tid];
       auto finish = [&](auto CLEAN, auto WHOLE) __attribute__((always_inline)) {  // WHOLE: no step is past the end
 #pragma unroll
         for (int i = kSteps - 1; i >= 0; i--) {
@@ -1011,6 +1019,11 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
       if (clean) finish(std::true_type{}, std::true_type{});
       else if (steps == kSteps) finish(std::false_type{}, std::true_type{});
       else finish(std::false_type{}, std::false_type{});
+      own[tid] = dD;
+      own[nt + tid] = dbias;
+      own[2 * nt + tid] = dcb;
+#pragma unroll
+      for (int k = 0; k < kTaps; k++) own[(3 + k) * nt + tid] = dw[k];
       if (in) {
         // the last K - 1 steps of a chunk that has a successor are finished by the halo's launch
         const bool halo = tend < aa.T && t0 + kSteps >= tend && K > 1;
@@ -1063,12 +1076,10 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
     float* p = ga.par + ((long)row * a.C + c) * ga.P;
     for (int q = 0; q < Q; q++) set_row4(p, 4 * q, a.N, sdA[q * nt + tid]);
     p += a.N;
-    p[0] = dD;
-    p[1] = dbias;
-    p[2] = dcb;
+    for (int k = 0; k < 3; k++) p[k] = own[k * nt + tid];
 #pragma unroll
     for (int k = 0; k < kTaps; k++)
-      if (k >= kTaps - K) p[3 + k - (kTaps - K)] = dw[k];
+      if (k >= kTaps - K) p[3 + k - (kTaps - K)] = own[(3 + k) * nt + tid];
   }
 }
 
@@ -1178,7 +1189,7 @@ Args args_of(const ph_ssm_args& p) {
 size_t fwd_lds(int Q, int nt) { return (size_t)4 * (8 * Q * nt + 2 * 64 * Q); }
 size_t bwd_lds(int Q, int nt) {
   const int waves = nt / 64;
-  return (size_t)4 * (12 * Q * nt + (2 + waves) * 64 * Q + waves * kSteps + 2 * kSteps);
+  return (size_t)4 * (12 * Q * nt + (2 + waves) * 64 * Q + waves * kSteps + 2 * kSteps + kOwn * nt);
 }
 
 // Threads of a block: whole wavefronts over a group's channels, at most four and as LDS holds (N = 64: one in the gradient).
@@ -1188,7 +1199,7 @@ int block_threads(const Args& a, bool grad) {
   while (nt > 64 && (grad ? bwd_lds(a.Q, nt) : fwd_lds(a.Q, nt)) > 64 * 1024) nt -= 64;
   return nt;
 }
-static_assert(4 * (12 * 16 * 64 + 3 * 64 * 16 + 3 * kSteps) <= 64 * 1024, "one wavefront at N = 64");
+static_assert(4 * (12 * 16 * 64 + 3 * 64 * 16 + 3 * kSteps + kOwn * 64) <= 64 * 1024, "one wavefront at N = 64");
 
 // Blocks of nt threads that run at a time in the gradient: two wavefronts to a SIMD, whole blocks to a CU.
 long resident(int nt) { return 256L * (8 / (nt / 64)); }
