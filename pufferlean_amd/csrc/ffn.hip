@@ -9,6 +9,10 @@
 // small; the epilogues (glu.hpp) keep the projections and dh from ever being written. bf16 rounds h, p, f and dab once
 // each from fp32: they are the operands of bf16 products, or (p, f) halve what the backward reads.
 //
+// Measured: 65536 x 512 x 1376 bf16 both directions 1166 us, 713 TFLOP/s (327 us h, 260 dab, 329 y and dx, 337 the weights'
+// gradients); the products' 592 us at the rate of a large library product are out of reach of their short K of 512.
+// 6699 x 203 x 531 fp32 232 us, 56 TFLOP/s: few tiles of padded columns for 256 CUs. 8 rows 12 us, launch and weight latency.
+//
 // The products want whole 16-byte accesses. Where D or F is not a multiple of 8, or a pointer or stride is off, the inputs'
 // rows and the weights are copied once, padded with zeros, which add nothing to any sum.
 #include "common.hpp"

@@ -8,6 +8,9 @@
 // writes dx. A row lives in the registers of LPR = 8..64 lanes (64 / LPR rows to a wavefront), so each value
 // is read once; the backward's wavefronts walk over many rows and keep their columns' dw and db in registers,
 // which leaves one partial row per block for a second, small launch to add in a fixed order.
+//
+// Measured, 262144 x 512 bf16: forward 103 us and backward 153 us, both 5.2 TB/s, what a large copy reaches on the card,
+// and 6 us for the partial rows. 6699 x 203 fp32 (rows of odd width): 5.4, 6.8 and 4.7 us, launch and load latency.
 #include "common.hpp"
 #include "kernels.hpp"
 #include "lanes.hpp"
@@ -130,7 +133,7 @@ __device__ __forceinline__ void get_weights(const Cols<V>& k, const float* w, fl
 
 // V elements per access, NCH accesses per lane: a row has at most LPR * V * NCH columns. A group of LPR lanes walks the
 // rows group, group + groups, ... with its columns of w and b in registers: loaded again for every row they cost
-// more than the row (262144x512 bf16: 475 us, 115 this way, 4.7 TB/s).
+// more than the row (262144x512 bf16: 475 us, 103 this way).
 template <typename T, int V, bool AL, int NCH, int LPR>
 __global__ void __launch_bounds__(64 * kWaves) k_norm_fwd(const T* __restrict__ x, long ldx, long M, int C,
                                                           const float* __restrict__ w, const float* __restrict__ b,

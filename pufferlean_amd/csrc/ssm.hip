@@ -13,8 +13,13 @@
 // converted once). Within those steps the states are taken four at a time: a lane's four states and decays rest in
 // LDS slots of its own and are in registers for the kSteps steps. So any N runs in the same few registers and short
 // code, and the state is fp32 throughout and never written per step. What a step costs is vector arithmetic: per state
-// one exponential (a quarter-rate instruction, 16 cycles of a wavefront), the decay's argument, the input, the update
-// and the output (4 cycles each), 32 cycles in all against 8 bytes of memory per channel and step.
+// one exponential (8 cycles of a wavefront), the decay's argument, the input, the update and the output (4 cycles each),
+// 24 cycles in all against 8 bytes of memory per channel and step; the gradient takes about three times as many.
+//
+// Measured, bf16, 16 states, four taps, gated: 64 steps of 2048 sequences x 512 channels forward 373 us, of which vector
+// instructions issue 70 % (the states' own 24 cycles would be 164 us), gradient 1139 us, 73 %; 8192 steps of 2 sequences
+// x 512 channels 102 us; 2048 steps of 8 x 384, two groups, both directions 313 us. What is left of the time is
+// wavefronts that wait: two on a SIMD in the gradient (its registers), four forward (its LDS slots).
 //
 // Long sequences of few channels do not fill the chip with one wavefront per 64 channels, so time is cut into
 // chunks: a first launch runs every chunk from a zero state and keeps its end state and the sum of d_t (the
@@ -506,7 +511,7 @@ __device__ __forceinline__ f4t quad_of(const uint16_t* p) {
 // One step of every sequence, the state updated in place: bound by the state's 8 bytes per element, so what a channel
 // needs once (convolution, time step, gate) is computed once, by the lane of that channel, and handed over through LDS to
 // the lanes that move the state, each four states of it as one 16-byte access (consecutive lanes, consecutive
-// addresses). QT: Q where it is 1, 2 or 4 and every access may be a vector one (VEC), with the decays in registers over
+// addresses). Measured, 4096 x 512 channels of 16 states: 82 us, 4.1 TB/s; a large copy would take 68. QT: Q where it is 1, 2 or 4 and every access may be a vector one (VEC), with the decays in registers over
 // the block's sequences; 0: any Q.
 template <typename T, int QT>
 __global__ void __launch_bounds__(256) k_ssm_step(Args a, float* __restrict__ hs, float* __restrict__ win, int per_block) {
