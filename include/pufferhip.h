@@ -438,8 +438,9 @@ int ph_ssm_step(const ph_ssm_args* a, void* y, long y_b, float* h, float* win, v
  * are part of that product's epilogue; w_out [D][F]. Both in dtype; PH_BF16 runs bf16 MFMA with fp32 accumulation,
  * PH_F32 fp32 MFMA. */
 typedef enum { PH_ACT_SILU = 0, PH_ACT_GELU = 1 } ph_act;
-/* pf [M][2 ph_ffn_pitch(F)] and h [M][ph_ffn_pitch(F)] (dtype, 16-byte aligned) receive what the gradient needs: the units
- * h_j = act(a_j) v_j, and the pairs v_j act'(a_j), act(a_j). Both NULL where no gradient follows. */
+/* pf and h (16-byte aligned) receive what the gradient needs: h [M][ph_ffn_pitch(F)] the units h_j = act(a_j) v_j in dtype, pf
+ * the pairs v_j act'(a_j), act(a_j) in a form of its own, rows of ph_ffn_pitch(F) pairs of 4-byte values for PH_F32 and of
+ * 3-byte ones for PH_BF16. Both NULL where no gradient follows. */
 int ph_ffn(int dtype, int act, size_t M, size_t D, size_t F, const void* x, size_t ldx, const void* w_in,
            const void* w_out, void* pf, void* h, void* y, size_t ldy, void* stream);
 /* Row pitch of `columns` values in whole 16-byte accesses. */

@@ -6,10 +6,10 @@
 //             dw_out = dy^T h;  dw_in = dab^T x;  dx = dab w_in
 //
 // All on the matrix cores: 6 M D F operations forward and 12 M D F backward, against which the activations' traffic is
-// small; the epilogues (glu.hpp) keep the projections and dh from ever being written. bf16 rounds h, p, f and dab once
-// each from fp32: they are the operands of bf16 products, or (p, f) halve what the backward reads.
+// small; the epilogues (glu.hpp) keep the projections and dh from ever being written. bf16 rounds h and dab once each from
+// fp32, as operands of bf16 products; p and f keep 24 bits.
 //
-// Measured: 65536 x 512 x 1376 bf16 both directions 1166 us, 713 TFLOP/s (327 us h, 260 dab, 329 y and dx, 337 the weights'
+// Measured: 65536 x 512 x 1376 bf16 both directions 1234 us, 673 TFLOP/s (357 us h, 298 dab, 350 y and dx, 337 the weights'
 // gradients); the products' 592 us at the rate of a large library product are out of reach of their short K of 512.
 // 6699 x 203 x 531 fp32 232 us, 56 TFLOP/s: few tiles of padded columns for 256 CUs. 8 rows 12 us, launch and weight latency.
 //
@@ -123,15 +123,23 @@ template <> struct Few<float> {
 
 __device__ __forceinline__ void put(uint16_t* p, float a, float b) { *reinterpret_cast<uint32_t*>(p) = bf16x2_rne(a, b); }
 __device__ __forceinline__ void put(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
-__device__ __forceinline__ void get(const uint16_t* p, float& a, float& b) {
-  const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
-  a = __builtin_bit_cast(float, u << 16);
-  b = __builtin_bit_cast(float, u & 0xffff0000u);
+// Values n .. n + 3, and the pair n, n + 1, of a row of pf (glu.hpp).
+__device__ __forceinline__ void keep4(uint16_t* row, long ld, long n, float p0, float f0, float p1, float f1) {
+  *reinterpret_cast<uint2*>(row + n) = make_uint2(keep_hi(p0, f0), keep_hi(p1, f1));
+  *reinterpret_cast<uint32_t*>(row + ld / 3 * 2 + n / 2) = keep_lo(p0, f0, p1, f1);
 }
-__device__ __forceinline__ void get(const float* p, float& a, float& b) {
-  const float2 u = *reinterpret_cast<const float2*>(p);
-  a = u.x;
-  b = u.y;
+__device__ __forceinline__ void keep4(float* row, long, long n, float p0, float f0, float p1, float f1) {
+  *reinterpret_cast<float4*>(row + n) = make_float4(p0, f0, p1, f1);
+}
+__device__ __forceinline__ void kept2(const uint16_t* row, long ld, long n, float& p, float& f) {
+  const uint32_t hi = *reinterpret_cast<const uint32_t*>(row + n), lo = row[ld / 3 * 2 + n / 2];
+  p = kept<0, 0>(hi, lo);
+  f = kept<1, 1>(hi, lo);
+}
+__device__ __forceinline__ void kept2(const float* row, long, long n, float& p, float& f) {
+  const float2 u = *reinterpret_cast<const float2*>(row + n);
+  p = u.x;
+  f = u.y;
 }
 __device__ __forceinline__ void put1(uint16_t* p, float a) { *p = bf16_rne(a); }
 __device__ __forceinline__ void put1(float* p, float a) { *p = a; }
@@ -186,14 +194,13 @@ __global__ void __launch_bounds__(64 * WAVES) k_few(FewArgs g) {
     glu_act(g.act, s[2], f1, d1);
     put(out + n / 2, f0 * s[1], f1 * s[3]);
     if (pf) {
-      put(pf + n, s[1] * d0, f0);
-      put(pf + n + 2, s[3] * d1, f1);
+      keep4(pf, g.ldpf, n, s[1] * d0, f0, s[3] * d1, f1);
     }
   } else if constexpr (MODE == kGrad) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       float p, f;
-      get(pf + 2 * (n + i), p, f);
+      kept2(pf, g.ldpf, 2 * (n + i), p, f);
       put(out + 2 * (n + i), s[i] * p, s[i] * f);
     }
   } else {
@@ -324,7 +331,7 @@ extern "C" int ph_ffn(int dtype, int act, size_t M, size_t D, size_t F, const vo
   if (M <= (size_t)kFewRows) {
     FewArgs g{};
     g.x = x; g.ldx = (long)ldx; g.w = w_in; g.ldw = g.K = (long)Dp; g.M = (int)M; g.N = (int)(2 * Fp); g.act = act;
-    g.out = h; g.ldo = (long)Fp; g.pf = pf; g.ldpf = (long)(2 * Fp);
+    g.out = h; g.ldo = (long)Fp; g.pf = pf; g.ldpf = keep_pitch(dtype, (long)Fp);
     PH_TRY(few<kIn>(dtype, g, c.st));
     FewArgs o{};
     o.x = h; o.ldx = (long)Fp; o.w = w_out; o.ldw = o.K = (long)Fp; o.M = (int)M; o.N = (int)D; o.out = y; o.ldo = (long)ldy;
@@ -332,7 +339,7 @@ extern "C" int ph_ffn(int dtype, int act, size_t M, size_t D, size_t F, const vo
   }
   GluProduct g{};
   g.dtype = dtype; g.act = act; g.M = (int)M; g.N = (int)(2 * Fp); g.K = (int)Dp;
-  g.A = x; g.lda = (long)ldx; g.B = w_in; g.ldb = (long)Dp; g.h = h; g.ldh = (long)Fp; g.pf = pf; g.ldpf = (long)(2 * Fp);
+  g.A = x; g.lda = (long)ldx; g.B = w_in; g.ldb = (long)Dp; g.h = h; g.ldh = (long)Fp; g.pf = pf; g.ldpf = keep_pitch(dtype, (long)Fp);
   PH_TRY(glu_product(g, c.st));
   return product(0, 1, M, D, Fp, dtype, h, Fp, w_out, Fp, dtype, y, ldy, c.st);
 }
@@ -392,13 +399,13 @@ extern "C" int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, con
   if (need_dab && few_rows) {
     FewArgs g{};
     g.x = dy; g.ldx = (long)lddy; g.w = w_out; g.ldw = g.K = (long)Dp; g.M = (int)M; g.N = (int)Fp; g.out = dab; g.ldo = (long)(2 * Fp);
-    g.pf = const_cast<void*>(pf); g.ldpf = (long)(2 * Fp);
+    g.pf = const_cast<void*>(pf); g.ldpf = keep_pitch(dtype, (long)Fp);
     PH_TRY(few<kGrad>(dtype, g, c.st));
   } else if (need_dab) {
     GluProduct g{};
     g.grad = 1; g.dtype = dtype; g.act = act; g.M = (int)M; g.N = (int)Fp; g.K = (int)Dp; g.b_kn = !trans;
     g.A = dy; g.lda = (long)lddy; g.B = w_out; g.ldb = (long)(trans ? Dp : Fp);
-    g.pf = const_cast<void*>(pf); g.ldpf = (long)(2 * Fp); g.dab = dab; g.lddab = (long)(2 * Fp);
+    g.pf = const_cast<void*>(pf); g.ldpf = keep_pitch(dtype, (long)Fp); g.dab = dab; g.lddab = (long)(2 * Fp);
     PH_TRY(glu_product(g, c.st));
   }
   if (dx && few_rows) {

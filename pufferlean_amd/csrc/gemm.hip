@@ -832,12 +832,23 @@ __device__ __forceinline__ void store4_once(uint16_t* p, const float* v) {
 }
 __device__ __forceinline__ void store4_once(float* p, const float* v) { store4(p, make_float4(v[0], v[1], v[2], v[3])); }
 
+// Values col .. col + 7 of a row of pf.
+__device__ __forceinline__ void keep8(uint16_t* row, long ld, int col, const float* v) {
+  typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+  const u32x4_t hi = {keep_hi(v[0], v[1]), keep_hi(v[2], v[3]), keep_hi(v[4], v[5]), keep_hi(v[6], v[7])};
+  const u32x2_t lo = {keep_lo(v[0], v[1], v[2], v[3]), keep_lo(v[4], v[5], v[6], v[7])};
+  __builtin_nontemporal_store(hi, reinterpret_cast<u32x4_t*>(row + col));
+  __builtin_nontemporal_store(lo, reinterpret_cast<u32x2_t*>(row + ld / 3 * 2 + col / 2));
+}
+__device__ __forceinline__ void keep8(float* row, long, int col, const float* v) { store8_of(row + col, v); }
+
 // kGluGrad's factors of a pass, loaded before the pass is staged and all waited for before its first store: loads and
 // stores share one counter, so a load behind a store would wait for that store's round trip.
 template <int GLU, typename TC, int BM, int BN, int NT>
 struct GluFactors {
   static constexpr int CPR = BN / 8, NCH = GLU == kGluGrad ? BM * CPR / NT : 1;
   Raw8<TC> v[NCH][2];
+  Raw8<uint16_t> lo[sizeof(TC) == 2 ? NCH : 1];  // the third bytes
   __device__ __forceinline__ void load(const GemmArgs& g, int m0, int n0, int mhi = -1) {
     if constexpr (GLU == kGluGrad) {
       if (mhi < 0) mhi = m0 + BM / 2;
@@ -849,15 +860,17 @@ struct GluFactors {
         const gptr<TC> p = (gptr<TC>)g.aux + (long)row * g.ldaux + 2 * col;
         v[q][0] = load_raw8(in ? p : zero_page<TC>());
         v[q][1] = load_raw8(in ? p + 8 : zero_page<TC>());
+        if constexpr (sizeof(TC) == 2)
+          lo[q] = load_raw8(in ? (gptr<uint16_t>)g.aux + (long)row * g.ldaux + g.ldaux / 3 * 2 + col : zero_page<uint16_t>());
       }
     }
   }
 };
-__device__ __forceinline__ void cvt8(const Raw8<uint16_t>& r, float (&v)[8]) {
-  const float4 a = cvt4(EpiRaw4<uint16_t>{make_uint2(r.v.x, r.v.y)}), b = cvt4(EpiRaw4<uint16_t>{make_uint2(r.v.z, r.v.w)});
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+__device__ __forceinline__ void cvt8(const Raw8<uint16_t>& r, uint32_t lo0, uint32_t lo1, float (&v)[8]) {
+  v[0] = kept<0, 0>(r.v.x, lo0); v[1] = kept<1, 1>(r.v.x, lo0); v[2] = kept<0, 2>(r.v.y, lo0); v[3] = kept<1, 3>(r.v.y, lo0);
+  v[4] = kept<0, 0>(r.v.z, lo1); v[5] = kept<1, 1>(r.v.z, lo1); v[6] = kept<0, 2>(r.v.w, lo1); v[7] = kept<1, 3>(r.v.w, lo1);
 }
-__device__ __forceinline__ void cvt8(const Raw8<float>& r, float (&v)[8]) {
+__device__ __forceinline__ void cvt8(const Raw8<float>& r, uint32_t, uint32_t, float (&v)[8]) {
   v[0] = r.a.x; v[1] = r.a.y; v[2] = r.a.z; v[3] = r.a.w; v[4] = r.b.x; v[5] = r.b.y; v[6] = r.b.z; v[7] = r.b.w;
 }
 
@@ -888,12 +901,13 @@ __device__ __forceinline__ void flush_glu(const GemmArgs& g, const float* sC, co
         pf[2 * j + 1] = f;
       }
       store4_once(out + col / 2, h);
-      if (g.C2) store8_of(reinterpret_cast<TC*>(g.C2) + (long)row * g.ldc2 + col, pf);
+      if (g.C2) keep8(reinterpret_cast<TC*>(g.C2) + (long)row * g.ldc2, g.ldc2, col, pf);
     } else {
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         float m[8], d[8];
-        cvt8(fac.v[q][half], m);
+        const uint4 lo = fac.lo[sizeof(TC) == 2 ? q : 0].v;
+        cvt8(fac.v[q][half], half ? lo.z : lo.x, half ? lo.w : lo.y, m);
 #pragma unroll
         for (int j = 0; j < 8; j++) d[j] = v[4 * half + j / 2] * m[j];
         store8_of(out + 2 * col + 8 * half, d);

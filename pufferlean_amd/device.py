@@ -685,6 +685,11 @@ def _pitch(n):
     return (n + 7) // 8 * 8
 
 
+def _kept(dt):
+    # bf16 units keep a pair of 24-bit values, fp32 ones two of their own
+    return 3 if dt == L.PH_BF16 else 2
+
+
 def gated_ffn(x, w_in, w_out, *, act="silu", out=None, save=False):
     """Gated feed-forward block (act(x Wg^T) * (x Wv^T)) Wo^T: x [M, D], w_in [2F, D] with the gate and value rows of unit
     j at 2j and 2j + 1, w_out [D, F], float32 or bfloat16. Returns y, or (y, saved) with save=True, saved being what
@@ -693,7 +698,7 @@ def gated_ffn(x, w_in, w_out, *, act="silu", out=None, save=False):
     y = x.new_empty((M, D)) if out is None else _like(out, x, x.shape, "out")
     pf = h = None
     if save:
-        pf, h = x.new_empty((M, 2 * _pitch(F))), x.new_empty((M, _pitch(F)))
+        pf, h = x.new_empty((M, _kept(dt) * _pitch(F))), x.new_empty((M, _pitch(F)))
     L.call("ph_ffn", dt, _ACT[act], M, D, F, x.data_ptr(), _rows(x), w_in.data_ptr(), w_out.data_ptr(), _ptr(pf), _ptr(h),
            y.data_ptr(), _rows(y), _stream())
     return (y, (pf, h)) if save else y
@@ -704,7 +709,7 @@ def gated_ffn_grad(x, w_in, w_out, saved, dy, *, act="silu", dx=None, dw_in=None
     dt, M, D, F = _ffn_shapes(x, w_in, w_out, act)
     _like(dy, x, x.shape, "dy")
     pf, h = saved
-    for t, cols in ((pf, 2 * _pitch(F)), (h, _pitch(F))):
+    for t, cols in ((pf, _kept(dt) * _pitch(F)), (h, _pitch(F))):
         if not _like(t, x, (M, cols), "saved").is_contiguous():
             raise ValueError("saved must be as gated_ffn returned it")
     dwt = dw_dtype or (x.dtype if dw_in is None else dw_in.dtype)

@@ -165,6 +165,27 @@ def test_graph_replays(gpu, M):
         (torch.ones(1000, device="cuda") * 2).sum().item()
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("M", [8, 130, 4096])
+def test_kept_pairs(gpu, M, act):
+    """bf16 keeps the first 24 bits of v act'(a) and act(a): cut off at 2^-15 of the value, not rounded at 2^-9. The fp32 sums of
+    64 exact products (of about 5 in all) are off by 2e-5 at most, which a pair takes up to 4 times (|v| under 5)."""
+    Dm, F = 64, 96
+    x, wi, wo, _ = case(M, Dm, F, torch.bfloat16)
+    _, (pf, _) = D.gated_ffn(x, wi, wo, act=act, save=True)
+    row = pf.cpu().contiguous().view(torch.uint8).numpy().reshape(M, 6 * F)
+    b = np.zeros((M, 2 * F, 4), np.uint8)
+    b[..., 2:] = row[:, :4 * F].reshape(M, 2 * F, 2)
+    b[..., 1] = row[:, 4 * F:]
+    got = b.view(np.float32)[..., 0].astype(np.float64)
+    a, v = (x.double() @ wi.double()[k::2].T for k in (0, 1))
+    a = a.cpu().requires_grad_(True)
+    f = R.glu(a, torch.ones_like(a), act)
+    p = torch.autograd.grad(f.sum(), a)[0] * v.cpu()
+    ref = torch.stack([p, f.detach()], -1).reshape(M, -1).numpy()
+    assert (np.abs(got - ref) <= 2.0 ** -15 * np.abs(ref) + 1e-4).all()
+
+
 def test_refusals(gpu):
     x, wi, wo, dy = case(4, 16, 24, torch.float32)
     with pytest.raises(TypeError):
