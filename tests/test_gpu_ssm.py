@@ -146,6 +146,34 @@ def test_many_sequences_and_long_ones(gpu):
     check(*inputs(200, 2, 24, 4), bar=4e-5)
 
 
+@pytest.mark.parametrize("T,N,K,carry,dt", [(13, 5, 3, True, torch.float32), (21, 16, 4, True, torch.bfloat16), (8, 4, 4, False, torch.float32)])
+def test_blocks_of_several_sequences(gpu, T, N, K, carry, dt):
+    """4500 sequences are more than the gradient's blocks run at a time (2048 of 64 channels), so a block goes on to its next
+    ones; in parts of 1500 it has one. A sequence's own outputs are the same bit for bit. The parameters' sums are over the same
+    terms in another order: chains of under 3000 additions that round by 2^-24 each, independently."""
+    s, c = inputs(T, 4500, 16, N, K=K, dt=dt, carry=carry)
+    dy = cu(20, T, 4500, 16, dtype=dt)
+    y, h, _, saved = forward(s, c)
+    g = backward(s, c, saved, dy)
+    sums = {}
+    for b in range(0, 4500, 1500):
+        part = slice(b, b + 1500)
+        sp = {k: v[:, part] if k in ("x", "delta", "Bm", "Cm", "z") and v is not None else v for k, v in s.items()}
+        cp = {k: v if v is None or k == "groups" else v[:, part].contiguous() if k == "done" else v[part].contiguous()
+              for k, v in c.items()}
+        yp, hp, _, kept = forward(sp, cp)
+        gp = backward(sp, cp, kept, dy[:, part].contiguous())
+        assert torch.equal(yp, y[:, part]) and torch.equal(hp, h[part])
+        for k, v in gp.items():
+            if k in ("dx", "ddelta", "dBm", "dCm", "dz"):
+                assert torch.equal(v, g[k][:, part]), k
+            else:
+                sums[k] = sums.get(k, 0) + v.double()
+    assert sums and set(sums) | {"dx", "ddelta", "dBm", "dCm", "dz"} == set(g)
+    for k, v in sums.items():
+        assert R.rel(g[k], v) <= 2e-5, k
+
+
 def test_every_step_ends_an_episode(gpu):
     s, c = inputs(40, 2, 16, 4, K=4)
     c["done"].fill_(1.0)
