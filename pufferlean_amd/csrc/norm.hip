@@ -436,16 +436,18 @@ template <typename T> struct NormCall {
       PH_LAUNCH_CHECK();
       return PH_OK;
     }
+    // the columns' sums first: dx may be written over x or dy
+    if (dw || db) {
+      long ry = (M + 31) / 32;
+      if (ry > 128) ry = 128;
+      float* part = (float*)scratch(kSlotNormPart, (size_t)ry * 2 * C * 4);
+      if (!part) return PH_ERR_NOMEM;
+      k_norm_cols_wide<T><<<dim3((C + 63) / 64, (unsigned)ry), 256, 0, st>>>(x, ldx, dy, lddy, M, C, cmean, crstd, part);
+      PH_LAUNCH_CHECK();
+      k_norm_fold<<<(unsigned)((2 * C + 15) / 16), 256, 0, st>>>(part, (int)ry, C, dw, db);
+      PH_LAUNCH_CHECK();
+    }
     k_norm_bwd_wide<T><<<(unsigned)M, 256, 0, st>>>(x, ldx, dy, lddy, C, w, cmean, crstd, dx, lddx);
-    PH_LAUNCH_CHECK();
-    if (!dw && !db) return PH_OK;
-    long ry = (M + 31) / 32;
-    if (ry > 128) ry = 128;
-    float* part = (float*)scratch(kSlotNormPart, (size_t)ry * 2 * C * 4);
-    if (!part) return PH_ERR_NOMEM;
-    k_norm_cols_wide<T><<<dim3((C + 63) / 64, (unsigned)ry), 256, 0, st>>>(x, ldx, dy, lddy, M, C, cmean, crstd, part);
-    PH_LAUNCH_CHECK();
-    k_norm_fold<<<(unsigned)((2 * C + 15) / 16), 256, 0, st>>>(part, (int)ry, C, dw, db);
     PH_LAUNCH_CHECK();
     return PH_OK;
   }

@@ -129,6 +129,20 @@ def test_in_place(gpu):
     assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("into", ["dy", "x"])
+@pytest.mark.parametrize("M,C", [(130, 96), (130, 203), (600, 2048), (3, 2049), (130, 2049), (600, 4096)])
+def test_gradient_into_its_inputs(gpu, M, C, into, dt):
+    """dx may be dy or x: nothing is read from either after it has been written, the columns' sums neither. Rows of every form, and
+    one block's as well as several blocks' sums."""
+    x, dy, w, b = case(M, C, dt)
+    _, mean, rstd = D.layer_norm(x, w, b)
+    ref = D.layer_norm_grad(x, w, mean, rstd, dy)
+    got = D.layer_norm_grad(x, w, mean, rstd, dy, dx=dy if into == "dy" else x)
+    for k, a, g in zip(("dx", "dw", "db"), ref, got):
+        assert torch.equal(a, g), k
+
+
 def test_gradient_against_differences(gpu):
     x, dy, w, b = case(40, 96, torch.float32)
     y, mean, rstd = D.layer_norm(x, w, b)
