@@ -560,13 +560,13 @@ _SSM_GRADS = struct.Struct("@5P10l5P")
 assert _SSM_ARGS.size == C.sizeof(L.SsmArgs) and _SSM_GRADS.size == C.sizeof(L.SsmGrads)
 
 
-def _ssm_args(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, done, first, h0, win0):
-    """The checked ph_ssm_args of [T, B, C] (or single-step [B, C]) inputs, and (T, B, C, N, K)."""
+def _ssm_args(seq, x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, done, first, h0, win0):
+    """The checked ph_ssm_args of [T, B, C] (seq) or single-step [B, C] inputs, and (T, B, C, N, K). A call takes one of the two
+    and passes its outputs' strides accordingly."""
     dt = _act_dtype(x, "ssm")
     shape = x.shape
-    seq = len(shape) == 3
-    if not seq and len(shape) != 2 or A.dim() != 2:
-        raise ValueError("x must be [T, B, C] or [B, C], and A [C, N]")
+    if len(shape) != (3 if seq else 2) or A.dim() != 2:
+        raise ValueError(f"x must be {'[T, B, C]' if seq else '[B, C]'} and A [C, N], not {tuple(shape)} and {tuple(A.shape)}")
     T, B, C_ = shape if seq else (1, *shape)
     N, K = A.shape[1], 0 if conv_w is None else conv_w.shape[-1]
     bc = (T, B, groups * N) if seq else (B, groups * N)
@@ -612,7 +612,7 @@ def ssm_scan(x, delta, A, Bm, Cm, *, D=None, z=None, dt_bias=None, conv_w=None, 
     A [C, N], D, dt_bias, conv_b [C], conv_w [C, K], done [T, B], first [B], h0 [B, C, N], win0 [B, K-1, C] float32.
     h_out and win_out receive the carried state (they may be h0 and win0). Returns y, or (y, saved) with save=True, saved
     being what ssm_scan_grad needs."""
-    a, T, B, C_, N, K = _ssm_args(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, done, first, h0, win0)
+    a, T, B, C_, N, K = _ssm_args(True, x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, done, first, h0, win0)
     y = x.new_empty(x.shape) if out is None else _like(out, x, x.shape, "out")
     if h_out is not None:
         _f32(h_out, (B, C_, N), "h_out")
@@ -630,7 +630,7 @@ def ssm_scan_grad(x, delta, A, Bm, Cm, saved, dy, *, D=None, z=None, dt_bias=Non
     """Gradient of ssm_scan from its arguments and what it saved. Returns a dict: dx, ddelta, dBm, dCm (and dz) in the
     activations' dtype, written into the given tensors where there are any, and dA (and dD, ddt_bias, dconv_w, dconv_b)
     in float32. The carried-in state and window are constants."""
-    a, T, B, C_, N, K = _ssm_args(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, done, first, None, win0)
+    a, T, B, C_, N, K = _ssm_args(True, x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, done, first, None, win0)
     _like(dy, x, x.shape, "dy")
     _f32(saved, (L.lib().ph_ssm_keep_floats(a),), "saved")
     g, ptrs, strides = {}, [], []
@@ -658,7 +658,7 @@ def ssm_step(x, delta, A, Bm, Cm, h, win=None, *, D=None, z=None, dt_bias=None, 
              first=None, out=None):
     """One step of ssm_scan for B sequences: x, delta, z [B, C], Bm, Cm [B, groups*N]; the state h [B, C, N] and the
     convolution's window win [B, K-1, C] (float32) are updated in place, cleared first where first[b] is set."""
-    a, _, _, _, _, K = _ssm_args(x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, None, first, h, win)
+    a, _, _, _, _, K = _ssm_args(False, x, delta, A, Bm, Cm, D, z, dt_bias, conv_w, conv_b, groups, None, first, h, win)
     if K > 1 and win is None:
         raise ValueError("win is needed for a convolution of two taps or more")
     y = x.new_empty(x.shape) if out is None else _like(out, x, x.shape, "out")
