@@ -400,10 +400,11 @@ int ph_layer_norm_grad(int dtype, const void* x, size_t ldx, const void* dy, siz
  *   y_t = (<h_t, C_t> + D u_t) z_t sigma(z_t)              (z NULL: no gate)
  * G groups of C / G channels share the rows of B and C. Element (t, b, i) of an array is at t * <name>_t + b * <name>_b
  * + i, so time-major and batch-major arrays and column slices of a wider one are all taken in place. A, D, dt_bias,
- * conv_w, conv_b are fp32 ([C][N], [C], [C], [C][K], [C]); D, dt_bias and conv_b may be NULL (0). done (fp32 [T][B], may
- * be NULL): where nonzero, step t ends an episode, and step t + 1 starts from a cleared state and an empty window; first
- * (fp32 [B], may be NULL): the same for the step before the call. h0 [B][C][N] and win0 [B][K-1][C] (fp32, each may
- * be NULL: zero) are the state and the last K - 1 inputs carried in. */
+ * conv_w, conv_b are fp32 ([C][N], [C], [C], [C][K], [C]); D, dt_bias and conv_b may be NULL (0); with K = 0 conv_b is
+ * not read and its gradient is zero. done (fp32 [T][B], may be NULL): where nonzero, step t ends an episode, and step
+ * t + 1 starts from a cleared state and an empty window; first (fp32 [B], may be NULL): the same for the step before
+ * the call. h0 [B][C][N] and win0 [B][K-1][C] (fp32, each may be NULL: zero) are the state and the last K - 1 inputs
+ * carried in. */
 typedef struct {
   int dtype;
   size_t T, B, C, N, G, K;

@@ -1081,7 +1081,9 @@ __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
     float* p = ga.par + ((long)row * a.C + c) * ga.P;
     for (int q = 0; q < Q; q++) set_row4(p, 4 * q, a.N, sdA[q * nt + tid]);
     p += a.N;
-    for (int k = 0; k < 3; k++) p[k] = own[k * nt + tid];
+    p[0] = own[tid];
+    p[1] = own[nt + tid];
+    p[2] = K ? own[2 * nt + tid] : 0.f;  // without taps there is no convolution for a bias to be of: u is x
 #pragma unroll
     for (int k = 0; k < kTaps; k++)
       if (k >= kTaps - K) p[3 + k - (kTaps - K)] = own[(3 + k) * nt + tid];

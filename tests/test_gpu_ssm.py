@@ -113,6 +113,24 @@ def test_taps_gates_and_ends(gpu, K, gate, done):
     check(*inputs(45, 3, 33, 6, K=K, gate=gate, done=done, carry=done, extras=gate))
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [9, 70])
+def test_bias_without_taps(gpu, T, dt):
+    """Without taps u is x: a bias of the convolution changes nothing, and its gradient is zero."""
+    s, c = inputs(T, 2, 40, 4, K=0, dt=dt)
+    dy = cu(20, T, 2, 40, dtype=dt)
+    y, h, _, saved = forward(s, c)
+    ref = backward(s, c, saved, dy)
+    for w in (None, torch.empty(40, 0, device="cuda")):
+        sb = dict(s, conv_w=w, conv_b=cu(10, 40))
+        yb, hb, _, kept = forward(sb, c)
+        g = backward(sb, c, kept, dy)
+        assert torch.equal(yb, y) and torch.equal(hb, h)
+        assert g["dconv_b"].shape == (40,) and not g["dconv_b"].any()
+        for k in ref:
+            assert torch.equal(g[k], ref[k]), k
+
+
 @pytest.mark.parametrize("C,G", [(1, 1), (64, 1), (65, 1), (128, 2), (130, 2), (300, 3), (520, 1), (600, 1), (1100, 2)])
 def test_channels_and_groups(gpu, C, G):
     check(*inputs(11, 2, C, 8, G=G, dt=torch.bfloat16))

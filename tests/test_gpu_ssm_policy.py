@@ -81,6 +81,25 @@ def test_gradient_in_fp32(gpu):
         assert R.rel(g[k], r) <= 5e-4, k
 
 
+def test_policy_without_taps(gpu):
+    """No convolution: its bias is no part of the model, so the gradient leaves it where it is. Bars as above."""
+    policy = SSMPolicy(OBS, A, width=24, inner=40, states=8, taps=0, ffn=36, layers=2, dtype=torch.float32, seed=5)
+    obs, done, first = columns()
+    out, saved = policy.forward(obs, done, first, save=True)
+    dout = cu(4, T, B, A + 1)
+    g = policy.backward(saved, dout)
+    p = {k: R.leaf(v) for k, v in policy.p.items()}
+    host = lambda t: t.double().cpu()
+    ref = reference(policy, p, host(obs), host(done), host(first), [(None, None)] * policy.layers)
+    assert R.rel(out.view(T * B, -1), ref) <= 2e-4
+    used = [k for k in p if "conv" not in k]
+    for k, r in zip(used, torch.autograd.grad(ref, [p[k] for k in used], host(dout).view(T * B, -1))):
+        assert R.rel(g[k], r) <= 5e-4, k
+    policy.update(g)
+    for i in range(policy.layers):
+        assert not g[f"{i}.conv_b"].any() and not policy.p[f"{i}.conv_b"].any()
+
+
 def test_bf16_gradient_points_the_same_way(gpu):
     obs, done, first = columns()
     dout = cu(4, T, B, A + 1)
