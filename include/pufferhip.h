@@ -447,7 +447,7 @@ int ph_ffn(int dtype, int act, size_t M, size_t D, size_t F, const void* x, size
 /* Row pitch of `columns` values in whole 16-byte accesses. */
 size_t ph_ffn_pitch(size_t columns);
 /* dx [M][D], dw_in [2F][D] and dw_out [D][F], each written where not NULL; the weights' gradients in dw_dtype (dtype or
- * PH_F32), overwritten. */
+ * PH_F32), overwritten. dx may be dy or x. */
 int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, const void* x, size_t ldx, const void* w_in,
                 const void* w_out, const void* pf, const void* h, const void* dy, size_t lddy, void* dx, size_t lddx,
                 int dw_dtype, void* dw_in, void* dw_out, void* stream);

@@ -408,11 +408,6 @@ extern "C" int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, con
     g.pf = const_cast<void*>(pf); g.ldpf = keep_pitch(dtype, (long)Fp); g.dab = dab; g.lddab = (long)(2 * Fp);
     PH_TRY(glu_product(g, c.st));
   }
-  if (dx && few_rows) {
-    FewArgs g{};
-    g.x = dab; g.ldx = (long)(2 * Fp); g.w = w_in; g.ldw = g.K = (long)(2 * Fp); g.M = (int)M; g.N = (int)D; g.out = dx; g.ldo = (long)lddx;
-    PH_TRY(few<kPlain>(dtype, g, c.st));
-  } else if (dx) PH_TRY(product(0, trans, M, D, 2 * Fp, dtype, dab, 2 * Fp, w_in, trans ? 2 * Fp : Dp, dtype, dx, lddx, c.st));
   // the weights' gradients; of padded operands through a padded copy
   Layer out;
   if (dw_in) {
@@ -425,5 +420,11 @@ extern "C" int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, con
     PH_TRY(weight_grad(w_ok ? D : Dp, w_ok ? F : Fp, M, dtype, dy, lddy, h, Fp, dw_dtype, q, c.st));
     if (!w_ok) PH_TRY(out.add(q, D, F, Fp, dw_out, D, F, false));
   }
+  // dx last: it may be written over x or dy
+  if (dx && few_rows) {
+    FewArgs g{};
+    g.x = dab; g.ldx = (long)(2 * Fp); g.w = w_in; g.ldw = g.K = (long)(2 * Fp); g.M = (int)M; g.N = (int)D; g.out = dx; g.ldo = (long)lddx;
+    PH_TRY(few<kPlain>(dtype, g, c.st));
+  } else if (dx) PH_TRY(product(0, trans, M, D, 2 * Fp, dtype, dab, 2 * Fp, w_in, trans ? 2 * Fp : Dp, dtype, dx, lddx, c.st));
   return out.run(dw_dtype, c.st);
 }

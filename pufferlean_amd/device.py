@@ -705,7 +705,7 @@ def gated_ffn(x, w_in, w_out, *, act="silu", out=None, save=False):
 
 
 def gated_ffn_grad(x, w_in, w_out, saved, dy, *, act="silu", dx=None, dw_in=None, dw_out=None, dw_dtype=None):
-    """Gradient of gated_ffn: (dx, dw_in, dw_out), the weights' in dw_dtype (x's dtype, or float32)."""
+    """Gradient of gated_ffn: (dx, dw_in, dw_out), the weights' in dw_dtype (x's dtype, or float32). dx may be dy or x."""
     dt, M, D, F = _ffn_shapes(x, w_in, w_out, act)
     _like(dy, x, x.shape, "dy")
     pf, h = saved

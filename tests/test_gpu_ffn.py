@@ -87,6 +87,19 @@ def test_strided_rows(gpu, dt, off):
     assert torch.all(out[:, :off] == 5) and torch.all(out[:, off + 128:] == 5)
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("into", ["dy", "x"])
+@pytest.mark.parametrize("M,Dm,F", [(8, 64, 96), (40, 203, 33), (300, 128, 96), (300, 203, 64), (2100, 64, 96)])
+def test_gradient_into_its_inputs(gpu, M, Dm, F, into, dt):
+    """dx may be dy or x: the weights' gradients read neither after it has been written."""
+    x, wi, wo, dy = case(M, Dm, F, dt)
+    _, saved = D.gated_ffn(x, wi, wo, save=True)
+    ref = D.gated_ffn_grad(x, wi, wo, saved, dy)
+    got = D.gated_ffn_grad(x, wi, wo, saved, dy, dx=dy if into == "dy" else x)
+    for k, a, g in zip(("dx", "dw_in", "dw_out"), ref, got):
+        assert torch.equal(a, g), k
+
+
 def test_saturated_gates(gpu):
     """Gates far on both sides: the activation is the identity or zero, and its gradient finite."""
     x, wi, wo, dy = case(40, 64, 48, torch.float32)
