@@ -1902,7 +1902,7 @@ int launch_glu(const GemmArgs& g, int dtype, hipStream_t st) {
   auto tiles = [&](long bm, long bn) { return (unsigned)((g.M + bm - 1) / bm * ((g.N + bn - 1) / bn)); };
   if (dtype == PH_BF16) {
     // tiles as for a plain NT product: 256x256 or 256x128 from 512 of 256x128 on, whichever pads the columns less
-    if (TB && tiles(256, 128) >= 512) {
+    if (TB && tiles(256, 128) >= 512 && dma_offsets_fit(false, g.lda, g.ldb)) {
       const long n256 = (g.N + 255) / 256 * 256, n128 = (g.N + 127) / 128 * 128;
       if (n256 <= n128 + n128 / 16)
         k_gemm_nt_dma<256, 256, uint16_t, false, 4, 4, 4, false, GLU><<<tiles(256, 256), 1024, 0, st>>>(g);
@@ -2006,7 +2006,8 @@ int gemm(const PhGemmDesc& d_in, hipStream_t st) {
   const long tiles256x128 = (long)((d.M + 255) / 256) * ((d.N + 127) / 128);
   const long tiles128 = (long)((d.M + 127) / 128) * ((d.N + 127) / 128);
   const long tiles64 = (long)((d.M + 63) / 64) * ((d.N + 63) / 64);
-  const bool big_ok = d.math == PH_MATH_BF16 && d.a_dtype == PH_BF16 && d.b_dtype == PH_BF16;
+  const bool big_ok = d.math == PH_MATH_BF16 && d.a_dtype == PH_BF16 && d.b_dtype == PH_BF16 &&
+                      (!d.trans_a == !d.trans_b || dma_offsets_fit(d.trans_a, d.lda, d.ldb));
   bool small = false, big = big_ok && tiles256x128 >= 512, wide_n = false;
   // NT outputs at most 64 wide (the policy heads): 256x64 tiles, half the wasted columns of 256x128
   int big_bn = !d.trans_a && d.trans_b && d.N <= 64 ? 64 : 128;

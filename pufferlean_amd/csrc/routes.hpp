@@ -5,6 +5,12 @@
 
 namespace ph {
 
+// ---- GEMM, load-to-LDS copies -----------------------------------------------------------------------------
+// Whether the kernels that copy their tiles straight into LDS may run: they keep an element's offset from its tile's first row
+// in 32 bits. NT tiles have 256 rows (k offset included, 256 leading dimensions at most), TN stages 32 rows of k.
+// Operands with longer rows (a column of a wide buffer, say) take the kernels that load through registers.
+inline bool dma_offsets_fit(bool tn, long lda, long ldb) { return (lda > ldb ? lda : ldb) <= (tn ? 1L << 26 : 1L << 23); }
+
 // ---- GEMM, reductions of k >= 4096 with a small output ------------------------------------------------
 // 64x64 split tiles instead of 128x128 ones, for outputs at most 64 wide or tall with fp32 operands (128x128 tiles
 // are mostly padding there) and, in fp32 math, where 128x128 splits of >= 512 leave most CUs idle. fp32 math is bound
