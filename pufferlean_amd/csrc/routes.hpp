@@ -151,4 +151,37 @@ inline RollForm rollout_form(bool bf16, long N, long H) {
   return c32 <= c128 ? kRoll32 : kRoll128;
 }
 
+// ---- Selective state-space scan ---------------------------------------------------------------------------
+// LDS bytes of a block of nt threads for 4 Q states a channel: the lanes' slots, the staged rows and (gradient) the wavefronts'
+// sums and the channels' own, kSsmOwn each.
+constexpr int kSsmSteps = 8, kSsmOwn = 7;
+constexpr long ssm_fwd_lds(int Q, int nt) { return 4L * (8 * Q * nt + 2 * 64 * Q); }
+constexpr long ssm_bwd_lds(int Q, int nt) {
+  return 4L * (12 * Q * nt + (2 + nt / 64) * 64 * Q + nt / 64 * kSsmSteps + 2 * kSsmSteps + kSsmOwn * nt);
+}
+// Threads of a block: whole wavefronts over the channels of a group, at most four and as LDS holds (64 states: one in the
+// gradient).
+inline int ssm_block_threads(long per, int Q, bool grad) {
+  const long w = (per + 63) / 64;
+  int nt = 64 * (int)(w < 4 ? w : 4);
+  while (nt > 64 && (grad ? ssm_bwd_lds(Q, nt) : ssm_fwd_lds(Q, nt)) > 64 * 1024) nt -= 64;
+  return nt;
+}
+// Blocks of nt threads that run at a time in the gradient: two wavefronts to a SIMD, whole blocks to a CU.
+inline long ssm_resident(int nt) { return 256L * (8 / (nt / 64)); }
+// Steps of a chunk of time of T steps, B sequences, G groups of `per` channels of N states: as many chunks as make one round of
+// blocks, in chunks of at least 32 steps (2048x8, two groups of 192 channels: a chunk more and a second round gave 401 us both
+// directions, 361 without). Chunks cost a second pass over their steps and three launches (about 20 us), so sequences
+// stay whole while one pass over all their steps is not longer than that: up to 128 steps of 16 states forward, 64 in the
+// gradient, whose steps take three times as long; the more the fewer the states. (33 steps of 203x96x5 fp32 both
+// directions: 104 us in two chunks, 84 whole.)
+inline long ssm_chunk(long T, long B, long G, long per, int N, bool grad) {
+  const int nt = ssm_block_threads(per, (N + 3) / 4, true);
+  const long most = (T + 31) / 32;
+  long want = ssm_resident(nt) / (B * G * ((per + nt - 1) / nt));
+  if (want > most) want = most;
+  if (want < 1 || T * (8 + N) <= (grad ? 64 : 128) * (8 + 16)) want = 1;
+  return ((T + want - 1) / want + kSsmSteps - 1) / kSsmSteps * kSsmSteps;
+}
+
 }  // namespace ph

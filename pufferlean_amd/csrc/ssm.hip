@@ -28,13 +28,14 @@
 #include "common.hpp"
 #include "kernels.hpp"
 #include "lanes.hpp"
+#include "routes.hpp"
 
 #include <type_traits>
 
 namespace ph {
 namespace {
 
-constexpr int kSteps = 8;  // steps of a batch: staged and loaded together, and between two kept states of the training forward
+constexpr int kSteps = kSsmSteps;  // steps of a batch: staged and loaded together, and between two kept states of the training forward
 constexpr int kTaps = 4;   // most taps of the convolution; fewer are padded with zero taps in front
 constexpr int kMaxStates = 64;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -746,6 +747,7 @@ __global__ void __launch_bounds__(256) k_ssm_bwd_join(Args a, GradArgs ga) {
 // block's wavefronts in LDS; the parameters' gradients stay in LDS and registers over all the block's work. A block
 // takes the items row, row + rows, ... of its channel block, an item being a chunk of a sequence.
 constexpr int kOwn = 3 + kTaps;  // a channel's own sums in the gradient
+static_assert(kOwn == kSsmOwn, "LDS of a block");
 template <typename T, int MOST>
 __global__ void __launch_bounds__(256, 2) k_ssm_bwd(Args a, GradArgs ga) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -1192,39 +1194,12 @@ Args args_of(const ph_ssm_args& p) {
   return a;
 }
 
-// LDS of a block of nt threads: the lanes' slots, the staged rows and (gradient) the wavefronts' sums.
-size_t fwd_lds(int Q, int nt) { return (size_t)4 * (8 * Q * nt + 2 * 64 * Q); }
-size_t bwd_lds(int Q, int nt) {
-  const int waves = nt / 64;
-  return (size_t)4 * (12 * Q * nt + (2 + waves) * 64 * Q + waves * kSteps + 2 * kSteps + kOwn * nt);
-}
+int block_threads(const Args& a, bool grad) { return ssm_block_threads(a.per, a.Q, grad); }
+static_assert(ssm_bwd_lds(kMaxStates / 4, 64) <= 64 * 1024, "one wavefront of the most states");
 
-// Threads of a block: whole wavefronts over a group's channels, at most four and as LDS holds (N = 64: one in the gradient).
-int block_threads(const Args& a, bool grad) {
-  const long w = (a.per + 63) / 64;
-  int nt = 64 * (int)(w < 4 ? w : 4);
-  while (nt > 64 && (grad ? bwd_lds(a.Q, nt) : fwd_lds(a.Q, nt)) > 64 * 1024) nt -= 64;
-  return nt;
-}
-static_assert(4 * (12 * 16 * 64 + 3 * 64 * 16 + 3 * kSteps + kOwn * 64) <= 64 * 1024, "one wavefront at N = 64");
-
-// Blocks of nt threads that run at a time in the gradient: two wavefronts to a SIMD, whole blocks to a CU.
-long resident(int nt) { return 256L * (8 / (nt / 64)); }
-
-// Chunks of time: as many as make one round of blocks, in chunks of at least 32 steps (2048x8, two groups of 192 channels: a
-// chunk more and a second round gave 401 us both directions, 361 without). Chunks cost a second pass over their steps and
-// three launches (about 20 us), so sequences stay whole while one pass over all their steps is not longer than that: up
-// to 128 steps of 16 states forward, 64 in the gradient, whose steps take three times as long; the more the fewer the
-// states. (33 steps of 203x96x5 fp32 both directions: 104 us in two chunks, 84 whole.)
 int set_chunks(Args& a, bool grad) {
-  const int nt = block_threads(a, true);
   const long waves = a.B * a.G * ((a.per + 63) / 64);
-  long want = resident(nt) / (a.B * a.G * ((a.per + nt - 1) / nt));
-  const long most = (a.T + 31) / 32;
-  if (want > most) want = most;
-  if (want < 1 || (long)a.T * (8 + a.N) <= (grad ? 64 : 128) * (8 + 16)) want = 1;
-  a.chunk = (a.T + want - 1) / want;
-  a.chunk = (a.chunk + kSteps - 1) / kSteps * kSteps;
+  a.chunk = (int)ssm_chunk(a.T, a.B, a.G, a.per, a.N, grad);
   a.chunks = (a.T + a.chunk - 1) / a.chunk;
   PH_REQUIRE(a.chunks * waves < (1L << 31), "ssm: %ld sequences of %ld channels in %ld chunks of time", a.B, a.C, a.chunks);
   return PH_OK;
@@ -1233,7 +1208,7 @@ int set_chunks(Args& a, bool grad) {
 template <typename T>
 int fwd_t(Args& a, hipStream_t st) {
   const int nt = block_threads(a, false);
-  const size_t lds = fwd_lds(a.Q, nt);
+  const size_t lds = ssm_fwd_lds(a.Q, nt);
   a.blocks_c = (unsigned)((a.per + nt - 1) / nt);
   const unsigned blocks = (unsigned)(a.chunks * a.B * a.G * a.blocks_c);
   const int most = (kSteps * 8 * a.Q + nt - 1) / nt;
@@ -1261,17 +1236,17 @@ int bwd_t(Args& a, GradArgs& ga, int nt, const ParOut& po, hipStream_t st) {
   const int most = (kSteps * 8 * a.Q + nt - 1) / nt;
   if (a.chunks > 1) {
     const unsigned blocks = (unsigned)(a.chunks * a.B * a.G * a.blocks_c);
-    if (most <= 1) k_ssm_bwd_local<T, 1><<<blocks, nt, fwd_lds(a.Q, nt), st>>>(a, ga);
-    else if (most <= 4) k_ssm_bwd_local<T, 4><<<blocks, nt, fwd_lds(a.Q, nt), st>>>(a, ga);
-    else k_ssm_bwd_local<T, 16><<<blocks, nt, fwd_lds(a.Q, nt), st>>>(a, ga);
+    if (most <= 1) k_ssm_bwd_local<T, 1><<<blocks, nt, ssm_fwd_lds(a.Q, nt), st>>>(a, ga);
+    else if (most <= 4) k_ssm_bwd_local<T, 4><<<blocks, nt, ssm_fwd_lds(a.Q, nt), st>>>(a, ga);
+    else k_ssm_bwd_local<T, 16><<<blocks, nt, ssm_fwd_lds(a.Q, nt), st>>>(a, ga);
     PH_LAUNCH_CHECK();
     k_ssm_bwd_join<<<ceil_div((size_t)(a.B * a.C * 4 * a.Q), 256), 256, 0, st>>>(a, ga);
     PH_LAUNCH_CHECK();
   }
   const unsigned blocks = (unsigned)(ga.rows * a.G * a.blocks_c);
-  if (most <= 1) k_ssm_bwd<T, 1><<<blocks, nt, bwd_lds(a.Q, nt), st>>>(a, ga);
-  else if (most <= 4) k_ssm_bwd<T, 4><<<blocks, nt, bwd_lds(a.Q, nt), st>>>(a, ga);
-  else k_ssm_bwd<T, 16><<<blocks, nt, bwd_lds(a.Q, nt), st>>>(a, ga);
+  if (most <= 1) k_ssm_bwd<T, 1><<<blocks, nt, ssm_bwd_lds(a.Q, nt), st>>>(a, ga);
+  else if (most <= 4) k_ssm_bwd<T, 4><<<blocks, nt, ssm_bwd_lds(a.Q, nt), st>>>(a, ga);
+  else k_ssm_bwd<T, 16><<<blocks, nt, ssm_bwd_lds(a.Q, nt), st>>>(a, ga);
   PH_LAUNCH_CHECK();
   if (a.chunks > 1 && a.K > 1 && ga.dx) {
     k_ssm_halo<T><<<ceil_div((size_t)((a.chunks - 1) * a.B * (a.K - 1) * a.C), 256), 256, 0, st>>>(a, ga);
@@ -1385,7 +1360,7 @@ extern "C" int ph_ssm_scan_grad(const ph_ssm_args* p, const float* keep, const v
   const long G = a.G, bc = (a.per + nt - 1) / nt;
   a.blocks_c = (unsigned)bc;
   // blocks of a channel block: as many as run at a time, with as equal shares of the items as there are
-  const long items = a.B * a.chunks, most = resident(nt) / (G * bc) > 0 ? resident(nt) / (G * bc) : 1;
+  const long items = a.B * a.chunks, most = ssm_resident(nt) / (G * bc) > 0 ? ssm_resident(nt) / (G * bc) : 1;
   const long rounds = (items + most - 1) / most;
   ga.rows = (items + rounds - 1) / rounds;
   if (ga.rows < 1) ga.rows = 1;

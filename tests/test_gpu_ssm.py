@@ -192,6 +192,97 @@ def test_blocks_of_several_sequences(gpu, T, N, K, carry, dt):
         assert R.rel(g[k], v) <= 2e-5, k
 
 
+# (T, C, N, G, K, dtype, gate) of three sequences that both directions cut into chunks of 32 steps: whole last chunks and ones of
+# 1 to 7 steps, every number of taps, groups, several wavefronts and blocks of channels, any number of states.
+CHUNKED = [(160, 20, 16, 1, 4, torch.float32, True), (150, 70, 16, 1, 4, torch.float32, True), (129, 40, 16, 1, 4, torch.bfloat16, True),
+           (129, 40, 16, 1, 3, torch.float32, True), (161, 96, 16, 2, 4, torch.bfloat16, True), (130, 33, 16, 1, 4, torch.float32, False),
+           (131, 66, 16, 2, 2, torch.float32, True), (135, 20, 16, 1, 1, torch.float32, True), (200, 70, 16, 1, 0, torch.bfloat16, True),
+           (290, 24, 4, 1, 4, torch.float32, True), (210, 90, 7, 1, 2, torch.bfloat16, False), (140, 130, 24, 2, 3, torch.bfloat16, True),
+           (150, 300, 16, 1, 4, torch.bfloat16, True), (134, 40, 64, 1, 4, torch.float32, True)]
+
+
+def chunked(T, C, N, G, K, dt, gate, B=3):
+    """Half of the channels decay slowly, so that what a chunk starts from shows to its end; episodes end on and around the
+    chunks' borders, at the last step, and in one sequence never."""
+    s, c = inputs(T, B, C, N, G=G, K=K, dt=dt, gate=gate)
+    s["A"][::2] *= 0.05
+    c["done"].zero_()
+    for b, steps in enumerate(((31, 95, T - 1), (28, 30, 32, 62, 63, 127))):
+        c["done"][list(steps), b] = 1.0
+    return s, c
+
+
+@pytest.mark.parametrize("T,C,N,G,K,dt,gate", CHUNKED)
+def test_chunks_of_time(gpu, T, C, N, G, K, dt, gate):
+    # the bar of the head of this file for T steps
+    check(*chunked(T, C, N, G, K, dt, gate), bar=max(FP32, 3 * T * 2.0 ** -24))
+
+
+@pytest.mark.parametrize("K", [1, 2, 3, 4])
+def test_chunks_carry_in_place(gpu, K):
+    """h_out and win_out may be h0 and win0, where the first chunk reads what the last one writes; and two calls that hand the
+    state on are one."""
+    s, c = chunked(300, 40, 16, 1, K, torch.float32, True)
+    y, h, win, _ = forward(s, c)
+    rest = {k: s[k] for k in ("D", "z", "dt_bias", "conv_w", "conv_b")}
+    hs, ws = c["h0"].clone(), None if K < 2 else c["win0"].clone()
+    own = {k: v for k, v in c.items() if k not in ("h0", "win0")}
+    yp = D.ssm_scan(s["x"], s["delta"], s["A"], s["Bm"], s["Cm"], h0=hs, win0=ws, h_out=hs, win_out=ws, **rest, **own)
+    assert torch.equal(yp, y) and torch.equal(hs, h) and (K < 2 or torch.equal(ws, win))
+    hs, ws, first = c["h0"].clone(), None if K < 2 else c["win0"].clone(), c["first"]
+    for t in (0, 150):
+        part = {k: v[t:t + 150] if k in ("x", "delta", "Bm", "Cm", "z") else v for k, v in s.items()}
+        rest = {k: part[k] for k in ("D", "z", "dt_bias", "conv_w", "conv_b")}
+        done = c["done"][t:t + 150].contiguous()
+        yp = D.ssm_scan(part["x"], part["delta"], s["A"], part["Bm"], part["Cm"], done=done, first=first, h0=hs, win0=ws,
+                        h_out=hs, win_out=ws, **rest)
+        assert R.rel(yp, y[t:t + 150]) <= 2 * 3 * 300 * 2.0 ** -24
+        first = done[-1].contiguous()
+    assert R.rel(hs, h) <= 2 * 3 * 300 * 2.0 ** -24 and (K < 2 or torch.equal(ws, win))
+
+
+def test_chunks_keep_non_finite_values_in_their_episode(gpu):
+    """Infinities and NaN in the first and the last chunk; the episode between them is the same bit for bit."""
+    T, lo, hi = 150, 40, 101
+    s, c = chunked(T, 40, 16, 1, 4, torch.float32, True)
+    c["done"].zero_()
+    c["done"][[lo - 1, hi - 1]] = 1.0
+    bad = {k: v.clone() if k in ("x", "delta", "Bm", "Cm", "z") else v for k, v in s.items()}
+    bad["x"][20], bad["x"][lo - 1], bad["x"][hi] = float("inf"), float("inf"), float("-inf")
+    bad["Bm"][25], bad["Cm"][140], bad["z"][hi] = float("nan"), float("inf"), float("nan")
+    dy = cu(20, T, 3, 40)
+    y, h, _, saved = forward(s, c)
+    g = backward(s, c, saved, dy)
+    yb, hb, _, kept = forward(bad, c)
+    gb = backward(bad, c, kept, dy)
+    assert torch.isfinite(y).all() and not torch.isfinite(yb[:lo]).all() and not torch.isfinite(yb[hi:]).all()
+    assert torch.equal(yb[lo:hi], y[lo:hi])
+    for k in ("dx", "ddelta", "dBm", "dCm", "dz"):
+        assert torch.equal(gb[k][lo:hi], g[k][lo:hi]), k
+
+
+def test_chunks_in_a_graph(gpu):
+    s, c = chunked(150, 72, 16, 1, 4, torch.bfloat16, True)
+    dy = cu(20, 150, 3, 72, dtype=torch.bfloat16)
+
+    def both():
+        y, h, win, saved = forward(s, c)
+        return [y, h, win, *backward(s, c, saved, dy).values()]
+    ref = [t.clone() for t in both()]
+    g, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st), torch.cuda.graph(g, stream=st):
+        out = both()
+    torch.cuda.current_stream().wait_stream(st)
+    for _ in range(3):
+        for t in out:
+            t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ref, out))
+        assert all(torch.equal(p, q) for p, q in zip(ref, both()))
+
+
 def test_every_step_ends_an_episode(gpu):
     s, c = inputs(40, 2, 16, 4, K=4)
     c["done"].fill_(1.0)

@@ -4,6 +4,8 @@ import subprocess
 
 import pytest
 
+import test_gpu_ssm as ssm
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 DRIVER = r"""
@@ -17,6 +19,8 @@ int main(int argc, char** argv) {
   for (int i = 2; i < argc && i < 10; i++) a[i - 2] = std::atol(argv[i]);
   long r = -1;
   if (!std::strcmp(argv[1], "dma_offsets_fit")) r = dma_offsets_fit(a[0], a[1], a[2]);
+  if (!std::strcmp(argv[1], "ssm_chunk")) r = ssm_chunk(a[0], a[1], a[2], a[3], (int)a[4], a[5]);
+  if (!std::strcmp(argv[1], "ssm_block_threads")) r = ssm_block_threads(a[0], (int)a[1], a[2]);
   std::printf("%ld\n", r);
   return 0;
 }
@@ -45,3 +49,27 @@ def test_dma_offsets_fit(route):
         assert not route("dma_offsets_fit", tn, most + 8, 8) and not route("dma_offsets_fit", tn, 8, most + 8)
         last = (rows - 1) * most + (255 if tn else most - 1)
         assert last < 2 ** 31
+
+
+@pytest.mark.parametrize("T,C,N,G,K,dt,gate", ssm.CHUNKED)
+def test_ssm_tests_reach_chunks(route, T, C, N, G, K, dt, gate):
+    """Their episodes end around the borders of chunks of 32 steps, in both directions."""
+    for grad in (0, 1):
+        assert route("ssm_chunk", T, 3, G, C // G, N, grad) == 32 < T
+
+
+def test_ssm_tests_reach_every_last_chunk(route):
+    assert {T % 32 for T, *_ in ssm.CHUNKED} >= {0, 1, 2, 3, 6, 7} and {K for _, _, _, _, K, *_ in ssm.CHUNKED} == set(range(5))
+    # blocks of one and of several channel blocks, and of one and four wavefronts
+    blocks = [(route("ssm_block_threads", C // G, (N + 3) // 4, 1), C // G) for _, C, N, G, *_ in ssm.CHUNKED]
+    assert {nt for nt, _ in blocks} >= {64, 128, 256} and any(nt < per for nt, per in blocks)
+    for T in (150, 300):
+        assert route("ssm_chunk", T, 3, 1, 40, 16, 0) == 32
+
+
+# (T, B, G, channels of a group, states, gradient) and the steps of a chunk
+@pytest.mark.parametrize("T,B,G,per,N,grad,chunk", [(128, 1, 1, 64, 16, 0, 128), (129, 1, 1, 64, 16, 0, 32), (64, 1, 1, 64, 16, 1, 64),
+                                                    (65, 1, 1, 64, 16, 1, 24), (8192, 2, 1, 512, 16, 0, 64), (2048, 8, 2, 192, 16, 1, 64),
+                                                    (33, 203, 1, 96, 5, 1, 40), (64, 2048, 1, 512, 16, 1, 64), (1, 1, 1, 1, 1, 0, 8)])
+def test_ssm_chunk(route, T, B, G, per, N, grad, chunk):
+    assert route("ssm_chunk", T, B, G, per, N, grad) == chunk
