@@ -1900,25 +1900,18 @@ int pad_operands(PhGemmDesc& d, int vec, hipStream_t st) {
 template <int GLU, bool TB>
 int launch_glu(const GemmArgs& g, int dtype, hipStream_t st) {
   auto tiles = [&](long bm, long bn) { return (unsigned)((g.M + bm - 1) / bm * ((g.N + bn - 1) / bn)); };
-  if (dtype == PH_BF16) {
-    // tiles as for a plain NT product: 256x256 or 256x128 from 512 of 256x128 on, whichever pads the columns less
-    if (TB && tiles(256, 128) >= 512 && dma_offsets_fit(false, g.lda, g.ldb)) {
-      const long n256 = (g.N + 255) / 256 * 256, n128 = (g.N + 127) / 128 * 128;
-      if (n256 <= n128 + n128 / 16)
-        k_gemm_nt_dma<256, 256, uint16_t, false, 4, 4, 4, false, GLU><<<tiles(256, 256), 1024, 0, st>>>(g);
-      else k_gemm_nt_dma<256, 128, uint16_t, false, 2, 2, 3, false, GLU><<<tiles(256, 128), 256, 0, st>>>(g);
-    } else if (tiles(128, 128) >= 128) {
-      k_gemm_bf16<128, 128, 64, 2, 2, false, TB, uint16_t, uint16_t, uint16_t, false, GLU><<<tiles(128, 128), 256, 0, st>>>(g);
-    } else {
-      k_gemm_bf16<64, 64, 64, 2, 2, false, TB, uint16_t, uint16_t, uint16_t, false, GLU><<<tiles(64, 64), 256, 0, st>>>(g);
-    }
-  } else if (tiles(128, 128) >= 512) {
-    // two blocks of 128x128 to a CU; below that 64x64 tiles keep more of the chip at work (6699x536x208: 49 us in 265 tiles of
-    // 128x128, 31 in 64x64; 6699x1072x208, 477 tiles: 48, 45 in 64x64). Their k tiles of 16 let eight blocks share a CU's
-    // LDS and waste less of a short K (6699x1072x208 at k tiles of 32: 50 us).
-    k_gemm_f32<128, 128, 32, false, TB, float, GLU><<<tiles(128, 128), 256, 0, st>>>(g);
-  } else {
-    k_gemm_f32<64, 64, 16, false, TB, float, GLU><<<tiles(64, 64), 256, 0, st>>>(g);
+  const GluTile tile = glu_tile(dtype == PH_BF16, TB, g.M, g.N, g.lda, g.ldb);
+  if (dtype != PH_BF16) {
+    if (tile == kGlu128) k_gemm_f32<128, 128, 32, false, TB, float, GLU><<<tiles(128, 128), 256, 0, st>>>(g);
+    else k_gemm_f32<64, 64, 16, false, TB, float, GLU><<<tiles(64, 64), 256, 0, st>>>(g);
+  } else if (tile == kGlu128) {
+    k_gemm_bf16<128, 128, 64, 2, 2, false, TB, uint16_t, uint16_t, uint16_t, false, GLU><<<tiles(128, 128), 256, 0, st>>>(g);
+  } else if (tile == kGlu64) {
+    k_gemm_bf16<64, 64, 64, 2, 2, false, TB, uint16_t, uint16_t, uint16_t, false, GLU><<<tiles(64, 64), 256, 0, st>>>(g);
+  } else if constexpr (TB) {
+    if (tile == kGlu256)
+      k_gemm_nt_dma<256, 256, uint16_t, false, 4, 4, 4, false, GLU><<<tiles(256, 256), 1024, 0, st>>>(g);
+    else k_gemm_nt_dma<256, 128, uint16_t, false, 2, 2, 3, false, GLU><<<tiles(256, 128), 256, 0, st>>>(g);
   }
   PH_LAUNCH_CHECK();
   return PH_OK;

@@ -151,6 +151,23 @@ inline RollForm rollout_form(bool bf16, long N, long H) {
   return c32 <= c128 ? kRoll32 : kRoll128;
 }
 
+// ---- Gated feed-forward, the products with the units in their epilogue ------------------------------------
+// Tiles of an M x N product (N: the projections, or the units' gradients). bf16 as for a plain NT product: 256x256 or 256x128 from
+// 512 of 256x128 on, whichever pads the columns less, else 128x128 from 128 tiles on. fp32: two blocks of 128x128 to a CU;
+// below that 64x64 tiles keep more of the chip at work (6699x536x208: 49 us in 265 tiles of 128x128, 31 in 64x64;
+// 6699x1072x208, 477 tiles: 48, 45 in 64x64). Their k tiles of 16 let eight blocks share a CU's LDS and waste less of a short
+// K (6699x1072x208 at k tiles of 32: 50 us).
+enum GluTile { kGlu64 = 0, kGlu128, kGlu256x128, kGlu256 };
+inline GluTile glu_tile(bool bf16, bool nt, long M, long N, long lda, long ldb) {
+  const auto tiles = [&](long bm, long bn) { return (M + bm - 1) / bm * ((N + bn - 1) / bn); };
+  if (!bf16) return tiles(128, 128) >= 512 ? kGlu128 : kGlu64;
+  if (nt && tiles(256, 128) >= 512 && dma_offsets_fit(false, lda, ldb)) {
+    const long n256 = (N + 255) / 256 * 256, n128 = (N + 127) / 128 * 128;
+    return n256 <= n128 + n128 / 16 ? kGlu256 : kGlu256x128;
+  }
+  return tiles(128, 128) >= 128 ? kGlu128 : kGlu64;
+}
+
 // ---- Selective state-space scan ---------------------------------------------------------------------------
 // LDS bytes of a block of nt threads for 4 Q states a channel: the lanes' slots, the staged rows and (gradient) the wavefronts'
 // sums and the channels' own, kSsmOwn each.

@@ -62,6 +62,35 @@ def test_many_rows(gpu, M, Dm, F, dt):
     check(*case(M, Dm, F, dt))
 
 
+# (M, D, F, dtype) whose products with the units in the epilogue take the larger tiles, with ragged rows, columns and sums, and the
+# tiles of the units and of their gradient
+LARGE = [(16500, 40, 1000, torch.bfloat16, "256", "256"), (16500, 40, 520, torch.bfloat16, "256x128", "128"),
+         (33000, 24, 536, torch.bfloat16, "256x128", "256x128"), (1500, 72, 1400, torch.bfloat16, "128", "128"),
+         (5000, 40, 1668, torch.float32, "128", "128"), (2000, 24, 4100, torch.float32, "128", "128")]
+
+
+@pytest.mark.parametrize("M,Dm,F,dt,units,grad", LARGE)
+def test_large_tiles(gpu, M, Dm, F, dt, units, grad):
+    check(*case(M, Dm, F, dt))
+
+
+@pytest.mark.parametrize("M,F", [(16500, 1000), (16500, 520), (1500, 1400)])
+def test_kept_pairs_of_large_tiles(gpu, M, F):
+    """As test_kept_pairs; of tens of millions of values |v| stays under 6."""
+    x, wi, wo, _ = case(M, 64, F, torch.bfloat16)
+    _, (pf, h) = D.gated_ffn(x, wi, wo, save=True)
+    row = pf.cpu().contiguous().view(torch.uint8).numpy().reshape(M, 6 * F)
+    b = np.zeros((M, 2 * F, 4), np.uint8)
+    b[..., 2:] = row[:, :4 * F].reshape(M, 2 * F, 2)
+    b[..., 1] = row[:, 4 * F:]
+    got = torch.from_numpy(b.view(np.float32)[..., 0]).double()
+    a, v = (x.double().cpu() @ wi.double().cpu()[k::2].T for k in (0, 1))
+    s = 1 / (1 + torch.exp(-a))
+    ref = torch.stack([v * s * (1 + a * (1 - s)), a * s], -1).reshape(M, -1)
+    assert ((got - ref).abs() <= 2.0 ** -15 * ref.abs() + 1.5e-4).all()
+    assert R.rel(h, a * s * v) <= R.BF16 + 1e-5
+
+
 def test_fp32_weight_gradients_of_bf16(gpu):
     x, wi, wo, dy = case(700, 128, 264, torch.bfloat16)
     _, _, dwi, dwo = check(x, wi, wo, dy, dw_dtype=torch.float32)

@@ -3,7 +3,9 @@ import os
 import subprocess
 
 import pytest
+import torch
 
+import test_gpu_ffn as ffn
 import test_gpu_ssm as ssm
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -21,6 +23,7 @@ int main(int argc, char** argv) {
   if (!std::strcmp(argv[1], "dma_offsets_fit")) r = dma_offsets_fit(a[0], a[1], a[2]);
   if (!std::strcmp(argv[1], "ssm_chunk")) r = ssm_chunk(a[0], a[1], a[2], a[3], (int)a[4], a[5]);
   if (!std::strcmp(argv[1], "ssm_block_threads")) r = ssm_block_threads(a[0], (int)a[1], a[2]);
+  if (!std::strcmp(argv[1], "glu_tile")) r = glu_tile(a[0], a[1], a[2], a[3], a[4], a[5]);
   std::printf("%ld\n", r);
   return 0;
 }
@@ -73,3 +76,23 @@ def test_ssm_tests_reach_every_last_chunk(route):
                                                     (33, 203, 1, 96, 5, 1, 40), (64, 2048, 1, 512, 16, 1, 64), (1, 1, 1, 1, 1, 0, 8)])
 def test_ssm_chunk(route, T, B, G, per, N, grad, chunk):
     assert route("ssm_chunk", T, B, G, per, N, grad) == chunk
+
+
+TILES = ("64", "128", "256x128", "256")
+
+
+@pytest.mark.parametrize("M,Dm,F,dt,units,grad", ffn.LARGE)
+def test_ffn_tests_reach_their_tiles(route, M, Dm, F, dt, units, grad):
+    bf, up = dt is torch.bfloat16, lambda n: (n + 7) // 8 * 8
+    assert M > 64  # fewer rows have kernels of their own
+    assert TILES[route("glu_tile", bf, 1, M, 2 * up(F), up(Dm), up(Dm))] == units
+    nt = M >= 2048  # from there on the gradient's product takes transposed weights
+    assert TILES[route("glu_tile", bf, nt, M, up(F), up(Dm), up(Dm) if nt else up(F))] == grad
+
+
+@pytest.mark.parametrize("bf,nt,M,N,ld,tile", [(1, 1, 65536, 2752, 512, "256"), (1, 1, 65536, 1376, 512, "256x128"), (1, 1, 2048, 16384, 16, "256"),
+                                               (1, 1, 2048, 16384, 2 ** 23 + 8, "128"), (1, 0, 65536, 2752, 512, "128"),
+                                               (1, 1, 2048, 1024, 512, "128"), (1, 1, 300, 256, 128, "64"), (0, 1, 6699, 1072, 208, "64"),
+                                               (0, 1, 65536, 512, 512, "128")])
+def test_glu_tile(route, bf, nt, M, N, ld, tile):
+    assert TILES[route("glu_tile", bf, nt, M, N, ld, ld)] == tile
