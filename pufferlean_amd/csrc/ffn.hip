@@ -7,7 +7,7 @@
 //
 // All on the matrix cores: 6 M D F operations forward and 12 M D F backward, against which the activations' traffic is
 // small; the epilogues (glu.hpp) keep the projections and dh from ever being written. bf16 rounds h and dab once each from
-// fp32, as operands of bf16 products; p and f keep 24 bits.
+// fp32, as operands of bf16 products (up to 64 rows only of those of the weights' gradients); p and f keep 24 bits.
 //
 // Measured: 65536 x 512 x 1376 bf16 both directions 1234 us, 673 TFLOP/s (357 us h, 298 dab, 350 y and dx, 337 the weights'
 // gradients); the products' 592 us at the rate of a large library product are out of reach of their short K of 512.
@@ -18,6 +18,8 @@
 #include "common.hpp"
 #include "glu.hpp"
 #include "kernels.hpp"
+
+#include <type_traits>
 
 namespace ph {
 namespace {
@@ -91,7 +93,8 @@ struct Layer {
 // Up to 64 rows are bound by the weights' bytes and by latency, so the weights go from memory straight into the operand
 // registers of 16-wide products (16 weight rows to a wavefront, 16 bytes of one to a lane), with the rows of x as the
 // other operand; the block's wavefronts share the reduction and are added through LDS. fp32 takes four products of
-// 16x16x4 for the four values of a lane: the same k of both operands, in an order of its own.
+// 16x16x4 for the four values of a lane: the same k of both operands, in an order of its own. What the first product leaves for
+// the second is a few KB, so of bf16 blocks it stays fp32 and enters as two bf16 halves, 16 bits: y and dx are rounded once.
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 constexpr int kFewRows = 64;
@@ -107,6 +110,28 @@ template <> struct Few<uint16_t> {
   static __device__ __forceinline__ f32x4_t mma(Frag a, Frag b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
+  // fp32 values as the sum of two of bf16: the upper half (cut off, so that no finite value becomes infinite), and what is left
+  // of it, rounded; nothing is left of an infinity.
+  struct Halves {
+    Frag hi, lo;
+  };
+  static __device__ __forceinline__ Halves load(const float* row, long k, long K) {
+    f32x4_t v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    if (k < K) {
+      v[0] = *reinterpret_cast<const f32x4_t*>(row + k);
+      v[1] = *reinterpret_cast<const f32x4_t*>(row + k + 4);
+    }
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float a = v[i / 2][2 * (i % 2)], b = v[i / 2][2 * (i % 2) + 1];
+      hi[i] = keep_hi(a, b);
+      const float ha = __builtin_bit_cast(float, hi[i] << 16), hb = __builtin_bit_cast(float, hi[i] & 0xffff0000u);
+      lo[i] = bf16x2_rne(a == ha ? 0.f : a - ha, b == hb ? 0.f : b - hb);
+    }
+    return {__builtin_bit_cast(Frag, make_uint4(hi[0], hi[1], hi[2], hi[3])), __builtin_bit_cast(Frag, make_uint4(lo[0], lo[1], lo[2], lo[3]))};
+  }
+  static __device__ __forceinline__ f32x4_t mma(Frag a, const Halves& b, f32x4_t c) { return mma(a, b.hi, mma(a, b.lo, c)); }
 };
 template <> struct Few<float> {
   static constexpr int kPer = 4;
@@ -145,27 +170,29 @@ __device__ __forceinline__ void put1(uint16_t* p, float a) { *p = bf16_rne(a); }
 __device__ __forceinline__ void put1(float* p, float a) { *p = a; }
 
 // The product of few rows: out[m][n] = sum_k x[m][k] w[n][k]. kIn: n are the projections, out is h (and pf); kGrad: n are
-// units, out is dab, from pf; kPlain: out has N columns. K and the leading dimensions are multiples of 8.
+// units, out is dab, from pf; kPlain: out has N columns. K and the leading dimensions are multiples of 8. X: the type of x. wide
+// receives h (dab) in fp32, in out's layout; of the two at least one is there.
 enum : int { kIn, kGrad, kPlain };
 struct FewArgs {
   const void *x, *w;
   long ldx, ldw, K;
   int M, N, act;
   void* out;
+  float* wide;
   long ldo;
   void* pf;
   long ldpf;
 };
-template <typename T, int MODE, int MT, int WAVES>
+template <typename T, typename X, int MODE, int MT, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) k_few(FewArgs g) {
   __shared__ f32x4_t red[WAVES][MT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, w0 = blockIdx.x * 16;
   const T* wr = (const T*)g.w + (long)min(w0 + r, g.N - 1) * g.ldw;  // rows past N and M repeat the last: not stored
-  const T* xr[MT];
+  const X* xr[MT];
   f32x4_t acc[MT];
 #pragma unroll
   for (int m = 0; m < MT; m++) {
-    xr[m] = (const T*)g.x + (long)min(16 * m + r, g.M - 1) * g.ldx;
+    xr[m] = (const X*)g.x + (long)min(16 * m + r, g.M - 1) * g.ldx;
     acc[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
   constexpr int kPer = Few<T>::kPer, kStep = 4 * kPer;
@@ -186,22 +213,24 @@ __global__ void __launch_bounds__(64 * WAVES) k_few(FewArgs g) {
   // the lane has columns n..n+3 of one row
   const int row = 16 * wave + r, n = w0 + 4 * (lane >> 4);
   if (row >= g.M || n >= g.N) return;
-  T* out = (T*)g.out + (long)row * g.ldo;
+  T* out = g.out ? (T*)g.out + (long)row * g.ldo : nullptr;
+  float* wide = MODE != kPlain && g.wide ? g.wide + (long)row * g.ldo : nullptr;
   T* pf = g.pf ? (T*)g.pf + (long)row * g.ldpf : nullptr;
   if constexpr (MODE == kIn) {
     float f0, d0, f1, d1;
     glu_act(g.act, s[0], f0, d0);
     glu_act(g.act, s[2], f1, d1);
-    put(out + n / 2, f0 * s[1], f1 * s[3]);
-    if (pf) {
-      keep4(pf, g.ldpf, n, s[1] * d0, f0, s[3] * d1, f1);
-    }
+    const float h0 = f0 * s[1], h1 = f1 * s[3];
+    if (out) put(out + n / 2, h0, h1);
+    if (wide) put(wide + n / 2, h0, h1);
+    if (pf) keep4(pf, g.ldpf, n, s[1] * d0, f0, s[3] * d1, f1);
   } else if constexpr (MODE == kGrad) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       float p, f;
       kept2(pf, g.ldpf, 2 * (n + i), p, f);
-      put(out + 2 * (n + i), s[i] * p, s[i] * f);
+      if (out) put(out + 2 * (n + i), s[i] * p, s[i] * f);
+      if (wide) put(wide + 2 * (n + i), s[i] * p, s[i] * f);
     }
   } else {
 #pragma unroll
@@ -210,18 +239,20 @@ __global__ void __launch_bounds__(64 * WAVES) k_few(FewArgs g) {
   }
 }
 
-template <typename T, int MODE>
+template <typename T, typename X, int MODE>
 int few_t(const FewArgs& g, hipStream_t st) {
   const unsigned blocks = (unsigned)((g.N + 15) / 16);
-  if (g.M <= 16) k_few<T, MODE, 1, 8><<<blocks, 512, 0, st>>>(g);
-  else if (g.M <= 32) k_few<T, MODE, 2, 8><<<blocks, 512, 0, st>>>(g);
-  else k_few<T, MODE, 4, 8><<<blocks, 512, 0, st>>>(g);
+  if (g.M <= 16) k_few<T, X, MODE, 1, 8><<<blocks, 512, 0, st>>>(g);
+  else if (g.M <= 32) k_few<T, X, MODE, 2, 8><<<blocks, 512, 0, st>>>(g);
+  else k_few<T, X, MODE, 4, 8><<<blocks, 512, 0, st>>>(g);
   PH_LAUNCH_CHECK();
   return PH_OK;
 }
+// x in dtype, of kPlain in fp32.
 template <int MODE>
 int few(int dtype, const FewArgs& g, hipStream_t st) {
-  return dtype == PH_BF16 ? few_t<uint16_t, MODE>(g, st) : few_t<float, MODE>(g, st);
+  typedef std::conditional_t<MODE == kPlain, float, uint16_t> X;
+  return dtype == PH_BF16 ? few_t<uint16_t, X, MODE>(g, st) : few_t<float, float, MODE>(g, st);
 }
 
 int product(int ta, int tb, size_t M, size_t N, size_t K, int dtype, const void* A, size_t lda, const void* B, size_t ldb,
@@ -311,7 +342,10 @@ extern "C" int ph_ffn(int dtype, int act, size_t M, size_t D, size_t F, const vo
   if (!x_ok) c.want(M * Dp, c.e);
   if (!wi_ok) c.want(2 * Fp * Dp, c.e);
   if (!wo_ok) c.want(D * Fp, c.e);
-  if (!h) c.want(M * Fp, c.e);
+  // the second product's operand where h is not it: few rows of bf16 units take it in fp32
+  const bool few_rows = M <= (size_t)kFewRows, wide = few_rows && dtype == PH_BF16;
+  if (wide) c.want(M * Fp, 4);
+  else if (!h) c.want(M * Fp, c.e);
   PH_TRY(c.take_all());
   Layer lay;
   auto padded = [&](const void*& p, size_t rows, size_t cols, size_t ld, size_t rows_p, size_t cols_p) {
@@ -327,14 +361,15 @@ extern "C" int ph_ffn(int dtype, int act, size_t M, size_t D, size_t F, const vo
   if (!wi_ok) PH_TRY(padded(w_in, 2 * F, D, D, 2 * Fp, Dp));
   if (!wo_ok) PH_TRY(padded(w_out, D, F, F, D, Fp));
   PH_TRY(lay.run(dtype, c.st));
-  if (!h) h = c.take(M * Fp, c.e);
-  if (M <= (size_t)kFewRows) {
+  float* hw = wide ? (float*)c.take(M * Fp, 4) : nullptr;
+  if (!h && !wide) h = c.take(M * Fp, c.e);
+  if (few_rows) {
     FewArgs g{};
     g.x = x; g.ldx = (long)ldx; g.w = w_in; g.ldw = g.K = (long)Dp; g.M = (int)M; g.N = (int)(2 * Fp); g.act = act;
-    g.out = h; g.ldo = (long)Fp; g.pf = pf; g.ldpf = keep_pitch(dtype, (long)Fp);
+    g.out = h; g.wide = hw; g.ldo = (long)Fp; g.pf = pf; g.ldpf = keep_pitch(dtype, (long)Fp);
     PH_TRY(few<kIn>(dtype, g, c.st));
     FewArgs o{};
-    o.x = h; o.ldx = (long)Fp; o.w = w_out; o.ldw = o.K = (long)Fp; o.M = (int)M; o.N = (int)D; o.out = y; o.ldo = (long)ldy;
+    o.x = wide ? hw : h; o.ldx = (long)Fp; o.w = w_out; o.ldw = o.K = (long)Fp; o.M = (int)M; o.N = (int)D; o.out = y; o.ldo = (long)ldy;
     return few<kPlain>(dtype, o, c.st);
   }
   GluProduct g{};
@@ -363,6 +398,7 @@ extern "C" int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, con
   // are faster by more than the copies take, and the kernel of few rows has no other form. In between the products
   // take the weights as they are (or padded).
   const bool few_rows = M <= (size_t)kFewRows, trans = M >= kTransposeRows || few_rows;
+  const bool wide = few_rows && dtype == PH_BF16;  // dx from fp32 gradients of the projections
   const bool wo_ok = !trans && c.whole(w_out, F, F, Fp) && D == Dp, wi_ok = !trans && c.whole(w_in, D, D, Dp) && F == Fp;
   const bool need_dab = dx || dw_in;
   if (!x_ok && dw_in) c.want(M * Dp, c.e);
@@ -370,7 +406,8 @@ extern "C" int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, con
   if (need_dab) {
     if (!wo_ok) c.want(Fp * Dp, c.e);
     if (!wi_ok && dx) c.want(2 * Fp * Dp, c.e);
-    c.want(M * 2 * Fp, c.e);
+    if (!wide || dw_in) c.want(M * 2 * Fp, c.e);
+    if (wide && dx) c.want(M * 2 * Fp, 4);
   }
   if (!w_ok) c.want(2 * Fp * Dp, we), c.want(Fp * Dp, we);
   PH_TRY(c.take_all());
@@ -390,15 +427,17 @@ extern "C" int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, con
     lddy = Dp;
   }
   void* dab = nullptr;
+  float* dabw = nullptr;
   if (need_dab) {
     if (!wo_ok) PH_TRY(laid(w_out, D, F, F, Dp, Fp, trans));
     if (!wi_ok && dx) PH_TRY(laid(w_in, 2 * F, D, D, 2 * Fp, Dp, trans));
-    dab = c.take(M * 2 * Fp, c.e);
+    if (!wide || dw_in) dab = c.take(M * 2 * Fp, c.e);
+    if (wide && dx) dabw = (float*)c.take(M * 2 * Fp, 4);
   }
   PH_TRY(lay.run(dtype, c.st));
   if (need_dab && few_rows) {
     FewArgs g{};
-    g.x = dy; g.ldx = (long)lddy; g.w = w_out; g.ldw = g.K = (long)Dp; g.M = (int)M; g.N = (int)Fp; g.out = dab; g.ldo = (long)(2 * Fp);
+    g.x = dy; g.ldx = (long)lddy; g.w = w_out; g.ldw = g.K = (long)Dp; g.M = (int)M; g.N = (int)Fp; g.out = dab; g.wide = dabw; g.ldo = (long)(2 * Fp);
     g.pf = const_cast<void*>(pf); g.ldpf = keep_pitch(dtype, (long)Fp);
     PH_TRY(few<kGrad>(dtype, g, c.st));
   } else if (need_dab) {
@@ -423,7 +462,7 @@ extern "C" int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, con
   // dx last: it may be written over x or dy
   if (dx && few_rows) {
     FewArgs g{};
-    g.x = dab; g.ldx = (long)(2 * Fp); g.w = w_in; g.ldw = g.K = (long)(2 * Fp); g.M = (int)M; g.N = (int)D; g.out = dx; g.ldo = (long)lddx;
+    g.x = wide ? dabw : dab; g.ldx = (long)(2 * Fp); g.w = w_in; g.ldw = g.K = (long)(2 * Fp); g.M = (int)M; g.N = (int)D; g.out = dx; g.ldo = (long)lddx;
     PH_TRY(few<kPlain>(dtype, g, c.st));
   } else if (dx) PH_TRY(product(0, trans, M, D, 2 * Fp, dtype, dab, 2 * Fp, w_in, trans ? 2 * Fp : Dp, dtype, dx, lddx, c.st));
   return out.run(dw_dtype, c.st);

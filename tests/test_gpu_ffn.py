@@ -91,6 +91,38 @@ def test_kept_pairs_of_large_tiles(gpu, M, F):
     assert R.rel(h, a * s * v) <= R.BF16 + 1e-5
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("M,Dm,F", [(1, 64, 96), (8, 512, 344), (16, 128, 128), (17, 96, 203), (33, 203, 64), (64, 64, 96), (40, 7, 5)])
+def test_few_rows_round_once(gpu, M, Dm, F, act):
+    """Up to 64 rows y and dx are rounded once, by 2^-8 of their own size at most. What enters the second products keeps 16 bits (a
+    share 2^-16 of each term), of dx also the pairs (2^-15); the fp32 sums' own error, 2^-24 of up to 512 terms each way, is
+    within another 2^-16 of the terms."""
+    x, wi, wo, dy = case(M, Dm, F, torch.bfloat16)
+    y, saved = D.gated_ffn(x, wi, wo, act=act, save=True)
+    assert torch.equal(D.gated_ffn(x, wi, wo, act=act), y)
+    dx, _, _ = D.gated_ffn_grad(x, wi, wo, saved, dy, act=act)
+    x, wi, wo, dy = (t.double().cpu() for t in (x, wi, wo, dy))
+    a, v = ((x @ wi[k::2].T).requires_grad_(True) for k in (0, 1))
+    h = R.glu(a, v, act)
+    da, dv = torch.autograd.grad(h, (a, v), dy @ wo)
+    h, dab = h.detach(), torch.stack([da, dv], -1).reshape(M, -1)
+    for got, l, r, eps in ((y, h, wo.T, 2 * 2.0 ** -16), (dx, dab, wi, 4 * 2.0 ** -16)):
+        assert ((got.double().cpu() - l @ r).abs() <= 2.0 ** -8 * (l @ r).abs() + eps * (l.abs() @ r.abs())).all()
+
+
+def test_few_rows_keep_infinities(gpu):
+    """An infinite unit is no NaN in the product that follows, and neither is the largest finite one."""
+    bf = dict(device="cuda", dtype=torch.bfloat16)
+    x, wi, wo = torch.zeros(2, 8, **bf), torch.zeros(16, 8, **bf), torch.zeros(8, 8, **bf)
+    x[0, 0] = x[1, 1] = 1.0
+    wi[0, 0] = wi[1, 0] = 2.0 ** 70  # unit 0 of row 0 is 2^140, past fp32
+    wi[2, 1], wi[3, 1] = 2.0 ** 64, 2.0 ** 64 * (1 - 2.0 ** -8)  # unit 1 of row 1 is 2^128 (1 - 2^-8), the largest bf16
+    wo[0, 0], wo[1, 1], wo[2, 1] = 1.0, 0.5, 0.25
+    y = D.gated_ffn(x, wi, wo)
+    top = 2.0 ** 127 * (1 - 2.0 ** -8)
+    assert y[0, 0] == float("inf") and torch.equal(y[1, :3], torch.tensor([0.0, top, top / 2], **bf))
+
+
 def test_fp32_weight_gradients_of_bf16(gpu):
     x, wi, wo, dy = case(700, 128, 264, torch.bfloat16)
     _, _, dwi, dwo = check(x, wi, wo, dy, dw_dtype=torch.float32)
