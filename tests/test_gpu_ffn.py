@@ -260,6 +260,24 @@ def test_kept_pairs(gpu, M, act):
     assert (np.abs(got - ref) <= 2.0 ** -15 * np.abs(ref) + 1e-4).all()
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,Dm,F", [(8, 64, 96), (40, 203, 33), (300, 203, 64), (2100, 64, 96)])
+def test_gradients_left_out(gpu, M, Dm, F, dt):
+    """Each of dx, dw_in and dw_out may be left out; the others stay the same."""
+    x, wi, wo, dy = case(M, Dm, F, dt)
+    _, saved = D.gated_ffn(x, wi, wo, save=True)
+    ref = D.gated_ffn_grad(x, wi, wo, saved, dy)
+    pf, h = saved
+    code = L.PH_F32 if dt is torch.float32 else L.PH_BF16
+    for keep in range(1, 8):
+        out = [torch.full_like(t, 7.0) if keep >> i & 1 else None for i, t in enumerate(ref)]
+        p = [None if t is None else t.data_ptr() for t in out]
+        L.call("ph_ffn_grad", code, L.PH_ACT_SILU, M, Dm, F, x.data_ptr(), Dm, wi.data_ptr(), wo.data_ptr(), pf.data_ptr(), h.data_ptr(),
+               dy.data_ptr(), Dm, p[0], Dm, code, p[1], p[2], D._stream())
+        for a, b in zip(out, ref):
+            assert a is None or torch.equal(a, b), keep
+
+
 def test_refusals(gpu):
     x, wi, wo, dy = case(4, 16, 24, torch.float32)
     with pytest.raises(TypeError):

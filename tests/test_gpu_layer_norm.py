@@ -189,6 +189,26 @@ def test_graph_replays(gpu):
         (torch.ones(1000, device="cuda") * 2).sum().item()
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,C", [(3, 96), (600, 96), (130, 203), (130, 2049)])
+def test_results_left_out(gpu, M, C, dt):
+    """The statistics, dw and db may each be left out; the others stay the same."""
+    x, dy, w, b = case(M, C, dt)
+    ref = D.layer_norm(x, w, b)
+    code = L.PH_F32 if dt is torch.float32 else L.PH_BF16
+    y = torch.full_like(x, 7.0)
+    L.call("ph_layer_norm", code, x.data_ptr(), C, M, C, w.data_ptr(), b.data_ptr(), 1e-5, y.data_ptr(), C, None, None, D._stream())
+    assert torch.equal(y, ref[0])
+    grads = D.layer_norm_grad(x, w, ref[1], ref[2], dy)
+    for keep in range(4):
+        out = [torch.full_like(dy, 7.0)] + [torch.full_like(w, 7.0) if keep >> i & 1 else None for i in range(2)]
+        p = [None if t is None else t.data_ptr() for t in out]
+        L.call("ph_layer_norm_grad", code, x.data_ptr(), C, dy.data_ptr(), C, M, C, w.data_ptr(), ref[1].data_ptr(), ref[2].data_ptr(),
+               p[0], C, p[1], p[2], D._stream())
+        for a, g in zip(out, grads):
+            assert a is None or torch.equal(a, g), keep
+
+
 def test_refusals(gpu):
     x = torch.ones(4, 8, device="cuda")
     w = torch.ones(8, device="cuda")

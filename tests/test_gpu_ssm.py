@@ -444,6 +444,27 @@ def test_graph_replays(gpu):
         (torch.ones(1000, device="cuda") * 2).sum().item()
 
 
+@pytest.mark.parametrize("T,C,G", [(21, 24, 1), (70, 66, 2), (70, 300, 1)])
+def test_gradients_left_out(gpu, T, C, G):
+    """Each gradient may be left out; the others stay the same. With whole sequences and with chunks of time, with one block of
+    channels and with two."""
+    s, c = inputs(T, 3, C, 16, G=G, dt=torch.bfloat16)
+    dy = cu(20, T, 3, C, dtype=torch.bfloat16)
+    _, _, _, saved = forward(s, c)
+    ref = backward(s, c, saved, dy)
+    a = D._ssm_args(True, s["x"], s["delta"], s["A"], s["Bm"], s["Cm"], s["D"], s["z"], s["dt_bias"], s["conv_w"], s["conv_b"], G, c["done"],
+                    c["first"], None, c["win0"])[0]
+    acts, pars = ("dx", "dz", "ddelta", "dBm", "dCm"), ("dA", "dD", "ddt_bias", "dconv_w", "dconv_b")
+    sets = [set(ref) - {k} for k in ref] + [{k} for k in ref] + [set()]
+    for keep in sets:
+        out = {k: torch.full_like(ref[k], 7.0) for k in keep}
+        ptr = lambda k: out[k].data_ptr() if k in out else 0
+        g = D._SSM_GRADS.pack(*map(ptr, acts), *(n for k in acts for n in ref[k].stride()[:2]), *map(ptr, pars))
+        L.call("ph_ssm_scan_grad", a, saved.data_ptr(), dy.data_ptr(), dy.stride(0), dy.stride(1), g, D._stream())
+        for k in keep:
+            assert torch.equal(out[k], ref[k]), (k, keep)
+
+
 def test_refusals(gpu):
     s, c = inputs(6, 2, 12, 4, done=False, carry=False)
     call = lambda **kw: forward({**s, **{k: v for k, v in kw.items() if k in s}}, {**c, **{k: v for k, v in kw.items() if k not in s}})
