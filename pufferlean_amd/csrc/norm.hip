@@ -183,41 +183,45 @@ __global__ void __launch_bounds__(64 * kWaves) k_norm_fwd(const T* __restrict__ 
   }
 }
 
-// Rows wider than the registers: one block per row, three passes over it.
+// Rows wider than the registers: one block per row, three passes over it. A launch of 2^32 threads or more would start the
+// remainder only, so past kWideBlocks rows a block goes on to its next ones.
+constexpr long kWideBlocks = 1L << 20;
 template <typename T>
-__global__ void __launch_bounds__(256) k_norm_fwd_wide(const T* __restrict__ x, long ldx, int C,
+__global__ void __launch_bounds__(256) k_norm_fwd_wide(const T* __restrict__ x, long ldx, long M, int C,
                                                        const float* __restrict__ w, const float* __restrict__ b,
                                                        float eps, T* __restrict__ y, long ldy,
                                                        float* __restrict__ mean, float* __restrict__ rstd) {
   __shared__ float sh[2][4];
-  const long row = blockIdx.x;
-  const T* xr = x + row * ldx;
   auto total = [&](float v, int k) {
     v = group_sum<64>(v);
     if ((threadIdx.x & 63) == 0) sh[k][threadIdx.x >> 6] = v;
     __syncthreads();
     return (sh[k][0] + sh[k][1]) + (sh[k][2] + sh[k][3]);
   };
-  float v, s = 0.f;
-  for (int c = threadIdx.x; c < C; c += 256) {
-    load_v<1, false>(xr + c, &v);
-    s += v;
-  }
-  const float mu = total(s, 0) / (float)C;
-  s = 0.f;
-  for (int c = threadIdx.x; c < C; c += 256) {
-    load_v<1, false>(xr + c, &v);
-    s += (v - mu) * (v - mu);
-  }
-  const float r = 1.f / sqrtf(total(s, 1) / (float)C + eps);
-  if (threadIdx.x == 0) {
-    if (mean) mean[row] = mu;
-    if (rstd) rstd[row] = r;
-  }
-  for (int c = threadIdx.x; c < C; c += 256) {
-    load_v<1, false>(xr + c, &v);
-    v = (v - mu) * r * (w ? w[c] : 1.f) + (b ? b[c] : 0.f);
-    store_v<1, false>(y + row * ldy + c, &v);
+  // a row's two sums have buffers of their own, so between reading one and writing it again there is the other's barrier
+  for (long row = blockIdx.x; row < M; row += gridDim.x) {
+    const T* xr = x + row * ldx;
+    float v, s = 0.f;
+    for (int c = threadIdx.x; c < C; c += 256) {
+      load_v<1, false>(xr + c, &v);
+      s += v;
+    }
+    const float mu = total(s, 0) / (float)C;
+    s = 0.f;
+    for (int c = threadIdx.x; c < C; c += 256) {
+      load_v<1, false>(xr + c, &v);
+      s += (v - mu) * (v - mu);
+    }
+    const float r = 1.f / sqrtf(total(s, 1) / (float)C + eps);
+    if (threadIdx.x == 0) {
+      if (mean) mean[row] = mu;
+      if (rstd) rstd[row] = r;
+    }
+    for (int c = threadIdx.x; c < C; c += 256) {
+      load_v<1, false>(xr + c, &v);
+      v = (v - mu) * r * (w ? w[c] : 1.f) + (b ? b[c] : 0.f);
+      store_v<1, false>(y + row * ldy + c, &v);
+    }
   }
 }
 
@@ -299,34 +303,36 @@ __global__ void __launch_bounds__(64 * kWaves) k_norm_bwd(const T* __restrict__ 
 
 template <typename T>
 __global__ void __launch_bounds__(256) k_norm_bwd_wide(const T* __restrict__ x, long ldx, const T* __restrict__ dy,
-                                                       long lddy, int C, const float* __restrict__ w,
+                                                       long lddy, long M, int C, const float* __restrict__ w,
                                                        const float* __restrict__ mean, const float* __restrict__ rstd,
                                                        T* __restrict__ dx, long lddx) {
-  __shared__ float sh[2][4];
-  const long row = blockIdx.x;
-  const float mu = mean[row], r = rstd[row];
-  float s1 = 0.f, s2 = 0.f, a, g;
-  for (int c = threadIdx.x; c < C; c += 256) {
-    load_v<1, false>(x + row * ldx + c, &a);
-    load_v<1, false>(dy + row * lddy + c, &g);
-    g *= w ? w[c] : 1.f;
-    s1 += g;
-    s2 += g * (a - mu) * r;
-  }
-  s1 = group_sum<64>(s1);
-  s2 = group_sum<64>(s2);
-  if ((threadIdx.x & 63) == 0) {
-    sh[0][threadIdx.x >> 6] = s1;
-    sh[1][threadIdx.x >> 6] = s2;
-  }
-  __syncthreads();
-  s1 = ((sh[0][0] + sh[0][1]) + (sh[0][2] + sh[0][3])) / (float)C;
-  s2 = ((sh[1][0] + sh[1][1]) + (sh[1][2] + sh[1][3])) / (float)C;
-  for (int c = threadIdx.x; c < C; c += 256) {
-    load_v<1, false>(x + row * ldx + c, &a);
-    load_v<1, false>(dy + row * lddy + c, &g);
-    a = r * (g * (w ? w[c] : 1.f) - s1 - (a - mu) * r * s2);
-    store_v<1, false>(dx + row * lddx + c, &a);
+  __shared__ float sh[2][2][4];  // of alternate rows: every thread has read a row's in front of the next one's barrier
+  int p = 0;
+  for (long row = blockIdx.x; row < M; row += gridDim.x, p ^= 1) {
+    const float mu = mean[row], r = rstd[row];
+    float s1 = 0.f, s2 = 0.f, a, g;
+    for (int c = threadIdx.x; c < C; c += 256) {
+      load_v<1, false>(x + row * ldx + c, &a);
+      load_v<1, false>(dy + row * lddy + c, &g);
+      g *= w ? w[c] : 1.f;
+      s1 += g;
+      s2 += g * (a - mu) * r;
+    }
+    s1 = group_sum<64>(s1);
+    s2 = group_sum<64>(s2);
+    if ((threadIdx.x & 63) == 0) {
+      sh[p][0][threadIdx.x >> 6] = s1;
+      sh[p][1][threadIdx.x >> 6] = s2;
+    }
+    __syncthreads();
+    s1 = ((sh[p][0][0] + sh[p][0][1]) + (sh[p][0][2] + sh[p][0][3])) / (float)C;
+    s2 = ((sh[p][1][0] + sh[p][1][1]) + (sh[p][1][2] + sh[p][1][3])) / (float)C;
+    for (int c = threadIdx.x; c < C; c += 256) {
+      load_v<1, false>(x + row * ldx + c, &a);
+      load_v<1, false>(dy + row * lddy + c, &g);
+      a = r * (g * (w ? w[c] : 1.f) - s1 - (a - mu) * r * s2);
+      store_v<1, false>(dx + row * lddx + c, &a);
+    }
   }
 }
 // dw and db partials of wide rows: 64 columns x a range of rows per block of four wavefronts.
@@ -431,8 +437,9 @@ template <typename T> struct NormCall {
   }
   template <int V, bool AL, int NCH, int LPR> int go() const { return dy ? backward<V, AL, NCH, LPR>() : forward<V, AL, NCH, LPR>(); }
   int wide() const {
+    const unsigned blocks = (unsigned)(M < kWideBlocks ? M : kWideBlocks);
     if (!dy) {
-      k_norm_fwd_wide<T><<<(unsigned)M, 256, 0, st>>>(x, ldx, C, w, b, eps, y, ldy, mean, rstd);
+      k_norm_fwd_wide<T><<<blocks, 256, 0, st>>>(x, ldx, M, C, w, b, eps, y, ldy, mean, rstd);
       PH_LAUNCH_CHECK();
       return PH_OK;
     }
@@ -447,7 +454,7 @@ template <typename T> struct NormCall {
       k_norm_fold<<<(unsigned)((2 * C + 15) / 16), 256, 0, st>>>(part, (int)ry, C, dw, db);
       PH_LAUNCH_CHECK();
     }
-    k_norm_bwd_wide<T><<<(unsigned)M, 256, 0, st>>>(x, ldx, dy, lddy, C, w, cmean, crstd, dx, lddx);
+    k_norm_bwd_wide<T><<<blocks, 256, 0, st>>>(x, ldx, dy, lddy, M, C, w, cmean, crstd, dx, lddx);
     PH_LAUNCH_CHECK();
     return PH_OK;
   }

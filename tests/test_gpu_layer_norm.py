@@ -91,6 +91,33 @@ def test_strided_rows_and_no_affine(gpu, dt, affine):
     assert torch.all(out[:, 0] == 7) and torch.all(out[:, 97:] == 7)
 
 
+def test_more_wide_rows_than_a_launch_has_blocks(gpu):
+    """2^24 rows of a block of 256 threads each are more than one launch takes. Copies of 64 rows, and eight of their own at the end;
+    the sums over the rows are too long for a bar of theirs and left out."""
+    M, C = 2 ** 24 + 8, 2049
+    if torch.cuda.mem_get_info()[0] < 150e9:
+        pytest.skip("needs 140 GB")
+    x, dy, w, b = case(72, C, torch.bfloat16)
+    y, mean, rstd = D.layer_norm(x, w, b)
+    dx, _, _ = D.layer_norm_grad(x, w, mean, rstd, dy)
+    far, g = (torch.empty(M, C, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    for t, v in ((far, x), (g, dy)):
+        t[:2 ** 24].view(2 ** 18, 64, C).copy_(v[:64])
+        t[2 ** 24:] = v[64:]
+    check = lambda t, v: [(t[:2 ** 24].view(2 ** 18, 64, C)[i::2 ** 14] == v[:64]).all().item() for i in (0, 1, 2 ** 14 - 1)] + [torch.equal(t[2 ** 24:], v[64:])]
+    stats = [torch.empty(M, device="cuda") for _ in range(2)]
+    D.layer_norm(far, w, b, out=far, mean=stats[0], rstd=stats[1])
+    assert all(check(far, y))
+    assert torch.equal(stats[0][-8:], mean[64:]) and torch.equal(stats[1][-8:], rstd[64:])
+    far[:2 ** 24].view(2 ** 18, 64, C).copy_(x[:64])
+    far[2 ** 24:] = x[64:]
+    L.call("ph_layer_norm_grad", L.PH_BF16, far.data_ptr(), C, g.data_ptr(), C, M, C, w.data_ptr(), stats[0].data_ptr(), stats[1].data_ptr(),
+           g.data_ptr(), C, None, None, D._stream())
+    assert all(check(g, dx))
+    del far, g
+    torch.cuda.empty_cache()
+
+
 def test_large_offset_keeps_its_digits(gpu):
     # the mean is 1000 times the deviation: x itself holds 2^-24 * 1000 of a deviation, and so does the mean
     x, dy, w, b = case(64, 512, torch.float32, offset=1000.0)
