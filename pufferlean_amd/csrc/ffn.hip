@@ -40,33 +40,38 @@ struct Lays {
   int n;
   unsigned blocks;
 };
-// All copies of a call in one launch, a 32 x 32 tile per block.
+// All copies of a call in one launch, a 32 x 32 tile per block. A launch of 2^32 threads or more would start the remainder only,
+// so past kLayBlocks tiles a block goes on to its next ones.
+constexpr unsigned kLayBlocks = 1u << 20;
 template <typename T>
 __global__ void __launch_bounds__(256) k_lay(Lays ls) {
   __shared__ T tile[32][33];
-  int w = 0;
-  while (w + 1 < ls.n && blockIdx.x >= ls.l[w + 1].first) w++;
-  const Lay& j = ls.l[w];
-  const T* src = (const T*)j.src;
-  T* dst = (T*)j.dst;
-  const long nc = (j.cols_p + 31) / 32, id = blockIdx.x - j.first, r0 = id / nc * 32, c0 = id % nc * 32;
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  for (unsigned at = blockIdx.x; at < ls.blocks; at += gridDim.x) {
+    int w = 0;
+    while (w + 1 < ls.n && at >= ls.l[w + 1].first) w++;
+    const Lay& j = ls.l[w];
+    const T* src = (const T*)j.src;
+    T* dst = (T*)j.dst;
+    const long nc = (j.cols_p + 31) / 32, id = at - j.first, r0 = id / nc * 32, c0 = id % nc * 32;
+    if (j.trans) __syncthreads();  // the tile before has been read
 #pragma unroll
-  for (int i = 0; i < 32; i += 8) {
-    const long r = r0 + y + i, c = c0 + x;
-    const T v = r < j.rows && c < j.cols ? src[r * j.ld + c] : T(0);
-    if (!j.trans) {
-      if (r < j.rows_p && c < j.cols_p) dst[r * j.cols_p + c] = v;
-    } else {
-      tile[y + i][x] = v;
+    for (int i = 0; i < 32; i += 8) {
+      const long r = r0 + y + i, c = c0 + x;
+      const T v = r < j.rows && c < j.cols ? src[r * j.ld + c] : T(0);
+      if (!j.trans) {
+        if (r < j.rows_p && c < j.cols_p) dst[r * j.cols_p + c] = v;
+      } else {
+        tile[y + i][x] = v;
+      }
     }
-  }
-  if (!j.trans) return;
-  __syncthreads();
+    if (!j.trans) continue;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 32; i += 8) {
-    const long c = c0 + y + i, r = r0 + x;
-    if (r < j.rows_p && c < j.cols_p) dst[c * j.rows_p + r] = tile[x][y + i];
+    for (int i = 0; i < 32; i += 8) {
+      const long c = c0 + y + i, r = r0 + x;
+      if (r < j.rows_p && c < j.cols_p) dst[c * j.rows_p + r] = tile[x][y + i];
+    }
   }
 }
 
@@ -82,8 +87,9 @@ struct Layer {
   }
   int run(int dtype, hipStream_t st) {
     if (!ls.n) return PH_OK;
-    if (dtype == PH_BF16) k_lay<uint16_t><<<ls.blocks, 256, 0, st>>>(ls);
-    else k_lay<float><<<ls.blocks, 256, 0, st>>>(ls);
+    const unsigned blocks = ls.blocks < kLayBlocks ? ls.blocks : kLayBlocks;
+    if (dtype == PH_BF16) k_lay<uint16_t><<<blocks, 256, 0, st>>>(ls);
+    else k_lay<float><<<blocks, 256, 0, st>>>(ls);
     PH_LAUNCH_CHECK();
     return PH_OK;
   }

@@ -161,6 +161,27 @@ def test_gradient_into_its_inputs(gpu, M, Dm, F, into, dt):
         assert torch.equal(a, g), k
 
 
+def test_more_copies_than_a_launch_has_blocks(gpu):
+    """2^24 tiles of rows of seven columns that are padded are more than one launch takes. Copies of 4096 rows, and 40 of their own
+    at the end; against a smaller call, each within its bar."""
+    M = 2 ** 29
+    if torch.cuda.mem_get_info()[0] < 60e9:
+        pytest.skip("needs 50 GB")
+    x, wi, wo, _ = case(4136, 7, 8, torch.bfloat16)
+    ref = D.gated_ffn(x, wi, wo)
+    far = torch.empty(M + 40, 7, device="cuda", dtype=torch.bfloat16)
+    far[:M].view(M // 4096, 4096, 7).copy_(x[:4096])
+    far[M:] = x[4096:]
+    y = D.gated_ffn(far, wi, wo)
+    assert R.rel(y[M:], ref[4096:]) <= 2 * BARS[torch.bfloat16] and R.rel(y[:4096], ref[:4096]) <= 2 * BARS[torch.bfloat16]
+    v = y[:M].view(M // 4096, 4096 * 7)
+    for part in v.split(2 ** 14):
+        assert (part == v[0]).all()
+    del far, y, v
+    torch.cuda.empty_cache()
+    L.call("ph_release_scratch")
+
+
 def test_saturated_gates(gpu):
     """Gates far on both sides: the activation is the identity or zero, and its gradient finite."""
     x, wi, wo, dy = case(40, 64, 48, torch.float32)
