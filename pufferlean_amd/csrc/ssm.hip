@@ -311,6 +311,12 @@ __global__ void __launch_bounds__(256) k_ssm_window(Args a) {
   if (i < a.B * a.C) store_window<T>(a, a.win_out, i / a.C, (unsigned)(i % a.C));
 }
 
+// A launch of 2^32 threads or more would start the remainder only: its blocks are rows of 2^22 (the last one's excess has no work).
+constexpr int kGridRow = 22;
+inline dim3 grid_rows(unsigned blocks) {
+  return blocks <= 1u << kGridRow ? dim3(blocks) : dim3(1u << kGridRow, (blocks + (1u << kGridRow) - 1) >> kGridRow);
+}
+
 // One chunk of one sequence. LOCAL: from a zero state, keeping only the end state and the decay's exponent.
 template <typename T, bool LOCAL, int MOST>
 __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
@@ -319,7 +325,8 @@ __global__ void __launch_bounds__(256) k_ssm_fwd(Args a) {
   f4t* sA = reinterpret_cast<f4t*>(lds);  // [Q][nt]
   f4t* sH = sA + Q * nt;                     // [Q][nt]
   float* sbc = lds + 8 * Q * nt;                // [2][Q][kSteps][2][4]
-  const Place pl = place(a, blockIdx.x);
+  const Place pl = place(a, (blockIdx.y << kGridRow) + blockIdx.x);
+  if (pl.s >= (unsigned)a.chunks) return;
   const long b = pl.b;
   const unsigned c = pl.c;
   const int tbeg = (int)pl.s * a.chunk, tend = min(a.T, tbeg + a.chunk);
@@ -1210,7 +1217,7 @@ int fwd_t(Args& a, hipStream_t st) {
   const int nt = block_threads(a, false);
   const size_t lds = ssm_fwd_lds(a.Q, nt);
   a.blocks_c = (unsigned)((a.per + nt - 1) / nt);
-  const unsigned blocks = (unsigned)(a.chunks * a.B * a.G * a.blocks_c);
+  const dim3 blocks = grid_rows((unsigned)(a.chunks * a.B * a.G * a.blocks_c));
   const int most = (kSteps * 8 * a.Q + nt - 1) / nt;
   if (a.chunks > 1) {
     if (most <= 1) k_ssm_fwd<T, true, 1><<<blocks, nt, lds, st>>>(a);

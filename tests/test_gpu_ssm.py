@@ -391,6 +391,24 @@ def test_offsets_past_32_bits(gpu):
     assert torch.equal(y, yf)
 
 
+def test_more_threads_than_a_launch_has(gpu):
+    """A group of one channel takes a wavefront, and 2^26 wavefronts are more than one row of a launch has. Copies of 4096 sequences,
+    and eight of their own at the end."""
+    n, B, C, N = 4096, 2 ** 20 + 8, 64, 1
+    s, c = inputs(1, n + 8, C, N, G=C, K=2, done=False)
+    ref = forward(s, c)
+    far = lambda t, d: torch.cat([t.narrow(d, 0, n).repeat(*(B // n if i == d else 1 for i in range(t.dim()))), t.narrow(d, n, 8)], d)
+    sf = {k: far(v, 1) if k in ("x", "delta", "Bm", "Cm", "z") else v for k, v in s.items()}
+    cf = dict(c, first=far(c["first"], 0), h0=far(c["h0"], 0), win0=far(c["win0"], 0))
+    got = forward(sf, cf)
+    for a, b, d in zip(got[:3], ref[:3], (1, 0, 0)):
+        assert torch.equal(a, far(b, d))
+    dy = cu(20, 1, n + 8, C)
+    gr, gg = backward(s, c, ref[3], dy), backward(sf, cf, got[3], far(dy, 1))
+    for k in ("dx", "ddelta", "dBm", "dCm", "dz"):
+        assert torch.equal(gg[k], far(gr[k], 1)), k
+
+
 def test_gradient_against_differences(gpu):
     s, c = inputs(40, 2, 24, 4)
     dy = cu(20, 40, 2, 24)
