@@ -1140,36 +1140,39 @@ __global__ void __launch_bounds__(256) k_ssm_fold_par(const float* __restrict__ 
                                                       ParOut o) {
   __shared__ float sh[4][64];
   const int e = threadIdx.x & 63, z = threadIdx.x >> 6;
-  const long i = (long)blockIdx.x * 64 + e;
   const long per = (rows + 3) / 4, end = min(rows, (z + 1) * per);
-  float s = 0.f;
-  if (i < CP) {
-    long r = z * per;
-    for (; r + 8 <= end; r += 8) {
-      float v[8];
+  for (long i0 = (long)blockIdx.x * 64; i0 < CP; i0 += (long)gridDim.x * 64) {
+    const long i = i0 + e;
+    float s = 0.f;
+    if (i < CP) {
+      long r = z * per;
+      for (; r + 8 <= end; r += 8) {
+        float v[8];
 #pragma unroll
-      for (int q = 0; q < 8; q++) v[q] = par[(r + q) * CP + i];
+        for (int q = 0; q < 8; q++) v[q] = par[(r + q) * CP + i];
 #pragma unroll
-      for (int q = 0; q < 8; q++) s += v[q];
+        for (int q = 0; q < 8; q++) s += v[q];
+      }
+      for (; r < end; r++) s += par[r * CP + i];
     }
-    for (; r < end; r++) s += par[r * CP + i];
-  }
-  sh[z][e] = s;
-  __syncthreads();
-  if (z || i >= CP) return;
-  s = (sh[0][e] + sh[1][e]) + (sh[2][e] + sh[3][e]);
-  const long c = i / P;
-  const int k = (int)(i % P);
-  if (k < N) {
-    if (o.dA) o.dA[c * N + k] = s;
-  } else if (k == N) {
-    if (o.dD) o.dD[c] = s;
-  } else if (k == N + 1) {
-    if (o.dbias) o.dbias[c] = s;
-  } else if (k == N + 2) {
-    if (o.dcb) o.dcb[c] = s;
-  } else if (o.dcw) {
-    o.dcw[c * K + k - N - 3] = s;
+    __syncthreads();  // the sums before have been read
+    sh[z][e] = s;
+    __syncthreads();
+    if (z || i >= CP) continue;
+    s = (sh[0][e] + sh[1][e]) + (sh[2][e] + sh[3][e]);
+    const long c = i / P;
+    const int k = (int)(i % P);
+    if (k < N) {
+      if (o.dA) o.dA[c * N + k] = s;
+    } else if (k == N) {
+      if (o.dD) o.dD[c] = s;
+    } else if (k == N + 1) {
+      if (o.dbias) o.dbias[c] = s;
+    } else if (k == N + 2) {
+      if (o.dcb) o.dcb[c] = s;
+    } else if (o.dcw) {
+      o.dcw[c * K + k - N - 3] = s;
+    }
   }
 }
 
@@ -1265,7 +1268,8 @@ int bwd_t(Args& a, GradArgs& ga, int nt, const ParOut& po, hipStream_t st) {
     PH_LAUNCH_CHECK();
   }
   const long CP = a.C * ga.P;
-  k_ssm_fold_par<<<ceil_div((size_t)CP, 64), 256, 0, st>>>(ga.par, ga.rows, CP, a.N, a.K, ga.P, po);
+  const size_t folds = (size_t)(CP + 63) / 64, most_folds = 1u << 20;  // (2^32 threads or more would not all start)
+  k_ssm_fold_par<<<(unsigned)(folds < most_folds ? folds : most_folds), 256, 0, st>>>(ga.par, ga.rows, CP, a.N, a.K, ga.P, po);
   PH_LAUNCH_CHECK();
   return PH_OK;
 }

@@ -409,6 +409,29 @@ def test_more_threads_than_a_launch_has(gpu):
         assert torch.equal(gg[k], far(gr[k], 1)), k
 
 
+def test_more_parameter_sums_than_a_launch_has(gpu):
+    """2^24 channels of 60 states have over 2^30 parameters, four threads each. Channels of one group are their own but for dB and dC,
+    so the first and the last ones are those of a small call."""
+    if torch.cuda.mem_get_info()[0] < 80e9:
+        pytest.skip("needs 50 GB")
+    C, n = 2 ** 24, 128
+    s, c = inputs(1, 1, n, 60, done=False, carry=False)
+    dy = cu(20, 1, 1, n)
+    _, _, _, saved = forward(s, c)
+    ref = backward(s, c, saved, dy)
+    chans = dict(x=-1, delta=-1, z=-1, A=0, D=0, dt_bias=0, conv_w=0, conv_b=0)
+    far = lambda t, d: t.repeat(*(C // n if i == d % t.dim() else 1 for i in range(t.dim())))
+    sf = {k: far(v, chans[k]) if k in chans else v for k, v in s.items()}
+    rest = {k: sf[k] for k in ("D", "z", "dt_bias", "conv_w", "conv_b")}
+    _, saved = D.ssm_scan(sf["x"], sf["delta"], sf["A"], sf["Bm"], sf["Cm"], save=True, **rest)
+    got = backward(sf, c, saved, far(dy, -1))
+    for k in ("dA", "dD", "ddt_bias", "dconv_w", "dconv_b"):
+        assert torch.equal(got[k][:n], ref[k]) and torch.equal(got[k][-n:], ref[k]) and torch.equal(got[k][C // 2:C // 2 + n], ref[k]), k
+    del sf, rest, saved, got
+    torch.cuda.empty_cache()
+    L.call("ph_release_scratch")
+
+
 def test_gradient_against_differences(gpu):
     s, c = inputs(40, 2, 24, 4)
     dy = cu(20, 40, 2, 24)
