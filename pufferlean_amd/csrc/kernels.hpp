@@ -30,7 +30,7 @@ enum : int {
   kSlotGemmPadB = 23,      // zero-padded copy of a GEMM's B operand (unaligned shapes)
   kSlotNormPart = 1,       // layer norm gradient: per-block column sums
   kSlotSsm = 5,            // state-space scan: chunk states, carries, per-block sums
-  kSlotFfn = 13,           // gated feed-forward: pre-activations, units and gradients the caller does not keep
+  kSlotFfn = 13,           // gated feed-forward: padded or transposed copies, units and gradients the caller does not keep
   kSlotLane = 24,     // 24..47: 8 concurrent update lanes x 3 slots (U, NS buffers, GEMM split-K)
   kSlotHost = 48,     // 48..127: host-buffer entry points
 };

@@ -183,7 +183,9 @@ __global__ void __launch_bounds__(64 * kWaves) k_norm_fwd(const T* __restrict__ 
   }
 }
 
-// Rows wider than the registers: one block per row, three passes over it. A launch of 2^32 threads or more would start the
+// Rows wider than the registers: one block per row, three passes over it in single elements; in the gradient two, behind one of
+// k_norm_cols_wide. 65536 x 2056 forward and gradient bf16 416 and 577 us, fp32 488 and 696 (2048 columns in
+// registers: 111 and 216, 184 and 291); 64 x 4096 take the host's call. A launch of 2^32 threads or more would start the
 // remainder only, so past kWideBlocks rows a block goes on to its next ones.
 constexpr long kWideBlocks = 1L << 20;
 template <typename T>

@@ -681,13 +681,10 @@ def _ffn_shapes(x, w_in, w_out, act):
     return dt, M, D, F
 
 
-def _pitch(n):
-    return (n + 7) // 8 * 8
-
-
-def _kept(dt):
-    # bf16 units keep a pair of 24-bit values, fp32 ones two of their own
-    return 3 if dt == L.PH_BF16 else 2
+def _saved_widths(dt, F):
+    """Columns of pf and h: rows of ph_ffn_pitch(F) pairs, of two 24-bit values for bf16 and of two fp32 ones, and of as many units."""
+    n = L.lib().ph_ffn_pitch(F)
+    return (3 if dt == L.PH_BF16 else 2) * n, n
 
 
 def gated_ffn(x, w_in, w_out, *, act="silu", out=None, save=False):
@@ -698,7 +695,7 @@ def gated_ffn(x, w_in, w_out, *, act="silu", out=None, save=False):
     y = x.new_empty((M, D)) if out is None else _like(out, x, x.shape, "out")
     pf = h = None
     if save:
-        pf, h = x.new_empty((M, _kept(dt) * _pitch(F))), x.new_empty((M, _pitch(F)))
+        pf, h = (x.new_empty((M, cols)) for cols in _saved_widths(dt, F))
     L.call("ph_ffn", dt, _ACT[act], M, D, F, x.data_ptr(), _rows(x), w_in.data_ptr(), w_out.data_ptr(), _ptr(pf), _ptr(h),
            y.data_ptr(), _rows(y), _stream())
     return (y, (pf, h)) if save else y
@@ -709,7 +706,7 @@ def gated_ffn_grad(x, w_in, w_out, saved, dy, *, act="silu", dx=None, dw_in=None
     dt, M, D, F = _ffn_shapes(x, w_in, w_out, act)
     _like(dy, x, x.shape, "dy")
     pf, h = saved
-    for t, cols in ((pf, _kept(dt) * _pitch(F)), (h, _pitch(F))):
+    for t, cols in zip(saved, _saved_widths(dt, F)):
         if not _like(t, x, (M, cols), "saved").is_contiguous():
             raise ValueError("saved must be as gated_ffn returned it")
     dwt = dw_dtype or (x.dtype if dw_in is None else dw_in.dtype)
