@@ -20,8 +20,9 @@ __device__ __forceinline__ void glu_act(int act, float a, float& f, float& df) {
 
 // What the gradient multiplies dh with: a unit's pair p = v act'(a), f = act(a), rows of them, pf. Their roundings would add to
 // those of the products' operands (a bf16 pair makes dx and dw_in 1.7 times as far from their exact values as one rounding of
-// the result; this way 1.4 times), so of bf16 units a pair has the first 24 bits of its fp32 values, 16 of mantissa: the
-// upper 16 bits of a row's 2F values first, then the next 8 of each. A row is keep_pitch values of the units' type.
+// the result; this way 1.4 times), so of bf16 units a pair has the first 24 bits of its fp32 values, 16 of mantissa, cut off: an
+// error of 2^-15 at most, where a bf16 operand's rounding costs up to 2^-8. The upper 16 bits of a row's 2F values come first,
+// then the next 8 of each. A row is keep_pitch values of the units' type.
 inline long keep_pitch(int dtype, long F) { return (dtype == PH_BF16 ? 3 : 2) * F; }
 // The upper halves of two fp32 values, and the bytes behind those of four.
 __device__ __forceinline__ uint32_t keep_hi(float a, float b) {
