@@ -452,6 +452,87 @@ int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, const void* x,
                 const void* w_out, const void* pf, const void* h, const void* dy, size_t lddy, void* dx, size_t lddx,
                 int dw_dtype, void* dw_in, void* dw_out, void* stream);
 
+/* ---------------------------------------------------------------------------------------------- */
+/* Operators of a delta-rule policy layer (no counterpart in the reference): the gated delta rule, RMS normalisation fused
+ * with the residual sum in front of it or the gate behind it, and the draw from filtered logits. dtype is PH_F32 or PH_BF16
+ * and holds for the activations and their gradients; sums, norms and states are fp32 or wider. */
+
+/* Gated delta rule of B sequences of T steps, H heads with a state of K x V each (K, V <= 128), per head and step t:
+ *   q^ = q / sqrt(|q|^2 + 1e-6),  k^ = k / sqrt(|k|^2 + 1e-6)
+ *   S_t = al S_{t-1} + k^ (be (v - (al S_{t-1})^T k^))^T,  al = exp(A softplus(a + dt_bias)), be = sigmoid(b)
+ *   y_t = scale S_t^T q^
+ * H / Hk heads share the rows of a q and k head. Element (t, b, head h, i) of q, k, v is at t * <name>_t + b * <name>_b + h *
+ * <name>_h + i, and (t, b, h) of a, b at t * <name>_t + b * <name>_b + h, so time-major and batch-major arrays and column
+ * slices of a wider one are all taken in place. A, dt_bias fp32 [H]; dt_bias may be NULL (0). done (fp32 [T][B], may be
+ * NULL): where nonzero, step t ends an episode, and step t + 1 starts from a cleared state, whatever it held; first (fp32
+ * [B], may be NULL): the same for the step before the call. h0 fp32 [B][H][K][V] (may be NULL: zero) is the state carried
+ * in. */
+typedef struct {
+  int dtype;
+  size_t T, B, Hk, H, K, V;
+  const void *q, *k, *v, *a, *b;
+  long q_t, q_b, q_h, k_t, k_b, k_h, v_t, v_b, v_h, a_t, a_b, b_t, b_b;
+  const float *A, *dt_bias, *done, *first, *h0;
+  float scale;
+} ph_delta_args;
+/* y [.., H, V], which may not be q, k or v; h_out (may be NULL) receives the state after the last step, before done[T-1]
+ * clears it (the next call's `first` does); it may be h0. keep (may be NULL): fp32, ph_delta_keep_floats values, the states
+ * that the gradient starts from. */
+int ph_delta_scan(const ph_delta_args* a, void* y, long y_t, long y_b, long y_h, float* h_out, float* keep, void* stream);
+size_t ph_delta_keep_floats(const ph_delta_args* a);
+/* Gradient from the forward's arguments (h0 is not read) and keep; dh (fp32, may be NULL: zero) is the gradient of h_out. Each
+ * output may be NULL; dq, dk, dv, da, db have the activations' dtype and strides of their own and may not be inputs; dA and
+ * ddt_bias (fp32 [H], overwritten) are summed in an order fixed by the shape; dh0 (may be dh) is the gradient of h0. */
+typedef struct {
+  void *dq, *dk, *dv, *da, *db;
+  long dq_t, dq_b, dq_h, dk_t, dk_b, dk_h, dv_t, dv_b, dv_h, da_t, da_b, db_t, db_b;
+  float *dA, *ddt_bias, *dh0;
+} ph_delta_grads;
+int ph_delta_scan_grad(const ph_delta_args* a, const float* keep, const void* dy, long dy_t, long dy_b, long dy_h,
+                       const float* dh, const ph_delta_grads* g, void* stream);
+/* One step (T = 1 or 0; the _t strides, done and h0 are not read): the state h [B][H][K][V] is updated in place, cleared
+ * first where first[b] is set. */
+int ph_delta_step(const ph_delta_args* a, void* y, long y_b, long y_h, float* h, void* stream);
+
+/* RMS normalisation of the rows [M][C] of r = x + scale * add, in G groups of C / G columns each:
+ *   out = r / sqrt(avg r^2 + eps) w silu(gate)
+ * add NULL: r = x; scale (fp32 [C], for G = 1) NULL: 1; w (fp32 [C / G]) NULL: 1; gate NULL: no gate. res (where there is an
+ * add; may be NULL) receives r, rstd (fp32 [M][G], may be NULL) the 1 / sqrt for the gradient. Row strides in elements. out
+ * and res may each be one of the inputs (same rows), but not the same one. */
+typedef struct {
+  int dtype;
+  size_t M, C, G;
+  const void *x, *add, *gate;
+  long ldx, ldadd, ldgate;
+  const float *w, *scale;
+  float eps;
+} ph_rms_args;
+int ph_rms_norm(const ph_rms_args* a, void* out, long ldout, void* res, long ldres, float* rstd, void* stream);
+/* Gradient from the forward's arguments and rstd, given dout (of out) and dres (of res; NULL: zero): dx, dadd = scale dx (where
+ * there is an add), dgate, and dw = the rows' and groups' sums, dscale = the rows' sums (fp32, overwritten; zero for M = 0). Each output may be
+ * NULL. dx, dadd and dgate may each be one of the inputs (same rows), but no two the same one. */
+typedef struct {
+  void *dx, *dadd, *dgate;
+  long lddx, lddadd, lddgate;
+  float *dw, *dscale;
+} ph_rms_grads;
+int ph_rms_norm_grad(const ph_rms_args* a, const float* rstd, const void* dout, long lddout, const void* dres, long lddres,
+                     const ph_rms_grads* g, void* stream);
+
+/* Draw of one of A entries per row of logits [N][A] (PH_F32 or PH_BF16, row stride ld; 0: one row for all draws) from given numbers u (fp32 [N], in
+ * [0, 1)), after filters that every row has its own of (device arrays of N; NULL: off). In this order:
+ *   temperature (fp32)  the logits are divided by it; 0 takes the largest logit
+ *   top_k (int32)       the k largest are left; 0 and less: all
+ *   top_p (fp32)        of these, by falling logit, as many as it takes for their share of the mass to reach p; the first always
+ *   min_p (fp32)        and of these the ones that have at least min_p times the largest one's mass; the largest always
+ * Of equal logits the one with the lower index counts as larger. What is left is summed up in the order of the indices, and
+ * the first entry with which the sum exceeds u times the total is taken. act (int32 [N]); logp (fp32 [N], may be NULL): the
+ * logarithm of its share of what is left. Logits of -inf and NaN are never taken; a row of nothing else gives act -1 and
+ * logp -inf; entries of +inf share the draw. A parameter that is NaN, or a temperature below zero, leaves its filter off (temperature 1).
+ * Masses are held in 64 bits. */
+int ph_sample_filtered(int dtype, const void* logits, long ld, size_t N, size_t A, const float* u, const float* temperature,
+                       const int* top_k, const float* top_p, const float* min_p, int* act, float* logp, void* stream);
+
 /* ============================================================================================== */
 /* Host-buffer entry points (layer 2). Each replaces the reference GPU symbol named beside it, with
  * the same argument order and meaning; FloatArray inputs become host `const double*`, the returned

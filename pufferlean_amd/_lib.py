@@ -64,6 +64,32 @@ class SsmGrads(C.Structure):
                 + [(n, C.c_void_p) for n in ("dA", "dD", "ddt_bias", "dconv_w", "dconv_b")])
 
 
+class DeltaArgs(C.Structure):
+    _fields_ = ([("dtype", C.c_int)] + [(n, C.c_size_t) for n in ("T", "B", "Hk", "H", "K", "V")]
+                + [(n, C.c_void_p) for n in ("q", "k", "v", "a", "b")]
+                + [(n + s, C.c_long) for n in ("q", "k", "v") for s in ("_t", "_b", "_h")]
+                + [(n + s, C.c_long) for n in ("a", "b") for s in ("_t", "_b")]
+                + [(n, C.c_void_p) for n in ("A", "dt_bias", "done", "first", "h0")] + [("scale", C.c_float)])
+
+
+class DeltaGrads(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("dq", "dk", "dv", "da", "db")]
+                + [(n + s, C.c_long) for n in ("dq", "dk", "dv") for s in ("_t", "_b", "_h")]
+                + [(n + s, C.c_long) for n in ("da", "db") for s in ("_t", "_b")]
+                + [(n, C.c_void_p) for n in ("dA", "ddt_bias", "dh0")])
+
+
+class RmsArgs(C.Structure):
+    _fields_ = ([("dtype", C.c_int)] + [(n, C.c_size_t) for n in ("M", "C", "G")]
+                + [(n, C.c_void_p) for n in ("x", "add", "gate")] + [(n, C.c_long) for n in ("ldx", "ldadd", "ldgate")]
+                + [(n, C.c_void_p) for n in ("w", "scale")] + [("eps", C.c_float)])
+
+
+class RmsGrads(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("dx", "dadd", "dgate")] + [(n, C.c_long) for n in ("lddx", "lddadd", "lddgate")]
+                + [(n, C.c_void_p) for n in ("dw", "dscale")])
+
+
 # name -> argtypes (all return int status unless listed in _RESTYPES)
 SIGNATURES: dict[str, list] = {
     "ph_last_error": [],
@@ -119,6 +145,13 @@ SIGNATURES: dict[str, list] = {
     "ph_ffn": [i32, i32, sz, sz, sz, vp, sz, vp, vp, vp, vp, vp, sz, vp],
     "ph_ffn_pitch": [sz],
     "ph_ffn_grad": [i32, i32, sz, sz, sz, vp, sz, vp, vp, vp, vp, vp, sz, vp, sz, i32, vp, vp, vp],
+    "ph_delta_scan": [vp, vp, i64, i64, i64, vp, vp, vp],
+    "ph_delta_keep_floats": [vp],
+    "ph_delta_scan_grad": [vp, vp, vp, i64, i64, i64, vp, vp, vp],
+    "ph_delta_step": [vp, vp, i64, i64, vp, vp],
+    "ph_rms_norm": [vp, vp, i64, vp, i64, vp, vp],
+    "ph_rms_norm_grad": [vp, vp, vp, i64, vp, i64, vp, vp],
+    "ph_sample_filtered": [i32, vp, i64, sz, sz, vp, vp, vp, vp, vp, vp, vp, vp],
     # host-buffer layer (reference Lean @[extern] GPU symbols)
     "ph_cuda_vtrace": [dptr, dptr, dptr, dptr, sz, sz, dbl, dbl, dbl, dbl, dptr],
     "ph_cuda_vtrace_mingru": [dptr, dptr, dptr, dptr, dptr, sz, sz, dbl, dbl, dbl, dbl, dptr],
@@ -178,7 +211,7 @@ SIGNATURES: dict[str, list] = {
     "ph_cuda_mingru_muon_resident": [sz, dptr, sz, sz, sz, sz, sz, dbl, dbl, dbl, dbl, dbl, dbl, dptr, szptr],
 }
 _RESTYPES = {"ph_last_error": C.c_char_p, "ph_mingru_param_count": C.c_long, "ph_mlp_param_count": C.c_long, "ph_ckpt_bytes": C.c_size_t, "ph_ssm_keep_floats": C.c_size_t,
-             "ph_ffn_pitch": C.c_size_t,
+             "ph_ffn_pitch": C.c_size_t, "ph_delta_keep_floats": C.c_size_t,
              "ph_ffi_bench_bf16_resident": C.c_double, "ph_ffi_bench_mlp2_bf16_resident": C.c_double,
              "ph_ffi_bench_mlp2_bf16_wres": C.c_double, "ph_ffi_mlp_policy_outputs": C.c_size_t, "ph_ffi_cuda_available": C.c_uint8}
 

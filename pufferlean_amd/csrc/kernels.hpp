@@ -33,6 +33,9 @@ enum : int {
   kSlotFfn = 13,           // gated feed-forward: padded or transposed copies, units and gradients the caller does not keep
   kSlotLane = 24,     // 24..47: 8 concurrent update lanes x 3 slots (U, NS buffers, GEMM split-K)
   kSlotHost = 48,     // 48..127: host-buffer entry points
+  kSlotDelta = 128,   // gated delta rule: gradients of shared heads, sums of the gates
+  kSlotRms = 129,     // rms norm gradient: per-block column sums
+  kSlotDraw = 130,    // filtered draw of wide rows
 };
 constexpr int kLanes = 8;
 

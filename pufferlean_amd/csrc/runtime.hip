@@ -21,7 +21,7 @@ void set_error(const char* fmt, ...) {
 
 namespace {
 constexpr int kMaxDev = 16;
-constexpr int kSlots = 128;
+constexpr int kSlots = 136;
 SlotTable<kSlots> g_tables[kMaxDev];
 std::mutex g_mu;
 std::set<void*> g_zeroed;  // word blocks ensure_zeroed_words has cleared (by address)

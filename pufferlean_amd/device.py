@@ -496,7 +496,7 @@ def _act_dtype(x, what):
 
 def _like(t, x, shape, what):
     """t has x's dtype, the given shape and a contiguous last dimension, on a GPU."""
-    if t.dtype is not x.dtype or t.shape != shape or not t.is_cuda or (t.stride(-1) != 1 and t.shape[-1] > 1):
+    if t.dtype is not x.dtype or t.shape != shape or not t.is_cuda or (t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel()):
         raise ValueError(f"{what} must be {x.dtype} {tuple(shape)} on a GPU with a contiguous last dimension, "
                          f"not {t.dtype} {tuple(t.shape)}")
     return t
@@ -720,3 +720,208 @@ def gated_ffn_grad(x, w_in, w_out, saved, dy, *, act="silu", dx=None, dw_in=None
            h.data_ptr(), dy.data_ptr(), _rows(dy), dx.data_ptr(), _rows(dx), _DT[dwt], dw_in.data_ptr(), dw_out.data_ptr(),
            _stream())
     return dx, dw_in, dw_out
+
+
+# ---- delta-rule policy layer: gated delta rule, fused RMS normalisation, filtered draw -------------------
+# ph_delta_args, ph_rms_args and their gradients as bytes, as the scan's above
+_DELTA_ARGS = struct.Struct("@i6N5P13l5Pf0P")
+_DELTA_GRADS = struct.Struct("@5P13l3P")
+_RMS_ARGS = struct.Struct("@i3N3P3l2Pf0P")
+_RMS_GRADS = struct.Struct("@3P3l2P")
+assert _DELTA_ARGS.size == C.sizeof(L.DeltaArgs) and _DELTA_GRADS.size == C.sizeof(L.DeltaGrads)
+assert _RMS_ARGS.size == C.sizeof(L.RmsArgs) and _RMS_GRADS.size == C.sizeof(L.RmsGrads)
+
+
+def _here(x, what):
+    """x is on the current device, whose stream the call takes."""
+    if not x.is_cuda or x.get_device() != torch._C._cuda_getDevice():
+        raise ValueError(f"{what} must be on the current GPU, not {x.device}")
+
+
+def _beside(x, *ts):
+    """The other tensors are on x's device."""
+    dev = x.get_device()
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"a tensor is on {t.device}, not on {x.device}")
+
+
+def _delta_args(seq, q, k, v, a, b, A, dt_bias, scale, done, first, h0):
+    """The checked ph_delta_args of [T, B, heads, .] (seq) or single-step [B, heads, .] inputs, and (T, B, H, K, V)."""
+    dt = _act_dtype(q, "the delta rule")
+    if q.dim() != (4 if seq else 3) or v.dim() != q.dim():
+        lead = "[T, B, " if seq else "[B, "
+        raise ValueError(f"q must be {lead}Hk, K] and v {lead}H, V], not {tuple(q.shape)} and {tuple(v.shape)}")
+    lead, (Hk, K), (H, V) = q.shape[:-2], q.shape[-2:], v.shape[-2:]
+    T, B = lead if seq else (1, *lead)
+    _here(q, "q")
+    _like(q, q, q.shape, "q"), _like(k, q, q.shape, "k"), _like(v, q, (*lead, H, V), "v")
+    _like(a, q, (*lead, H), "a"), _like(b, q, (*lead, H), "b")
+    _f32(A, (H,), "A")
+    if dt_bias is not None:
+        _f32(dt_bias, (H,), "dt_bias")
+    if done is not None:
+        _f32(done, (T, B), "done")
+    if first is not None:
+        _f32(first, (B,), "first")
+    if h0 is not None:
+        _f32(h0, (B, H, K, V), "h0")
+    _beside(q, k, v, a, b, A, dt_bias, done, first, h0)
+    st = [s for t in (q, k, v) for s in (t.stride()[:3] if seq else (0, *t.stride()[:2]))]
+    st += [s for t in (a, b) for s in (t.stride()[:2] if seq else (0, t.stride(0)))]
+    p = _DELTA_ARGS.pack(dt, T, B, Hk, H, K, V, q.data_ptr(), k.data_ptr(), v.data_ptr(), a.data_ptr(), b.data_ptr(), *st,
+                         A.data_ptr(), _ptr(dt_bias), _ptr(done), _ptr(first), _ptr(h0), K ** -0.5 if scale is None else scale)
+    return p, T, B, H, K, V
+
+
+def delta_scan(q, k, v, a, b, A, *, dt_bias=None, scale=None, done=None, first=None, h0=None, out=None, h_out=None, save=False):
+    """Gated delta rule over [T, B] steps (ph_delta_scan): q, k [T, B, Hk, K], v [T, B, H, V] (K, V <= 128, H a multiple of
+    Hk), the decay's and the write strength's arguments a, b [T, B, H], in float32 or bfloat16, any strides with a contiguous
+    last dimension; A, dt_bias [H], done [T, B], first [B], h0 [B, H, K, V] float32; scale defaults to K ** -0.5. q and k
+    enter with unit length. h_out receives the carried state (it may be h0); out may not be an input. Returns y [T, B, H, V],
+    or (y, saved) with save=True, saved being what delta_scan_grad needs."""
+    p, T, B, H, K, V = _delta_args(True, q, k, v, a, b, A, dt_bias, scale, done, first, h0)
+    y = q.new_empty(v.shape) if out is None else _like(out, q, v.shape, "out")
+    if h_out is not None:
+        _f32(h_out, (B, H, K, V), "h_out")
+    _beside(q, out, h_out)
+    keep = q.new_empty(L.lib().ph_delta_keep_floats(p), dtype=_F32) if save else None
+    L.call("ph_delta_scan", p, y.data_ptr(), *y.stride()[:3], _ptr(h_out), _ptr(keep), _stream())
+    return (y, keep) if save else y
+
+
+def delta_scan_grad(q, k, v, a, b, A, saved, dy, *, dt_bias=None, scale=None, done=None, first=None, dh=None, dq=None, dk=None,
+                    dv=None, da=None, db=None, dh0=None):
+    """Gradient of delta_scan from its arguments and what it saved. Returns a dict: dq, dk, dv, da, db in the activations'
+    dtype, written into the given tensors where there are any (they may not be inputs), and dA (and ddt_bias) in float32. dh
+    is the gradient of h_out (None: zero), dh0 receives h0's (it may be dh)."""
+    p, T, B, H, K, V = _delta_args(True, q, k, v, a, b, A, dt_bias, scale, done, first, None)
+    _like(dy, q, v.shape, "dy")
+    _f32(saved, (L.lib().ph_delta_keep_floats(p),), "saved")
+    for t, what in ((dh, "dh"), (dh0, "dh0")):
+        if t is not None:
+            _f32(t, (B, H, K, V), what)
+    g, ptrs, strides = {}, [], []
+    for name, t, like, n in (("dq", dq, q, 3), ("dk", dk, k, 3), ("dv", dv, v, 3), ("da", da, a, 2), ("db", db, b, 2)):
+        g[name] = t = q.new_empty(like.shape) if t is None else _like(t, q, like.shape, name)
+        ptrs.append(t.data_ptr())
+        strides += t.stride()[:n]
+    _beside(q, dy, saved, dh, dh0, *g.values())
+    g["dA"] = torch.empty_like(A)
+    if dt_bias is not None:
+        g["ddt_bias"] = torch.empty_like(dt_bias)
+    L.call("ph_delta_scan_grad", p, saved.data_ptr(), dy.data_ptr(), *dy.stride()[:3], _ptr(dh),
+           _DELTA_GRADS.pack(*ptrs, *strides, g["dA"].data_ptr(), _ptr(g.get("ddt_bias")), _ptr(dh0)), _stream())
+    return g
+
+
+def delta_step(q, k, v, a, b, A, h, *, dt_bias=None, scale=None, first=None, out=None):
+    """One step of delta_scan for B sequences: q, k [B, Hk, K], v [B, H, V], a, b [B, H]; the state h [B, H, K, V] (float32) is
+    updated in place, cleared first where first[b] is set. Returns y [B, H, V]."""
+    p, _, B, H, K, V = _delta_args(False, q, k, v, a, b, A, dt_bias, scale, None, first, h)
+    y = q.new_empty(v.shape) if out is None else _like(out, q, v.shape, "out")
+    _beside(q, out)
+    L.call("ph_delta_step", p, y.data_ptr(), *y.stride()[:2], h.data_ptr(), _stream())
+    return y
+
+
+def _rms_args(x, w, add, scale, gate, groups, eps):
+    dt = _act_dtype(x, "rms_norm")
+    shape = x.shape
+    M, C_ = shape
+    if groups < 1 or C_ % groups:
+        raise ValueError(f"rms_norm: {groups} groups do not divide {C_} columns")
+    _here(x, "x")
+    _like(x, x, shape, "x")
+    if add is not None:
+        _like(add, x, shape, "add")
+    if gate is not None:
+        _like(gate, x, shape, "gate")
+    if w is not None:
+        _f32(w, (C_ // groups,), "w")
+    if scale is not None:
+        if add is None or groups != 1:
+            raise ValueError("rms_norm: a scale needs an add, and one group")
+        _f32(scale, (C_,), "scale")
+    _beside(x, add, gate, w, scale)
+    ld = [0 if t is None else _rows(t) for t in (x, add, gate)]
+    return _RMS_ARGS.pack(dt, M, C_, groups, x.data_ptr(), _ptr(add), _ptr(gate), *ld, _ptr(w), _ptr(scale), eps), shape
+
+
+def rms_norm(x, w=None, *, add=None, scale=None, gate=None, groups=1, eps=1e-6, out=None, res=None, rstd=None):
+    """RMS normalisation of r = x + scale * add, by groups of columns, times w and silu(gate) (ph_rms_norm): x, add, gate
+    [M, C] (float32 or bfloat16, row strides honoured), w float32 [C // groups], scale float32 [C] (for one group). Returns
+    (out, res, rstd): res is r (None without an add), rstd float32 [M, groups] for rms_norm_grad. out and res may each be one
+    of the inputs."""
+    p, shape = _rms_args(x, w, add, scale, gate, groups, eps)
+    out = x.new_empty(shape) if out is None else _like(out, x, shape, "out")
+    if add is None:
+        res = None
+    else:
+        res = x.new_empty(shape) if res is None else _like(res, x, shape, "res")
+    rs = (shape[0], groups)
+    rstd = x.new_empty(rs, dtype=_F32) if rstd is None else _f32(rstd, rs, "rstd")
+    _beside(x, out, res, rstd)
+    L.call("ph_rms_norm", p, out.data_ptr(), _rows(out), _ptr(res), 0 if res is None else _rows(res), rstd.data_ptr(), _stream())
+    return out, res, rstd
+
+
+def rms_norm_grad(x, w, rstd, dout, *, dres=None, add=None, scale=None, gate=None, groups=1, eps=1e-6, dx=None, dadd=None,
+                  dgate=None, dw=None, dscale=None):
+    """Gradient of rms_norm from its arguments and rstd; dout is the gradient of out, dres that of res, or of x past the norm
+    (None: zero). Returns a dict: dx, dw (where there is a w), dadd (the same tensor as dx without a scale, unless one is
+    given), dscale, dgate. dx, dadd and dgate may each be one of the inputs."""
+    p, shape = _rms_args(x, w, add, scale, gate, groups, eps)
+    _like(dout, x, shape, "dout")
+    if dres is not None:
+        _like(dres, x, shape, "dres")
+    _f32(rstd, (shape[0], groups), "rstd")
+    g = dict(dx=x.new_empty(shape) if dx is None else _like(dx, x, shape, "dx"))
+    own_add = add is not None and (scale is not None or dadd is not None)
+    for name, t, on in (("dadd", dadd, own_add), ("dgate", dgate, gate is not None)):
+        if on:
+            g[name] = x.new_empty(shape) if t is None else _like(t, x, shape, name)
+    for name, t, like in (("dw", dw, w), ("dscale", dscale, scale)):
+        if like is not None:
+            g[name] = torch.empty_like(like) if t is None else _f32(t, like.shape, name)
+    _beside(x, dout, dres, rstd, *g.values())
+    ts = [g["dx"], g.get("dadd"), g.get("dgate")]
+    L.call("ph_rms_norm_grad", p, rstd.data_ptr(), dout.data_ptr(), _rows(dout), _ptr(dres), 0 if dres is None else _rows(dres),
+           _RMS_GRADS.pack(*map(_ptr, ts), *[0 if t is None else _rows(t) for t in ts], _ptr(g.get("dw")), _ptr(g.get("dscale"))),
+           _stream())
+    if add is not None and not own_add:
+        g["dadd"] = g["dx"]
+    return g
+
+
+def _per_row(v, N, dtype, like, what):
+    """A row's own parameter as a tensor of N: a tensor, a number for all rows, or None."""
+    if v is None:
+        return None
+    if not isinstance(v, torch.Tensor):
+        return torch.full((N,), v, dtype=dtype, device=like.device)
+    if v.dtype is not dtype or v.shape != (N,) or not v.is_cuda or not v.is_contiguous():
+        raise ValueError(f"{what} must be a number or contiguous {dtype} {(N,)} on a GPU, not {v.dtype} {tuple(v.shape)}")
+    return v
+
+
+def sample_filtered(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, act=None, logp=None):
+    """Draw one entry per row of logits [N, A] (float32 or bfloat16, row stride honoured) from the given numbers u (float32
+    [N], in [0, 1)) after temperature (0: the largest logit), top_k (0: all), top_p and min_p, in this order
+    (ph_sample_filtered). Each is a number, or float32 (top_k: int32) [N], a row's own. Returns (act int32 [N], logp float32 [N]),
+    logp being that of the filtered distribution; a row of -inf gives act -1."""
+    dt = _act_dtype(logits, "sample_filtered")
+    N, A = logits.shape
+    _here(logits, "logits")
+    _like(logits, logits, logits.shape, "logits")
+    _f32(u, (N,), "u")
+    t, p, m = (_per_row(v, N, _F32, logits, n) for v, n in ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p")))
+    k = _per_row(top_k, N, torch.int32, logits, "top_k")
+    act = torch.empty(N, dtype=torch.int32, device=logits.device) if act is None else act
+    if act.dtype is not torch.int32 or act.shape != (N,) or not act.is_cuda or not act.is_contiguous():
+        raise ValueError(f"act must be contiguous int32 {(N,)} on a GPU, not {act.dtype} {tuple(act.shape)}")
+    logp = logits.new_empty(N, dtype=_F32) if logp is None else _f32(logp, (N,), "logp")
+    _beside(logits, u, t, k, p, m, act, logp)
+    L.call("ph_sample_filtered", dt, logits.data_ptr(), _rows(logits), N, A, u.data_ptr(), _ptr(t), _ptr(k), _ptr(p), _ptr(m),
+           act.data_ptr(), logp.data_ptr(), _stream())
+    return act, logp
