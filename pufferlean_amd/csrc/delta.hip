@@ -64,10 +64,15 @@ struct Args {
   long q_t, q_b, q_h, k_t, k_b, k_h, v_t, v_b, v_h, a_t, a_b, b_t, b_b;
   const float *A, *dt_bias, *done, *first, *h0;
   float scale;
-  int vec;  // rows of q, k, v (and dy) can be read 16 bytes at a time
+  int segs;  // segments of time, of seg_chunks chunks each
+  long seg_chunks;
   void* y;
   long y_t, y_b, y_h;
   float *h_out, *keep;
+  float* start;  // [segs][units] states at the segments' starts (more than one segment)
+  float *psi, *phi;  // [segs][units]: what a segment adds to its start state, and what it multiplies it with
+  int* cut;          // [segs][units]: an episode starts in the segment, and nothing passes it
+  int local_from, parts;  // of these: segments from local_from on, segs - 1 of them; both, or phi alone
 };
 
 struct GradArgs {
@@ -78,8 +83,22 @@ struct GradArgs {
   long dq_t, dq_b, dq_h, dk_t, dk_b, dk_h, dv_t, dv_b, dv_h, da_t, da_b, db_t, db_b;
   float* dh0;
   float *qpart, *kpart;  // [T][B][H][K] of every value head, where heads share their keys
-  float* gpart;          // [2][H][B]: sums of dlog al softplus and of dlog al A sigmoid
+  float* gpart;          // [2][H][segs B]: sums of dlog al softplus and of dlog al A sigmoid
+  float *dend, *xi;      // [segs][units] gradients of the segments' end states; [segs][units] what a segment adds on the way back
 };
+
+// The kernel's own arguments, read again from where the launch put them: Args first, GradArgs behind. The compiler reads
+// arguments once, at the kernel's start, and what the scalar registers cannot hold over the loops it keeps in lanes of
+// vector registers.
+template <typename A> __device__ __forceinline__ A again(unsigned at) {
+  static_assert(sizeof(A) % 8 == 0 && alignof(A) == 8, "read in words of eight bytes");
+  auto p = (const __attribute__((address_space(4))) uint64_t*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm("" : "+s"(p));
+  uint64_t w[sizeof(A) / 8];
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(A) / 8; i++) w[i] = p[at / 8 + i];
+  return __builtin_bit_cast(A, w);
+}
 
 // ---- elements ------------------------------------------------------------------------------------------
 __device__ __forceinline__ float ldf(const uint16_t* p) { return bf16_to_f32(*p); }
@@ -100,6 +119,13 @@ __device__ __forceinline__ float log_decay(float A, float sp) {
   return g < -1e9f ? -1e9f : g;  // differences of sums stay numbers
 }
 __device__ __forceinline__ bool finite(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7f800000u) != 0x7f800000u; }
+
+// From here on the compiler takes the lane's number as new: what depends on it alone is formed where it is used and does not wait
+// in registers over all chunks.
+__device__ __forceinline__ void renew(int& tid, int& l) {
+  asm volatile("" : "+v"(tid));
+  l = tid & 63;
+}
 
 // ---- matrix operands -------------------------------------------------------------------------------------
 // Operands are taken in units of 16 of the contraction, of which lane l holds 4 (l / 16) + 0..3.
@@ -188,21 +214,21 @@ __device__ __forceinline__ f4 dot2r(const Pair<BF>* a, const typename Elem<BF>::
 // operand with the contraction over columns, or the right one of the transposed matrix); col_unit: rows `row` + 4 (l / 16) +
 // 0..3, column `col` + l % 16 (contraction over rows), for 16-bit elements by the transposing load, which gives lane l of
 // sixteen the column l of the four rows that the sixteen lanes' addresses cover.
-template <int LD> __device__ __forceinline__ s4 row_unit(const uint16_t* m, int row, int col) {
-  const int l = threadIdx.x & 63;
+template <int LD> __device__ __forceinline__ s4 row_unit(int tid, const uint16_t* m, int row, int col) {
+  const int l = tid & 63;
   return *reinterpret_cast<const s4*>(m + (row + (l & 15)) * LD + col + 4 * (l >> 4));
 }
-template <int LD> __device__ __forceinline__ f4 row_unit(const float* m, int row, int col) {
-  const int l = threadIdx.x & 63;
+template <int LD> __device__ __forceinline__ f4 row_unit(int tid, const float* m, int row, int col) {
+  const int l = tid & 63;
   return *reinterpret_cast<const f4*>(m + (row + (l & 15)) * LD + col + 4 * (l >> 4));
 }
-template <int LD> __device__ __forceinline__ s4 col_unit(const uint16_t* m, int row, int col) {
-  const int l = threadIdx.x & 63;
+template <int LD> __device__ __forceinline__ s4 col_unit(int tid, const uint16_t* m, int row, int col) {
+  const int l = tid & 63;
   const uint16_t* p = m + (row + 4 * (l >> 4) + ((l & 15) >> 2)) * LD + col + 4 * (l & 3);
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
 }
-template <int LD> __device__ __forceinline__ f4 col_unit(const float* m, int row, int col) {
-  const int l = threadIdx.x & 63;
+template <int LD> __device__ __forceinline__ f4 col_unit(int tid, const float* m, int row, int col) {
+  const int l = tid & 63;
   const float* p = m + (row + 4 * (l >> 4)) * LD + col + (l & 15);
   return f4{p[0], p[LD], p[2 * LD], p[3 * LD]};
 }
@@ -212,25 +238,32 @@ __device__ __forceinline__ f4 widen(s4 v) {
 __device__ __forceinline__ f4 widen(f4 v) { return v; }
 
 // ---- a chunk's rows ------------------------------------------------------------------------------------
-// The 16 bytes of a row of W columns that a thread stages: row tid / (P / V), columns from V (tid % (P / V)) on; zero where
-// the row or the columns end.
+// The 16 bytes of a row of W columns that a thread stages: row tid / (P / V), columns from V (tid % (P / V)) on, at p; zero
+// where the rows or the columns end. Any alignment: the hardware takes 16 bytes at that of an element. The last columns of a row
+// come from an access that ends with it, shifted down.
 template <bool BF, int P, typename T = typename Elem<BF>::type>
-__device__ __forceinline__ u4 load_row(const T* base, long stride, int rows, int W, bool vec) {
+__device__ __forceinline__ u4 load_row(int tid, const T* p, int rows, int W) {
   constexpr int V = Elem<BF>::V;
-  const int row = threadIdx.x / (P / V), c = threadIdx.x % (P / V) * V;
+  const int row = tid / (P / V), c = tid % (P / V) * V;
   u4 r = {0, 0, 0, 0};
   if (row < rows && c < W) {
-    const T* p = base + row * stride + c;
-    if (vec) {
-      r = *reinterpret_cast<const u4*>(p);
+    const int over = c + V - W;
+    if (W >= V) {
+      const int skip = over > 0 ? over : 0;
+      __builtin_memcpy(&r, p - skip, 16);
+      if (over > 0) r = __builtin_bit_cast(u4, __builtin_bit_cast(unsigned __int128, r) >> (skip * 8 * (int)sizeof(T)));
     } else {
-      T v[V];
-#pragma unroll
-      for (int i = 0; i < V; i++) v[i] = c + i < W ? p[i] : T(0);
-      __builtin_memcpy(&r, v, 16);
+      unsigned __int128 x = 0;
+#pragma unroll 1
+      for (int i = W - 1; i >= 0; i--) x = x << (8 * (int)sizeof(T)) | (sizeof(T) == 2 ? (unsigned)__builtin_bit_cast(uint16_t, (uint16_t)*(const uint16_t*)(p + i)) : *(const unsigned*)(p + i));
+      r = __builtin_bit_cast(u4, x);
     }
   }
   return r;
+}
+template <bool BF, int P, typename T> __device__ __forceinline__ const T* thread_row(int tid, const T* base, long stride, long t0) {
+  constexpr int V = Elem<BF>::V;
+  return base + (t0 + tid / (P / V)) * stride + tid % (P / V) * V;
 }
 template <bool BF> __device__ __forceinline__ float square_sum(u4 r) {
   float s = 0.f;
@@ -287,19 +320,33 @@ template <typename T> __device__ __forceinline__ Gate load_gate(const Args& s, l
   }
   return g;
 }
-// Fills r for rows lo..hi-1 from the gates of wavefront 0's lanes (all of it calls).
-template <int CH> __device__ __forceinline__ void fill_rows(Rows<CH>& r, const Gate& g, float A, int lo, int hi) {
-  const int i = threadIdx.x;
+template <int CTL> __device__ __forceinline__ double dpp_f64(double v) {  // zero where the shift leaves the row of lanes
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTL, 0xF, 0xF, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Fills r for rows lo..hi-1 from the gates in a wavefront's lanes (all of it calls), but for the norms.
+template <int CH> __device__ __forceinline__ void fill_rows(int tid, Rows<CH>& r, const Gate& g, float A, int lo, int hi) {
+  const int i = tid & 63;
   const bool in = i >= lo && i < hi;
   const float sp = softplus(g.a);
   double G = in ? (double)log_decay(A, sp) * kLog2e : 0.0;
   const unsigned long long starts = __ballot(in && g.start != 0.f);
-#pragma unroll
-  for (int d = 1; d < CH; d *= 2) {
-    const double o = __shfl_up(G, d);
-    if (i >= d) G += o;
+  G += dpp_f64<0x111>(G);  // sums along the rows of 16 lanes
+  G += dpp_f64<0x112>(G);
+  G += dpp_f64<0x114>(G);
+  G += dpp_f64<0x118>(G);
+  if constexpr (CH == 32) {
+    const double low = lane_f64(G, 15);
+    if (i & 16) G += low;
   }
-  const double last = __shfl(G, CH - 1);
+  const double last = lane_f64(G, CH - 1);
   if (i < CH) {
     const int seg = __popcll(starts & ((2ull << i) - 1)), all = __popcll(starts);
     r.G[i] = G;
@@ -316,7 +363,7 @@ template <int CH> __device__ __forceinline__ void fill_rows(Rows<CH>& r, const G
     }
   }
 }
-__device__ __forceinline__ f4 rows4(const float* r, int at) { return *reinterpret_cast<const f4*>(r + at + 4 * ((threadIdx.x & 63) >> 4)); }
+__device__ __forceinline__ f4 rows4(int tid, const float* r, int at) { return *reinterpret_cast<const f4*>(r + at + 4 * ((tid & 63) >> 4)); }
 // c x where c is not zero: what a start hides may be anything
 __device__ __forceinline__ f4 sel_mul(f4 c, f4 x) {
 #pragma unroll
@@ -325,19 +372,19 @@ __device__ __forceinline__ f4 sel_mul(f4 c, f4 x) {
 }
 
 // M (and P, transposed by the reader) of the chunk: tiles on and below the diagonal, dealt out over the wavefronts.
-template <bool BF, int P, int LD>
-__device__ __forceinline__ void score_tiles(const Rows<Elem<BF>::CH>& r, const typename Elem<BF>::type* Qs,
+template <bool BF, int P, int LD, bool WITH_P>
+__device__ __forceinline__ void score_tiles(int tid, const Rows<Elem<BF>::CH>& r, const typename Elem<BF>::type* Qs,
                                             const typename Elem<BF>::type* Ks, float* Mm, float* Pm, float scale) {
   constexpr int CH = Elem<BF>::CH, NB = CH / 16, NT = P / 16, CP = CH + 4, TILES = NB * (NB + 1) / 2;
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-  for (int id = w; id < 2 * TILES; id += NT) {
-    const bool isP = id >= TILES;
+  const int l = tid & 63, w = tid >> 6;
+  for (int id = w; id < (WITH_P ? 2 : 1) * TILES; id += NT) {
+    const bool isP = WITH_P && id >= TILES;
     const int tile = isP ? id - TILES : id, bi = tile == 0 ? 0 : 1, bj = tile == 2 ? 1 : 0;  // (0,0) (1,0) (1,1)
     typename Elem<BF>::unit x[NT], y[NT];
 #pragma unroll
     for (int m = 0; m < NT; m++) {
-      x[m] = row_unit<LD>(isP ? Qs : Ks, 16 * bi, 16 * m);
-      y[m] = row_unit<LD>(Ks, 16 * bj, 16 * m);
+      x[m] = row_unit<LD>(tid, isP ? Qs : Ks, 16 * bi, 16 * m);
+      y[m] = row_unit<LD>(tid, Ks, 16 * bj, 16 * m);
     }
     f4 acc = dot<NT>(x, y, f4{0.f, 0.f, 0.f, 0.f});
     const int j = 16 * bj + (l & 15);
@@ -355,9 +402,9 @@ __device__ __forceinline__ void score_tiles(const Rows<Elem<BF>::CH>& r, const t
 }
 
 // The diagonal blocks of (I + M)^-1 into Tm, one column per lane of wavefront 0.
-template <int CH> __device__ __forceinline__ void invert_blocks(const float* Mm, float* Tm) {
+template <int CH> __device__ __forceinline__ void invert_blocks(int tid, const float* Mm, float* Tm) {
   constexpr int CP = CH + 4;
-  const int l = threadIdx.x;
+  const int l = tid;
   if (l >= CH) return;
   const int o = l & ~15, c = l & 15;
   float x[16];
@@ -377,153 +424,244 @@ template <int CH> __device__ __forceinline__ void invert_blocks(const float* Mm,
 }
 
 // U = T Y by blocks, T's blocks below the diagonal through M.
-template <bool BF> __device__ __forceinline__ void solve(const float* Tm, const float* Mm, const f4* Y, f4* U) {
+template <bool BF> __device__ __forceinline__ void solve(int tid, const float* Tm, const float* Mm, const f4* Y, f4* U) {
   constexpr int CH = Elem<BF>::CH, NB = CH / 16, CP = CH + 4;
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
   Pair<BF> t, y, u;
-  t.set(row_unit<CP>(Tm, 0, 0));
+  t.set(row_unit<CP>(tid, Tm, 0, 0));
   y.set(Y[0]);
   U[0] = dot3<BF, 1>(&t, &y, zero);
   if constexpr (NB == 2) {
     u.set(-U[0]);
-    t.set(row_unit<CP>(Mm, 16, 0));
+    t.set(row_unit<CP>(tid, Mm, 16, 0));
     y.set(dot3<BF, 1>(&t, &u, Y[1]));
-    t.set(row_unit<CP>(Tm, 16, 16));
+    t.set(row_unit<CP>(tid, Tm, 16, 16));
     U[1] = dot3<BF, 1>(&t, &y, zero);
   }
 }
 // dY = T^T dU
-template <bool BF> __device__ __forceinline__ void solve_t(const float* Tm, const float* Mm, const f4* dU, f4* dY) {
+template <bool BF> __device__ __forceinline__ void solve_t(int tid, const float* Tm, const float* Mm, const f4* dU, f4* dY) {
   constexpr int CH = Elem<BF>::CH, NB = CH / 16, CP = CH + 4;
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
   Pair<BF> t, y;
   f4 top = dU[0];
   if constexpr (NB == 2) {
     y.set(dU[1]);
-    t.set(col_unit<CP>(Tm, 16, 16));
+    t.set(col_unit<CP>(tid, Tm, 16, 16));
     dY[1] = dot3<BF, 1>(&t, &y, zero);
     y.set(-dY[1]);
-    t.set(col_unit<CP>(Mm, 16, 0));
+    t.set(col_unit<CP>(tid, Mm, 16, 0));
     top = dot3<BF, 1>(&t, &y, top);
   }
   y.set(top);
-  t.set(col_unit<CP>(Tm, 0, 0));
+  t.set(col_unit<CP>(tid, Tm, 0, 0));
   dY[0] = dot3<BF, 1>(&t, &y, zero);
 }
 
-// Tile m of a [K][V] matrix's column block w: rows 16 m + 4 (l / 16) + 0..3, column 16 w + l % 16; zero outside.
-__device__ __forceinline__ f4 state_tile(const float* s, int K, int V, int m, int w) {
-  const int l = threadIdx.x & 63, r = 16 * m + 4 * (l >> 4), c = 16 * w + (l & 15);
-  f4 x = {0.f, 0.f, 0.f, 0.f};
-  if (s && c < V) {
+// States in memory: [K][V] as the caller holds them, or [up(K)][up(V)], both rounded up to whole tiles, as the library does.
+__host__ __device__ __forceinline__ int up16(int n) { return (n + 15) & ~15; }
+// Tile m of a state's column block w: rows 16 m + 4 (l / 16) + 0..3, column 16 w + l % 16; zero outside. Addresses are clamped
+// and not skipped: a load that a branch guards is waited for before the next one.
+__device__ __forceinline__ f4 state_tile(int tid, const float* s, int K, int V, int m, int w) {
+  const int l = tid & 63, r = 16 * m + 4 * (l >> 4), c = 16 * w + (l & 15);
+  const float* p = s + (c < V ? c : 0);
+  f4 x;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (r + i < K) x[i] = s[(long)(r + i) * V + c];
-  }
+  for (int i = 0; i < 4; i++) x[i] = p[(r + i < K ? r + i : 0) * V];
+#pragma unroll
+  for (int i = 0; i < 4; i++) x[i] = r + i < K && c < V ? x[i] : 0.f;
   return x;
 }
-__device__ __forceinline__ void put_state_tile(float* s, int K, int V, int m, int w, f4 x) {
-  const int l = threadIdx.x & 63, r = 16 * m + 4 * (l >> 4), c = 16 * w + (l & 15);
+__device__ __forceinline__ void put_state_tile(int tid, float* s, int K, int V, int m, int w, f4 x) {
+  const int l = tid & 63, r = 16 * m + 4 * (l >> 4), c = 16 * w + (l & 15);
   if (c < V) {
 #pragma unroll
     for (int i = 0; i < 4; i++)
-      if (r + i < K) s[(long)(r + i) * V + c] = x[i];
+      if (r + i < K) s[(r + i) * V + c] = x[i];
   }
 }
-// The transposed matrix's tile m of block w: columns of V 16 m + 4 (l / 16) + 0..3, row 16 w + l % 16.
-__device__ __forceinline__ f4 state_tile_t(const float* s, int K, int V, int m, int w) {
-  const int l = threadIdx.x & 63, c = 16 * m + 4 * (l >> 4), r = 16 * w + (l & 15);
-  f4 x = {0.f, 0.f, 0.f, 0.f};
-  if (s && r < K) {
+// The transposed state's tile m of block w: columns of V 16 m + 4 (l / 16) + 0..3, row 16 w + l % 16.
+__device__ __forceinline__ f4 state_tile_t(int tid, const float* s, int K, int V, int m, int w) {
+  const int l = tid & 63, c = 16 * m + 4 * (l >> 4), r = 16 * w + (l & 15);
+  const float* p = s + (r < K ? r : 0) * V;
+  f4 x;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (c + i < V) x[i] = s[(long)r * V + c + i];
+  for (int i = 0; i < 4; i++) x[i] = p[c + i < V ? c + i : 0];
+#pragma unroll
+  for (int i = 0; i < 4; i++) x[i] = r < K && c + i < V ? x[i] : 0.f;
+  return x;
+}
+// The same of the library's own states: whole tiles, of which those past the last are not there.
+__device__ __forceinline__ f4 own_tile(int tid, const float* s, int Ku, int Vu, int m, int w) {
+  const int l = tid & 63;
+  f4 x = {0.f, 0.f, 0.f, 0.f};
+  if (16 * m < Ku && 16 * w < Vu) {
+    const float* p = s + (16 * m + 4 * (l >> 4)) * Vu + 16 * w + (l & 15);
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = p[i * Vu];
   }
   return x;
 }
+__device__ __forceinline__ f4 own_tile_t(int tid, const float* s, int Ku, int Vu, int m, int w) {
+  const int l = tid & 63;
+  f4 x = {0.f, 0.f, 0.f, 0.f};
+  if (16 * m < Vu && 16 * w < Ku) x = *reinterpret_cast<const f4*>(s + (16 * w + (l & 15)) * Vu + 16 * m + 4 * (l >> 4));
+  return x;
+}
+__device__ __forceinline__ void put_own_tile(int tid, float* s, int Ku, int Vu, int m, int w, f4 x) {
+  const int l = tid & 63;
+  if (16 * m < Ku && 16 * w < Vu) {
+    float* p = s + (16 * m + 4 * (l >> 4)) * Vu + 16 * w + (l & 15);
+#pragma unroll
+    for (int i = 0; i < 4; i++) p[i * Vu] = x[i];
+  }
+}
 
 template <bool BF, int P, typename T = typename Elem<BF>::type>
-__device__ __forceinline__ void put_row(T* tile, u4 r, int lo, int hi) {
+__device__ __forceinline__ void put_row(int tid, T* tile, u4 r, int lo, int hi) {
   constexpr int V = Elem<BF>::V, LD = P + Elem<BF>::pad;
-  const int row = threadIdx.x / (P / V), c = threadIdx.x % (P / V) * V;
+  const int row = tid / (P / V), c = tid % (P / V) * V;
   if (row < lo || row >= hi) r = u4{0, 0, 0, 0};
   *reinterpret_cast<u4*>(tile + row * LD + c) = r;
 }
 // 1 / sqrt(|row|^2 + eps) of the staged rows, 0 for those left out
-template <bool BF, int P> __device__ __forceinline__ void put_norm(float* out, u4 r, int lo, int hi) {
+template <bool BF, int P> __device__ __forceinline__ void put_norm(int tid, float* out, u4 r, int lo, int hi) {
   constexpr int L = P / Elem<BF>::V;  // lanes of a row
   float s = square_sum<BF>(r);
 #pragma unroll
   for (int d = 1; d < L; d *= 2) s += __shfl_xor(s, d);
-  const int row = threadIdx.x / L;
-  if (threadIdx.x % L == 0) out[row] = row >= lo && row < hi ? 1.f / sqrtf(s + kEps) : 0.f;
+  const int row = tid / L;
+  if (tid % L == 0) out[row] = row >= lo && row < hi ? 1.f / sqrtf(s + kEps) : 0.f;
 }
 
 // ---- sequences ------------------------------------------------------------------------------------------
-template <bool BF, int P> __global__ void __launch_bounds__(4 * P) k_delta_fwd(const Args s) {
+// Wavefronts of a SIMD, at least: as many as registers and LDS leave room for.
+template <bool BF, int P> constexpr int fwd_waves() { return P == 128 ? 2 : 4; }
+template <bool BF, int P> constexpr int bwd_waves() { return P == 128 ? 2 : 3; }
+
+// One segment of one sequence's head. LOCAL: without outputs, from a zero state (what the segment adds to its start state) or,
+// without values to write, from the unit matrix (what it multiplies it with).
+template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (fwd_waves<BF, P>())) k_delta_fwd(const Args s) {
   using T = typename Elem<BF>::type;
   using unit = typename Elem<BF>::unit;
   constexpr int CH = Elem<BF>::CH, NB = CH / 16, NT = P / 16, LD = P + Elem<BF>::pad, CP = CH + 4;
-  __shared__ __attribute__((aligned(16))) T Qs[CH * LD], Ks[CH * LD], Vs[CH * LD];
-  __shared__ __attribute__((aligned(16))) float Mm[CH * CP], Tm[CH * CP], Pm[CH * CP];
-  __shared__ Rows<CH> R;
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  __shared__ __attribute__((aligned(16))) T Qs[LOCAL ? 1 : CH * LD], Ks[CH * LD], Vs[CH * LD];
+  __shared__ __attribute__((aligned(16))) float Mm[CH * CP], Tm[CH * CP], Pm[LOCAL ? 1 : CH * CP];
+  __shared__ Rows<CH> Rs[2];
+  int tid = threadIdx.x, l = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
-  for (long unit_id = blockIdx.x; unit_id < s.units; unit_id += gridDim.x) {
-    const long bt = unit_id / s.H;
-    const int h = (int)(unit_id % s.H), hk = h / (s.H / s.Hk);
-    const T* qp = (const T*)s.q + bt * s.q_b + hk * s.q_h;
-    const T* kp = (const T*)s.k + bt * s.k_b + hk * s.k_h;
-    const T* vp = (const T*)s.v + bt * s.v_b + h * s.v_h;
-    T* yp = (T*)s.y + bt * s.y_b + h * s.y_h;
-    const long kv = (long)s.K * s.V;
+  const long items = s.units * (LOCAL ? (s.segs - 1) * s.parts : s.segs);
+  for (long item = blockIdx.x; item < items; item += gridDim.x) {
+    const unsigned units = (unsigned)s.units, round = (unsigned)item / units;
+    const long unit_id = (unsigned)item - round * units;
+    const int part = LOCAL ? (s.parts == 1 ? 1 : (int)round & 1) : 0;
+    const long seg = LOCAL ? (s.parts == 1 ? round : round >> 1) + s.local_from : round;
+    const long bt = (unsigned)unit_id / (unsigned)s.H;
+    const int h = (int)(unit_id - bt * s.H), hk = (int)((unsigned)h / (unsigned)(s.H / s.Hk));
+    const int Ku = up16(s.K), Vu = up16(s.V), W = part ? s.K : s.V;  // columns of the state
+    const long first = seg * s.seg_chunks * CH;
+    const long last = first + s.seg_chunks * CH < s.T ? first + s.seg_chunks * CH : s.T;
+    const T* qp = thread_row<BF, P>(tid, (const T*)s.q + bt * s.q_b + hk * s.q_h, s.q_t, first);
+    const T* kp = thread_row<BF, P>(tid, (const T*)s.k + bt * s.k_b + hk * s.k_h, s.k_t, first);
+    const T* vp = thread_row<BF, P>(tid, (const T*)s.v + bt * s.v_b + h * s.v_h, s.v_t, first);
+    const int W_v = part ? 0 : s.V;
     const float A = s.A[h];
+    auto rows_at = [&](long t0) { return (int)(t0 >= last ? 0 : last - t0 < CH ? last - t0 : CH); };
     f4 S[NT];
+    if (LOCAL) {
 #pragma unroll
-    for (int m = 0; m < NT; m++) S[m] = state_tile(s.h0 ? s.h0 + unit_id * kv : nullptr, s.K, s.V, m, w);
-    for (long t0 = 0; t0 < s.T; t0 += CH) {
-      const int rows = (int)(s.T - t0 < CH ? s.T - t0 : CH);
-      if (s.keep) {
+      for (int m = 0; m < NT; m++) {
+        S[m] = zero;
+        if (part && m == w) {
 #pragma unroll
-        for (int m = 0; m < NT; m++) put_state_tile(s.keep + (t0 / CH * s.units + unit_id) * kv, s.K, s.V, m, w, S[m]);
+          for (int i = 0; i < 4; i++) S[m][i] = 4 * (l >> 4) + i == (l & 15) ? 1.f : 0.f;
+        }
       }
-      const u4 q = load_row<BF, P>(qp + t0 * s.q_t, s.q_t, rows, s.K, s.vec);
-      const u4 k = load_row<BF, P>(kp + t0 * s.k_t, s.k_t, rows, s.K, s.vec);
-      const u4 v = load_row<BF, P>(vp + t0 * s.v_t, s.v_t, rows, s.V, s.vec);
-      Gate g;
-      if (w == 0) g = load_gate<T>(s, bt, h, t0, rows, l);
-      for (int lo = 0, hi = rows; lo < rows;) {
+    } else if (s.segs > 1) {
+#pragma unroll
+      for (int m = 0; m < NT; m++) S[m] = own_tile(tid, s.start + (seg * s.units + unit_id) * Ku * Vu, Ku, Vu, m, w);
+    } else if (s.h0) {
+#pragma unroll
+      for (int m = 0; m < NT; m++) S[m] = state_tile(tid, s.h0 + unit_id * s.K * s.V, s.K, s.V, m, w);
+    } else {
+#pragma unroll
+      for (int m = 0; m < NT; m++) S[m] = zero;
+    }
+    int rows = rows_at(first);
+    u4 q = {0, 0, 0, 0}, k, v;
+    auto load = [&]() {
+      if (!LOCAL) q = load_row<BF, P>(tid, qp, rows, s.K);
+      k = load_row<BF, P>(tid, kp, rows, s.K);
+      v = load_row<BF, P>(tid, vp, rows, W_v);
+    };
+    load();
+    // the last wavefront sees to the gates, a chunk ahead
+    Gate g = {0.f, 0.f, 0.f}, gn = g;
+    if (w == NT - 1) {
+      g = load_gate<T>(s, bt, h, first, rows, l);
+      gn = load_gate<T>(s, bt, h, first + CH, rows_at(first + CH), l);
+      __builtin_amdgcn_s_waitcnt(0);
+    }
+    __syncthreads();  // the item before has been read
+    if (w == NT - 1) fill_rows<CH>(tid, Rs[0], g, A, 0, rows);
+    int cur = 0, cut = 0;
+    for (long t0 = first; t0 < last; t0 += CH) {
+      Rows<CH>& R = Rs[cur];
+      if (!LOCAL && s.keep) {
+#pragma unroll
+        for (int m = 0; m < NT; m++) put_own_tile(tid, s.keep + (t0 / CH * s.units + unit_id) * Ku * Vu, Ku, Vu, m, w, S[m]);
+      }
+      const int all = rows;  // rows of this chunk
+      for (int lo = 0, hi = all, once = 1; lo < all; once = 0) {
         __syncthreads();  // the rows before have been read
-        put_row<BF, P>(Qs, q, lo, hi);
-        put_row<BF, P>(Ks, k, lo, hi);
-        put_row<BF, P>(Vs, v, lo, hi);
-        put_norm<BF, P>(R.rq, q, lo, hi);
-        put_norm<BF, P>(R.rk, k, lo, hi);
+        renew(tid, l);
+        if (!once) {  // one episode at a time: rows and gates again
+          rows = all;
+          load();
+        }
+        if (!LOCAL) put_row<BF, P>(tid, Qs, q, lo, hi);
+        put_row<BF, P>(tid, Ks, k, lo, hi);
+        put_row<BF, P>(tid, Vs, v, lo, hi);
+        if (!LOCAL) put_norm<BF, P>(tid, R.rq, q, lo, hi);
+        put_norm<BF, P>(tid, R.rk, k, lo, hi);
+        if (!once && w == NT - 1) fill_rows<CH>(tid, R, g, A, lo, hi);
         __syncthreads();
-        if (w == 0) fill_rows<CH>(R, g, A, lo, hi);
+        if (once) {  // the next chunk's are on their way while this one computes
+          qp += CH * s.q_t;
+          kp += CH * s.k_t;
+          vp += CH * s.v_t;
+          rows = rows_at(t0 + CH);
+          load();
+        }
+        score_tiles<BF, P, LD, !LOCAL>(tid, R, Qs, Ks, Mm, Pm, s.scale);
         __syncthreads();
-        score_tiles<BF, P, LD>(R, Qs, Ks, Mm, Pm, s.scale);
-        __syncthreads();
-        if (w == 0) invert_blocks<CH>(Mm, Tm);
-        Pair<BF> Sp[NT];
-#pragma unroll
-        for (int m = 0; m < NT; m++) Sp[m].set(S[m]);
+        if (w == 0) invert_blocks<CH>(tid, Mm, Tm);
+        if (w == NT - 1 && once) fill_rows<CH>(tid, Rs[cur ^ 1], gn, A, 0, rows);
         f4 Y[NB], O[NB];
+        {
+          Pair<BF> Sp[NT];
 #pragma unroll
-        for (int n = 0; n < NB; n++) {
-          unit x[NT];
+          for (int m = 0; m < NT; m++) Sp[m].set(S[m]);
 #pragma unroll
-          for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(Ks, 16 * n, 16 * m);
-          const f4 ks = dot2<BF, NT>(x, Sp, zero);
-          Y[n] = rows4(R.be, 16 * n) * (widen(col_unit<LD>(Vs, 16 * n, 16 * w)) - sel_mul(rows4(R.d0, 16 * n) * rows4(R.rk, 16 * n), ks));
+          for (int n = 0; n < NB; n++) {
+            unit x[NT];
 #pragma unroll
-          for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(Qs, 16 * n, 16 * m);
-          O[n] = sel_mul(s.scale * rows4(R.d0, 16 * n) * rows4(R.rq, 16 * n), dot2<BF, NT>(x, Sp, zero));
+            for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, Ks, 16 * n, 16 * m);
+            const f4 ks = dot2<BF, NT>(x, Sp, zero);
+            Y[n] = rows4(tid, R.be, 16 * n) * (widen(col_unit<LD>(tid, Vs, 16 * n, 16 * w)) -
+                                          sel_mul(rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n), ks));
+            if constexpr (!LOCAL) {
+#pragma unroll
+              for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, Qs, 16 * n, 16 * m);
+              O[n] = sel_mul(s.scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n), dot2<BF, NT>(x, Sp, zero));
+            }
+          }
         }
         __syncthreads();
         f4 U[NB];
-        solve<BF>(Tm, Mm, Y, U);
-        const int inside = R.starts & ~(1 << lo);
+        solve<BF>(tid, Tm, Mm, Y, U);
+        const int starts = R.starts, inside = starts & ~(1 << lo);
         if (inside) {
           bool bad = false;
 #pragma unroll
@@ -531,51 +669,146 @@ template <bool BF, int P> __global__ void __launch_bounds__(4 * P) k_delta_fwd(c
 #pragma unroll
             for (int i = 0; i < 4; i++) bad |= !finite(U[n][i]);
           if (__syncthreads_or(bad)) {
+            qp -= once ? CH * s.q_t : 0;
+            kp -= once ? CH * s.k_t : 0;
+            vp -= once ? CH * s.v_t : 0;
             hi = __ffs(inside) - 1;
             continue;
           }
         }
-        Pair<BF> Up[NB], x[NB];
+        Pair<BF> Up[NB];
+        if constexpr (!LOCAL) {
+          Pair<BF> x[NB];
 #pragma unroll
-        for (int n = 0; n < NB; n++) Up[n].set(U[n]);
-        x[0].set(row_unit<CP>(Pm, 0, 0));
-        O[0] = dot3<BF, 1>(x, Up, O[0]);
-        if constexpr (NB == 2) {
-          x[0].set(row_unit<CP>(Pm, 16, 0));
-          x[1].set(row_unit<CP>(Pm, 16, 16));
-          O[1] = dot3<BF, 2>(x, Up, O[1]);
-        }
-        const int c = 16 * w + (l & 15);
-#pragma unroll
-        for (int n = 0; n < NB; n++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int row = 16 * n + 4 * (l >> 4) + i;
-            if (row >= lo && row < hi && c < s.V) stf(yp + (t0 + row) * s.y_t + c, O[n][i]);
+          for (int n = 0; n < NB; n++) Up[n].set(U[n]);
+          x[0].set(row_unit<CP>(tid, Pm, 0, 0));
+          O[0] = dot3<BF, 1>(x, Up, O[0]);
+          if constexpr (NB == 2) {
+            x[0].set(row_unit<CP>(tid, Pm, 16, 0));
+            x[1].set(row_unit<CP>(tid, Pm, 16, 16));
+            O[1] = dot3<BF, 2>(x, Up, O[1]);
           }
+          const Args a = again<Args>(0);
+          T* yp = (T*)a.y + bt * a.y_b + h * a.y_h + t0 * a.y_t;
+          const int c = 16 * w + (l & 15);
 #pragma unroll
-        for (int n = 0; n < NB; n++) Up[n].set(sel_mul(rows4(R.dc, 16 * n) * rows4(R.rk, 16 * n), U[n]));
+          for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const int row = 16 * n + 4 * (l >> 4) + i;
+              if (row >= lo && row < hi && c < a.V) stf(yp + row * a.y_t + c, O[n][i]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NB; n++) Up[n].set(sel_mul(rows4(tid, R.dc, 16 * n) * rows4(tid, R.rk, 16 * n), U[n]));
         const float c0 = R.c0;
 #pragma unroll
         for (int m = 0; m < NT; m++) {
           unit kt[NB];
 #pragma unroll
-          for (int n = 0; n < NB; n++) kt[n] = col_unit<LD>(Ks, 16 * n, 16 * m);
+          for (int n = 0; n < NB; n++) kt[n] = col_unit<LD>(tid, Ks, 16 * n, 16 * m);
           S[m] = dot2<BF, NB>(kt, Up, sel_mul(f4{c0, c0, c0, c0}, S[m]));
         }
+        cut |= starts;
         lo = hi;
-        hi = rows;
+        hi = all;
+        if (!once && lo >= all) {  // on to the next chunk's rows
+          qp += CH * s.q_t;
+          kp += CH * s.k_t;
+          vp += CH * s.v_t;
+          rows = rows_at(t0 + CH);
+          load();
+        }
       }
+      if (w == NT - 1) {
+        g = gn;
+        gn = load_gate<T>(s, bt, h, t0 + 2 * CH, rows_at(t0 + 2 * CH), l);
+      }
+      cur ^= 1;
     }
-    if (s.h_out) {
+    if (LOCAL) {
+      const long at = seg * s.units + unit_id;
+      float* out = part ? s.phi + at * Ku * Ku : s.psi + at * Ku * Vu;
 #pragma unroll
-      for (int m = 0; m < NT; m++) put_state_tile(s.h_out + unit_id * kv, s.K, s.V, m, w, S[m]);
+      for (int m = 0; m < NT; m++) put_own_tile(tid, out, Ku, up16(W), m, w, S[m]);
+      if (part && tid == 0) s.cut[at] = cut != 0;
+    } else if (s.h_out && last == s.T) {
+#pragma unroll
+      for (int m = 0; m < NT; m++) put_state_tile(tid, s.h_out + unit_id * s.K * s.V, s.K, s.V, m, w, S[m]);
     }
   }
 }
 
-// The gradient of one sequence's head, chunks in reverse. Wavefront w holds dS's columns 16 w .. and, for the products
-// that contract over V, the transposed dS's (rows 16 w .. of dS).
+// The segments' start states in order, S <- Phi S + Psi, a block per sequence's head (back: the gradients of their end states in
+// reverse, dS <- Phi^T dS + Xi). An episode's start in a segment leaves only what the segment adds.
+template <bool BF, int P, bool BACK> __global__ void __launch_bounds__(4 * P) k_delta_join(const Args s, const GradArgs o) {
+  constexpr int NT = P / 16, LD = P + 4;
+  __shared__ __attribute__((aligned(16))) float F[64 * LD];  // half of Phi's rows (P = 128), or all
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), Ku = up16(s.K), Vu = up16(s.V);
+  const f4 zero = {0.f, 0.f, 0.f, 0.f};
+  for (long unit_id = blockIdx.x; unit_id < s.units; unit_id += gridDim.x) {
+    f4 S[NT];
+    const float* from = BACK ? o.dh : s.h0;
+#pragma unroll
+    for (int m = 0; m < NT; m++) {
+      S[m] = from ? state_tile(tid, from + unit_id * s.K * s.V, s.K, s.V, m, w) : zero;
+      put_own_tile(tid, (BACK ? o.dend + (s.segs - 1) * s.units * Ku * Vu : s.start) + unit_id * Ku * Vu, Ku, Vu, m, w, S[m]);
+    }
+    for (long i = 0; i + 1 < s.segs; i++) {
+      const long seg = BACK ? s.segs - 1 - i : i;  // the segment that is passed
+      const long at = (BACK ? seg - 1 : seg) * s.units + unit_id;
+      const long fat = seg * s.units + unit_id;
+      const float* add = BACK ? o.xi + fat * Ku * Vu : s.psi + at * Ku * Vu;
+      const float* phi = s.phi + fat * Ku * Ku;
+      f4 N[NT];
+#pragma unroll
+      for (int m = 0; m < NT; m++) N[m] = own_tile(tid, add, Ku, Vu, m, w);
+      if (!s.cut[fat]) {
+        Pair<BF> Sp[NT];
+#pragma unroll
+        for (int m = 0; m < NT; m++) Sp[m].set(S[m]);
+#pragma unroll
+        for (int half = 0; half < (P + 63) / 64; half++) {
+          __syncthreads();
+          for (int e = tid; e < 64 * (P / 4); e += 4 * P) {
+            const int r = e / (P / 4), c = e % (P / 4) * 4;
+            f4 x = zero;
+            if (64 * half + r < Ku && c < Ku) x = *reinterpret_cast<const f4*>(phi + (64 * half + r) * Ku + c);
+            *reinterpret_cast<f4*>(F + r * LD + c) = x;
+          }
+          __syncthreads();
+          constexpr int HT = P < 64 ? NT : 4;  // tiles of rows here
+          if constexpr (!BACK) {
+#pragma unroll
+            for (int m = 0; m < HT; m++) {
+              Pair<BF> x[NT];
+#pragma unroll
+              for (int n = 0; n < NT; n++) x[n].set(row_unit<LD>(tid, F, 16 * m, 16 * n));
+              N[HT * half + m] = dot3<BF, NT>(x, Sp, N[HT * half + m]);
+            }
+          } else {
+#pragma unroll
+            for (int m = 0; m < NT; m++) {
+              Pair<BF> x[HT];
+#pragma unroll
+              for (int n = 0; n < HT; n++) x[n].set(col_unit<LD>(tid, F, 16 * n, 16 * m));
+              N[m] = dot3<BF, HT>(x, Sp + HT * half, N[m]);
+            }
+          }
+        }
+      }
+      float* out = (BACK ? o.dend + at * Ku * Vu : s.start + (at + s.units) * Ku * Vu);
+#pragma unroll
+      for (int m = 0; m < NT; m++) {
+        S[m] = N[m];
+        put_own_tile(tid, out, Ku, Vu, m, w, S[m]);
+      }
+    }
+  }
+}
+
+// The gradient of one segment of one sequence's head, chunks in reverse. Wavefront w holds dS's columns 16 w .. and, for the
+// products that contract over V, the transposed dS's (rows 16 w .. of dS). LOCAL: what the segment adds to dS alone.
 template <bool BF, int P> struct BwdLds {
   using T = typename Elem<BF>::type;
   static constexpr int CH = Elem<BF>::CH, LD = P + Elem<BF>::pad, UD = CH + 4, CP = CH + 4, NT = P / 16;
@@ -600,27 +833,34 @@ template <bool BF, int P> struct BwdLds {
     float W[CH * CP];  // P_ij dO_i U_j - M_ij dY_i U_j
   };
   float ysum[NT][CH], pairs[CH / 16][CH], tot[NT];
-  Rows<CH> R;
+  Rows<CH> R[2];
+};
+template <bool BF, int P> struct BwdLocalLds {
+  using T = typename Elem<BF>::type;
+  static constexpr int CH = Elem<BF>::CH, LD = P + Elem<BF>::pad, CP = CH + 4;
+  T Q[CH * LD], K[CH * LD], dO[CH * LD];
+  float M[CH * CP], Pm[CH * CP], Tm[CH * CP];
+  Rows<CH> R[2];
 };
 
 // A tile's values into a transposed buffer pair at rows 16 w + l % 16, columns `at` + 4 (l / 16) + 0..3; and units of it.
-template <bool BF, int UD, typename T> __device__ __forceinline__ void put_t(T* hi, T* lo, int w, int at, f4 v) {
-  const int l = threadIdx.x & 63, o = (16 * w + (l & 15)) * UD + at + 4 * (l >> 4);
+template <bool BF, int UD, typename T> __device__ __forceinline__ void put_t(int tid, T* hi, T* lo, int w, int at, f4 v) {
+  const int l = tid & 63, o = (16 * w + (l & 15)) * UD + at + 4 * (l >> 4);
   Pair<BF> p;
   p.set(v);
   *reinterpret_cast<typename Elem<BF>::unit*>(hi + o) = p.hi;
   if constexpr (BF) *reinterpret_cast<s4*>(lo + o) = p.lo;
 }
-template <bool BF, int UD, typename T> __device__ __forceinline__ Pair<BF> col_pair(const T* hi, const T* lo, int row, int col) {
+template <bool BF, int UD, typename T> __device__ __forceinline__ Pair<BF> col_pair(int tid, const T* hi, const T* lo, int row, int col) {
   Pair<BF> p;
-  p.hi = col_unit<UD>(hi, row, col);
-  if constexpr (BF) p.lo = col_unit<UD>(lo, row, col);
+  p.hi = col_unit<UD>(tid, hi, row, col);
+  if constexpr (BF) p.lo = col_unit<UD>(tid, lo, row, col);
   return p;
 }
-template <bool BF, int UD, typename T> __device__ __forceinline__ Pair<BF> row_pair(const T* hi, const T* lo, int row, int col) {
+template <bool BF, int UD, typename T> __device__ __forceinline__ Pair<BF> row_pair(int tid, const T* hi, const T* lo, int row, int col) {
   Pair<BF> p;
-  p.hi = row_unit<UD>(hi, row, col);
-  if constexpr (BF) p.lo = row_unit<UD>(lo, row, col);
+  p.hi = row_unit<UD>(tid, hi, row, col);
+  if constexpr (BF) p.lo = row_unit<UD>(tid, lo, row, col);
   return p;
 }
 __device__ __forceinline__ float row16_sum(float v) {
@@ -631,123 +871,189 @@ __device__ __forceinline__ float row16_sum(float v) {
   return v;
 }
 
-template <bool BF, int P> __global__ void __launch_bounds__(4 * P) k_delta_bwd(const Args s, const GradArgs o) {
+template <bool BF, int P, bool LOCAL>
+__global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const Args s, const GradArgs o) {
   using T = typename Elem<BF>::type;
   using unit = typename Elem<BF>::unit;
-  using Lds = BwdLds<BF, P>;
-  constexpr int CH = Lds::CH, NB = CH / 16, NT = Lds::NT, LD = Lds::LD, CP = Lds::CP, UD = Lds::UD;
+  using Lds = std::conditional_t<LOCAL, BwdLocalLds<BF, P>, BwdLds<BF, P>>;
+  constexpr int CH = Lds::CH, NB = CH / 16, NT = P / 16, LD = Lds::LD, CP = Lds::CP, UD = CH + 4;
   constexpr int TILES = NB * (NB + 1) / 2;
   static_assert(sizeof(Lds) <= kMaxLdsBytes, "LDS of a block");
   __shared__ __attribute__((aligned(16))) Lds L;
-  Rows<CH>& R = L.R;
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int tid = threadIdx.x, l = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
-  for (long unit_id = blockIdx.x; unit_id < s.units; unit_id += gridDim.x) {
-    const long bt = unit_id / s.H;
-    const int h = (int)(unit_id % s.H), hk = h / (s.H / s.Hk);
-    const T* qp = (const T*)s.q + bt * s.q_b + hk * s.q_h;
-    const T* kp = (const T*)s.k + bt * s.k_b + hk * s.k_h;
-    const T* vp = (const T*)s.v + bt * s.v_b + h * s.v_h;
-    const T* op = (const T*)o.dy + bt * o.dy_b + h * o.dy_h;
-    const long kv = (long)s.K * s.V;
+  const long items = s.units * (LOCAL ? s.segs - 1 : s.segs);
+  for (long item = blockIdx.x; item < items; item += gridDim.x) {
+    const unsigned units = (unsigned)s.units, round = (unsigned)item / units;
+    const long unit_id = (unsigned)item - round * units, seg = round + (LOCAL ? 1 : 0), bt = (unsigned)unit_id / (unsigned)s.H;
+    const int h = (int)(unit_id - bt * s.H), hk = (int)((unsigned)h / (unsigned)(s.H / s.Hk)), Ku = up16(s.K), Vu = up16(s.V);
+    const long c_first = seg * s.seg_chunks, c_all = (s.T + CH - 1) / CH;
+    long c = c_first + s.seg_chunks < c_all ? c_first + s.seg_chunks - 1 : c_all - 1;
+    const T* qp = thread_row<BF, P>(tid, (const T*)s.q + bt * s.q_b + hk * s.q_h, s.q_t, c * CH);
+    const T* kp = thread_row<BF, P>(tid, (const T*)s.k + bt * s.k_b + hk * s.k_h, s.k_t, c * CH);
+    const T* vp = thread_row<BF, P>(tid, (const T*)s.v + bt * s.v_b + h * s.v_h, s.v_t, c * CH);
+    const T* op = thread_row<BF, P>(tid, (const T*)o.dy + bt * o.dy_b + h * o.dy_h, o.dy_t, c * CH);
     const float A = s.A[h];
-    double sumA = 0.0, sumB = 0.0;  // of wavefront 0's lanes
-    f4 dS[NT], dSt[NT];
+    auto rows_at = [&](long ch) { return (int)(ch < c_first ? 0 : s.T - ch * CH < CH ? s.T - ch * CH : CH); };
+    double sumA = 0.0, sumB = 0.0;  // of the lanes that see to the gates
+    f4 dS[NT], dSt[LOCAL ? 1 : NT];
+    if (!LOCAL && s.segs > 1) {
+      const float* d = o.dend + (seg * s.units + unit_id) * Ku * Vu;
 #pragma unroll
-    for (int m = 0; m < NT; m++) {
-      dS[m] = state_tile(o.dh ? o.dh + unit_id * kv : nullptr, s.K, s.V, m, w);
-      dSt[m] = state_tile_t(o.dh ? o.dh + unit_id * kv : nullptr, s.K, s.V, m, w);
+      for (int m = 0; m < NT; m++) {
+        dS[m] = own_tile(tid, d, Ku, Vu, m, w);
+        if constexpr (!LOCAL) dSt[m] = own_tile_t(tid, d, Ku, Vu, m, w);
+      }
+    } else if (!LOCAL && o.dh) {
+#pragma unroll
+      for (int m = 0; m < NT; m++) {
+        dS[m] = state_tile(tid, o.dh + unit_id * s.K * s.V, s.K, s.V, m, w);
+        if constexpr (!LOCAL) dSt[m] = state_tile_t(tid, o.dh + unit_id * s.K * s.V, s.K, s.V, m, w);
+      }
+    } else {
+#pragma unroll
+      for (int m = 0; m < NT; m++) {
+        dS[m] = zero;
+        if constexpr (!LOCAL) dSt[m] = zero;
+      }
     }
-    for (long c = (s.T + CH - 1) / CH - 1; c >= 0; c--) {
+    int rows = rows_at(c);
+    u4 q, k, v = {0, 0, 0, 0}, d;
+    auto load = [&]() {
+      q = load_row<BF, P>(tid, qp, rows, s.K);
+      k = load_row<BF, P>(tid, kp, rows, s.K);
+      if (!LOCAL) v = load_row<BF, P>(tid, vp, rows, s.V);
+      d = load_row<BF, P>(tid, op, rows, s.V);
+    };
+    auto walk = [&](long chunks) {
+      qp += chunks * CH * s.q_t;
+      kp += chunks * CH * s.k_t;
+      vp += chunks * CH * s.v_t;
+      op += chunks * CH * o.dy_t;
+    };
+    load();
+    // the last wavefront sees to the gates, a chunk ahead
+    Gate g = {0.f, 0.f, 0.f}, gn = g;
+    if (w == NT - 1) {
+      g = load_gate<T>(s, bt, h, c * CH, rows, l);
+      gn = load_gate<T>(s, bt, h, (c - 1) * CH, rows_at(c - 1), l);
+    }
+    __syncthreads();  // the item before has been read
+    if (w == NT - 1) fill_rows<CH>(tid, L.R[0], g, A, 0, rows);
+    int cur = 0;
+    for (; c >= c_first; c--) {
+      Rows<CH>& R = L.R[cur];
       const long t0 = c * CH;
-      const int rows = (int)(s.T - t0 < CH ? s.T - t0 : CH);
-      const float* S0 = o.keep + (c * s.units + unit_id) * kv;
-      const u4 q = load_row<BF, P>(qp + t0 * s.q_t, s.q_t, rows, s.K, s.vec);
-      const u4 k = load_row<BF, P>(kp + t0 * s.k_t, s.k_t, rows, s.K, s.vec);
-      const u4 v = load_row<BF, P>(vp + t0 * s.v_t, s.v_t, rows, s.V, s.vec);
-      const u4 d = load_row<BF, P>(op + t0 * o.dy_t, o.dy_t, rows, s.V, s.vec);
-      Gate g;
-      if (w == 0) g = load_gate<T>(s, bt, h, t0, rows, l);
-      for (int lo = 0, hi = rows; hi > 0;) {
+      const int all = rows;  // rows of this chunk
+      for (int lo = 0, hi = all, once = 1; hi > 0; once = 0) {
         __syncthreads();  // the rows before have been read
-        put_row<BF, P>(L.Q, q, lo, hi);
-        put_row<BF, P>(L.K, k, lo, hi);
-        put_row<BF, P>(L.V, v, lo, hi);
-        put_row<BF, P>(L.dO, d, lo, hi);
-        put_norm<BF, P>(R.rq, q, lo, hi);
-        put_norm<BF, P>(R.rk, k, lo, hi);
+        renew(tid, l);
+        if (!once) {  // one episode at a time: rows and gates again
+          rows = all;
+          load();
+        }
+        const bool odd = tid / (P / Elem<BF>::V) >= lo && tid / (P / Elem<BF>::V) < hi && (!all_finite<BF>(q) || !all_finite<BF>(d));
+        put_row<BF, P>(tid, L.Q, q, lo, hi);
+        put_row<BF, P>(tid, L.K, k, lo, hi);
+        if constexpr (!LOCAL) put_row<BF, P>(tid, L.V, v, lo, hi);
+        put_row<BF, P>(tid, L.dO, d, lo, hi);
+        put_norm<BF, P>(tid, R.rq, q, lo, hi);
+        put_norm<BF, P>(tid, R.rk, k, lo, hi);
+        if (!once && w == NT - 1) fill_rows<CH>(tid, R, g, A, lo, hi);
+        f4 S0[LOCAL ? 1 : NT];
+        if constexpr (!LOCAL) {
+#pragma unroll
+          for (int m = 0; m < NT; m++) S0[m] = own_tile(tid, o.keep + (c * s.units + unit_id) * Ku * Vu, Ku, Vu, m, w);
+        }
         __syncthreads();
-        if (w == 0) fill_rows<CH>(R, g, A, lo, hi);
+        if (once) {  // the next chunk's are on their way while this one computes
+          walk(-1);
+          rows = rows_at(c - 1);
+          load();
+        }
+        score_tiles<BF, P, LD, true>(tid, R, L.Q, L.K, L.M, L.Pm, s.scale);
         __syncthreads();
-        score_tiles<BF, P, LD>(R, L.Q, L.K, L.M, L.Pm, s.scale);
-        __syncthreads();
-        if (w == 0) invert_blocks<CH>(L.M, L.Tm);
+        if (w == 0) invert_blocks<CH>(tid, L.M, L.Tm);
+        if (w == NT - 1 && once) fill_rows<CH>(tid, L.R[cur ^ 1], gn, A, 0, rows);
         f4 Y[NB], dU[NB], sd = zero;
         {
-          Pair<BF> Sp[NT], Dp[NT];
+          Pair<BF> Sp[NT];
+          if constexpr (!LOCAL) {
 #pragma unroll
-          for (int m = 0; m < NT; m++) {
-            const f4 S = state_tile(S0, s.K, s.V, m, w);
-            sd += S * dS[m];
-            Sp[m].set(S);
-            Dp[m].set(dS[m]);
+            for (int m = 0; m < NT; m++) {
+              sd += S0[m] * dS[m];
+              Sp[m].set(S0[m]);
+            }
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+              unit x[NT];
+#pragma unroll
+              for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, L.K, 16 * n, 16 * m);
+              Y[n] = rows4(tid, R.be, 16 * n) * (widen(col_unit<LD>(tid, L.V, 16 * n, 16 * w)) -
+                                            sel_mul(rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n), dot2<BF, NT>(x, Sp, zero)));
+            }
           }
+#pragma unroll
+          for (int m = 0; m < NT; m++) Sp[m].set(dS[m]);
 #pragma unroll
           for (int n = 0; n < NB; n++) {
             unit x[NT];
 #pragma unroll
-            for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(L.K, 16 * n, 16 * m);
-            Y[n] = rows4(R.be, 16 * n) * (widen(col_unit<LD>(L.V, 16 * n, 16 * w)) -
-                                          sel_mul(rows4(R.d0, 16 * n) * rows4(R.rk, 16 * n), dot2<BF, NT>(x, Sp, zero)));
-            dU[n] = sel_mul(rows4(R.dc, 16 * n) * rows4(R.rk, 16 * n), dot2<BF, NT>(x, Dp, zero));
+            for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, L.K, 16 * n, 16 * m);
+            dU[n] = sel_mul(rows4(tid, R.dc, 16 * n) * rows4(tid, R.rk, 16 * n), dot2<BF, NT>(x, Sp, zero));
           }
         }
         __syncthreads();
-        // dU, dY, U: this wavefront's columns of V
+        renew(tid, l);
+        // U, dU, dY: this wavefront's columns of V
         f4 U[NB], dY[NB];
         unit dOc[NB];
         {
-          solve<BF>(L.Tm, L.M, Y, U);
+          if constexpr (!LOCAL) solve<BF>(tid, L.Tm, L.M, Y, U);
           Pair<BF> x[NB];
 #pragma unroll
-          for (int n = 0; n < NB; n++) dOc[n] = col_unit<LD>(L.dO, 16 * n, 16 * w);
-          x[0].set(col_unit<CP>(L.Pm, 0, 0));
+          for (int n = 0; n < NB; n++) dOc[n] = col_unit<LD>(tid, L.dO, 16 * n, 16 * w);
+          x[0].set(col_unit<CP>(tid, L.Pm, 0, 0));
           if constexpr (NB == 2) {
-            x[1].set(col_unit<CP>(L.Pm, 16, 0));
+            x[1].set(col_unit<CP>(tid, L.Pm, 16, 0));
             dU[0] = dot2r<BF, 2>(x, dOc, dU[0]);
-            x[0].set(col_unit<CP>(L.Pm, 16, 16));
+            x[0].set(col_unit<CP>(tid, L.Pm, 16, 16));
             dU[1] = dot2r<BF, 1>(x, dOc + 1, dU[1]);
           } else {
             dU[0] = dot2r<BF, 1>(x, dOc, dU[0]);
           }
-          solve_t<BF>(L.Tm, L.M, dU, dY);
+          solve_t<BF>(tid, L.Tm, L.M, dU, dY);
         }
-        const int inside = R.starts & ~(1 << lo);
+        const int starts = R.starts, inside = starts & ~(1 << lo);
         if (inside) {
-          const int row = threadIdx.x / (P / Elem<BF>::V);
-          bool bad = row >= lo && row < hi && (!all_finite<BF>(q) || !all_finite<BF>(d));
+          bool bad = odd;
 #pragma unroll
           for (int n = 0; n < NB; n++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) bad |= !finite(U[n][i]) || !finite(dY[n][i]);
+            for (int i = 0; i < 4; i++) bad |= (!LOCAL && !finite(U[n][i])) || !finite(dY[n][i]);
           if (__syncthreads_or(bad)) {
+            if (once) walk(1);
             lo = 31 - __clz(inside);
             continue;
           }
         }
         const int col = 16 * w + (l & 15);
+        if constexpr (!LOCAL) {
+          const GradArgs a = again<GradArgs>(sizeof(Args));
+          T* dvp = (T*)a.dv + bt * a.dv_b + h * a.dv_h + t0 * a.dv_t + col;
 #pragma unroll
-        for (int n = 0; n < NB; n++) {
-          const f4 be = rows4(R.be, 16 * n);
-          put_t<BF, UD>(L.U, L.Ulo, w, 16 * n, U[n]);
-          put_t<BF, UD>(L.dY, L.dYlo, w, 16 * n, dY[n]);
+          for (int n = 0; n < NB; n++) {
+            const f4 be = rows4(tid, R.be, 16 * n);
+            put_t<BF, UD>(tid, L.U, L.Ulo, w, 16 * n, U[n]);
+            put_t<BF, UD>(tid, L.dY, L.dYlo, w, 16 * n, dY[n]);
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int row = 16 * n + 4 * (l >> 4) + i;
-            if (o.dv && row >= lo && row < hi && col < s.V)
-              stf((T*)o.dv + bt * o.dv_b + h * o.dv_h + (t0 + row) * o.dv_t + col, be[i] * dY[n][i]);
-            const float sum = row16_sum(dY[n][i] * U[n][i]);
-            if ((l & 15) == 0) L.ysum[w][row] = sum;
+            for (int i = 0; i < 4; i++) {
+              const int row = 16 * n + 4 * (l >> 4) + i;
+              if (a.dv && row >= lo && row < hi && col < s.V) stf(dvp + row * a.dv_t, be[i] * dY[n][i]);
+              const float sum = row16_sum(dY[n][i] * U[n][i]);
+              if ((l & 15) == 0) L.ysum[w][row] = sum;
+            }
           }
         }
         const float c0 = R.c0;
@@ -757,249 +1063,272 @@ template <bool BF, int P> __global__ void __launch_bounds__(4 * P) k_delta_bwd(c
           Pair<BF> x[NB], y[NB];
 #pragma unroll
           for (int n = 0; n < NB; n++) {
-            x[n].set(sel_mul(s.scale * rows4(R.d0, 16 * n) * rows4(R.rq, 16 * n), widen(dOc[n])));
-            y[n].set(sel_mul(-rows4(R.d0, 16 * n) * rows4(R.rk, 16 * n) * rows4(R.be, 16 * n), dY[n]));
+            x[n].set(sel_mul(s.scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n), widen(dOc[n])));
+            y[n].set(sel_mul(-rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n) * rows4(tid, R.be, 16 * n), dY[n]));
           }
 #pragma unroll
           for (int m = 0; m < NT; m++) {
             unit a[NB];
 #pragma unroll
-            for (int n = 0; n < NB; n++) a[n] = col_unit<LD>(L.Q, 16 * n, 16 * m);
+            for (int n = 0; n < NB; n++) a[n] = col_unit<LD>(tid, L.Q, 16 * n, 16 * m);
             dS[m] = dot2<BF, NB>(a, x, sel_mul(f4{c0, c0, c0, c0}, dS[m]));
 #pragma unroll
-            for (int n = 0; n < NB; n++) a[n] = col_unit<LD>(L.K, 16 * n, 16 * m);
+            for (int n = 0; n < NB; n++) a[n] = col_unit<LD>(tid, L.K, 16 * n, 16 * m);
             dS[m] = dot2<BF, NB>(a, y, dS[m]);
           }
         }
-        __syncthreads();
-        for (int tile = w; tile < TILES; tile += NT) {
-          const int bi = tile == 0 ? 0 : 1, bj = tile == 2 ? 1 : 0;  // (0,0) (1,0) (1,1)
-          f4 e = zero, f = zero;
-          {
-            Pair<BF> y[NT], x[NT];
-            unit z[NT];
+        if constexpr (!LOCAL) {
+          Pair<BF> Xt[NT];  // S_0 transposed, then dS
 #pragma unroll
-            for (int m = 0; m < NT; m++) {
-              y[m] = col_pair<BF, UD>(L.U, L.Ulo, 16 * m, 16 * bj);
-              z[m] = row_unit<LD>(L.dO, 16 * bi, 16 * m);
-              x[m] = col_pair<BF, UD>(L.dY, L.dYlo, 16 * m, 16 * bi);
+          for (int m = 0; m < NT; m++) S0[m] = own_tile_t(tid, o.keep + (c * s.units + unit_id) * Ku * Vu, Ku, Vu, m, w);
+          __syncthreads();
+        renew(tid, l);
+          for (int tile = w; tile < TILES; tile += NT) {
+            const int bi = tile == 0 ? 0 : 1, bj = tile == 2 ? 1 : 0;  // (0,0) (1,0) (1,1)
+            f4 e = zero, f = zero;
+            {
+              Pair<BF> y[NT], x[NT];
+              unit z[NT];
+#pragma unroll
+              for (int m = 0; m < NT; m++) {
+                y[m] = col_pair<BF, UD>(tid, L.U, L.Ulo, 16 * m, 16 * bj);
+                z[m] = row_unit<LD>(tid, L.dO, 16 * bi, 16 * m);
+              }
+              e = dot2<BF, NT>(z, y, e);
+#pragma unroll
+              for (int m = 0; m < NT; m++) x[m] = col_pair<BF, UD>(tid, L.dY, L.dYlo, 16 * m, 16 * bi);
+              f = dot3<BF, NT>(x, y, f);
             }
-            e = dot2<BF, NT>(z, y, e);
-            f = dot3<BF, NT>(x, y, f);
-          }
-          const int j = 16 * bj + (l & 15);
-          const double Gj = R.G[j];
-          const int segj = R.seg[j];
+            const int j = 16 * bj + (l & 15);
+            const double Gj = R.G[j];
+            const int segj = R.seg[j];
 #pragma unroll
-          for (int i4 = 0; i4 < 4; i4++) {
-            const int i = 16 * bi + 4 * (l >> 4) + i4, at = i * CP + j;
-            const bool on = segj == R.seg[i] && j <= i;
-            const float d = ex2((float)(R.G[i] - Gj));
-            L.W[at] = on && j < i ? L.Pm[at] * e[i4] - L.M[at] * f[i4] : 0.f;
-            L.E[at] = on ? d * s.scale * e[i4] : 0.f;
-            L.F[at] = on && j < i ? -d * R.be[i] * f[i4] : 0.f;
+            for (int i4 = 0; i4 < 4; i4++) {
+              const int i = 16 * bi + 4 * (l >> 4) + i4, at = i * CP + j;
+              const bool on = segj == R.seg[i] && j <= i;
+              const float dec = ex2((float)(R.G[i] - Gj));
+              L.W[at] = on && j < i ? L.Pm[at] * e[i4] - L.M[at] * f[i4] : 0.f;
+              L.E[at] = on ? dec * s.scale * e[i4] : 0.f;
+              L.F[at] = on && j < i ? -dec * R.be[i] * f[i4] : 0.f;
+            }
           }
-        }
-        // products over V for this wavefront's columns of K: dO S_0^T, dY S_0^T, U dS^T
-        f4 X1[NB], X2[NB], X3[NB];
-        {
-          Pair<BF> St[NT], Dt[NT];
+          renew(tid, l);
+          // products over V for this wavefront's columns of K: dO S_0^T, dY S_0^T, U dS^T
+          f4 X1[NB], X2[NB], X3[NB];
 #pragma unroll
-          for (int m = 0; m < NT; m++) {
-            St[m].set(state_tile_t(S0, s.K, s.V, m, w));
-            Dt[m].set(dSt[m]);
-          }
+          for (int m = 0; m < NT; m++) Xt[m].set(S0[m]);
 #pragma unroll
           for (int n = 0; n < NB; n++) {
             unit x[NT];
 #pragma unroll
-            for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(L.dO, 16 * n, 16 * m);
-            X1[n] = sel_mul(s.scale * rows4(R.d0, 16 * n), dot2<BF, NT>(x, St, zero));
+            for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, L.dO, 16 * n, 16 * m);
+            X1[n] = sel_mul(s.scale * rows4(tid, R.d0, 16 * n), dot2<BF, NT>(x, Xt, zero));
             Pair<BF> y[NT];
 #pragma unroll
-            for (int m = 0; m < NT; m++) y[m] = col_pair<BF, UD>(L.dY, L.dYlo, 16 * m, 16 * n);
-            X2[n] = sel_mul(-rows4(R.d0, 16 * n) * rows4(R.be, 16 * n), dot3<BF, NT>(y, St, zero));
-#pragma unroll
-            for (int m = 0; m < NT; m++) y[m] = col_pair<BF, UD>(L.U, L.Ulo, 16 * m, 16 * n);
-            X3[n] = sel_mul(rows4(R.dc, 16 * n), dot3<BF, NT>(y, Dt, zero));
+            for (int m = 0; m < NT; m++) y[m] = col_pair<BF, UD>(tid, L.dY, L.dYlo, 16 * m, 16 * n);
+            X2[n] = sel_mul(-rows4(tid, R.d0, 16 * n) * rows4(tid, R.be, 16 * n), dot3<BF, NT>(y, Xt, zero));
           }
-        }
-        unit Kc[NB], Qc[NB];  // this wavefront's columns of K and Q
 #pragma unroll
-        for (int n = 0; n < NB; n++) {
-          Kc[n] = col_unit<LD>(L.K, 16 * n, 16 * w);
-          Qc[n] = col_unit<LD>(L.Q, 16 * n, 16 * w);
-        }
-        {
-          Pair<BF> x[NB], y[NB];
+          for (int m = 0; m < NT; m++) Xt[m].set(dSt[m]);
 #pragma unroll
           for (int n = 0; n < NB; n++) {
-            x[n].set(sel_mul(s.scale * rows4(R.d0, 16 * n) * rows4(R.rq, 16 * n), widen(Qc[n])));
-            y[n].set(sel_mul(-rows4(R.d0, 16 * n) * rows4(R.rk, 16 * n) * rows4(R.be, 16 * n), widen(Kc[n])));
+            Pair<BF> y[NT];
+#pragma unroll
+            for (int m = 0; m < NT; m++) y[m] = col_pair<BF, UD>(tid, L.U, L.Ulo, 16 * m, 16 * n);
+            X3[n] = sel_mul(rows4(tid, R.dc, 16 * n), dot3<BF, NT>(y, Xt, zero));
           }
-#pragma unroll
-          for (int m = 0; m < NT; m++) {
-            unit a[NB];
-#pragma unroll
-            for (int n = 0; n < NB; n++) a[n] = col_unit<LD>(L.dO, 16 * n, 16 * m);
-            dSt[m] = dot2<BF, NB>(a, x, sel_mul(f4{c0, c0, c0, c0}, dSt[m]));
-            Pair<BF> b[NB];
-#pragma unroll
-            for (int n = 0; n < NB; n++) b[n] = row_pair<BF, UD>(L.dY, L.dYlo, 16 * m, 16 * n);
-            dSt[m] = dot3<BF, NB>(b, y, dSt[m]);
-          }
-        }
-        __syncthreads();
-        // E K, F K (rows as i), F^T K, E^T Q (rows as j); the norms' factors go into E and F
-        f4 dQ[NB], dKi[NB], dKj[NB];
-        {
-          f4 rk[NB], rq[NB];
+          renew(tid, l);
+          unit Kc[NB], Qc[NB];  // this wavefront's columns of K and Q
 #pragma unroll
           for (int n = 0; n < NB; n++) {
-            rk[n] = rows4(R.rk, 16 * n);
-            rq[n] = rows4(R.rq, 16 * n);
+            Kc[n] = col_unit<LD>(tid, L.K, 16 * n, 16 * w);
+            Qc[n] = col_unit<LD>(tid, L.Q, 16 * n, 16 * w);
           }
+          {
+            Pair<BF> x[NB], y[NB];
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+              x[n].set(sel_mul(s.scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n), widen(Qc[n])));
+              y[n].set(sel_mul(-rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n) * rows4(tid, R.be, 16 * n), widen(Kc[n])));
+            }
+#pragma unroll
+            for (int m = 0; m < NT; m++) {
+              unit a[NB];
+#pragma unroll
+              for (int n = 0; n < NB; n++) a[n] = col_unit<LD>(tid, L.dO, 16 * n, 16 * m);
+              dSt[m] = dot2<BF, NB>(a, x, sel_mul(f4{c0, c0, c0, c0}, dSt[m]));
+              Pair<BF> b[NB];
+#pragma unroll
+              for (int n = 0; n < NB; n++) b[n] = row_pair<BF, UD>(tid, L.dY, L.dYlo, 16 * m, 16 * n);
+              dSt[m] = dot3<BF, NB>(b, y, dSt[m]);
+            }
+          }
+          __syncthreads();
+        renew(tid, l);
+          // E K, F K (rows as i), F^T K, E^T Q (rows as j); the norms' factors go into E and F
+          f4 dQ[NB], dK[NB];
+          {
+            f4 rk[NB], rq[NB];
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+              rk[n] = rows4(tid, R.rk, 16 * n);
+              rq[n] = rows4(tid, R.rq, 16 * n);
+            }
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+              const f4 qn = widen(Qc[n]) * rq[n], kn = widen(Kc[n]) * rk[n];
+              const f4 from0 = qn * X1[n] + kn * X2[n], fromc = kn * X3[n];
+              Pair<BF> e[NB], f[NB];
+#pragma unroll
+              for (int m = 0; m <= n; m++) {
+                e[m].set(row_unit<CP>(tid, L.E, 16 * n, 16 * m) * rk[m]);
+                f[m].set(row_unit<CP>(tid, L.F, 16 * n, 16 * m) * rk[m]);
+              }
+              if (n == 0) {
+                dQ[n] = dot2r<BF, 1>(e, Kc, X1[n]);
+                dK[n] = dot2r<BF, 1>(f, Kc, X2[n] + X3[n]);
+              } else {
+                dQ[n] = dot2r<BF, NB>(e, Kc, X1[n]);
+                dK[n] = dot2r<BF, NB>(f, Kc, X2[n] + X3[n]);
+              }
+#pragma unroll
+              for (int m = n; m < NB; m++) {
+                e[m].set(col_unit<CP>(tid, L.E, 16 * m, 16 * n) * rq[m]);
+                f[m].set(col_unit<CP>(tid, L.F, 16 * m, 16 * n) * rk[m]);
+              }
+              if (n == NB - 1) dK[n] = dot2r<BF, 1>(f + n, Kc + n, dot2r<BF, 1>(e + n, Qc + n, dK[n]));
+              else dK[n] = dot2r<BF, NB>(f, Kc, dot2r<BF, NB>(e, Qc, dK[n]));
+              const f4 sq = qn * dQ[n], sk = kn * dK[n];
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                const float x[4] = {row16_sum(sq[i]), row16_sum(sk[i]), row16_sum(from0[i]), row16_sum(fromc[i])};
+                if ((l & 15) == 0) {
+#pragma unroll
+                  for (int j = 0; j < 4; j++) L.sums[j][w][16 * n + 4 * (l >> 4) + i] = x[j];
+                }
+              }
+            }
+          }
+          // sums over the pairs j < t <= i, rows t: a triangle of ones times W, then along the row
+          for (int tile = w; tile < TILES; tile += NT) {
+            const int bt_ = tile == 0 ? 0 : 1, bj = tile == 2 ? 1 : 0, t = 16 * bt_ + (l & 15);
+            f4 acc = zero;
+            for (int m = bt_; m < NB; m++) {
+              f4 ones;
+#pragma unroll
+              for (int i = 0; i < 4; i++) ones[i] = 16 * m + 4 * (l >> 4) + i >= t ? 1.f : 0.f;
+              const f4 x = col_unit<CP>(tid, L.W, 16 * m, 16 * bj);
+              acc = dot<1>(&ones, &x, acc);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const int row = 16 * bt_ + 4 * (l >> 4) + i;
+              const float sum = row16_sum(16 * bj + (l & 15) < row ? acc[i] : 0.f);
+              if ((l & 15) == 0) L.pairs[bj][row] = sum;
+            }
+          }
+          tot = group_sum<64>(tot);
+          if (l == 0) L.tot[w] = tot;
+          __syncthreads();
+        renew(tid, l);
+          // through the norms
+          const GradArgs a = again<GradArgs>(sizeof(Args));
+          const Args sa = again<Args>(0);
 #pragma unroll
           for (int n = 0; n < NB; n++) {
-            Pair<BF> e[NB], f[NB];
+            const f4 rq = rows4(tid, R.rq, 16 * n), rk = rows4(tid, R.rk, 16 * n);
+            f4 sq = zero, sk = zero;
 #pragma unroll
-            for (int m = 0; m <= n; m++) {
-              e[m].set(row_unit<CP>(L.E, 16 * n, 16 * m) * rk[m]);
-              f[m].set(row_unit<CP>(L.F, 16 * n, 16 * m) * rk[m]);
+            for (int m = 0; m < NT; m++) {
+              sq += rows4(tid, L.sums[0][m], 16 * n);
+              sk += rows4(tid, L.sums[1][m], 16 * n);
             }
-            if (n == 0) {
-              dQ[n] = dot2r<BF, 1>(e, Kc, zero);
-              dKi[n] = dot2r<BF, 1>(f, Kc, zero);
-            } else {
-              dQ[n] = dot2r<BF, NB>(e, Kc, zero);
-              dKi[n] = dot2r<BF, NB>(f, Kc, zero);
-            }
+            const f4 dq = rq * (dQ[n] - widen(Qc[n]) * rq * sq), dk = rk * (dK[n] - widen(Kc[n]) * rk * sk);
 #pragma unroll
-            for (int m = n; m < NB; m++) {
-              e[m].set(col_unit<CP>(L.E, 16 * m, 16 * n) * rq[m]);
-              f[m].set(col_unit<CP>(L.F, 16 * m, 16 * n) * rk[m]);
+            for (int i = 0; i < 4; i++) {
+              const int row = 16 * n + 4 * (l >> 4) + i;
+              if (row < lo || row >= hi || col >= sa.K) continue;
+              if (a.qpart) {
+                const long at = (((t0 + row) * sa.B + bt) * sa.H + h) * sa.K + col;
+                a.qpart[at] = dq[i];
+                a.kpart[at] = dk[i];
+              } else {
+                if (a.dq) stf((T*)a.dq + bt * a.dq_b + h * a.dq_h + (t0 + row) * a.dq_t + col, dq[i]);
+                if (a.dk) stf((T*)a.dk + bt * a.dk_b + h * a.dk_h + (t0 + row) * a.dk_t + col, dk[i]);
+              }
             }
-            if (n == NB - 1) {
-              dKj[n] = dot2r<BF, 1>(f + n, Kc + n, dot2r<BF, 1>(e + n, Qc + n, zero));
-            } else {
-              dKj[n] = dot2r<BF, NB>(f, Kc, dot2r<BF, NB>(e, Qc, zero));
+          }
+          if (w == NT - 1) {  // the gates
+            float from0 = 0.f, fromc = 0.f, dbr = 0.f, sum = 0.f;
+            const int i = l < CH ? l : CH - 1;
+#pragma unroll
+            for (int m = 0; m < NT; m++) {
+              from0 += L.sums[2][m][i];
+              fromc += L.sums[3][m][i];
+              dbr += L.ysum[m][i];
+              sum += L.tot[m];
+            }
+            if (l >= CH) from0 = fromc = 0.f;
+#pragma unroll
+            for (int e = 1; e < CH; e *= 2) {  // of the rows from t on, of the rows up to t
+              const float x = __shfl_down(from0, e), y = __shfl_up(fromc, e);
+              if (l + e < CH) from0 += x;
+              if (l >= e) fromc += y;
+            }
+            fromc = __shfl_up(fromc, 1);
+            if (l == 0) fromc = 0.f;
+            float dg = L.pairs[0][i] + from0 + fromc + sum;
+            if (NB == 2 && i >= 16) dg += L.pairs[NB - 1][i];
+            if (l >= lo && l < hi) {
+              const float be = R.be[l], arg = R.arg[l];
+              const float da = dg * A * sigma(arg);
+              if (a.da) stf((T*)a.da + (t0 + l) * a.da_t + bt * a.da_b + h, da);
+              if (a.db) stf((T*)a.db + (t0 + l) * a.db_t + bt * a.db_b + h, dbr * (1.f - be));
+              sumA += (double)dg * (double)R.sp[l];
+              sumB += (double)da;
             }
           }
         }
-#pragma unroll
-        for (int n = 0; n < NB; n++) {
-          const f4 qn = widen(Qc[n]) * rows4(R.rq, 16 * n), kn = widen(Kc[n]) * rows4(R.rk, 16 * n);
-          const f4 from0 = qn * X1[n] + kn * X2[n], fromc = kn * X3[n];
-          dQ[n] += X1[n];
-          dKi[n] += X2[n];
-          dKi[n] += dKj[n] + X3[n];
-          const f4 sq = qn * dQ[n], sk = kn * dKi[n];
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const float v[4] = {row16_sum(sq[i]), row16_sum(sk[i]), row16_sum(from0[i]), row16_sum(fromc[i])};
-            if ((l & 15) == 0) {
-#pragma unroll
-              for (int e = 0; e < 4; e++) L.sums[e][w][16 * n + 4 * (l >> 4) + i] = v[e];
-            }
-          }
-        }
-        // sums over the pairs j < t <= i, rows t: a triangle of ones times W, then along the row
-        for (int tile = w; tile < TILES; tile += NT) {
-          const int bt = tile == 0 ? 0 : 1, bj = tile == 2 ? 1 : 0, t = 16 * bt + (l & 15);
-          f4 acc = zero;
-          for (int m = bt; m < NB; m++) {
-            f4 ones;
-#pragma unroll
-            for (int i = 0; i < 4; i++) ones[i] = 16 * m + 4 * (l >> 4) + i >= t ? 1.f : 0.f;
-            const f4 x = m == bt && bj > bt ? zero : col_unit<CP>(L.W, 16 * m, 16 * bj);
-            acc = dot<1>(&ones, &x, acc);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int row = 16 * bt + 4 * (l >> 4) + i;
-            const float sum = row16_sum(16 * bj + (l & 15) < row ? acc[i] : 0.f);
-            if ((l & 15) == 0) L.pairs[bj][row] = sum;
-          }
-        }
-        tot = group_sum<64>(tot);
-        if (l == 0) L.tot[w] = tot;
-        __syncthreads();
-        // through the norms
-#pragma unroll
-        for (int n = 0; n < NB; n++) {
-          const f4 rq = rows4(R.rq, 16 * n), rk = rows4(R.rk, 16 * n);
-          f4 sq = zero, sk = zero;
+        if (starts >> lo & 1) {  // nothing passes to the steps before, whatever these hold
 #pragma unroll
           for (int m = 0; m < NT; m++) {
-            sq += rows4(L.sums[0][m], 16 * n);
-            sk += rows4(L.sums[1][m], 16 * n);
+            dS[m] = zero;
+            if constexpr (!LOCAL) dSt[m] = zero;
           }
-          const f4 dq = rq * (dQ[n] - widen(Qc[n]) * rq * sq), dk = rk * (dKi[n] - widen(Kc[n]) * rk * sk);
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int row = 16 * n + 4 * (l >> 4) + i;
-            if (row < lo || row >= hi || col >= s.K) continue;
-            if (o.qpart) {
-              const long at = (((t0 + row) * s.B + bt) * s.H + h) * s.K + col;
-              o.qpart[at] = dq[i];
-              o.kpart[at] = dk[i];
-            } else {
-              if (o.dq) stf((T*)o.dq + bt * o.dq_b + h * o.dq_h + (t0 + row) * o.dq_t + col, dq[i]);
-              if (o.dk) stf((T*)o.dk + bt * o.dk_b + h * o.dk_h + (t0 + row) * o.dk_t + col, dk[i]);
-            }
-          }
-        }
-        if (w == 0) {  // the gates
-          float from0 = 0.f, fromc = 0.f, dbr = 0.f, all = 0.f;
-          const int i = l < CH ? l : CH - 1;
-#pragma unroll
-          for (int m = 0; m < NT; m++) {
-            from0 += L.sums[2][m][i];
-            fromc += L.sums[3][m][i];
-            dbr += L.ysum[m][i];
-            all += L.tot[m];
-          }
-          if (l >= CH) from0 = fromc = 0.f;
-#pragma unroll
-          for (int e = 1; e < CH; e *= 2) {  // of the rows from t on, of the rows up to t
-            const float x = __shfl_down(from0, e), y = __shfl_up(fromc, e);
-            if (l + e < CH) from0 += x;
-            if (l >= e) fromc += y;
-          }
-          fromc = __shfl_up(fromc, 1);
-          if (l == 0) fromc = 0.f;
-          float dg = L.pairs[0][i] + from0 + fromc + all;
-          if (NB == 2 && i >= 16) dg += L.pairs[NB - 1][i];
-          if (l >= lo && l < hi) {
-            const float be = R.be[l], arg = R.arg[l];
-            const float da = dg * A * sigma(arg);
-            if (o.da) stf((T*)o.da + (t0 + l) * o.da_t + bt * o.da_b + h, da);
-            if (o.db) stf((T*)o.db + (t0 + l) * o.db_t + bt * o.db_b + h, dbr * (1.f - be));
-            sumA += (double)dg * (double)R.sp[l];
-            sumB += (double)da;
-          }
-        }
-        if (R.starts >> lo & 1) {  // nothing passes to the steps before, whatever these hold
-#pragma unroll
-          for (int m = 0; m < NT; m++) dS[m] = dSt[m] = zero;
         }
         hi = lo;
         lo = 0;
+        if (!once && hi <= 0) {  // on to the next chunk's rows
+          walk(-1);
+          rows = rows_at(c - 1);
+          load();
+        }
       }
-    }
-    if (o.dh0) {
-#pragma unroll
-      for (int m = 0; m < NT; m++) put_state_tile(o.dh0 + unit_id * kv, s.K, s.V, m, w, dS[m]);
-    }
-    if (w == 0 && o.gpart) {
-#pragma unroll
-      for (int e = 1; e < CH; e *= 2) {
-        sumA += __shfl_xor(sumA, e);
-        sumB += __shfl_xor(sumB, e);
+      if (w == NT - 1) {
+        g = gn;
+        gn = load_gate<T>(s, bt, h, (c - 2) * CH, rows_at(c - 2), l);
       }
-      if (l == 0) {
-        o.gpart[(long)h * s.B + bt] = (float)sumA;
-        o.gpart[((long)s.H + h) * s.B + bt] = (float)sumB;
+      cur ^= 1;
+    }
+    if (LOCAL) {
+#pragma unroll
+      for (int m = 0; m < NT; m++) put_own_tile(tid, o.xi + (seg * s.units + unit_id) * Ku * Vu, Ku, Vu, m, w, dS[m]);
+    } else {
+      if (o.dh0 && seg == 0) {
+#pragma unroll
+        for (int m = 0; m < NT; m++) put_state_tile(tid, o.dh0 + unit_id * s.K * s.V, s.K, s.V, m, w, dS[m]);
+      }
+      if (w == NT - 1 && o.gpart) {
+#pragma unroll
+        for (int e = 1; e < CH; e *= 2) {
+          sumA += __shfl_xor(sumA, e);
+          sumB += __shfl_xor(sumB, e);
+        }
+        if (l == 0) {
+          const long n = s.segs * s.B, at = seg * s.B + bt;
+          o.gpart[(long)h * n + at] = (float)sumA;
+          o.gpart[((long)s.H + h) * n + at] = (float)sumB;
+        }
       }
     }
   }
@@ -1152,16 +1481,12 @@ int check(const ph_delta_args& p, const char* who) {
   PH_REQUIRE(p.dtype == PH_F32 || p.dtype == PH_BF16, "%s: dtype must be F32 or BF16", who);
   PH_REQUIRE(p.K >= 1 && p.K <= kMaxDim && p.V >= 1 && p.V <= kMaxDim, "%s: heads of K = %zu, V = %zu (at most 128)", who, p.K, p.V);
   PH_REQUIRE(p.Hk >= 1 && p.H >= p.Hk && p.H % p.Hk == 0 && p.H <= (1u << 16), "%s: %zu heads on %zu key heads", who, p.H, p.Hk);
-  PH_REQUIRE(p.T <= (1u << 30) && p.B <= (1u << 24) && p.T * p.B <= (1ull << 40), "%s: T = %zu, B = %zu out of range", who, p.T, p.B);
+  PH_REQUIRE(p.T <= (1u << 30) && p.B <= (1u << 24) && p.B * p.H < (1ull << 30), "%s: T = %zu, B = %zu, H = %zu out of range",
+             who, p.T, p.B, p.H);
   PH_REQUIRE(p.scale == p.scale, "%s: scale is not a number", who);
   if (p.T == 0 || p.B == 0) return PH_OK;
   PH_REQUIRE(p.q && p.k && p.v && p.a && p.b && p.A, "%s: q, k, v, a, b or A missing", who);
   return PH_OK;
-}
-
-bool rows_aligned(int dtype, const void* p, size_t width, long t, long b, long h) {
-  const int v = dtype == PH_BF16 ? 8 : 4;
-  return ((uintptr_t)p % 16) == 0 && width % v == 0 && t % v == 0 && b % v == 0 && h % v == 0;
 }
 
 Args args_of(const ph_delta_args& p) {
@@ -1173,8 +1498,6 @@ Args args_of(const ph_delta_args& p) {
   a.v_t = p.v_t; a.v_b = p.v_b; a.v_h = p.v_h; a.a_t = p.a_t; a.a_b = p.a_b; a.b_t = p.b_t; a.b_b = p.b_b;
   a.A = p.A; a.dt_bias = p.dt_bias; a.done = p.done; a.first = p.first; a.h0 = p.h0;
   a.scale = p.scale;
-  a.vec = rows_aligned(p.dtype, p.q, p.K, p.q_t, p.q_b, p.q_h) && rows_aligned(p.dtype, p.k, p.K, p.k_t, p.k_b, p.k_h) &&
-          rows_aligned(p.dtype, p.v, p.V, p.v_t, p.v_b, p.v_h);
   return a;
 }
 
@@ -1184,28 +1507,42 @@ int padded(const Args& a) {
 }
 unsigned blocks_of(long n) { return (unsigned)(n < kMaxBlocks ? n : kMaxBlocks); }
 
-template <bool BF> int fwd_t(const Args& a, hipStream_t st) {
-  const unsigned n = blocks_of(a.units);
+// Calls f with the padded size as a constant.
+template <typename F> void by_size(const Args& a, F f) {
   switch (padded(a)) {
-    case 32: k_delta_fwd<BF, 32><<<n, 128, 0, st>>>(a); break;
-    case 64: k_delta_fwd<BF, 64><<<n, 256, 0, st>>>(a); break;
-    default: k_delta_fwd<BF, 128><<<n, 512, 0, st>>>(a);
+    case 32: f(std::integral_constant<int, 32>()); break;
+    case 64: f(std::integral_constant<int, 64>()); break;
+    default: f(std::integral_constant<int, 128>());
   }
+}
+
+template <bool BF> int fwd_t(const Args& a, hipStream_t st) {
+  by_size(a, [&](auto p) {
+    constexpr int P = decltype(p)::value;
+    if (a.segs > 1) {
+      k_delta_fwd<BF, P, true><<<blocks_of(a.units * (a.segs - 1) * a.parts), 4 * P, 0, st>>>(a);
+      k_delta_join<BF, P, false><<<blocks_of(a.units), 4 * P, 0, st>>>(a, GradArgs{});
+    }
+    k_delta_fwd<BF, P, false><<<blocks_of(a.units * a.segs), 4 * P, 0, st>>>(a);
+  });
   PH_LAUNCH_CHECK();
   return PH_OK;
 }
 
 template <bool BF> int bwd_t(const Args& a, const GradArgs& o, float* dA, float* dbias, hipStream_t st) {
   using T = typename Elem<BF>::type;
-  const unsigned n = blocks_of(a.units);
-  switch (padded(a)) {
-    case 32: k_delta_bwd<BF, 32><<<n, 128, 0, st>>>(a, o); break;
-    case 64: k_delta_bwd<BF, 64><<<n, 256, 0, st>>>(a, o); break;
-    default: k_delta_bwd<BF, 128><<<n, 512, 0, st>>>(a, o);
-  }
+  by_size(a, [&](auto p) {
+    constexpr int P = decltype(p)::value;
+    if (a.segs > 1) {
+      k_delta_fwd<BF, P, true><<<blocks_of(a.units * (a.segs - 1)), 4 * P, 0, st>>>(a);
+      k_delta_bwd<BF, P, true><<<blocks_of(a.units * (a.segs - 1)), 4 * P, 0, st>>>(a, o);
+      k_delta_join<BF, P, true><<<blocks_of(a.units), 4 * P, 0, st>>>(a, o);
+    }
+    k_delta_bwd<BF, P, false><<<blocks_of(a.units * a.segs), 4 * P, 0, st>>>(a, o);
+  });
   PH_LAUNCH_CHECK();
   if (o.gpart) {
-    k_delta_fold_gates<<<2 * a.H, 256, 0, st>>>(o.gpart, a.B, a.H, dA, dbias);
+    k_delta_fold_gates<<<2 * a.H, 256, 0, st>>>(o.gpart, a.segs * a.B, a.H, dA, dbias);
     PH_LAUNCH_CHECK();
   }
   if (o.qpart) {
@@ -1245,6 +1582,18 @@ template <typename T> int step_t(const Args& a, float* h, hipStream_t st) {
   return a.V <= 16 ? step_rows<T, 1, 16>(a, h, st) : step_rows<T, 1, 64>(a, h, st);
 }
 
+// Segments of time, and where their states are: `states` buffers of [segs][units] states, Phi and the cuts.
+void set_segments(Args& a, bool grad, int dtype) {
+  const long c = dtype == PH_BF16 ? Elem<true>::CH : Elem<false>::CH, chunks = (a.T + c - 1) / c;
+  a.segs = (int)delta_segments(chunks, a.units, padded(a), grad);
+  a.seg_chunks = (chunks + a.segs - 1) / a.segs;
+  a.segs = (int)((chunks + a.seg_chunks - 1) / a.seg_chunks);
+  a.local_from = grad ? 1 : 0;
+  a.parts = grad ? 1 : 2;
+}
+long state_floats(const Args& a) { return a.segs > 1 ? a.segs * a.units * up16(a.K) * up16(a.V) : 0; }
+long phi_floats(const Args& a) { return a.segs > 1 ? a.segs * a.units * up16(a.K) * up16(a.K) : 0; }
+
 long chunk_steps(int dtype) { return dtype == PH_BF16 ? Elem<true>::CH : Elem<false>::CH; }
 
 }  // namespace
@@ -1255,7 +1604,7 @@ using namespace ph;
 extern "C" size_t ph_delta_keep_floats(const ph_delta_args* p) {
   if (!p) return 0;
   const size_t c = (size_t)chunk_steps(p->dtype);
-  return (p->T + c - 1) / c * p->B * p->H * p->K * p->V;
+  return (p->T + c - 1) / c * p->B * p->H * up16((int)p->K) * up16((int)p->V);
 }
 
 extern "C" int ph_delta_scan(const ph_delta_args* p, void* y, long y_t, long y_b, long y_h, float* h_out, float* keep,
@@ -1268,6 +1617,16 @@ extern "C" int ph_delta_scan(const ph_delta_args* p, void* y, long y_t, long y_b
   PH_REQUIRE(y != p->q && y != p->k && y != p->v, "delta_scan: y may not be q, k or v");
   Args a = args_of(*p);
   a.y = y; a.y_t = y_t; a.y_b = y_b; a.y_h = y_h; a.h_out = h_out; a.keep = keep;
+  set_segments(a, false, p->dtype);
+  if (a.segs > 1) {
+    const long ns = state_floats(a), nf = phi_floats(a);
+    float* ws = (float*)scratch(kSlotDelta, (size_t)(2 * ns + nf + a.segs * a.units) * 4);
+    if (!ws) return PH_ERR_NOMEM;
+    a.start = ws;
+    a.psi = ws + ns;
+    a.phi = ws + 2 * ns;
+    a.cut = (int*)(ws + 2 * ns + nf);
+  }
   return p->dtype == PH_BF16 ? fwd_t<true>(a, as_stream(stream)) : fwd_t<false>(a, as_stream(stream));
 }
 
@@ -1286,7 +1645,6 @@ extern "C" int ph_delta_scan_grad(const ph_delta_args* p, const float* keep, con
   for (const void* out : {(const void*)g->dq, (const void*)g->dk, (const void*)g->dv})
     PH_REQUIRE(!out || (out != p->q && out != p->k && out != p->v && out != dy), "delta_scan_grad: a gradient may not be an input");
   Args a = args_of(*p);
-  a.vec = a.vec && rows_aligned(p->dtype, dy, p->V, dy_t, dy_b, dy_h);
   GradArgs o{};
   o.dy = dy; o.dy_t = dy_t; o.dy_b = dy_b; o.dy_h = dy_h; o.keep = keep; o.dh = dh;
   o.dq = g->dq; o.dq_t = g->dq_t; o.dq_b = g->dq_b; o.dq_h = g->dq_h;
@@ -1296,10 +1654,17 @@ extern "C" int ph_delta_scan_grad(const ph_delta_args* p, const float* keep, con
   o.db = g->db; o.db_t = g->db_t; o.db_b = g->db_b;
   o.dh0 = g->dh0;
   const bool shared = p->Hk != p->H && (g->dq || g->dk), gates = g->dA || g->ddt_bias;
-  const size_t nq = shared ? p->T * p->B * p->H * p->K : 0, ng = gates ? 2 * p->H * p->B : 0;
-  if (nq + ng) {
-    float* ws = (float*)scratch(kSlotDelta, (2 * nq + ng) * 4);
+  set_segments(a, true, p->dtype);
+  const size_t nq = shared ? p->T * p->B * p->H * p->K : 0, ng = gates ? 2 * p->H * p->B * a.segs : 0;
+  const size_t ns = state_floats(a), nf = phi_floats(a), nc = a.segs > 1 ? a.segs * a.units : 0;
+  if (nq + ng + ns) {
+    float* ws = (float*)scratch(kSlotDelta, (2 * ns + nf + 2 * nq + ng + nc) * 4);
     if (!ws) return PH_ERR_NOMEM;
+    o.dend = ws;
+    o.xi = ws + ns;
+    a.phi = ws + 2 * ns;
+    ws += 2 * ns + nf;
+    a.cut = (int*)(ws + 2 * nq + ng);
     o.qpart = nq ? ws : nullptr;
     o.kpart = nq ? ws + nq : nullptr;
     o.gpart = ng ? ws + 2 * nq : nullptr;

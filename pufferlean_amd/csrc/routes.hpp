@@ -201,4 +201,12 @@ inline long ssm_chunk(long T, long B, long G, long per, int N, bool grad) {
   return ((T + want - 1) / want + kSsmSteps - 1) / kSsmSteps * kSsmSteps;
 }
 
+// ---- Gated delta rule ---------------------------------------------------------------------------------------
+// Segments of time of `chunks` chunks, of `units` sequences' heads with states padded to P x P.
+inline long delta_segments(long chunks, long units, int P, bool grad) {
+  const long most = (chunks + 3) / 4, want = (P <= 32 ? 2048 : P <= 64 ? 768 : 256) / units;
+  const long n = want < most ? want : most;
+  return n < 2 || chunks < 8 ? 1 : n;
+}
+
 }  // namespace ph

@@ -111,6 +111,16 @@ def test_sizes(gpu, T, B, Hk, H, K, V, dt):
 
 
 @pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("p_done", [0.0, 0.004, 0.05])
+@pytest.mark.parametrize("T,B,Hk,H,K,V", [(300, 2, 1, 1, 16, 24), (530, 1, 1, 2, 64, 33), (515, 1, 1, 1, 100, 128), (767, 1, 1, 1, 33, 64)])
+def test_long_sequences(gpu, T, B, Hk, H, K, V, p_done, dt):
+    """In segments of time, with and without an episode's start in each."""
+    p = inputs(T, B, Hk, H, K, V, dt)
+    p["A"] *= 0.05  # states that outlive a segment
+    check(p, flags(3, p_done, T, B), flags(4, 0.5, B), cu(5, B, H, K, V, scale=0.3))
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
 @pytest.mark.parametrize("layout", ["odd", "batch", "packed"])
 def test_layouts(gpu, layout, dt):
     p = inputs(70, 3, 2, 4, 32, 48, dt, layout=layout)
@@ -154,14 +164,15 @@ def test_hard_gates(gpu, dt):
 @pytest.mark.parametrize("dt", [F32, BF])
 @pytest.mark.parametrize("name", ["q", "k", "v", "a", "b", "dy"])
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
-def test_an_episode_does_not_see_the_one_before(gpu, name, value, dt):
-    """Non-finite values in steps 0..9 and 45..49; the episodes of steps 10..44 and 50..69 give what they give alone."""
-    T, B, H, K, V = 70, 2, 2, 16, 24
+@pytest.mark.parametrize("T", [70, 410])
+def test_an_episode_does_not_see_the_one_before(gpu, T, name, value, dt):
+    """Non-finite values in steps 0..9 and 45..49; the episodes of steps 10..44 and from 50 on give what they give alone."""
+    B, H, K, V = 2, 2, 16, 24
     p = {n: t.clone() for n, t in inputs(T, B, 1, H, K, V, dt).items()}
     dy = cu(50, T, B, H, V, dtype=dt)
     done = torch.zeros(T, B, device="cuda")
     done[[9, 44, 49]] = 1
-    clean = [slice(10, 45), slice(50, 70)]
+    clean = [slice(10, 45), slice(50, T)]
     x = dict(p, dy=dy)[name]
     x[4, :, ..., 0] = value
     x[47] = value
@@ -220,8 +231,9 @@ def test_steps_follow_the_sequence(gpu, Hk, H, K, V, dt, layout):
     close(h, hr, BAR[dt], "h")
 
 
-def test_state_in_place_and_rows_left_alone(gpu):
-    T, B, H, K, V = 40, 2, 2, 16, 24
+@pytest.mark.parametrize("T", [40, 600])
+def test_state_in_place_and_rows_left_alone(gpu, T):
+    B, H, K, V = 2, 2, 16, 24
     p = inputs(T, B, 1, H, K, V, BF)
     args = [p[n] for n in "qkvabA"]
     h0, h = cu(5, B, H, K, V), torch.empty(B, H, K, V, device="cuda")
@@ -233,9 +245,10 @@ def test_state_in_place_and_rows_left_alone(gpu):
     assert (wide[T:] == 7).all() and (wide[..., :3] == 7).all() and (wide[..., V + 3:] == 7).all()
 
 
-def test_whole_and_in_parts(gpu):
+@pytest.mark.parametrize("T", [90, 500])
+def test_whole_and_in_parts(gpu, T):
     """A sequence in two calls, the state and its gradient handed over, is the sequence in one."""
-    T, B, H, K, V = 90, 2, 2, 32, 24
+    B, H, K, V = 2, 2, 32, 24
     p = inputs(T, B, 2, H, K, V, F32)
     done, dy = flags(3, 0.05, T, B), cu(6, T, B, H, V)
     args = lambda s: [p[n][s] for n in "qkvab"] + [p["A"]]
@@ -275,9 +288,10 @@ def test_gradient_against_differences(gpu):
 
 
 @pytest.mark.parametrize("dt", [F32, BF])
-def test_same_call_same_bits(gpu, dt):
-    p = inputs(100, 9, 2, 4, 32, 32, dt)
-    dy, done = cu(6, 100, 9, 4, 32, dtype=dt), flags(3, 0.1, 100, 9)
+@pytest.mark.parametrize("T", [100, 700])
+def test_same_call_same_bits(gpu, T, dt):
+    p = inputs(T, 9, 2, 4, 32, 32, dt)
+    dy, done = cu(6, T, 9, 4, 32, dtype=dt), flags(3, 0.1, T, 9)
     args = [p[n] for n in "qkvabA"]
     runs = []
     for _ in range(2):
@@ -298,9 +312,10 @@ def test_no_sequences(gpu):
 
 
 @pytest.mark.parametrize("dt", [F32, BF])
-def test_captured(gpu, dt):
+@pytest.mark.parametrize("T", [50, 400])
+def test_captured(gpu, T, dt):
     """Forward, gradient and a step in one graph on a stream of its own, replayed between eager work."""
-    T, B, Hk, H, K, V = 50, 4, 1, 2, 32, 32
+    B, Hk, H, K, V = 4, 1, 2, 32, 32
     p = inputs(T, B, Hk, H, K, V, dt)
     dy, h = cu(6, T, B, H, V, dtype=dt), cu(5, B, H, K, V)
     args = [p[n] for n in "qkvabA"]
