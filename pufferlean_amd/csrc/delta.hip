@@ -132,7 +132,9 @@ __device__ __forceinline__ void renew(int& tid, int& l) {
 template <bool BF> struct Elem { using type = uint16_t; using unit = s4; static constexpr int CH = 32, pad = 8, V = 8; };
 template <> struct Elem<false> { using type = float; using unit = f4; static constexpr int CH = 16, pad = 4, V = 4; };
 
-// acc += a b over N units. bf16 units go in pairs where there are two.
+// acc += a b over N units. bf16 units go in pairs where there are two. No accumulator goes straight from an instruction over
+// 32 to one over 16 or back: of two such instructions in a row the second has read values that the first had not written yet. Their
+// results are added instead.
 template <int N> __device__ __forceinline__ f4 dot(const s4* a, const s4* b, f4 acc) {
 #pragma unroll
   for (int i = 0; i + 1 < N; i += 2) {
@@ -261,6 +263,17 @@ __device__ __forceinline__ u4 load_row(int tid, const T* p, int rows, int W) {
   }
   return r;
 }
+// The first n of 16 bytes' elements from LDS to a row.
+template <bool BF, typename T = typename Elem<BF>::type> __device__ __forceinline__ void store_row(T* p, const T* from, int n) {
+  constexpr int V = Elem<BF>::V;
+  if (n >= V) {
+    const u4 r = *reinterpret_cast<const u4*>(from);
+    __builtin_memcpy(p, &r, 16);
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < n; i++) p[i] = from[i];
+  }
+}
 template <bool BF, int P, typename T> __device__ __forceinline__ const T* thread_row(int tid, const T* base, long stride, long t0) {
   constexpr int V = Elem<BF>::V;
   return base + (t0 + tid / (P / V)) * stride + tid % (P / V) * V;
@@ -331,6 +344,9 @@ __device__ __forceinline__ double lane_f64(double v, int lane) {
   const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+__device__ __forceinline__ float lane_f32(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
 // Fills r for rows lo..hi-1 from the gates in a wavefront's lanes (all of it calls), but for the norms.
 template <int CH> __device__ __forceinline__ void fill_rows(int tid, Rows<CH>& r, const Gate& g, float A, int lo, int hi) {
   const int i = tid & 63;
@@ -364,19 +380,54 @@ template <int CH> __device__ __forceinline__ void fill_rows(int tid, Rows<CH>& r
   }
 }
 __device__ __forceinline__ f4 rows4(int tid, const float* r, int at) { return *reinterpret_cast<const f4*>(r + at + 4 * ((tid & 63) >> 4)); }
-// c x where c is not zero: what a start hides may be anything
-__device__ __forceinline__ f4 sel_mul(f4 c, f4 x) {
-#pragma unroll
-  for (int i = 0; i < 4; i++) x[i] = c[i] == 0.f ? 0.f : c[i] * x[i];
-  return x;
+
+// Small matrices of a chunk are kept transposed, as pairs: a tile's lane holds four rows of a column, one access of them.
+template <bool BF, int LD> struct alignas(16) Mat {
+  using T = typename Elem<BF>::type;
+  T hi[LD], lo[BF ? LD : 1];  // LD: elements
+};
+template <bool BF, int LD, int N> __device__ __forceinline__ void put_mat(int tid, Mat<BF, N>& m, int row, int col, f4 v) {
+  const int l = tid & 63, o = (row + (l & 15)) * LD + col + 4 * (l >> 4);
+  Pair<BF> p;
+  p.set(v);
+  *reinterpret_cast<typename Elem<BF>::unit*>(m.hi + o) = p.hi;
+  if constexpr (BF) *reinterpret_cast<s4*>(m.lo + o) = p.lo;
+}
+// The left operand of the matrix itself (tile's row `row`, column `col` of the stored, transposed one) and of its transpose.
+template <bool BF, int LD, int N> __device__ __forceinline__ Pair<BF> mat_col(int tid, const Mat<BF, N>& m, int row, int col) {
+  Pair<BF> p;
+  p.hi = col_unit<LD>(tid, m.hi, row, col);
+  if constexpr (BF) p.lo = col_unit<LD>(tid, m.lo, row, col);
+  return p;
+}
+template <bool BF, int LD, int N> __device__ __forceinline__ Pair<BF> mat_row(int tid, const Mat<BF, N>& m, int row, int col) {
+  Pair<BF> p;
+  p.hi = row_unit<LD>(tid, m.hi, row, col);
+  if constexpr (BF) p.lo = row_unit<LD>(tid, m.lo, row, col);
+  return p;
+}
+// The four values that put_mat of the same place took.
+template <bool BF, int LD, int N> __device__ __forceinline__ f4 mat_values(int tid, const Mat<BF, N>& m, int row, int col) {
+  const Pair<BF> p = mat_row<BF, LD>(tid, m, row, col);
+  if constexpr (BF) return widen(p.hi) + widen(p.lo);
+  else return p.hi;
 }
 
-// M (and P, transposed by the reader) of the chunk: tiles on and below the diagonal, dealt out over the wavefronts.
+// A chunk's M, P and T = (I + M)^-1. Of T the diagonal blocks; of M these also as they are, for the substitution.
+template <bool BF, bool WITH_P> struct Scores {
+  static constexpr int CH = Elem<BF>::CH, UD = CH + 4, TD = 20;
+  Mat<BF, CH * UD> M;
+  Mat<BF, WITH_P ? CH * UD : 1> P;
+  Mat<BF, CH * TD> Tinv;
+};
+
+// M (and P) of the chunk: tiles on and below the diagonal, dealt out over the wavefronts.
 template <bool BF, int P, int LD, bool WITH_P>
 __device__ __forceinline__ void score_tiles(int tid, const Rows<Elem<BF>::CH>& r, const typename Elem<BF>::type* Qs,
-                                            const typename Elem<BF>::type* Ks, float* Mm, float* Pm, float scale) {
-  constexpr int CH = Elem<BF>::CH, NB = CH / 16, NT = P / 16, CP = CH + 4, TILES = NB * (NB + 1) / 2;
-  const int l = tid & 63, w = tid >> 6;
+                                            const typename Elem<BF>::type* Ks, Mat<BF, Scores<BF, WITH_P>::CH * Scores<BF, WITH_P>::UD>& M,
+                                            Mat<BF, WITH_P ? Scores<BF, WITH_P>::CH * Scores<BF, WITH_P>::UD : 1>& Pm, float* diag, float scale) {
+  constexpr int CH = Elem<BF>::CH, NB = CH / 16, NT = P / 16, UD = CH + 4, TILES = NB * (NB + 1) / 2;
+  const int l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   for (int id = w; id < (WITH_P ? 2 : 1) * TILES; id += NT) {
     const bool isP = WITH_P && id >= TILES;
     const int tile = isP ? id - TILES : id, bi = tile == 0 ? 0 : 1, bj = tile == 2 ? 1 : 0;  // (0,0) (1,0) (1,1)
@@ -387,24 +438,34 @@ __device__ __forceinline__ void score_tiles(int tid, const Rows<Elem<BF>::CH>& r
       y[m] = row_unit<LD>(tid, Ks, 16 * bj, 16 * m);
     }
     f4 acc = dot<NT>(x, y, f4{0.f, 0.f, 0.f, 0.f});
-    const int j = 16 * bj + (l & 15);
-    const double Gj = r.G[j];
-    const int segj = r.seg[j];
-    const float rkj = r.rk[j];
+    const int j = l & 15, i0 = 4 * (l >> 4);
+    const double Gj = r.G[16 * bj + j];
+    const int segj = r.seg[16 * bj + j];
+    const float rkj = r.rk[16 * bj + j];
+    const f4 ci = isP ? scale * rows4(tid, r.rq, 16 * bi) : rows4(tid, r.be, 16 * bi) * rows4(tid, r.rk, 16 * bi);
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      const int i = 16 * bi + 4 * (l >> 4) + k;
-      const bool on = segj == r.seg[i] && (isP ? j <= i : j < i);
-      const float c = ex2((float)(r.G[i] - Gj)) * rkj * (isP ? scale * r.rq[i] : r.be[i] * r.rk[i]);
-      (isP ? Pm : Mm)[i * CP + j] = on ? c * acc[k] : 0.f;
+      const int i = 16 * bi + i0 + k;
+      const bool on = segj == r.seg[i] && (bi != bj || (isP ? j <= i0 + k : j < i0 + k));
+      acc[k] = on ? ex2((float)(r.G[i] - Gj)) * rkj * ci[k] * acc[k] : 0.f;
+    }
+    if constexpr (WITH_P) {
+      if (isP) {
+        put_mat<BF, UD>(tid, Pm, 16 * bj, 16 * bi, acc);
+        continue;
+      }
+    }
+    put_mat<BF, UD>(tid, M, 16 * bj, 16 * bi, acc);
+    if (bi == bj) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) diag[(16 * bi + i0 + k) * 16 + j] = acc[k];
     }
   }
 }
 
-// The diagonal blocks of (I + M)^-1 into Tm, one column per lane of wavefront 0.
-template <int CH> __device__ __forceinline__ void invert_blocks(int tid, const float* Mm, float* Tm) {
-  constexpr int CP = CH + 4;
-  const int l = tid;
+// The diagonal blocks of (I + M)^-1, one column per lane of a wavefront's first CH.
+template <bool BF, int CH, int N> __device__ __forceinline__ void invert_blocks(int tid, const float* diag, Mat<BF, N>& Tinv) {
+  const int l = tid & 63;
   if (l >= CH) return;
   const int o = l & ~15, c = l & 15;
   float x[16];
@@ -413,85 +474,60 @@ template <int CH> __device__ __forceinline__ void invert_blocks(int tid, const f
     float s = i == c ? 1.f : 0.f;
 #pragma unroll
     for (int j4 = 0; j4 < i; j4 += 4) {
-      const f4 m = *reinterpret_cast<const f4*>(Mm + (o + i) * CP + o + j4);
+      const f4 m = *reinterpret_cast<const f4*>(diag + (o + i) * 16 + j4);
 #pragma unroll
       for (int k = 0; k < 4; k++)
         if (j4 + k < i) s = fmaf(-m[k], x[j4 + k], s);
     }
     x[i] = s;
-    Tm[(o + i) * CP + o + c] = s;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    Pair<BF> p;
+    p.set(f4{x[i], x[i + 1], x[i + 2], x[i + 3]});
+    *reinterpret_cast<typename Elem<BF>::unit*>(Tinv.hi + l * 20 + i) = p.hi;
+    if constexpr (BF) *reinterpret_cast<s4*>(Tinv.lo + l * 20 + i) = p.lo;
   }
 }
 
 // U = T Y by blocks, T's blocks below the diagonal through M.
-template <bool BF> __device__ __forceinline__ void solve(int tid, const float* Tm, const float* Mm, const f4* Y, f4* U) {
-  constexpr int CH = Elem<BF>::CH, NB = CH / 16, CP = CH + 4;
+template <bool BF, int NM, int NI> __device__ __forceinline__ void solve(int tid, const Mat<BF, NI>& Tinv, const Mat<BF, NM>& M, const f4* Y, f4* U) {
+  constexpr int CH = Elem<BF>::CH, NB = CH / 16, UD = CH + 4;
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
-  Pair<BF> t, y, u;
-  t.set(row_unit<CP>(tid, Tm, 0, 0));
+  Pair<BF> t = mat_col<BF, 20>(tid, Tinv, 0, 0), y;
   y.set(Y[0]);
   U[0] = dot3<BF, 1>(&t, &y, zero);
   if constexpr (NB == 2) {
-    u.set(-U[0]);
-    t.set(row_unit<CP>(tid, Mm, 16, 0));
-    y.set(dot3<BF, 1>(&t, &u, Y[1]));
-    t.set(row_unit<CP>(tid, Tm, 16, 16));
+    y.set(-U[0]);
+    t = mat_col<BF, UD>(tid, M, 0, 16);
+    y.set(dot3<BF, 1>(&t, &y, Y[1]));
+    t = mat_col<BF, 20>(tid, Tinv, 16, 0);
     U[1] = dot3<BF, 1>(&t, &y, zero);
   }
 }
 // dY = T^T dU
-template <bool BF> __device__ __forceinline__ void solve_t(int tid, const float* Tm, const float* Mm, const f4* dU, f4* dY) {
-  constexpr int CH = Elem<BF>::CH, NB = CH / 16, CP = CH + 4;
+template <bool BF, int NM, int NI> __device__ __forceinline__ void solve_t(int tid, const Mat<BF, NI>& Tinv, const Mat<BF, NM>& M, const f4* dU, f4* dY) {
+  constexpr int CH = Elem<BF>::CH, NB = CH / 16, UD = CH + 4;
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
   Pair<BF> t, y;
   f4 top = dU[0];
   if constexpr (NB == 2) {
     y.set(dU[1]);
-    t.set(col_unit<CP>(tid, Tm, 16, 16));
+    t = mat_row<BF, 20>(tid, Tinv, 16, 0);
     dY[1] = dot3<BF, 1>(&t, &y, zero);
     y.set(-dY[1]);
-    t.set(col_unit<CP>(tid, Mm, 16, 0));
-    top = dot3<BF, 1>(&t, &y, top);
+    t = mat_row<BF, UD>(tid, M, 0, 16);
+    top += dot3<BF, 1>(&t, &y, zero);
   }
   y.set(top);
-  t.set(col_unit<CP>(tid, Tm, 0, 0));
+  t = mat_row<BF, 20>(tid, Tinv, 0, 0);
   dY[0] = dot3<BF, 1>(&t, &y, zero);
 }
 
 // States in memory: [K][V] as the caller holds them, or [up(K)][up(V)], both rounded up to whole tiles, as the library does.
 __host__ __device__ __forceinline__ int up16(int n) { return (n + 15) & ~15; }
-// Tile m of a state's column block w: rows 16 m + 4 (l / 16) + 0..3, column 16 w + l % 16; zero outside. Addresses are clamped
-// and not skipped: a load that a branch guards is waited for before the next one.
-__device__ __forceinline__ f4 state_tile(int tid, const float* s, int K, int V, int m, int w) {
-  const int l = tid & 63, r = 16 * m + 4 * (l >> 4), c = 16 * w + (l & 15);
-  const float* p = s + (c < V ? c : 0);
-  f4 x;
-#pragma unroll
-  for (int i = 0; i < 4; i++) x[i] = p[(r + i < K ? r + i : 0) * V];
-#pragma unroll
-  for (int i = 0; i < 4; i++) x[i] = r + i < K && c < V ? x[i] : 0.f;
-  return x;
-}
-__device__ __forceinline__ void put_state_tile(int tid, float* s, int K, int V, int m, int w, f4 x) {
-  const int l = tid & 63, r = 16 * m + 4 * (l >> 4), c = 16 * w + (l & 15);
-  if (c < V) {
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (r + i < K) s[(r + i) * V + c] = x[i];
-  }
-}
-// The transposed state's tile m of block w: columns of V 16 m + 4 (l / 16) + 0..3, row 16 w + l % 16.
-__device__ __forceinline__ f4 state_tile_t(int tid, const float* s, int K, int V, int m, int w) {
-  const int l = tid & 63, c = 16 * m + 4 * (l >> 4), r = 16 * w + (l & 15);
-  const float* p = s + (r < K ? r : 0) * V;
-  f4 x;
-#pragma unroll
-  for (int i = 0; i < 4; i++) x[i] = p[c + i < V ? c + i : 0];
-#pragma unroll
-  for (int i = 0; i < 4; i++) x[i] = r < K && c + i < V ? x[i] : 0.f;
-  return x;
-}
-// The same of the library's own states: whole tiles, of which those past the last are not there.
+// Tile m of a library's state's column block w: rows 16 m + 4 (l / 16) + 0..3, column 16 w + l % 16; the transposed state's:
+// columns of V 16 m + 4 (l / 16) + 0..3, row 16 w + l % 16. Whole tiles, of which those past the last are not there.
 __device__ __forceinline__ f4 own_tile(int tid, const float* s, int Ku, int Vu, int m, int w) {
   const int l = tid & 63;
   f4 x = {0.f, 0.f, 0.f, 0.f};
@@ -517,6 +553,38 @@ __device__ __forceinline__ void put_own_tile(int tid, float* s, int Ku, int Vu, 
   }
 }
 
+// The same of a caller's state of any size, zero outside. Addresses are clamped
+// and not skipped: a load that a branch guards is waited for before the next one.
+__device__ __forceinline__ f4 state_tile(int tid, const float* s, int K, int V, int m, int w) {
+  if (((K | V) & 15) == 0) return own_tile(tid, s, K, V, m, w);
+  const int l = tid & 63, r = 16 * m + 4 * (l >> 4), c = 16 * w + (l & 15);
+  const float* p = s + (c < V ? c : 0);
+  f4 x;
+#pragma unroll
+  for (int i = 0; i < 4; i++) x[i] = p[(r + i < K ? r + i : 0) * V];
+#pragma unroll
+  for (int i = 0; i < 4; i++) x[i] = r + i < K && c < V ? x[i] : 0.f;
+  return x;
+}
+__device__ __forceinline__ void put_state_tile(int tid, float* s, int K, int V, int m, int w, f4 x) {
+  if (((K | V) & 15) == 0) return put_own_tile(tid, s, K, V, m, w, x);
+  const int l = tid & 63, r = 16 * m + 4 * (l >> 4), c = 16 * w + (l & 15);
+  if (c < V) {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (r + i < K) s[(r + i) * V + c] = x[i];
+  }
+}
+__device__ __forceinline__ f4 state_tile_t(int tid, const float* s, int K, int V, int m, int w) {
+  const int l = tid & 63, c = 16 * m + 4 * (l >> 4), r = 16 * w + (l & 15);
+  const float* p = s + (r < K ? r : 0) * V;
+  f4 x;
+#pragma unroll
+  for (int i = 0; i < 4; i++) x[i] = p[c + i < V ? c + i : 0];
+#pragma unroll
+  for (int i = 0; i < 4; i++) x[i] = r < K && c + i < V ? x[i] : 0.f;
+  return x;
+}
 template <bool BF, int P, typename T = typename Elem<BF>::type>
 __device__ __forceinline__ void put_row(int tid, T* tile, u4 r, int lo, int hi) {
   constexpr int V = Elem<BF>::V, LD = P + Elem<BF>::pad;
@@ -528,8 +596,11 @@ __device__ __forceinline__ void put_row(int tid, T* tile, u4 r, int lo, int hi) 
 template <bool BF, int P> __device__ __forceinline__ void put_norm(int tid, float* out, u4 r, int lo, int hi) {
   constexpr int L = P / Elem<BF>::V;  // lanes of a row
   float s = square_sum<BF>(r);
-#pragma unroll
-  for (int d = 1; d < L; d *= 2) s += __shfl_xor(s, d);
+  s += dpp_mov<0xB1>(s);
+  s += dpp_mov<0x4E>(s);
+  if constexpr (L >= 8) s += dpp_mov<0x141>(s);
+  if constexpr (L >= 16) s += dpp_mov<0x140>(s);
+  if constexpr (L >= 32) s += __shfl_xor(s, 16);
   const int row = tid / L;
   if (tid % L == 0) out[row] = row >= lo && row < hi ? 1.f / sqrtf(s + kEps) : 0.f;
 }
@@ -544,9 +615,10 @@ template <bool BF, int P> constexpr int bwd_waves() { return P == 128 ? 2 : 3; }
 template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (fwd_waves<BF, P>())) k_delta_fwd(const Args s) {
   using T = typename Elem<BF>::type;
   using unit = typename Elem<BF>::unit;
-  constexpr int CH = Elem<BF>::CH, NB = CH / 16, NT = P / 16, LD = P + Elem<BF>::pad, CP = CH + 4;
+  constexpr int CH = Elem<BF>::CH, NB = CH / 16, NT = P / 16, LD = P + Elem<BF>::pad, UD = CH + 4;
   __shared__ __attribute__((aligned(16))) T Qs[LOCAL ? 1 : CH * LD], Ks[CH * LD], Vs[CH * LD];
-  __shared__ __attribute__((aligned(16))) float Mm[CH * CP], Tm[CH * CP], Pm[LOCAL ? 1 : CH * CP];
+  __shared__ __attribute__((aligned(16))) Scores<BF, !LOCAL> X;
+  __shared__ __attribute__((aligned(16))) float diag[CH * 16];
   __shared__ Rows<CH> Rs[2];
   int tid = threadIdx.x, l = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -605,7 +677,14 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
     }
     __syncthreads();  // the item before has been read
     if (w == NT - 1) fill_rows<CH>(tid, Rs[0], g, A, 0, rows);
-    int cur = 0, cut = 0;
+    int cur = 0, cut = 0, y_lo = 0, y_hi = 0;
+    long y_at = first;
+    auto put_y = [&](long at, int lo, int hi) {  // a thread stores the 16 bytes that it stages next
+      const Args a = again<Args>(0);
+      const int row = tid / (P / Elem<BF>::V), c = tid % (P / Elem<BF>::V) * Elem<BF>::V;
+      if (row >= lo && row < hi)
+        store_row<BF>((T*)a.y + bt * a.y_b + h * a.y_h + (at + row) * a.y_t + c, Vs + row * LD + c, a.V - c);
+    };
     for (long t0 = first; t0 < last; t0 += CH) {
       Rows<CH>& R = Rs[cur];
       if (!LOCAL && s.keep) {
@@ -616,6 +695,10 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
       for (int lo = 0, hi = all, once = 1; lo < all; once = 0) {
         __syncthreads();  // the rows before have been read
         renew(tid, l);
+        if (!LOCAL) {
+          put_y(y_at, y_lo, y_hi);
+          y_hi = 0;
+        }
         if (!once) {  // one episode at a time: rows and gates again
           rows = all;
           load();
@@ -634,9 +717,13 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
           rows = rows_at(t0 + CH);
           load();
         }
-        score_tiles<BF, P, LD, !LOCAL>(tid, R, Qs, Ks, Mm, Pm, s.scale);
+        if (R.starts >> lo & 1) {  // whatever the steps before left
+#pragma unroll
+          for (int m = 0; m < NT; m++) S[m] = zero;
+        }
+        score_tiles<BF, P, LD, !LOCAL>(tid, R, Qs, Ks, X.M, X.P, diag, s.scale);
         __syncthreads();
-        if (w == 0) invert_blocks<CH>(tid, Mm, Tm);
+        if (w == 0) invert_blocks<BF, CH>(tid, diag, X.Tinv);
         if (w == NT - 1 && once) fill_rows<CH>(tid, Rs[cur ^ 1], gn, A, 0, rows);
         f4 Y[NB], O[NB];
         {
@@ -650,17 +737,17 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
             for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, Ks, 16 * n, 16 * m);
             const f4 ks = dot2<BF, NT>(x, Sp, zero);
             Y[n] = rows4(tid, R.be, 16 * n) * (widen(col_unit<LD>(tid, Vs, 16 * n, 16 * w)) -
-                                          sel_mul(rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n), ks));
+                                          (rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n)) * (ks));
             if constexpr (!LOCAL) {
 #pragma unroll
               for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, Qs, 16 * n, 16 * m);
-              O[n] = sel_mul(s.scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n), dot2<BF, NT>(x, Sp, zero));
+              O[n] = (s.scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n)) * (dot2<BF, NT>(x, Sp, zero));
             }
           }
         }
         __syncthreads();
         f4 U[NB];
-        solve<BF>(tid, Tm, Mm, Y, U);
+        solve<BF>(tid, X.Tinv, X.M, Y, U);
         const int starts = R.starts, inside = starts & ~(1 << lo);
         if (inside) {
           bool bad = false;
@@ -681,35 +768,33 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
           Pair<BF> x[NB];
 #pragma unroll
           for (int n = 0; n < NB; n++) Up[n].set(U[n]);
-          x[0].set(row_unit<CP>(tid, Pm, 0, 0));
+          x[0] = mat_col<BF, UD>(tid, X.P, 0, 0);
           O[0] = dot3<BF, 1>(x, Up, O[0]);
           if constexpr (NB == 2) {
-            x[0].set(row_unit<CP>(tid, Pm, 16, 0));
-            x[1].set(row_unit<CP>(tid, Pm, 16, 16));
+            x[0] = mat_col<BF, UD>(tid, X.P, 0, 16);
+            x[1] = mat_col<BF, UD>(tid, X.P, 16, 16);
             O[1] = dot3<BF, 2>(x, Up, O[1]);
           }
-          const Args a = again<Args>(0);
-          T* yp = (T*)a.y + bt * a.y_b + h * a.y_h + t0 * a.y_t;
-          const int c = 16 * w + (l & 15);
+          // y rests where V was, until the rows are stored behind the next barrier
 #pragma unroll
           for (int n = 0; n < NB; n++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const int row = 16 * n + 4 * (l >> 4) + i;
-              if (row >= lo && row < hi && c < a.V) stf(yp + row * a.y_t + c, O[n][i]);
-            }
+            for (int i = 0; i < 4; i++) stf(Vs + (16 * n + 4 * (l >> 4) + i) * LD + 16 * w + (l & 15), O[n][i]);
         }
 #pragma unroll
-        for (int n = 0; n < NB; n++) Up[n].set(sel_mul(rows4(tid, R.dc, 16 * n) * rows4(tid, R.rk, 16 * n), U[n]));
+        for (int n = 0; n < NB; n++) Up[n].set((rows4(tid, R.dc, 16 * n) * rows4(tid, R.rk, 16 * n)) * (U[n]));
         const float c0 = R.c0;
 #pragma unroll
         for (int m = 0; m < NT; m++) {
           unit kt[NB];
 #pragma unroll
           for (int n = 0; n < NB; n++) kt[n] = col_unit<LD>(tid, Ks, 16 * n, 16 * m);
-          S[m] = dot2<BF, NB>(kt, Up, sel_mul(f4{c0, c0, c0, c0}, S[m]));
+          S[m] = dot2<BF, NB>(kt, Up, c0 * S[m]);
         }
         cut |= starts;
+        y_at = t0;
+        y_lo = lo;
+        y_hi = hi;
         lo = hi;
         hi = all;
         if (!once && lo >= all) {  // on to the next chunk's rows
@@ -725,6 +810,10 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
         gn = load_gate<T>(s, bt, h, t0 + 2 * CH, rows_at(t0 + 2 * CH), l);
       }
       cur ^= 1;
+    }
+    if (!LOCAL) {
+      __syncthreads();
+      put_y(y_at, y_lo, y_hi);
     }
     if (LOCAL) {
       const long at = seg * s.units + unit_id;
@@ -820,26 +909,26 @@ template <bool BF, int P> struct BwdLds {
     float sums[4][NT][CH];  // when U has been read: <q^, dQ^>, <k^, dK^>, the parts of S_0 and of dS_c
   };
   T dY[P * UD], Ulo[BF ? P * UD : 1], dYlo[BF ? P * UD : 1];
+  Mat<BF, CH * UD> M, Pm;  // then F and E
   union {
-    float M[CH * CP];
-    float F[CH * CP];
-  };
-  union {
-    float Pm[CH * CP];
-    float E[CH * CP];
-  };
-  union {
-    float Tm[CH * CP];
+    Mat<BF, CH * 20> Tinv;
     float W[CH * CP];  // P_ij dO_i U_j - M_ij dY_i U_j
   };
-  float ysum[NT][CH], pairs[CH / 16][CH], tot[NT];
+  union {
+    float diag[CH * 16];
+    struct {
+      float ysum[NT][CH], pairs[CH / 16][CH], tot[NT];
+    };
+  };
   Rows<CH> R[2];
 };
 template <bool BF, int P> struct BwdLocalLds {
   using T = typename Elem<BF>::type;
-  static constexpr int CH = Elem<BF>::CH, LD = P + Elem<BF>::pad, CP = CH + 4;
+  static constexpr int CH = Elem<BF>::CH, LD = P + Elem<BF>::pad, CP = CH + 4, UD = CH + 4;
   T Q[CH * LD], K[CH * LD], dO[CH * LD];
-  float M[CH * CP], Pm[CH * CP], Tm[CH * CP];
+  Mat<BF, CH * UD> M, Pm;
+  Mat<BF, CH * 20> Tinv;
+  float diag[CH * 16];
   Rows<CH> R[2];
 };
 
@@ -941,7 +1030,17 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
     }
     __syncthreads();  // the item before has been read
     if (w == NT - 1) fill_rows<CH>(tid, L.R[0], g, A, 0, rows);
-    int cur = 0;
+    int cur = 0, y_lo = 0, y_hi = 0;
+    long y_at = 0;
+    auto put_grads = [&](long at, int lo, int hi) {  // a thread stores the 16 bytes that it stages next
+      const GradArgs a = again<GradArgs>(sizeof(Args));
+      const Args sa = again<Args>(0);
+      const int row = tid / (P / Elem<BF>::V), c = tid % (P / Elem<BF>::V) * Elem<BF>::V, from = row * LD + c;
+      if (row < lo || row >= hi) return;
+      if (a.dv) store_row<BF>((T*)a.dv + bt * a.dv_b + h * a.dv_h + (at + row) * a.dv_t + c, L.dO + from, sa.V - c);
+      if (a.dq && !a.qpart) store_row<BF>((T*)a.dq + bt * a.dq_b + h * a.dq_h + (at + row) * a.dq_t + c, L.Q + from, sa.K - c);
+      if (a.dk && !a.qpart) store_row<BF>((T*)a.dk + bt * a.dk_b + h * a.dk_h + (at + row) * a.dk_t + c, L.K + from, sa.K - c);
+    };
     for (; c >= c_first; c--) {
       Rows<CH>& R = L.R[cur];
       const long t0 = c * CH;
@@ -949,6 +1048,10 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
       for (int lo = 0, hi = all, once = 1; hi > 0; once = 0) {
         __syncthreads();  // the rows before have been read
         renew(tid, l);
+        if constexpr (!LOCAL) {
+          put_grads(y_at, y_lo, y_hi);
+          y_hi = 0;
+        }
         if (!once) {  // one episode at a time: rows and gates again
           rows = all;
           load();
@@ -972,9 +1075,10 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
           rows = rows_at(c - 1);
           load();
         }
-        score_tiles<BF, P, LD, true>(tid, R, L.Q, L.K, L.M, L.Pm, s.scale);
+        const bool fresh = R.starts >> lo & 1;  // S_0 may be anything
+        score_tiles<BF, P, LD, true>(tid, R, L.Q, L.K, L.M, L.Pm, L.diag, s.scale);
         __syncthreads();
-        if (w == 0) invert_blocks<CH>(tid, L.M, L.Tm);
+        if (w == 0) invert_blocks<BF, CH>(tid, L.diag, L.Tinv);
         if (w == NT - 1 && once) fill_rows<CH>(tid, L.R[cur ^ 1], gn, A, 0, rows);
         f4 Y[NB], dU[NB], sd = zero;
         {
@@ -982,6 +1086,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
           if constexpr (!LOCAL) {
 #pragma unroll
             for (int m = 0; m < NT; m++) {
+              if (fresh) S0[m] = zero;
               sd += S0[m] * dS[m];
               Sp[m].set(S0[m]);
             }
@@ -991,7 +1096,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
 #pragma unroll
               for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, L.K, 16 * n, 16 * m);
               Y[n] = rows4(tid, R.be, 16 * n) * (widen(col_unit<LD>(tid, L.V, 16 * n, 16 * w)) -
-                                            sel_mul(rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n), dot2<BF, NT>(x, Sp, zero)));
+                                            (rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n)) * (dot2<BF, NT>(x, Sp, zero)));
             }
           }
 #pragma unroll
@@ -1001,7 +1106,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             unit x[NT];
 #pragma unroll
             for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, L.K, 16 * n, 16 * m);
-            dU[n] = sel_mul(rows4(tid, R.dc, 16 * n) * rows4(tid, R.rk, 16 * n), dot2<BF, NT>(x, Sp, zero));
+            dU[n] = (rows4(tid, R.dc, 16 * n) * rows4(tid, R.rk, 16 * n)) * (dot2<BF, NT>(x, Sp, zero));
           }
         }
         __syncthreads();
@@ -1010,20 +1115,20 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
         f4 U[NB], dY[NB];
         unit dOc[NB];
         {
-          if constexpr (!LOCAL) solve<BF>(tid, L.Tm, L.M, Y, U);
+          if constexpr (!LOCAL) solve<BF>(tid, L.Tinv, L.M, Y, U);
           Pair<BF> x[NB];
 #pragma unroll
           for (int n = 0; n < NB; n++) dOc[n] = col_unit<LD>(tid, L.dO, 16 * n, 16 * w);
-          x[0].set(col_unit<CP>(tid, L.Pm, 0, 0));
+          x[0] = mat_row<BF, UD>(tid, L.Pm, 0, 0);
           if constexpr (NB == 2) {
-            x[1].set(col_unit<CP>(tid, L.Pm, 16, 0));
+            x[1] = mat_row<BF, UD>(tid, L.Pm, 0, 16);
             dU[0] = dot2r<BF, 2>(x, dOc, dU[0]);
-            x[0].set(col_unit<CP>(tid, L.Pm, 16, 16));
+            x[0] = mat_row<BF, UD>(tid, L.Pm, 16, 16);
             dU[1] = dot2r<BF, 1>(x, dOc + 1, dU[1]);
           } else {
             dU[0] = dot2r<BF, 1>(x, dOc, dU[0]);
           }
-          solve_t<BF>(tid, L.Tm, L.M, dU, dY);
+          solve_t<BF>(tid, L.Tinv, L.M, dU, dY);
         }
         const int starts = R.starts, inside = starts & ~(1 << lo);
         if (inside) {
@@ -1040,19 +1145,14 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
         }
         const int col = 16 * w + (l & 15);
         if constexpr (!LOCAL) {
-          const GradArgs a = again<GradArgs>(sizeof(Args));
-          T* dvp = (T*)a.dv + bt * a.dv_b + h * a.dv_h + t0 * a.dv_t + col;
 #pragma unroll
           for (int n = 0; n < NB; n++) {
-            const f4 be = rows4(tid, R.be, 16 * n);
             put_t<BF, UD>(tid, L.U, L.Ulo, w, 16 * n, U[n]);
             put_t<BF, UD>(tid, L.dY, L.dYlo, w, 16 * n, dY[n]);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-              const int row = 16 * n + 4 * (l >> 4) + i;
-              if (a.dv && row >= lo && row < hi && col < s.V) stf(dvp + row * a.dv_t, be[i] * dY[n][i]);
               const float sum = row16_sum(dY[n][i] * U[n][i]);
-              if ((l & 15) == 0) L.ysum[w][row] = sum;
+              if ((l & 15) == 0) L.ysum[w][16 * n + 4 * (l >> 4) + i] = sum;
             }
           }
         }
@@ -1063,15 +1163,15 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
           Pair<BF> x[NB], y[NB];
 #pragma unroll
           for (int n = 0; n < NB; n++) {
-            x[n].set(sel_mul(s.scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n), widen(dOc[n])));
-            y[n].set(sel_mul(-rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n) * rows4(tid, R.be, 16 * n), dY[n]));
+            x[n].set((s.scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n)) * (widen(dOc[n])));
+            y[n].set((-rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n) * rows4(tid, R.be, 16 * n)) * (dY[n]));
           }
 #pragma unroll
           for (int m = 0; m < NT; m++) {
             unit a[NB];
 #pragma unroll
             for (int n = 0; n < NB; n++) a[n] = col_unit<LD>(tid, L.Q, 16 * n, 16 * m);
-            dS[m] = dot2<BF, NB>(a, x, sel_mul(f4{c0, c0, c0, c0}, dS[m]));
+            dS[m] = dot2<BF, NB>(a, x, c0 * dS[m]);
 #pragma unroll
             for (int n = 0; n < NB; n++) a[n] = col_unit<LD>(tid, L.K, 16 * n, 16 * m);
             dS[m] = dot2<BF, NB>(a, y, dS[m]);
@@ -1102,31 +1202,35 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             const int j = 16 * bj + (l & 15);
             const double Gj = R.G[j];
             const int segj = R.seg[j];
+            const f4 pv = mat_values<BF, UD>(tid, L.Pm, 16 * bj, 16 * bi), mv = mat_values<BF, UD>(tid, L.M, 16 * bj, 16 * bi);
+            const f4 be = rows4(tid, R.be, 16 * bi);
 #pragma unroll
             for (int i4 = 0; i4 < 4; i4++) {
-              const int i = 16 * bi + 4 * (l >> 4) + i4, at = i * CP + j;
+              const int i = 16 * bi + 4 * (l >> 4) + i4;
               const bool on = segj == R.seg[i] && j <= i;
               const float dec = ex2((float)(R.G[i] - Gj));
-              L.W[at] = on && j < i ? L.Pm[at] * e[i4] - L.M[at] * f[i4] : 0.f;
-              L.E[at] = on ? dec * s.scale * e[i4] : 0.f;
-              L.F[at] = on && j < i ? -dec * R.be[i] * f[i4] : 0.f;
+              L.W[i * CP + j] = on && j < i ? pv[i4] * e[i4] - mv[i4] * f[i4] : 0.f;
+              e[i4] = on ? dec * s.scale * e[i4] : 0.f;
+              f[i4] = on && j < i ? -dec * be[i4] * f[i4] : 0.f;
             }
+            put_mat<BF, UD>(tid, L.Pm, 16 * bj, 16 * bi, e);
+            put_mat<BF, UD>(tid, L.M, 16 * bj, 16 * bi, f);
           }
           renew(tid, l);
           // products over V for this wavefront's columns of K: dO S_0^T, dY S_0^T, U dS^T
           f4 X1[NB], X2[NB], X3[NB];
 #pragma unroll
-          for (int m = 0; m < NT; m++) Xt[m].set(S0[m]);
+          for (int m = 0; m < NT; m++) Xt[m].set(fresh ? zero : S0[m]);
 #pragma unroll
           for (int n = 0; n < NB; n++) {
             unit x[NT];
 #pragma unroll
             for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, L.dO, 16 * n, 16 * m);
-            X1[n] = sel_mul(s.scale * rows4(tid, R.d0, 16 * n), dot2<BF, NT>(x, Xt, zero));
+            X1[n] = (s.scale * rows4(tid, R.d0, 16 * n)) * (dot2<BF, NT>(x, Xt, zero));
             Pair<BF> y[NT];
 #pragma unroll
             for (int m = 0; m < NT; m++) y[m] = col_pair<BF, UD>(tid, L.dY, L.dYlo, 16 * m, 16 * n);
-            X2[n] = sel_mul(-rows4(tid, R.d0, 16 * n) * rows4(tid, R.be, 16 * n), dot3<BF, NT>(y, Xt, zero));
+            X2[n] = (-rows4(tid, R.d0, 16 * n) * rows4(tid, R.be, 16 * n)) * (dot3<BF, NT>(y, Xt, zero));
           }
 #pragma unroll
           for (int m = 0; m < NT; m++) Xt[m].set(dSt[m]);
@@ -1135,7 +1239,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             Pair<BF> y[NT];
 #pragma unroll
             for (int m = 0; m < NT; m++) y[m] = col_pair<BF, UD>(tid, L.U, L.Ulo, 16 * m, 16 * n);
-            X3[n] = sel_mul(rows4(tid, R.dc, 16 * n), dot3<BF, NT>(y, Xt, zero));
+            X3[n] = (rows4(tid, R.dc, 16 * n)) * (dot3<BF, NT>(y, Xt, zero));
           }
           renew(tid, l);
           unit Kc[NB], Qc[NB];  // this wavefront's columns of K and Q
@@ -1148,15 +1252,15 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             Pair<BF> x[NB], y[NB];
 #pragma unroll
             for (int n = 0; n < NB; n++) {
-              x[n].set(sel_mul(s.scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n), widen(Qc[n])));
-              y[n].set(sel_mul(-rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n) * rows4(tid, R.be, 16 * n), widen(Kc[n])));
+              x[n].set((s.scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n)) * (widen(Qc[n])));
+              y[n].set((-rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n) * rows4(tid, R.be, 16 * n)) * (widen(Kc[n])));
             }
 #pragma unroll
             for (int m = 0; m < NT; m++) {
               unit a[NB];
 #pragma unroll
               for (int n = 0; n < NB; n++) a[n] = col_unit<LD>(tid, L.dO, 16 * n, 16 * m);
-              dSt[m] = dot2<BF, NB>(a, x, sel_mul(f4{c0, c0, c0, c0}, dSt[m]));
+              dSt[m] = dot2<BF, NB>(a, x, c0 * dSt[m]);
               Pair<BF> b[NB];
 #pragma unroll
               for (int n = 0; n < NB; n++) b[n] = row_pair<BF, UD>(tid, L.dY, L.dYlo, 16 * m, 16 * n);
@@ -1165,40 +1269,42 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
           }
           __syncthreads();
         renew(tid, l);
-          // E K, F K (rows as i), F^T K, E^T Q (rows as j); the norms' factors go into E and F
+          // E K^, F K^ (rows as i), F^T K^, E^T Q^ (rows as j): E and F rest where P and M were
           f4 dQ[NB], dK[NB];
           {
-            f4 rk[NB], rq[NB];
+            f4 qn[NB], kn[NB];
+            Pair<BF> kp2[NB], qp2[NB];
 #pragma unroll
             for (int n = 0; n < NB; n++) {
-              rk[n] = rows4(tid, R.rk, 16 * n);
-              rq[n] = rows4(tid, R.rq, 16 * n);
+              qn[n] = widen(Qc[n]) * rows4(tid, R.rq, 16 * n);
+              kn[n] = widen(Kc[n]) * rows4(tid, R.rk, 16 * n);
+              qp2[n].set(qn[n]);
+              kp2[n].set(kn[n]);
             }
 #pragma unroll
             for (int n = 0; n < NB; n++) {
-              const f4 qn = widen(Qc[n]) * rq[n], kn = widen(Kc[n]) * rk[n];
-              const f4 from0 = qn * X1[n] + kn * X2[n], fromc = kn * X3[n];
+              const f4 from0 = qn[n] * X1[n] + kn[n] * X2[n], fromc = kn[n] * X3[n];
               Pair<BF> e[NB], f[NB];
 #pragma unroll
               for (int m = 0; m <= n; m++) {
-                e[m].set(row_unit<CP>(tid, L.E, 16 * n, 16 * m) * rk[m]);
-                f[m].set(row_unit<CP>(tid, L.F, 16 * n, 16 * m) * rk[m]);
+                e[m] = mat_col<BF, UD>(tid, L.Pm, 16 * m, 16 * n);
+                f[m] = mat_col<BF, UD>(tid, L.M, 16 * m, 16 * n);
               }
               if (n == 0) {
-                dQ[n] = dot2r<BF, 1>(e, Kc, X1[n]);
-                dK[n] = dot2r<BF, 1>(f, Kc, X2[n] + X3[n]);
+                dQ[n] = dot3<BF, 1>(e, kp2, X1[n]);
+                dK[n] = dot3<BF, 1>(f, kp2, X2[n] + X3[n]);
               } else {
-                dQ[n] = dot2r<BF, NB>(e, Kc, X1[n]);
-                dK[n] = dot2r<BF, NB>(f, Kc, X2[n] + X3[n]);
+                dQ[n] = dot3<BF, NB>(e, kp2, X1[n]);
+                dK[n] = dot3<BF, NB>(f, kp2, X2[n] + X3[n]);
               }
 #pragma unroll
               for (int m = n; m < NB; m++) {
-                e[m].set(col_unit<CP>(tid, L.E, 16 * m, 16 * n) * rq[m]);
-                f[m].set(col_unit<CP>(tid, L.F, 16 * m, 16 * n) * rk[m]);
+                e[m] = mat_row<BF, UD>(tid, L.Pm, 16 * n, 16 * m);
+                f[m] = mat_row<BF, UD>(tid, L.M, 16 * n, 16 * m);
               }
-              if (n == NB - 1) dK[n] = dot2r<BF, 1>(f + n, Kc + n, dot2r<BF, 1>(e + n, Qc + n, dK[n]));
-              else dK[n] = dot2r<BF, NB>(f, Kc, dot2r<BF, NB>(e, Qc, dK[n]));
-              const f4 sq = qn * dQ[n], sk = kn * dK[n];
+              if (n == NB - 1) dK[n] += dot3<BF, 1>(f + n, kp2 + n, dot3<BF, 1>(e + n, qp2 + n, zero));
+              else dK[n] += dot3<BF, NB>(f, kp2, dot3<BF, NB>(e, qp2, zero));
+              const f4 sq = qn[n] * dQ[n], sk = kn[n] * dK[n];
 #pragma unroll
               for (int i = 0; i < 4; i++) {
                 const float x[4] = {row16_sum(sq[i]), row16_sum(sk[i]), row16_sum(from0[i]), row16_sum(fromc[i])};
@@ -1231,12 +1337,12 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
           if (l == 0) L.tot[w] = tot;
           __syncthreads();
         renew(tid, l);
-          // through the norms
+          // through the norms; dq, dk and dv rest where Q, K and dO were, until the rows are stored behind the next barrier
           const GradArgs a = again<GradArgs>(sizeof(Args));
           const Args sa = again<Args>(0);
 #pragma unroll
           for (int n = 0; n < NB; n++) {
-            const f4 rq = rows4(tid, R.rq, 16 * n), rk = rows4(tid, R.rk, 16 * n);
+            const f4 rq = rows4(tid, R.rq, 16 * n), rk = rows4(tid, R.rk, 16 * n), be = rows4(tid, R.be, 16 * n);
             f4 sq = zero, sk = zero;
 #pragma unroll
             for (int m = 0; m < NT; m++) {
@@ -1244,20 +1350,29 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
               sk += rows4(tid, L.sums[1][m], 16 * n);
             }
             const f4 dq = rq * (dQ[n] - widen(Qc[n]) * rq * sq), dk = rk * (dK[n] - widen(Kc[n]) * rk * sk);
+            const Pair<BF> dy = row_pair<BF, UD>(tid, L.dY, L.dYlo, 16 * w, 16 * n);
+            f4 dv;
+            if constexpr (BF) dv = be * (widen(dy.hi) + widen(dy.lo));
+            else dv = be * dy.hi;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-              const int row = 16 * n + 4 * (l >> 4) + i;
-              if (row < lo || row >= hi || col >= sa.K) continue;
+              const int row = 16 * n + 4 * (l >> 4) + i, at = row * LD + col;
+              stf(L.dO + at, dv[i]);
               if (a.qpart) {
-                const long at = (((t0 + row) * sa.B + bt) * sa.H + h) * sa.K + col;
-                a.qpart[at] = dq[i];
-                a.kpart[at] = dk[i];
+                if (row >= lo && row < hi && col < sa.K) {
+                  const long to = (((t0 + row) * sa.B + bt) * sa.H + h) * sa.K + col;
+                  a.qpart[to] = dq[i];
+                  a.kpart[to] = dk[i];
+                }
               } else {
-                if (a.dq) stf((T*)a.dq + bt * a.dq_b + h * a.dq_h + (t0 + row) * a.dq_t + col, dq[i]);
-                if (a.dk) stf((T*)a.dk + bt * a.dk_b + h * a.dk_h + (t0 + row) * a.dk_t + col, dk[i]);
+                stf(L.Q + at, dq[i]);
+                stf(L.K + at, dk[i]);
               }
             }
           }
+          y_at = t0;
+          y_lo = lo;
+          y_hi = hi;
           if (w == NT - 1) {  // the gates
             float from0 = 0.f, fromc = 0.f, dbr = 0.f, sum = 0.f;
             const int i = l < CH ? l : CH - 1;
@@ -1268,15 +1383,21 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
               dbr += L.ysum[m][i];
               sum += L.tot[m];
             }
-            if (l >= CH) from0 = fromc = 0.f;
-#pragma unroll
-            for (int e = 1; e < CH; e *= 2) {  // of the rows from t on, of the rows up to t
-              const float x = __shfl_down(from0, e), y = __shfl_up(fromc, e);
-              if (l + e < CH) from0 += x;
-              if (l >= e) fromc += y;
+            from0 += dpp_mov<0x101>(from0);  // of the rows from t on: sums along the rows of 16 lanes
+            from0 += dpp_mov<0x102>(from0);
+            from0 += dpp_mov<0x104>(from0);
+            from0 += dpp_mov<0x108>(from0);
+            fromc += dpp_mov<0x111>(fromc);  // of the rows up to t
+            fromc += dpp_mov<0x112>(fromc);
+            fromc += dpp_mov<0x114>(fromc);
+            fromc += dpp_mov<0x118>(fromc);
+            const float low = lane_f32(fromc, 15);
+            fromc = dpp_mov<0x111>(fromc);  // and before t
+            if constexpr (NB == 2) {
+              const float high = lane_f32(from0, 16);
+              if (l < 16) from0 += high;
+              else fromc += low;
             }
-            fromc = __shfl_up(fromc, 1);
-            if (l == 0) fromc = 0.f;
             float dg = L.pairs[0][i] + from0 + fromc + sum;
             if (NB == 2 && i >= 16) dg += L.pairs[NB - 1][i];
             if (l >= lo && l < hi) {
@@ -1309,6 +1430,10 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
         gn = load_gate<T>(s, bt, h, (c - 2) * CH, rows_at(c - 2), l);
       }
       cur ^= 1;
+    }
+    if constexpr (!LOCAL) {
+      __syncthreads();
+      put_grads(y_at, y_lo, y_hi);
     }
     if (LOCAL) {
 #pragma unroll
