@@ -53,6 +53,8 @@ typedef short s8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef u4 u4_any __attribute__((aligned(2)));  // 16 bytes at the alignment of an element
+typedef f4 f4_any __attribute__((aligned(4)));
 
 constexpr float kEps = 1e-6f;
 constexpr double kLog2e = 1.4426950408889634;
@@ -100,10 +102,19 @@ template <typename A> __device__ __forceinline__ A again(unsigned at) {
   return __builtin_bit_cast(A, w);
 }
 
+// Global pointers as such: of one that `again` has read the compiler does not know that it is none to LDS.
+#define PH_GLOBAL __attribute__((address_space(1)))
+template <typename T> using gin = const PH_GLOBAL T*;
+template <typename T> using gout = PH_GLOBAL T*;
+
 // ---- elements ------------------------------------------------------------------------------------------
 __device__ __forceinline__ float ldf(const uint16_t* p) { return bf16_to_f32(*p); }
+__device__ __forceinline__ float ldf(gin<uint16_t> p) { return bf16_to_f32(*p); }
+__device__ __forceinline__ float ldf(gin<float> p) { return *p; }
 __device__ __forceinline__ float ldf(const float* p) { return *p; }
 __device__ __forceinline__ void stf(uint16_t* p, float v) { *p = bf16_rne(v); }
+__device__ __forceinline__ void stf(gout<uint16_t> p, float v) { *p = bf16_rne(v); }
+__device__ __forceinline__ void stf(gout<float> p, float v) { *p = v; }
 __device__ __forceinline__ void stf(float* p, float v) { *p = v; }
 __device__ __forceinline__ float ex2(float v) { return __builtin_amdgcn_exp2f(v); }
 // softplus, max(v, 0) + log(1 + e) with e = exp(-|v|). What rounding 1 + e to w dropped is added back as it is, so small e
@@ -244,7 +255,7 @@ __device__ __forceinline__ f4 widen(f4 v) { return v; }
 // where the rows or the columns end. Any alignment: the hardware takes 16 bytes at that of an element. The last columns of a row
 // come from an access that ends with it, shifted down.
 template <bool BF, int P, typename T = typename Elem<BF>::type>
-__device__ __forceinline__ u4 load_row(int tid, const T* p, int rows, int W) {
+__device__ __forceinline__ u4 load_row(int tid, gin<T> p, int rows, int W) {
   constexpr int V = Elem<BF>::V;
   const int row = tid / (P / V), c = tid % (P / V) * V;
   u4 r = {0, 0, 0, 0};
@@ -252,31 +263,30 @@ __device__ __forceinline__ u4 load_row(int tid, const T* p, int rows, int W) {
     const int over = c + V - W;
     if (W >= V) {
       const int skip = over > 0 ? over : 0;
-      __builtin_memcpy(&r, p - skip, 16);
+      r = *(gin<u4_any>)(p - skip);
       if (over > 0) r = __builtin_bit_cast(u4, __builtin_bit_cast(unsigned __int128, r) >> (skip * 8 * (int)sizeof(T)));
     } else {
       unsigned __int128 x = 0;
 #pragma unroll 1
-      for (int i = W - 1; i >= 0; i--) x = x << (8 * (int)sizeof(T)) | (sizeof(T) == 2 ? (unsigned)__builtin_bit_cast(uint16_t, (uint16_t)*(const uint16_t*)(p + i)) : *(const unsigned*)(p + i));
+      for (int i = W - 1; i >= 0; i--) x = x << (8 * (int)sizeof(T)) | (sizeof(T) == 2 ? (unsigned)*(gin<uint16_t>)(p + i) : *(gin<unsigned>)(p + i));
       r = __builtin_bit_cast(u4, x);
     }
   }
   return r;
 }
 // The first n of 16 bytes' elements from LDS to a row.
-template <bool BF, typename T = typename Elem<BF>::type> __device__ __forceinline__ void store_row(T* p, const T* from, int n) {
+template <bool BF, typename T = typename Elem<BF>::type> __device__ __forceinline__ void store_row(gout<T> p, const T* from, int n) {
   constexpr int V = Elem<BF>::V;
   if (n >= V) {
-    const u4 r = *reinterpret_cast<const u4*>(from);
-    __builtin_memcpy(p, &r, 16);
+    *(gout<u4_any>)p = *reinterpret_cast<const u4*>(from);
   } else {
 #pragma unroll 1
     for (int i = 0; i < n; i++) p[i] = from[i];
   }
 }
-template <bool BF, int P, typename T> __device__ __forceinline__ const T* thread_row(int tid, const T* base, long stride, long t0) {
+template <bool BF, int P, typename T> __device__ __forceinline__ gin<T> thread_row(int tid, const T* base, long stride, long t0) {
   constexpr int V = Elem<BF>::V;
-  return base + (t0 + tid / (P / V)) * stride + tid % (P / V) * V;
+  return (gin<T>)base + (t0 + tid / (P / V)) * stride + tid % (P / V) * V;
 }
 template <bool BF> __device__ __forceinline__ float square_sum(u4 r) {
   float s = 0.f;
@@ -322,14 +332,15 @@ template <int CH> struct Rows {
 struct Gate {
   float a, b, start;
 };
-template <typename T> __device__ __forceinline__ Gate load_gate(const Args& s, long bt, int h, long t0, int rows, int i) {
+template <typename T> __device__ __forceinline__ Gate load_gate(long bt, int h, long t0, int rows, int i) {
   Gate g = {0.f, 0.f, 0.f};
+  const Args s = again<Args>(0);
   if (i < rows) {
     const long t = t0 + i;
-    g.a = ldf((const T*)s.a + t * s.a_t + bt * s.a_b + h) + (s.dt_bias ? s.dt_bias[h] : 0.f);
-    g.b = ldf((const T*)s.b + t * s.b_t + bt * s.b_b + h);
-    if (t > 0) g.start = s.done ? s.done[(t - 1) * s.B + bt] : 0.f;
-    else g.start = s.first ? s.first[bt] : 0.f;
+    g.a = ldf((gin<T>)s.a + t * s.a_t + bt * s.a_b + h) + (s.dt_bias ? ((gin<float>)s.dt_bias)[h] : 0.f);
+    g.b = ldf((gin<T>)s.b + t * s.b_t + bt * s.b_b + h);
+    if (t > 0) g.start = s.done ? ((gin<float>)s.done)[(t - 1) * s.B + bt] : 0.f;
+    else g.start = s.first ? ((gin<float>)s.first)[bt] : 0.f;
   }
   return g;
 }
@@ -524,67 +535,72 @@ template <bool BF, int NM, int NI> __device__ __forceinline__ void solve_t(int t
   dY[0] = dot3<BF, 1>(&t, &y, zero);
 }
 
-// States in memory: [K][V] as the caller holds them, or [up(K)][up(V)], both rounded up to whole tiles, as the library does.
+// States in memory: [K][V] as the caller holds them; the library's own in whole tiles of 16x16, [K tiles][V tiles], each as the
+// lanes hold it: lane l's four rows 4 (l / 16) + 0..3 of column l % 16.
 __host__ __device__ __forceinline__ int up16(int n) { return (n + 15) & ~15; }
-// Tile m of a library's state's column block w: rows 16 m + 4 (l / 16) + 0..3, column 16 w + l % 16; the transposed state's:
-// columns of V 16 m + 4 (l / 16) + 0..3, row 16 w + l % 16. Whole tiles, of which those past the last are not there.
-__device__ __forceinline__ f4 own_tile(int tid, const float* s, int Ku, int Vu, int m, int w) {
-  const int l = tid & 63;
-  f4 x = {0.f, 0.f, 0.f, 0.f};
-  if (16 * m < Ku && 16 * w < Vu) {
-    const float* p = s + (16 * m + 4 * (l >> 4)) * Vu + 16 * w + (l & 15);
+struct Own {
+  int tk, tv;  // tiles
+  __device__ __forceinline__ long floats() const { return (long)tk * tv * 256; }
+};
+// Tile m of column block w; one past the last is taken as the last: its rows meet keys and queries of zero.
+__device__ __forceinline__ f4 own_tile(int tid, gin<float> s, Own d, int m, int w) {
+  const int tile = (m < d.tk ? m : d.tk - 1) * d.tv + (w < d.tv ? w : d.tv - 1);
+  return *reinterpret_cast<gin<f4>>(s + tile * 256 + 4 * (tid & 63));
+}
+// The transposed state's tile m of block w: columns of V 16 m + 4 (l / 16) + 0..3, row 16 w + l % 16.
+__device__ __forceinline__ f4 own_tile_t(int tid, gin<float> s, Own d, int m, int w) {
+  const int l = tid & 63, tile = (w < d.tk ? w : d.tk - 1) * d.tv + (m < d.tv ? m : d.tv - 1);
+  gin<float> p = s + tile * 256 + ((l >> 2 & 3) * 16 + 4 * (l >> 4)) * 4 + (l & 3);
+  return f4{p[0], p[4], p[8], p[12]};
+}
+__device__ __forceinline__ void put_own_tile(int tid, gout<float> s, Own d, int m, int w, f4 x) {
+  if (m < d.tk && w < d.tv) *reinterpret_cast<gout<f4>>(s + (m * d.tv + w) * 256 + 4 * (tid & 63)) = x;
+}
+// All tiles of column block w of a caller's state, or (T) of the transposed one's; zero outside. Addresses are clamped and not
+// skipped: a load that a branch guards is waited for before the next one.
+template <int NT, bool TR> __device__ __forceinline__ void get_state(int tid, gin<float> s, int K, int V, int w, f4* S) {
+  const int l = tid & 63, in = l & 15, four = 4 * (l >> 4);
+  if (((K | V) & 15) == 0) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = p[i * Vu];
+    for (int m = 0; m < NT; m++) {
+      S[m] = f4{0.f, 0.f, 0.f, 0.f};
+      if (16 * m < (TR ? V : K) && 16 * w < (TR ? K : V)) {
+        if constexpr (TR) {
+          S[m] = *(gin<f4_any>)(s + (16 * w + in) * V + 16 * m + four);
+        } else {
+          gin<float> p = s + four * V + 16 * w + in;
+#pragma unroll
+          for (int i = 0; i < 4; i++) S[m][i] = p[(16 * m + i) * V];
+        }
+      }
+    }
+    return;
   }
-  return x;
-}
-__device__ __forceinline__ f4 own_tile_t(int tid, const float* s, int Ku, int Vu, int m, int w) {
-  const int l = tid & 63;
-  f4 x = {0.f, 0.f, 0.f, 0.f};
-  if (16 * m < Vu && 16 * w < Ku) x = *reinterpret_cast<const f4*>(s + (16 * w + (l & 15)) * Vu + 16 * m + 4 * (l >> 4));
-  return x;
-}
-__device__ __forceinline__ void put_own_tile(int tid, float* s, int Ku, int Vu, int m, int w, f4 x) {
-  const int l = tid & 63;
-  if (16 * m < Ku && 16 * w < Vu) {
-    float* p = s + (16 * m + 4 * (l >> 4)) * Vu + 16 * w + (l & 15);
+#pragma unroll 1
+  for (int m = 0; m < NT; m++) {
+    f4 x;
 #pragma unroll
-    for (int i = 0; i < 4; i++) p[i * Vu] = x[i];
+    for (int i = 0; i < 4; i++) {
+      const int k = TR ? 16 * w + in : 16 * m + four + i, v = TR ? 16 * m + four + i : 16 * w + in;
+      const float y = s[k < K && v < V ? k * V + v : 0];
+      x[i] = k < K && v < V ? y : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; j++) S[j] = j == m ? x : S[j];
+  }
+}
+template <int NT> __device__ __forceinline__ void put_state(int tid, gout<float> s, int K, int V, int w, const f4* S) {
+  const int l = tid & 63, c = 16 * w + (l & 15), four = 4 * (l >> 4);
+  if (c >= V) return;
+#pragma unroll
+  for (int m = 0; m < NT; m++) {
+    gout<float> p = s + (16 * m + four) * V + c;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (16 * m + four + i < K) p[i * V] = S[m][i];
   }
 }
 
-// The same of a caller's state of any size, zero outside. Addresses are clamped
-// and not skipped: a load that a branch guards is waited for before the next one.
-__device__ __forceinline__ f4 state_tile(int tid, const float* s, int K, int V, int m, int w) {
-  if (((K | V) & 15) == 0) return own_tile(tid, s, K, V, m, w);
-  const int l = tid & 63, r = 16 * m + 4 * (l >> 4), c = 16 * w + (l & 15);
-  const float* p = s + (c < V ? c : 0);
-  f4 x;
-#pragma unroll
-  for (int i = 0; i < 4; i++) x[i] = p[(r + i < K ? r + i : 0) * V];
-#pragma unroll
-  for (int i = 0; i < 4; i++) x[i] = r + i < K && c < V ? x[i] : 0.f;
-  return x;
-}
-__device__ __forceinline__ void put_state_tile(int tid, float* s, int K, int V, int m, int w, f4 x) {
-  if (((K | V) & 15) == 0) return put_own_tile(tid, s, K, V, m, w, x);
-  const int l = tid & 63, r = 16 * m + 4 * (l >> 4), c = 16 * w + (l & 15);
-  if (c < V) {
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (r + i < K) s[(r + i) * V + c] = x[i];
-  }
-}
-__device__ __forceinline__ f4 state_tile_t(int tid, const float* s, int K, int V, int m, int w) {
-  const int l = tid & 63, c = 16 * m + 4 * (l >> 4), r = 16 * w + (l & 15);
-  const float* p = s + (r < K ? r : 0) * V;
-  f4 x;
-#pragma unroll
-  for (int i = 0; i < 4; i++) x[i] = p[c + i < V ? c + i : 0];
-#pragma unroll
-  for (int i = 0; i < 4; i++) x[i] = r < K && c + i < V ? x[i] : 0.f;
-  return x;
-}
 template <bool BF, int P, typename T = typename Elem<BF>::type>
 __device__ __forceinline__ void put_row(int tid, T* tile, u4 r, int lo, int hi) {
   constexpr int V = Elem<BF>::V, LD = P + Elem<BF>::pad;
@@ -631,12 +647,12 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
     const long seg = LOCAL ? (s.parts == 1 ? round : round >> 1) + s.local_from : round;
     const long bt = (unsigned)unit_id / (unsigned)s.H;
     const int h = (int)(unit_id - bt * s.H), hk = (int)((unsigned)h / (unsigned)(s.H / s.Hk));
-    const int Ku = up16(s.K), Vu = up16(s.V), W = part ? s.K : s.V;  // columns of the state
+    const Own own = {up16(s.K) / 16, up16(part ? s.K : s.V) / 16};
     const long first = seg * s.seg_chunks * CH;
     const long last = first + s.seg_chunks * CH < s.T ? first + s.seg_chunks * CH : s.T;
-    const T* qp = thread_row<BF, P>(tid, (const T*)s.q + bt * s.q_b + hk * s.q_h, s.q_t, first);
-    const T* kp = thread_row<BF, P>(tid, (const T*)s.k + bt * s.k_b + hk * s.k_h, s.k_t, first);
-    const T* vp = thread_row<BF, P>(tid, (const T*)s.v + bt * s.v_b + h * s.v_h, s.v_t, first);
+    gin<T> qp = thread_row<BF, P>(tid, (const T*)s.q + bt * s.q_b + hk * s.q_h, s.q_t, first);
+    gin<T> kp = thread_row<BF, P>(tid, (const T*)s.k + bt * s.k_b + hk * s.k_h, s.k_t, first);
+    gin<T> vp = thread_row<BF, P>(tid, (const T*)s.v + bt * s.v_b + h * s.v_h, s.v_t, first);
     const int W_v = part ? 0 : s.V;
     const float A = s.A[h];
     auto rows_at = [&](long t0) { return (int)(t0 >= last ? 0 : last - t0 < CH ? last - t0 : CH); };
@@ -652,10 +668,12 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
       }
     } else if (s.segs > 1) {
 #pragma unroll
-      for (int m = 0; m < NT; m++) S[m] = own_tile(tid, s.start + (seg * s.units + unit_id) * Ku * Vu, Ku, Vu, m, w);
+      for (int m = 0; m < NT; m++) {
+        S[m] = own_tile(tid, (gin<float>)s.start + (seg * s.units + unit_id) * own.floats(), own, m, w);
+        if (m >= own.tk || w >= own.tv) S[m] = zero;
+      }
     } else if (s.h0) {
-#pragma unroll
-      for (int m = 0; m < NT; m++) S[m] = state_tile(tid, s.h0 + unit_id * s.K * s.V, s.K, s.V, m, w);
+      get_state<NT, false>(tid, (gin<float>)s.h0 + unit_id * s.K * s.V, s.K, s.V, w, S);
     } else {
 #pragma unroll
       for (int m = 0; m < NT; m++) S[m] = zero;
@@ -667,13 +685,18 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
       k = load_row<BF, P>(tid, kp, rows, s.K);
       v = load_row<BF, P>(tid, vp, rows, W_v);
     };
-    load();
+    auto walk = [&](int chunks) {
+      const Args a = again<Args>(0);
+      qp += chunks * CH * a.q_t;
+      kp += chunks * CH * a.k_t;
+      vp += chunks * CH * a.v_t;
+    };
+    bool have = false;  // this chunk's rows are there
     // the last wavefront sees to the gates, a chunk ahead
     Gate g = {0.f, 0.f, 0.f}, gn = g;
     if (w == NT - 1) {
-      g = load_gate<T>(s, bt, h, first, rows, l);
-      gn = load_gate<T>(s, bt, h, first + CH, rows_at(first + CH), l);
-      __builtin_amdgcn_s_waitcnt(0);
+      g = load_gate<T>(bt, h, first, rows, l);
+      gn = load_gate<T>(bt, h, first + CH, rows_at(first + CH), l);
     }
     __syncthreads();  // the item before has been read
     if (w == NT - 1) fill_rows<CH>(tid, Rs[0], g, A, 0, rows);
@@ -683,13 +706,17 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
       const Args a = again<Args>(0);
       const int row = tid / (P / Elem<BF>::V), c = tid % (P / Elem<BF>::V) * Elem<BF>::V;
       if (row >= lo && row < hi)
-        store_row<BF>((T*)a.y + bt * a.y_b + h * a.y_h + (at + row) * a.y_t + c, Vs + row * LD + c, a.V - c);
+        store_row<BF>((gout<T>)a.y + bt * a.y_b + h * a.y_h + (at + row) * a.y_t + c, Vs + row * LD + c, a.V - c);
     };
     for (long t0 = first; t0 < last; t0 += CH) {
       Rows<CH>& R = Rs[cur];
-      if (!LOCAL && s.keep) {
+      if (!LOCAL) {
+        const Args a = again<Args>(0);
+        if (a.keep) {
+          gout<float> to = (gout<float>)a.keep + (t0 / CH * a.units + unit_id) * own.floats();
 #pragma unroll
-        for (int m = 0; m < NT; m++) put_own_tile(tid, s.keep + (t0 / CH * s.units + unit_id) * Ku * Vu, Ku, Vu, m, w, S[m]);
+          for (int m = 0; m < NT; m++) put_own_tile(tid, to, own, m, w, S[m]);
+        }
       }
       const int all = rows;  // rows of this chunk
       for (int lo = 0, hi = all, once = 1; lo < all; once = 0) {
@@ -699,10 +726,7 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
           put_y(y_at, y_lo, y_hi);
           y_hi = 0;
         }
-        if (!once) {  // one episode at a time: rows and gates again
-          rows = all;
-          load();
-        }
+        if (!have) load();  // the first ones, or one episode at a time again
         if (!LOCAL) put_row<BF, P>(tid, Qs, q, lo, hi);
         put_row<BF, P>(tid, Ks, k, lo, hi);
         put_row<BF, P>(tid, Vs, v, lo, hi);
@@ -710,10 +734,9 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
         put_norm<BF, P>(tid, R.rk, k, lo, hi);
         if (!once && w == NT - 1) fill_rows<CH>(tid, R, g, A, lo, hi);
         __syncthreads();
+        have = once;
         if (once) {  // the next chunk's are on their way while this one computes
-          qp += CH * s.q_t;
-          kp += CH * s.k_t;
-          vp += CH * s.v_t;
+          walk(1);
           rows = rows_at(t0 + CH);
           load();
         }
@@ -756,9 +779,9 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
 #pragma unroll
             for (int i = 0; i < 4; i++) bad |= !finite(U[n][i]);
           if (__syncthreads_or(bad)) {
-            qp -= once ? CH * s.q_t : 0;
-            kp -= once ? CH * s.k_t : 0;
-            vp -= once ? CH * s.v_t : 0;
+            if (once) walk(-1);
+            have = false;
+            rows = all;
             hi = __ffs(inside) - 1;
             continue;
           }
@@ -798,16 +821,13 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
         lo = hi;
         hi = all;
         if (!once && lo >= all) {  // on to the next chunk's rows
-          qp += CH * s.q_t;
-          kp += CH * s.k_t;
-          vp += CH * s.v_t;
+          walk(1);
           rows = rows_at(t0 + CH);
-          load();
         }
       }
       if (w == NT - 1) {
         g = gn;
-        gn = load_gate<T>(s, bt, h, t0 + 2 * CH, rows_at(t0 + 2 * CH), l);
+        gn = load_gate<T>(bt, h, t0 + 2 * CH, rows_at(t0 + 2 * CH), l);
       }
       cur ^= 1;
     }
@@ -817,13 +837,12 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
     }
     if (LOCAL) {
       const long at = seg * s.units + unit_id;
-      float* out = part ? s.phi + at * Ku * Ku : s.psi + at * Ku * Vu;
+      gout<float> out = (gout<float>)(part ? s.phi : s.psi) + at * own.floats();
 #pragma unroll
-      for (int m = 0; m < NT; m++) put_own_tile(tid, out, Ku, up16(W), m, w, S[m]);
+      for (int m = 0; m < NT; m++) put_own_tile(tid, out, own, m, w, S[m]);
       if (part && tid == 0) s.cut[at] = cut != 0;
     } else if (s.h_out && last == s.T) {
-#pragma unroll
-      for (int m = 0; m < NT; m++) put_state_tile(tid, s.h_out + unit_id * s.K * s.V, s.K, s.V, m, w, S[m]);
+      put_state<NT>(tid, (gout<float>)s.h_out + unit_id * s.K * s.V, s.K, s.V, w, S);
     }
   }
 }
@@ -833,25 +852,33 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
 template <bool BF, int P, bool BACK> __global__ void __launch_bounds__(4 * P) k_delta_join(const Args s, const GradArgs o) {
   constexpr int NT = P / 16, LD = P + 4;
   __shared__ __attribute__((aligned(16))) float F[64 * LD];  // half of Phi's rows (P = 128), or all
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), Ku = up16(s.K), Vu = up16(s.V);
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Own own = {up16(s.K) / 16, up16(s.V) / 16}, sq = {own.tk, own.tk};
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
   for (long unit_id = blockIdx.x; unit_id < s.units; unit_id += gridDim.x) {
     f4 S[NT];
     const float* from = BACK ? o.dh : s.h0;
+    if (from) {
+      get_state<NT, false>(tid, (gin<float>)from + unit_id * s.K * s.V, s.K, s.V, w, S);
+    } else {
 #pragma unroll
-    for (int m = 0; m < NT; m++) {
-      S[m] = from ? state_tile(tid, from + unit_id * s.K * s.V, s.K, s.V, m, w) : zero;
-      put_own_tile(tid, (BACK ? o.dend + (s.segs - 1) * s.units * Ku * Vu : s.start) + unit_id * Ku * Vu, Ku, Vu, m, w, S[m]);
+      for (int m = 0; m < NT; m++) S[m] = zero;
     }
+#pragma unroll
+    for (int m = 0; m < NT; m++)
+      put_own_tile(tid, (gout<float>)(BACK ? o.dend + (s.segs - 1) * s.units * own.floats() : s.start) + unit_id * own.floats(), own, m, w, S[m]);
     for (long i = 0; i + 1 < s.segs; i++) {
       const long seg = BACK ? s.segs - 1 - i : i;  // the segment that is passed
       const long at = (BACK ? seg - 1 : seg) * s.units + unit_id;
       const long fat = seg * s.units + unit_id;
-      const float* add = BACK ? o.xi + fat * Ku * Vu : s.psi + at * Ku * Vu;
-      const float* phi = s.phi + fat * Ku * Ku;
+      gin<float> add = (gin<float>)(BACK ? o.xi : s.psi) + fat * own.floats();
+      gin<float> phi = (gin<float>)s.phi + fat * sq.floats();
       f4 N[NT];
 #pragma unroll
-      for (int m = 0; m < NT; m++) N[m] = own_tile(tid, add, Ku, Vu, m, w);
+      for (int m = 0; m < NT; m++) {
+        N[m] = own_tile(tid, add, own, m, w);
+        if (m >= own.tk || w >= own.tv) N[m] = zero;
+      }
       if (!s.cut[fat]) {
         Pair<BF> Sp[NT];
 #pragma unroll
@@ -859,14 +886,16 @@ template <bool BF, int P, bool BACK> __global__ void __launch_bounds__(4 * P) k_
 #pragma unroll
         for (int half = 0; half < (P + 63) / 64; half++) {
           __syncthreads();
-          for (int e = tid; e < 64 * (P / 4); e += 4 * P) {
-            const int r = e / (P / 4), c = e % (P / 4) * 4;
+          constexpr int HT = P < 64 ? NT : 4;  // tiles of rows here
+          for (int tile = w; tile < HT * NT; tile += NT) {
+            const int m = HT * half + tile / NT, n = tile % NT, l = tid & 63;
             f4 x = zero;
-            if (64 * half + r < Ku && c < Ku) x = *reinterpret_cast<const f4*>(phi + (64 * half + r) * Ku + c);
-            *reinterpret_cast<f4*>(F + r * LD + c) = x;
+            if (m < own.tk && n < own.tk) x = own_tile(tid, phi, sq, m, n);
+            float* to = F + (16 * (tile / NT) + 4 * (l >> 4)) * LD + 16 * n + (l & 15);
+#pragma unroll
+            for (int r = 0; r < 4; r++) to[r * LD] = x[r];
           }
           __syncthreads();
-          constexpr int HT = P < 64 ? NT : 4;  // tiles of rows here
           if constexpr (!BACK) {
 #pragma unroll
             for (int m = 0; m < HT; m++) {
@@ -886,11 +915,11 @@ template <bool BF, int P, bool BACK> __global__ void __launch_bounds__(4 * P) k_
           }
         }
       }
-      float* out = (BACK ? o.dend + at * Ku * Vu : s.start + (at + s.units) * Ku * Vu);
+      gout<float> out = (gout<float>)(BACK ? o.dend + at * own.floats() : s.start + (at + s.units) * own.floats());
 #pragma unroll
       for (int m = 0; m < NT; m++) {
         S[m] = N[m];
-        put_own_tile(tid, out, Ku, Vu, m, w, S[m]);
+        put_own_tile(tid, out, own, m, w, S[m]);
       }
     }
   }
@@ -976,30 +1005,32 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
   for (long item = blockIdx.x; item < items; item += gridDim.x) {
     const unsigned units = (unsigned)s.units, round = (unsigned)item / units;
     const long unit_id = (unsigned)item - round * units, seg = round + (LOCAL ? 1 : 0), bt = (unsigned)unit_id / (unsigned)s.H;
-    const int h = (int)(unit_id - bt * s.H), hk = (int)((unsigned)h / (unsigned)(s.H / s.Hk)), Ku = up16(s.K), Vu = up16(s.V);
+    const int h = (int)(unit_id - bt * s.H), hk = (int)((unsigned)h / (unsigned)(s.H / s.Hk));
+    const Own own = {up16(s.K) / 16, up16(s.V) / 16};
     const long c_first = seg * s.seg_chunks, c_all = (s.T + CH - 1) / CH;
     long c = c_first + s.seg_chunks < c_all ? c_first + s.seg_chunks - 1 : c_all - 1;
-    const T* qp = thread_row<BF, P>(tid, (const T*)s.q + bt * s.q_b + hk * s.q_h, s.q_t, c * CH);
-    const T* kp = thread_row<BF, P>(tid, (const T*)s.k + bt * s.k_b + hk * s.k_h, s.k_t, c * CH);
-    const T* vp = thread_row<BF, P>(tid, (const T*)s.v + bt * s.v_b + h * s.v_h, s.v_t, c * CH);
-    const T* op = thread_row<BF, P>(tid, (const T*)o.dy + bt * o.dy_b + h * o.dy_h, o.dy_t, c * CH);
+    gin<T> qp = thread_row<BF, P>(tid, (const T*)s.q + bt * s.q_b + hk * s.q_h, s.q_t, c * CH);
+    gin<T> kp = thread_row<BF, P>(tid, (const T*)s.k + bt * s.k_b + hk * s.k_h, s.k_t, c * CH);
+    gin<T> vp = thread_row<BF, P>(tid, (const T*)s.v + bt * s.v_b + h * s.v_h, s.v_t, c * CH);
+    gin<T> op = thread_row<BF, P>(tid, (const T*)o.dy + bt * o.dy_b + h * o.dy_h, o.dy_t, c * CH);
     const float A = s.A[h];
     auto rows_at = [&](long ch) { return (int)(ch < c_first ? 0 : s.T - ch * CH < CH ? s.T - ch * CH : CH); };
     double sumA = 0.0, sumB = 0.0;  // of the lanes that see to the gates
     f4 dS[NT], dSt[LOCAL ? 1 : NT];
     if (!LOCAL && s.segs > 1) {
-      const float* d = o.dend + (seg * s.units + unit_id) * Ku * Vu;
+      gin<float> d = (gin<float>)o.dend + (seg * s.units + unit_id) * own.floats();
 #pragma unroll
       for (int m = 0; m < NT; m++) {
-        dS[m] = own_tile(tid, d, Ku, Vu, m, w);
-        if constexpr (!LOCAL) dSt[m] = own_tile_t(tid, d, Ku, Vu, m, w);
+        dS[m] = own_tile(tid, d, own, m, w);
+        if (m >= own.tk || w >= own.tv) dS[m] = zero;
+        if constexpr (!LOCAL) {
+          dSt[m] = own_tile_t(tid, d, own, m, w);
+          if (m >= own.tv || w >= own.tk) dSt[m] = zero;
+        }
       }
     } else if (!LOCAL && o.dh) {
-#pragma unroll
-      for (int m = 0; m < NT; m++) {
-        dS[m] = state_tile(tid, o.dh + unit_id * s.K * s.V, s.K, s.V, m, w);
-        if constexpr (!LOCAL) dSt[m] = state_tile_t(tid, o.dh + unit_id * s.K * s.V, s.K, s.V, m, w);
-      }
+      get_state<NT, false>(tid, (gin<float>)o.dh + unit_id * s.K * s.V, s.K, s.V, w, dS);
+      if constexpr (!LOCAL) get_state<NT, true>(tid, (gin<float>)o.dh + unit_id * s.K * s.V, s.K, s.V, w, dSt);
     } else {
 #pragma unroll
       for (int m = 0; m < NT; m++) {
@@ -1015,18 +1046,24 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
       if (!LOCAL) v = load_row<BF, P>(tid, vp, rows, s.V);
       d = load_row<BF, P>(tid, op, rows, s.V);
     };
-    auto walk = [&](long chunks) {
-      qp += chunks * CH * s.q_t;
-      kp += chunks * CH * s.k_t;
-      vp += chunks * CH * s.v_t;
-      op += chunks * CH * o.dy_t;
+    auto walk = [&](int chunks) {
+      const Args a = again<Args>(0);
+      const GradArgs b = again<GradArgs>(sizeof(Args));
+      qp += chunks * CH * a.q_t;
+      kp += chunks * CH * a.k_t;
+      vp += chunks * CH * a.v_t;
+      op += chunks * CH * b.dy_t;
     };
-    load();
+    auto keep_at = [&](long ch) {
+      const Args a = again<Args>(0);
+      return (gin<float>)again<GradArgs>(sizeof(Args)).keep + (ch * a.units + unit_id) * own.floats();
+    };
+    bool have = false;  // this chunk's rows are there
     // the last wavefront sees to the gates, a chunk ahead
     Gate g = {0.f, 0.f, 0.f}, gn = g;
     if (w == NT - 1) {
-      g = load_gate<T>(s, bt, h, c * CH, rows, l);
-      gn = load_gate<T>(s, bt, h, (c - 1) * CH, rows_at(c - 1), l);
+      g = load_gate<T>(bt, h, c * CH, rows, l);
+      gn = load_gate<T>(bt, h, (c - 1) * CH, rows_at(c - 1), l);
     }
     __syncthreads();  // the item before has been read
     if (w == NT - 1) fill_rows<CH>(tid, L.R[0], g, A, 0, rows);
@@ -1037,9 +1074,9 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
       const Args sa = again<Args>(0);
       const int row = tid / (P / Elem<BF>::V), c = tid % (P / Elem<BF>::V) * Elem<BF>::V, from = row * LD + c;
       if (row < lo || row >= hi) return;
-      if (a.dv) store_row<BF>((T*)a.dv + bt * a.dv_b + h * a.dv_h + (at + row) * a.dv_t + c, L.dO + from, sa.V - c);
-      if (a.dq && !a.qpart) store_row<BF>((T*)a.dq + bt * a.dq_b + h * a.dq_h + (at + row) * a.dq_t + c, L.Q + from, sa.K - c);
-      if (a.dk && !a.qpart) store_row<BF>((T*)a.dk + bt * a.dk_b + h * a.dk_h + (at + row) * a.dk_t + c, L.K + from, sa.K - c);
+      if (a.dv) store_row<BF>((gout<T>)a.dv + bt * a.dv_b + h * a.dv_h + (at + row) * a.dv_t + c, L.dO + from, sa.V - c);
+      if (a.dq && !a.qpart) store_row<BF>((gout<T>)a.dq + bt * a.dq_b + h * a.dq_h + (at + row) * a.dq_t + c, L.Q + from, sa.K - c);
+      if (a.dk && !a.qpart) store_row<BF>((gout<T>)a.dk + bt * a.dk_b + h * a.dk_h + (at + row) * a.dk_t + c, L.K + from, sa.K - c);
     };
     for (; c >= c_first; c--) {
       Rows<CH>& R = L.R[cur];
@@ -1052,10 +1089,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
           put_grads(y_at, y_lo, y_hi);
           y_hi = 0;
         }
-        if (!once) {  // one episode at a time: rows and gates again
-          rows = all;
-          load();
-        }
+        if (!have) load();  // the first ones, or one episode at a time again
         const bool odd = tid / (P / Elem<BF>::V) >= lo && tid / (P / Elem<BF>::V) < hi && (!all_finite<BF>(q) || !all_finite<BF>(d));
         put_row<BF, P>(tid, L.Q, q, lo, hi);
         put_row<BF, P>(tid, L.K, k, lo, hi);
@@ -1067,9 +1101,10 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
         f4 S0[LOCAL ? 1 : NT];
         if constexpr (!LOCAL) {
 #pragma unroll
-          for (int m = 0; m < NT; m++) S0[m] = own_tile(tid, o.keep + (c * s.units + unit_id) * Ku * Vu, Ku, Vu, m, w);
+          for (int m = 0; m < NT; m++) S0[m] = own_tile(tid, keep_at(c), own, m, w);
         }
         __syncthreads();
+        have = once;
         if (once) {  // the next chunk's are on their way while this one computes
           walk(-1);
           rows = rows_at(c - 1);
@@ -1139,6 +1174,8 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             for (int i = 0; i < 4; i++) bad |= (!LOCAL && !finite(U[n][i])) || !finite(dY[n][i]);
           if (__syncthreads_or(bad)) {
             if (once) walk(1);
+            have = false;
+            rows = all;
             lo = 31 - __clz(inside);
             continue;
           }
@@ -1180,7 +1217,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
         if constexpr (!LOCAL) {
           Pair<BF> Xt[NT];  // S_0 transposed, then dS
 #pragma unroll
-          for (int m = 0; m < NT; m++) S0[m] = own_tile_t(tid, o.keep + (c * s.units + unit_id) * Ku * Vu, Ku, Vu, m, w);
+          for (int m = 0; m < NT; m++) S0[m] = own_tile_t(tid, keep_at(c), own, m, w);
           __syncthreads();
         renew(tid, l);
           for (int tile = w; tile < TILES; tile += NT) {
@@ -1361,8 +1398,8 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
               if (a.qpart) {
                 if (row >= lo && row < hi && col < sa.K) {
                   const long to = (((t0 + row) * sa.B + bt) * sa.H + h) * sa.K + col;
-                  a.qpart[to] = dq[i];
-                  a.kpart[to] = dk[i];
+                  ((gout<float>)a.qpart)[to] = dq[i];
+                  ((gout<float>)a.kpart)[to] = dk[i];
                 }
               } else {
                 stf(L.Q + at, dq[i]);
@@ -1403,8 +1440,8 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             if (l >= lo && l < hi) {
               const float be = R.be[l], arg = R.arg[l];
               const float da = dg * A * sigma(arg);
-              if (a.da) stf((T*)a.da + (t0 + l) * a.da_t + bt * a.da_b + h, da);
-              if (a.db) stf((T*)a.db + (t0 + l) * a.db_t + bt * a.db_b + h, dbr * (1.f - be));
+              if (a.da) stf((gout<T>)a.da + (t0 + l) * a.da_t + bt * a.da_b + h, da);
+              if (a.db) stf((gout<T>)a.db + (t0 + l) * a.db_t + bt * a.db_b + h, dbr * (1.f - be));
               sumA += (double)dg * (double)R.sp[l];
               sumB += (double)da;
             }
@@ -1422,12 +1459,11 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
         if (!once && hi <= 0) {  // on to the next chunk's rows
           walk(-1);
           rows = rows_at(c - 1);
-          load();
         }
       }
       if (w == NT - 1) {
         g = gn;
-        gn = load_gate<T>(s, bt, h, (c - 2) * CH, rows_at(c - 2), l);
+        gn = load_gate<T>(bt, h, (c - 2) * CH, rows_at(c - 2), l);
       }
       cur ^= 1;
     }
@@ -1437,12 +1473,9 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
     }
     if (LOCAL) {
 #pragma unroll
-      for (int m = 0; m < NT; m++) put_own_tile(tid, o.xi + (seg * s.units + unit_id) * Ku * Vu, Ku, Vu, m, w, dS[m]);
+      for (int m = 0; m < NT; m++) put_own_tile(tid, (gout<float>)o.xi + (seg * s.units + unit_id) * own.floats(), own, m, w, dS[m]);
     } else {
-      if (o.dh0 && seg == 0) {
-#pragma unroll
-        for (int m = 0; m < NT; m++) put_state_tile(tid, o.dh0 + unit_id * s.K * s.V, s.K, s.V, m, w, dS[m]);
-      }
+      if (o.dh0 && seg == 0) put_state<NT>(tid, (gout<float>)o.dh0 + unit_id * s.K * s.V, s.K, s.V, w, dS);
       if (w == NT - 1 && o.gpart) {
 #pragma unroll
         for (int e = 1; e < CH; e *= 2) {
