@@ -123,7 +123,7 @@ __device__ __forceinline__ float softplus(float v) {
   const float e = ex2(-fabsf(v) * (float)kLog2e), w = 1.f + e;
   return fmaxf(v, 0.f) + fmaf(__builtin_amdgcn_logf(w), (float)(1 / kLog2e), e - (w - 1.f));
 }
-__device__ __forceinline__ float sigma(float v) { return 1.f / (1.f + ex2(v * -(float)kLog2e)); }
+__device__ __forceinline__ float sigma(float v) { return __builtin_amdgcn_rcpf(1.f + ex2(v * -(float)kLog2e)); }
 // max and comparisons with a NaN drop it; a gate of NaN stays one
 __device__ __forceinline__ float log_decay(float A, float sp) {
   const float g = A * sp;
@@ -258,6 +258,7 @@ template <bool BF, int P, typename T = typename Elem<BF>::type>
 __device__ __forceinline__ u4 load_row(int tid, gin<T> p, int rows, int W) {
   constexpr int V = Elem<BF>::V;
   const int row = tid / (P / V), c = tid % (P / V) * V;
+  if (rows == Elem<BF>::CH && W == P) return *(gin<u4_any>)p;
   u4 r = {0, 0, 0, 0};
   if (row < rows && c < W) {
     const int over = c + V - W;
@@ -568,9 +569,9 @@ template <int NT, bool TR> __device__ __forceinline__ void get_state(int tid, gi
         if constexpr (TR) {
           S[m] = *(gin<f4_any>)(s + (16 * w + in) * V + 16 * m + four);
         } else {
-          gin<float> p = s + four * V + 16 * w + in;
+          const unsigned at = (four * V + in) * 4;
 #pragma unroll
-          for (int i = 0; i < 4; i++) S[m][i] = p[(16 * m + i) * V];
+          for (int i = 0; i < 4; i++) S[m][i] = *(gin<float>)((gin<char>)(s + (16 * m + i) * V + 16 * w) + at);
         }
       }
     }
@@ -591,6 +592,18 @@ template <int NT, bool TR> __device__ __forceinline__ void get_state(int tid, gi
 }
 template <int NT> __device__ __forceinline__ void put_state(int tid, gout<float> s, int K, int V, int w, const f4* S) {
   const int l = tid & 63, c = 16 * w + (l & 15), four = 4 * (l >> 4);
+  if (((K | V) & 15) == 0) {
+    const unsigned at = (four * V + (l & 15)) * 4;
+    if (16 * w < V) {
+#pragma unroll
+      for (int m = 0; m < NT; m++)
+        if (16 * m < K) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) *(gout<float>)((gout<char>)(s + (16 * m + i) * V + 16 * w) + at) = S[m][i];
+        }
+    }
+    return;
+  }
   if (c >= V) return;
 #pragma unroll
   for (int m = 0; m < NT; m++) {
@@ -602,10 +615,10 @@ template <int NT> __device__ __forceinline__ void put_state(int tid, gout<float>
 }
 
 template <bool BF, int P, typename T = typename Elem<BF>::type>
-__device__ __forceinline__ void put_row(int tid, T* tile, u4 r, int lo, int hi) {
+__device__ __forceinline__ void put_row(int tid, T* tile, u4 r, int lo, int hi, bool part) {
   constexpr int V = Elem<BF>::V, LD = P + Elem<BF>::pad;
   const int row = tid / (P / V), c = tid % (P / V) * V;
-  if (row < lo || row >= hi) r = u4{0, 0, 0, 0};
+  if (part && (row < lo || row >= hi)) r = u4{0, 0, 0, 0};
   *reinterpret_cast<u4*>(tile + row * LD + c) = r;
 }
 // 1 / sqrt(|row|^2 + eps) of the staged rows, 0 for those left out
@@ -618,17 +631,17 @@ template <bool BF, int P> __device__ __forceinline__ void put_norm(int tid, floa
   if constexpr (L >= 16) s += dpp_mov<0x140>(s);
   if constexpr (L >= 32) s += __shfl_xor(s, 16);
   const int row = tid / L;
-  if (tid % L == 0) out[row] = row >= lo && row < hi ? 1.f / sqrtf(s + kEps) : 0.f;
+  if (tid % L == 0) out[row] = row >= lo && row < hi ? __builtin_amdgcn_rsqf(s + kEps) : 0.f;
 }
 
 // ---- sequences ------------------------------------------------------------------------------------------
 // Wavefronts of a SIMD, at least: as many as registers and LDS leave room for.
 template <bool BF, int P> constexpr int fwd_waves() { return P == 128 ? 2 : 4; }
-template <bool BF, int P> constexpr int bwd_waves() { return P == 128 ? 2 : 3; }
+template <bool BF, int P> constexpr int bwd_waves() { return P == 32 || (P == 64 && !BF) ? 3 : 2; }
 
 // One segment of one sequence's head. LOCAL: without outputs, from a zero state (what the segment adds to its start state) or,
 // without values to write, from the unit matrix (what it multiplies it with).
-template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (fwd_waves<BF, P>())) k_delta_fwd(const Args s) {
+template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (fwd_waves<BF, P>())) k_delta_fwd(const Args args) {
   using T = typename Elem<BF>::type;
   using unit = typename Elem<BF>::unit;
   constexpr int CH = Elem<BF>::CH, NB = CH / 16, NT = P / 16, LD = P + Elem<BF>::pad, UD = CH + 4;
@@ -639,8 +652,9 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
   int tid = threadIdx.x, l = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
-  const long items = s.units * (LOCAL ? (s.segs - 1) * s.parts : s.segs);
-  for (long item = blockIdx.x; item < items; item += gridDim.x) {
+  for (long item = blockIdx.x;; item += gridDim.x) {
+    const Args s = again<Args>(0);
+    if (item >= s.units * (LOCAL ? (s.segs - 1) * s.parts : s.segs)) break;
     const unsigned units = (unsigned)s.units, round = (unsigned)item / units;
     const long unit_id = (unsigned)item - round * units;
     const int part = LOCAL ? (s.parts == 1 ? 1 : (int)round & 1) : 0;
@@ -653,8 +667,7 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
     gin<T> qp = thread_row<BF, P>(tid, (const T*)s.q + bt * s.q_b + hk * s.q_h, s.q_t, first);
     gin<T> kp = thread_row<BF, P>(tid, (const T*)s.k + bt * s.k_b + hk * s.k_h, s.k_t, first);
     gin<T> vp = thread_row<BF, P>(tid, (const T*)s.v + bt * s.v_b + h * s.v_h, s.v_t, first);
-    const int W_v = part ? 0 : s.V;
-    const float A = s.A[h];
+    const float A = s.A[h], scale = s.scale;
     auto rows_at = [&](long t0) { return (int)(t0 >= last ? 0 : last - t0 < CH ? last - t0 : CH); };
     f4 S[NT];
     if (LOCAL) {
@@ -681,9 +694,10 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
     int rows = rows_at(first);
     u4 q = {0, 0, 0, 0}, k, v;
     auto load = [&]() {
-      if (!LOCAL) q = load_row<BF, P>(tid, qp, rows, s.K);
-      k = load_row<BF, P>(tid, kp, rows, s.K);
-      v = load_row<BF, P>(tid, vp, rows, W_v);
+      const Args a = again<Args>(0);
+      if (!LOCAL) q = load_row<BF, P>(tid, qp, rows, a.K);
+      k = load_row<BF, P>(tid, kp, rows, a.K);
+      v = load_row<BF, P>(tid, vp, rows, part ? 0 : a.V);
     };
     auto walk = [&](int chunks) {
       const Args a = again<Args>(0);
@@ -727,9 +741,9 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
           y_hi = 0;
         }
         if (!have) load();  // the first ones, or one episode at a time again
-        if (!LOCAL) put_row<BF, P>(tid, Qs, q, lo, hi);
-        put_row<BF, P>(tid, Ks, k, lo, hi);
-        put_row<BF, P>(tid, Vs, v, lo, hi);
+        if (!LOCAL) put_row<BF, P>(tid, Qs, q, lo, hi, !once);
+        put_row<BF, P>(tid, Ks, k, lo, hi, !once);
+        put_row<BF, P>(tid, Vs, v, lo, hi, !once);
         if (!LOCAL) put_norm<BF, P>(tid, R.rq, q, lo, hi);
         put_norm<BF, P>(tid, R.rk, k, lo, hi);
         if (!once && w == NT - 1) fill_rows<CH>(tid, R, g, A, lo, hi);
@@ -744,7 +758,7 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
 #pragma unroll
           for (int m = 0; m < NT; m++) S[m] = zero;
         }
-        score_tiles<BF, P, LD, !LOCAL>(tid, R, Qs, Ks, X.M, X.P, diag, s.scale);
+        score_tiles<BF, P, LD, !LOCAL>(tid, R, Qs, Ks, X.M, X.P, diag, scale);
         __syncthreads();
         if (w == 0) invert_blocks<BF, CH>(tid, diag, X.Tinv);
         if (w == NT - 1 && once) fill_rows<CH>(tid, Rs[cur ^ 1], gn, A, 0, rows);
@@ -764,7 +778,7 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
             if constexpr (!LOCAL) {
 #pragma unroll
               for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, Qs, 16 * n, 16 * m);
-              O[n] = (s.scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n)) * (dot2<BF, NT>(x, Sp, zero));
+              O[n] = (scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n)) * (dot2<BF, NT>(x, Sp, zero));
             }
           }
         }
@@ -835,14 +849,15 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
       __syncthreads();
       put_y(y_at, y_lo, y_hi);
     }
+    const Args e = again<Args>(0);
     if (LOCAL) {
-      const long at = seg * s.units + unit_id;
-      gout<float> out = (gout<float>)(part ? s.phi : s.psi) + at * own.floats();
+      const long at = seg * e.units + unit_id;
+      gout<float> out = (gout<float>)(part ? e.phi : e.psi) + at * own.floats();
 #pragma unroll
       for (int m = 0; m < NT; m++) put_own_tile(tid, out, own, m, w, S[m]);
-      if (part && tid == 0) s.cut[at] = cut != 0;
-    } else if (s.h_out && last == s.T) {
-      put_state<NT>(tid, (gout<float>)s.h_out + unit_id * s.K * s.V, s.K, s.V, w, S);
+      if (part && tid == 0) e.cut[at] = cut != 0;
+    } else if (e.h_out && last == e.T) {
+      put_state<NT>(tid, (gout<float>)e.h_out + unit_id * e.K * e.V, e.K, e.V, w, S);
     }
   }
 }
@@ -990,7 +1005,7 @@ __device__ __forceinline__ float row16_sum(float v) {
 }
 
 template <bool BF, int P, bool LOCAL>
-__global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const Args s, const GradArgs o) {
+__global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const Args args, const GradArgs gargs) {
   using T = typename Elem<BF>::type;
   using unit = typename Elem<BF>::unit;
   using Lds = std::conditional_t<LOCAL, BwdLocalLds<BF, P>, BwdLds<BF, P>>;
@@ -1001,8 +1016,10 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
   int tid = threadIdx.x, l = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
-  const long items = s.units * (LOCAL ? s.segs - 1 : s.segs);
-  for (long item = blockIdx.x; item < items; item += gridDim.x) {
+  for (long item = blockIdx.x;; item += gridDim.x) {
+    const Args s = again<Args>(0);
+    const GradArgs o = again<GradArgs>(sizeof(Args));
+    if (item >= s.units * (LOCAL ? s.segs - 1 : s.segs)) break;
     const unsigned units = (unsigned)s.units, round = (unsigned)item / units;
     const long unit_id = (unsigned)item - round * units, seg = round + (LOCAL ? 1 : 0), bt = (unsigned)unit_id / (unsigned)s.H;
     const int h = (int)(unit_id - bt * s.H), hk = (int)((unsigned)h / (unsigned)(s.H / s.Hk));
@@ -1013,8 +1030,9 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
     gin<T> kp = thread_row<BF, P>(tid, (const T*)s.k + bt * s.k_b + hk * s.k_h, s.k_t, c * CH);
     gin<T> vp = thread_row<BF, P>(tid, (const T*)s.v + bt * s.v_b + h * s.v_h, s.v_t, c * CH);
     gin<T> op = thread_row<BF, P>(tid, (const T*)o.dy + bt * o.dy_b + h * o.dy_h, o.dy_t, c * CH);
-    const float A = s.A[h];
-    auto rows_at = [&](long ch) { return (int)(ch < c_first ? 0 : s.T - ch * CH < CH ? s.T - ch * CH : CH); };
+    const float A = s.A[h], scale = s.scale;
+    const long steps = s.T;
+    auto rows_at = [&](long ch) { return (int)(ch < c_first ? 0 : steps - ch * CH < CH ? steps - ch * CH : CH); };
     double sumA = 0.0, sumB = 0.0;  // of the lanes that see to the gates
     f4 dS[NT], dSt[LOCAL ? 1 : NT];
     if (!LOCAL && s.segs > 1) {
@@ -1041,10 +1059,11 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
     int rows = rows_at(c);
     u4 q, k, v = {0, 0, 0, 0}, d;
     auto load = [&]() {
-      q = load_row<BF, P>(tid, qp, rows, s.K);
-      k = load_row<BF, P>(tid, kp, rows, s.K);
-      if (!LOCAL) v = load_row<BF, P>(tid, vp, rows, s.V);
-      d = load_row<BF, P>(tid, op, rows, s.V);
+      const Args a = again<Args>(0);
+      q = load_row<BF, P>(tid, qp, rows, a.K);
+      k = load_row<BF, P>(tid, kp, rows, a.K);
+      if (!LOCAL) v = load_row<BF, P>(tid, vp, rows, a.V);
+      d = load_row<BF, P>(tid, op, rows, a.V);
     };
     auto walk = [&](int chunks) {
       const Args a = again<Args>(0);
@@ -1054,11 +1073,17 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
       vp += chunks * CH * a.v_t;
       op += chunks * CH * b.dy_t;
     };
+    bool have = false;  // this chunk's rows are there
+    auto next = [&]() {  // the next chunk's rows are on their way while this one computes
+      walk(-1);
+      rows = rows_at(c - 1);
+      load();
+      have = true;
+    };
     auto keep_at = [&](long ch) {
       const Args a = again<Args>(0);
       return (gin<float>)again<GradArgs>(sizeof(Args)).keep + (ch * a.units + unit_id) * own.floats();
     };
-    bool have = false;  // this chunk's rows are there
     // the last wavefront sees to the gates, a chunk ahead
     Gate g = {0.f, 0.f, 0.f}, gn = g;
     if (w == NT - 1) {
@@ -1090,11 +1115,12 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
           y_hi = 0;
         }
         if (!have) load();  // the first ones, or one episode at a time again
+        have = false;
         const bool odd = tid / (P / Elem<BF>::V) >= lo && tid / (P / Elem<BF>::V) < hi && (!all_finite<BF>(q) || !all_finite<BF>(d));
-        put_row<BF, P>(tid, L.Q, q, lo, hi);
-        put_row<BF, P>(tid, L.K, k, lo, hi);
-        if constexpr (!LOCAL) put_row<BF, P>(tid, L.V, v, lo, hi);
-        put_row<BF, P>(tid, L.dO, d, lo, hi);
+        put_row<BF, P>(tid, L.Q, q, lo, hi, !once);
+        put_row<BF, P>(tid, L.K, k, lo, hi, !once);
+        if constexpr (!LOCAL) put_row<BF, P>(tid, L.V, v, lo, hi, !once);
+        put_row<BF, P>(tid, L.dO, d, lo, hi, !once);
         put_norm<BF, P>(tid, R.rq, q, lo, hi);
         put_norm<BF, P>(tid, R.rk, k, lo, hi);
         if (!once && w == NT - 1) fill_rows<CH>(tid, R, g, A, lo, hi);
@@ -1104,45 +1130,43 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
           for (int m = 0; m < NT; m++) S0[m] = own_tile(tid, keep_at(c), own, m, w);
         }
         __syncthreads();
-        have = once;
-        if (once) {  // the next chunk's are on their way while this one computes
-          walk(-1);
-          rows = rows_at(c - 1);
-          load();
-        }
         const bool fresh = R.starts >> lo & 1;  // S_0 may be anything
-        score_tiles<BF, P, LD, true>(tid, R, L.Q, L.K, L.M, L.Pm, L.diag, s.scale);
+        score_tiles<BF, P, LD, true>(tid, R, L.Q, L.K, L.M, L.Pm, L.diag, scale);
         __syncthreads();
         if (w == 0) invert_blocks<BF, CH>(tid, L.diag, L.Tinv);
-        if (w == NT - 1 && once) fill_rows<CH>(tid, L.R[cur ^ 1], gn, A, 0, rows);
+        if (w == NT - 1 && once) fill_rows<CH>(tid, L.R[cur ^ 1], gn, A, 0, rows_at(c - 1));
+        // contractions over the state's rows, HT tiles at a time: all of a wide state's operands would not fit the registers
+        constexpr int HT = NT < 4 ? NT : 4;
         f4 Y[NB], dU[NB], sd = zero;
-        {
-          Pair<BF> Sp[NT];
-          if constexpr (!LOCAL) {
 #pragma unroll
-            for (int m = 0; m < NT; m++) {
-              if (fresh) S0[m] = zero;
-              sd += S0[m] * dS[m];
-              Sp[m].set(S0[m]);
+        for (int n = 0; n < NB; n++) Y[n] = dU[n] = zero;
+#pragma unroll
+        for (int m0 = 0; m0 < NT; m0 += HT) {
+          Pair<BF> Sp[HT], Dp[HT];
+#pragma unroll
+          for (int m = 0; m < HT; m++) {
+            if constexpr (!LOCAL) {
+              if (fresh) S0[m0 + m] = zero;
+              sd += S0[m0 + m] * dS[m0 + m];
+              Sp[m].set(S0[m0 + m]);
             }
-#pragma unroll
-            for (int n = 0; n < NB; n++) {
-              unit x[NT];
-#pragma unroll
-              for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, L.K, 16 * n, 16 * m);
-              Y[n] = rows4(tid, R.be, 16 * n) * (widen(col_unit<LD>(tid, L.V, 16 * n, 16 * w)) -
-                                            (rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n)) * (dot2<BF, NT>(x, Sp, zero)));
-            }
+            Dp[m].set(dS[m0 + m]);
           }
-#pragma unroll
-          for (int m = 0; m < NT; m++) Sp[m].set(dS[m]);
 #pragma unroll
           for (int n = 0; n < NB; n++) {
-            unit x[NT];
+            unit x[HT];
 #pragma unroll
-            for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, L.K, 16 * n, 16 * m);
-            dU[n] = (rows4(tid, R.dc, 16 * n) * rows4(tid, R.rk, 16 * n)) * (dot2<BF, NT>(x, Sp, zero));
+            for (int m = 0; m < HT; m++) x[m] = row_unit<LD>(tid, L.K, 16 * n, 16 * (m0 + m));
+            if constexpr (!LOCAL) Y[n] = dot2<BF, HT>(x, Sp, Y[n]);
+            dU[n] = dot2<BF, HT>(x, Dp, dU[n]);
           }
+        }
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+          const f4 rk = rows4(tid, R.rk, 16 * n);
+          if constexpr (!LOCAL)
+            Y[n] = rows4(tid, R.be, 16 * n) * (widen(col_unit<LD>(tid, L.V, 16 * n, 16 * w)) - rows4(tid, R.d0, 16 * n) * rk * Y[n]);
+          dU[n] = rows4(tid, R.dc, 16 * n) * rk * dU[n];
         }
         __syncthreads();
         renew(tid, l);
@@ -1173,9 +1197,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
 #pragma unroll
             for (int i = 0; i < 4; i++) bad |= (!LOCAL && !finite(U[n][i])) || !finite(dY[n][i]);
           if (__syncthreads_or(bad)) {
-            if (once) walk(1);
             have = false;
-            rows = all;
             lo = 31 - __clz(inside);
             continue;
           }
@@ -1193,6 +1215,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             }
           }
         }
+        if (LOCAL && once) next();
         const float c0 = R.c0;
         float tot = c0 == 0.f ? 0.f : c0 * (sd[0] + sd[1] + sd[2] + sd[3]);
         // dS of the chunk's start; the transposed one below, when its old values have been used
@@ -1200,7 +1223,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
           Pair<BF> x[NB], y[NB];
 #pragma unroll
           for (int n = 0; n < NB; n++) {
-            x[n].set((s.scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n)) * (widen(dOc[n])));
+            x[n].set((scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n)) * (widen(dOc[n])));
             y[n].set((-rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n) * rows4(tid, R.be, 16 * n)) * (dY[n]));
           }
 #pragma unroll
@@ -1215,7 +1238,6 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
           }
         }
         if constexpr (!LOCAL) {
-          Pair<BF> Xt[NT];  // S_0 transposed, then dS
 #pragma unroll
           for (int m = 0; m < NT; m++) S0[m] = own_tile_t(tid, keep_at(c), own, m, w);
           __syncthreads();
@@ -1223,18 +1245,18 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
           for (int tile = w; tile < TILES; tile += NT) {
             const int bi = tile == 0 ? 0 : 1, bj = tile == 2 ? 1 : 0;  // (0,0) (1,0) (1,1)
             f4 e = zero, f = zero;
-            {
-              Pair<BF> y[NT], x[NT];
-              unit z[NT];
 #pragma unroll
-              for (int m = 0; m < NT; m++) {
-                y[m] = col_pair<BF, UD>(tid, L.U, L.Ulo, 16 * m, 16 * bj);
-                z[m] = row_unit<LD>(tid, L.dO, 16 * bi, 16 * m);
+            for (int m0 = 0; m0 < NT; m0 += HT) {
+              Pair<BF> y[HT], x[HT];
+              unit z[HT];
+#pragma unroll
+              for (int m = 0; m < HT; m++) {
+                y[m] = col_pair<BF, UD>(tid, L.U, L.Ulo, 16 * (m0 + m), 16 * bj);
+                z[m] = row_unit<LD>(tid, L.dO, 16 * bi, 16 * (m0 + m));
+                x[m] = col_pair<BF, UD>(tid, L.dY, L.dYlo, 16 * (m0 + m), 16 * bi);
               }
-              e = dot2<BF, NT>(z, y, e);
-#pragma unroll
-              for (int m = 0; m < NT; m++) x[m] = col_pair<BF, UD>(tid, L.dY, L.dYlo, 16 * m, 16 * bi);
-              f = dot3<BF, NT>(x, y, f);
+              e = dot2<BF, HT>(z, y, e);
+              f = dot3<BF, HT>(x, y, f);
             }
             const int j = 16 * bj + (l & 15);
             const double Gj = R.G[j];
@@ -1247,7 +1269,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
               const bool on = segj == R.seg[i] && j <= i;
               const float dec = ex2((float)(R.G[i] - Gj));
               L.W[i * CP + j] = on && j < i ? pv[i4] * e[i4] - mv[i4] * f[i4] : 0.f;
-              e[i4] = on ? dec * s.scale * e[i4] : 0.f;
+              e[i4] = on ? dec * scale * e[i4] : 0.f;
               f[i4] = on && j < i ? -dec * be[i4] * f[i4] : 0.f;
             }
             put_mat<BF, UD>(tid, L.Pm, 16 * bj, 16 * bi, e);
@@ -1257,28 +1279,38 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
           // products over V for this wavefront's columns of K: dO S_0^T, dY S_0^T, U dS^T
           f4 X1[NB], X2[NB], X3[NB];
 #pragma unroll
-          for (int m = 0; m < NT; m++) Xt[m].set(fresh ? zero : S0[m]);
+          for (int n = 0; n < NB; n++) X1[n] = X2[n] = X3[n] = zero;
 #pragma unroll
-          for (int n = 0; n < NB; n++) {
-            unit x[NT];
+          for (int m0 = 0; m0 < NT; m0 += HT) {
+            Pair<BF> St[HT], Dt[HT];
 #pragma unroll
-            for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, L.dO, 16 * n, 16 * m);
-            X1[n] = (s.scale * rows4(tid, R.d0, 16 * n)) * (dot2<BF, NT>(x, Xt, zero));
-            Pair<BF> y[NT];
+            for (int m = 0; m < HT; m++) {
+              St[m].set(fresh ? zero : S0[m0 + m]);
+              Dt[m].set(dSt[m0 + m]);
+            }
 #pragma unroll
-            for (int m = 0; m < NT; m++) y[m] = col_pair<BF, UD>(tid, L.dY, L.dYlo, 16 * m, 16 * n);
-            X2[n] = (-rows4(tid, R.d0, 16 * n) * rows4(tid, R.be, 16 * n)) * (dot3<BF, NT>(y, Xt, zero));
+            for (int n = 0; n < NB; n++) {
+              unit x[HT];
+#pragma unroll
+              for (int m = 0; m < HT; m++) x[m] = row_unit<LD>(tid, L.dO, 16 * n, 16 * (m0 + m));
+              X1[n] = dot2<BF, HT>(x, St, X1[n]);
+              Pair<BF> y[HT];
+#pragma unroll
+              for (int m = 0; m < HT; m++) y[m] = col_pair<BF, UD>(tid, L.dY, L.dYlo, 16 * (m0 + m), 16 * n);
+              X2[n] = dot3<BF, HT>(y, St, X2[n]);
+#pragma unroll
+              for (int m = 0; m < HT; m++) y[m] = col_pair<BF, UD>(tid, L.U, L.Ulo, 16 * (m0 + m), 16 * n);
+              X3[n] = dot3<BF, HT>(y, Dt, X3[n]);
+            }
           }
 #pragma unroll
-          for (int m = 0; m < NT; m++) Xt[m].set(dSt[m]);
-#pragma unroll
           for (int n = 0; n < NB; n++) {
-            Pair<BF> y[NT];
-#pragma unroll
-            for (int m = 0; m < NT; m++) y[m] = col_pair<BF, UD>(tid, L.U, L.Ulo, 16 * m, 16 * n);
-            X3[n] = (rows4(tid, R.dc, 16 * n)) * (dot3<BF, NT>(y, Xt, zero));
+            const f4 d0 = rows4(tid, R.d0, 16 * n);
+            X1[n] = scale * d0 * X1[n];
+            X2[n] = -d0 * rows4(tid, R.be, 16 * n) * X2[n];
+            X3[n] = rows4(tid, R.dc, 16 * n) * X3[n];
           }
-          renew(tid, l);
+        renew(tid, l);
           unit Kc[NB], Qc[NB];  // this wavefront's columns of K and Q
 #pragma unroll
           for (int n = 0; n < NB; n++) {
@@ -1289,7 +1321,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             Pair<BF> x[NB], y[NB];
 #pragma unroll
             for (int n = 0; n < NB; n++) {
-              x[n].set((s.scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n)) * (widen(Qc[n])));
+              x[n].set((scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n)) * (widen(Qc[n])));
               y[n].set((-rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n) * rows4(tid, R.be, 16 * n)) * (widen(Kc[n])));
             }
 #pragma unroll
@@ -1306,6 +1338,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
           }
           __syncthreads();
         renew(tid, l);
+          if (once) next();
           // E K^, F K^ (rows as i), F^T K^, E^T Q^ (rows as j): E and F rest where P and M were
           f4 dQ[NB], dK[NB];
           {
@@ -1391,20 +1424,25 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             f4 dv;
             if constexpr (BF) dv = be * (widen(dy.hi) + widen(dy.lo));
             else dv = be * dy.hi;
+            if (a.qpart) {
+              const unsigned step = (unsigned)(sa.H * sa.K);  // elements of a sequence's step
+              const long to = (((t0 + 16 * n + 4 * (l >> 4)) * sa.B + bt) * sa.H + h) * sa.K + col;
+#pragma unroll 1
+              for (int i = 0; i < 4; i++) {
+                const int row = 16 * n + 4 * (l >> 4) + i;
+                if (row >= lo && row < hi && col < sa.K) {
+                  const float x = i == 0 ? dq[0] : i == 1 ? dq[1] : i == 2 ? dq[2] : dq[3], z = i == 0 ? dk[0] : i == 1 ? dk[1] : i == 2 ? dk[2] : dk[3];
+                  ((gout<float>)a.qpart)[to + (long)i * sa.B * step] = x;
+                  ((gout<float>)a.kpart)[to + (long)i * sa.B * step] = z;
+                }
+              }
+            }
+            const int at = (16 * n + 4 * (l >> 4)) * LD + col;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-              const int row = 16 * n + 4 * (l >> 4) + i, at = row * LD + col;
-              stf(L.dO + at, dv[i]);
-              if (a.qpart) {
-                if (row >= lo && row < hi && col < sa.K) {
-                  const long to = (((t0 + row) * sa.B + bt) * sa.H + h) * sa.K + col;
-                  ((gout<float>)a.qpart)[to] = dq[i];
-                  ((gout<float>)a.kpart)[to] = dk[i];
-                }
-              } else {
-                stf(L.Q + at, dq[i]);
-                stf(L.K + at, dk[i]);
-              }
+              stf(L.dO + at + i * LD, dv[i]);
+              stf(L.Q + at + i * LD, dq[i]);
+              stf(L.K + at + i * LD, dk[i]);
             }
           }
           y_at = t0;
@@ -1471,21 +1509,23 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
       __syncthreads();
       put_grads(y_at, y_lo, y_hi);
     }
+    const Args e = again<Args>(0);
+    const GradArgs eo = again<GradArgs>(sizeof(Args));
     if (LOCAL) {
 #pragma unroll
-      for (int m = 0; m < NT; m++) put_own_tile(tid, (gout<float>)o.xi + (seg * s.units + unit_id) * own.floats(), own, m, w, dS[m]);
+      for (int m = 0; m < NT; m++) put_own_tile(tid, (gout<float>)eo.xi + (seg * e.units + unit_id) * own.floats(), own, m, w, dS[m]);
     } else {
-      if (o.dh0 && seg == 0) put_state<NT>(tid, (gout<float>)o.dh0 + unit_id * s.K * s.V, s.K, s.V, w, dS);
-      if (w == NT - 1 && o.gpart) {
+      if (eo.dh0 && seg == 0) put_state<NT>(tid, (gout<float>)eo.dh0 + unit_id * e.K * e.V, e.K, e.V, w, dS);
+      if (w == NT - 1 && eo.gpart) {
 #pragma unroll
-        for (int e = 1; e < CH; e *= 2) {
-          sumA += __shfl_xor(sumA, e);
-          sumB += __shfl_xor(sumB, e);
+        for (int d2 = 1; d2 < CH; d2 *= 2) {
+          sumA += __shfl_xor(sumA, d2);
+          sumB += __shfl_xor(sumB, d2);
         }
         if (l == 0) {
-          const long n = s.segs * s.B, at = seg * s.B + bt;
-          o.gpart[(long)h * n + at] = (float)sumA;
-          o.gpart[((long)s.H + h) * n + at] = (float)sumB;
+          const long n = e.segs * e.B, at = seg * e.B + bt;
+          eo.gpart[(long)h * n + at] = (float)sumA;
+          eo.gpart[((long)e.H + h) * n + at] = (float)sumB;
         }
       }
     }
@@ -1577,7 +1617,7 @@ __global__ void __launch_bounds__(256) k_delta_step(const Args s, float* __restr
       qq = fmaf(qv[i], qv[i], qq);
     }
     group_sum<64>(kk, qq);
-    const float rk = 1.f / sqrtf(kk + kEps), rq = 1.f / sqrtf(qq + kEps);
+    const float rk = __builtin_amdgcn_rsqf(kk + kEps), rq = __builtin_amdgcn_rsqf(qq + kEps);
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       sh[w][0][l + 64 * i] = kv[i] * rk;
