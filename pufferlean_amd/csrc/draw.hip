@@ -2,13 +2,15 @@
 //
 // What the filters leave is every entry above a threshold key, and of those at the threshold the ones up to an index:
 // top-k's threshold is the k-th largest key, top-p's the one at which the mass of the larger ones reaches p of the total.
-// Neither needs the row sorted: a key is a 32-bit number that orders like the logit, and the threshold is found digit by
-// digit from the top, by how much (count, or mass) lies at and above each value of the digit. A whole row is then summed up in the
-// order of its indices to where the sum exceeds u times the total.
+// Neither needs the row sorted: a key is a 32-bit number that orders like the logit; the keys among which the threshold lies are
+// narrowed down by how much (count, or mass) is above some, until few enough are left to be compared with each other. What is
+// left of the row is then summed up in the order of its indices to where the sum exceeds u times the total.
 //
-// Masses are exp((l - max) / temperature) in 64-bit floating point, held as whole numbers of 2^-bits with as many bits as the
+// Masses are exp((l - max) / temperature) from 64-bit floating point, held as whole numbers of 2^-bits with as many bits as the
 // sum of A of them has room for (45 at 131072 entries, 51 up to 2048): sums do not depend on their order, so the
 // borders that u and p are compared with are the same however the row is split.
+//
+// Bound by vector instructions, the 64-bit exponential (some 25 of them) of each entry first.
 #include "common.hpp"
 #include "kernels.hpp"
 #include "lanes.hpp"
@@ -33,7 +35,7 @@ __device__ __forceinline__ float logit_of(uint32_t k) {
 
 // A row's parameters, with the filters that are off in a form that lets everything pass.
 struct Par {
-  double t, p;
+  double c, p;  // log2(e) / temperature
   float minp, u;
   long k;
   bool greedy;
@@ -50,7 +52,7 @@ struct DrawArgs {
 __device__ __forceinline__ Par par_of(const DrawArgs& a, long n) {
   Par r;
   const float t = a.temperature ? a.temperature[n] : 1.f, p = a.top_p ? a.top_p[n] : 1.f, m = a.min_p ? a.min_p[n] : 0.f;
-  r.t = t > 0.f ? (double)t : 1.0;
+  r.c = 1.4426950408889634074 / (t > 0.f ? (double)t : 1.0);
   r.k = a.top_k && a.top_k[n] > 0 ? a.top_k[n] : a.A;
   r.greedy = t == 0.f || p <= 0.f;
   r.p = p < 1.f ? (double)p : 1.0;
@@ -58,12 +60,42 @@ __device__ __forceinline__ Par par_of(const DrawArgs& a, long n) {
   r.u = a.u[n];
   return r;
 }
-// The mass of a key in units of 2^-bits; nothing below min_p.
-__device__ __forceinline__ double mass_of(uint32_t key, uint32_t top, double t) {
-  if (key == top) return 1.0;
-  return exp(((double)logit_of(key) - (double)logit_of(top)) / t);
+// 2^y for y <= 0 as a factor in 0.7..1.42 and an exponent: exp by its series, to z^12 for |z| <= ln 2 / 2 (what is left out is
+// below 2^-52).
+struct Mass {
+  double r;
+  int n;
+};
+__device__ __forceinline__ Mass mass_of(uint32_t key, uint32_t top, double c) {  // c = log2(e) / temperature
+  const double d = (double)logit_of(key) - (double)logit_of(top);
+  double y = d * c;
+  y = y > -1000.0 ? y : -1000.0;
+  const double n = rint(y), z = (y - n) * 0.6931471805599453094;
+  double p = 1.0 / 479001600;
+  p = fma(p, z, 1.0 / 39916800);
+  p = fma(p, z, 1.0 / 3628800);
+  p = fma(p, z, 1.0 / 362880);
+  p = fma(p, z, 1.0 / 40320);
+  p = fma(p, z, 1.0 / 5040);
+  p = fma(p, z, 1.0 / 720);
+  p = fma(p, z, 1.0 / 120);
+  p = fma(p, z, 1.0 / 24);
+  p = fma(p, z, 1.0 / 6);
+  p = fma(p, z, 0.5);
+  p = fma(p, z, 1.0);
+  p = fma(p, z, 1.0);
+  Mass m = {p, (int)n};
+  if (key == top) m = {1.0, 0};  // of an infinite logit too, whose difference is none
+  return m;
 }
-__device__ __forceinline__ u64 units(double e, int bits) { return (u64)__double2ll_rn(ldexp(e, bits)); }
+// In units of 2^-bits, to the nearest.
+__device__ __forceinline__ u64 units(Mass m, int bits) {
+  const u64 b = __builtin_bit_cast(u64, m.r);
+  const int shift = 52 - ((int)(b >> 52) - 1023) - m.n - bits;  // the double's sign is 0
+  const u64 f = (b & 0xfffffffffffffull) | 0x10000000000000ull;
+  return shift > 53 ? 0 : (f + (1ull << (shift - 1))) >> shift;
+}
+__device__ __forceinline__ bool reaches(Mass m, float minp) { return minp == 0.f || ldexp(m.r, m.n) >= (double)minp; }
 
 // ---- sums over a wavefront --------------------------------------------------------------------------------
 template <int CTL> __device__ __forceinline__ u64 dpp64(u64 v) {
@@ -105,10 +137,18 @@ __device__ __forceinline__ u64 wave_scan(u64 v) {  // inclusive
   return v;
 }
 
+// Order of two entries: the larger key, of equal ones the lower index.
+__device__ __forceinline__ u64 order_of(uint32_t key, uint32_t index) { return (u64)key << 32 | (0xffffffffu - index); }
+
 // ---- rows in the registers of a wavefront ---------------------------------------------------------------------
-// Entry 64 e + lane in register e; the digits are single bits, a count or sum over the wavefront each.
+// Entry 64 e + lane in register e.
+struct WaveLds {
+  u64 order[64], mass[64];
+};
 template <typename T, int E> __global__ void __launch_bounds__(256) k_draw_wave(const DrawArgs a) {
+  __shared__ WaveLds lds[4];
   const int l = threadIdx.x & 63;
+  WaveLds& L = lds[threadIdx.x >> 6];
   for (long n = (long)blockIdx.x * 4 + (threadIdx.x >> 6); n < a.N; n += (long)gridDim.x * 4) {
     const T* row = (const T*)a.x + n * a.ld;
     uint32_t key[E], top = 0;
@@ -118,8 +158,8 @@ template <typename T, int E> __global__ void __launch_bounds__(256) k_draw_wave(
       key[e] = i < a.A ? key_of(ldf(row + i)) : 0;
       top = key[e] > top ? key[e] : top;
     }
-    top = wave_max(top);
     const Par par = par_of(a, n);
+    top = wave_max(top);
     int act = -1;
     float logp = -INFINITY;
     // the entries at `key` in the order of their indices: the index of the count-th (from 1)
@@ -146,10 +186,10 @@ template <typename T, int E> __global__ void __launch_bounds__(256) k_draw_wave(
       uint32_t thr = 1;
       int cut = a.A;
       auto left = [&](int e) { return key[e] > thr || (key[e] == thr && 64 * e + l <= cut); };
-      if (par.k < a.A) {
+      if (E > 1 && par.k < a.A) {
         uint32_t cur = 0;
         long at_least = 0;
-        for (int bit = 31; bit >= 0; bit--) {
+        for (int bit = 31; bit >= (sizeof(T) == 2 ? 16 : 0); bit--) {
           const uint32_t c = cur | (1u << bit);
           long cnt = 0;
 #pragma unroll
@@ -160,6 +200,7 @@ template <typename T, int E> __global__ void __launch_bounds__(256) k_draw_wave(
           }
         }
         if (cur) {  // else there are fewer than k
+          if (sizeof(T) == 2) cur |= cur >> 31 ? 0 : 0xffff;  // of a bf16 logit the key's lower half goes by its sign
           thr = cur;
           if (at_least > par.k) {
             long above = 0;
@@ -169,63 +210,129 @@ template <typename T, int E> __global__ void __launch_bounds__(256) k_draw_wave(
           }
         }
       }
-      u64 m[E];
-      u64 total = 0;
+      Mass r[E];
+      u64 m[E], total = 0;
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        m[e] = key[e] && left(e) ? units(mass_of(key[e], top, par.t), a.bits) : 0;
+        r[e] = mass_of(key[e], top, par.c);
+        m[e] = key[e] && left(e) ? units(r[e], a.bits) : 0;
         total += m[e];
       }
-      if (par.p < 1.0) {
+      // of at most 64 entries in LDS, lane i's: how many and how much mass is in front of it
+      auto compare = [&](int count, u64 mine, int& rank, u64& before) {
+        for (int j = 0; j < count; j++) {
+          const bool first = L.order[j] > mine;
+          rank += first;
+          before += first ? L.mass[j] : 0;
+        }
+      };
+      if constexpr (E == 1) {
+        if (par.k < a.A || par.p < 1.0) {
+          const u64 mine = order_of(key[0], l);
+          L.order[l] = mine;
+          L.mass[l] = m[0];
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          int rank = 0;
+          u64 before = 0;
+          compare(a.A, mine, rank, before);
+          if (rank >= par.k) m[0] = 0;
+          if (par.p < 1.0) {
+            const u64 want = (u64)ceil(par.p * (double)wave_sum(m[0]));
+            if (before >= want) m[0] = 0;
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+      } else if (par.p < 1.0) {
         total = wave_sum(total);
         const u64 want = (u64)ceil(par.p * (double)total);
-        auto above = [&](uint32_t c) {  // mass of the keys over c
-          u64 s = 0;
+        // the threshold lies in lo + 1..hi: at least `want` is above lo, less above hi
+        uint32_t lo = thr - 1, hi = top;
+        long over_lo = (long)a.A, over_hi = 0;  // entries above them
+        u64 above_hi = 0;
+        while (over_lo - over_hi > 64 && hi - lo > 1) {
+          const uint32_t mid = lo + (hi - lo) / 2;
+          u64 sum = 0;
+          long cnt = 0;
 #pragma unroll
-          for (int e = 0; e < E; e++) s += key[e] > c ? m[e] : 0;
-          return wave_sum(s);
-        };
-        uint32_t cur = 0;
-        for (int bit = 31; bit >= 0; bit--) {
-          const uint32_t c = cur | (1u << bit);
-          if (above(c) >= want) cur = c;
+          for (int e = 0; e < E; e++) {
+            const bool on = key[e] > mid;
+            sum += on ? m[e] : 0;
+            cnt += __popcll(__ballot(on));
+          }
+          sum = wave_sum(sum);
+          if (sum >= want) {
+            lo = mid;
+            over_lo = cnt;
+          } else {
+            hi = mid;
+            over_hi = cnt;
+            above_hi = sum;
+          }
         }
-        cur += 1;  // the smallest key with less than that above it
-        const u64 each = units(mass_of(cur, top, par.t), a.bits), rest = want - above(cur);
-        const u64 count = each ? (rest + each - 1) / each : 1;
-        const int at = index_at(cur, (long)count);
-        if (cur > thr) cut = a.A;
-        thr = cur;
-        cut = at < cut ? at : cut;
+        int count = 0;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          const bool on = key[e] > lo && key[e] <= hi && m[e];
+          const u64 all = __ballot(on);
+          const int at = count + __popcll(all & ((1ull << l) - 1));
+          if (on && at < 64) {
+            L.order[at] = order_of(key[e], 64 * e + l);
+            L.mass[at] = m[e];
+          }
+          count += __popcll(all);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (count <= 64) {
+          const u64 mine = l < count ? L.order[l] : 0;
+          int rank = 0;
+          u64 before = above_hi;
+          compare(count, mine, rank, before);
+          const u64 kept = __ballot(l < count && before < want);
+          const int last = __ffsll((unsigned long long)__ballot(l < count && rank == __popcll(kept) - 1)) - 1;
+          const u64 o = __shfl(mine, last);
+          thr = (uint32_t)(o >> 32);
+          cut = (int)(0xffffffffu - (uint32_t)o);
+        } else {  // equal ones, of which the first few are left (top-k may have cut them already)
+          const u64 each = units(mass_of(hi, top, par.c), a.bits), of = (want - above_hi + each - 1) / each;
+          const int at = index_at(hi, (long)of);
+          if (hi > thr) cut = a.A;
+          thr = hi;
+          cut = at < cut ? at : cut;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       }
-      // in the order of the indices
-      u64 sums[E];
-      total = 0;
+      // in the order of the indices: through[e] is the lane's share of the first e + 1 registers
+      u64 through[E], run = 0;
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        const bool on = key[e] && left(e) && (par.minp == 0.f || mass_of(key[e], top, par.t) >= (double)par.minp);
-        m[e] = on ? m[e] : 0;
-        sums[e] = wave_sum(m[e]);
-        total += sums[e];
+        if (!(left(e) && reaches(r[e], par.minp))) m[e] = 0;
+        run += m[e];
+        through[e] = run;
       }
+      total = wave_sum(run);
       const u64 target = (u64)((double)par.u * (double)total);  // a sum exceeds u total where it exceeds this
-      u64 run = 0, got = 0;
-      bool open = true;
+      int tile = 0;  // registers that end at or below the target
+      run = 0;
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        if (sums[e] == 0 || !open) continue;
-        if (run + sums[e] > target || run + sums[e] == total) {
-          const u64 at = run + wave_scan(m[e]);
-          u64 hit = __ballot(m[e] > 0 && at > target);
-          if (!hit) hit = 1ull << (63 - __clzll((long long)__ballot(m[e] > 0)));  // u rounded up to 1: the last
-          const int lane = __ffsll((unsigned long long)hit) - 1;
-          act = 64 * e + lane;
-          got = __shfl(m[e], lane);
-          open = false;
+      for (int step = E / 2; step > 0; step /= 2) {
+        u64 x = 0;
+#pragma unroll
+        for (int e = 0; e < E; e++) x = e == tile + step - 1 ? through[e] : x;
+        x = wave_sum(x);
+        if (x <= target && x < total) {
+          tile += step;
+          run = x;
         }
-        run += sums[e];
       }
-      logp = (float)log((double)got / (double)total);
+      u64 mine = 0;
+#pragma unroll
+      for (int e = 0; e < E; e++) mine = e == tile ? m[e] : mine;
+      const u64 at = run + wave_scan(mine);
+      u64 hit = __ballot(mine > 0 && at > target);
+      if (!hit) hit = 1ull << (63 - __clzll((long long)__ballot(mine > 0)));  // u rounded up to 1: the last
+      const int lane = __ffsll((unsigned long long)hit) - 1;
+      act = 64 * tile + lane;
+      logp = (float)log((double)__shfl(mine, lane) / (double)total);
     }
     if (l == 0) {
       a.act[n] = act;
@@ -235,20 +342,21 @@ template <typename T, int E> __global__ void __launch_bounds__(256) k_draw_wave(
 }
 
 // ---- wide rows: a block each ----------------------------------------------------------------------------------
-// Digits of 11, 11 and 10 bits, each by a histogram in LDS.
-constexpr int kWide = 1024, kBins = 2048;
+// The wavefronts take a part of the row each, lanes 16 bytes at a time.
+constexpr int kWide = 1024, kBins = 2048, kList = 1024;
 
 struct WideLds {
-  u64 bins[kBins], wave[16], out[2];
+  u64 bins[kBins], wave[16], above;
+  u64 order[kList], mass[kList];
   uint32_t key;
-  int found;
+  int found, count;
 };
 
 // The largest bin b with sum(bins[b..]) >= want, in every thread: found, and above = sum(bins[b + 1 ..]). Every thread calls.
 __device__ __forceinline__ void pick_bin(WideLds& L, int nbins, u64 want, int& bin, u64& above) {
   const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
   __syncthreads();
-  if (tid == 0) L.found = 0, L.out[0] = 0;
+  if (tid == 0) L.found = 0, L.above = 0;
   // thread t has the bins nbins - 1 - 2 t and the one below
   const int b0 = nbins - 1 - 2 * tid;
   const u64 x0 = b0 >= 0 ? L.bins[b0] : 0, x1 = b0 >= 1 ? L.bins[b0 - 1] : 0;
@@ -260,33 +368,77 @@ __device__ __forceinline__ void pick_bin(WideLds& L, int nbins, u64 want, int& b
   if (before < want) {
     if (before + x0 >= want) {
       L.found = b0;
-      L.out[0] = before;
+      L.above = before;
     } else if (before + x0 + x1 >= want) {
       L.found = b0 - 1;
-      L.out[0] = before + x0;
+      L.above = before + x0;
     }
   }
   __syncthreads();
   bin = L.found;
-  above = L.out[0];
+  above = L.above;
 }
+
+template <typename T> struct Row {
+  static constexpr int V = 16 / sizeof(T);
+  const T* x;
+  int from, to;  // this wavefront's entries
+  __device__ __forceinline__ Row(const DrawArgs& a, long n) {
+    x = (const T*)a.x + n * a.ld;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = (a.A + 16 * 64 * V - 1) / (16 * 64 * V) * (64 * V);
+    from = w * part < a.A ? w * part : a.A;
+    to = from + part < a.A ? from + part : a.A;
+  }
+  // The keys of the lane's entries at `at` + V lane .., 0 behind the part's end.
+  __device__ __forceinline__ void keys(int at, uint32_t* k) const {
+    const int i = at + V * (threadIdx.x & 63);
+    T v[V];
+    if (i + V <= to) {
+      __builtin_memcpy(v, x + i, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; j++) v[j] = i + j < to ? x[i + j] : T(0);
+    }
+#pragma unroll
+    for (int j = 0; j < V; j++) k[j] = i + j < to ? key_of(raw(v[j])) : 0;
+  }
+  static __device__ __forceinline__ float raw(uint16_t v) { return bf16_to_f32(v); }
+  static __device__ __forceinline__ float raw(float v) { return v; }
+  // f(key, index) for every entry of the lane that may be taken; whole wavefronts, so that f may exchange values.
+  template <typename F> __device__ __forceinline__ void each(F f) const {
+    for (int at = from; at < to; at += 64 * V) {
+      uint32_t k[V];
+      keys(at, k);
+#pragma unroll
+      for (int j = 0; j < V; j++) f(k[j], at + V * (int)(threadIdx.x & 63) + j);
+    }
+  }
+};
 
 template <typename T> __global__ void __launch_bounds__(kWide) k_draw_wide(const DrawArgs a) {
   __shared__ WideLds L;
+  constexpr int V = Row<T>::V;
   const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
-  // the wavefront's part of the row, in whole tiles of 64 entries
-  const int part = (a.A + 16 * 64 - 1) / (16 * 64) * 64, from = w * part < a.A ? w * part : a.A, to = from + part < a.A ? from + part : a.A;
   for (long n = blockIdx.x; n < a.N; n += gridDim.x) {
-    const T* row = (const T*)a.x + n * a.ld;
+    const Row<T> row(a, n);
     const Par par = par_of(a, n);
-    auto key_at = [&](int i) { return key_of(ldf(row + i)); };
+    auto block_sum = [&](u64 v) {
+      v = wave_sum(v);
+      __syncthreads();
+      if (l == 0) L.wave[w] = v;
+      __syncthreads();
+      u64 all = 0;
+      for (int i = 0; i < 16; i++) all += L.wave[i];
+      return all;
+    };
     __syncthreads();
-    uint32_t top = 0;
-    for (int i = tid; i < a.A; i += kWide) {
-      const uint32_t k = key_at(i);
-      top = k > top ? k : top;
-    }
-    top = wave_max(top);
+    uint32_t best = 0;  // of the thread
+    int valid = 0;
+    row.each([&](uint32_t k, int) {
+      best = k > best ? k : best;
+      valid += k != 0;
+    });
+    uint32_t top = wave_max(best);
     if (l == 0) L.wave[w] = top;
     __syncthreads();
     for (int i = 0; i < 16; i++) top = (uint32_t)L.wave[i] > top ? (uint32_t)L.wave[i] : top;
@@ -300,20 +452,27 @@ template <typename T> __global__ void __launch_bounds__(kWide) k_draw_wide(const
     // the index of the count-th entry (from 1) with this key, by the wavefronts' parts
     auto index_at = [&](uint32_t k, u64 count) {
       int c = 0;
-      for (int i = from + l; i < from + part; i += 64) c += __popcll(__ballot(i < to && key_at(i) == k));
+      row.each([&](uint32_t x, int) { c += x == k; });
+      const u64 mine = wave_sum((u64)c);
       __syncthreads();
-      if (l == 0) L.wave[w] = (u64)c;
+      if (l == 0) L.wave[w] = mine;
       if (tid == 0) L.found = a.A;
       __syncthreads();
       u64 before = 0;
       for (int i = 0; i < w; i++) before += L.wave[i];
-      if (before < count && count <= before + c) {
-        for (int i = from + l; i < from + part; i += 64) {
-          const u64 on = __ballot(i < to && key_at(i) == k);
-          const int here = __popcll(on);
-          if (before < count && count <= before + here && ((on >> l) & 1) && before + __popcll(on & ((2ull << l) - 1)) == count)
-            L.found = i;
-          before += here;
+      if (before < count && count <= before + mine) {
+        for (int at = row.from; at < row.to; at += 64 * V) {
+          uint32_t x[V];
+          row.keys(at, x);
+          int here = 0;
+#pragma unroll
+          for (int j = 0; j < V; j++) here += x[j] == k;
+          const u64 incl = wave_scan((u64)here);
+          u64 rank = before + incl - here;
+#pragma unroll
+          for (int j = 0; j < V; j++)
+            if (x[j] == k && ++rank == count) L.found = at + V * l + j;
+          before += __shfl(incl, 63);
         }
       }
       __syncthreads();
@@ -329,23 +488,58 @@ template <typename T> __global__ void __launch_bounds__(kWide) k_draw_wide(const
     }
     uint32_t thr = 1;
     int cut = a.A;
-    auto mass_at = [&](uint32_t k, int i) {
-      return k > thr || (k == thr && i <= cut) ? units(mass_of(k, top, par.t), a.bits) : 0ull;
+    auto left = [&](uint32_t k, int i) { return k > thr || (k == thr && i <= cut); };
+    auto mass_at = [&](uint32_t k) { return units(mass_of(k, top, par.c), a.bits); };
+    // The entries between two keys into the list, in any order; false (and no list) if there are too many.
+    auto gather = [&](uint32_t lo, uint32_t hi, bool mass) {  // lo <= key <= hi
+      __syncthreads();
+      if (tid == 0) L.count = 0;
+      __syncthreads();
+      row.each([&](uint32_t k, int i) {
+        if (k && k >= lo && k <= hi && left(k, i)) {
+          const int at = atomicAdd(&L.count, 1);
+          if (at < kList) {
+            L.order[at] = order_of(k, (uint32_t)i);
+            if (mass) L.mass[at] = mass_at(k);
+          }
+        }
+      });
+      __syncthreads();
+      return L.count <= kList;
     };
-    // the threshold: the largest key at and above which there is `want` (entries, or mass), and what is wanted of those at it
+    // The thread's entry of the list: how many and how much mass is in front of it.
+    auto compare = [&](u64 mine, int& rank, u64& before) {
+      const int count = L.count;
+      for (int j = 0; j < count; j++) {
+        const bool first = L.order[j] > mine;
+        rank += first;
+        before += first ? L.mass[j] : 0;
+      }
+    };
+    // the entry that is `rank`-th of the list is the last that is left
+    auto cut_at = [&](bool is_it, u64 mine) {
+      if (is_it) {
+        L.key = (uint32_t)(mine >> 32);
+        L.found = (int)(0xffffffffu - (uint32_t)mine);
+      }
+      __syncthreads();
+      thr = L.key;
+      cut = L.found;
+    };
+    // The threshold by digits of the key of 11, 11 and 10 bits, a histogram in LDS each: the largest key at and above which there is
+    // `want` (entries, or mass), and what is wanted of those at it.
     auto select = [&](bool mass, u64 want, u64& rest) {
       uint32_t key = 0;
       int have = 0;  // bits of the key that are known
       for (int d = 0; d < 3; d++) {
         const int bits = d < 2 ? 11 : 10, shift = 32 - have - bits;
+        __syncthreads();
         for (int i = tid; i < kBins; i += kWide) L.bins[i] = 0;
         __syncthreads();
-        for (int i = tid; i < a.A; i += kWide) {
-          const uint32_t k = key_at(i);
-          if (!k || (have && (k >> (32 - have)) != key >> (32 - have))) continue;
-          const u64 v = mass ? mass_at(k, i) : 1;
-          if (v) atomicAdd(&L.bins[k >> shift & ((1u << bits) - 1)], v);
-        }
+        row.each([&](uint32_t k, int i) {
+          if (!k || !left(k, i) || (have && (k >> (32 - have)) != key >> (32 - have))) return;
+          atomicAdd(&L.bins[k >> shift & ((1u << bits) - 1)], mass ? mass_at(k) : 1ull);
+        });
         int bin;
         u64 above;
         pick_bin(L, 1 << bits, want, bin, above);
@@ -356,74 +550,150 @@ template <typename T> __global__ void __launch_bounds__(kWide) k_draw_wide(const
       rest = want;
       return key;
     };
-    if (par.k < a.A) {
-      int valid = 0;
-      for (int i = tid; i < a.A; i += kWide) valid += key_at(i) != 0;
-      const u64 v = wave_sum((u64)valid);
-      __syncthreads();
-      if (l == 0) L.wave[w] = v;
-      __syncthreads();
-      u64 all = 0;
-      for (int i = 0; i < 16; i++) all += L.wave[i];
-      if (all > (u64)par.k) {
+    bool listed = false;  // all that is left is in the list
+    if (par.k < a.A && block_sum((u64)valid) > (u64)par.k) {
+      if (par.k <= kWide) {
+        // the k-th largest of the threads' largest keys bounds the k-th largest of all from below
+        uint32_t cur = 0;
+        for (int bit = 31; bit >= (sizeof(T) == 2 ? 16 : 0); bit--)
+          if (__syncthreads_count(best >= (cur | (1u << bit))) >= par.k) cur |= 1u << bit;
+        if (cur && gather(cur, top, true)) {
+          const u64 mine = tid < L.count ? L.order[tid] : 0;
+          int rank = 0;
+          u64 before = 0;
+          compare(mine, rank, before);
+          cut_at(tid < L.count && rank == par.k - 1, mine);
+          listed = true;
+        }
+      }
+      if (!listed) {
         u64 rest;
         const uint32_t k = select(false, (u64)par.k, rest);
         cut = index_at(k, rest);
         thr = k;
       }
     }
-    auto block_sum = [&](u64 v) {
-      v = wave_sum(v);
-      __syncthreads();
-      if (l == 0) L.wave[w] = v;
-      __syncthreads();
-      u64 all = 0;
-      for (int i = 0; i < 16; i++) all += L.wave[i];
-      return all;
-    };
-    if (par.p < 1.0) {
-      u64 s = 0;
-      for (int i = tid; i < a.A; i += kWide) {
-        const uint32_t k = key_at(i);
-        if (k) s += mass_at(k, i);
+    if (listed) {  // the rest of the filters and the draw among the list's entries, one a thread
+      const int count = L.count;
+      const u64 mine = tid < count ? L.order[tid] : 0;
+      const uint32_t k = (uint32_t)(mine >> 32);
+      const int i = (int)(0xffffffffu - (uint32_t)mine);
+      u64 m = tid < count && left(k, i) ? L.mass[tid] : 0;
+      const u64 of = block_sum(m);
+      if (par.p < 1.0) {
+        int rank = 0;
+        u64 before = 0;
+        compare(mine, rank, before);
+        if (before >= (u64)ceil(par.p * (double)of)) m = 0;
       }
+      if (m && !reaches(mass_of(k, top, par.c), par.minp)) m = 0;
+      const u64 total = block_sum(m);
+      L.mass[tid] = m;
+      if (tid == 0) L.found = a.A;
+      __syncthreads();
+      const u64 target = (u64)((double)par.u * (double)total);
+      u64 run = 0;  // up to this entry, in the order of the indices
+      for (int j = 0; j < count; j++) run += (uint32_t)L.order[j] >= (uint32_t)mine ? L.mass[j] : 0;
+      if (m && (run > target || run == total)) atomicMin(&L.found, i);
+      __syncthreads();
+      if (m && i == L.found) {
+        a.act[n] = i;
+        if (a.logp) a.logp[n] = (float)log((double)m / (double)total);
+      }
+      continue;
+    }
+    if (par.p < 1.0) {
+      // Bins of equal width in the logit below the largest, down to masses of 2^-bits: what falls into the one where the threshold
+      // lies is few enough for the list, unless many are equal.
+      const float ltop = logit_of(top), width = (float)(((double)a.bits + 1) / par.c), per = (float)(kBins - 1) / width;
+      auto bin_of = [&](uint32_t k) {  // falls with the key
+        const float d = (ltop - logit_of(k)) * per;
+        return k == top || !(d > 0.f) ? 0 : d < (float)(kBins - 1) ? (int)d : kBins - 1;
+      };
+      __syncthreads();
+      for (int i = tid; i < kBins; i += kWide) L.bins[i] = 0;
+      __syncthreads();
+      u64 s = 0;
+      row.each([&](uint32_t k, int i) {
+        if (!k || !left(k, i)) return;
+        const u64 m = mass_at(k);
+        s += m;
+        if (m) atomicAdd(&L.bins[kBins - 1 - bin_of(k)], m);
+      });
       const u64 want = (u64)ceil(par.p * (double)block_sum(s));
-      u64 rest;
-      const uint32_t k = select(true, want, rest);
-      const u64 each = units(mass_of(k, top, par.t), a.bits), count = each ? (rest + each - 1) / each : 1;
-      const int at = index_at(k, count);
-      if (k > thr) cut = a.A;
-      thr = k;
-      cut = at < cut ? at : cut;
+      int bin;
+      u64 above;
+      pick_bin(L, kBins, want, bin, above);
+      bin = kBins - 1 - bin;
+      __syncthreads();
+      if (tid == 0) L.count = 0;
+      __syncthreads();
+      row.each([&](uint32_t k, int i) {
+        if (!k || bin_of(k) != bin || !left(k, i)) return;
+        const int at = atomicAdd(&L.count, 1);
+        if (at < kList) {
+          L.order[at] = order_of(k, (uint32_t)i);
+          L.mass[at] = mass_at(k);
+        }
+      });
+      __syncthreads();
+      if (L.count <= kList) {
+        const u64 mine = tid < L.count ? L.order[tid] : 0;
+        int rank = 0;
+        u64 before = above;
+        compare(mine, rank, before);
+        const int kept = __syncthreads_count(tid < L.count && before < want);
+        cut_at(tid < L.count && rank == kept - 1, mine);
+      } else {
+        u64 rest;
+        const uint32_t k = select(true, want, rest);
+        const u64 each = mass_at(k), of = each ? (rest + each - 1) / each : 1;
+        const int at = index_at(k, of);
+        if (k > thr) cut = a.A;
+        thr = k;
+        cut = at < cut ? at : cut;
+      }
     }
     auto left_at = [&](uint32_t k, int i) {
-      if (!k || !(k > thr || (k == thr && i <= cut))) return 0ull;
-      const double e = mass_of(k, top, par.t);
-      return e >= (double)par.minp ? units(e, a.bits) : 0ull;
+      if (!k || !left(k, i)) return 0ull;
+      const Mass m = mass_of(k, top, par.c);
+      return reaches(m, par.minp) ? units(m, a.bits) : 0ull;
     };
     u64 s = 0;
-    for (int i = from + l; i < to; i += 64) s += left_at(key_at(i), i);
+    row.each([&](uint32_t k, int i) { s += left_at(k, i); });
     const u64 mine = wave_sum(s);
     const u64 total = block_sum(s);  // L.wave: the wavefronts' sums
     u64 before = 0;
     for (int i = 0; i < w; i++) before += L.wave[i];
     const u64 target = (u64)((double)par.u * (double)total);
     if (mine && before <= target && (before + mine > target || before + mine == total)) {
-      bool open = true;
-      for (int i = from + l; i < from + part && open; i += 64) {
-        const u64 m = i < to ? left_at(key_at(i), i) : 0;
-        const u64 here = wave_sum(m);
-        if (here && (before + here > target || before + here == total)) {
-          const u64 at = before + wave_scan(m);
-          u64 hit = __ballot(m > 0 && at > target);
-          if (!hit) hit = 1ull << (63 - __clzll((long long)__ballot(m > 0)));
-          if (l == __ffsll((unsigned long long)hit) - 1) {
-            a.act[n] = i;
-            if (a.logp) a.logp[n] = (float)log((double)m / (double)total);
+      for (int at = row.from; at < row.to; at += 64 * V) {
+        uint32_t k[V];
+        u64 m[V], here = 0;
+        row.keys(at, k);
+#pragma unroll
+        for (int j = 0; j < V; j++) here += m[j] = left_at(k[j], at + V * l + j);
+        const u64 incl = wave_scan(here), all = __shfl(incl, 63);
+        if (all && (before + all > target || before + all == total)) {
+          u64 run = before + incl - here;
+          int first = -1;  // of the lane's entries: the first that exceeds, or (u rounded up to 1) the last there is
+          u64 got = 0;
+#pragma unroll
+          for (int j = 0; j < V; j++) {
+            run += m[j];
+            if (m[j] && (run > target || run == total) && first < 0) {
+              first = j;
+              got = m[j];
+            }
           }
-          open = false;
+          const u64 who = __ballot(first >= 0);
+          if (l == __ffsll((unsigned long long)who) - 1) {
+            a.act[n] = at + V * l + first;
+            if (a.logp) a.logp[n] = (float)log((double)got / (double)total);
+          }
+          break;
         }
-        before += here;
+        before += all;
       }
     }
   }
