@@ -88,6 +88,18 @@ __device__ __forceinline__ Mass mass_of(uint32_t key, uint32_t top, double c) { 
   if (key == top) m = {1.0, 0};  // of an infinite logit too, whose difference is none
   return m;
 }
+// The same by a table of 2^(i / 1024), i = 0..1023: the series ends with z^3 for |z| <= ln 2 / 2048 (left out: below 2^-50), half the
+// instructions. For rows that are worth the table.
+constexpr int kTable = 1024;
+__device__ __forceinline__ Mass mass_of(uint32_t key, uint32_t top, double c, const double* table) {
+  double y = ((double)logit_of(key) - (double)logit_of(top)) * (c * kTable);
+  y = y > -1000.0 * kTable ? y : -1000.0 * kTable;
+  const double n = rint(y), z = (y - n) * (0.6931471805599453094 / kTable);
+  const int i = (int)n;
+  Mass m = {table[i & (kTable - 1)] * fma(z, fma(z, fma(z, 1.0 / 6, 0.5), 1.0), 1.0), i >> 10};
+  if (key == top) m = {1.0, 0};
+  return m;
+}
 // In units of 2^-bits, to the nearest.
 __device__ __forceinline__ u64 units(Mass m, int bits) {
   const u64 b = __builtin_bit_cast(u64, m.r);
@@ -95,7 +107,8 @@ __device__ __forceinline__ u64 units(Mass m, int bits) {
   const u64 f = (b & 0xfffffffffffffull) | 0x10000000000000ull;
   return shift > 53 ? 0 : (f + (1ull << (shift - 1))) >> shift;
 }
-__device__ __forceinline__ bool reaches(Mass m, float minp) { return minp == 0.f || ldexp(m.r, m.n) >= (double)minp; }
+// What an entry has to have by min_p, in these units.
+__device__ __forceinline__ u64 least(float minp, int bits) { return (u64)ceil(ldexp((double)minp, bits)); }
 
 // ---- sums over a wavefront --------------------------------------------------------------------------------
 template <int CTL> __device__ __forceinline__ u64 dpp64(u64 v) {
@@ -145,34 +158,41 @@ __device__ __forceinline__ u64 order_of(uint32_t key, uint32_t index) { return (
 struct WaveLds {
   u64 order[64], mass[64];
 };
-template <typename T, int E> __global__ void __launch_bounds__(256) k_draw_wave(const DrawArgs a) {
+template <typename T, int E> __global__ void __launch_bounds__(256, 4) k_draw_wave(const DrawArgs a) {
   __shared__ WaveLds lds[4];
-  const int l = threadIdx.x & 63;
+  int l = threadIdx.x & 63;
+  // what goes by the lane's number is formed again from here on, and does not wait in registers
+  auto renew = [&] { asm volatile("" : "+v"(l)); };
   WaveLds& L = lds[threadIdx.x >> 6];
   for (long n = (long)blockIdx.x * 4 + (threadIdx.x >> 6); n < a.N; n += (long)gridDim.x * 4) {
     const T* row = (const T*)a.x + n * a.ld;
     uint32_t key[E], top = 0;
+    {
+      T x[E];
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-      const int i = 64 * e + l;
-      key[e] = i < a.A ? key_of(ldf(row + i)) : 0;
-      top = key[e] > top ? key[e] : top;
+      for (int e = 0; e < E; e++) x[e] = row[64 * e + l < a.A ? 64 * e + l : 0];
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const uint32_t k = key_of(ldf(&x[e]));
+        key[e] = 64 * e + l < a.A ? k : 0;
+        top = key[e] > top ? key[e] : top;
+      }
     }
+    renew();
     const Par par = par_of(a, n);
     top = wave_max(top);
     int act = -1;
     float logp = -INFINITY;
-    // the entries at `key` in the order of their indices: the index of the count-th (from 1)
+    // the entries at `key` in the order of their indices: the index of the count-th (from 1). Few rows ask, so it reads them again.
     auto index_at = [&](uint32_t k, long count) {
       int cut = a.A;
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        const u64 on = __ballot(key[e] == k);
+#pragma unroll 1
+      for (int at = 0; at < a.A && count > 0; at += 64) {
+        const u64 on = __ballot(at + l < a.A && key_of(ldf(row + (at + l < a.A ? at + l : 0))) == k);
         const int c = __popcll(on);
-        if (count > 0 && count <= c) {
-          const u64 mine = on & ((2ull << l) - 1);
-          const u64 at = __ballot(((on >> l) & 1) && __popcll(mine) == count);
-          cut = 64 * e + __ffsll((unsigned long long)at) - 1;
+        if (count <= c) {
+          const u64 is = __ballot(((on >> l) & 1) && __popcll(on & ((2ull << l) - 1)) == count);
+          cut = at + __ffsll((unsigned long long)is) - 1;
         }
         count -= c;
       }
@@ -185,39 +205,50 @@ template <typename T, int E> __global__ void __launch_bounds__(256) k_draw_wave(
     } else {
       uint32_t thr = 1;
       int cut = a.A;
-      auto left = [&](int e) { return key[e] > thr || (key[e] == thr && 64 * e + l <= cut); };
+      auto left = [&](int e) { return (key[e] > thr) | ((key[e] == thr) & (64 * e + l <= cut)); };
       if (E > 1 && par.k < a.A) {
-        uint32_t cur = 0;
-        long at_least = 0;
-        for (int bit = 31; bit >= (sizeof(T) == 2 ? 16 : 0); bit--) {
-          const uint32_t c = cur | (1u << bit);
-          long cnt = 0;
+        // at least k keys are lo and above, fewer hi and above: until there are k, or equal ones at the border
+        auto count = [&](uint32_t c) {
+          int n = 0;
 #pragma unroll
-          for (int e = 0; e < E; e++) cnt += __popcll(__ballot(key[e] >= c));
-          if (cnt >= par.k) {
-            cur = c;
-            at_least = cnt;
+          for (int e = 0; e < E; e++) n += __popcll(__ballot(key[e] >= c));
+          return n;
+        };
+        uint32_t lo = 1, hi = top;
+        int at_least = count(1), above = 0;
+        if (at_least > par.k) {
+          above = count(top);
+          if (above >= par.k) {  // the largest alone are as many
+            lo = top;
+            at_least = above;
+            above = 0;
+          } else {
+            while (at_least > par.k && hi - lo > 1) {
+              const uint32_t mid = lo + (hi - lo) / 2;
+              const int c = count(mid);
+              if (c >= par.k) {
+                lo = mid;
+                at_least = c;
+              } else {
+                hi = mid;
+                above = c;
+              }
+            }
           }
-        }
-        if (cur) {  // else there are fewer than k
-          if (sizeof(T) == 2) cur |= cur >> 31 ? 0 : 0xffff;  // of a bf16 logit the key's lower half goes by its sign
-          thr = cur;
-          if (at_least > par.k) {
-            long above = 0;
-#pragma unroll
-            for (int e = 0; e < E; e++) above += __popcll(__ballot(key[e] > thr));
-            cut = index_at(thr, par.k - above);
-          }
+          thr = lo;
+          if (at_least > par.k) cut = index_at(thr, par.k - above);
         }
       }
-      Mass r[E];
+      renew();
       u64 m[E], total = 0;
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        r[e] = mass_of(key[e], top, par.c);
-        m[e] = key[e] && left(e) ? units(r[e], a.bits) : 0;
+        const u64 x = units(mass_of(key[e], top, par.c), a.bits);
+        m[e] = (key[e] != 0) & left(e) ? x : 0;
         total += m[e];
+        if (E > 4 && e % 2) __builtin_amdgcn_sched_barrier(0);  // or all registers' series run side by side, and do not fit
       }
+      renew();
       // of at most 64 entries in LDS, lane i's: how many and how much mass is in front of it
       auto compare = [&](int count, u64 mine, int& rank, u64& before) {
         for (int j = 0; j < count; j++) {
@@ -269,6 +300,7 @@ template <typename T, int E> __global__ void __launch_bounds__(256) k_draw_wave(
             above_hi = sum;
           }
         }
+        renew();
         int count = 0;
 #pragma unroll
         for (int e = 0; e < E; e++) {
@@ -301,11 +333,13 @@ template <typename T, int E> __global__ void __launch_bounds__(256) k_draw_wave(
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       }
+      renew();
+      const u64 need = least(par.minp, a.bits);
       // in the order of the indices: through[e] is the lane's share of the first e + 1 registers
       u64 through[E], run = 0;
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        if (!(left(e) && reaches(r[e], par.minp))) m[e] = 0;
+        m[e] = left(e) & (m[e] >= need) ? m[e] : 0;
         run += m[e];
         through[e] = run;
       }
@@ -417,6 +451,9 @@ template <typename T> struct Row {
 
 template <typename T> __global__ void __launch_bounds__(kWide) k_draw_wide(const DrawArgs a) {
   __shared__ WideLds L;
+  __shared__ double table[kTable];
+  table[threadIdx.x] = exp2((double)threadIdx.x / kTable);
+  static_assert(kTable == kWide, "an entry each");
   constexpr int V = Row<T>::V;
   const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
   for (long n = blockIdx.x; n < a.N; n += gridDim.x) {
@@ -489,7 +526,8 @@ template <typename T> __global__ void __launch_bounds__(kWide) k_draw_wide(const
     uint32_t thr = 1;
     int cut = a.A;
     auto left = [&](uint32_t k, int i) { return k > thr || (k == thr && i <= cut); };
-    auto mass_at = [&](uint32_t k) { return units(mass_of(k, top, par.c), a.bits); };
+    auto mass_at = [&](uint32_t k) { return units(mass_of(k, top, par.c, table), a.bits); };
+    const u64 need = least(par.minp, a.bits);
     // The entries between two keys into the list, in any order; false (and no list) if there are too many.
     auto gather = [&](uint32_t lo, uint32_t hi, bool mass) {  // lo <= key <= hi
       __syncthreads();
@@ -586,7 +624,7 @@ template <typename T> __global__ void __launch_bounds__(kWide) k_draw_wide(const
         compare(mine, rank, before);
         if (before >= (u64)ceil(par.p * (double)of)) m = 0;
       }
-      if (m && !reaches(mass_of(k, top, par.c), par.minp)) m = 0;
+      if (m < need) m = 0;
       const u64 total = block_sum(m);
       L.mass[tid] = m;
       if (tid == 0) L.found = a.A;
@@ -656,8 +694,8 @@ template <typename T> __global__ void __launch_bounds__(kWide) k_draw_wide(const
     }
     auto left_at = [&](uint32_t k, int i) {
       if (!k || !left(k, i)) return 0ull;
-      const Mass m = mass_of(k, top, par.c);
-      return reaches(m, par.minp) ? units(m, a.bits) : 0ull;
+      const u64 m = mass_at(k);
+      return m >= need ? m : 0ull;
     };
     u64 s = 0;
     row.each([&](uint32_t k, int i) { s += left_at(k, i); });
