@@ -1176,6 +1176,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             if constexpr (!LOCAL) Y[n] = dot2<BF, HT>(x, Sp, Y[n]);
             dU[n] = dot2<BF, HT>(x, Dp, dU[n]);
           }
+          if (NT > 4) __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int n = 0; n < NB; n++) {
@@ -1251,6 +1252,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
 #pragma unroll
             for (int n = 0; n < NB; n++) a[n] = col_unit<LD>(tid, L.K, 16 * n, 16 * m);
             dS[m] = dot2<BF, NB>(a, y, dS[m]);
+            if (NT > 4) __builtin_amdgcn_sched_barrier(0);  // or the operands of all tiles are loaded at once, and do not fit
           }
         }
         if constexpr (!LOCAL) {
@@ -1273,6 +1275,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
               }
               e = dot2<BF, HT>(z, y, e);
               f = dot3<BF, HT>(x, y, f);
+              if (NT > 4) __builtin_amdgcn_sched_barrier(0);
             }
             const int j = 16 * bj + (l & 15);
             const double Gj = R.G[j];
@@ -1317,6 +1320,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
 #pragma unroll
               for (int m = 0; m < HT; m++) y[m] = col_pair<BF, UD>(tid, L.U, L.Ulo, 16 * (m0 + m), 16 * n);
               X3[n] = dot3<BF, HT>(y, Dt, X3[n]);
+              if (NT > 4) __builtin_amdgcn_sched_barrier(0);
             }
           }
 #pragma unroll
@@ -1350,6 +1354,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
 #pragma unroll
               for (int n = 0; n < NB; n++) b[n] = row_pair<BF, UD>(tid, L.dY, L.dYlo, 16 * m, 16 * n);
               dSt[m] = dot3<BF, NB>(b, y, dSt[m]);
+              if (NT > 4) __builtin_amdgcn_sched_barrier(0);
             }
           }
           __syncthreads();
@@ -1799,7 +1804,7 @@ template <typename T> int step_t(const Args& a, float* h, hipStream_t st) {
 // Segments of time, and where their states are: `states` buffers of [segs][units] states, Phi and the cuts.
 void set_segments(Args& a, bool grad, int dtype) {
   const long c = dtype == PH_BF16 ? Elem<true>::CH : Elem<false>::CH, chunks = (a.T + c - 1) / c;
-  a.segs = (int)delta_segments(chunks, a.units, padded(a), grad);
+  a.segs = (int)delta_segments(chunks, a.units, padded(a));
   a.seg_chunks = (chunks + a.segs - 1) / a.segs;
   a.segs = (int)((chunks + a.seg_chunks - 1) / a.seg_chunks);
   a.local_from = grad ? 1 : 0;

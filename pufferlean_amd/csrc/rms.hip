@@ -396,6 +396,7 @@ template <typename T> struct RmsCall {
       if (accesses <= 16) return by_form<V, AL, 1, 16>();
       if (accesses <= 32) return by_form<V, AL, 1, 32>();
       if (accesses <= 64) return by_form<V, AL, 1, 64>();
+      if (accesses <= 128) return by_form<V, AL, 2, 64>();
       if (accesses <= 256) return by_form<V, AL, 1, 256>();
       if (accesses <= 512) return by_form<V, AL, 2, 256>();
     }

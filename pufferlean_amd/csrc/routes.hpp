@@ -202,9 +202,14 @@ inline long ssm_chunk(long T, long B, long G, long per, int N, bool grad) {
 }
 
 // ---- Gated delta rule ---------------------------------------------------------------------------------------
-// Segments of time of `chunks` chunks, of `units` sequences' heads with states padded to P x P.
-inline long delta_segments(long chunks, long units, int P, bool grad) {
-  const long most = (chunks + 3) / 4, want = (P <= 32 ? 2048 : P <= 64 ? 768 : 256) / units;
+// Segments of time of `chunks` chunks, of `units` sequences' heads with states padded to P x P: as many as make one round of
+// blocks at the occupancy that their registers leave (P = 32: four blocks of two wavefronts to a CU, 64: two of four, 128: one of
+// eight). A segment more costs a step of the join and, past the round, the others' share of the CU; and there are two passes
+// over the steps, so whole sequences of less than eight chunks stay one. Forward and gradient, bf16, us by segments: 8192 steps of 16
+// units of 64x64 8: 315, 703; 16: 190, 382; 32: 154, 260; 48: 173, 300; 64: 187, 280. 1024 of 64 units of 64x64 4: 100, 202; 8: 74, 134;
+// 16: 78, 133; 32: 102, 165; of 32x32 8: 61, 126; 16: 49, 87; 32: 60, 106. 2048 of 32 units of 128x128 4: 202, 630; 8: 167, 388; 16: 198, 411.
+inline long delta_segments(long chunks, long units, int P) {
+  const long most = (chunks + 1) / 2, want = (P <= 32 ? 1024 : P <= 64 ? 512 : 256) / units;
   const long n = want < most ? want : most;
   return n < 2 || chunks < 8 ? 1 : n;
 }
