@@ -14,6 +14,7 @@
 #include "common.hpp"
 #include "kernels.hpp"
 #include "lanes.hpp"
+#include "routes.hpp"
 
 namespace ph {
 namespace {
@@ -417,12 +418,13 @@ template <typename T> struct Row {
   static constexpr int V = 16 / sizeof(T);
   const T* x;
   int from, to;  // this wavefront's entries
-  __device__ __forceinline__ Row(const DrawArgs& a, long n) {
+  __device__ __forceinline__ Row(const DrawArgs& a, long n, int w, int parts) {
     x = (const T*)a.x + n * a.ld;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = (a.A + 16 * 64 * V - 1) / (16 * 64 * V) * (64 * V);
+    const int part = size(a.A, parts);
     from = w * part < a.A ? w * part : a.A;
     to = from + part < a.A ? from + part : a.A;
   }
+  static __device__ __forceinline__ int size(int A, int parts) { return (A + parts * 64 * V - 1) / (parts * 64 * V) * (64 * V); }
   // The keys of the lane's entries at `at` + V lane .., 0 behind the part's end.
   __device__ __forceinline__ void keys(int at, uint32_t* k) const {
     const int i = at + V * (threadIdx.x & 63);
@@ -449,291 +451,567 @@ template <typename T> struct Row {
   }
 };
 
-template <typename T> __global__ void __launch_bounds__(kWide) k_draw_wide(const DrawArgs a) {
-  __shared__ WideLds L;
-  __shared__ double table[kTable];
-  table[threadIdx.x] = exp2((double)threadIdx.x / kTable);
-  static_assert(kTable == kWide, "an entry each");
+// Bins of equal width in the logit below the largest, down to masses of 2^-bits; they fall with the key.
+struct Bins {
+  float ltop, per;
+  uint32_t top;
+  __device__ __forceinline__ Bins(const DrawArgs& a, const Par& par, uint32_t t) : top(t) {
+    ltop = logit_of(t);
+    per = (float)(kBins - 1) / (float)(((double)a.bits + 1) / par.c);
+  }
+  __device__ __forceinline__ int operator()(uint32_t k) const {
+    const float d = (ltop - logit_of(k)) * per;
+    return k == top || !(d > 0.f) ? 0 : d < (float)(kBins - 1) ? (int)d : kBins - 1;
+  }
+};
+
+__device__ __forceinline__ u64 block_sum(WideLds& L, u64 v) {
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  v = wave_sum(v);
+  __syncthreads();
+  if (l == 0) L.wave[w] = v;
+  __syncthreads();
+  u64 all = 0;
+  for (int i = 0; i < 16; i++) all += L.wave[i];
+  return all;
+}
+
+// The thread's entry of the list: how many and how much mass is in front of it.
+__device__ __forceinline__ void compare(const WideLds& L, u64 mine, int& rank, u64& before) {
+  const int count = L.count;
+  for (int j = 0; j < count; j++) {
+    const bool first = L.order[j] > mine;
+    rank += first;
+    before += first ? L.mass[j] : 0;
+  }
+}
+// The entry that `is_it` holds for is the last that is left.
+__device__ __forceinline__ void cut_at(WideLds& L, bool is_it, u64 mine, uint32_t& thr, int& cut) {
+  if (is_it) {
+    L.key = (uint32_t)(mine >> 32);
+    L.found = (int)(0xffffffffu - (uint32_t)mine);
+  }
+  __syncthreads();
+  thr = L.key;
+  cut = L.found;
+}
+
+// All that top-k leaves is in the list, one entry a thread: the rest of the filters and the draw.
+__device__ __forceinline__ void draw_listed(WideLds& L, const DrawArgs& a, long n, const Par& par, uint32_t thr, int cut) {
+  const int tid = threadIdx.x, count = L.count;
+  const u64 mine = tid < count ? L.order[tid] : 0;
+  const uint32_t k = (uint32_t)(mine >> 32);
+  const int i = (int)(0xffffffffu - (uint32_t)mine);
+  u64 m = tid < count && (k > thr || (k == thr && i <= cut)) ? L.mass[tid] : 0;
+  const u64 of = block_sum(L, m);
+  if (par.p < 1.0) {
+    int rank = 0;
+    u64 before = 0;
+    compare(L, mine, rank, before);
+    if (before >= (u64)ceil(par.p * (double)of)) m = 0;
+  }
+  if (m < least(par.minp, a.bits)) m = 0;
+  const u64 total = block_sum(L, m);
+  L.mass[tid] = m;
+  if (tid == 0) L.found = a.A;
+  __syncthreads();
+  const u64 target = (u64)((double)par.u * (double)total);
+  u64 run = 0;  // up to this entry, in the order of the indices
+  for (int j = 0; j < count; j++) run += (uint32_t)L.order[j] >= (uint32_t)mine ? L.mass[j] : 0;
+  if (m && (run > target || run == total)) atomicMin(&L.found, i);
+  __syncthreads();
+  if (m && i == L.found) {
+    a.act[n] = i;
+    if (a.logp) a.logp[n] = (float)log((double)m / (double)total);
+  }
+}
+
+// The wavefront's part of the row is where the sum, `before` in front of it, exceeds the target.
+template <typename T, typename F>
+__device__ __forceinline__ void draw_in_part(const DrawArgs& a, long n, const Row<T>& row, F left_at, u64 before, u64 target, u64 total) {
   constexpr int V = Row<T>::V;
-  const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
-  for (long n = blockIdx.x; n < a.N; n += gridDim.x) {
-    const Row<T> row(a, n);
-    const Par par = par_of(a, n);
-    auto block_sum = [&](u64 v) {
-      v = wave_sum(v);
-      __syncthreads();
-      if (l == 0) L.wave[w] = v;
-      __syncthreads();
-      u64 all = 0;
-      for (int i = 0; i < 16; i++) all += L.wave[i];
-      return all;
-    };
-    __syncthreads();
-    uint32_t best = 0;  // of the thread
-    int valid = 0;
-    row.each([&](uint32_t k, int) {
-      best = k > best ? k : best;
-      valid += k != 0;
-    });
-    uint32_t top = wave_max(best);
-    if (l == 0) L.wave[w] = top;
-    __syncthreads();
-    for (int i = 0; i < 16; i++) top = (uint32_t)L.wave[i] > top ? (uint32_t)L.wave[i] : top;
-    if (top == 0) {
-      if (tid == 0) {
-        a.act[n] = -1;
-        if (a.logp) a.logp[n] = -INFINITY;
-      }
-      continue;
-    }
-    // the index of the count-th entry (from 1) with this key, by the wavefronts' parts
-    auto index_at = [&](uint32_t k, u64 count) {
-      int c = 0;
-      row.each([&](uint32_t x, int) { c += x == k; });
-      const u64 mine = wave_sum((u64)c);
-      __syncthreads();
-      if (l == 0) L.wave[w] = mine;
-      if (tid == 0) L.found = a.A;
-      __syncthreads();
-      u64 before = 0;
-      for (int i = 0; i < w; i++) before += L.wave[i];
-      if (before < count && count <= before + mine) {
-        for (int at = row.from; at < row.to; at += 64 * V) {
-          uint32_t x[V];
-          row.keys(at, x);
-          int here = 0;
+  const int l = threadIdx.x & 63;
+  for (int at = row.from; at < row.to; at += 64 * V) {
+    uint32_t k[V];
+    u64 m[V], here = 0;
+    row.keys(at, k);
 #pragma unroll
-          for (int j = 0; j < V; j++) here += x[j] == k;
-          const u64 incl = wave_scan((u64)here);
-          u64 rank = before + incl - here;
+    for (int j = 0; j < V; j++) here += m[j] = left_at(k[j], at + V * l + j);
+    const u64 incl = wave_scan(here), all = __shfl(incl, 63);
+    if (all && (before + all > target || before + all == total)) {
+      u64 run = before + incl - here;
+      int first = -1;  // of the lane's entries: the first that exceeds, or (u rounded up to 1) the last there is
+      u64 got = 0;
 #pragma unroll
-          for (int j = 0; j < V; j++)
-            if (x[j] == k && ++rank == count) L.found = at + V * l + j;
-          before += __shfl(incl, 63);
+      for (int j = 0; j < V; j++) {
+        run += m[j];
+        if (m[j] && (run > target || run == total) && first < 0) {
+          first = j;
+          got = m[j];
         }
       }
-      __syncthreads();
-      return L.found;
-    };
-    if (par.greedy) {
-      const int i = index_at(top, 1);
-      if (tid == 0) {
-        a.act[n] = i;
-        if (a.logp) a.logp[n] = 0.f;
+      const u64 who = __ballot(first >= 0);
+      if (l == __ffsll((unsigned long long)who) - 1) {
+        a.act[n] = at + V * l + first;
+        if (a.logp) a.logp[n] = (float)log((double)got / (double)total);
       }
-      continue;
+      break;
     }
-    uint32_t thr = 1;
-    int cut = a.A;
-    auto left = [&](uint32_t k, int i) { return k > thr || (k == thr && i <= cut); };
-    auto mass_at = [&](uint32_t k) { return units(mass_of(k, top, par.c, table), a.bits); };
-    const u64 need = least(par.minp, a.bits);
-    // The entries between two keys into the list, in any order; false (and no list) if there are too many.
-    auto gather = [&](uint32_t lo, uint32_t hi, bool mass) {  // lo <= key <= hi
-      __syncthreads();
-      if (tid == 0) L.count = 0;
-      __syncthreads();
-      row.each([&](uint32_t k, int i) {
-        if (k && k >= lo && k <= hi && left(k, i)) {
-          const int at = atomicAdd(&L.count, 1);
-          if (at < kList) {
-            L.order[at] = order_of(k, (uint32_t)i);
-            if (mass) L.mass[at] = mass_at(k);
-          }
-        }
-      });
-      __syncthreads();
-      return L.count <= kList;
-    };
-    // The thread's entry of the list: how many and how much mass is in front of it.
-    auto compare = [&](u64 mine, int& rank, u64& before) {
-      const int count = L.count;
-      for (int j = 0; j < count; j++) {
-        const bool first = L.order[j] > mine;
-        rank += first;
-        before += first ? L.mass[j] : 0;
-      }
-    };
-    // the entry that is `rank`-th of the list is the last that is left
-    auto cut_at = [&](bool is_it, u64 mine) {
-      if (is_it) {
-        L.key = (uint32_t)(mine >> 32);
-        L.found = (int)(0xffffffffu - (uint32_t)mine);
-      }
-      __syncthreads();
-      thr = L.key;
-      cut = L.found;
-    };
-    // The threshold by digits of the key of 11, 11 and 10 bits, a histogram in LDS each: the largest key at and above which there is
-    // `want` (entries, or mass), and what is wanted of those at it.
-    auto select = [&](bool mass, u64 want, u64& rest) {
-      uint32_t key = 0;
-      int have = 0;  // bits of the key that are known
-      for (int d = 0; d < 3; d++) {
-        const int bits = d < 2 ? 11 : 10, shift = 32 - have - bits;
-        __syncthreads();
-        for (int i = tid; i < kBins; i += kWide) L.bins[i] = 0;
-        __syncthreads();
-        row.each([&](uint32_t k, int i) {
-          if (!k || !left(k, i) || (have && (k >> (32 - have)) != key >> (32 - have))) return;
-          atomicAdd(&L.bins[k >> shift & ((1u << bits) - 1)], mass ? mass_at(k) : 1ull);
-        });
-        int bin;
-        u64 above;
-        pick_bin(L, 1 << bits, want, bin, above);
-        want -= above;
-        key |= (uint32_t)bin << shift;
-        have += bits;
-      }
-      rest = want;
-      return key;
-    };
-    bool listed = false;  // all that is left is in the list
-    if (par.k < a.A && block_sum((u64)valid) > (u64)par.k) {
-      if (par.k <= kWide) {
-        // the k-th largest of the threads' largest keys bounds the k-th largest of all from below
-        uint32_t cur = 0;
-        for (int bit = 31; bit >= (sizeof(T) == 2 ? 16 : 0); bit--)
-          if (__syncthreads_count(best >= (cur | (1u << bit))) >= par.k) cur |= 1u << bit;
-        if (cur && gather(cur, top, true)) {
-          const u64 mine = tid < L.count ? L.order[tid] : 0;
-          int rank = 0;
-          u64 before = 0;
-          compare(mine, rank, before);
-          cut_at(tid < L.count && rank == par.k - 1, mine);
-          listed = true;
-        }
-      }
-      if (!listed) {
-        u64 rest;
-        const uint32_t k = select(false, (u64)par.k, rest);
-        cut = index_at(k, rest);
-        thr = k;
+    before += all;
+  }
+}
+
+template <typename T> __device__ __forceinline__ void draw_row(WideLds& L, const double* table, const DrawArgs& a, long n) {
+  constexpr int V = Row<T>::V;
+  const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Row<T> row(a, n, w, 16);
+  const Par par = par_of(a, n);
+  __syncthreads();
+  uint32_t best = 0;  // of the thread
+  int valid = 0;
+  row.each([&](uint32_t k, int) {
+    best = k > best ? k : best;
+    valid += k != 0;
+  });
+  uint32_t top = wave_max(best);
+  if (l == 0) L.wave[w] = top;
+  __syncthreads();
+  for (int i = 0; i < 16; i++) top = (uint32_t)L.wave[i] > top ? (uint32_t)L.wave[i] : top;
+  if (top == 0) {
+    if (tid == 0) {
+      a.act[n] = -1;
+      if (a.logp) a.logp[n] = -INFINITY;
+    }
+    return;
+  }
+  // the index of the count-th entry (from 1) with this key, by the wavefronts' parts
+  auto index_at = [&](uint32_t k, u64 count) {
+    int c = 0;
+    row.each([&](uint32_t x, int) { c += x == k; });
+    const u64 mine = wave_sum((u64)c);
+    __syncthreads();
+    if (l == 0) L.wave[w] = mine;
+    if (tid == 0) L.found = a.A;
+    __syncthreads();
+    u64 before = 0;
+    for (int i = 0; i < w; i++) before += L.wave[i];
+    if (before < count && count <= before + mine) {
+      for (int at = row.from; at < row.to; at += 64 * V) {
+        uint32_t x[V];
+        row.keys(at, x);
+        int here = 0;
+#pragma unroll
+        for (int j = 0; j < V; j++) here += x[j] == k;
+        const u64 incl = wave_scan((u64)here);
+        u64 rank = before + incl - here;
+#pragma unroll
+        for (int j = 0; j < V; j++)
+          if (x[j] == k && ++rank == count) L.found = at + V * l + j;
+        before += __shfl(incl, 63);
       }
     }
-    if (listed) {  // the rest of the filters and the draw among the list's entries, one a thread
-      const int count = L.count;
-      const u64 mine = tid < count ? L.order[tid] : 0;
-      const uint32_t k = (uint32_t)(mine >> 32);
-      const int i = (int)(0xffffffffu - (uint32_t)mine);
-      u64 m = tid < count && left(k, i) ? L.mass[tid] : 0;
-      const u64 of = block_sum(m);
-      if (par.p < 1.0) {
-        int rank = 0;
-        u64 before = 0;
-        compare(mine, rank, before);
-        if (before >= (u64)ceil(par.p * (double)of)) m = 0;
-      }
-      if (m < need) m = 0;
-      const u64 total = block_sum(m);
-      L.mass[tid] = m;
-      if (tid == 0) L.found = a.A;
-      __syncthreads();
-      const u64 target = (u64)((double)par.u * (double)total);
-      u64 run = 0;  // up to this entry, in the order of the indices
-      for (int j = 0; j < count; j++) run += (uint32_t)L.order[j] >= (uint32_t)mine ? L.mass[j] : 0;
-      if (m && (run > target || run == total)) atomicMin(&L.found, i);
-      __syncthreads();
-      if (m && i == L.found) {
-        a.act[n] = i;
-        if (a.logp) a.logp[n] = (float)log((double)m / (double)total);
-      }
-      continue;
+    __syncthreads();
+    return L.found;
+  };
+  if (par.greedy) {
+    const int i = index_at(top, 1);
+    if (tid == 0) {
+      a.act[n] = i;
+      if (a.logp) a.logp[n] = 0.f;
     }
-    if (par.p < 1.0) {
-      // Bins of equal width in the logit below the largest, down to masses of 2^-bits: what falls into the one where the threshold
-      // lies is few enough for the list, unless many are equal.
-      const float ltop = logit_of(top), width = (float)(((double)a.bits + 1) / par.c), per = (float)(kBins - 1) / width;
-      auto bin_of = [&](uint32_t k) {  // falls with the key
-        const float d = (ltop - logit_of(k)) * per;
-        return k == top || !(d > 0.f) ? 0 : d < (float)(kBins - 1) ? (int)d : kBins - 1;
-      };
-      __syncthreads();
-      for (int i = tid; i < kBins; i += kWide) L.bins[i] = 0;
-      __syncthreads();
-      u64 s = 0;
-      row.each([&](uint32_t k, int i) {
-        if (!k || !left(k, i)) return;
-        const u64 m = mass_at(k);
-        s += m;
-        if (m) atomicAdd(&L.bins[kBins - 1 - bin_of(k)], m);
-      });
-      const u64 want = (u64)ceil(par.p * (double)block_sum(s));
-      int bin;
-      u64 above;
-      pick_bin(L, kBins, want, bin, above);
-      bin = kBins - 1 - bin;
-      __syncthreads();
-      if (tid == 0) L.count = 0;
-      __syncthreads();
-      row.each([&](uint32_t k, int i) {
-        if (!k || bin_of(k) != bin || !left(k, i)) return;
+    return;
+  }
+  uint32_t thr = 1;
+  int cut = a.A;
+  auto left = [&](uint32_t k, int i) { return k > thr || (k == thr && i <= cut); };
+  auto mass_at = [&](uint32_t k) { return units(mass_of(k, top, par.c, table), a.bits); };
+  const u64 need = least(par.minp, a.bits);
+  // The entries between two keys into the list, in any order; false (and no list) if there are too many.
+  auto gather = [&](uint32_t lo, uint32_t hi, bool mass) {  // lo <= key <= hi
+    __syncthreads();
+    if (tid == 0) L.count = 0;
+    __syncthreads();
+    row.each([&](uint32_t k, int i) {
+      if (k && k >= lo && k <= hi && left(k, i)) {
         const int at = atomicAdd(&L.count, 1);
         if (at < kList) {
           L.order[at] = order_of(k, (uint32_t)i);
-          L.mass[at] = mass_at(k);
+          if (mass) L.mass[at] = mass_at(k);
         }
-      });
+      }
+    });
+    __syncthreads();
+    return L.count <= kList;
+  };
+  // The threshold by digits of the key of 11, 11 and 10 bits, a histogram in LDS each: the largest key at and above which there is
+  // `want` (entries, or mass), and what is wanted of those at it.
+  auto select = [&](bool mass, u64 want, u64& rest) {
+    uint32_t key = 0;
+    int have = 0;  // bits of the key that are known
+    for (int d = 0; d < 3; d++) {
+      const int bits = d < 2 ? 11 : 10, shift = 32 - have - bits;
       __syncthreads();
-      if (L.count <= kList) {
+      for (int i = tid; i < kBins; i += kWide) L.bins[i] = 0;
+      __syncthreads();
+      row.each([&](uint32_t k, int i) {
+        if (!k || !left(k, i) || (have && (k >> (32 - have)) != key >> (32 - have))) return;
+        atomicAdd(&L.bins[k >> shift & ((1u << bits) - 1)], mass ? mass_at(k) : 1ull);
+      });
+      int bin;
+      u64 above;
+      pick_bin(L, 1 << bits, want, bin, above);
+      want -= above;
+      key |= (uint32_t)bin << shift;
+      have += bits;
+    }
+    rest = want;
+    return key;
+  };
+  bool listed = false;  // all that is left is in the list
+  if (par.k < a.A && block_sum(L, (u64)valid) > (u64)par.k) {
+    if (par.k <= kWide) {
+      // the k-th largest of the threads' largest keys bounds the k-th largest of all from below
+      uint32_t cur = 0;
+      for (int bit = 31; bit >= (sizeof(T) == 2 ? 16 : 0); bit--)
+        if (__syncthreads_count(best >= (cur | (1u << bit))) >= par.k) cur |= 1u << bit;
+      if (cur && gather(cur, top, true)) {
         const u64 mine = tid < L.count ? L.order[tid] : 0;
         int rank = 0;
-        u64 before = above;
-        compare(mine, rank, before);
-        const int kept = __syncthreads_count(tid < L.count && before < want);
-        cut_at(tid < L.count && rank == kept - 1, mine);
-      } else {
-        u64 rest;
-        const uint32_t k = select(true, want, rest);
-        const u64 each = mass_at(k), of = each ? (rest + each - 1) / each : 1;
-        const int at = index_at(k, of);
-        if (k > thr) cut = a.A;
-        thr = k;
-        cut = at < cut ? at : cut;
+        u64 before = 0;
+        compare(L, mine, rank, before);
+        cut_at(L, tid < L.count && rank == par.k - 1, mine, thr, cut);
+        listed = true;
       }
     }
-    auto left_at = [&](uint32_t k, int i) {
-      if (!k || !left(k, i)) return 0ull;
-      const u64 m = mass_at(k);
-      return m >= need ? m : 0ull;
-    };
+    if (!listed) {
+      u64 rest;
+      const uint32_t k = select(false, (u64)par.k, rest);
+      cut = index_at(k, rest);
+      thr = k;
+    }
+  }
+  if (listed) {
+    draw_listed(L, a, n, par, thr, cut);
+    return;
+  }
+  if (par.p < 1.0) {
+    // What falls into the bin where the threshold lies is few enough for the list, unless many are equal.
+    const Bins bins(a, par, top);
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kWide) L.bins[i] = 0;
+    __syncthreads();
     u64 s = 0;
-    row.each([&](uint32_t k, int i) { s += left_at(k, i); });
-    const u64 mine = wave_sum(s);
-    const u64 total = block_sum(s);  // L.wave: the wavefronts' sums
-    u64 before = 0;
-    for (int i = 0; i < w; i++) before += L.wave[i];
-    const u64 target = (u64)((double)par.u * (double)total);
-    if (mine && before <= target && (before + mine > target || before + mine == total)) {
-      for (int at = row.from; at < row.to; at += 64 * V) {
-        uint32_t k[V];
-        u64 m[V], here = 0;
-        row.keys(at, k);
-#pragma unroll
-        for (int j = 0; j < V; j++) here += m[j] = left_at(k[j], at + V * l + j);
-        const u64 incl = wave_scan(here), all = __shfl(incl, 63);
-        if (all && (before + all > target || before + all == total)) {
-          u64 run = before + incl - here;
-          int first = -1;  // of the lane's entries: the first that exceeds, or (u rounded up to 1) the last there is
-          u64 got = 0;
-#pragma unroll
-          for (int j = 0; j < V; j++) {
-            run += m[j];
-            if (m[j] && (run > target || run == total) && first < 0) {
-              first = j;
-              got = m[j];
-            }
-          }
-          const u64 who = __ballot(first >= 0);
-          if (l == __ffsll((unsigned long long)who) - 1) {
-            a.act[n] = at + V * l + first;
-            if (a.logp) a.logp[n] = (float)log((double)got / (double)total);
-          }
-          break;
-        }
-        before += all;
+    row.each([&](uint32_t k, int i) {
+      if (!k || !left(k, i)) return;
+      const u64 m = mass_at(k);
+      s += m;
+      if (m) atomicAdd(&L.bins[kBins - 1 - bins(k)], m);
+    });
+    const u64 want = (u64)ceil(par.p * (double)block_sum(L, s));
+    int bin;
+    u64 above;
+    pick_bin(L, kBins, want, bin, above);
+    bin = kBins - 1 - bin;
+    __syncthreads();
+    if (tid == 0) L.count = 0;
+    __syncthreads();
+    row.each([&](uint32_t k, int i) {
+      if (!k || bins(k) != bin || !left(k, i)) return;
+      const int at = atomicAdd(&L.count, 1);
+      if (at < kList) {
+        L.order[at] = order_of(k, (uint32_t)i);
+        L.mass[at] = mass_at(k);
       }
+    });
+    __syncthreads();
+    if (L.count <= kList) {
+      const u64 mine = tid < L.count ? L.order[tid] : 0;
+      int rank = 0;
+      u64 before = above;
+      compare(L, mine, rank, before);
+      const int kept = __syncthreads_count(tid < L.count && before < want);
+      cut_at(L, tid < L.count && rank == kept - 1, mine, thr, cut);
+    } else {
+      u64 rest;
+      const uint32_t k = select(true, want, rest);
+      const u64 each = mass_at(k), of = each ? (rest + each - 1) / each : 1;
+      const int at = index_at(k, of);
+      if (k > thr) cut = a.A;
+      thr = k;
+      cut = at < cut ? at : cut;
     }
+  }
+  auto left_at = [&](uint32_t k, int i) {
+    if (!k || !left(k, i)) return 0ull;
+    const u64 m = mass_at(k);
+    return m >= need ? m : 0ull;
+  };
+  u64 s = 0;
+  row.each([&](uint32_t k, int i) { s += left_at(k, i); });
+  const u64 mine = wave_sum(s);
+  const u64 total = block_sum(L, s);  // L.wave: the wavefronts' sums
+  u64 before = 0;
+  for (int i = 0; i < w; i++) before += L.wave[i];
+  const u64 target = (u64)((double)par.u * (double)total);
+  if (mine && before <= target && (before + mine > target || before + mine == total))
+    draw_in_part<T>(a, n, row, left_at, before, target, total);
+}
+
+template <typename T> __global__ void __launch_bounds__(kWide) k_draw_wide(const DrawArgs a) {
+  __shared__ WideLds L;
+  __shared__ double table[kTable];
+  static_assert(kTable == kWide, "an entry each");
+  table[threadIdx.x] = exp2((double)threadIdx.x / kTable);
+  for (long n = blockIdx.x; n < a.N; n += gridDim.x) draw_row<T>(L, table, a, n);
+}
+
+// ---- few wide rows: several blocks each -------------------------------------------------------------------------
+// A row's entries in 64 parts, a wavefront each, 16 blocks to a row; what they find out goes through memory from one launch to the next:
+//   k_split_keys   the largest key, how many may be taken, a lower bound of the k-th largest
+//   k_split_masses top-k: the entries above that bound, listed; top-p: the masses by bins; neither: the parts' sums
+//   k_split_bin    top-p: the bin where the threshold lies
+//   k_split_border top-p: that bin's entries, listed, and the parts' sums of the ones above it
+//   k_split_draw   the threshold among the listed, the draw; or all of it from the start, where a list is too short
+// Whole numbers add up in any order, so the launches may use atomics.
+constexpr int kSplit = 16, kParts = 64;
+struct SplitRow {
+  u64 bins[kBins], order[kList], mass[kList], sums[kParts], want, above;
+  uint32_t top[kSplit], bound[kSplit], share[kSplit];
+  int valid[kSplit], count, bin, greedy, pad;  // (whole words of 64 bits)
+};
+enum SplitKind { kNone, kGreedy, kTopK, kTopP, kPlain, kFallBack };
+
+struct SplitState {
+  Par par;
+  uint32_t top, bound;
+  SplitKind kind;
+  __device__ __forceinline__ SplitState(const DrawArgs& a, const SplitRow& r, long n) : par(par_of(a, n)), top(0), bound(0) {
+    long valid = 0;
+    uint32_t share = 0xffffffffu;
+    for (int i = 0; i < kSplit; i++) {
+      top = r.top[i] > top ? r.top[i] : top;
+      bound = r.bound[i] > bound ? r.bound[i] : bound;
+      share = r.share[i] < share ? r.share[i] : share;
+      valid += r.valid[i];
+    }
+    bound = share > bound ? share : bound;
+    kind = top == 0 ? kNone : par.greedy ? kGreedy : par.k < valid ? (bound ? kTopK : kFallBack) : par.p < 1.0 ? kTopP : kPlain;
+  }
+};
+
+template <typename T> __global__ void __launch_bounds__(256) k_split_keys(const DrawArgs a, SplitRow* rows) {
+  __shared__ uint32_t tops[4];
+  __shared__ int valids[4];
+  const long n = blockIdx.y;
+  const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), b = blockIdx.x;
+  SplitRow& r = rows[n];
+  const Par par = par_of(a, n);
+  for (int i = b * 256 + tid; i < kBins; i += kSplit * 256) r.bins[i] = 0;
+  if (b == 0 && tid == 0) r.count = 0, r.greedy = a.A;
+  const Row<T> row(a, n, 4 * b + w, kParts);
+  uint32_t best = 0;
+  int valid = 0;
+  row.each([&](uint32_t k, int) {
+    best = k > best ? k : best;
+    valid += k != 0;
+  });
+  const uint32_t top = wave_max(best);
+  const u64 v = wave_sum((u64)valid);
+  if (l == 0) tops[w] = top, valids[w] = (int)v;
+  // of the threads' largest keys the k-th, one of at least k; and the (k / blocks)-th: with every block's, the least of these is too
+  uint32_t bound = 0, share = 0;
+  const int blocks = (a.A + 4 * Row<T>::size(a.A, kParts) - 1) / (4 * Row<T>::size(a.A, kParts));  // that have entries
+  const long of = (par.k + blocks - 1) / blocks;
+  if (!par.greedy && par.k <= kList && par.k < a.A) {
+    for (int bit = 31; bit >= (sizeof(T) == 2 ? 16 : 0); bit--) {
+      if (__syncthreads_count(best >= (bound | (1u << bit))) >= par.k) bound |= 1u << bit;
+      if (__syncthreads_count(best >= (share | (1u << bit))) >= of) share |= 1u << bit;
+    }
+  }
+  if (b >= blocks) share = 0xffffffffu;
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t t = 0;
+    int all = 0;
+    for (int i = 0; i < 4; i++) {
+      t = tops[i] > t ? tops[i] : t;
+      all += valids[i];
+    }
+    r.top[b] = t;
+    r.valid[b] = all;
+    r.bound[b] = bound;
+    r.share[b] = share;
+  }
+}
+
+// An entry into the row's list, while there is room.
+__device__ __forceinline__ void list(SplitRow& r, uint32_t k, int i, u64 m) {
+  const int at = atomicAdd(&r.count, 1);
+  if (at < kList) {
+    r.order[at] = order_of(k, (uint32_t)i);
+    r.mass[at] = m;
+  }
+}
+
+template <typename T> __global__ void __launch_bounds__(256) k_split_masses(const DrawArgs a, SplitRow* rows) {
+  __shared__ double table[kTable];
+  __shared__ u64 bins[kBins];
+  const long n = blockIdx.y;
+  const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), b = blockIdx.x;
+  SplitRow& r = rows[n];
+  const SplitState s(a, r, n);
+  if (s.kind == kNone || s.kind == kFallBack) return;
+  const Row<T> row(a, n, 4 * b + w, kParts);
+  if (s.kind == kGreedy) {
+    int first = a.A;
+    row.each([&](uint32_t k, int i) { first = k == s.top && i < first ? i : first; });
+    if (first < a.A) atomicMin(&r.greedy, first);
+    return;
+  }
+  for (int i = tid; i < kTable; i += 256) table[i] = exp2((double)i / kTable);
+  for (int i = tid; i < kBins; i += 256) bins[i] = 0;
+  __syncthreads();
+  auto mass_at = [&](uint32_t k) { return units(mass_of(k, s.top, s.par.c, table), a.bits); };
+  if (s.kind == kTopK) {
+    row.each([&](uint32_t k, int i) {
+      if (k >= s.bound) list(r, k, i, mass_at(k));
+    });
+  } else if (s.kind == kTopP) {
+    const Bins bin(a, s.par, s.top);
+    row.each([&](uint32_t k, int) {
+      const u64 m = k ? mass_at(k) : 0;
+      if (m) atomicAdd(&bins[kBins - 1 - bin(k)], m);
+    });
+    __syncthreads();
+    for (int i = tid; i < kBins; i += 256)
+      if (bins[i]) atomicAdd(&r.bins[i], bins[i]);
+  } else {
+    const u64 need = least(s.par.minp, a.bits);
+    u64 sum = 0;
+    row.each([&](uint32_t k, int) {
+      const u64 m = k ? mass_at(k) : 0;
+      sum += m >= need ? m : 0;
+    });
+    sum = wave_sum(sum);
+    if (l == 0) r.sums[4 * b + w] = sum;
+  }
+}
+
+__global__ void __launch_bounds__(kWide) k_split_bin(const DrawArgs a, SplitRow* rows) {
+  __shared__ WideLds L;
+  const long n = blockIdx.x;
+  SplitRow& r = rows[n];
+  const SplitState s(a, r, n);
+  if (s.kind != kTopP) return;
+  u64 all = 0;
+  for (int i = threadIdx.x; i < kBins; i += kWide) {
+    L.bins[i] = r.bins[i];
+    all += r.bins[i];
+  }
+  const u64 want = (u64)ceil(s.par.p * (double)block_sum(L, all));
+  int bin;
+  u64 above;
+  pick_bin(L, kBins, want, bin, above);
+  if (threadIdx.x == 0) {
+    r.want = want;
+    r.above = above;
+    r.bin = kBins - 1 - bin;
+  }
+}
+
+template <typename T> __global__ void __launch_bounds__(256) k_split_border(const DrawArgs a, SplitRow* rows) {
+  __shared__ double table[kTable];
+  const long n = blockIdx.y;
+  const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), b = blockIdx.x;
+  SplitRow& r = rows[n];
+  const SplitState s(a, r, n);
+  if (s.kind != kTopP) return;
+  for (int i = tid; i < kTable; i += 256) table[i] = exp2((double)i / kTable);
+  __syncthreads();
+  const Row<T> row(a, n, 4 * b + w, kParts);
+  const Bins bin(a, s.par, s.top);
+  const int border = r.bin;
+  const u64 need = least(s.par.minp, a.bits);
+  u64 sum = 0;
+  row.each([&](uint32_t k, int i) {
+    const int at = k ? bin(k) : kBins;
+    if (at > border) return;
+    const u64 m = units(mass_of(k, s.top, s.par.c, table), a.bits);
+    if (at == border) list(r, k, i, m);
+    else sum += m >= need ? m : 0;
+  });
+  sum = wave_sum(sum);
+  if (l == 0) r.sums[4 * b + w] = sum;
+}
+
+template <typename T> __global__ void __launch_bounds__(kWide) k_split_draw(const DrawArgs a, SplitRow* rows) {
+  __shared__ WideLds L;
+  __shared__ double table[kTable];
+  __shared__ u64 sums[kParts];
+  const long n = blockIdx.x;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  SplitRow& r = rows[n];
+  const SplitState s(a, r, n);
+  if (s.kind == kNone || s.kind == kGreedy) {
+    if (tid == 0) {
+      a.act[n] = s.kind == kNone ? -1 : r.greedy;
+      if (a.logp) a.logp[n] = s.kind == kNone ? -INFINITY : 0.f;
+    }
+    return;
+  }
+  table[tid] = exp2((double)tid / kTable);
+  const bool uses_list = s.kind == kTopK || s.kind == kTopP;
+  if (s.kind == kFallBack || (uses_list && r.count > kList)) {
+    draw_row<T>(L, table, a, n);
+    return;
+  }
+  uint32_t thr = 1;
+  int cut = a.A;
+  u64 mine = 0, before = r.above;
+  int rank = 0;
+  if (uses_list) {
+    if (tid == 0) L.count = r.count;
+    if (tid < r.count) {
+      mine = L.order[tid] = r.order[tid];
+      L.mass[tid] = r.mass[tid];
+    }
+    __syncthreads();
+    if (s.kind == kTopK) {
+      before = 0;
+      compare(L, mine, rank, before);
+      cut_at(L, tid < L.count && rank == s.par.k - 1, mine, thr, cut);
+      draw_listed(L, a, n, s.par, thr, cut);
+      return;
+    }
+    compare(L, mine, rank, before);
+  }
+  if (tid < kParts) sums[tid] = r.sums[tid];
+  const bool kept = s.kind == kTopP && tid < L.count && before < r.want;
+  if (s.kind == kTopP) {
+    const int of = __syncthreads_count(kept);
+    cut_at(L, kept && rank == of - 1, mine, thr, cut);
+  }
+  __syncthreads();
+  const u64 need = least(s.par.minp, a.bits);
+  if (kept && L.mass[tid] >= need) atomicAdd(&sums[(int)(0xffffffffu - (uint32_t)mine) / Row<T>::size(a.A, kParts)], L.mass[tid]);
+  __syncthreads();
+  u64 total = 0, front = 0, part = 0;
+  for (int i = 0; i < kParts; i++) total += sums[i];
+  const u64 target = (u64)((double)s.par.u * (double)total);
+  for (int i = 0; i < kParts; i++) {  // the part where the sum exceeds, for the first wavefront
+    part = sums[i];
+    if (part && (front + part > target || front + part == total)) {
+      if (w == 0) {
+        auto left_at = [&](uint32_t k, int e) {
+          if (!k || !(k > thr || (k == thr && e <= cut))) return 0ull;
+          const u64 m = units(mass_of(k, s.top, s.par.c, table), a.bits);
+          return m >= need ? m : 0ull;
+        };
+        draw_in_part<T>(a, n, Row<T>(a, n, i, kParts), left_at, front, target, total);
+      }
+      return;
+    }
+    front += part;
   }
 }
 
@@ -743,7 +1021,20 @@ template <typename T> int draw_t(const DrawArgs& a, hipStream_t st) {
   if (a.A <= 64) k_draw_wave<T, 1><<<n, 256, 0, st>>>(a);
   else if (a.A <= 256) k_draw_wave<T, 4><<<n, 256, 0, st>>>(a);
   else if (a.A <= 1024) k_draw_wave<T, 16><<<n, 256, 0, st>>>(a);
-  else k_draw_wide<T><<<(unsigned)(a.N < most ? a.N : most), kWide, 0, st>>>(a);
+  else if (draw_split(a.N, a.A)) {
+    SplitRow* rows = (SplitRow*)scratch(kSlotDraw, (size_t)a.N * sizeof(SplitRow));
+    if (!rows) return PH_ERR_NOMEM;
+    const dim3 parts(kSplit, (unsigned)a.N);
+    k_split_keys<T><<<parts, 256, 0, st>>>(a, rows);
+    k_split_masses<T><<<parts, 256, 0, st>>>(a, rows);
+    if (a.top_p) {
+      k_split_bin<<<(unsigned)a.N, kWide, 0, st>>>(a, rows);
+      k_split_border<T><<<parts, 256, 0, st>>>(a, rows);
+    }
+    k_split_draw<T><<<(unsigned)a.N, kWide, 0, st>>>(a, rows);
+  } else {
+    k_draw_wide<T><<<(unsigned)(a.N < most ? a.N : most), kWide, 0, st>>>(a);
+  }
   PH_LAUNCH_CHECK();
   return PH_OK;
 }

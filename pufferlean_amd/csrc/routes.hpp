@@ -214,4 +214,8 @@ inline long delta_segments(long chunks, long units, int P) {
   return n < 2 || chunks < 8 ? 1 : n;
 }
 
+// ---- Draw from filtered logits ------------------------------------------------------------------------------
+// Whether N rows of A entries take several blocks each.
+inline bool draw_split(long N, long A) { return N <= 128 && A >= 16384; }
+
 }  // namespace ph

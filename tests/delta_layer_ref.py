@@ -55,27 +55,21 @@ def filtered(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
     t = t if t >= 0 else 1.0
     if x.max() == -np.inf:
         return -1, -np.inf, 1.0
-    order = sorted((i for i in range(len(x)) if x[i] > -np.inf), key=lambda i: (-x[i], i))
+    order = np.lexsort((np.arange(len(x)), -x))  # by falling logit, of equal ones by index
+    order = order[x[order] > -np.inf]
     if t == 0 or p <= 0:
-        return order[0], 0.0, 1.0
+        return int(order[0]), 0.0, 1.0
     with np.errstate(invalid="ignore", over="ignore"):
         mass = np.where(x == x.max(), 1.0, np.exp((x - x.max()) / t))
     if top_k is not None and top_k > 0:
         order = order[:top_k]
     near = 1.0
     if p < 1:
-        total, got, left = sum(mass[order]), 0.0, []
-        for i in order:
-            if left and got >= p * total:
-                break
-            left.append(i)
-            got += mass[i]
-            near = min(near, abs(got - p * total) / total) if len(set(x[order])) > 1 else near
-        order = left
-    order = sorted(i for i in order if mass[i] >= min(m, 1.0))
-    total, got, act = sum(mass[order]), 0.0, None
-    for i in order:
-        got += mass[i]
-        if act is None and got > u * total:
-            act = i
-    return act, float(np.log(mass[act] / total)), near
+        got = np.cumsum(mass[order])
+        if len(set(x[order])) > 1:
+            near = float(np.abs(got - p * got[-1]).min() / got[-1])
+        order = order[:1 + int(np.sum(got[:-1] < p * got[-1]))]
+    order = np.sort(order[mass[order] >= min(m, 1.0)])
+    got = np.cumsum(mass[order])
+    act = int(order[np.argmax(got > u * got[-1])])
+    return act, float(np.log(mass[act] / got[-1])), near
