@@ -776,8 +776,8 @@ template <typename T> __global__ void __launch_bounds__(kWide) k_draw_wide(const
 constexpr int kSplit = 16, kParts = 64;
 struct SplitRow {
   u64 bins[kBins], order[kList], mass[kList], sums[kParts], want, above;
-  uint32_t top[kSplit], bound[kSplit], share[kSplit];
-  int valid[kSplit], count, bin, greedy, pad;  // (whole words of 64 bits)
+  uint32_t top[kSplit], share[kSplit];
+  int valid[kSplit], count, bin, greedy, pad;
 };
 enum SplitKind { kNone, kGreedy, kTopK, kTopP, kPlain, kFallBack };
 
@@ -787,14 +787,12 @@ struct SplitState {
   SplitKind kind;
   __device__ __forceinline__ SplitState(const DrawArgs& a, const SplitRow& r, long n) : par(par_of(a, n)), top(0), bound(0) {
     long valid = 0;
-    uint32_t share = 0xffffffffu;
+    bound = 0xffffffffu;
     for (int i = 0; i < kSplit; i++) {
       top = r.top[i] > top ? r.top[i] : top;
-      bound = r.bound[i] > bound ? r.bound[i] : bound;
-      share = r.share[i] < share ? r.share[i] : share;
+      bound = r.share[i] < bound ? r.share[i] : bound;
       valid += r.valid[i];
     }
-    bound = share > bound ? share : bound;
     kind = top == 0 ? kNone : par.greedy ? kGreedy : par.k < valid ? (bound ? kTopK : kFallBack) : par.p < 1.0 ? kTopP : kPlain;
   }
 };
@@ -818,15 +816,13 @@ template <typename T> __global__ void __launch_bounds__(256) k_split_keys(const 
   const uint32_t top = wave_max(best);
   const u64 v = wave_sum((u64)valid);
   if (l == 0) tops[w] = top, valids[w] = (int)v;
-  // of the threads' largest keys the k-th, one of at least k; and the (k / blocks)-th: with every block's, the least of these is too
-  uint32_t bound = 0, share = 0;
+  // of the threads' largest keys the (k / blocks)-th: at least that many entries reach it, and in all at least k the least block's
+  uint32_t share = 0;
   const int blocks = (a.A + 4 * Row<T>::size(a.A, kParts) - 1) / (4 * Row<T>::size(a.A, kParts));  // that have entries
   const long of = (par.k + blocks - 1) / blocks;
   if (!par.greedy && par.k <= kList && par.k < a.A) {
-    for (int bit = 31; bit >= (sizeof(T) == 2 ? 16 : 0); bit--) {
-      if (__syncthreads_count(best >= (bound | (1u << bit))) >= par.k) bound |= 1u << bit;
+    for (int bit = 31; bit >= (sizeof(T) == 2 ? 16 : 0); bit--)
       if (__syncthreads_count(best >= (share | (1u << bit))) >= of) share |= 1u << bit;
-    }
   }
   if (b >= blocks) share = 0xffffffffu;
   __syncthreads();
@@ -839,7 +835,6 @@ template <typename T> __global__ void __launch_bounds__(256) k_split_keys(const 
     }
     r.top[b] = t;
     r.valid[b] = all;
-    r.bound[b] = bound;
     r.share[b] = share;
   }
 }

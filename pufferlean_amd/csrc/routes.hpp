@@ -215,7 +215,10 @@ inline long delta_segments(long chunks, long units, int P) {
 }
 
 // ---- Draw from filtered logits ------------------------------------------------------------------------------
-// Whether N rows of A entries take several blocks each.
-inline bool draw_split(long N, long A) { return N <= 128 && A >= 16384; }
+// Whether N rows of A entries take sixteen blocks each, in three launches or (top-p) five, or one block in one. One block to a row
+// leaves CUs idle, but a launch more costs 5 us, and top-k alone is short either way. Several blocks / one, bf16, us without a
+// filter, with top-k and with top-p: 128x16384 27 / 18, 36 / 22, 54 / 37; 128x32768 30 / 30, 42 / 24, 70 / 63; 128x65536 38 / 54,
+// 51 / 30, 90 / 113; 64x131072, filters mixed: 95 / 205.
+inline bool draw_split(long N, long A) { return N <= 128 && A >= 49152; }
 
 }  // namespace ph

@@ -11,7 +11,8 @@ DRIVER = r"""
 #include <cstdlib>
 #include "routes.hpp"
 int main(int, char** a) {
-  std::printf("%ld\n", ph::delta_segments(std::atol(a[1]), std::atol(a[2]), std::atoi(a[3])));
+  if (a[3][0] == 's') std::printf("%d\n", ph::draw_split(std::atol(a[1]), std::atol(a[2])));
+  else std::printf("%ld\n", ph::delta_segments(std::atol(a[1]), std::atol(a[2]), std::atoi(a[3])));
   return 0;
 }
 """
@@ -37,3 +38,8 @@ def test_long_tests_reach_segments(segments):
     for T, units, P in ((300, 2, 32), (530, 2, 64), (515, 1, 128), (767, 1, 64), (410, 4, 32), (400, 8, 32), (600, 4, 32), (700, 36, 32)):
         for steps in (16, 32):
             assert segments(-(-T // steps), units, P) > 1
+
+
+@pytest.mark.parametrize("N,A,split", [(1, 49151, 0), (1, 49152, 1), (128, 60001, 1), (129, 60001, 0), (4096, 1000, 0)])
+def test_wide_rows_of_the_draw(segments, N, A, split):
+    assert segments(N, A, "s") == split
