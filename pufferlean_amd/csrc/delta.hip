@@ -35,8 +35,21 @@
 // transposed state too), in the accumulator layout of the 16x16 matrix instructions: lane l holds rows 4 (l / 16) + r, column
 // l % 16. That layout is also the one of the instruction's right operand when the contraction runs over
 // those rows, so S, U and dY go from one product to the next without leaving the registers, and all of a wavefront's chain
-// stays in its columns. bf16 rows enter the products as they are (their norms are factors outside) and values
-// held in fp32 as the sum of two bf16, 16 bits of them; fp32 takes the fp32 matrix instructions.
+// stays in its columns. bf16 rows enter the products as they are (their norms are factors outside). Values held in fp32 enter
+// as sums of bf16: of three, 24 bits, on the way of the state (its own and U's part in it; M, T and the join are fp32
+// products), of two, 16 bits, elsewhere, where the result is rounded to bf16 anyway; only dA and ddt_bias, sums in fp32 of terms
+// of either sign, show it (6e-6 of their norm; three parts everywhere would not fit the LDS of 128x128). fp32 takes the fp32
+// matrix instructions.
+//
+// Long sequences of few heads do not fill the chip, so time is cut into segments: a first launch runs each from a zero state and,
+// without values, from the unit matrix, which gives what it adds to a state (Psi) and what it multiplies it with (Phi); a second
+// joins the segments' start states in order; the third runs them again from those. The gradient does the same in reverse, with Phi^T.
+//
+// Measured, bf16: 64 steps of 2048 sequences x 8 heads of 64x64 forward with kept states 396 us (4.1 TB/s of what it moves; a large
+// copy 5.2), gradient 1054 us: vector instructions issue for half of it, matrix instructions for an eighth, two wavefronts on a
+// SIMD wait at ten barriers a chunk for the rest (three, with 168 registers, spill: 1548 us). 2048 steps of 8 x 4 heads of
+// 128x128 183 and 400 us; 8192 of 2 x 8 of 64x64 162 and 276 (in one piece 1575 and 4663 at first). A single step of 4096 x 8 heads of
+// 64x64 195 us, 5.6 TB/s.
 #include "common.hpp"
 #include "kernels.hpp"
 #include "lanes.hpp"
@@ -182,9 +195,23 @@ template <> struct Pair<false> {
   f4 hi;
   __device__ __forceinline__ void set(f4 v) { hi = v; }
 };
+// With a third part, 24 bits: what the state itself is made of.
+template <bool BF> struct Trip : Pair<BF> {
+  s4 low;
+  __device__ __forceinline__ void set(f4 v) {
+    Pair<BF>::set(v);
+    const u2 h = __builtin_bit_cast(u2, this->hi), m = __builtin_bit_cast(u2, this->lo);
+    const f4 r = {v[0] - __builtin_bit_cast(float, h[0] << 16) - __builtin_bit_cast(float, m[0] << 16),
+                  v[1] - __builtin_bit_cast(float, h[0] & 0xffff0000u) - __builtin_bit_cast(float, m[0] & 0xffff0000u),
+                  v[2] - __builtin_bit_cast(float, h[1] << 16) - __builtin_bit_cast(float, m[1] << 16),
+                  v[3] - __builtin_bit_cast(float, h[1] & 0xffff0000u) - __builtin_bit_cast(float, m[1] & 0xffff0000u)};
+    low = __builtin_bit_cast(s4, u2{bf16x2_rne(r[0], r[1]), bf16x2_rne(r[2], r[3])});
+  }
+};
+template <> struct Trip<false> : Pair<false> {};
 // acc += a b: a exact rows and b of pairs, and both of pairs (the product of the two remainders is below what they keep).
-template <bool BF, int N>
-__device__ __forceinline__ f4 dot2(const typename Elem<BF>::unit* a, const Pair<BF>* b, f4 acc) {
+template <bool BF, int N, typename B>
+__device__ __forceinline__ f4 dot2(const typename Elem<BF>::unit* a, const B* b, f4 acc) {
   typename Elem<BF>::unit h[N];
 #pragma unroll
   for (int i = 0; i < N; i++) h[i] = b[i].hi;
@@ -195,6 +222,17 @@ __device__ __forceinline__ f4 dot2(const typename Elem<BF>::unit* a, const Pair<
     acc = dot<N>(a, h, acc);
   }
   return acc;
+}
+// a exact rows and all three parts of b, the smallest first.
+template <bool BF, int N>
+__device__ __forceinline__ f4 dot2w(const typename Elem<BF>::unit* a, const Trip<BF>* b, f4 acc) {
+  if constexpr (BF) {
+    typename Elem<BF>::unit h[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) h[i] = b[i].low;
+    acc = dot<N>(a, h, acc);
+  }
+  return dot2<BF, N>(a, b, acc);
 }
 template <bool BF, int N> __device__ __forceinline__ f4 dot3(const Pair<BF>* a, const Pair<BF>* b, f4 acc) {
   typename Elem<BF>::unit h[N];
@@ -429,18 +467,19 @@ template <bool BF, int LD, int N> __device__ __forceinline__ f4 mat_values(int t
   else return p.hi;
 }
 
-// A chunk's M, P and T = (I + M)^-1. Of T the diagonal blocks; of M these also as they are, for the substitution.
+// A chunk's M, P and T = (I + M)^-1. Of T the diagonal blocks; of M these also as they are, for the substitution. M and T, through
+// which the state goes, stay fp32, and so do their products: small ones, and fp32 saves cutting their operands in parts.
 template <bool BF, bool WITH_P> struct Scores {
   static constexpr int CH = Elem<BF>::CH, UD = CH + 4, TD = 20;
-  Mat<BF, CH * UD> M;
+  Mat<false, CH * UD> M;
   Mat<BF, WITH_P ? CH * UD : 1> P;
-  Mat<BF, CH * TD> Tinv;
+  Mat<false, CH * TD> Tinv;
 };
 
 // M (and P) of the chunk: tiles on and below the diagonal, dealt out over the wavefronts.
 template <bool BF, int P, int LD, bool WITH_P>
 __device__ __forceinline__ void score_tiles(int tid, const Rows<Elem<BF>::CH>& r, const typename Elem<BF>::type* Qs,
-                                            const typename Elem<BF>::type* Ks, Mat<BF, Scores<BF, WITH_P>::CH * Scores<BF, WITH_P>::UD>& M,
+                                            const typename Elem<BF>::type* Ks, Mat<false, Scores<BF, WITH_P>::CH * Scores<BF, WITH_P>::UD>& M,
                                             Mat<BF, WITH_P ? Scores<BF, WITH_P>::CH * Scores<BF, WITH_P>::UD : 1>& Pm, float* diag, float scale) {
   constexpr int CH = Elem<BF>::CH, NB = CH / 16, NT = P / 16, UD = CH + 4, TILES = NB * (NB + 1) / 2;
   const int l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -471,7 +510,7 @@ __device__ __forceinline__ void score_tiles(int tid, const Rows<Elem<BF>::CH>& r
         continue;
       }
     }
-    put_mat<BF, UD>(tid, M, 16 * bj, 16 * bi, acc);
+    put_mat<false, UD>(tid, M, 16 * bj, 16 * bi, acc);
     if (bi == bj) {
 #pragma unroll
       for (int k = 0; k < 4; k++) diag[(16 * bi + i0 + k) * 16 + j] = acc[k];
@@ -480,7 +519,7 @@ __device__ __forceinline__ void score_tiles(int tid, const Rows<Elem<BF>::CH>& r
 }
 
 // The diagonal blocks of (I + M)^-1, one column per lane of a wavefront's first CH.
-template <bool BF, int CH, int N> __device__ __forceinline__ void invert_blocks(int tid, const float* diag, Mat<BF, N>& Tinv) {
+template <int CH, int N> __device__ __forceinline__ void invert_blocks(int tid, const float* diag, Mat<false, N>& Tinv) {
   const int l = tid & 63;
   if (l >= CH) return;
   const int o = l & ~15, c = l & 15;
@@ -498,46 +537,37 @@ template <bool BF, int CH, int N> __device__ __forceinline__ void invert_blocks(
     x[i] = s;
   }
 #pragma unroll
-  for (int i = 0; i < 16; i += 4) {
-    Pair<BF> p;
-    p.set(f4{x[i], x[i + 1], x[i + 2], x[i + 3]});
-    *reinterpret_cast<typename Elem<BF>::unit*>(Tinv.hi + l * 20 + i) = p.hi;
-    if constexpr (BF) *reinterpret_cast<s4*>(Tinv.lo + l * 20 + i) = p.lo;
-  }
+  for (int i = 0; i < 16; i += 4) *reinterpret_cast<f4*>(Tinv.hi + l * 20 + i) = f4{x[i], x[i + 1], x[i + 2], x[i + 3]};
 }
 
 // U = T Y by blocks, T's blocks below the diagonal through M.
-template <bool BF, int NM, int NI> __device__ __forceinline__ void solve(int tid, const Mat<BF, NI>& Tinv, const Mat<BF, NM>& M, const f4* Y, f4* U) {
+template <bool BF, int NM, int NI> __device__ __forceinline__ void solve(int tid, const Mat<false, NI>& Tinv, const Mat<false, NM>& M, const f4* Y, f4* U) {
   constexpr int CH = Elem<BF>::CH, NB = CH / 16, UD = CH + 4;
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
-  Pair<BF> t = mat_col<BF, 20>(tid, Tinv, 0, 0), y;
-  y.set(Y[0]);
-  U[0] = dot3<BF, 1>(&t, &y, zero);
+  f4 t = mat_col<false, 20>(tid, Tinv, 0, 0).hi;
+  U[0] = dot<1>(&t, Y, zero);
   if constexpr (NB == 2) {
-    y.set(-U[0]);
-    t = mat_col<BF, UD>(tid, M, 0, 16);
-    y.set(dot3<BF, 1>(&t, &y, Y[1]));
-    t = mat_col<BF, 20>(tid, Tinv, 16, 0);
-    U[1] = dot3<BF, 1>(&t, &y, zero);
+    f4 y = -U[0];
+    t = mat_col<false, UD>(tid, M, 0, 16).hi;
+    y = dot<1>(&t, &y, Y[1]);
+    t = mat_col<false, 20>(tid, Tinv, 16, 0).hi;
+    U[1] = dot<1>(&t, &y, zero);
   }
 }
 // dY = T^T dU
-template <bool BF, int NM, int NI> __device__ __forceinline__ void solve_t(int tid, const Mat<BF, NI>& Tinv, const Mat<BF, NM>& M, const f4* dU, f4* dY) {
+template <bool BF, int NM, int NI> __device__ __forceinline__ void solve_t(int tid, const Mat<false, NI>& Tinv, const Mat<false, NM>& M, const f4* dU, f4* dY) {
   constexpr int CH = Elem<BF>::CH, NB = CH / 16, UD = CH + 4;
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
-  Pair<BF> t, y;
-  f4 top = dU[0];
+  f4 top = dU[0], t;
   if constexpr (NB == 2) {
-    y.set(dU[1]);
-    t = mat_row<BF, 20>(tid, Tinv, 16, 0);
-    dY[1] = dot3<BF, 1>(&t, &y, zero);
-    y.set(-dY[1]);
-    t = mat_row<BF, UD>(tid, M, 0, 16);
-    top += dot3<BF, 1>(&t, &y, zero);
+    t = mat_row<false, 20>(tid, Tinv, 16, 0).hi;
+    dY[1] = dot<1>(&t, dU + 1, zero);
+    const f4 y = -dY[1];
+    t = mat_row<false, UD>(tid, M, 0, 16).hi;
+    top += dot<1>(&t, &y, zero);
   }
-  y.set(top);
-  t = mat_row<BF, 20>(tid, Tinv, 0, 0);
-  dY[0] = dot3<BF, 1>(&t, &y, zero);
+  t = mat_row<false, 20>(tid, Tinv, 0, 0).hi;
+  dY[0] = dot<1>(&t, &top, zero);
 }
 
 // States in memory: [K][V] as the caller holds them; the library's own in whole tiles of 16x16, [K tiles][V tiles], each as the
@@ -764,11 +794,11 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
         }
         score_tiles<BF, P, LD, !LOCAL>(tid, R, Qs, Ks, X.M, X.P, diag, scale);
         __syncthreads();
-        if (w == 0) invert_blocks<BF, CH>(tid, diag, X.Tinv);
+        if (w == 0) invert_blocks<CH>(tid, diag, X.Tinv);
         if (w == NT - 1 && once) fill_rows<CH>(tid, Rs[cur ^ 1], gn, A, 0, rows);
         f4 Y[NB], O[NB];
         {
-          Pair<BF> Sp[NT];
+          Trip<BF> Sp[NT];
 #pragma unroll
           for (int m = 0; m < NT; m++) Sp[m].set(S[m]);
 #pragma unroll
@@ -776,7 +806,7 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
             unit x[NT];
 #pragma unroll
             for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, Ks, 16 * n, 16 * m);
-            const f4 ks = dot2<BF, NT>(x, Sp, zero);
+            const f4 ks = dot2w<BF, NT>(x, Sp, zero);
             Y[n] = rows4(tid, R.be, 16 * n) * (widen(col_unit<LD>(tid, Vs, 16 * n, 16 * w)) -
                                           (rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n)) * (ks));
             if constexpr (!LOCAL) {
@@ -804,9 +834,8 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
             continue;
           }
         }
-        Pair<BF> Up[NB];
         if constexpr (!LOCAL) {
-          Pair<BF> x[NB];
+          Pair<BF> Up[NB], x[NB];
 #pragma unroll
           for (int n = 0; n < NB; n++) Up[n].set(U[n]);
           x[0] = mat_col<BF, UD>(tid, X.P, 0, 0);
@@ -822,15 +851,16 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
 #pragma unroll
             for (int i = 0; i < 4; i++) stf(Vs + (16 * n + 4 * (l >> 4) + i) * LD + 16 * w + (l & 15), O[n][i]);
         }
+        Trip<BF> Uw[NB];
 #pragma unroll
-        for (int n = 0; n < NB; n++) Up[n].set((rows4(tid, R.dc, 16 * n) * rows4(tid, R.rk, 16 * n)) * (U[n]));
+        for (int n = 0; n < NB; n++) Uw[n].set((rows4(tid, R.dc, 16 * n) * rows4(tid, R.rk, 16 * n)) * (U[n]));
         const float c0 = R.c0;
 #pragma unroll
         for (int m = 0; m < NT; m++) {
           unit kt[NB];
 #pragma unroll
           for (int n = 0; n < NB; n++) kt[n] = col_unit<LD>(tid, Ks, 16 * n, 16 * m);
-          S[m] = dot2<BF, NB>(kt, Up, c0 * S[m]);
+          S[m] = dot2w<BF, NB>(kt, Uw, c0 * S[m]);
         }
         cut |= starts;
         y_at = t0;
@@ -868,7 +898,7 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
 
 // The segments' start states in order, S <- Phi S + Psi, a block per sequence's head (back: the gradients of their end states in
 // reverse, dS <- Phi^T dS + Xi). An episode's start in a segment leaves only what the segment adds.
-template <bool BF, int P, bool BACK> __global__ void __launch_bounds__(4 * P) k_delta_join(const Args s, const GradArgs o) {
+template <int P, bool BACK> __global__ void __launch_bounds__(4 * P) k_delta_join(const Args s, const GradArgs o) {
   constexpr int NT = P / 16, LD = P + 4;
   __shared__ __attribute__((aligned(16))) float F[64 * LD];  // half of Phi's rows (P = 128), or all
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -910,9 +940,6 @@ template <bool BF, int P, bool BACK> __global__ void __launch_bounds__(4 * P) k_
       f4 next[NT];
 #pragma unroll
       for (int m = 0; m < NT; m++) next[m] = m < own.tk && w < own.tv ? N[m] : zero;
-      Pair<BF> Sp[NT];
-#pragma unroll
-      for (int m = 0; m < NT; m++) Sp[m].set(S[m]);
 #pragma unroll
       for (int half = 0; half < HALVES; half++) {
         __syncthreads();
@@ -931,18 +958,18 @@ template <bool BF, int P, bool BACK> __global__ void __launch_bounds__(4 * P) k_
         if constexpr (!BACK) {
 #pragma unroll
           for (int m = 0; m < HT; m++) {
-            Pair<BF> x[NT];
+            f4 x[NT];
 #pragma unroll
-            for (int n = 0; n < NT; n++) x[n].set(row_unit<LD>(tid, F, 16 * m, 16 * n));
-            next[HT * half + m] = dot3<BF, NT>(x, Sp, next[HT * half + m]);
+            for (int n = 0; n < NT; n++) x[n] = row_unit<LD>(tid, F, 16 * m, 16 * n);
+            next[HT * half + m] = dot<NT>(x, S, next[HT * half + m]);
           }
         } else {
 #pragma unroll
           for (int m = 0; m < NT; m++) {
-            Pair<BF> x[HT];
+            f4 x[HT];
 #pragma unroll
-            for (int n = 0; n < HT; n++) x[n].set(col_unit<LD>(tid, F, 16 * n, 16 * m));
-            next[m] = dot3<BF, HT>(x, Sp + HT * half, next[m]);
+            for (int n = 0; n < HT; n++) x[n] = col_unit<LD>(tid, F, 16 * n, 16 * m);
+            next[m] = dot<HT>(x, S + HT * half, next[m]);
           }
         }
       }
@@ -969,9 +996,10 @@ template <bool BF, int P> struct BwdLds {
     float sums[4][NT][CH];  // when U has been read: <q^, dQ^>, <k^, dK^>, the parts of S_0 and of dS_c
   };
   T dY[P * UD], Ulo[BF ? P * UD : 1], dYlo[BF ? P * UD : 1];
-  Mat<BF, CH * UD> M, Pm;  // then F and E
+  Mat<false, CH * UD> M;  // then F
+  Mat<BF, CH * UD> Pm;    // then E
   union {
-    Mat<BF, CH * 20> Tinv;
+    Mat<false, CH * 20> Tinv;
     float W[CH * CP];  // P_ij dO_i U_j - M_ij dY_i U_j
   };
   union {
@@ -986,8 +1014,9 @@ template <bool BF, int P> struct BwdLocalLds {
   using T = typename Elem<BF>::type;
   static constexpr int CH = Elem<BF>::CH, LD = P + Elem<BF>::pad, CP = CH + 4, UD = CH + 4;
   T Q[CH * LD], K[CH * LD], dO[CH * LD];
-  Mat<BF, CH * UD> M, Pm;
-  Mat<BF, CH * 20> Tinv;
+  Mat<false, CH * UD> M;
+  Mat<BF, CH * UD> Pm;
+  Mat<false, CH * 20> Tinv;
   float diag[CH * 16];
   Rows<CH> R[2];
 };
@@ -1149,7 +1178,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
         const bool fresh = R.starts >> lo & 1;  // S_0 may be anything
         score_tiles<BF, P, LD, true>(tid, R, L.Q, L.K, L.M, L.Pm, L.diag, scale);
         __syncthreads();
-        if (w == 0) invert_blocks<BF, CH>(tid, L.diag, L.Tinv);
+        if (w == 0) invert_blocks<CH>(tid, L.diag, L.Tinv);
         if (w == NT - 1 && once) fill_rows<CH>(tid, L.R[cur ^ 1], gn, A, 0, rows_at(c - 1));
         // contractions over the state's rows, HT tiles at a time: all of a wide state's operands would not fit the registers
         constexpr int HT = NT < 4 ? NT : 4;
@@ -1280,7 +1309,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             const int j = 16 * bj + (l & 15);
             const double Gj = R.G[j];
             const int segj = R.seg[j];
-            const f4 pv = mat_values<BF, UD>(tid, L.Pm, 16 * bj, 16 * bi), mv = mat_values<BF, UD>(tid, L.M, 16 * bj, 16 * bi);
+            const f4 pv = mat_values<BF, UD>(tid, L.Pm, 16 * bj, 16 * bi), mv = mat_row<false, UD>(tid, L.M, 16 * bj, 16 * bi).hi;
             const f4 be = rows4(tid, R.be, 16 * bi);
 #pragma unroll
             for (int i4 = 0; i4 < 4; i4++) {
@@ -1292,7 +1321,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
               f[i4] = on && j < i ? -dec * be[i4] * f[i4] : 0.f;
             }
             put_mat<BF, UD>(tid, L.Pm, 16 * bj, 16 * bi, e);
-            put_mat<BF, UD>(tid, L.M, 16 * bj, 16 * bi, f);
+            put_mat<false, UD>(tid, L.M, 16 * bj, 16 * bi, f);
           }
           renew(tid, l);
           // products over V for this wavefront's columns of K: dO S_0^T, dY S_0^T, U dS^T
@@ -1379,7 +1408,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
 #pragma unroll
               for (int m = 0; m <= n; m++) {
                 e[m] = mat_col<BF, UD>(tid, L.Pm, 16 * m, 16 * n);
-                f[m] = mat_col<BF, UD>(tid, L.M, 16 * m, 16 * n);
+                f[m].set(mat_col<false, UD>(tid, L.M, 16 * m, 16 * n).hi);
               }
               if (n == 0) {
                 dQ[n] = dot3<BF, 1>(e, kp2, X1[n]);
@@ -1391,7 +1420,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
 #pragma unroll
               for (int m = n; m < NB; m++) {
                 e[m] = mat_row<BF, UD>(tid, L.Pm, 16 * n, 16 * m);
-                f[m] = mat_row<BF, UD>(tid, L.M, 16 * n, 16 * m);
+                f[m].set(mat_row<false, UD>(tid, L.M, 16 * n, 16 * m).hi);
               }
               if (n == NB - 1) dK[n] += dot3<BF, 1>(f + n, kp2 + n, dot3<BF, 1>(e + n, qp2 + n, zero));
               else dK[n] += dot3<BF, NB>(f, kp2, dot3<BF, NB>(e, qp2, zero));
@@ -1740,7 +1769,7 @@ template <bool BF> int fwd_t(const Args& a, hipStream_t st) {
     constexpr int P = decltype(p)::value;
     if (a.segs > 1) {
       k_delta_fwd<BF, P, true><<<blocks_of(a.units * (a.segs - 1) * a.parts), 4 * P, 0, st>>>(a);
-      k_delta_join<BF, P, false><<<blocks_of(a.units), 4 * P, 0, st>>>(a, GradArgs{});
+      k_delta_join<P, false><<<blocks_of(a.units), 4 * P, 0, st>>>(a, GradArgs{});
     }
     k_delta_fwd<BF, P, false><<<blocks_of(a.units * a.segs), 4 * P, 0, st>>>(a);
   });
@@ -1755,7 +1784,7 @@ template <bool BF> int bwd_t(const Args& a, const GradArgs& o, float* dA, float*
     if (a.segs > 1) {
       k_delta_fwd<BF, P, true><<<blocks_of(a.units * (a.segs - 1)), 4 * P, 0, st>>>(a);
       k_delta_bwd<BF, P, true><<<blocks_of(a.units * (a.segs - 1)), 4 * P, 0, st>>>(a, o);
-      k_delta_join<BF, P, true><<<blocks_of(a.units), 4 * P, 0, st>>>(a, o);
+      k_delta_join<P, true><<<blocks_of(a.units), 4 * P, 0, st>>>(a, o);
     }
     k_delta_bwd<BF, P, false><<<blocks_of(a.units * a.segs), 4 * P, 0, st>>>(a, o);
   });
