@@ -475,13 +475,13 @@ typedef struct {
   const float *A, *dt_bias, *done, *first, *h0;
   float scale;
 } ph_delta_args;
-/* y [.., H, V], which may not be q, k or v; h_out (may be NULL) receives the state after the last step, before done[T-1]
+/* y [.., H, V], which may not be an input; h_out (may be NULL) receives the state after the last step, before done[T-1]
  * clears it (the next call's `first` does); it may be h0. keep (may be NULL): fp32, ph_delta_keep_floats values, the states
  * that the gradient starts from. */
 int ph_delta_scan(const ph_delta_args* a, void* y, long y_t, long y_b, long y_h, float* h_out, float* keep, void* stream);
 size_t ph_delta_keep_floats(const ph_delta_args* a);
 /* Gradient from the forward's arguments (h0 is not read) and keep; dh (fp32, may be NULL: zero) is the gradient of h_out. Each
- * output may be NULL; dq, dk, dv, da, db have the activations' dtype and strides of their own and may not be inputs; dA and
+ * output may be NULL; dq, dk, dv, da, db have the activations' dtype and strides of their own and may not be inputs or one another; dA and
  * ddt_bias (fp32 [H], overwritten) are summed in an order fixed by the shape; dh0 (may be dh) is the gradient of h0. */
 typedef struct {
   void *dq, *dk, *dv, *da, *db;

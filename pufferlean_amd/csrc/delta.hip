@@ -1849,6 +1849,8 @@ long chunk_steps(int dtype) { return dtype == PH_BF16 ? Elem<true>::CH : Elem<fa
 
 using namespace ph;
 
+bool is_input(const ph_delta_args& p, const void* t) { return t == p.q || t == p.k || t == p.v || t == p.a || t == p.b; }
+
 extern "C" size_t ph_delta_keep_floats(const ph_delta_args* p) {
   if (!p) return 0;
   const size_t c = (size_t)chunk_steps(p->dtype);
@@ -1862,7 +1864,7 @@ extern "C" int ph_delta_scan(const ph_delta_args* p, void* y, long y_t, long y_b
   if (p->B == 0) return PH_OK;
   PH_REQUIRE(p->T >= 1, "delta_scan: no steps");
   PH_REQUIRE(y, "delta_scan: y missing");
-  PH_REQUIRE(y != p->q && y != p->k && y != p->v, "delta_scan: y may not be q, k or v");
+  PH_REQUIRE(!is_input(*p, y), "delta_scan: y may not be an input");
   Args a = args_of(*p);
   a.y = y; a.y_t = y_t; a.y_b = y_b; a.y_h = y_h; a.h_out = h_out; a.keep = keep;
   set_segments(a, false, p->dtype);
@@ -1890,8 +1892,12 @@ extern "C" int ph_delta_scan_grad(const ph_delta_args* p, const float* keep, con
   }
   PH_REQUIRE(p->T >= 1, "delta_scan_grad: no steps");
   PH_REQUIRE(dy && keep, "delta_scan_grad: dy or the kept states missing");
-  for (const void* out : {(const void*)g->dq, (const void*)g->dk, (const void*)g->dv})
-    PH_REQUIRE(!out || (out != p->q && out != p->k && out != p->v && out != dy), "delta_scan_grad: a gradient may not be an input");
+  const void* outs[] = {g->dq, g->dk, g->dv, g->da, g->db};
+  for (int i = 0; i < 5; i++) {
+    if (!outs[i]) continue;
+    PH_REQUIRE(!is_input(*p, outs[i]) && outs[i] != dy, "delta_scan_grad: a gradient may not be an input");
+    for (int j = 0; j < i; j++) PH_REQUIRE(outs[i] != outs[j], "delta_scan_grad: two gradients are the same");
+  }
   Args a = args_of(*p);
   GradArgs o{};
   o.dy = dy; o.dy_t = dy_t; o.dy_b = dy_b; o.dy_h = dy_h; o.keep = keep; o.dh = dh;
@@ -1926,7 +1932,7 @@ extern "C" int ph_delta_step(const ph_delta_args* p, void* y, long y_b, long y_h
   PH_TRY(check(*p, "delta_step"));
   if (p->T == 0 || p->B == 0) return PH_OK;
   PH_REQUIRE(y && h, "delta_step: y or the state missing");
-  PH_REQUIRE(y != p->q && y != p->k && y != p->v, "delta_step: y may not be q, k or v");
+  PH_REQUIRE(!is_input(*p, y), "delta_step: y may not be an input");
   Args a = args_of(*p);
   a.y = y; a.y_b = y_b; a.y_h = y_h;
   return p->dtype == PH_BF16 ? step_t<uint16_t>(a, h, as_stream(stream)) : step_t<float>(a, h, as_stream(stream));

@@ -134,3 +134,14 @@ def test_draw_refuses(kw, text):
     k = dict(dtype=L.PH_F32, x=NZ, ld=1 << 21, N=3, A=4, u=NZ, act=NZ)
     k.update(kw)
     refused(L.lib().ph_sample_filtered(k["dtype"], k["x"], k["ld"], k["N"], k["A"], k["u"], None, None, None, None, k["act"], None, None), text)
+
+
+def test_scan_refuses_what_it_would_overwrite():
+    lib, a = L.lib(), delta_args(a=6 * NZ, b=7 * NZ)
+    for y in (a.a, a.b):
+        refused(lib.ph_delta_scan(C.byref(a), y, 1, 1, 1, None, None, None), "y may not be")
+        refused(lib.ph_delta_step(C.byref(delta_args(T=1, a=6 * NZ, b=7 * NZ)), y, 1, 1, NZ, None), "y may not be")
+    for kw in (dict(da=a.a), dict(db=a.a), dict(da=a.b), dict(dk=a.b)):
+        refused(lib.ph_delta_scan_grad(C.byref(a), NZ, 5 * NZ, 1, 1, 1, None, C.byref(L.DeltaGrads(**kw)), None), "may not be an input")
+    for kw in (dict(dq=9 * NZ, dk=9 * NZ), dict(dk=9 * NZ, dv=9 * NZ), dict(da=9 * NZ, db=9 * NZ), dict(dv=9 * NZ, da=9 * NZ)):
+        refused(lib.ph_delta_scan_grad(C.byref(a), NZ, 5 * NZ, 1, 1, 1, None, C.byref(L.DeltaGrads(**kw)), None), "two gradients")

@@ -157,3 +157,14 @@ def test_captured(gpu, A):
         assert torch.equal(out[0], act) and torch.equal(out[1], logp)
         D.sample_filtered(x.flip(1).contiguous(), u, **par)
         torch.cuda.synchronize()
+
+
+def test_the_widest_rows(gpu):
+    """2^20 entries in sixteen blocks, and the same rows in one block each where there are more than 128 of them."""
+    A = 1 << 20
+    x, u = cu(1, 2, A, scale=2.0), numbers(2, 130)
+    for par in (dict(), dict(temperature=0.8, top_k=700, top_p=0.9, min_p=1e-3), dict(top_p=0.7)):
+        check(x, u[:2], **par)
+        act, logp = D.sample_filtered(x[:1].expand(130, A), u, **par)
+        few = [D.sample_filtered(x[:1].expand(65, A), u[i:i + 65], **par) for i in (0, 65)]
+        assert torch.equal(act, torch.cat([f[0] for f in few])) and torch.equal(logp, torch.cat([f[1] for f in few]))
