@@ -45,10 +45,10 @@
 // without values, from the unit matrix, which gives what it adds to a state (Psi) and what it multiplies it with (Phi); a second
 // joins the segments' start states in order; the third runs them again from those. The gradient does the same in reverse, with Phi^T.
 //
-// Measured, bf16: 64 steps of 2048 sequences x 8 heads of 64x64 forward with kept states 396 us (4.1 TB/s of what it moves; a large
-// copy 5.2), gradient 1054 us: vector instructions issue for half of it, matrix instructions for an eighth, two wavefronts on a
+// Measured, bf16: 64 steps of 2048 sequences x 8 heads of 64x64 forward with kept states 400 us (4.1 TB/s of what it moves; a large
+// copy 5.2), gradient 1051 us: vector instructions issue for half of it, matrix instructions for an eighth, two wavefronts on a
 // SIMD wait at ten barriers a chunk for the rest (three, with 168 registers, spill: 1548 us). 2048 steps of 8 x 4 heads of
-// 128x128 183 and 400 us; 8192 of 2 x 8 of 64x64 162 and 276 (in one piece 1575 and 4663 at first). A single step of 4096 x 8 heads of
+// 128x128 174 and 389 us; 8192 of 2 x 8 of 64x64 139 and 246 (in one piece 1575 and 4663 at first). A single step of 4096 x 8 heads of
 // 64x64 195 us, 5.6 TB/s.
 #include "common.hpp"
 #include "kernels.hpp"
@@ -85,7 +85,7 @@ struct Args {
   long y_t, y_b, y_h;
   float *h_out, *keep;
   float* start;  // [segs][units] states at the segments' starts (more than one segment)
-  float *psi, *phi;  // [segs][units]: what a segment adds to its start state, and what it multiplies it with
+  float *psi, *phi;  // [segs][units]: what a segment adds to its start state, and what it multiplies it with (parts = 2: tiles transposed)
   int* cut;          // [segs][units]: an episode starts in the segment, and nothing passes it
   int local_from, parts;  // of these: segments from local_from on, segs - 1 of them; both, or phi alone
 };
@@ -591,6 +591,12 @@ __device__ __forceinline__ f4 own_tile_t(int tid, gin<float> s, Own d, int m, in
 __device__ __forceinline__ void put_own_tile(int tid, gout<float> s, Own d, int m, int w, f4 x) {
   if (m < d.tk && w < d.tv) *reinterpret_cast<gout<f4>>(s + (m * d.tv + w) * 256 + 4 * (tid & 63)) = x;
 }
+// The same into a matrix whose tiles lie transposed: there a lane's four values are columns 4 (l / 16) + 0..3 of row l % 16.
+__device__ __forceinline__ void put_own_tile_t(int tid, gout<float> s, Own d, int m, int w, f4 x) {
+  const int l = tid & 63;
+  gout<float> p = s + (m * d.tv + w) * 256 + (4 * (l >> 4) + 16 * (l >> 2 & 3)) * 4 + (l & 3);
+  if (m < d.tk && w < d.tv) p[0] = x[0], p[4] = x[1], p[8] = x[2], p[12] = x[3];
+}
 // All tiles of column block w of a caller's state, or (T) of the transposed one's; zero outside. Addresses are clamped and not
 // skipped: a load that a branch guards is waited for before the next one.
 template <int NT, bool TR> __device__ __forceinline__ void get_state(int tid, gin<float> s, int K, int V, int w, f4* S) {
@@ -888,7 +894,9 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
       const long at = seg * e.units + unit_id;
       gout<float> out = (gout<float>)(part ? e.phi : e.psi) + at * own.floats();
 #pragma unroll
-      for (int m = 0; m < NT; m++) put_own_tile(tid, out, own, m, w, S[m]);
+      for (int m = 0; m < NT; m++)
+        if (part && e.parts == 2) put_own_tile_t(tid, out, own, m, w, S[m]);  // for Phi S; the gradient takes Phi^T dS
+        else put_own_tile(tid, out, own, m, w, S[m]);
       if (part && tid == 0) e.cut[at] = cut != 0;
     } else if (e.h_out && last == e.T) {
       put_state<NT>(tid, (gout<float>)e.h_out + unit_id * e.K * e.V, e.K, e.V, w, S);
@@ -896,88 +904,61 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
   }
 }
 
-// The segments' start states in order, S <- Phi S + Psi, a block per sequence's head (back: the gradients of their end states in
-// reverse, dS <- Phi^T dS + Xi). An episode's start in a segment leaves only what the segment adds.
+__host__ __device__ __forceinline__ long join_blocks(const Args& s) { return (s.units + 7) / 8 * 8 * (up16(s.V) / 16); }
+// The segments' start states in order, S <- Phi S + Psi (back: the gradients of their end states in reverse, dS <- Phi^T dS + Xi). An
+// episode's start in a segment leaves only what the segment adds. A chain of small fp32 products, so it is spread thin: a block
+// per 16 columns of a sequence's head, a wavefront per 16 rows, which exchange their tiles through LDS; Phi's come from memory as
+// they are needed, DEEP segments ahead. 32 segments of 2 x 8 heads of 64x64 24 us (54 with all columns in one block and Phi in LDS), 8
+// of 8 x 4 heads of 128x128 11 to 13 (25; 27 with a head's columns on different XCDs).
 template <int P, bool BACK> __global__ void __launch_bounds__(4 * P) k_delta_join(const Args s, const GradArgs o) {
-  constexpr int NT = P / 16, LD = P + 4;
-  __shared__ __attribute__((aligned(16))) float F[64 * LD];  // half of Phi's rows (P = 128), or all
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int NT = P / 16, DEEP = P <= 64 ? 4 : 2;
+  __shared__ __attribute__((aligned(16))) f4 X[2][NT][64];
+  __shared__ int cuts[kMostSegments];
+  const int tid = threadIdx.x, l = tid & 63, m = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Own own = {up16(s.K) / 16, up16(s.V) / 16}, sq = {own.tk, own.tk};
-  const f4 zero = {0.f, 0.f, 0.f, 0.f};
-  for (long unit_id = blockIdx.x; unit_id < s.units; unit_id += gridDim.x) {
-    f4 S[NT];
+  const long n = s.segs - 1, items = join_blocks(s);
+  for (long item = blockIdx.x; item < items; item += gridDim.x) {
+    // a head's columns share its Phi: on one XCD (every eighth block), in whose L2 it then lies
+    const long unit_id = item / 8 / own.tv * 8 + item % 8;
+    const int w = (int)(item / 8 % own.tv);
+    if (unit_id >= s.units) continue;
+    __syncthreads();
+    for (int i = tid; i < n; i += 4 * P) cuts[i] = s.cut[(BACK ? n - i : i) * s.units + unit_id];
+    f4 S = {0.f, 0.f, 0.f, 0.f}, phi[DEEP][NT], add[DEEP];
     const float* from = BACK ? o.dh : s.h0;
-    if (from) {
-      get_state<NT, false>(tid, (gin<float>)from + unit_id * s.K * s.V, s.K, s.V, w, S);
-    } else {
-#pragma unroll
-      for (int m = 0; m < NT; m++) S[m] = zero;
-    }
-#pragma unroll
-    for (int m = 0; m < NT; m++)
-      put_own_tile(tid, (gout<float>)(BACK ? o.dend + (s.segs - 1) * s.units * own.floats() : s.start) + unit_id * own.floats(), own, m, w, S[m]);
-    // a segment's Phi (the wavefront's tiles of it) and what it adds are loaded while the one before is passed, where the
-    // registers hold both (128: 26 us for seven segments that way, 15 without)
-    constexpr bool AHEAD = P <= 64;
-    constexpr int HALVES = (P + 63) / 64, HT = P < 64 ? NT : 4;  // Phi goes through LDS by HT tiles of rows
-    f4 phi[HALVES][HT], N[NT];
-    int cut;
-    auto load = [&](long i) {
-      const long at = (BACK ? s.segs - 1 - i : i) * s.units + unit_id;  // the segment that is passed
-      gin<float> add = (gin<float>)(BACK ? o.xi : s.psi) + at * own.floats(), f = (gin<float>)s.phi + at * sq.floats();
-      cut = ((gin<int>)s.cut)[at];
-#pragma unroll
-      for (int m = 0; m < NT; m++) N[m] = own_tile(tid, add, own, m, w);
-#pragma unroll
-      for (int half = 0; half < HALVES; half++)
-#pragma unroll
-        for (int m = 0; m < HT; m++) phi[half][m] = own_tile(tid, f, sq, HT * half + m, w);
+    if (from && m < own.tk)
+      get_state<1, false>(tid, (gin<float>)from + unit_id * s.K * s.V + 16 * m * s.V, s.K - 16 * m, s.V, w, &S);
+    auto out = [&](long i) {  // the state that is handed to segment i, in the order of the passes
+      return (gout<float>)(BACK ? o.dend : s.start) + ((BACK ? n - i : i) * s.units + unit_id) * own.floats();
     };
-    if (AHEAD && s.segs > 1) load(0);
-    for (long i = 0; i + 1 < s.segs; i++) {
-      if (!AHEAD) load(i);
-      const bool passes = !__builtin_amdgcn_readfirstlane(cut);
-      f4 next[NT];
+    put_own_tile(tid, out(0), own, m, w, S);
+    auto load = [&](int d, long i) {
+      const long at = (BACK ? n - i : i) * s.units + unit_id;  // the segment that is passed
+      gin<float> f = (gin<float>)s.phi + at * sq.floats();
+      add[d] = own_tile(tid, (gin<float>)(BACK ? o.xi : s.psi) + at * own.floats(), own, m, w);
 #pragma unroll
-      for (int m = 0; m < NT; m++) next[m] = m < own.tk && w < own.tv ? N[m] : zero;
+      for (int j = 0; j < NT; j++) phi[d][j] = BACK ? own_tile(tid, f, sq, j, m) : own_tile(tid, f, sq, m, j);
+    };
 #pragma unroll
-      for (int half = 0; half < HALVES; half++) {
-        __syncthreads();
-        if (passes) {
+    for (int d = 0; d < DEEP; d++) load(d, d < n ? d : n - 1);
+    for (long i0 = 0; i0 < n; i0 += DEEP) {
 #pragma unroll
-          for (int m = 0; m < HT; m++) {
-            const int l = tid & 63;
-            float* to = F + (16 * m + 4 * (l >> 4)) * LD + 16 * w + (l & 15);
+      for (int d = 0; d < DEEP; d++) {
+        const long i = i0 + d;
+        if (i >= n) break;
+        X[i & 1][m][l] = S;
+        __syncthreads();  // tiles of the segment before last may be overwritten: all have read them in front of this
+        S = add[d];
+        if (!__builtin_amdgcn_readfirstlane(cuts[i])) {
 #pragma unroll
-            for (int r = 0; r < 4; r++) to[r * LD] = HT * half + m < own.tk && w < own.tk ? phi[half][m][r] : 0.f;
+          for (int j = 0; j < NT; j++) {
+            if (j >= own.tk) break;
+            const f4 x = X[i & 1][j][l];
+            S = dot<1>(&phi[d][j], &x, S);
           }
         }
-        __syncthreads();
-        if (AHEAD && half == HALVES - 1 && i + 2 < s.segs) load(i + 1);
-        if (!passes) continue;
-        if constexpr (!BACK) {
-#pragma unroll
-          for (int m = 0; m < HT; m++) {
-            f4 x[NT];
-#pragma unroll
-            for (int n = 0; n < NT; n++) x[n] = row_unit<LD>(tid, F, 16 * m, 16 * n);
-            next[HT * half + m] = dot<NT>(x, S, next[HT * half + m]);
-          }
-        } else {
-#pragma unroll
-          for (int m = 0; m < NT; m++) {
-            f4 x[HT];
-#pragma unroll
-            for (int n = 0; n < HT; n++) x[n] = col_unit<LD>(tid, F, 16 * n, 16 * m);
-            next[m] = dot<HT>(x, S + HT * half, next[m]);
-          }
-        }
-      }
-      gout<float> out = (gout<float>)(BACK ? o.dend + (s.segs - 2 - i) * s.units * own.floats() : s.start + (i + 1) * s.units * own.floats()) + unit_id * own.floats();
-#pragma unroll
-      for (int m = 0; m < NT; m++) {
-        S[m] = next[m];
-        put_own_tile(tid, out, own, m, w, S[m]);
+        load(d, i + DEEP < n ? i + DEEP : n - 1);
+        put_own_tile(tid, out(i + 1), own, m, w, S);
       }
     }
   }
@@ -1769,7 +1750,7 @@ template <bool BF> int fwd_t(const Args& a, hipStream_t st) {
     constexpr int P = decltype(p)::value;
     if (a.segs > 1) {
       k_delta_fwd<BF, P, true><<<blocks_of(a.units * (a.segs - 1) * a.parts), 4 * P, 0, st>>>(a);
-      k_delta_join<P, false><<<blocks_of(a.units), 4 * P, 0, st>>>(a, GradArgs{});
+      k_delta_join<P, false><<<blocks_of(join_blocks(a)), 4 * P, 0, st>>>(a, GradArgs{});
     }
     k_delta_fwd<BF, P, false><<<blocks_of(a.units * a.segs), 4 * P, 0, st>>>(a);
   });
@@ -1784,7 +1765,7 @@ template <bool BF> int bwd_t(const Args& a, const GradArgs& o, float* dA, float*
     if (a.segs > 1) {
       k_delta_fwd<BF, P, true><<<blocks_of(a.units * (a.segs - 1)), 4 * P, 0, st>>>(a);
       k_delta_bwd<BF, P, true><<<blocks_of(a.units * (a.segs - 1)), 4 * P, 0, st>>>(a, o);
-      k_delta_join<P, true><<<blocks_of(a.units), 4 * P, 0, st>>>(a, o);
+      k_delta_join<P, true><<<blocks_of(join_blocks(a)), 4 * P, 0, st>>>(a, o);
     }
     k_delta_bwd<BF, P, false><<<blocks_of(a.units * a.segs), 4 * P, 0, st>>>(a, o);
   });

@@ -206,10 +206,11 @@ inline long ssm_chunk(long T, long B, long G, long per, int N, bool grad) {
 // blocks at the occupancy that their registers leave (P = 32: four blocks of two wavefronts to a CU, 64: two of four, 128: one of
 // eight). A segment more costs a step of the join and, past the round, the others' share of the CU; and there are two passes
 // over the steps, so whole sequences of less than eight chunks stay one. Forward and gradient, bf16, us by segments: 8192 steps of 16
-// units of 64x64 8: 315, 703; 16: 190, 382; 32: 154, 260; 48: 173, 300; 64: 187, 280. 1024 of 64 units of 64x64 4: 100, 202; 8: 74, 134;
-// 16: 78, 133; 32: 102, 165; of 32x32 8: 61, 126; 16: 49, 87; 32: 60, 106. 2048 of 32 units of 128x128 4: 202, 630; 8: 167, 388; 16: 198, 411.
+// units of 64x64 8: 308, 709; 16: 178, 375; 32: 133, 246; 48: 144, 280; 64: 144, 259. 1024 of 64 units of 64x64 4: 101, 204; 8: 75, 134;
+// 16: 74, 138; 32: 87, 158; of 32x32 8: 62, 128; 16: 48, 87; 32: 58, 105. 2048 of 32 units of 128x128 4: 215, 641; 8: 168, 389; 16: 185, 402.
+constexpr int kMostSegments = 1024;
 inline long delta_segments(long chunks, long units, int P) {
-  const long most = (chunks + 1) / 2, want = (P <= 32 ? 1024 : P <= 64 ? 512 : 256) / units;
+  const long most = (chunks + 1) / 2, want = (P <= 32 ? kMostSegments : P <= 64 ? 512 : 256) / units;
   const long n = want < most ? want : most;
   return n < 2 || chunks < 8 ? 1 : n;
 }
