@@ -36,10 +36,8 @@
 // l % 16. That layout is also the one of the instruction's right operand when the contraction runs over
 // those rows, so S, U and dY go from one product to the next without leaving the registers, and all of a wavefront's chain
 // stays in its columns. bf16 rows enter the products as they are (their norms are factors outside). Values held in fp32 enter
-// as sums of bf16: of three, 24 bits, on the way of the state (its own and U's part in it; M, T and the join are fp32
-// products), of two, 16 bits, elsewhere, where the result is rounded to bf16 anyway; only dA and ddt_bias, sums in fp32 of terms
-// of either sign, show it (6e-6 of their norm; three parts everywhere would not fit the LDS of 128x128). fp32 takes the fp32
-// matrix instructions.
+// as sums of bf16: of three, 24 bits, on the way of the state and of y (M, P, T and the join are fp32 products), of two, 16 bits, in
+// the gradient. fp32 takes the fp32 matrix instructions.
 //
 // Long sequences of few heads do not fill the chip, so time is cut into segments: a first launch runs each from a zero state and,
 // without values, from the unit matrix, which gives what it adds to a state (Psi) and what it multiplies it with (Phi); a second
@@ -467,20 +465,20 @@ template <bool BF, int LD, int N> __device__ __forceinline__ f4 mat_values(int t
   else return p.hi;
 }
 
-// A chunk's M, P and T = (I + M)^-1. Of T the diagonal blocks; of M these also as they are, for the substitution. M and T, through
-// which the state goes, stay fp32, and so do their products: small ones, and fp32 saves cutting their operands in parts.
+// A chunk's M, P and T = (I + M)^-1. Of T the diagonal blocks; of M these also as they are, for the substitution. They stay
+// fp32, and so do their products: small ones, and fp32 saves cutting their operands in parts.
 template <bool BF, bool WITH_P> struct Scores {
   static constexpr int CH = Elem<BF>::CH, UD = CH + 4, TD = 20;
   Mat<false, CH * UD> M;
-  Mat<BF, WITH_P ? CH * UD : 1> P;
+  Mat<false, WITH_P ? CH * UD : 1> P;
   Mat<false, CH * TD> Tinv;
 };
 
 // M (and P) of the chunk: tiles on and below the diagonal, dealt out over the wavefronts.
-template <bool BF, int P, int LD, bool WITH_P>
+template <bool BF, int P, int LD, bool WITH_P, bool PARTS, int NP>
 __device__ __forceinline__ void score_tiles(int tid, const Rows<Elem<BF>::CH>& r, const typename Elem<BF>::type* Qs,
                                             const typename Elem<BF>::type* Ks, Mat<false, Scores<BF, WITH_P>::CH * Scores<BF, WITH_P>::UD>& M,
-                                            Mat<BF, WITH_P ? Scores<BF, WITH_P>::CH * Scores<BF, WITH_P>::UD : 1>& Pm, float* diag, float scale) {
+                                            Mat<PARTS, NP>& Pm, float* diag, float scale) {
   constexpr int CH = Elem<BF>::CH, NB = CH / 16, NT = P / 16, UD = CH + 4, TILES = NB * (NB + 1) / 2;
   const int l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   for (int id = w; id < (WITH_P ? 2 : 1) * TILES; id += NT) {
@@ -506,7 +504,7 @@ __device__ __forceinline__ void score_tiles(int tid, const Rows<Elem<BF>::CH>& r
     }
     if constexpr (WITH_P) {
       if (isP) {
-        put_mat<BF, UD>(tid, Pm, 16 * bj, 16 * bi, acc);
+        put_mat<PARTS, UD>(tid, Pm, 16 * bj, 16 * bi, acc);
         continue;
       }
     }
@@ -798,7 +796,7 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
 #pragma unroll
           for (int m = 0; m < NT; m++) S[m] = zero;
         }
-        score_tiles<BF, P, LD, !LOCAL>(tid, R, Qs, Ks, X.M, X.P, diag, scale);
+        score_tiles<BF, P, LD, !LOCAL, false>(tid, R, Qs, Ks, X.M, X.P, diag, scale);
         __syncthreads();
         if (w == 0) invert_blocks<CH>(tid, diag, X.Tinv);
         if (w == NT - 1 && once) fill_rows<CH>(tid, Rs[cur ^ 1], gn, A, 0, rows);
@@ -818,7 +816,7 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
             if constexpr (!LOCAL) {
 #pragma unroll
               for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, Qs, 16 * n, 16 * m);
-              O[n] = (scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n)) * (dot2<BF, NT>(x, Sp, zero));
+              O[n] = (scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n)) * (dot2w<BF, NT>(x, Sp, zero));
             }
           }
         }
@@ -841,16 +839,13 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
           }
         }
         if constexpr (!LOCAL) {
-          Pair<BF> Up[NB], x[NB];
 #pragma unroll
-          for (int n = 0; n < NB; n++) Up[n].set(U[n]);
-          x[0] = mat_col<BF, UD>(tid, X.P, 0, 0);
-          O[0] = dot3<BF, 1>(x, Up, O[0]);
-          if constexpr (NB == 2) {
-            x[0] = mat_col<BF, UD>(tid, X.P, 0, 16);
-            x[1] = mat_col<BF, UD>(tid, X.P, 16, 16);
-            O[1] = dot3<BF, 2>(x, Up, O[1]);
-          }
+          for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int m = 0; m <= n; m++) {
+              const f4 x = mat_col<false, UD>(tid, X.P, 16 * m, 16 * n).hi;
+              O[n] = dot<1>(&x, U + m, O[n]);
+            }
           // y rests where V was, until the rows are stored behind the next barrier
 #pragma unroll
           for (int n = 0; n < NB; n++)
@@ -1157,7 +1152,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
         }
         __syncthreads();
         const bool fresh = R.starts >> lo & 1;  // S_0 may be anything
-        score_tiles<BF, P, LD, true>(tid, R, L.Q, L.K, L.M, L.Pm, L.diag, scale);
+        score_tiles<BF, P, LD, true, BF>(tid, R, L.Q, L.K, L.M, L.Pm, L.diag, scale);
         __syncthreads();
         if (w == 0) invert_blocks<CH>(tid, L.diag, L.Tinv);
         if (w == NT - 1 && once) fill_rows<CH>(tid, L.R[cur ^ 1], gn, A, 0, rows_at(c - 1));
