@@ -36,8 +36,8 @@
 // l % 16. That layout is also the one of the instruction's right operand when the contraction runs over
 // those rows, so S, U and dY go from one product to the next without leaving the registers, and all of a wavefront's chain
 // stays in its columns. bf16 rows enter the products as they are (their norms are factors outside). Values held in fp32 enter
-// as sums of bf16: of three, 24 bits, on the way of the state and of y (M, P, T and the join are fp32 products), of two, 16 bits, in
-// the gradient. fp32 takes the fp32 matrix instructions.
+// as sums of three bf16, all 24 bits, and the products of a chunk's small matrices and of the join are fp32 ones, so that what is not
+// rounded to bf16 in the end is as precise as from fp32 inputs. fp32 takes the fp32 matrix instructions.
 //
 // Long sequences of few heads do not fill the chip, so time is cut into segments: a first launch runs each from a zero state and,
 // without values, from the unit matrix, which gives what it adds to a state (Psi) and what it multiplies it with (Phi); a second
@@ -156,17 +156,15 @@ __device__ __forceinline__ void renew(int& tid, int& l) {
 template <bool BF> struct Elem { using type = uint16_t; using unit = s4; static constexpr int CH = 32, pad = 8, V = 8; };
 template <> struct Elem<false> { using type = float; using unit = f4; static constexpr int CH = 16, pad = 4, V = 4; };
 
-// acc += a b over N units. bf16 units go in pairs where there are two. No accumulator goes straight from an instruction over
-// 32 to one over 16 or back: of two such instructions in a row the second has read values that the first had not written yet. Their
-// results are added instead.
+// acc += a b over N units; bf16 units go in pairs.
 template <int N> __device__ __forceinline__ f4 dot(const s4* a, const s4* b, f4 acc) {
+  static_assert(N % 2 == 0, "whole pairs");
 #pragma unroll
-  for (int i = 0; i + 1 < N; i += 2) {
+  for (int i = 0; i < N; i += 2) {
     const s8 x = __builtin_shufflevector(a[i], a[i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
     const s8 y = __builtin_shufflevector(b[i], b[i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
     acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), acc, 0, 0, 0);
   }
-  if constexpr (N & 1) acc = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a[N - 1], b[N - 1], acc, 0, 0, 0);
   return acc;
 }
 template <int N> __device__ __forceinline__ f4 dot(const f4* a, const f4* b, f4 acc) {
@@ -177,88 +175,68 @@ template <int N> __device__ __forceinline__ f4 dot(const f4* a, const f4* b, f4 
   return acc;
 }
 
-// fp32 values as operands: for bf16 the nearest bf16 and what it leaves, also rounded to bf16 (the sum is within 2^-17 of
-// the value), else the values themselves.
-template <bool BF> struct Pair {
-  s4 hi, lo;
+// fp32 values as operands: for bf16 three parts, each the nearest bf16 to what the ones before leave (24 bits, all there are), else
+// the values themselves.
+template <bool BF> struct Parts {
+  s4 hi, mid, low;
   __device__ __forceinline__ void set(f4 v) {
-    const uint32_t a = bf16x2_rne(v[0], v[1]), b = bf16x2_rne(v[2], v[3]);
-    hi = __builtin_bit_cast(s4, u2{a, b});
-    const float h0 = __builtin_bit_cast(float, a << 16), h1 = __builtin_bit_cast(float, a & 0xffff0000u);
-    const float h2 = __builtin_bit_cast(float, b << 16), h3 = __builtin_bit_cast(float, b & 0xffff0000u);
-    lo = __builtin_bit_cast(s4, u2{bf16x2_rne(v[0] - h0, v[1] - h1), bf16x2_rne(v[2] - h2, v[3] - h3)});
+    hi = nearest(v);
+    mid = nearest(v);
+    low = nearest(v);
+  }
+  __device__ __forceinline__ f4 sum() const { return (wide(low) + wide(mid)) + wide(hi); }
+
+ private:
+  static __device__ __forceinline__ f4 wide(s4 p) {
+    const u2 u = __builtin_bit_cast(u2, p);
+    return f4{__builtin_bit_cast(float, u[0] << 16), __builtin_bit_cast(float, u[0] & 0xffff0000u), __builtin_bit_cast(float, u[1] << 16),
+              __builtin_bit_cast(float, u[1] & 0xffff0000u)};
+  }
+  static __device__ __forceinline__ s4 nearest(f4& v) {  // and what it leaves of v
+    const s4 p = __builtin_bit_cast(s4, u2{bf16x2_rne(v[0], v[1]), bf16x2_rne(v[2], v[3])});
+    v -= wide(p);
+    return p;
   }
 };
-template <> struct Pair<false> {
+template <> struct Parts<false> {
   f4 hi;
   __device__ __forceinline__ void set(f4 v) { hi = v; }
+  __device__ __forceinline__ f4 sum() const { return hi; }
 };
-// With a third part, 24 bits: what the state itself is made of.
-template <bool BF> struct Trip : Pair<BF> {
-  s4 low;
-  __device__ __forceinline__ void set(f4 v) {
-    Pair<BF>::set(v);
-    const u2 h = __builtin_bit_cast(u2, this->hi), m = __builtin_bit_cast(u2, this->lo);
-    const f4 r = {v[0] - __builtin_bit_cast(float, h[0] << 16) - __builtin_bit_cast(float, m[0] << 16),
-                  v[1] - __builtin_bit_cast(float, h[0] & 0xffff0000u) - __builtin_bit_cast(float, m[0] & 0xffff0000u),
-                  v[2] - __builtin_bit_cast(float, h[1] << 16) - __builtin_bit_cast(float, m[1] << 16),
-                  v[3] - __builtin_bit_cast(float, h[1] & 0xffff0000u) - __builtin_bit_cast(float, m[1] & 0xffff0000u)};
-    low = __builtin_bit_cast(s4, u2{bf16x2_rne(r[0], r[1]), bf16x2_rne(r[2], r[3])});
-  }
-};
-template <> struct Trip<false> : Pair<false> {};
-// acc += a b: a exact rows and b of pairs, and both of pairs (the product of the two remainders is below what they keep).
-template <bool BF, int N, typename B>
-__device__ __forceinline__ f4 dot2(const typename Elem<BF>::unit* a, const B* b, f4 acc) {
-  typename Elem<BF>::unit h[N];
-#pragma unroll
-  for (int i = 0; i < N; i++) h[i] = b[i].hi;
-  acc = dot<N>(a, h, acc);
-  if constexpr (BF) {
-#pragma unroll
-    for (int i = 0; i < N; i++) h[i] = b[i].lo;
-    acc = dot<N>(a, h, acc);
-  }
-  return acc;
-}
-// a exact rows and all three parts of b, the smallest first.
+// acc += a b, the smallest products first: a exact rows and b in parts, and both in parts (products below 2^-24 of the largest
+// are left out).
 template <bool BF, int N>
-__device__ __forceinline__ f4 dot2w(const typename Elem<BF>::unit* a, const Trip<BF>* b, f4 acc) {
+__device__ __forceinline__ f4 dot_parts(const typename Elem<BF>::unit* a, const Parts<BF>* b, f4 acc) {
+  typename Elem<BF>::unit h[N];
   if constexpr (BF) {
-    typename Elem<BF>::unit h[N];
 #pragma unroll
     for (int i = 0; i < N; i++) h[i] = b[i].low;
     acc = dot<N>(a, h, acc);
+#pragma unroll
+    for (int i = 0; i < N; i++) h[i] = b[i].mid;
+    acc = dot<N>(a, h, acc);
   }
-  return dot2<BF, N>(a, b, acc);
+#pragma unroll
+  for (int i = 0; i < N; i++) h[i] = b[i].hi;
+  return dot<N>(a, h, acc);
 }
-template <bool BF, int N> __device__ __forceinline__ f4 dot3(const Pair<BF>* a, const Pair<BF>* b, f4 acc) {
+template <bool BF, int N> __device__ __forceinline__ f4 dot_parts(const Parts<BF>* a, const Parts<BF>* b, f4 acc) {
   typename Elem<BF>::unit h[N];
   if constexpr (BF) {
-#pragma unroll
-    for (int i = 0; i < N; i++) h[i] = a[i].lo;
     typename Elem<BF>::unit g[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) h[i] = a[i].low, g[i] = b[i].hi;
+    acc = dot<N>(h, g, acc);
+#pragma unroll
+    for (int i = 0; i < N; i++) h[i] = a[i].mid, g[i] = b[i].mid;
+    acc = dot<N>(h, g, acc);
 #pragma unroll
     for (int i = 0; i < N; i++) g[i] = b[i].hi;
     acc = dot<N>(h, g, acc);
   }
 #pragma unroll
   for (int i = 0; i < N; i++) h[i] = a[i].hi;
-  return dot2<BF, N>(h, b, acc);
-}
-// acc += a b: a of pairs, b exact columns.
-template <bool BF, int N>
-__device__ __forceinline__ f4 dot2r(const Pair<BF>* a, const typename Elem<BF>::unit* b, f4 acc) {
-  typename Elem<BF>::unit h[N];
-#pragma unroll
-  for (int i = 0; i < N; i++) h[i] = a[i].hi;
-  acc = dot<N>(h, b, acc);
-  if constexpr (BF) {
-#pragma unroll
-    for (int i = 0; i < N; i++) h[i] = a[i].lo;
-    acc = dot<N>(h, b, acc);
-  }
-  return acc;
+  return dot_parts<BF, N>(h, b, acc);
 }
 
 // Units of a matrix in LDS, leading dimension LD. row_unit: row `row` + l % 16, columns `col` + 4 (l / 16) + 0..3 (left
@@ -433,52 +411,36 @@ template <int CH, typename T> __device__ __forceinline__ void fill_rows(int tid,
 }
 __device__ __forceinline__ f4 rows4(int tid, const float* r, int at) { return *reinterpret_cast<const f4*>(r + at + 4 * ((tid & 63) >> 4)); }
 
-// Small matrices of a chunk are kept transposed, as pairs: a tile's lane holds four rows of a column, one access of them.
-template <bool BF, int LD> struct alignas(16) Mat {
-  using T = typename Elem<BF>::type;
-  T hi[LD], lo[BF ? LD : 1];  // LD: elements
+// Small matrices of a chunk are kept transposed, in fp32: a tile's lane holds four rows of a column, one access of them. Their
+// products are fp32 ones: few, and fp32 saves cutting their operands in parts.
+template <int N> struct alignas(16) Mat {
+  float v[N];
 };
-template <bool BF, int LD, int N> __device__ __forceinline__ void put_mat(int tid, Mat<BF, N>& m, int row, int col, f4 v) {
-  const int l = tid & 63, o = (row + (l & 15)) * LD + col + 4 * (l >> 4);
-  Pair<BF> p;
-  p.set(v);
-  *reinterpret_cast<typename Elem<BF>::unit*>(m.hi + o) = p.hi;
-  if constexpr (BF) *reinterpret_cast<s4*>(m.lo + o) = p.lo;
+template <int LD, int N> __device__ __forceinline__ void put_mat(int tid, Mat<N>& m, int row, int col, f4 v) {
+  const int l = tid & 63;
+  *reinterpret_cast<f4*>(m.v + (row + (l & 15)) * LD + col + 4 * (l >> 4)) = v;
 }
-// The left operand of the matrix itself (tile's row `row`, column `col` of the stored, transposed one) and of its transpose.
-template <bool BF, int LD, int N> __device__ __forceinline__ Pair<BF> mat_col(int tid, const Mat<BF, N>& m, int row, int col) {
-  Pair<BF> p;
-  p.hi = col_unit<LD>(tid, m.hi, row, col);
-  if constexpr (BF) p.lo = col_unit<LD>(tid, m.lo, row, col);
-  return p;
+// The left operand of the matrix itself (tile's row `row`, column `col` of the stored, transposed one) and of its transpose, which is
+// also the four values that put_mat of the same place took.
+template <int LD, int N> __device__ __forceinline__ f4 mat_col(int tid, const Mat<N>& m, int row, int col) {
+  return col_unit<LD>(tid, m.v, row, col);
 }
-template <bool BF, int LD, int N> __device__ __forceinline__ Pair<BF> mat_row(int tid, const Mat<BF, N>& m, int row, int col) {
-  Pair<BF> p;
-  p.hi = row_unit<LD>(tid, m.hi, row, col);
-  if constexpr (BF) p.lo = row_unit<LD>(tid, m.lo, row, col);
-  return p;
-}
-// The four values that put_mat of the same place took.
-template <bool BF, int LD, int N> __device__ __forceinline__ f4 mat_values(int tid, const Mat<BF, N>& m, int row, int col) {
-  const Pair<BF> p = mat_row<BF, LD>(tid, m, row, col);
-  if constexpr (BF) return widen(p.hi) + widen(p.lo);
-  else return p.hi;
+template <int LD, int N> __device__ __forceinline__ f4 mat_row(int tid, const Mat<N>& m, int row, int col) {
+  return row_unit<LD>(tid, m.v, row, col);
 }
 
-// A chunk's M, P and T = (I + M)^-1. Of T the diagonal blocks; of M these also as they are, for the substitution. They stay
-// fp32, and so do their products: small ones, and fp32 saves cutting their operands in parts.
+// A chunk's M, P and T = (I + M)^-1. Of T the diagonal blocks; of M these also as they are, for the substitution.
 template <bool BF, bool WITH_P> struct Scores {
   static constexpr int CH = Elem<BF>::CH, UD = CH + 4, TD = 20;
-  Mat<false, CH * UD> M;
-  Mat<false, WITH_P ? CH * UD : 1> P;
-  Mat<false, CH * TD> Tinv;
+  Mat<CH * UD> M;
+  Mat<WITH_P ? CH * UD : 1> P;
+  Mat<CH * TD> Tinv;
 };
 
 // M (and P) of the chunk: tiles on and below the diagonal, dealt out over the wavefronts.
-template <bool BF, int P, int LD, bool WITH_P, bool PARTS, int NP>
+template <bool BF, int P, int LD, bool WITH_P, int NM, int NP>
 __device__ __forceinline__ void score_tiles(int tid, const Rows<Elem<BF>::CH>& r, const typename Elem<BF>::type* Qs,
-                                            const typename Elem<BF>::type* Ks, Mat<false, Scores<BF, WITH_P>::CH * Scores<BF, WITH_P>::UD>& M,
-                                            Mat<PARTS, NP>& Pm, float* diag, float scale) {
+                                            const typename Elem<BF>::type* Ks, Mat<NM>& M, Mat<NP>& Pm, float* diag, float scale) {
   constexpr int CH = Elem<BF>::CH, NB = CH / 16, NT = P / 16, UD = CH + 4, TILES = NB * (NB + 1) / 2;
   const int l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   for (int id = w; id < (WITH_P ? 2 : 1) * TILES; id += NT) {
@@ -504,11 +466,11 @@ __device__ __forceinline__ void score_tiles(int tid, const Rows<Elem<BF>::CH>& r
     }
     if constexpr (WITH_P) {
       if (isP) {
-        put_mat<PARTS, UD>(tid, Pm, 16 * bj, 16 * bi, acc);
+        put_mat<UD>(tid, Pm, 16 * bj, 16 * bi, acc);
         continue;
       }
     }
-    put_mat<false, UD>(tid, M, 16 * bj, 16 * bi, acc);
+    put_mat<UD>(tid, M, 16 * bj, 16 * bi, acc);
     if (bi == bj) {
 #pragma unroll
       for (int k = 0; k < 4; k++) diag[(16 * bi + i0 + k) * 16 + j] = acc[k];
@@ -517,7 +479,7 @@ __device__ __forceinline__ void score_tiles(int tid, const Rows<Elem<BF>::CH>& r
 }
 
 // The diagonal blocks of (I + M)^-1, one column per lane of a wavefront's first CH.
-template <int CH, int N> __device__ __forceinline__ void invert_blocks(int tid, const float* diag, Mat<false, N>& Tinv) {
+template <int CH, int N> __device__ __forceinline__ void invert_blocks(int tid, const float* diag, Mat<N>& Tinv) {
   const int l = tid & 63;
   if (l >= CH) return;
   const int o = l & ~15, c = l & 15;
@@ -535,36 +497,36 @@ template <int CH, int N> __device__ __forceinline__ void invert_blocks(int tid, 
     x[i] = s;
   }
 #pragma unroll
-  for (int i = 0; i < 16; i += 4) *reinterpret_cast<f4*>(Tinv.hi + l * 20 + i) = f4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+  for (int i = 0; i < 16; i += 4) *reinterpret_cast<f4*>(Tinv.v + l * 20 + i) = f4{x[i], x[i + 1], x[i + 2], x[i + 3]};
 }
 
 // U = T Y by blocks, T's blocks below the diagonal through M.
-template <bool BF, int NM, int NI> __device__ __forceinline__ void solve(int tid, const Mat<false, NI>& Tinv, const Mat<false, NM>& M, const f4* Y, f4* U) {
+template <bool BF, int NM, int NI> __device__ __forceinline__ void solve(int tid, const Mat<NI>& Tinv, const Mat<NM>& M, const f4* Y, f4* U) {
   constexpr int CH = Elem<BF>::CH, NB = CH / 16, UD = CH + 4;
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
-  f4 t = mat_col<false, 20>(tid, Tinv, 0, 0).hi;
+  f4 t = mat_col<20>(tid, Tinv, 0, 0);
   U[0] = dot<1>(&t, Y, zero);
   if constexpr (NB == 2) {
     f4 y = -U[0];
-    t = mat_col<false, UD>(tid, M, 0, 16).hi;
+    t = mat_col<UD>(tid, M, 0, 16);
     y = dot<1>(&t, &y, Y[1]);
-    t = mat_col<false, 20>(tid, Tinv, 16, 0).hi;
+    t = mat_col<20>(tid, Tinv, 16, 0);
     U[1] = dot<1>(&t, &y, zero);
   }
 }
 // dY = T^T dU
-template <bool BF, int NM, int NI> __device__ __forceinline__ void solve_t(int tid, const Mat<false, NI>& Tinv, const Mat<false, NM>& M, const f4* dU, f4* dY) {
+template <bool BF, int NM, int NI> __device__ __forceinline__ void solve_t(int tid, const Mat<NI>& Tinv, const Mat<NM>& M, const f4* dU, f4* dY) {
   constexpr int CH = Elem<BF>::CH, NB = CH / 16, UD = CH + 4;
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
   f4 top = dU[0], t;
   if constexpr (NB == 2) {
-    t = mat_row<false, 20>(tid, Tinv, 16, 0).hi;
+    t = mat_row<20>(tid, Tinv, 16, 0);
     dY[1] = dot<1>(&t, dU + 1, zero);
     const f4 y = -dY[1];
-    t = mat_row<false, UD>(tid, M, 0, 16).hi;
+    t = mat_row<UD>(tid, M, 0, 16);
     top += dot<1>(&t, &y, zero);
   }
-  t = mat_row<false, 20>(tid, Tinv, 0, 0).hi;
+  t = mat_row<20>(tid, Tinv, 0, 0);
   dY[0] = dot<1>(&t, &top, zero);
 }
 
@@ -796,13 +758,13 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
 #pragma unroll
           for (int m = 0; m < NT; m++) S[m] = zero;
         }
-        score_tiles<BF, P, LD, !LOCAL, false>(tid, R, Qs, Ks, X.M, X.P, diag, scale);
+        score_tiles<BF, P, LD, !LOCAL>(tid, R, Qs, Ks, X.M, X.P, diag, scale);
         __syncthreads();
         if (w == 0) invert_blocks<CH>(tid, diag, X.Tinv);
         if (w == NT - 1 && once) fill_rows<CH>(tid, Rs[cur ^ 1], gn, A, 0, rows);
         f4 Y[NB], O[NB];
         {
-          Trip<BF> Sp[NT];
+          Parts<BF> Sp[NT];
 #pragma unroll
           for (int m = 0; m < NT; m++) Sp[m].set(S[m]);
 #pragma unroll
@@ -810,13 +772,13 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
             unit x[NT];
 #pragma unroll
             for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, Ks, 16 * n, 16 * m);
-            const f4 ks = dot2w<BF, NT>(x, Sp, zero);
+            const f4 ks = dot_parts<BF, NT>(x, Sp, zero);
             Y[n] = rows4(tid, R.be, 16 * n) * (widen(col_unit<LD>(tid, Vs, 16 * n, 16 * w)) -
                                           (rows4(tid, R.d0, 16 * n) * rows4(tid, R.rk, 16 * n)) * (ks));
             if constexpr (!LOCAL) {
 #pragma unroll
               for (int m = 0; m < NT; m++) x[m] = row_unit<LD>(tid, Qs, 16 * n, 16 * m);
-              O[n] = (scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n)) * (dot2w<BF, NT>(x, Sp, zero));
+              O[n] = (scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n)) * (dot_parts<BF, NT>(x, Sp, zero));
             }
           }
         }
@@ -843,7 +805,7 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
           for (int n = 0; n < NB; n++)
 #pragma unroll
             for (int m = 0; m <= n; m++) {
-              const f4 x = mat_col<false, UD>(tid, X.P, 16 * m, 16 * n).hi;
+              const f4 x = mat_col<UD>(tid, X.P, 16 * m, 16 * n);
               O[n] = dot<1>(&x, U + m, O[n]);
             }
           // y rests where V was, until the rows are stored behind the next barrier
@@ -852,7 +814,7 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
 #pragma unroll
             for (int i = 0; i < 4; i++) stf(Vs + (16 * n + 4 * (l >> 4) + i) * LD + 16 * w + (l & 15), O[n][i]);
         }
-        Trip<BF> Uw[NB];
+        Parts<BF> Uw[NB];
 #pragma unroll
         for (int n = 0; n < NB; n++) Uw[n].set((rows4(tid, R.dc, 16 * n) * rows4(tid, R.rk, 16 * n)) * (U[n]));
         const float c0 = R.c0;
@@ -861,7 +823,7 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
           unit kt[NB];
 #pragma unroll
           for (int n = 0; n < NB; n++) kt[n] = col_unit<LD>(tid, Ks, 16 * n, 16 * m);
-          S[m] = dot2w<BF, NB>(kt, Uw, c0 * S[m]);
+          S[m] = dot_parts<BF, NB>(kt, Uw, c0 * S[m]);
         }
         cut |= starts;
         y_at = t0;
@@ -959,23 +921,72 @@ template <int P, bool BACK> __global__ void __launch_bounds__(4 * P) k_delta_joi
   }
 }
 
+// U and dY of a chunk, transposed: [V][step]. For bf16 in their three parts, cut once by who writes them (16 cuts instead of some 200);
+// of 128 columns in fp32, cut by each reader, since the third parts would not fit a block's LDS.
+template <bool BF, int P> struct Cols {
+  using T = typename Elem<BF>::type;
+  static constexpr int UD = Elem<BF>::CH + 4;
+  static constexpr bool PARTS = BF && P <= 64;
+  std::conditional_t<PARTS, T, float> hi[P * UD];
+  T mid[PARTS ? P * UD : 1], low[PARTS ? P * UD : 1];
+  // A tile's values at rows 16 w + l % 16, columns `at` + 4 (l / 16) + 0..3; and units.
+  __device__ __forceinline__ void put(int tid, int w, int at, f4 v) {
+    const int l = tid & 63, o = (16 * w + (l & 15)) * UD + at + 4 * (l >> 4);
+    if constexpr (PARTS) {
+      Parts<BF> p;
+      p.set(v);
+      *reinterpret_cast<s4*>(hi + o) = p.hi;
+      *reinterpret_cast<s4*>(mid + o) = p.mid;
+      *reinterpret_cast<s4*>(low + o) = p.low;
+    } else {
+      *reinterpret_cast<f4*>(hi + o) = v;
+    }
+  }
+  __device__ __forceinline__ Parts<BF> col(int tid, int row, int col) const {
+    Parts<BF> p;
+    if constexpr (PARTS) {
+      p.hi = col_unit<UD>(tid, hi, row, col);
+      p.mid = col_unit<UD>(tid, mid, row, col);
+      p.low = col_unit<UD>(tid, low, row, col);
+    } else {
+      p.set(col_unit<UD>(tid, hi, row, col));
+    }
+    return p;
+  }
+  __device__ __forceinline__ Parts<BF> row(int tid, int row, int col) const {
+    Parts<BF> p;
+    if constexpr (PARTS) {
+      p.hi = row_unit<UD>(tid, hi, row, col);
+      p.mid = row_unit<UD>(tid, mid, row, col);
+      p.low = row_unit<UD>(tid, low, row, col);
+    } else {
+      p.set(row_unit<UD>(tid, hi, row, col));
+    }
+    return p;
+  }
+  __device__ __forceinline__ f4 values(int tid, int r, int c) const {
+    if constexpr (PARTS) return row(tid, r, c).sum();
+    else return row_unit<UD>(tid, hi, r, c);
+  }
+};
+
 // The gradient of one segment of one sequence's head, chunks in reverse. Wavefront w holds dS's columns 16 w .. and, for the
 // products that contract over V, the transposed dS's (rows 16 w .. of dS). LOCAL: what the segment adds to dS alone.
 template <bool BF, int P> struct BwdLds {
   using T = typename Elem<BF>::type;
   static constexpr int CH = Elem<BF>::CH, LD = P + Elem<BF>::pad, UD = CH + 4, CP = CH + 4, NT = P / 16;
   T Q[CH * LD], K[CH * LD], dO[CH * LD];
-  // values of fp32 transposed, [V][step]: U and dY, for bf16 both halves. V rests where U comes: it is read before.
+  // V rests where U comes: it is read before.
   union {
     T V[CH * LD];
-    T U[P * UD];
+    Cols<BF, P> U;
     float sums[4][NT][CH];  // when U has been read: <q^, dQ^>, <k^, dK^>, the parts of S_0 and of dS_c
   };
-  T dY[P * UD], Ulo[BF ? P * UD : 1], dYlo[BF ? P * UD : 1];
-  Mat<false, CH * UD> M;  // then F
-  Mat<BF, CH * UD> Pm;    // then E
+  Cols<BF, P> dY;
+  Mat<CH * UD> M;   // then F
+  Mat<CH * UD> Pm;  // then E
   union {
-    Mat<false, CH * 20> Tinv;
+    Mat<CH * 20> Tinv;
     float W[CH * CP];  // P_ij dO_i U_j - M_ij dY_i U_j
   };
   union {
@@ -990,33 +1001,12 @@ template <bool BF, int P> struct BwdLocalLds {
   using T = typename Elem<BF>::type;
   static constexpr int CH = Elem<BF>::CH, LD = P + Elem<BF>::pad, CP = CH + 4, UD = CH + 4;
   T Q[CH * LD], K[CH * LD], dO[CH * LD];
-  Mat<false, CH * UD> M;
-  Mat<BF, CH * UD> Pm;
-  Mat<false, CH * 20> Tinv;
+  Mat<CH * UD> M, Pm;
+  Mat<CH * 20> Tinv;
   float diag[CH * 16];
   Rows<CH> R[2];
 };
 
-// A tile's values into a transposed buffer pair at rows 16 w + l % 16, columns `at` + 4 (l / 16) + 0..3; and units of it.
-template <bool BF, int UD, typename T> __device__ __forceinline__ void put_t(int tid, T* hi, T* lo, int w, int at, f4 v) {
-  const int l = tid & 63, o = (16 * w + (l & 15)) * UD + at + 4 * (l >> 4);
-  Pair<BF> p;
-  p.set(v);
-  *reinterpret_cast<typename Elem<BF>::unit*>(hi + o) = p.hi;
-  if constexpr (BF) *reinterpret_cast<s4*>(lo + o) = p.lo;
-}
-template <bool BF, int UD, typename T> __device__ __forceinline__ Pair<BF> col_pair(int tid, const T* hi, const T* lo, int row, int col) {
-  Pair<BF> p;
-  p.hi = col_unit<UD>(tid, hi, row, col);
-  if constexpr (BF) p.lo = col_unit<UD>(tid, lo, row, col);
-  return p;
-}
-template <bool BF, int UD, typename T> __device__ __forceinline__ Pair<BF> row_pair(int tid, const T* hi, const T* lo, int row, int col) {
-  Pair<BF> p;
-  p.hi = row_unit<UD>(tid, hi, row, col);
-  if constexpr (BF) p.lo = row_unit<UD>(tid, lo, row, col);
-  return p;
-}
 __device__ __forceinline__ float row16_sum(float v) {
   v += dpp_mov<0xB1>(v);
   v += dpp_mov<0x4E>(v);
@@ -1152,18 +1142,18 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
         }
         __syncthreads();
         const bool fresh = R.starts >> lo & 1;  // S_0 may be anything
-        score_tiles<BF, P, LD, true, BF>(tid, R, L.Q, L.K, L.M, L.Pm, L.diag, scale);
+        score_tiles<BF, P, LD, true>(tid, R, L.Q, L.K, L.M, L.Pm, L.diag, scale);
         __syncthreads();
         if (w == 0) invert_blocks<CH>(tid, L.diag, L.Tinv);
         if (w == NT - 1 && once) fill_rows<CH>(tid, L.R[cur ^ 1], gn, A, 0, rows_at(c - 1));
-        // contractions over the state's rows, HT tiles at a time: all of a wide state's operands would not fit the registers
-        constexpr int HT = NT < 4 ? NT : 4;
+        // contractions over the state's rows, HT tiles at a time: the operands of all would not fit the registers
+        constexpr int HT = 2;
         f4 Y[NB], dU[NB], sd = zero;
 #pragma unroll
         for (int n = 0; n < NB; n++) Y[n] = dU[n] = zero;
 #pragma unroll
         for (int m0 = 0; m0 < NT; m0 += HT) {
-          Pair<BF> Sp[HT], Dp[HT];
+          Parts<BF> Sp[HT], Dp[HT];
 #pragma unroll
           for (int m = 0; m < HT; m++) {
             if constexpr (!LOCAL) {
@@ -1178,8 +1168,8 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             unit x[HT];
 #pragma unroll
             for (int m = 0; m < HT; m++) x[m] = row_unit<LD>(tid, L.K, 16 * n, 16 * (m0 + m));
-            if constexpr (!LOCAL) Y[n] = dot2<BF, HT>(x, Sp, Y[n]);
-            dU[n] = dot2<BF, HT>(x, Dp, dU[n]);
+            if constexpr (!LOCAL) Y[n] = dot_parts<BF, HT>(x, Sp, Y[n]);
+            dU[n] = dot_parts<BF, HT>(x, Dp, dU[n]);
           }
           if (NT > 4) __builtin_amdgcn_sched_barrier(0);
         }
@@ -1197,17 +1187,15 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
         unit dOc[NB];
         {
           if constexpr (!LOCAL) solve<BF>(tid, L.Tinv, L.M, Y, U);
-          Pair<BF> x[NB];
 #pragma unroll
-          for (int n = 0; n < NB; n++) dOc[n] = col_unit<LD>(tid, L.dO, 16 * n, 16 * w);
-          x[0] = mat_row<BF, UD>(tid, L.Pm, 0, 0);
-          if constexpr (NB == 2) {
-            x[1] = mat_row<BF, UD>(tid, L.Pm, 0, 16);
-            dU[0] = dot2r<BF, 2>(x, dOc, dU[0]);
-            x[0] = mat_row<BF, UD>(tid, L.Pm, 16, 16);
-            dU[1] = dot2r<BF, 1>(x, dOc + 1, dU[1]);
-          } else {
-            dU[0] = dot2r<BF, 1>(x, dOc, dU[0]);
+          for (int m = 0; m < NB; m++) {
+            dOc[m] = col_unit<LD>(tid, L.dO, 16 * m, 16 * w);
+            const f4 d = widen(dOc[m]);
+#pragma unroll
+            for (int n = 0; n <= m; n++) {
+              const f4 x = mat_row<UD>(tid, L.Pm, 16 * n, 16 * m);
+              dU[n] = dot<1>(&x, &d, dU[n]);
+            }
           }
           solve_t<BF>(tid, L.Tinv, L.M, dU, dY);
         }
@@ -1228,8 +1216,8 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
         if constexpr (!LOCAL) {
 #pragma unroll
           for (int n = 0; n < NB; n++) {
-            put_t<BF, UD>(tid, L.U, L.Ulo, w, 16 * n, U[n]);
-            put_t<BF, UD>(tid, L.dY, L.dYlo, w, 16 * n, dY[n]);
+            L.U.put(tid, w, 16 * n, U[n]);
+            L.dY.put(tid, w, 16 * n, dY[n]);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
               const float sum = row16_sum(dY[n][i] * U[n][i]);
@@ -1242,7 +1230,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
         float tot = c0 == 0.f ? 0.f : c0 * (sd[0] + sd[1] + sd[2] + sd[3]);
         // dS of the chunk's start; the transposed one below, when its old values have been used
         {
-          Pair<BF> x[NB], y[NB];
+          Parts<BF> x[NB], y[NB];
 #pragma unroll
           for (int n = 0; n < NB; n++) {
             x[n].set((scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n)) * (widen(dOc[n])));
@@ -1253,10 +1241,10 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             unit a[NB];
 #pragma unroll
             for (int n = 0; n < NB; n++) a[n] = col_unit<LD>(tid, L.Q, 16 * n, 16 * m);
-            dS[m] = dot2<BF, NB>(a, x, c0 * dS[m]);
+            dS[m] = dot_parts<BF, NB>(a, x, c0 * dS[m]);
 #pragma unroll
             for (int n = 0; n < NB; n++) a[n] = col_unit<LD>(tid, L.K, 16 * n, 16 * m);
-            dS[m] = dot2<BF, NB>(a, y, dS[m]);
+            dS[m] = dot_parts<BF, NB>(a, y, dS[m]);
             if (NT > 4) __builtin_amdgcn_sched_barrier(0);  // or the operands of all tiles are loaded at once, and do not fit
           }
         }
@@ -1270,22 +1258,22 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             f4 e = zero, f = zero;
 #pragma unroll
             for (int m0 = 0; m0 < NT; m0 += HT) {
-              Pair<BF> y[HT], x[HT];
+              Parts<BF> y[HT], x[HT];
               unit z[HT];
 #pragma unroll
               for (int m = 0; m < HT; m++) {
-                y[m] = col_pair<BF, UD>(tid, L.U, L.Ulo, 16 * (m0 + m), 16 * bj);
+                y[m] = L.U.col(tid, 16 * (m0 + m), 16 * bj);
                 z[m] = row_unit<LD>(tid, L.dO, 16 * bi, 16 * (m0 + m));
-                x[m] = col_pair<BF, UD>(tid, L.dY, L.dYlo, 16 * (m0 + m), 16 * bi);
+                x[m] = L.dY.col(tid, 16 * (m0 + m), 16 * bi);
               }
-              e = dot2<BF, HT>(z, y, e);
-              f = dot3<BF, HT>(x, y, f);
+              e = dot_parts<BF, HT>(z, y, e);
+              f = dot_parts<BF, HT>(x, y, f);
               if (NT > 4) __builtin_amdgcn_sched_barrier(0);
             }
             const int j = 16 * bj + (l & 15);
             const double Gj = R.G[j];
             const int segj = R.seg[j];
-            const f4 pv = mat_values<BF, UD>(tid, L.Pm, 16 * bj, 16 * bi), mv = mat_row<false, UD>(tid, L.M, 16 * bj, 16 * bi).hi;
+            const f4 pv = mat_row<UD>(tid, L.Pm, 16 * bj, 16 * bi), mv = mat_row<UD>(tid, L.M, 16 * bj, 16 * bi);
             const f4 be = rows4(tid, R.be, 16 * bi);
 #pragma unroll
             for (int i4 = 0; i4 < 4; i4++) {
@@ -1296,8 +1284,8 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
               e[i4] = on ? dec * scale * e[i4] : 0.f;
               f[i4] = on && j < i ? -dec * be[i4] * f[i4] : 0.f;
             }
-            put_mat<BF, UD>(tid, L.Pm, 16 * bj, 16 * bi, e);
-            put_mat<false, UD>(tid, L.M, 16 * bj, 16 * bi, f);
+            put_mat<UD>(tid, L.Pm, 16 * bj, 16 * bi, e);
+            put_mat<UD>(tid, L.M, 16 * bj, 16 * bi, f);
           }
           renew(tid, l);
           // products over V for this wavefront's columns of K: dO S_0^T, dY S_0^T, U dS^T
@@ -1306,7 +1294,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
           for (int n = 0; n < NB; n++) X1[n] = X2[n] = X3[n] = zero;
 #pragma unroll
           for (int m0 = 0; m0 < NT; m0 += HT) {
-            Pair<BF> St[HT], Dt[HT];
+            Parts<BF> St[HT], Dt[HT];
 #pragma unroll
             for (int m = 0; m < HT; m++) {
               St[m].set(fresh ? zero : S0[m0 + m]);
@@ -1317,14 +1305,14 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
               unit x[HT];
 #pragma unroll
               for (int m = 0; m < HT; m++) x[m] = row_unit<LD>(tid, L.dO, 16 * n, 16 * (m0 + m));
-              X1[n] = dot2<BF, HT>(x, St, X1[n]);
-              Pair<BF> y[HT];
+              X1[n] = dot_parts<BF, HT>(x, St, X1[n]);
+              Parts<BF> y[HT];
 #pragma unroll
-              for (int m = 0; m < HT; m++) y[m] = col_pair<BF, UD>(tid, L.dY, L.dYlo, 16 * (m0 + m), 16 * n);
-              X2[n] = dot3<BF, HT>(y, St, X2[n]);
+              for (int m = 0; m < HT; m++) y[m] = L.dY.col(tid, 16 * (m0 + m), 16 * n);
+              X2[n] = dot_parts<BF, HT>(y, St, X2[n]);
 #pragma unroll
-              for (int m = 0; m < HT; m++) y[m] = col_pair<BF, UD>(tid, L.U, L.Ulo, 16 * (m0 + m), 16 * n);
-              X3[n] = dot3<BF, HT>(y, Dt, X3[n]);
+              for (int m = 0; m < HT; m++) y[m] = L.U.col(tid, 16 * (m0 + m), 16 * n);
+              X3[n] = dot_parts<BF, HT>(y, Dt, X3[n]);
               if (NT > 4) __builtin_amdgcn_sched_barrier(0);
             }
           }
@@ -1343,7 +1331,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             Qc[n] = col_unit<LD>(tid, L.Q, 16 * n, 16 * w);
           }
           {
-            Pair<BF> x[NB], y[NB];
+            Parts<BF> x[NB], y[NB];
 #pragma unroll
             for (int n = 0; n < NB; n++) {
               x[n].set((scale * rows4(tid, R.d0, 16 * n) * rows4(tid, R.rq, 16 * n)) * (widen(Qc[n])));
@@ -1354,11 +1342,11 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
               unit a[NB];
 #pragma unroll
               for (int n = 0; n < NB; n++) a[n] = col_unit<LD>(tid, L.dO, 16 * n, 16 * m);
-              dSt[m] = dot2<BF, NB>(a, x, c0 * dSt[m]);
-              Pair<BF> b[NB];
+              dSt[m] = dot_parts<BF, NB>(a, x, c0 * dSt[m]);
+              Parts<BF> b[NB];
 #pragma unroll
-              for (int n = 0; n < NB; n++) b[n] = row_pair<BF, UD>(tid, L.dY, L.dYlo, 16 * m, 16 * n);
-              dSt[m] = dot3<BF, NB>(b, y, dSt[m]);
+              for (int n = 0; n < NB; n++) b[n] = L.dY.row(tid, 16 * m, 16 * n);
+              dSt[m] = dot_parts<BF, NB>(b, y, dSt[m]);
               if (NT > 4) __builtin_amdgcn_sched_barrier(0);
             }
           }
@@ -1369,37 +1357,28 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
           f4 dQ[NB], dK[NB];
           {
             f4 qn[NB], kn[NB];
-            Pair<BF> kp2[NB], qp2[NB];
 #pragma unroll
             for (int n = 0; n < NB; n++) {
               qn[n] = widen(Qc[n]) * rows4(tid, R.rq, 16 * n);
               kn[n] = widen(Kc[n]) * rows4(tid, R.rk, 16 * n);
-              qp2[n].set(qn[n]);
-              kp2[n].set(kn[n]);
             }
 #pragma unroll
             for (int n = 0; n < NB; n++) {
               const f4 from0 = qn[n] * X1[n] + kn[n] * X2[n], fromc = kn[n] * X3[n];
-              Pair<BF> e[NB], f[NB];
+              dQ[n] = X1[n];
+              dK[n] = X2[n] + X3[n];
 #pragma unroll
               for (int m = 0; m <= n; m++) {
-                e[m] = mat_col<BF, UD>(tid, L.Pm, 16 * m, 16 * n);
-                f[m].set(mat_col<false, UD>(tid, L.M, 16 * m, 16 * n).hi);
-              }
-              if (n == 0) {
-                dQ[n] = dot3<BF, 1>(e, kp2, X1[n]);
-                dK[n] = dot3<BF, 1>(f, kp2, X2[n] + X3[n]);
-              } else {
-                dQ[n] = dot3<BF, NB>(e, kp2, X1[n]);
-                dK[n] = dot3<BF, NB>(f, kp2, X2[n] + X3[n]);
+                const f4 e = mat_col<UD>(tid, L.Pm, 16 * m, 16 * n), f = mat_col<UD>(tid, L.M, 16 * m, 16 * n);
+                dQ[n] = dot<1>(&e, kn + m, dQ[n]);
+                dK[n] = dot<1>(&f, kn + m, dK[n]);
               }
 #pragma unroll
               for (int m = n; m < NB; m++) {
-                e[m] = mat_row<BF, UD>(tid, L.Pm, 16 * n, 16 * m);
-                f[m].set(mat_row<false, UD>(tid, L.M, 16 * n, 16 * m).hi);
+                const f4 e = mat_row<UD>(tid, L.Pm, 16 * n, 16 * m), f = mat_row<UD>(tid, L.M, 16 * n, 16 * m);
+                dK[n] = dot<1>(&e, qn + m, dK[n]);
+                dK[n] = dot<1>(&f, kn + m, dK[n]);
               }
-              if (n == NB - 1) dK[n] += dot3<BF, 1>(f + n, kp2 + n, dot3<BF, 1>(e + n, qp2 + n, zero));
-              else dK[n] += dot3<BF, NB>(f, kp2, dot3<BF, NB>(e, qp2, zero));
               const f4 sq = qn[n] * dQ[n], sk = kn[n] * dK[n];
 #pragma unroll
               for (int i = 0; i < 4; i++) {
@@ -1446,10 +1425,7 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
               sk += rows4(tid, L.sums[1][m], 16 * n);
             }
             const f4 dq = rq * (dQ[n] - widen(Qc[n]) * rq * sq), dk = rk * (dK[n] - widen(Kc[n]) * rk * sk);
-            const Pair<BF> dy = row_pair<BF, UD>(tid, L.dY, L.dYlo, 16 * w, 16 * n);
-            f4 dv;
-            if constexpr (BF) dv = be * (widen(dy.hi) + widen(dy.lo));
-            else dv = be * dy.hi;
+            const f4 dv = be * L.dY.values(tid, 16 * w, 16 * n);
             if (a.qpart) {
               const unsigned step = (unsigned)(sa.H * sa.K);  // elements of a sequence's step
               const long to = (((t0 + 16 * n + 4 * (l >> 4)) * sa.B + bt) * sa.H + h) * sa.K + col;

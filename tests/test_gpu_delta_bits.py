@@ -54,3 +54,27 @@ def test_outputs(gpu, T, B, Hk, H, K, V):
     yr, hr = R.delta({n: host(t) for n, t in p.items()}, None, host(done), host(first), host(h0))
     assert rel(h, hr) <= STATE, rel(h, hr)
     rounded(y, yr, FLIPS, "y")
+
+
+@pytest.mark.parametrize("T,B,Hk,H,K,V", CASES)
+def test_gradients(gpu, T, B, Hk, H, K, V):
+    p, done, first, h0 = case(T, B, Hk, H, K, V)
+    dy, dh = cu(50, T, B, H, V, dtype=BF), cu(51, B, H, K, V)
+    ref = {n: leaf(t) for n, t in p.items()}
+    wide = {n: host(p[n]).expand(T, B, H).clone().requires_grad_(True) for n in ("A", "dt_bias")}  # a step's own
+    h0r = leaf(h0)
+    yr, hr = R.delta({**ref, **wide}, None, host(done), host(first), h0r)
+    names = list("qkv")
+    got = torch.autograd.grad((yr * host(dy)).sum() + (hr * host(dh)).sum(), [ref[n] for n in names] + [wide["A"], wide["dt_bias"], h0r])
+    grads = dict(zip(names + ["A", "dt_bias", "h0"], got))
+    _, _, saved = forward(p, done, first, h0)
+    dh0 = torch.empty_like(h0)
+    g = D.delta_scan_grad(*[p[n] for n in "qkvabA"], saved, dy, dt_bias=p["dt_bias"], done=done, first=first, dh=dh, dh0=dh0)
+    found = {"h0": rel(dh0, grads["h0"])}
+    for n in ("A", "dt_bias"):
+        found[n] = float((host(g["d" + n]) - grads[n].sum((0, 1))).norm() / grads[n].norm())
+    for n in names:
+        found[n] = rel(g["d" + n], grads[n].to(BF).double())
+    bars = dict(h0=STATE, A=TERMS, dt_bias=TERMS, v=FLIPS, q=FLIPS, k=FLIPS * 2 ** 0.5)  # dk: the sum of two such parts
+    over = {n: x for n, x in found.items() if x > bars[n]}
+    assert not over, (over, found)
