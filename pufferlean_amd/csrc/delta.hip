@@ -28,8 +28,9 @@
 //   dS_0 = D_c0 dS_c + Q^T (scale D_i0 dO) - K^T (D_i0 be dY)
 //
 // Steps hidden by an episode's start are selected away: D is 0 there and what it multiplies is dropped, so an infinite
-// state does not pass. Inside the products 0 times a non-finite U would; a chunk that holds an episode's start and finds a
-// non-finite value is done again episode by episode, with the other rows zero.
+// state does not pass. Inside the products 0 times a non-finite value would; a chunk that finds one is done again in parts, with the
+// other rows zero: episode by episode, and forward, where a step may not see the ones behind it, up to each step at which a column turns
+// non-finite. (Backward every step sees the ones behind it.)
 //
 // Layout. A block owns one head of one sequence, wavefront w the state's columns 16 w .. 16 w + 15 (gradient: rows of the
 // transposed state too), in the accumulator layout of the 16x16 matrix instructions: lane l holds rows 4 (l / 16) + r, column
@@ -341,8 +342,9 @@ template <int CH> struct Rows {
   float be[CH], rq[CH], rk[CH];       // write strength, 1 / norms
   float d0[CH], dc[CH];               // D_i0, D_cj
   float sp[CH], arg[CH];              // softplus and its argument (gradient)
-  float c0, pad;                      // D_c0
+  float c0;                           // D_c0
   int starts;                         // bit i: row i starts an episode
+  int odd, split;                     // what mark_odd has found
 };
 
 // The lane's row of the gates, loaded ahead: as it is in memory, for what is computed from it would be waited for.
@@ -401,13 +403,39 @@ template <int CH, typename T> __device__ __forceinline__ void fill_rows(int tid,
     r.sp[i] = sp;
     r.arg[i] = arg;
     const float d0 = ex2((float)G), dc = ex2((float)(last - G));
-    r.d0[i] = in && seg == 0 ? d0 : 0.f;
+    r.d0[i] = in && (seg == 0 || d0 != d0) ? d0 : 0.f;  // a gate that is none shows in Y also behind an episode's start
     r.dc[i] = in && seg == all ? dc : 0.f;
     if (i == CH - 1) {
       r.c0 = all == 0 ? d0 : 0.f;
       r.starts = (int)(starts & 0xffffffffu);
+      r.odd = last > 40.0;  // a decay that grows (A above 0) may pass fp32's range in M, which Y does not show
+      r.split = CH;
     }
   }
+}
+// Rows lo..hi-1 of a wavefront's columns of Y that are not finite (nor far enough from the largest number for sums of them to be): that there
+// are any, and the first one that has a row in front of it in its column. Those in front may not meet it in a product; behind it all of
+// the column's are none either.
+template <int CH, int NB> __device__ __forceinline__ void mark_odd(int tid, Rows<CH>& r, const f4* Y, int lo, int hi) {
+  bool odd = false;
+#pragma unroll
+  for (int n = 0; n < NB; n++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) odd |= !(fabsf(Y[n][i]) < 1e30f);
+  if (!__any(odd)) return;
+  const int l = tid & 63;
+  unsigned rows = 0;
+#pragma unroll
+  for (int n = 0; n < NB; n++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) rows |= !(fabsf(Y[n][i]) < 1e30f) ? 1u << (16 * n + 4 * (l >> 4) + i) : 0u;
+  rows |= (unsigned)__shfl_xor((int)rows, 16);
+  rows |= (unsigned)__shfl_xor((int)rows, 32);
+  rows &= (2u << (hi - 1)) - (1u << lo);
+  if (!rows) return;
+  r.odd = 1;
+  const int at = __ffs((int)rows) - 1;
+  if (at > lo) atomicMin(&r.split, at);
 }
 __device__ __forceinline__ f4 rows4(int tid, const float* r, int at) { return *reinterpret_cast<const f4*>(r + at + 4 * ((tid & 63) >> 4)); }
 
@@ -621,8 +649,9 @@ __device__ __forceinline__ void put_row(int tid, T* tile, u4 r, int lo, int hi, 
   if (part && (row < lo || row >= hi)) r = u4{0, 0, 0, 0};
   *reinterpret_cast<u4*>(tile + row * LD + c) = r;
 }
-// 1 / sqrt(|row|^2 + eps) of the staged rows, 0 for those left out
-template <bool BF, int P> __device__ __forceinline__ void put_norm(int tid, float* out, u4 r, int lo, int hi) {
+// 1 / sqrt(|row|^2 + eps) of the staged rows, 0 for those left out; LONG_NAN: none for rows longer than fp32 can say, whose products are
+// no numbers either
+template <bool BF, int P, bool LONG_NAN = false> __device__ __forceinline__ void put_norm(int tid, float* out, u4 r, int lo, int hi) {
   constexpr int L = P / Elem<BF>::V;  // lanes of a row
   float s = square_sum<BF>(r);
   s += dpp_mov<0xB1>(s);
@@ -631,7 +660,7 @@ template <bool BF, int P> __device__ __forceinline__ void put_norm(int tid, floa
   if constexpr (L >= 16) s += dpp_mov<0x140>(s);
   if constexpr (L >= 32) s += __shfl_xor(s, 16);
   const int row = tid / L;
-  if (tid % L == 0) out[row] = row >= lo && row < hi ? __builtin_amdgcn_rsqf(s + kEps) : 0.f;
+  if (tid % L == 0) out[row] = row >= lo && row < hi ? (LONG_NAN && s == INFINITY ? NAN : __builtin_amdgcn_rsqf(s + kEps)) : 0.f;
 }
 
 // ---- sequences ------------------------------------------------------------------------------------------
@@ -745,7 +774,7 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
         put_row<BF, P>(tid, Ks, k, lo, hi, !once);
         put_row<BF, P>(tid, Vs, v, lo, hi, !once);
         if (!LOCAL) put_norm<BF, P>(tid, R.rq, q, lo, hi);
-        put_norm<BF, P>(tid, R.rk, k, lo, hi);
+        put_norm<BF, P, true>(tid, R.rk, k, lo, hi);
         if (!once && w == NT - 1) fill_rows<CH>(tid, R, g, A, lo, hi);
         __syncthreads();
         have = once;
@@ -782,24 +811,21 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
             }
           }
         }
+        mark_odd<CH, NB>(tid, R, Y, lo, hi);
         __syncthreads();
-        f4 U[NB];
-        solve<BF>(tid, X.Tinv, X.M, Y, U);
         const int starts = R.starts, inside = starts & ~(1 << lo);
-        if (inside) {
-          bool bad = false;
-#pragma unroll
-          for (int n = 0; n < NB; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) bad |= !finite(U[n][i]);
-          if (__syncthreads_or(bad)) {
+        if (__builtin_amdgcn_readfirstlane(R.odd)) {  // only the rows up to the next episode, or to a row that the ones in front may not see
+          const int next = inside ? __ffs(inside) - 1 : CH, stop = LOCAL || next < R.split ? next : R.split;
+          if (stop < hi) {
             if (once) walk(-1);
             have = false;
             rows = all;
-            hi = __ffs(inside) - 1;
+            hi = __builtin_amdgcn_readfirstlane(stop);
             continue;
           }
         }
+        f4 U[NB];
+        solve<BF>(tid, X.Tinv, X.M, Y, U);
         if constexpr (!LOCAL) {
 #pragma unroll
           for (int n = 0; n < NB; n++)
