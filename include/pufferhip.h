@@ -527,9 +527,10 @@ int ph_rms_norm_grad(const ph_rms_args* a, const float* rstd, const void* dout, 
  *   min_p (fp32)        and of these the ones that have at least min_p times the largest one's mass; the largest always
  * Of equal logits the one with the lower index counts as larger. What is left is summed up in the order of the indices, and
  * the first entry with which the sum exceeds u times the total is taken. act (int32 [N]); logp (fp32 [N], may be NULL): the
- * logarithm of its share of what is left. Logits of -inf and NaN are never taken; a row of nothing else gives act -1 and
- * logp -inf; entries of +inf share the draw. A parameter that is NaN, or a temperature below zero, leaves its filter off (temperature 1).
- * Masses are held in 64 bits. */
+ * logarithm of its share of what is left, formed from the logit. Logits of -inf and NaN are never taken; a row of nothing else gives act -1
+ * and logp -inf; entries of +inf share the draw. A parameter that is NaN, or a temperature below zero, leaves its filter off (temperature
+ * 1). Masses are whole numbers of 2^-bits of the largest one's, bits = 62 less the bits of A - 1 and at most 51 (45 at A = 131072, 42 at
+ * 2^20): an entry of less than half a unit is never taken, not even with u = 0. */
 int ph_sample_filtered(int dtype, const void* logits, long ld, size_t N, size_t A, const float* u, const float* temperature,
                        const int* top_k, const float* top_p, const float* min_p, int* act, float* logp, void* stream);
 

@@ -110,6 +110,11 @@ __device__ __forceinline__ u64 units(Mass m, int bits) {
   const u64 f = (b & 0xfffffffffffffull) | 0x10000000000000ull;
   return shift > 53 ? 0 : (f + (1ull << (shift - 1))) >> shift;
 }
+// The logarithm of an entry's share of the total: from its logit, not from its units, of which it may have few.
+__device__ __forceinline__ float log_share(uint32_t key, uint32_t top, double c, u64 total, int bits) {
+  const double d = key == top ? 0.0 : ((double)logit_of(key) - (double)logit_of(top)) * c * 0.6931471805599453094;
+  return (float)(d - log(ldexp((double)total, -bits)));
+}
 // What an entry has to have by min_p, in these units.
 __device__ __forceinline__ u64 least(float minp, int bits) { return (u64)ceil(ldexp((double)minp, bits)); }
 
@@ -166,8 +171,9 @@ template <typename T, int E> __global__ void __launch_bounds__(256, 4) k_draw_wa
   int l = threadIdx.x & 63;
   // what goes by the lane's number is formed again from here on, and does not wait in registers
   auto renew = [&] { asm volatile("" : "+v"(l)); };
-  WaveLds& L = lds[threadIdx.x >> 6];
-  for (long n = (long)blockIdx.x * 4 + (threadIdx.x >> 6); n < a.N; n += (long)gridDim.x * 4) {
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  WaveLds& L = lds[w];
+  for (long n = (long)blockIdx.x * 4 + w; n < a.N; n += (long)gridDim.x * 4) {
     const T* row = (const T*)a.x + n * a.ld;
     uint32_t key[E], top = 0;
     {
@@ -183,7 +189,7 @@ template <typename T, int E> __global__ void __launch_bounds__(256, 4) k_draw_wa
     }
     renew();
     const Par par = par_of(a, n);
-    top = wave_max(top);
+    top = (uint32_t)__builtin_amdgcn_readfirstlane((int)wave_max(top));
     int act = -1;
     float logp = -INFINITY;
     // the entries at `key` in the order of their indices: the index of the count-th (from 1). Few rows ask, so it reads them again.
@@ -364,12 +370,14 @@ template <typename T, int E> __global__ void __launch_bounds__(256, 4) k_draw_wa
       u64 mine = 0;
 #pragma unroll
       for (int e = 0; e < E; e++) mine = e == tile ? m[e] : mine;
+      tile = __builtin_amdgcn_readfirstlane(tile);
+      const float logit = ldf(row + (64 * tile + l < a.A ? 64 * tile + l : 0));  // again: the keys did not wait in registers
       const u64 at = run + wave_scan(mine);
       u64 hit = __ballot(mine > 0 && at > target);
       if (!hit) hit = 1ull << (63 - __clzll((long long)__ballot(mine > 0)));  // u rounded up to 1: the last
       const int lane = __ffsll((unsigned long long)hit) - 1;
       act = 64 * tile + lane;
-      logp = (float)log((double)__shfl(mine, lane) / (double)total);
+      logp = log_share(key_of(__shfl(logit, lane)), top, par.c, total, a.bits);
     }
     if (l == 0) {
       a.act[n] = act;
@@ -499,7 +507,7 @@ __device__ __forceinline__ void cut_at(WideLds& L, bool is_it, u64 mine, uint32_
 }
 
 // All that top-k leaves is in the list, one entry a thread: the rest of the filters and the draw.
-__device__ __forceinline__ void draw_listed(WideLds& L, const DrawArgs& a, long n, const Par& par, uint32_t thr, int cut) {
+__device__ __forceinline__ void draw_listed(WideLds& L, const DrawArgs& a, long n, const Par& par, uint32_t top, uint32_t thr, int cut) {
   const int tid = threadIdx.x, count = L.count;
   const u64 mine = tid < count ? L.order[tid] : 0;
   const uint32_t k = (uint32_t)(mine >> 32);
@@ -524,13 +532,14 @@ __device__ __forceinline__ void draw_listed(WideLds& L, const DrawArgs& a, long 
   __syncthreads();
   if (m && i == L.found) {
     a.act[n] = i;
-    if (a.logp) a.logp[n] = (float)log((double)m / (double)total);
+    if (a.logp) a.logp[n] = log_share(k, top, par.c, total, a.bits);
   }
 }
 
 // The wavefront's part of the row is where the sum, `before` in front of it, exceeds the target.
 template <typename T, typename F>
-__device__ __forceinline__ void draw_in_part(const DrawArgs& a, long n, const Row<T>& row, F left_at, u64 before, u64 target, u64 total) {
+__device__ __forceinline__ void draw_in_part(const DrawArgs& a, long n, const Row<T>& row, F left_at, u64 before, u64 target, u64 total,
+                                             uint32_t top, double c) {
   constexpr int V = Row<T>::V;
   const int l = threadIdx.x & 63;
   for (int at = row.from; at < row.to; at += 64 * V) {
@@ -543,19 +552,19 @@ __device__ __forceinline__ void draw_in_part(const DrawArgs& a, long n, const Ro
     if (all && (before + all > target || before + all == total)) {
       u64 run = before + incl - here;
       int first = -1;  // of the lane's entries: the first that exceeds, or (u rounded up to 1) the last there is
-      u64 got = 0;
+      uint32_t got = 0;
 #pragma unroll
       for (int j = 0; j < V; j++) {
         run += m[j];
         if (m[j] && (run > target || run == total) && first < 0) {
           first = j;
-          got = m[j];
+          got = k[j];
         }
       }
       const u64 who = __ballot(first >= 0);
       if (l == __ffsll((unsigned long long)who) - 1) {
         a.act[n] = at + V * l + first;
-        if (a.logp) a.logp[n] = (float)log((double)got / (double)total);
+        if (a.logp) a.logp[n] = log_share(got, top, c, total, a.bits);
       }
       break;
     }
@@ -693,7 +702,7 @@ template <typename T> __device__ __forceinline__ void draw_row(WideLds& L, const
     }
   }
   if (listed) {
-    draw_listed(L, a, n, par, thr, cut);
+    draw_listed(L, a, n, par, top, thr, cut);
     return;
   }
   if (par.p < 1.0) {
@@ -756,7 +765,7 @@ template <typename T> __device__ __forceinline__ void draw_row(WideLds& L, const
   for (int i = 0; i < w; i++) before += L.wave[i];
   const u64 target = (u64)((double)par.u * (double)total);
   if (mine && before <= target && (before + mine > target || before + mine == total))
-    draw_in_part<T>(a, n, row, left_at, before, target, total);
+    draw_in_part<T>(a, n, row, left_at, before, target, total, top, par.c);
 }
 
 template <typename T> __global__ void __launch_bounds__(kWide) k_draw_wide(const DrawArgs a) {
@@ -977,7 +986,7 @@ template <typename T> __global__ void __launch_bounds__(kWide) k_split_draw(cons
       before = 0;
       compare(L, mine, rank, before);
       cut_at(L, tid < L.count && rank == s.par.k - 1, mine, thr, cut);
-      draw_listed(L, a, n, s.par, thr, cut);
+      draw_listed(L, a, n, s.par, s.top, thr, cut);
       return;
     }
     compare(L, mine, rank, before);
@@ -1004,7 +1013,7 @@ template <typename T> __global__ void __launch_bounds__(kWide) k_split_draw(cons
           const u64 m = units(mass_of(k, s.top, s.par.c, table), a.bits);
           return m >= need ? m : 0ull;
         };
-        draw_in_part<T>(a, n, Row<T>(a, n, i, kParts), left_at, front, target, total);
+        draw_in_part<T>(a, n, Row<T>(a, n, i, kParts), left_at, front, target, total, s.top, s.par.c);
       }
       return;
     }
