@@ -1827,7 +1827,7 @@ long chunk_steps(int dtype) { return dtype == PH_BF16 ? Elem<true>::CH : Elem<fa
 
 using namespace ph;
 
-bool is_input(const ph_delta_args& p, const void* t) { return t == p.q || t == p.k || t == p.v || t == p.a || t == p.b; }
+static bool is_input(const ph_delta_args& p, const void* t) { return t == p.q || t == p.k || t == p.v || t == p.a || t == p.b; }
 
 extern "C" size_t ph_delta_keep_floats(const ph_delta_args* p) {
   if (!p) return 0;
