@@ -475,13 +475,13 @@ typedef struct {
   const float *A, *dt_bias, *done, *first, *h0;
   float scale;
 } ph_delta_args;
-/* y [.., H, V], which may not be an input; h_out (may be NULL) receives the state after the last step, before done[T-1]
+/* y [.., H, V], which may neither be an input nor share elements with one; h_out (may be NULL) receives the state after the last step, before done[T-1]
  * clears it (the next call's `first` does); it may be h0. keep (may be NULL): fp32, ph_delta_keep_floats values, the states
  * that the gradient starts from. */
 int ph_delta_scan(const ph_delta_args* a, void* y, long y_t, long y_b, long y_h, float* h_out, float* keep, void* stream);
 size_t ph_delta_keep_floats(const ph_delta_args* a);
 /* Gradient from the forward's arguments (h0 is not read) and keep; dh (fp32, may be NULL: zero) is the gradient of h_out. Each
- * output may be NULL; dq, dk, dv, da, db have the activations' dtype and strides of their own and may not be inputs or one another; dA and
+ * output may be NULL; dq, dk, dv, da, db have the activations' dtype and strides of their own and may not be inputs or one another, nor share elements with them; dA and
  * ddt_bias (fp32 [H], overwritten) are summed in an order fixed by the shape; dh0 (may be dh) is the gradient of h0. */
 typedef struct {
   void *dq, *dk, *dv, *da, *db;
@@ -498,7 +498,7 @@ int ph_delta_step(const ph_delta_args* a, void* y, long y_b, long y_h, float* h,
  *   out = r / sqrt(avg r^2 + eps) w silu(gate)
  * add NULL: r = x; scale (fp32 [C], for G = 1) NULL: 1; w (fp32 [C / G]) NULL: 1; gate NULL: no gate. res (where there is an
  * add; may be NULL) receives r, rstd (fp32 [M][G], may be NULL) the 1 / sqrt for the gradient. Row strides in elements. out
- * and res may each be one of the inputs (same rows), but not the same one. */
+ * and res may each be one of the inputs (same rows), but not the same one, and not lie across the rows of another. */
 typedef struct {
   int dtype;
   size_t M, C, G;
@@ -510,7 +510,7 @@ typedef struct {
 int ph_rms_norm(const ph_rms_args* a, void* out, long ldout, void* res, long ldres, float* rstd, void* stream);
 /* Gradient from the forward's arguments and rstd, given dout (of out) and dres (of res; NULL: zero): dx, dadd = scale dx (where
  * there is an add), dgate, and dw = the rows' and groups' sums, dscale = the rows' sums (fp32, overwritten; zero for M = 0). Each output may be
- * NULL. dx, dadd and dgate may each be one of the inputs (same rows), but no two the same one. */
+ * NULL. dx, dadd and dgate may each be one of the inputs (same rows), but no two the same one, and not lie across the rows of another. */
 typedef struct {
   void *dx, *dadd, *dgate;
   long lddx, lddadd, lddgate;
@@ -530,7 +530,7 @@ int ph_rms_norm_grad(const ph_rms_args* a, const float* rstd, const void* dout, 
  * logarithm of its share of what is left, formed from the logit. Logits of -inf and NaN are never taken; a row of nothing else gives act -1
  * and logp -inf; entries of +inf share the draw. A parameter that is NaN, or a temperature below zero, leaves its filter off (temperature
  * 1). Masses are whole numbers of 2^-bits of the largest one's, bits = 62 less the bits of A - 1 and at most 51 (45 at A = 131072, 42 at
- * 2^20): an entry of less than half a unit is never taken, not even with u = 0. */
+ * 2^20): an entry of less than half a unit is never taken, not even with u = 0. act and logp may not share elements with the logits. */
 int ph_sample_filtered(int dtype, const void* logits, long ld, size_t N, size_t A, const float* u, const float* temperature,
                        const int* top_k, const float* top_p, const float* min_p, int* act, float* logp, void* stream);
 

@@ -53,6 +53,7 @@
 #include "kernels.hpp"
 #include "lanes.hpp"
 #include "routes.hpp"
+#include "spans.hpp"
 
 #include <type_traits>
 
@@ -1822,12 +1823,41 @@ long phi_floats(const Args& a) { return a.segs > 1 ? a.segs * a.units * up16(a.K
 
 long chunk_steps(int dtype) { return dtype == PH_BF16 ? Elem<true>::CH : Elem<false>::CH; }
 
+// The memory of a call's arrays: blocks read inputs while others write, so no output may share an element with an input.
+Span rows_of(const ph_delta_args& p, const void* at, long t, long b, long h, size_t heads, size_t width) {
+  const long e = p.dtype == PH_BF16 ? 2 : 4;
+  return {at, (long)width * e, {(long)p.T, (long)p.B, (long)heads}, {t * e, b * e, h * e}};
+}
+Span floats(const void* at, size_t n) { return flat(at, (long)n * 4); }
+Span state_of(const ph_delta_args& p, const void* at) { return floats(at, p.B * p.H * p.K * p.V); }
+struct Spans {
+  Span s[16];
+  int n = 0;
+  void add(const Span& x) { s[n++] = x; }
+  bool meet(const Span& x) const {
+    for (int i = 0; i < n; i++)
+      if (ph::meet(s[i], x)) return true;
+    return false;
+  }
+};
+Spans inputs_of(const ph_delta_args& p, bool seq) {
+  Spans in;
+  in.add(rows_of(p, p.q, p.q_t, p.q_b, p.q_h, p.Hk, p.K));
+  in.add(rows_of(p, p.k, p.k_t, p.k_b, p.k_h, p.Hk, p.K));
+  in.add(rows_of(p, p.v, p.v_t, p.v_b, p.v_h, p.H, p.V));
+  in.add(rows_of(p, p.a, p.a_t, p.a_b, 0, 1, p.H));
+  in.add(rows_of(p, p.b, p.b_t, p.b_b, 0, 1, p.H));
+  in.add(floats(p.A, p.H));
+  in.add(floats(p.dt_bias, p.H));
+  in.add(floats(p.first, p.B));
+  if (seq) in.add(floats(p.done, p.T * p.B));
+  return in;
+}
+
 }  // namespace
 }  // namespace ph
 
 using namespace ph;
-
-static bool is_input(const ph_delta_args& p, const void* t) { return t == p.q || t == p.k || t == p.v || t == p.a || t == p.b; }
 
 extern "C" size_t ph_delta_keep_floats(const ph_delta_args* p) {
   if (!p) return 0;
@@ -1842,7 +1872,13 @@ extern "C" int ph_delta_scan(const ph_delta_args* p, void* y, long y_t, long y_b
   if (p->B == 0) return PH_OK;
   PH_REQUIRE(p->T >= 1, "delta_scan: no steps");
   PH_REQUIRE(y, "delta_scan: y missing");
-  PH_REQUIRE(!is_input(*p, y), "delta_scan: y may not be an input");
+  const Span ys = rows_of(*p, y, y_t, y_b, y_h, p->H, p->V), out = state_of(*p, h_out), kept = floats(keep, ph_delta_keep_floats(p));
+  Spans in = inputs_of(*p, true);
+  PH_REQUIRE(!in.meet(ys) && !meet(state_of(*p, p->h0), ys), "delta_scan: y may not be an input or share elements with one");
+  PH_REQUIRE(!folds(ys), "delta_scan: y holds elements twice");
+  PH_REQUIRE(!in.meet(out) && !in.meet(kept) && (h_out == p->h0 || !meet(state_of(*p, p->h0), out)) && !meet(state_of(*p, p->h0), kept) &&
+                 !meet(ys, out) && !meet(ys, kept) && !meet(out, kept),
+             "delta_scan: h_out or the kept states share elements with an input or another output");
   Args a = args_of(*p);
   a.y = y; a.y_t = y_t; a.y_b = y_b; a.y_h = y_h; a.h_out = h_out; a.keep = keep;
   set_segments(a, false, p->dtype);
@@ -1870,12 +1906,18 @@ extern "C" int ph_delta_scan_grad(const ph_delta_args* p, const float* keep, con
   }
   PH_REQUIRE(p->T >= 1, "delta_scan_grad: no steps");
   PH_REQUIRE(dy && keep, "delta_scan_grad: dy or the kept states missing");
-  const void* outs[] = {g->dq, g->dk, g->dv, g->da, g->db};
-  for (int i = 0; i < 5; i++) {
-    if (!outs[i]) continue;
-    PH_REQUIRE(!is_input(*p, outs[i]) && outs[i] != dy, "delta_scan_grad: a gradient may not be an input");
-    for (int j = 0; j < i; j++) PH_REQUIRE(outs[i] != outs[j], "delta_scan_grad: two gradients are the same");
+  Spans in = inputs_of(*p, true);
+  in.add(rows_of(*p, dy, dy_t, dy_b, dy_h, p->H, p->V));
+  in.add(floats(keep, ph_delta_keep_floats(p)));
+  const Span outs[] = {rows_of(*p, g->dq, g->dq_t, g->dq_b, g->dq_h, p->Hk, p->K), rows_of(*p, g->dk, g->dk_t, g->dk_b, g->dk_h, p->Hk, p->K),
+                       rows_of(*p, g->dv, g->dv_t, g->dv_b, g->dv_h, p->H, p->V), rows_of(*p, g->da, g->da_t, g->da_b, 0, 1, p->H),
+                       rows_of(*p, g->db, g->db_t, g->db_b, 0, 1, p->H), state_of(*p, g->dh0)};
+  for (int i = 0; i < 6; i++) {
+    PH_REQUIRE(!in.meet(outs[i]) && ((i == 5 && g->dh0 == dh) || !meet(state_of(*p, dh), outs[i])),
+               "delta_scan_grad: a gradient may not be an input or share elements with one");
+    for (int j = 0; j < i; j++) PH_REQUIRE(!meet(outs[i], outs[j]), "delta_scan_grad: two gradients are the same or share elements");
   }
+  for (const Span& out : outs) PH_REQUIRE(!folds(out), "delta_scan_grad: a gradient holds elements twice");
   Args a = args_of(*p);
   GradArgs o{};
   o.dy = dy; o.dy_t = dy_t; o.dy_b = dy_b; o.dy_h = dy_h; o.keep = keep; o.dh = dh;
@@ -1910,7 +1952,11 @@ extern "C" int ph_delta_step(const ph_delta_args* p, void* y, long y_b, long y_h
   PH_TRY(check(*p, "delta_step"));
   if (p->T == 0 || p->B == 0) return PH_OK;
   PH_REQUIRE(y && h, "delta_step: y or the state missing");
-  PH_REQUIRE(!is_input(*p, y), "delta_step: y may not be an input");
+  const Span ys = rows_of(*p, y, 0, y_b, y_h, p->H, p->V), state = state_of(*p, h);
+  Spans in = inputs_of(*p, false);
+  PH_REQUIRE(!in.meet(ys), "delta_step: y may not be an input or share elements with one");
+  PH_REQUIRE(!folds(ys), "delta_step: y holds elements twice");
+  PH_REQUIRE(!in.meet(state) && !meet(ys, state), "delta_step: the state shares elements with y or an input");
   Args a = args_of(*p);
   a.y = y; a.y_b = y_b; a.y_h = y_h;
   return p->dtype == PH_BF16 ? step_t<uint16_t>(a, h, as_stream(stream)) : step_t<float>(a, h, as_stream(stream));

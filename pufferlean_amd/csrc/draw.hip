@@ -17,6 +17,7 @@
 #include "kernels.hpp"
 #include "lanes.hpp"
 #include "routes.hpp"
+#include "spans.hpp"
 
 namespace ph {
 namespace {
@@ -1058,6 +1059,14 @@ extern "C" int ph_sample_filtered(int dtype, const void* logits, long ld, size_t
   PH_REQUIRE(ld == 0 || ld >= (long)A, "sample_filtered: row stride %ld below %zu entries", ld, A);
   if (N == 0) return PH_OK;
   PH_REQUIRE(logits && u && act, "sample_filtered: logits, u or act missing");
+  const long e = dtype == PH_BF16 ? 2 : 4;
+  const Span x = {logits, (long)A * e, {(long)N, 1, 1}, {ld * e, 0, 0}}, outs[] = {flat(act, (long)N * 4), flat(logp, (long)N * 4)};
+  const void* rows[] = {u, temperature, top_k, top_p, min_p};
+  for (const Span& o : outs) {  // over a row's own number or parameter an output may lie: it is written when that has been read
+    PH_REQUIRE(!meet(o, x), "sample_filtered: an output shares elements with the logits");
+    for (const void* r : rows) PH_REQUIRE(o.p == r || !meet(o, flat(r, (long)N * 4)), "sample_filtered: an output lies across an input");
+  }
+  PH_REQUIRE(!meet(outs[0], outs[1]), "sample_filtered: act and logp share elements");
   DrawArgs a{};
   a.x = logits; a.ld = ld; a.N = (long)N; a.A = (int)A; a.u = u; a.temperature = temperature; a.top_k = top_k; a.top_p = top_p;
   a.min_p = min_p; a.act = act; a.logp = logp;

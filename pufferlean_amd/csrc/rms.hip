@@ -16,6 +16,7 @@
 #include "kernels.hpp"
 #include "lanes.hpp"
 #include "rows.hpp"
+#include "spans.hpp"
 
 namespace ph {
 namespace {
@@ -426,6 +427,23 @@ int check(const ph_rms_args& p, const char* who) {
   PH_REQUIRE(p.ldx >= C && (!p.add || p.ldadd >= C) && (!p.gate || p.ldgate >= C), "%s: a row stride is below %zu columns", who, p.C);
   return PH_OK;
 }
+// A row is read whole before it is written, by the same lanes: an output may be an input in place, but not lie across one's rows.
+struct Rows {
+  const void* p;
+  long ld;
+};
+Span span_of(const ph_rms_args& a, const Rows& r) {
+  const long e = a.dtype == PH_BF16 ? 2 : 4;
+  return {r.p, (long)a.C * e, {(long)a.M, 1, 1}, {r.ld * e, 0, 0}};
+}
+bool apart(const ph_rms_args& a, const Rows& out, const Rows* in, int n, const float* rstd) {
+  for (int i = 0; i < n; i++) {
+    const bool same = out.p == in[i].p && (out.ld == in[i].ld || a.M == 1);
+    if (!same && meet(span_of(a, out), span_of(a, in[i]))) return false;
+  }
+  const Span o = span_of(a, out);
+  return !meet(o, flat(a.w, (long)(a.C / a.G) * 4)) && !meet(o, flat(a.scale, (long)a.C * 4)) && !meet(o, flat(rstd, (long)(a.M * a.G) * 4));
+}
 template <typename T> RmsCall<T> call_of(const ph_rms_args& p, void* stream) {
   RmsCall<T> c{};
   RmsArgs<T>& a = c.a;
@@ -467,7 +485,9 @@ extern "C" int ph_rms_norm(const ph_rms_args* p, void* out, long ldout, void* re
   PH_REQUIRE(ldout >= C && (!p->add || !res || ldres >= C), "rms_norm: a row stride is below %zu columns", p->C);
   if (p->M == 0) return PH_OK;
   PH_REQUIRE(p->x && out, "rms_norm: x or out missing");
-  PH_REQUIRE(out != res || !p->add, "rms_norm: out and res are the same");
+  const Rows in[] = {{p->x, p->ldx}, {p->add, p->ldadd}, {p->gate, p->ldgate}}, o = {out, ldout}, r = {p->add ? res : nullptr, ldres};
+  PH_REQUIRE(!meet(span_of(*p, o), span_of(*p, r)), "rms_norm: out and res are the same or share elements");
+  PH_REQUIRE(apart(*p, o, in, 3, rstd) && apart(*p, r, in, 3, rstd), "rms_norm: out or res shares elements with an input that it is not");
   return p->dtype == PH_BF16 ? fwd_t<uint16_t>(*p, out, ldout, res, ldres, rstd, stream)
                              : fwd_t<float>(*p, out, ldout, res, ldres, rstd, stream);
 }
@@ -480,8 +500,12 @@ extern "C" int ph_rms_norm_grad(const ph_rms_args* p, const float* rstd, const v
   const bool add = p->add && g->dadd, gate = p->gate && g->dgate;
   PH_REQUIRE(lddout >= C && (!dres || lddres >= C) && (!g->dx || g->lddx >= C) && (!add || g->lddadd >= C) && (!gate || g->lddgate >= C),
              "rms_norm_grad: a row stride is below %zu columns", p->C);
-  PH_REQUIRE(!(add && g->dadd == g->dx) && !(gate && (g->dgate == g->dx || (add && g->dgate == g->dadd))),
-             "rms_norm_grad: two gradients are the same");
+  const Rows outs[] = {{g->dx, g->lddx}, {add ? g->dadd : nullptr, g->lddadd}, {gate ? g->dgate : nullptr, g->lddgate}};
+  const Rows in[] = {{p->x, p->ldx}, {p->add, p->ldadd}, {p->gate, p->ldgate}, {dout, lddout}, {dres, lddres}};
+  for (int i = 0; i < 3; i++)
+    for (int j = 0; j < i; j++)
+      PH_REQUIRE(!meet(span_of(*p, outs[i]), span_of(*p, outs[j])), "rms_norm_grad: two gradients are the same or share elements");
+  for (const Rows& o : outs) PH_REQUIRE(apart(*p, o, in, 5, rstd), "rms_norm_grad: a gradient shares elements with an input that it is not");
   if (p->M == 0) {  // no rows: the columns' sums are zero
     if (!g->dw && !g->dscale) return PH_OK;
     k_rms_zero<<<ceil_div(p->C, 256), 256, 0, as_stream(stream)>>>(g->dw, (int)(p->C / p->G), p->scale ? g->dscale : nullptr, (int)p->C);
