@@ -144,7 +144,8 @@ __device__ __forceinline__ float log_decay(float A, float sp) {
   const float g = A * sp;
   return g < -1e9f ? -1e9f : g;  // differences of sums stay numbers
 }
-__device__ __forceinline__ bool finite(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7f800000u) != 0x7f800000u; }
+// Sums of a chunk's values below this are finite.
+constexpr float kFar = 0x1p100f;
 
 // From here on the compiler takes the lane's number as new: what depends on it alone is formed where it is used and does not wait
 // in registers over all chunks.
@@ -325,13 +326,15 @@ template <bool BF> __device__ __forceinline__ float square_sum(u4 r) {
   }
   return s;
 }
-template <bool BF> __device__ __forceinline__ bool all_finite(u4 r) {
+// All below kFar.
+template <bool BF> __device__ __forceinline__ bool all_near(u4 r) {
+  constexpr uint32_t far = __builtin_bit_cast(uint32_t, kFar);
   bool ok = true;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const uint32_t u = r[i];
-    if constexpr (BF) ok = ok && (u & 0x7f80u) != 0x7f80u && (u & 0x7f800000u) != 0x7f800000u;
-    else ok = ok && (u & 0x7f800000u) != 0x7f800000u;
+    if constexpr (BF) ok = ok && (u & 0x7f80u) < far >> 16;
+    ok = ok && (u & 0x7f800000u) < far;
   }
   return ok;
 }
@@ -396,11 +399,13 @@ template <int CH, typename T> __device__ __forceinline__ void fill_rows(int tid,
     if (i & 16) G += low;
   }
   const double last = lane_f64(G, CH - 1);
+  const float be = in ? sigma(raw_f32(g.b)) : 0.f;
+  const bool none = __any(!(be <= 1.f) || G != G);
   if (i < CH) {
     const int seg = __popcll(starts & ((2ull << i) - 1)), all = __popcll(starts);
     r.G[i] = G;
     r.seg[i] = seg;
-    r.be[i] = in ? sigma(raw_f32(g.b)) : 0.f;
+    r.be[i] = be;
     r.sp[i] = sp;
     r.arg[i] = arg;
     const float d0 = ex2((float)G), dc = ex2((float)(last - G));
@@ -409,7 +414,7 @@ template <int CH, typename T> __device__ __forceinline__ void fill_rows(int tid,
     if (i == CH - 1) {
       r.c0 = all == 0 ? d0 : 0.f;
       r.starts = (int)(starts & 0xffffffffu);
-      r.odd = last > 40.0;  // a decay that grows (A above 0) may pass fp32's range in M, which Y does not show
+      r.odd = none || last > 40.0;  // a decay that grows (A above 0) may pass fp32's range in M, which Y does not show
       r.split = CH;
     }
   }
@@ -422,14 +427,14 @@ template <int CH, int NB> __device__ __forceinline__ void mark_odd(int tid, Rows
 #pragma unroll
   for (int n = 0; n < NB; n++)
 #pragma unroll
-    for (int i = 0; i < 4; i++) odd |= !(fabsf(Y[n][i]) < 1e30f);
+    for (int i = 0; i < 4; i++) odd |= !(fabsf(Y[n][i]) < kFar);
   if (!__any(odd)) return;
   const int l = tid & 63;
   unsigned rows = 0;
 #pragma unroll
   for (int n = 0; n < NB; n++)
 #pragma unroll
-    for (int i = 0; i < 4; i++) rows |= !(fabsf(Y[n][i]) < 1e30f) ? 1u << (16 * n + 4 * (l >> 4) + i) : 0u;
+    for (int i = 0; i < 4; i++) rows |= !(fabsf(Y[n][i]) < kFar) ? 1u << (16 * n + 4 * (l >> 4) + i) : 0u;
   rows |= (unsigned)__shfl_xor((int)rows, 16);
   rows |= (unsigned)__shfl_xor((int)rows, 32);
   rows &= (2u << (hi - 1)) - (1u << lo);
@@ -650,9 +655,9 @@ __device__ __forceinline__ void put_row(int tid, T* tile, u4 r, int lo, int hi, 
   if (part && (row < lo || row >= hi)) r = u4{0, 0, 0, 0};
   *reinterpret_cast<u4*>(tile + row * LD + c) = r;
 }
-// 1 / sqrt(|row|^2 + eps) of the staged rows, 0 for those left out; LONG_NAN: none for rows longer than fp32 can say, whose products are
-// no numbers either
-template <bool BF, int P, bool LONG_NAN = false> __device__ __forceinline__ void put_norm(int tid, float* out, u4 r, int lo, int hi) {
+// 1 / sqrt(|row|^2 + eps) of the staged rows, 0 for those left out, NaN for rows longer than fp32 can say, whose products are no
+// numbers either. Returns whether the thread's row is such a one, or holds what is not finite.
+template <bool BF, int P> __device__ __forceinline__ bool put_norm(int tid, float* out, u4 r, int lo, int hi) {
   constexpr int L = P / Elem<BF>::V;  // lanes of a row
   float s = square_sum<BF>(r);
   s += dpp_mov<0xB1>(s);
@@ -661,13 +666,15 @@ template <bool BF, int P, bool LONG_NAN = false> __device__ __forceinline__ void
   if constexpr (L >= 16) s += dpp_mov<0x140>(s);
   if constexpr (L >= 32) s += __shfl_xor(s, 16);
   const int row = tid / L;
-  if (tid % L == 0) out[row] = row >= lo && row < hi ? (LONG_NAN && s == INFINITY ? NAN : __builtin_amdgcn_rsqf(s + kEps)) : 0.f;
+  const bool in = row >= lo && row < hi, odd = in && !(s < INFINITY);
+  if (tid % L == 0) out[row] = odd ? NAN : in ? __builtin_amdgcn_rsqf(s + kEps) : 0.f;
+  return odd;
 }
 
 // ---- sequences ------------------------------------------------------------------------------------------
 // Wavefronts of a SIMD, at least: as many as registers and LDS leave room for.
-template <bool BF, int P> constexpr int fwd_waves() { return P == 128 ? 2 : 4; }
-template <bool BF, int P> constexpr int bwd_waves() { return P == 32 || (P == 64 && !BF) ? 3 : 2; }
+template <bool BF, int P> constexpr int fwd_waves() { return P == 128 ? 2 : BF && P == 32 ? 3 : 4; }
+template <bool BF, int P> constexpr int bwd_waves() { return BF || P == 128 ? 2 : 3; }
 
 // One segment of one sequence's head. LOCAL: without outputs, from a zero state (what the segment adds to its start state) or,
 // without values to write, from the unit matrix (what it multiplies it with).
@@ -775,7 +782,7 @@ template <bool BF, int P, bool LOCAL> __global__ void __launch_bounds__(4 * P, (
         put_row<BF, P>(tid, Ks, k, lo, hi, !once);
         put_row<BF, P>(tid, Vs, v, lo, hi, !once);
         if (!LOCAL) put_norm<BF, P>(tid, R.rq, q, lo, hi);
-        put_norm<BF, P, true>(tid, R.rk, k, lo, hi);
+        put_norm<BF, P>(tid, R.rk, k, lo, hi);
         if (!once && w == NT - 1) fill_rows<CH>(tid, R, g, A, lo, hi);
         __syncthreads();
         have = once;
@@ -1154,13 +1161,13 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
         }
         if (!have) load();  // the first ones, or one episode at a time again
         have = false;
-        const bool odd = tid / (P / Elem<BF>::V) >= lo && tid / (P / Elem<BF>::V) < hi && (!all_finite<BF>(q) || !all_finite<BF>(d));
         put_row<BF, P>(tid, L.Q, q, lo, hi, !once);
         put_row<BF, P>(tid, L.K, k, lo, hi, !once);
         if constexpr (!LOCAL) put_row<BF, P>(tid, L.V, v, lo, hi, !once);
         put_row<BF, P>(tid, L.dO, d, lo, hi, !once);
-        put_norm<BF, P>(tid, R.rq, q, lo, hi);
-        put_norm<BF, P>(tid, R.rk, k, lo, hi);
+        bool odd = put_norm<BF, P>(tid, R.rq, q, lo, hi);
+        odd |= put_norm<BF, P>(tid, R.rk, k, lo, hi);
+        odd |= tid / (P / Elem<BF>::V) >= lo && tid / (P / Elem<BF>::V) < hi && !all_near<BF>(d);
         if (!once && w == NT - 1) fill_rows<CH>(tid, R, g, A, lo, hi);
         f4 S0[LOCAL ? 1 : NT];
         if constexpr (!LOCAL) {
@@ -1207,8 +1214,21 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             Y[n] = rows4(tid, R.be, 16 * n) * (widen(col_unit<LD>(tid, L.V, 16 * n, 16 * w)) - rows4(tid, R.d0, 16 * n) * rk * Y[n]);
           dU[n] = rows4(tid, R.dc, 16 * n) * rk * dU[n];
         }
+        {  // what would pass to other episodes in the products, before it does
+          bool any = odd;
+#pragma unroll
+          for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) any |= (!LOCAL && !(fabsf(Y[n][i]) < kFar)) || !(fabsf(dU[n][i]) < kFar);
+          if (any) R.odd = 1;
+        }
         __syncthreads();
         renew(tid, l);
+        const int starts = R.starts, inside = starts & ~(1 << lo);
+        if (inside && __builtin_amdgcn_readfirstlane(R.odd)) {
+          lo = 31 - __clz(inside);
+          continue;
+        }
         // U, dU, dY: this wavefront's columns of V
         f4 U[NB], dY[NB];
         unit dOc[NB];
@@ -1225,19 +1245,6 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
             }
           }
           solve_t<BF>(tid, L.Tinv, L.M, dU, dY);
-        }
-        const int starts = R.starts, inside = starts & ~(1 << lo);
-        if (inside) {
-          bool bad = odd;
-#pragma unroll
-          for (int n = 0; n < NB; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) bad |= (!LOCAL && !finite(U[n][i])) || !finite(dY[n][i]);
-          if (__syncthreads_or(bad)) {
-            have = false;
-            lo = 31 - __clz(inside);
-            continue;
-          }
         }
         const int col = 16 * w + (l & 15);
         if constexpr (!LOCAL) {
@@ -1395,15 +1402,18 @@ __global__ void __launch_bounds__(4 * P, (bwd_waves<BF, P>())) k_delta_bwd(const
               dQ[n] = X1[n];
               dK[n] = X2[n] + X3[n];
 #pragma unroll
-              for (int m = 0; m <= n; m++) {
-                const f4 e = mat_col<UD>(tid, L.Pm, 16 * m, 16 * n), f = mat_col<UD>(tid, L.M, 16 * m, 16 * n);
-                dQ[n] = dot<1>(&e, kn + m, dQ[n]);
-                dK[n] = dot<1>(&f, kn + m, dK[n]);
-              }
-#pragma unroll
-              for (int m = n; m < NB; m++) {
-                const f4 e = mat_row<UD>(tid, L.Pm, 16 * n, 16 * m), f = mat_row<UD>(tid, L.M, 16 * n, 16 * m);
-                dK[n] = dot<1>(&e, qn + m, dK[n]);
+              for (int m = 0; m < NB; m++) {  // F and F^T take K^ both
+                f4 f = zero;
+                if (m <= n) {
+                  const f4 e = mat_col<UD>(tid, L.Pm, 16 * m, 16 * n);
+                  dQ[n] = dot<1>(&e, kn + m, dQ[n]);
+                  f = mat_col<UD>(tid, L.M, 16 * m, 16 * n);
+                }
+                if (m >= n) {
+                  const f4 e = mat_row<UD>(tid, L.Pm, 16 * n, 16 * m);
+                  dK[n] = dot<1>(&e, qn + m, dK[n]);
+                  f += mat_row<UD>(tid, L.M, 16 * n, 16 * m);
+                }
                 dK[n] = dot<1>(&f, kn + m, dK[n]);
               }
               const f4 sq = qn[n] * dQ[n], sk = kn[n] * dK[n];

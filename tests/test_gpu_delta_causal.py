@@ -106,3 +106,30 @@ def test_a_decay_that_grows_past_fp32_stays_in_its_episode(gpu, dt):
         if s.start:
             same(y[s], y0[s], s)
     assert not y[8].isfinite().any() and not y[46].isfinite().any()
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("name,value", [("q", 3e19), ("k", 3e19), ("v", 3e38), ("dy", 3e38), ("b", float("nan")), ("a", float("nan")), ("a", 20000.0)])
+@pytest.mark.parametrize("T", [70, 410])
+def test_what_overflows_stays_in_its_episode(gpu, T, name, value, dt):
+    """Finite values whose sums or squares pass fp32's range, gates that are none, and a decay that grows: y and the gradients of the
+    episodes of steps 10..44 and from 50 on are those without them."""
+    B, H, K, V = 2, 2, 16, 24
+    clean = dict(inputs(T, B, 1, H, K, V, dt), dy=cu(50, T, B, H, V, dtype=dt))
+    clean["A"] = torch.full((H,), 0.01 if value == 20000.0 else -0.4, device="cuda")
+    done, h0 = torch.zeros(T, B, device="cuda"), cu(5, B, H, K, V)
+    done[[9, 44, 49]] = 1
+
+    def run(p):
+        args = [p[n] for n in "qkvabA"]
+        y, saved = D.delta_scan(*args, dt_bias=p["dt_bias"], done=done, h0=h0, save=True)
+        return dict(D.delta_scan_grad(*args, saved, p["dy"], dt_bias=p["dt_bias"], done=done), y=y)
+
+    want = run(clean)
+    p = {n: t.clone() for n, t in clean.items()}
+    p[name][2:7], p[name][46] = value, value
+    got = run(p)
+    for s in (slice(10, 45), slice(50, T)):
+        for n in ("y", "dq", "dk", "dv", "da", "db"):
+            bar = 2 * BAR[dt] * (10 if n == "da" else 1) + (2 * R.BF16 if dt == BF else 0)
+            assert got[n][s].isfinite().all() and rel(got[n][s], want[n][s]) <= bar, (n, s)
