@@ -466,7 +466,8 @@ int ph_ffn_grad(int dtype, int act, size_t M, size_t D, size_t F, const void* x,
  * slices of a wider one are all taken in place. A, dt_bias fp32 [H]; dt_bias may be NULL (0). done (fp32 [T][B], may be
  * NULL): where nonzero, step t ends an episode, and step t + 1 starts from a cleared state, whatever it held; first (fp32
  * [B], may be NULL): the same for the step before the call. h0 fp32 [B][H][K][V] (may be NULL: zero) is the state carried
- * in. */
+ * in. Sums, states and their gradients are fp32 also for bf16 arrays, which are read as they are and rounded to once. What is not finite
+ * enters y from its step on, in v only its own column; rows of q and k whose square sum passes fp32 count as not finite. */
 typedef struct {
   int dtype;
   size_t T, B, Hk, H, K, V;

@@ -44,10 +44,11 @@
 // without values, from the unit matrix, which gives what it adds to a state (Psi) and what it multiplies it with (Phi); a second
 // joins the segments' start states in order; the third runs them again from those. The gradient does the same in reverse, with Phi^T.
 //
-// Measured, bf16: 64 steps of 2048 sequences x 8 heads of 64x64 forward with kept states 400 us (4.1 TB/s of what it moves; a large
-// copy 5.2), gradient 1051 us: vector instructions issue for half of it, matrix instructions for an eighth, two wavefronts on a
-// SIMD wait at ten barriers a chunk for the rest (three, with 168 registers, spill: 1548 us). 2048 steps of 8 x 4 heads of
-// 128x128 174 and 389 us; 8192 of 2 x 8 of 64x64 139 and 246 (in one piece 1575 and 4663 at first). A single step of 4096 x 8 heads of
+// Measured, bf16: 64 steps of 2048 sequences x 8 heads of 64x64 forward with kept states 390 us (4.2 TB/s of what it moves; a large
+// copy 5.2), gradient 1190 us: vector instructions issue for 44 % of it, matrix instructions for 22 %, two wavefronts on a SIMD wait at
+// seven barriers a chunk for the rest (three wavefronts, with 168 registers, spill and took half as long again). With operands of
+// two parts, 16 bits, in the gradient it was 1051 us, and dh0 off by 3e-6 of its norm where it is 2e-7. 2048 steps of 8 x 4 heads of
+// 128x128 178 and 383 us; 8192 of 2 x 8 of 64x64 142 and 270 (in one piece 1575 and 4663 at first). A single step of 4096 x 8 heads of
 // 64x64 195 us, 5.6 TB/s.
 #include "common.hpp"
 #include "kernels.hpp"
@@ -672,7 +673,8 @@ template <bool BF, int P> __device__ __forceinline__ bool put_norm(int tid, floa
 }
 
 // ---- sequences ------------------------------------------------------------------------------------------
-// Wavefronts of a SIMD, at least: as many as registers and LDS leave room for.
+// Wavefronts of a SIMD, at least: as many as registers and LDS leave room for (three in the 64-wide fp32 gradient, 16 registers of it
+// spilled: 64 steps of 512 x 8 heads 400 us, 467 with two and none spilled).
 template <bool BF, int P> constexpr int fwd_waves() { return P == 128 ? 2 : BF && P == 32 ? 3 : 4; }
 template <bool BF, int P> constexpr int bwd_waves() { return BF || P == 128 ? 2 : 3; }
 
@@ -955,8 +957,8 @@ template <int P, bool BACK> __global__ void __launch_bounds__(4 * P) k_delta_joi
   }
 }
 
-// U and dY of a chunk, transposed: [V][step]. For bf16 in their three parts, cut once by who writes them (16 cuts instead of some 200);
-// of 128 columns in fp32, cut by each reader, since the third parts would not fit a block's LDS.
+// U and dY of a chunk, transposed: [V][step]. For bf16 in their three parts, cut once by who writes them (16 tiles of a chunk, which
+// are read 120 times); of 128 columns in fp32, cut by each reader, since the third parts would not fit a block's LDS.
 template <bool BF, int P> struct Cols {
   using T = typename Elem<BF>::type;
   static constexpr int UD = Elem<BF>::CH + 4;
@@ -1615,7 +1617,9 @@ __global__ void __launch_bounds__(256) k_delta_fold_heads(const float* part, lon
 
 // ---- single step ------------------------------------------------------------------------------------------
 // Bound by the state, read and written once in fp32. A wavefront takes one head of one sequence and LPR * V of its columns: lane
-// l the columns V (l % LPR) .. of the rows l / LPR, + 64 / LPR, ..., all in registers between the two passes over them.
+// l the columns V (l % LPR) .. of the rows l / LPR, + 64 / LPR, ..., all in registers between the two passes over them. 4096 x 8 heads of
+// 64x64 bf16 195 us, 5.6 TB/s; 1024 x 8 of 128x128 237 us, 4.5 TB/s (one wavefront a SIMD); of 128x63, whose rows no 16-byte access
+// fits, 296 us, 1.8 TB/s (a column a lane, 57 registers spilled).
 template <typename T, int VEC, int LPR, int ROWS>
 __global__ void __launch_bounds__(256) k_delta_step(const Args s, float* __restrict__ state, long items, int blocks_v) {
   constexpr int RG = 64 / LPR;

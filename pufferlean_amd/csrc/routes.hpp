@@ -205,9 +205,11 @@ inline long ssm_chunk(long T, long B, long G, long per, int N, bool grad) {
 // Segments of time of `chunks` chunks, of `units` sequences' heads with states padded to P x P: as many as make one round of
 // blocks at the occupancy that their registers leave (P = 32: four blocks of two wavefronts to a CU, 64: two of four, 128: one of
 // eight). A segment more costs a step of the join and, past the round, the others' share of the CU; and there are two passes
-// over the steps, so whole sequences of less than eight chunks stay one. Forward and gradient, bf16, us by segments: 8192 steps of 16
-// units of 64x64 8: 308, 709; 16: 178, 375; 32: 133, 246; 48: 144, 280; 64: 144, 259. 1024 of 64 units of 64x64 4: 101, 204; 8: 75, 134;
-// 16: 74, 138; 32: 87, 158; of 32x32 8: 62, 128; 16: 48, 87; 32: 58, 105. 2048 of 32 units of 128x128 4: 215, 641; 8: 168, 389; 16: 185, 402.
+// over the steps, so whole sequences of less than eight chunks stay one. Forward (kept states) and gradient, us by segments. bf16: 8192
+// steps of 16 units of 64x64 8: 321, 771; 16: 185, 406; 32: 142, 270; 48: 151, 310; 64: 154, 271. 1024 of 64 units of 64x64 4: 98, 211; 8: 77,
+// 144; 16: 81, 145; of 32x32 4: 95, 204; 8: 60, 131; 16: 50, 89. 2048 of 32 units of 128x128 4: 217, 673; 8: 178, 383; 16: 203, 417. fp32, whose
+// chunks have half the steps: 4096 of 16 units of 64x64 16: 165, 327; 32: 132, 235; 48: 145, 225; 64: 146, 230. 512 of 64 units of 64x64 1: 151,
+// 350; 4: 88, 170; 8: 71, 125; 16: 77, 122; of 32x32 8: 47, 92; 16: 40, 65. 1024 of 32 units of 128x128 4: 230, 542; 8: 187, 304; 16: 213, 330.
 constexpr int kMostSegments = 1024;
 inline long delta_segments(long chunks, long units, int P) {
   const long most = (chunks + 1) / 2, want = (P <= 32 ? kMostSegments : P <= 64 ? 512 : 256) / units;
@@ -217,9 +219,11 @@ inline long delta_segments(long chunks, long units, int P) {
 
 // ---- Draw from filtered logits ------------------------------------------------------------------------------
 // Whether N rows of A entries take sixteen blocks each, in three launches or (top-p) five, or one block in one. One block to a row
-// leaves CUs idle, but a launch more costs 5 us, and top-k alone is short either way. Several blocks / one, bf16, us without a
-// filter, with top-k and with top-p: 128x16384 27 / 18, 36 / 22, 54 / 37; 128x32768 30 / 30, 42 / 24, 70 / 63; 128x65536 38 / 54,
-// 51 / 30, 90 / 113; 64x131072, filters mixed: 95 / 205.
+// leaves CUs idle, but a launch more costs 5 us. Several blocks / one, us without a filter, with top-p, and with top-k of 50 alone, which
+// one block would do sooner (the rule does not see which filters there are). bf16: 128x16384 26 / 19, 55 / 37, 44 / 23; 128x32768 28 / 30,
+// 67 / 64, 48 / 26; 64x49152 28 / 42, 65 / 86, 40 / 29; 128x65536 37 / 54, 89 / 111, 52 / 32. fp32: 128x16384 24 / 19, 53 / 37, 57 / 29; 128x32768
+// 28 / 32, 64 / 64, 54 / 34; 64x49152 26 / 43, 61 / 87, 47 / 35; 128x65536 38 / 57, 89 / 117, 58 / 41. A top-k of more than 1024 is done by one block
+// in the end: 64x49152 86 / 79.
 inline bool draw_split(long N, long A) { return N <= 128 && A >= 49152; }
 
 }  // namespace ph
