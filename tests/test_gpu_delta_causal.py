@@ -110,11 +110,11 @@ def test_a_decay_that_grows_past_fp32_stays_in_its_episode(gpu, dt):
 
 @pytest.mark.parametrize("dt", [F32, BF])
 @pytest.mark.parametrize("name,value", [("q", 3e19), ("k", 3e19), ("v", 3e38), ("dy", 3e38), ("b", float("nan")), ("a", float("nan")), ("a", 20000.0)])
-@pytest.mark.parametrize("T", [70, 410])
-def test_what_overflows_stays_in_its_episode(gpu, T, name, value, dt):
+@pytest.mark.parametrize("T,K,V", [(70, 16, 24), (410, 16, 24), (70, 64, 64), (70, 100, 128)])
+def test_what_overflows_stays_in_its_episode(gpu, T, K, V, name, value, dt):
     """Finite values whose sums or squares pass fp32's range, gates that are none, and a decay that grows: y and the gradients of the
     episodes of steps 10..44 and from 50 on are those without them."""
-    B, H, K, V = 2, 2, 16, 24
+    B, H = 2, 2
     clean = dict(inputs(T, B, 1, H, K, V, dt), dy=cu(50, T, B, H, V, dtype=dt))
     clean["A"] = torch.full((H,), 0.01 if value == 20000.0 else -0.4, device="cuda")
     done, h0 = torch.zeros(T, B, device="cuda"), cu(5, B, H, K, V)
