@@ -1660,7 +1660,7 @@ __global__ void __launch_bounds__(256) k_delta_step(const Args s, float* __restr
       qq = fmaf(qv[i], qv[i], qq);
     }
     group_sum<64>(kk, qq);
-    const float rk = __builtin_amdgcn_rsqf(kk + kEps), rq = __builtin_amdgcn_rsqf(qq + kEps);
+    const float rk = kk == INFINITY ? NAN : __builtin_amdgcn_rsqf(kk + kEps), rq = qq == INFINITY ? NAN : __builtin_amdgcn_rsqf(qq + kEps);
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       sh[w][0][l + 64 * i] = kv[i] * rk;

@@ -133,3 +133,19 @@ def test_what_overflows_stays_in_its_episode(gpu, T, K, V, name, value, dt):
         for n in ("y", "dq", "dk", "dv", "da", "db"):
             bar = 2 * BAR[dt] * (10 if n == "da" else 1) + (2 * R.BF16 if dt == BF else 0)
             assert got[n][s].isfinite().all() and rel(got[n][s], want[n][s]) <= bar, (n, s)
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("name", ["q", "k"])
+def test_rows_too_long_for_fp32_are_none_in_scan_and_step(gpu, name, dt):
+    """Not rows of zero: their unit rows could not be told."""
+    B, H, K, V = 3, 2, 16, 24
+    p = {n: t.clone() for n, t in inputs(1, B, 1, H, K, V, dt).items()}
+    p[name][0, 1] = 3e19
+    h0 = cu(5, B, H, K, V)
+    y, h = scan(p, h0)
+    step = h0.clone()
+    ys = D.delta_step(*[p[n][0] for n in "qkvab"], p["A"], step, dt_bias=p["dt_bias"])
+    for out, state in ((y[0], h), (ys, step)):
+        assert not out[1].isfinite().any() and out[[0, 2]].isfinite().all()
+        assert state[[0, 2]].isfinite().all() and state[1].isfinite().any() == (name == "q")
